@@ -180,6 +180,48 @@ int bf16n_router_topk_route(const float * logits, int64_t logits_stride, int n_t
                             int32_t * ids, float * weights, int64_t out_stride, int n_slots, int n_listed,
                             int32_t * ids_src1, int32_t * ids_dst, int32_t * bounds, int nchannels_y, int sis1, void * stream);
 
+/* ---- 4-bit weights with group scales (lossy; beside the lossless formats).  The reference holds a draft copy of the
+ * output projection in such a form (core/include/bf16n/draft_head.cuh:22-220); here they are products of any shape, of experts and
+ * with gate and up together. ---- */
+/*   w[r, k] = scale[r, k / group] * (code[r, k] - zero[r, k / group])
+ * codes: [rows, K / 2] bytes, two codes 0..15 each, the even column in the low half; 16-byte aligned device memory.
+ * scales: [rows, ceil(K / group)] BF16 (or FP16 with scales_f16).  zeros: a byte for every scale, or null: 8 everywhere.
+ * K: a multiple of 32, at most 16384; group: a power of two from 32 on (the last group of a row may be cut short). */
+typedef struct bf16n_int4_weight {
+    const uint8_t * codes;
+    const void * scales;
+    const uint8_t * zeros;
+    int64_t K, rows;
+    int32_t group, scales_f16;
+} bf16n_int4_weight;
+/* bf16n_mmv for such a matrix: y = W x per column, sums in FP32, no weight rounded (the codes are exact operands; scales and
+ * zero points are applied to FP32 sums).  up given: silu(W x) * (up x), gate and up of one shape, K and group.  Arguments as in
+ * bf16n_mmv_args (rows_per_matrix = nrows, row0 = 0; any number of dense columns, at most 65535 with ids); ids: int32, or int64 with
+ * ids_i64; an id that names no matrix gives a column of zeros.  x: BF16 or FP32, 16-byte aligned columns.  The result must
+ * not overlap x.  An activation that is not finite makes every result of its column not finite (NaN or infinite). */
+int bf16n_int4_mmv(const bf16n_int4_weight * w, const bf16n_int4_weight * up, const bf16n_mmv_args * a, int ids_i64, void * stream);
+/* The (token, slot) pairs t * n_used + slot sorted by the matrix that their id names, ascending within one; pairs whose id names
+ * none (outside [0, n_matrices)) come last.  Every pair is listed, also where a token names a matrix twice.  pairs:
+ * n_tok * n_used entries; bounds: n_matrices + 2 (matrix m has pairs[bounds[m]] .. pairs[bounds[m + 1] - 1], the last range is
+ * that of the pairs without one).  Strides of ids in bytes. */
+int bf16n_int4_route(const void * ids, int ids_i64, int64_t ids_s0, int64_t ids_s1, int n_matrices, int n_tok, int n_used, int32_t * pairs,
+                     int32_t * bounds, void * stream);
+/* bf16n_mm_ids for such stacks (up given: gated): dst[pair] = W_e x, rows dst_col elements apart, for every pair of
+ * bf16n_int4_route's lists, zeros for those without a matrix.  x: BF16, rows x_row elements apart, one for every token or,
+ * with per_slot, for every pair. */
+int bf16n_int4_mm_ids(const bf16n_int4_weight * w, const bf16n_int4_weight * up, const void * x_bf16, int64_t x_row, int per_slot,
+                      const int32_t * pairs, const int32_t * bounds, void * dst, int dst_bf16, int64_t dst_col, int n_experts, int n_tok,
+                      int n_used, void * stream);
+/* The router's selection with scores, a bias and groups: p = softmax(logits) or, with sigmoid, 1 / (1 + exp(-logits));
+ * c = p + bias (bias: n_experts FP32 or null); the experts lie in n_groups groups of equal size, ranked by their largest c, or
+ * with top2 by the sum of their two largest; the k largest c of the topk_groups first groups are taken (ties: lower index),
+ * in that order.  weights: their p, over the sum of the k with renorm (zeros where that is zero), times scale.  Scores and sums are held in
+ * 64 bits, so that the choice does not hang on roundings.  NaN logits count as -inf: the score 0, and last in the order.  At most
+ * 1024 experts and k <= 64, 64 groups, k <= topk_groups * (n_experts / n_groups).  Rows of out_stride >= k elements. */
+int bf16n_router_topk_grouped(const float * logits, int64_t logits_stride, const float * bias, int n_tok, int n_experts, int n_groups,
+                              int topk_groups, int k, int sigmoid, int top2, int renorm, float scale, int32_t * ids, float * weights,
+                              int64_t out_stride, void * stream);
+
 /* ---- load-time conversion and the registry of resident tensors: the reference's llama.cpp adapter without ggml types
  * (engines/llamacpp/patches/0002-ggml-cuda-thin-BF16N-adapter-over-the-shared-core.patch).  An engine stores a converted
  * tensor as rows * K bytes of device memory (the plane); the aux buffer is allocated here and found again by the

@@ -25,9 +25,14 @@ class MmvArgs(C.Structure):
                 ("pad_", C.c_uint8 * 2)]
 
 
+class Int4Weight(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("zeros", C.c_void_p), ("K", C.c_int64), ("rows", C.c_int64),
+                ("group", C.c_int32), ("scales_f16", C.c_int32)]
+
+
 # name -> (restype, argtypes); every symbol declared in include/bf16n_c.h
 _i, _i64, _u32, _vp, _cp = C.c_int, C.c_int64, C.c_uint32, C.c_void_p, C.c_char_p
-_WP, _AP = C.POINTER(Weight), C.POINTER(MmvArgs)
+_WP, _AP, _QP = C.POINTER(Weight), C.POINTER(MmvArgs), C.POINTER(Int4Weight)
 SYMBOLS = {
     "bf16n_last_error": (_cp, []),
     "bf16n_last_kernel": (_cp, []),
@@ -64,6 +69,10 @@ SYMBOLS = {
     "bf16n_router_topk_strided": (_i, [_vp, _i64, _i, _i, _i, _i, _vp, _vp, _i64, _vp]),
     "bf16n_router_topk_route_fits": (_i, [_i, _i, _i]),
     "bf16n_router_topk_route": (_i, [_vp, _i64, _i, _i, _i, _i, _vp, _vp, _i64, _i, _i, _vp, _vp, _vp, _i, _i, _vp]),
+    "bf16n_int4_mmv": (_i, [_QP, _QP, _AP, _i, _vp]),
+    "bf16n_int4_route": (_i, [_vp, _i, _i64, _i64, _i, _i, _i, _vp, _vp, _vp]),
+    "bf16n_int4_mm_ids": (_i, [_QP, _QP, _vp, _i64, _i, _vp, _vp, _vp, _i, _i64, _i, _i, _i, _vp]),
+    "bf16n_router_topk_grouped": (_i, [_vp, _i64, _vp, _i, _i, _i, _i, _i, _i, _i, _i, C.c_float, _vp, _vp, _i64, _vp]),
     "bf16n_adapter_choose": (_i, [_i64, _i64, _i64, _cp, _i64, _i, _i]),
     "bf16n_adapter_convert": (_i, [_vp, _vp, _i64, _i64, _i64, _i, _i, _i, _vp, _cp, _i, C.POINTER(_i)]),
     "bf16n_verify_roundtrip": (_i, [_WP, _vp, C.POINTER(_i)]),

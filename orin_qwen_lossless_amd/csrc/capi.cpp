@@ -81,6 +81,7 @@ per_device & ensure_init() {
         dev::w64_init();
         dev::mm_ids_init();
         dev::tile_init();
+        dev::int4_init();
         void * p = nullptr;
         hip_check(hipGetSymbolAddress(&p, HIP_SYMBOL(scratch)), "hipGetSymbolAddress (routing lists)");
         d.lists = static_cast<route_lists *>(p);
@@ -692,6 +693,106 @@ int bf16n_router_topk_route(const float * logits, int64_t logits_stride, int n_t
 int bf16n_router_topk(const float * logits, int64_t logits_stride, int n_tok, int n_experts, int k, int renorm,
                       int32_t * ids, float * weights, void * stream) {
     return bf16n_router_topk_strided(logits, logits_stride, n_tok, n_experts, k, renorm, ids, weights, k, stream);
+}
+
+// ---------------------------------------------------------------- 4-bit weights with group scales
+
+namespace {
+
+void check_int4(const bf16n_int4_weight * w, const bf16n_int4_weight * up) {
+    require(w != nullptr, "int4: null weight");
+    for (const bf16n_int4_weight * m : {w, up}) {
+        if (!m) {
+            continue;
+        }
+        require(m->K % 32 == 0 && m->K >= 32 && m->K <= 16384, "int4: K must be a multiple of 32 in [32, 16384]");
+        require(m->group >= 32 && (m->group & (m->group - 1)) == 0, "int4: the group must be a power of two from 32 on");
+        require(m->rows >= 0, "int4: rows must be nonnegative");
+        require(m->rows == 0 || (m->codes && m->scales), "int4: null codes or scales");
+        require(((uintptr_t) m->codes & 15) == 0 && ((uintptr_t) m->scales & 1) == 0, "int4: codes must be 16-byte, scales 2-byte aligned");
+    }
+    require(!up || (up->K == w->K && up->rows == w->rows && up->group == w->group), "int4: gate/up shapes and groups must match");
+}
+
+} // namespace
+
+int bf16n_int4_mmv(const bf16n_int4_weight * w, const bf16n_int4_weight * up, const bf16n_mmv_args * a, int ids_i64, void * stream) {
+    return guarded([&] {
+        ensure_init();
+        dev::g_last_kernel.name = nullptr;
+        check_int4(w, up);
+        require(a && a->ncols > 0, "int4_mmv: ncols out of range");
+        require(a->row0 == 0 && a->nrows == a->rows_per_matrix, "int4_mmv: a product takes whole matrices");
+        if (a->nrows == 0) {
+            return;
+        }
+        require(a->x && a->y, "int4_mmv: null pointer");
+        require(((uintptr_t) a->x & 15) == 0 && a->x_tok % 16 == 0 && a->x_slot % 16 == 0, "int4_mmv: x must be 16-byte aligned with 16-byte strides");
+        const int64_t el = a->y_bf16 ? 2 : 4;
+        require((uintptr_t) a->y % el == 0 && a->y_tok % el == 0 && a->y_slot % el == 0, "int4_mmv: y must be aligned to its elements");
+        if (a->ids) {
+            const int64_t ib = ids_i64 ? 8 : 4;
+            require(a->ncols <= 65535 && a->n_used > 0, "int4_mmv: at most 65535 columns with ids");
+            require(a->nrows > 0 && w->rows % a->nrows == 0, "int4_mmv: rows_per_matrix must divide the rows");
+            require((uintptr_t) a->ids % ib == 0 && a->ids_s0 % ib == 0 && a->ids_s1 % ib == 0, "int4_mmv: ids must be aligned to their elements");
+        } else {
+            require(a->nrows == w->rows, "int4_mmv: a dense product uses the whole matrix");
+        }
+        dev::launch_int4_mmv(*w, up, *a, ids_i64 != 0, g_cus, (hipStream_t) stream);
+        launch_check("int4_mmv");
+    });
+}
+
+int bf16n_int4_route(const void * ids, int ids_i64, int64_t ids_s0, int64_t ids_s1, int n_matrices, int n_tok, int n_used, int32_t * pairs,
+                     int32_t * bounds, void * stream) {
+    return guarded([&] {
+        ensure_init();
+        const int64_t ib = ids_i64 ? 8 : 4;
+        require(n_matrices > 0 && n_matrices <= 65534 && n_tok > 0 && n_used > 0 && (int64_t) n_tok * n_used <= (1 << 28), "int4_route: sizes out of range");
+        require(ids && pairs && bounds, "int4_route: null pointer");
+        require((uintptr_t) ids % ib == 0 && ids_s0 % ib == 0 && ids_s1 % ib == 0, "int4_route: ids must be aligned to their elements");
+        dev::launch_int4_route(ids, ids_i64 != 0, ids_s0, ids_s1, n_matrices, n_tok, n_used, pairs, bounds, (hipStream_t) stream);
+        launch_check("int4_route");
+    });
+}
+
+int bf16n_int4_mm_ids(const bf16n_int4_weight * w, const bf16n_int4_weight * up, const void * x_bf16, int64_t x_row, int per_slot,
+                      const int32_t * pairs, const int32_t * bounds, void * dst, int dst_bf16, int64_t dst_col, int n_experts, int n_tok,
+                      int n_used, void * stream) {
+    return guarded([&] {
+        ensure_init();
+        dev::g_last_kernel.name = nullptr;
+        check_int4(w, up);
+        require(n_experts > 0 && n_experts <= 65534 && w->rows % n_experts == 0, "int4_mm_ids: rows must split into n_experts");
+        require(n_tok > 0 && n_used > 0 && (int64_t) n_tok * n_used <= (1 << 28), "int4_mm_ids: sizes out of range");
+        if (w->rows == 0) {
+            return;
+        }
+        require(x_bf16 && pairs && bounds && dst, "int4_mm_ids: null pointer");
+        require(((uintptr_t) x_bf16 & 15) == 0 && x_row % 8 == 0, "activations must be 16-byte aligned with 16-byte row strides");
+        require((uintptr_t) dst % (dst_bf16 ? 2 : 4) == 0 && dst_col >= w->rows / n_experts, "int4_mm_ids: dst must be aligned to its elements, its rows apart");
+        dev::launch_int4_mm_ids(*w, up, x_bf16, x_row, per_slot != 0, pairs, bounds, dst, dst_bf16 != 0, dst_col, n_experts, n_tok, n_used,
+                                g_cus, (hipStream_t) stream);
+        launch_check("int4_mm_ids");
+    });
+}
+
+int bf16n_router_topk_grouped(const float * logits, int64_t logits_stride, const float * bias, int n_tok, int n_experts, int n_groups,
+                              int topk_groups, int k, int sigmoid, int top2, int renorm, float scale, int32_t * ids, float * weights,
+                              int64_t out_stride, void * stream) {
+    return guarded([&] {
+        ensure_init();
+        require(n_tok > 0 && n_experts > 0 && n_experts <= 1024, "router_topk_grouped: at most 1024 experts");
+        require(n_groups > 0 && n_groups <= 64 && n_experts % n_groups == 0, "router_topk_grouped: at most 64 groups of one size");
+        require(topk_groups > 0 && topk_groups <= n_groups, "router_topk_grouped: need 0 < topk_groups <= n_groups");
+        require(k > 0 && k <= 64 && k <= topk_groups * (n_experts / n_groups), "router_topk_grouped: need 0 < k <= min(the experts of topk_groups groups, 64)");
+        require(out_stride >= k, "router_topk_grouped: the output row stride must be at least k");
+        require(logits && ids && weights, "router_topk_grouped: null pointer");
+        dev::router_grouped_args a = {logits, logits_stride, bias, n_experts, n_groups, topk_groups, k, sigmoid != 0, top2 != 0, renorm != 0, scale,
+                                      ids, weights, out_stride};
+        dev::launch_router_topk_grouped(a, n_tok, (hipStream_t) stream);
+        launch_check("router_topk_grouped");
+    });
 }
 
 } // extern "C"

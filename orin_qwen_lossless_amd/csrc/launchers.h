@@ -95,6 +95,24 @@ void launch_router_topk_route(const float * logits, int64_t stride, int n_tok, i
                               float * weights, int64_t out_stride, int n_slots, int n_listed, int32_t * ids_src1, int32_t * ids_dst,
                               int32_t * bounds, int nchannels_y, int sis1, hipStream_t stream);
 
+// the selection with scores, a bias and groups (kernels_router.hip)
+struct router_grouped_args {
+    const float * logits; int64_t stride; // [n_tok, n_experts]
+    const float * bias;                   // [n_experts] or null
+    int n_experts, n_groups, topk_groups, k;
+    bool sigmoid, top2, renorm;
+    float scale;
+    int32_t * ids; float * weights; int64_t out_stride;
+};
+void launch_router_topk_grouped(const router_grouped_args & a, int n_tok, hipStream_t stream);
+
+// 4-bit weights with group scales (kernels_int4.hip)
+void int4_init();
+void launch_int4_mmv(const bf16n_int4_weight & w, const bf16n_int4_weight * up, const bf16n_mmv_args & a, bool ids_i64, int cus, hipStream_t stream);
+void launch_int4_route(const void * ids, bool i64, int64_t s0, int64_t s1, int n_matrices, int n_tok, int n_used, int32_t * pairs, int32_t * bounds,
+                       hipStream_t stream);
+void launch_int4_mm_ids(const bf16n_int4_weight & w, const bf16n_int4_weight * up, const void * x, int64_t x_row, bool per_slot, const int32_t * pairs,
+                        const int32_t * bounds, void * y, bool y_bf16, int64_t y_row, int n_matrices, int n_tok, int n_used, int cus, hipStream_t stream);
 
 // batched MoE prefill (kernels_mm_ids.hip)
 void mm_ids_init();

@@ -862,3 +862,289 @@ def moe_experts(x: torch.Tensor, gate: Weight, up: Weight, down: Weight, topk_we
     """Routed experts of one MoE layer, BF16 out: for every token the weighted sum over its top-k experts of
     down_e(silu(gate_e x) * (up_e x)) (engines/vllm/vllm_bf16n/ops.py:251-271); see moe_experts_rows for the paths."""
     return moe_combine(moe_experts_rows(x, gate, up, down, topk_ids, n_experts), topk_weights, torch.bfloat16)
+
+
+# ---------------------------------------------------------------- 4-bit weights with group scales
+
+@dataclass(frozen=True)
+class Int4Weight:
+    """A matrix (or a stack of matrices) of 4-bit codes with group scales on a device:
+    w[r, k] = scales[r, k // group] * (code[r, k] - zeros[r, k // group]).
+
+    codes: uint8 [rows, K / 2], two codes 0..15 each, the even column in the low half; scales: bf16 or f16
+    [rows, ceil(K / group)]; zeros: uint8 of the scales' shape, or None: 8 everywhere.  All contiguous and on one device.
+    K: a multiple of 32, at most 16384; group: a power of two from 32 on."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    zeros: torch.Tensor | None = None
+    group: int = 128
+
+    def __post_init__(self):
+        c, s, z, g = self.codes, self.scales, self.zeros, self.group
+        if c.dtype is not torch.uint8 or c.dim() != 2 or not c.is_contiguous():
+            raise ValueError("bf16n.Int4Weight: codes must be contiguous uint8 [rows, K / 2]")
+        K = 2 * c.shape[1]
+        if K % 32 or not 32 <= K <= 16384:
+            raise ValueError("bf16n.Int4Weight: K must be a multiple of 32 in [32, 16384]")
+        if not isinstance(g, int) or g < 32 or g & (g - 1) or g > 1 << 30:
+            raise ValueError("bf16n.Int4Weight: group must be a power of two from 32 on")
+        shape = (c.shape[0], -(-K // g))
+        if s.dtype not in (torch.bfloat16, torch.float16) or tuple(s.shape) != shape or not s.is_contiguous():
+            raise ValueError(f"bf16n.Int4Weight: scales must be contiguous bf16 or f16 {list(shape)}")
+        if z is not None and (z.dtype is not torch.uint8 or tuple(z.shape) != shape or not z.is_contiguous()):
+            raise ValueError(f"bf16n.Int4Weight: zeros must be contiguous uint8 {list(shape)}")
+        if s.device != c.device or (z is not None and z.device != c.device):
+            raise ValueError("bf16n.Int4Weight: codes, scales and zeros on different devices")
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
+
+    @property
+    def K(self) -> int:
+        return 2 * self.codes.shape[1]
+
+    @property
+    def nbytes(self) -> int:
+        """Bytes the matrix occupies in device memory."""
+        return sum(t.numel() * t.element_size() for t in (self.codes, self.scales, self.zeros) if t is not None)
+
+    def to(self, device: torch.device | str) -> "Int4Weight":
+        return Int4Weight(self.codes.to(device), self.scales.to(device), None if self.zeros is None else self.zeros.to(device), self.group)
+
+
+def int4_quantize(w: torch.Tensor, group: int = 128, symmetric: bool = True, scale_dtype: torch.dtype = torch.bfloat16) -> Int4Weight:
+    """The nearest codes of a BF16 / FP32 matrix [..., K] (leading axes are rows), on its device, for load time: torch
+    operations in pieces.  symmetric: scale = max|w| / 7 of a group, zero point 8; otherwise scale = (max - min) / 15 over the
+    group's range with 0 in it, and a zero point.  Codes are taken against the rounded scale."""
+    if w.dim() < 2 or w.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("bf16n.int4_quantize: weight must be bf16 or f32, at least 2-D (rows x K)")
+    if scale_dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("bf16n.int4_quantize: scales are bf16 or f16")
+    K = w.shape[-1]
+    if K % 32 or not 32 <= K <= 16384 or group < 32 or group & (group - 1):
+        raise ValueError("bf16n.int4_quantize: K must be a multiple of 32 in [32, 16384], group a power of two from 32 on")
+    w = w.reshape(-1, K)
+    rows, n = w.shape[0], -(-K // group)
+    codes = torch.empty((rows, K // 2), dtype=torch.uint8, device=w.device)
+    scales = torch.empty((rows, n), dtype=scale_dtype, device=w.device)
+    zeros = None if symmetric else torch.empty((rows, n), dtype=torch.uint8, device=w.device)
+    step = max(1, DEQUANT_CHUNK_BYTES // (4 * K))
+    for r in range(0, rows, step):
+        v = w[r: r + step].float()
+        v = torch.nn.functional.pad(v, (0, n * group - K)).view(v.shape[0], n, group)
+        if symmetric:
+            s = (v.abs().amax(2) / 7.0).to(scale_dtype)
+            z = torch.full_like(s, 8.0, dtype=torch.float32)
+        else:
+            lo = v.amin(2).clamp_max(0.0)
+            s = ((v.amax(2).clamp_min(0.0) - lo) / 15.0).to(scale_dtype)
+            z = torch.nan_to_num(torch.round(-lo / s.float()), nan=8.0).clamp(0, 15)
+            zeros[r: r + step] = z.to(torch.uint8)
+        q = torch.nan_to_num(torch.round(v / s.float()[:, :, None]), nan=0.0).add_(z[:, :, None]).clamp_(0, 15).to(torch.uint8)
+        q = q.view(v.shape[0], n * group)[:, :K]
+        codes[r: r + step] = q[:, 0::2] | (q[:, 1::2] << 4)
+        scales[r: r + step] = s
+    return Int4Weight(codes, scales, zeros, group)
+
+
+def _c_int4(w: Int4Weight) -> _lib.Int4Weight:
+    c, s, z = w.codes, w.scales, w.zeros
+    if not c.is_cuda:
+        raise ValueError("bf16n: an Int4Weight must be on a device")
+    return _lib.Int4Weight(c.data_ptr(), s.data_ptr(), None if z is None else z.data_ptr(), 2 * c.shape[1], c.shape[0], w.group,
+                           s.dtype is torch.float16)
+
+
+def _int4_mmv(what: str, x: torch.Tensor, w: Int4Weight, up: Int4Weight | None, ids: torch.Tensor | None, rows_per_matrix: int,
+              out_dtype: torch.dtype) -> torch.Tensor:
+    cw = _c_int4(w)
+    cu = None
+    if up is not None:
+        if up.codes.shape != w.codes.shape or up.group != w.group:
+            raise ValueError(f"bf16n.{what}: gate/up shapes and groups must match")
+        cu = C.byref(_c_int4(up))
+    _check_x(x, cw.K, "x")
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"bf16n.{what}: results are bf16 or f32")
+    dev = x.device
+    if w.codes.device != dev or (up is not None and up.codes.device != dev) or (ids is not None and ids.device != dev):
+        raise ValueError(f"bf16n.{what}: operands on different devices")
+    x_bf16, out_bf16 = x.dtype is torch.bfloat16, out_dtype is torch.bfloat16
+    xsz, osz = 2 if x_bf16 else 4, 2 if out_bf16 else 4
+    i64 = 0
+    if ids is None:
+        if x.dim() != 2:
+            raise ValueError(f"bf16n.{what}: dense x must be [tokens, K]")
+        if rows_per_matrix not in (0, cw.rows):
+            raise ValueError(f"bf16n.{what}: a dense product uses the whole matrix")
+        T, n = x.shape[0], cw.rows
+        y = torch.empty((T, n), dtype=out_dtype, device=dev)
+        if T == 0 or n == 0:
+            return y
+        a = _lib.MmvArgs(x.data_ptr(), y.data_ptr(), None, x.stride(0) * xsz, n * osz, 0, 0, 0, 0, n, 0, n, T, 1, 1, x_bf16, out_bf16)
+    else:
+        _check_ids(ids)
+        T, n_used = ids.shape
+        if rows_per_matrix <= 0 or cw.rows % rows_per_matrix:
+            raise ValueError(f"bf16n.{what}: rows_per_matrix must divide the rows")
+        if not ((x.dim() == 2 and x.shape[0] == T) or (x.dim() == 3 and x.shape[0] == T and x.shape[1] == n_used)):
+            raise ValueError(f"bf16n.{what}: x must be [tokens, K] or [tokens, n_used, K]")
+        n = rows_per_matrix
+        y = torch.empty((T, n_used, n), dtype=out_dtype, device=dev)
+        if T == 0 or n_used == 0:
+            return y
+        if cw.rows == 0:
+            return y.zero_()  # no matrix: no id names one
+        i64 = ids.dtype is torch.int64
+        isz, per_slot = 8 if i64 else 4, x.dim() == 3
+        a = _lib.MmvArgs(x.data_ptr(), y.data_ptr(), ids.data_ptr(), x.stride(0) * xsz, n_used * n * osz, isz, ids.stride(0) * isz,
+                         x.stride(1) * xsz if per_slot else 0, n * osz, n, 0, n, T * n_used, n_used, n_used if per_slot else 1, x_bf16, out_bf16)
+    with _on(dev):
+        _lib.check(_lib.lib().bf16n_int4_mmv(C.byref(cw), cu, C.byref(a), i64, _stream()))
+    return y
+
+
+def int4_mmv(x: torch.Tensor, w: Int4Weight, ids: torch.Tensor | None = None, rows_per_matrix: int = 0,
+             out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """mmv for 4-bit weights with group scales: x [tokens, K] BF16 or FP32 -> [tokens, rows], or with expert ids [tokens, n_used]
+    the rows of the matrices that they name, [tokens, n_used, rows_per_matrix], zeros where an id names none.  No weight is
+    rounded: exact codes, FP32 sums, the scales applied to the sums."""
+    return _int4_mmv("int4_mmv", x, w, None, ids, rows_per_matrix, out_dtype)
+
+
+def int4_mmv_glu2(x: torch.Tensor, gate: Int4Weight, up: Int4Weight, ids: torch.Tensor | None = None, rows_per_matrix: int = 0,
+                  out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """silu(gate x) * (up x) in one launch for two matrices of one shape and group, dense or with expert ids (mmv_glu2)."""
+    return _int4_mmv("int4_mmv_glu2", x, gate, up, ids, rows_per_matrix, out_dtype)
+
+
+def int4_linear(x: torch.Tensor, w: Int4Weight, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """y = x W^T (+ bias) in BF16 for any number of tokens; the bias is added in FP32 before the one rounding."""
+    if x.dtype is not torch.bfloat16:
+        raise ValueError("bf16n.int4_linear: x must be bf16")
+    if x.dim() == 0 or x.shape[-1] != w.K:
+        raise ValueError(f"bf16n.int4_linear: x last dim must be K = {w.K}")
+    x2 = x if x.dim() == 2 else x.reshape(-1, w.K)
+    if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.data_ptr() % 16:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    if bias is None:
+        y = _int4_mmv("int4_linear", x2, w, None, None, 0, torch.bfloat16)
+    else:
+        y = _int4_mmv("int4_linear", x2, w, None, None, 0, torch.float32).add_(bias).to(torch.bfloat16)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], w.rows)
+
+
+def int4_route(topk_ids: torch.Tensor, n_experts: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """(pairs, bounds) int32: the (token, slot) pairs token * n_used + slot sorted by the expert that their id names, those that
+    name none (outside [0, n_experts)) last; expert e has pairs[bounds[e]: bounds[e + 1]] (bf16n_int4_route)."""
+    _check_ids(topk_ids)
+    T, n_used = topk_ids.shape
+    dev, sz = topk_ids.device, topk_ids.element_size()
+    pairs = torch.empty(T * n_used, dtype=torch.int32, device=dev)
+    if T * n_used == 0:
+        return pairs, torch.zeros(n_experts + 2, dtype=torch.int32, device=dev)
+    bounds = torch.empty(n_experts + 2, dtype=torch.int32, device=dev)
+    with _on(dev):
+        _lib.check(_lib.lib().bf16n_int4_route(topk_ids.data_ptr(), int(sz == 8), sz, topk_ids.stride(0) * sz, n_experts, T, n_used,
+                                               pairs.data_ptr(), bounds.data_ptr(), _stream()))
+    return pairs, bounds
+
+
+def int4_moe_mm_ids(x: torch.Tensor, topk_ids: torch.Tensor, w: Int4Weight, n_experts: int, up: Int4Weight | None = None,
+                    out_dtype: torch.dtype = torch.float32, routes=None) -> torch.Tensor:
+    """moe_mm_ids for 4-bit weights with group scales: x [T, K] (gate / up) or [T, n_used, K] (down), contiguous BF16; out
+    [T, n_used, N]; up given: gate / up + SwiGLU together.  A pair whose id names no expert gets zeros, and a token may name an
+    expert more than once.  routes: int4_route(topk_ids, n_experts) if the caller has it."""
+    cw = _c_int4(w)
+    cu = None
+    if up is not None:
+        if up.codes.shape != w.codes.shape or up.group != w.group:
+            raise ValueError("bf16n.int4_moe_mm_ids: gate/up shapes and groups must match")
+        cu = C.byref(_c_int4(up))
+    _check_ids(topk_ids)
+    _check_x(x, cw.K, "x")
+    if x.dtype is not torch.bfloat16 or not x.is_contiguous():
+        raise ValueError("bf16n.int4_moe_mm_ids: x must be contiguous bf16 (BF16 activations)")
+    if n_experts <= 0 or cw.rows % n_experts:
+        raise ValueError("bf16n.int4_moe_mm_ids: rows must split into n_experts")
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("bf16n.int4_moe_mm_ids: results are bf16 or f32")
+    T, n_used = topk_ids.shape
+    N, per_slot, dev = cw.rows // n_experts, x.dim() == 3, x.device
+    if not ((x.dim() == 2 and x.shape[0] == T) or (per_slot and x.shape[0] == T and x.shape[1] == n_used)):
+        raise ValueError("bf16n.int4_moe_mm_ids: x must be [tokens, K] or [tokens, n_used, K]")
+    if w.codes.device != dev or topk_ids.device != dev or (up is not None and up.codes.device != dev):
+        raise ValueError("bf16n.int4_moe_mm_ids: operands on different devices")
+    y = torch.empty((T, n_used, N), dtype=out_dtype, device=dev)
+    if y.numel() == 0:
+        return y
+    pairs, bounds = routes if routes is not None else int4_route(topk_ids, n_experts)
+    if not (pairs.dtype is bounds.dtype is torch.int32 and pairs.numel() == T * n_used and bounds.numel() == n_experts + 2
+            and pairs.is_contiguous() and bounds.is_contiguous() and pairs.device == dev and bounds.device == dev):
+        raise ValueError("bf16n.int4_moe_mm_ids: routes must be int4_route's for these ids")
+    with _on(dev):
+        _lib.check(_lib.lib().bf16n_int4_mm_ids(C.byref(cw), cu, x.data_ptr(), cw.K, per_slot, pairs.data_ptr(), bounds.data_ptr(), y.data_ptr(),
+                                                out_dtype is torch.bfloat16, N, n_experts, T, n_used, _stream()))
+    return y
+
+
+def int4_moe_experts_batched(n_tokens: int, n_used: int, n_experts: int) -> bool:
+    """Whether int4_moe_experts_rows sorts the pairs by expert first, rather than running every pair by itself."""
+    return n_tokens * n_used > max(16, n_experts // 4)
+
+
+def int4_moe_experts_rows(x: torch.Tensor, gate: Int4Weight, up: Int4Weight, down: Int4Weight, topk_ids: torch.Tensor,
+                          n_experts: int) -> torch.Tensor:
+    """The per-(token, slot) outputs down_e(silu(gate_e x) * (up_e x)) of the routed experts, FP32 [T, n_used, H]
+    (moe_experts_rows).  While the pairs are few each is a column of its own with FP32 between the products; beyond that
+    the pairs are sorted by expert, every expert that is named is read once, and the hidden rows are BF16, the matrix cores' operand
+    (a relative 2^-9 each, as in moe_experts_rows; the sum over them averages it out)."""
+    n_mid, n_out = gate.rows // max(n_experts, 1), down.rows // max(n_experts, 1)
+    x = x.contiguous()
+    if int4_moe_experts_batched(x.shape[0], topk_ids.shape[1], n_experts):
+        routes = int4_route(topk_ids, n_experts)
+        hidden = int4_moe_mm_ids(x, topk_ids, gate, n_experts, up=up, out_dtype=torch.bfloat16, routes=routes)
+        return int4_moe_mm_ids(hidden, topk_ids, down, n_experts, routes=routes)
+    return int4_mmv(int4_mmv_glu2(x, gate, up, topk_ids, n_mid), down, topk_ids, n_out)
+
+
+def int4_moe_experts(x: torch.Tensor, gate: Int4Weight, up: Int4Weight, down: Int4Weight, topk_weights: torch.Tensor,
+                     topk_ids: torch.Tensor, n_experts: int) -> torch.Tensor:
+    """Routed experts of one MoE layer on 4-bit weights with group scales, BF16 out (moe_experts)."""
+    return moe_combine(int4_moe_experts_rows(x, gate, up, down, topk_ids, n_experts), topk_weights, torch.bfloat16)
+
+
+def router_topk_grouped(logits: torch.Tensor, k: int, bias: torch.Tensor | None = None, n_groups: int = 1, topk_groups: int | None = None,
+                        scoring: str = "softmax", group_score: str = "max", renorm: bool = True, scale: float = 1.0,
+                        out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """router_topk with softmax or sigmoid scores p, a bias for balance that only the choice sees (c = p + bias, [n_experts] f32)
+    and experts in n_groups equal groups, of which the topk_groups first by their largest c ("max") or the sum of their two
+    largest ("top2") stay open: (weights f32 [T, k], ids int32 [T, k]) of the k largest c, ties to the lower index.  weights: p of the
+    chosen, over their sum if renorm, times scale.  Scores are held in 64 bits.  out as in router_topk."""
+    if not (logits.is_cuda and logits.dim() == 2 and logits.dtype == torch.float32 and logits.stride(1) == 1):
+        raise ValueError("bf16n.router_topk_grouped: logits must be f32 [tokens, n_experts], contiguous along experts")
+    if scoring not in ("softmax", "sigmoid") or group_score not in ("max", "top2"):
+        raise ValueError("bf16n.router_topk_grouped: scoring is softmax or sigmoid, group_score max or top2")
+    T, E = logits.shape
+    dev = logits.device
+    if bias is not None and not (bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == E and bias.device == dev):
+        raise ValueError("bf16n.router_topk_grouped: bias must be contiguous f32 [n_experts] on the logits' device")
+    if out is None:
+        ids = torch.empty((T, k), dtype=torch.int32, device=dev)
+        wts = torch.empty((T, k), dtype=torch.float32, device=dev)
+    else:
+        wts, ids = out
+        if not (wts.dtype == torch.float32 and ids.dtype == torch.int32 and wts.shape == ids.shape and wts.dim() == 2
+                and wts.shape[0] == T and wts.shape[1] >= k and wts.is_contiguous() and ids.is_contiguous()
+                and wts.device == dev and ids.device == dev):
+            raise ValueError("bf16n.router_topk_grouped: out must be contiguous (f32, int32) [tokens, m >= k] tensors on the logits' device")
+    if T == 0:
+        return wts, ids
+    with _on(dev):
+        _lib.check(_lib.lib().bf16n_router_topk_grouped(
+            logits.data_ptr(), logits.stride(0), None if bias is None else bias.data_ptr(), T, E, n_groups,
+            n_groups if topk_groups is None else topk_groups, k, scoring == "sigmoid", group_score == "top2", bool(renorm), C.c_float(scale),
+            ids.data_ptr(), wts.data_ptr(), ids.shape[1], _stream()))
+    return wts, ids

@@ -1,0 +1,258 @@
+"""Products with 4-bit weights and group scales against their definition in 64 bits (int4_exact: the bounds are derived there)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import int4_exact as X
+
+pytestmark = pytest.mark.gpu
+
+
+def weight(ops, rows, K, group, seed, zeros=True, f16=False):
+    m = X.make(rows, K, group, seed, zeros, f16)
+    return (*m, group), ops.Int4Weight(*(None if t is None else t.cuda() for t in m), group)
+
+
+def acts(tokens, K, seed, dtype=torch.bfloat16):
+    return torch.randn((tokens, K), generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+@pytest.mark.parametrize("rows,K,tokens,group", [
+    (1, 32, 1, 32), (15, 64, 2, 64), (17, 96, 3, 32), (33, 160, 5, 128), (256, 2048, 1, 128), (512, 2048, 16, 128), (300, 2048, 17, 64),
+    (129, 2080, 33, 32), (70, 4096, 7, 256), (64, 512, 64, 512), (31, 1024, 100, 128), (40, 9600, 4, 4096), (20, 16384, 6, 64), (5000, 256, 1, 64),
+    (2500, 640, 20, 128)])
+@pytest.mark.parametrize("zeros,f16", [(True, False), (False, True)])
+def test_dense(ops, rows, K, tokens, group, zeros, f16):
+    w, dw = weight(ops, rows, K, group, rows + K, zeros, f16)
+    for dtype in (torch.bfloat16, torch.float32):
+        x = acts(tokens, K, tokens, dtype)
+        y, b = X.product(x, w)
+        for out in (torch.float32, torch.bfloat16):
+            X.check(ops.int4_mmv(x.cuda(), dw, out_dtype=out), y, X.rounded(y, b, out), (dtype, out))
+        w2, dw2 = weight(ops, rows, K, group, rows + K + 1, zeros, not f16)
+        h, hb = X.gated(y, b, *X.product(x, w2))
+        X.check(ops.int4_mmv_glu2(x.cuda(), dw, dw2), h, hb, dtype)
+
+
+@pytest.mark.parametrize("rows,K,tokens,group", [(5, 64, 1, 32), (130, 2048, 9, 128), (257, 1056, 130, 64), (512, 2048, 517, 128), (1000, 512, 300, 32)])
+def test_linear(ops, rows, K, tokens, group):
+    w, dw = weight(ops, rows, K, group, 3)
+    x = acts(tokens, K, 4)
+    y, b = X.product(x, w)
+    X.check(ops.int4_linear(x.cuda(), dw), y, X.rounded(y, b, torch.bfloat16))
+    bias = torch.randn(rows).to(torch.bfloat16)
+    yb = y + bias.double()
+    X.check(ops.int4_linear(x.cuda(), dw, bias.cuda()), yb, X.rounded(yb, b + X.STEP32 * yb.abs(), torch.bfloat16), "bias")
+
+
+def test_linear_takes_views(ops):
+    """Rows apart by more than their length, leading axes, rows that are not 16-byte aligned, no tokens."""
+    w, dw = weight(ops, 48, 128, 64, 5)
+    wide = acts(6, 300, 6).cuda()
+    for x in (wide[:, :128], wide[:, 8:136], wide[:, 3:131], wide.view(2, 3, 300)[..., :128], wide[:0, :128]):
+        y, b = X.product(x.reshape(-1, 128), w)
+        got = ops.int4_linear(x, dw)
+        assert got.shape == (*x.shape[:-1], 48)
+        if x.numel():
+            X.check(got.reshape(-1, 48), y, X.rounded(y, b, torch.bfloat16))
+
+
+@pytest.mark.parametrize("E,N,K,T,n_used,group", [(4, 32, 64, 1, 2, 32), (16, 48, 512, 3, 4, 128), (8, 100, 2048, 2, 8, 64)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_expert_columns(ops, E, N, K, T, n_used, group, dtype):
+    w, dw = weight(ops, E * N, K, group, 7)
+    w2, dw2 = weight(ops, E * N, K, group, 8)
+    g = torch.Generator().manual_seed(9)
+    ids = torch.randint(0, E, (T, n_used), generator=g, dtype=torch.int32)
+    ids[0, 0], ids[-1, -1] = -1, E  # no such expert
+    for x in (acts(T, K, 10, dtype), acts(T * n_used, K, 11, dtype).view(T, n_used, K)):
+        xp = x[:, None].expand(T, n_used, K) if x.dim() == 2 else x
+        for idt in (torch.int32, torch.int64):
+            got = ops.int4_mmv(x.cuda(), dw, ids.to(idt).cuda(), N)
+            glu = ops.int4_mmv_glu2(x.cuda(), dw, dw2, ids.to(idt).cuda(), N, torch.bfloat16)
+            for t in range(T):
+                for i in range(n_used):
+                    e = int(ids[t, i])
+                    if not 0 <= e < E:
+                        assert not got[t, i].any() and not glu[t, i].any()
+                        continue
+                    cut = lambda m: (*(None if p is None else p[e * N: e * N + N] for p in m[:3]), group)  # noqa: E731
+                    y, b = X.product(xp[t, i: i + 1], cut(w))
+                    X.check(got[t, i: i + 1], y, b)
+                    h, hb = X.gated(y, b, *X.product(xp[t, i: i + 1], cut(w2)))
+                    X.check(glu[t, i: i + 1], h, X.rounded(h, hb, torch.bfloat16))
+
+
+@pytest.mark.parametrize("E,T,n_used", [(1, 1, 1), (5, 3, 2), (256, 77, 8), (300, 1, 8), (16, 700, 6), (3, 5000, 4)])
+def test_route(ops, E, T, n_used):
+    ids = torch.randint(-1, E + 1, (T, n_used + 2), generator=torch.Generator().manual_seed(T))
+    for idt in (torch.int32, torch.int64):
+        use = ids.to(idt).cuda()[:, 1: 1 + n_used]
+        if idt is torch.int64:
+            use = use.clone()
+            use[0, 0] += 1 << 32  # an expert only in its lower half
+        pairs, bounds = ops.int4_route(use, E)
+        flat = use.cpu().reshape(-1).long()
+        flat = torch.where((flat >= 0) & (flat < E), flat, E)
+        want = torch.sort(flat, stable=True)
+        assert torch.equal(pairs.cpu().long(), want.indices)
+        assert torch.equal(bounds.cpu().long(), torch.searchsorted(want.values, torch.arange(E + 2)))
+
+
+@pytest.mark.parametrize("E,N,K,T,n_used,group", [(8, 48, 128, 1, 1, 32), (8, 48, 256, 40, 2, 64), (16, 64, 512, 300, 4, 128), (5, 33, 96, 7, 3, 32), (2, 160, 2048, 700, 2, 128)])
+def test_batched_experts(ops, E, N, K, T, n_used, group):
+    w, dw = weight(ops, E * N, K, group, 12)
+    w2, dw2 = weight(ops, E * N, K, group, 13, f16=True)
+    g = torch.Generator().manual_seed(14)
+    ids = torch.randint(0, E, (T, n_used), generator=g, dtype=torch.int32)  # a token may name an expert twice
+    ids[T // 2, 0] = -1
+    ids[-1, -1] = E + 3
+    cut = lambda m, e: (*(None if p is None else p[e * N: e * N + N] for p in m[:3]), group)  # noqa: E731
+    for x in (acts(T, K, 15), acts(T * n_used, K, 16).view(T, n_used, K)):
+        xp = (x[:, None].expand(T, n_used, K) if x.dim() == 2 else x).reshape(-1, K)
+        for out in (torch.float32, torch.bfloat16):
+            got = ops.int4_moe_mm_ids(x.cuda(), ids.cuda(), dw, E, out_dtype=out).reshape(-1, N)
+            glu = ops.int4_moe_mm_ids(x.cuda(), ids.cuda(), dw, E, up=dw2, out_dtype=out).reshape(-1, N)
+            for e in range(E):
+                at = (ids.reshape(-1) == e).nonzero()[:, 0]
+                if len(at):
+                    y, b = X.product(xp[at], cut(w, e))
+                    X.check(got[at.cuda()], y, X.rounded(y, b, out))
+                    h, hb = X.gated(y, b, *X.product(xp[at], cut(w2, e)))
+                    X.check(glu[at.cuda()], h, X.rounded(h, hb, out))
+            none = ((ids < 0) | (ids >= E)).reshape(-1).cuda()
+            assert not got[none].any() and not glu[none].any()
+
+
+def experts_exact(x, ws, E, ids, wts, batched):
+    """(moe_experts' result, bound) with the roundings of either path"""
+    K, T = x.shape[1], x.shape[0]
+    (gate, up, down), n = ws, ids.shape[1]
+    mid = gate[0].shape[0] // E
+    y, b = torch.zeros((T, K), dtype=torch.float64), torch.zeros((T, K), dtype=torch.float64)
+    for e in range(E):
+        tok, slot = (ids == e).nonzero(as_tuple=True)
+        if not len(tok):
+            continue
+        cut = lambda m, r: (*(None if p is None else p[e * r: e * r + r] for p in m[:3]), m[3])  # noqa: E731
+        h, hb = X.gated(*X.product(x[tok], cut(gate, mid)), *X.product(x[tok], cut(up, mid)))
+        if batched:
+            hb = X.rounded(h, hb, torch.bfloat16)
+        d = cut(down, K)
+        o, ob = X.product(h, d)
+        u, s, z = X.parts(*d)
+        ob = ob * 1.01 + hb @ (s * (u - z)).abs().t()
+        wt = wts[tok, slot].double()[:, None]
+        y.index_add_(0, tok, o * wt)
+        b.index_add_(0, tok, (ob + (n + 1) * X.STEP32 * o.abs()) * wt)
+    return y, b
+
+
+@pytest.mark.parametrize("T", [1, 4, 50])
+def test_router_and_experts_together(ops, T):
+    """The selection in groups, then the experts that it named, as a layer runs them, eagerly and as a captured graph."""
+    E, mid, K, k, group = 32, 64, 256, 4, 64
+    ms = [weight(ops, E * r, c, group, 20 + i) for i, (r, c) in enumerate(((mid, K), (mid, K), (K, mid)))]
+    x = acts(T, K, 24)
+    logits = torch.randn((T, E), generator=torch.Generator().manual_seed(25))
+    bias = torch.randn(E, generator=torch.Generator().manual_seed(26)) * 0.1
+    xd, ld, bd = x.cuda(), logits.cuda(), bias.cuda()
+
+    def layer():
+        wts, ids = ops.router_topk_grouped(ld, k, bias=bd, n_groups=4, topk_groups=2, scoring="sigmoid", group_score="top2")
+        return wts, ids, ops.int4_moe_experts(xd, *(d for _, d in ms), wts, ids, E)
+
+    wts, ids, got = layer()
+    y, b = experts_exact(x, [m for m, _ in ms], E, ids.cpu(), wts.cpu(), ops.int4_moe_experts_batched(T, k, E))
+    X.check(got, y, X.rounded(y, b, torch.bfloat16))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = layer()
+    for i in range(3):
+        ld.copy_(torch.randn((T, E), generator=torch.Generator().manual_seed(30 + i)))
+        xd.copy_(acts(T, K, 40 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, e in zip(again, layer()):
+            assert torch.equal(a, e)
+
+
+def test_same_bits_again(ops):
+    _, dw = weight(ops, 4000, 2048, 128, 50)
+    x = acts(20, 2048, 51).cuda()
+    first = ops.int4_mmv(x, dw)
+    assert all(torch.equal(first, ops.int4_mmv(x, dw)) for _ in range(5))
+
+
+def test_not_finite(ops):
+    """An activation that is not finite reaches every result of its own column and no other; so does a scale its row."""
+    _, dw = weight(ops, 64, 256, 64, 52)
+    for dtype in (torch.bfloat16, torch.float32):
+        for bad in (float("inf"), float("-inf"), float("nan")):
+            x = acts(5, 256, 53, dtype)
+            x[2, 77] = bad
+            y = ops.int4_mmv(x.cuda(), dw)
+            assert not torch.isfinite(y[2]).any() and torch.isfinite(y[[0, 1, 3, 4]]).all()
+    dw.scales[7, 1] = float("nan")
+    y = ops.int4_mmv(acts(5, 256, 54).cuda(), dw)
+    assert torch.isnan(y[:, 7]).all() and torch.isfinite(y[:, torch.arange(64) != 7]).all()
+
+
+def test_large_and_small_f32(ops):
+    """FP32 activations keep all their bits over the range of exponents."""
+    w, dw = weight(ops, 32, 256, 64, 55)
+    for scale in (1e-30, 1.0, 1e30):
+        x = acts(3, 256, 56, torch.float32) * scale
+        y, b = X.product(x, w)
+        X.check(ops.int4_mmv(x.cuda(), dw), y, b, scale)
+
+
+def test_other_stream(ops):
+    w, dw = weight(ops, 300, 512, 64, 57)
+    x = acts(9, 512, 58)
+    y, b = X.product(x, w)
+    s = torch.cuda.Stream()
+    xd = x.cuda()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.int4_mmv(xd, dw)
+    s.synchronize()
+    X.check(got, y, b)
+
+
+def test_quantize(ops):
+    """Codes are within half a step of the weight (and a rounding of the scale: the largest weight may lie past the last code by that)."""
+    w = torch.randn((300, 1056), generator=torch.Generator().manual_seed(60)).mul_(0.02).to(torch.bfloat16)
+    w[5, :64] = 0
+    for symmetric in (True, False):
+        for group in (32, 128, 2048):
+            for dt, eps in ((torch.bfloat16, 2.0 ** -8), (torch.float16, 2.0 ** -11)):
+                q = ops.int4_quantize(w.cuda(), group, symmetric, dt)
+                u, s, z = X.parts(q.codes, q.scales, q.zeros, group)
+                # fp16 scales below 2^-14 are denormal: a step of 2^-24
+                slack = 15 * (eps * s.abs() + (2.0 ** -24 if dt is torch.float16 else 0))
+                assert ((s * (u - z) - w.double()).abs() <= (0.5 if symmetric else 1.0) * s * (1 + 2.0 ** -20) + slack).all()
+                assert not (s * (u - z))[5, :32].any()
+
+
+def test_refusals(ops):
+    _, dw = weight(ops, 64, 256, 64, 61)
+    x = acts(4, 256, 62).cuda()
+    ids = torch.zeros((4, 2), dtype=torch.int32, device="cuda")
+    for call in (lambda: ops.int4_mmv(x.half(), dw), lambda: ops.int4_mmv(x[:, :128], dw), lambda: ops.int4_mmv(x.cpu(), dw),
+                 lambda: ops.int4_mmv(x, dw, out_dtype=torch.float16), lambda: ops.int4_mmv(x, dw, rows_per_matrix=32),
+                 lambda: ops.int4_mmv(x, dw, ids, 48), lambda: ops.int4_mmv(x, dw, ids[:3], 32), lambda: ops.int4_mmv(x, dw, ids.float(), 32),
+                 lambda: ops.int4_mmv(x, dw, ids.cpu(), 32), lambda: ops.int4_mmv(x[None], dw),
+                 lambda: ops.int4_mmv(torch.zeros(1028, device="cuda", dtype=torch.bfloat16)[4:].view(4, 256), dw),
+                 lambda: ops.int4_mmv_glu2(x, dw, weight(ops, 32, 256, 64, 1)[1]), lambda: ops.int4_mmv_glu2(x, dw, weight(ops, 64, 256, 32, 1)[1]),
+                 lambda: ops.int4_linear(x.float(), dw), lambda: ops.int4_linear(x[:, :32], dw),
+                 lambda: ops.int4_moe_mm_ids(x, ids, dw, 3), lambda: ops.int4_moe_mm_ids(x.float(), ids, dw, 2),
+                 lambda: ops.int4_moe_mm_ids(x, ids, dw, 2, routes=ops.int4_route(ids, 3)), lambda: ops.int4_route(ids[0], 2)):
+        with pytest.raises(ValueError):
+            call()
