@@ -199,7 +199,11 @@ typedef struct bf16n_int4_weight {
  * bf16n_mmv_args (rows_per_matrix = nrows, row0 = 0; any number of dense columns, at most 65535 with ids); ids: int32, or int64 with
  * ids_i64; an id that names no matrix gives a column of zeros.  x: BF16 or FP32, 16-byte aligned columns.  The result must
  * not overlap x.  An activation that is not finite makes every result of its column not finite (NaN or infinite). */
-int bf16n_int4_mmv(const bf16n_int4_weight * w, const bf16n_int4_weight * up, const bf16n_mmv_args * a, int ids_i64, void * stream);
+int bf16n_int4_mmv(const bf16n_int4_weight * w, const bf16n_int4_weight * up, const bf16n_mmv_args * a, int ids_i64, void * workspace,
+                   uint64_t workspace_bytes, void * stream);
+/* workspace of the products of many columns (more than 32 BF16 columns, or many pairs per matrix): 16-byte aligned device memory,
+ * *bytes for x_rows rows of activations; a call that finds none or less (null and 0 are fine) takes the kernels for few columns. */
+int bf16n_int4_workspace_bytes(const bf16n_int4_weight * w, int64_t x_rows, uint64_t * bytes);
 /* The (token, slot) pairs t * n_used + slot sorted by the matrix that their id names, ascending within one; pairs whose id names
  * none (outside [0, n_matrices)) come last.  Every pair is listed, also where a token names a matrix twice.  pairs:
  * n_tok * n_used entries; bounds: n_matrices + 2 (matrix m has pairs[bounds[m]] .. pairs[bounds[m + 1] - 1], the last range is
@@ -211,7 +215,7 @@ int bf16n_int4_route(const void * ids, int ids_i64, int64_t ids_s0, int64_t ids_
  * with per_slot, for every pair. */
 int bf16n_int4_mm_ids(const bf16n_int4_weight * w, const bf16n_int4_weight * up, const void * x_bf16, int64_t x_row, int per_slot,
                       const int32_t * pairs, const int32_t * bounds, void * dst, int dst_bf16, int64_t dst_col, int n_experts, int n_tok,
-                      int n_used, void * stream);
+                      int n_used, void * workspace, uint64_t workspace_bytes, void * stream);
 /* The router's selection with scores, a bias and groups: p = softmax(logits) or, with sigmoid, 1 / (1 + exp(-logits));
  * c = p + bias (bias: n_experts FP32 or null); the experts lie in n_groups groups of equal size, ranked by their largest c, or
  * with top2 by the sum of their two largest; the k largest c of the topk_groups first groups are taken (ties: lower index),

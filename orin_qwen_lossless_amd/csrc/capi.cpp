@@ -716,7 +716,16 @@ void check_int4(const bf16n_int4_weight * w, const bf16n_int4_weight * up) {
 
 } // namespace
 
-int bf16n_int4_mmv(const bf16n_int4_weight * w, const bf16n_int4_weight * up, const bf16n_mmv_args * a, int ids_i64, void * stream) {
+int bf16n_int4_workspace_bytes(const bf16n_int4_weight * w, int64_t x_rows, uint64_t * bytes) {
+    return guarded([&] {
+        check_int4(w, nullptr);
+        require(bytes && x_rows >= 0, "int4_workspace_bytes: null pointer or negative rows");
+        *bytes = (uint64_t) dev::int4_workspace_bytes(*w, x_rows);
+    });
+}
+
+int bf16n_int4_mmv(const bf16n_int4_weight * w, const bf16n_int4_weight * up, const bf16n_mmv_args * a, int ids_i64, void * workspace,
+                   uint64_t workspace_bytes, void * stream) {
     return guarded([&] {
         ensure_init();
         dev::g_last_kernel.name = nullptr;
@@ -738,7 +747,8 @@ int bf16n_int4_mmv(const bf16n_int4_weight * w, const bf16n_int4_weight * up, co
         } else {
             require(a->nrows == w->rows, "int4_mmv: a dense product uses the whole matrix");
         }
-        dev::launch_int4_mmv(*w, up, *a, ids_i64 != 0, g_cus, (hipStream_t) stream);
+        require(((uintptr_t) workspace & 15) == 0, "int4_mmv: the workspace must be 16-byte aligned");
+        dev::launch_int4_mmv(*w, up, *a, ids_i64 != 0, workspace, workspace ? workspace_bytes : 0, g_cus, (hipStream_t) stream);
         launch_check("int4_mmv");
     });
 }
@@ -758,7 +768,7 @@ int bf16n_int4_route(const void * ids, int ids_i64, int64_t ids_s0, int64_t ids_
 
 int bf16n_int4_mm_ids(const bf16n_int4_weight * w, const bf16n_int4_weight * up, const void * x_bf16, int64_t x_row, int per_slot,
                       const int32_t * pairs, const int32_t * bounds, void * dst, int dst_bf16, int64_t dst_col, int n_experts, int n_tok,
-                      int n_used, void * stream) {
+                      int n_used, void * workspace, uint64_t workspace_bytes, void * stream) {
     return guarded([&] {
         ensure_init();
         dev::g_last_kernel.name = nullptr;
@@ -771,8 +781,9 @@ int bf16n_int4_mm_ids(const bf16n_int4_weight * w, const bf16n_int4_weight * up,
         require(x_bf16 && pairs && bounds && dst, "int4_mm_ids: null pointer");
         require(((uintptr_t) x_bf16 & 15) == 0 && x_row % 8 == 0, "activations must be 16-byte aligned with 16-byte row strides");
         require((uintptr_t) dst % (dst_bf16 ? 2 : 4) == 0 && dst_col >= w->rows / n_experts, "int4_mm_ids: dst must be aligned to its elements, its rows apart");
+        require(((uintptr_t) workspace & 15) == 0, "int4_mm_ids: the workspace must be 16-byte aligned");
         dev::launch_int4_mm_ids(*w, up, x_bf16, x_row, per_slot != 0, pairs, bounds, dst, dst_bf16 != 0, dst_col, n_experts, n_tok, n_used,
-                                g_cus, (hipStream_t) stream);
+                                workspace, workspace ? workspace_bytes : 0, g_cus, (hipStream_t) stream);
         launch_check("int4_mm_ids");
     });
 }

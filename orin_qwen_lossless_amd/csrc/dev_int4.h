@@ -34,6 +34,15 @@ __device__ __forceinline__ bf16x8_t i4_operand(uint32_t w) {
     return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// the same in the columns' own order, two instructions more
+__device__ __forceinline__ bf16x8_t i4_operand_in_order(uint32_t w) {
+    const uint32_t lo = w & 0x0F0F0F0Fu, hi = (w >> 4) & 0x0F0F0F0Fu;
+    const uint32_t l = __builtin_amdgcn_perm(hi, lo, 0x05010400u), h = __builtin_amdgcn_perm(hi, lo, 0x07030602u);
+    const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(l, 512.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(l, 512.f, true);
+    const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(h, 512.f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(h, 512.f, true);
+    return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
 // eight BF16 activations in the operands' column order
 __device__ __forceinline__ u32x4_t i4_order(u32x4_t v) {
     return u32x4_t{__builtin_amdgcn_perm(v[1], v[0], 0x05040100u), __builtin_amdgcn_perm(v[3], v[2], 0x05040100u),

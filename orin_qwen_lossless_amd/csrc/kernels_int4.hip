@@ -309,6 +309,306 @@ __global__ void __launch_bounds__(NW * 64) k_i4_few(const i4_launch p) {
     }
 }
 
+// ---------------------------------------------------------------- many columns
+//
+// The zero points' part of a product,  - sum_g s[r, g] z[r, g] X[t, g]  with X the sum of the activations over group g (of 128
+// columns where it is larger), is a product of its own over the groups.  Both factors are cut into three BF16 parts that add
+// up to them, so that it runs on the matrix cores as well: eight columns for a group, X1 X2 X1 X3 X2 X1 0 0 against
+// Z1 Z1 Z2 Z1 Z2 Z3 0 0 (what is left out is below 2^-23 of the product), instead of four FMAs per result tile and group.
+
+// X of every activation row, in parts: one thread to 32 columns
+__global__ void __launch_bounds__(256) k_i4_sums(const char * x, int64_t x_row, int64_t K, int group, int64_t n_rows, u32x4_t * sums, int64_t sums_row) {
+    const int per = group / 32;                               // threads to a group: 1, 2 or 4
+    const int64_t segs = (K / 32 + per - 1) / per * per;
+    const int64_t i = (int64_t) blockIdx.x * blockDim.x + threadIdx.x;
+    const int64_t row = i / segs, seg = i % segs;
+    float v = 0.f;
+    if (row < n_rows && seg < K / 32) {
+        const u32x4_t * at = (const u32x4_t *) (x + row * x_row + seg * 64);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const u32x4_t d = at[j];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                v += __uint_as_float(d[e] << 16) + __uint_as_float(d[e] & 0xFFFF0000u);
+            }
+        }
+    }
+    if (per > 1) {
+        v += __shfl_xor(v, 1, 64);
+    }
+    if (per > 2) {
+        v += __shfl_xor(v, 2, 64);
+    }
+    if (row < n_rows && seg % per == 0) {
+        uint32_t a, b, c;
+        f32_parts(v, a, b, c);
+        sums[row * sums_row + seg / per] = u32x4_t{a | b << 16, a | c << 16, b | a << 16, 0};
+    }
+}
+
+struct i4_many {
+    i4_matrix w, up;
+    int64_t K, nrows;
+    int group_log2, n_groups;
+    const char * x; int64_t x_row;          // bytes
+    char * y; int64_t y_row;                // bytes
+    bool y_bf16;
+    const u32x4_t * sums; int sums_row;     // groups of a row, of sum_group_log2 columns
+    int sum_group_log2;
+    int ncols;
+    const int32_t * pairs, * bounds;        // lists of columns by matrix, or null
+    int n_matrices, n_used, per_slot;
+    int row_tiles, col_tiles;               // dense: the grid
+};
+
+constexpr int MANY_MAX_MATRICES = 1024;
+
+// A block takes WM * MT * 16 columns and WN * NT * 16 rows (half of them of either matrix where they are gated) and 128 columns of K
+// at a time: the activations' piece goes straight into LDS (two buffers, 16-byte places exchanged by the row's low bits so that
+// the operands' reads find every bank), the codes into registers, both a step ahead; a wavefront turns its own codes into operands,
+// which serve MT tiles.  Every product over a group starts from zero and is added to the result times its scale.
+// Bound by the vector instructions beside the matrix cores' (nine for eight codes and tile of rows, four for a tile of results and group).
+template <int WM, int WN, int MT, int NT, int GM, bool GLU>
+__global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
+    constexpr int THREADS = WM * WN * 64, COLS = WM * MT * 16, ROWS = WN * NT * 16 / (GLU ? 2 : 1);
+    constexpr int NG = GM == 0 ? 1 : GM == 1 ? 2 : 4, LOADS = COLS * 16 / THREADS;
+    static_assert(THREADS == 256 && LOADS * THREADS == COLS * 16, "a thread copies the same place of rows 16 apart");
+    extern __shared__ __align__(16) char lds[]; // two pieces of activations, then the columns' rows
+    int32_t * const x_at = (int32_t *) (lds + 2 * COLS * 256), * const y_at = x_at + COLS;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m16 = lane & 15, q = lane >> 4;
+    const int wm = wave % WM, wn = wave / WM;
+
+    // the block's rows and columns
+    int64_t matrix = 0;
+    int c0, nc, row_tile;
+    if (p.bounds) {
+        // blocks are (matrix, piece of its columns) by row tile: the pieces are counted from the lists' bounds
+        row_tile = blockIdx.x % p.row_tiles;
+        int piece = blockIdx.x / p.row_tiles;
+        int * const found = x_at;
+        if (threadIdx.x == 0) {
+            found[0] = -1;
+        }
+        __syncthreads();
+        if (wave == 0) {
+            int before = 0;
+            for (int b = 0; b < p.n_matrices; b += 64) {
+                const int m = b + lane;
+                const int n = m < p.n_matrices ? p.bounds[m + 1] - p.bounds[m] : 0;
+                const int pieces = (n + COLS - 1) / COLS;
+                int upto = pieces;
+#pragma unroll
+                for (int o = 1; o < 64; o <<= 1) {
+                    const int v = __shfl_up(upto, o, 64);
+                    upto += lane >= o ? v : 0;
+                }
+                const int first = before + upto - pieces;
+                if (piece >= first && piece < first + pieces) {
+                    found[0] = m;
+                    found[1] = piece - first;
+                }
+                before += __shfl(upto, 63, 64);
+            }
+        }
+        __syncthreads();
+        const int m = found[0], k = found[1];
+        __syncthreads();
+        if (m < 0) {
+            return;
+        }
+        matrix = m;
+        c0 = p.bounds[m] + k * COLS;
+        nc = min(COLS, p.bounds[m + 1] - c0);
+    } else {
+        // an XCD takes every eighth block: neighbours there are column tiles of the same rows
+        const int n = p.row_tiles * p.col_tiles, per = (n + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+        if (id >= n) {
+            return;
+        }
+        row_tile = id / p.col_tiles;
+        c0 = id % p.col_tiles * COLS;
+        nc = min(COLS, p.ncols - c0);
+    }
+    for (int i = threadIdx.x; i < COLS; i += THREADS) {
+        const int c = c0 + min(i, nc - 1);
+        const int pair = p.pairs ? p.pairs[c] : c;
+        x_at[i] = p.pairs && !p.per_slot ? pair / p.n_used : pair;
+        y_at[i] = pair;
+    }
+    __syncthreads();
+
+    const int64_t row0 = (int64_t) row_tile * ROWS;
+    const int S = (int) ((p.K + I4_STEP - 1) / I4_STEP), E = (p.sums_row + 15) / 16;
+    const int place = threadIdx.x & 15, octet = place ^ (threadIdx.x >> 4); // what this thread copies: places of rows (threadIdx.x >> 4) + 16 i
+    const auto copy = [&](int step, int buf) {
+        char * const to = lds + buf * COLS * 256 + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int64_t r = x_at[i * 16 + (threadIdx.x >> 4)];
+            const char * src;
+            if (step < E) {
+                src = (const char *) (p.sums + r * p.sums_row + min(step * 16 + octet, p.sums_row - 1));
+            } else {
+                const int64_t k = (int64_t) (step - E) * I4_STEP + octet * 8;
+                src = p.x + r * p.x_row + (k < p.K ? k : 0) * 2; // (behind the last column the codes are zeros)
+            }
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) src,
+                                             (__attribute__((address_space(3))) void *) (to + i * 4096), 16, 0, 0);
+        }
+    };
+    const auto row_of = [&](int n) -> int64_t { // this lane's row of tile n
+        const int t = GLU ? n % (NT / 2) : n;
+        return min(row0 + (wn * (GLU ? NT / 2 : NT) + t) * 16 + m16, p.nrows - 1) + matrix * p.nrows;
+    };
+    const auto of = [&](int n) -> const i4_matrix & { return GLU && n >= NT / 2 ? p.up : p.w; };
+    u32x4_t code[NT], code_next[NT];
+    uint32_t sc[NT * NG], sc_next[NT * NG];
+    const auto load = [&](int s, u32x4_t * c, uint32_t * g) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const int64_t r = row_of(n), at = (int64_t) s * I4_STEP + q * 32;
+            c[n] = *(const u32x4_t *) (of(n).codes + r * (p.K / 2) + (at < p.K ? at : 0) / 2);
+            if (at >= p.K) {
+                c[n] = u32x4_t{};
+            }
+#pragma unroll
+            for (int i = 0; i < NG; i++) {
+                g[n * NG + i] = of(n).scales[r * p.n_groups + min((int) (((int64_t) s * I4_STEP + i * (I4_STEP / NG)) >> p.group_log2), p.n_groups - 1)];
+            }
+        }
+    };
+
+    f32x4_t acc[MT][NT];
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            acc[m][n] = f32x4_t{};
+        }
+    }
+    const f32x4_t none = {};
+    const auto operand = [&](int buf, int m, int o) { // activations of tile m, eight columns from 8 o on
+        const char * at = lds + buf * COLS * 256 + (wm * MT * 16 + m * 16 + m16) * 256 + ((o ^ m16) * 16);
+        return __builtin_bit_cast(bf16x8_t, *(const u32x4_t *) at);
+    };
+    copy(0, 0);
+    for (int step = 0; step < E + S; step++) {
+        const int buf = step & 1;
+        __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0): this wavefront's copies are in LDS
+        __syncthreads();                    // all of them are, and nothing reads the other buffer any more
+        if (step + 1 < E + S) {
+            copy(step + 1, buf ^ 1);
+            if (step + 1 >= E) {
+                load(step + 1 - E, code_next, sc_next);
+            }
+        }
+        if (step < E) {
+            // the zero points' part: groups step * 16 ..
+            const int left = p.sums_row - step * 16;
+            for (int j = 0; j < 4 && j * 4 < left; j++) {
+                const int g = step * 16 + j * 4 + q;
+                const int64_t gi = min((int) (((int64_t) g << p.sum_group_log2) >> p.group_log2), p.n_groups - 1);
+                bf16x8_t zf[NT];
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const int64_t at = row_of(n) * p.n_groups + gi;
+                    const float z = of(n).zeros ? (float) of(n).zeros[at] : 8.f;
+                    const float sz = -i4_scale(of(n).scales[at], of(n).f16) * z;
+                    uint32_t a, b, c;
+                    f32_parts(g < p.sums_row ? sz : 0.f, a, b, c);
+                    zf[n] = __builtin_bit_cast(bf16x8_t, u32x4_t{a | a << 16, b | a << 16, b | c << 16, 0});
+                }
+#pragma unroll
+                for (int m = 0; m < MT; m++) {
+                    const bf16x8_t xf = operand(buf, m, j * 4 + q);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf, zf[n], acc[m][n], 0, 0, 0);
+                    }
+                }
+            }
+        } else {
+            bf16x8_t wf[NT][4];
+            float sv[NT * NG];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const u32x4_t d = GM == 0 ? code[n] : i4_transpose(code[n]);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    wf[n][j] = i4_operand_in_order(d[j]);
+                }
+#pragma unroll
+                for (int i = 0; i < NG; i++) {
+                    sv[n * NG + i] = i4_scale(sc[n * NG + i], of(n).f16);
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                bf16x8_t xf[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    xf[j] = operand(buf, m, GM == 0 ? q * 4 + j : j * 4 + q);
+                }
+#pragma unroll
+                for (int i = 0; i < NG; i++) {
+                    constexpr int J = 4 / NG;
+                    f32x4_t part[NT];
+#pragma unroll
+                    for (int j = 0; j < J; j++) {
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
+                            part[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[i * J + j], wf[n][i * J + j], j ? part[n] : none, 0, 0, 0);
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            acc[m][n][e] = fmaf(sv[n * NG + i], part[n][e], acc[m][n][e]);
+                        }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            code[n] = code_next[n];
+#pragma unroll
+            for (int i = 0; i < NG; i++) {
+                sc[n * NG + i] = sc_next[n * NG + i];
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int c = wm * MT * 16 + m * 16 + q * 4 + e;
+            if (c < nc) {
+                char * const y = p.y + y_at[c] * p.y_row;
+#pragma unroll
+                for (int n = 0; n < (GLU ? NT / 2 : NT); n++) {
+                    const int64_t r = row0 + (wn * (GLU ? NT / 2 : NT) + n) * 16 + m16;
+                    if (r < p.nrows) {
+                        store_y(y, p.y_bf16, r, GLU ? silu(acc[m][n][e]) * acc[m][n + (GLU ? NT / 2 : 0)][e] : acc[m][n][e]);
+                    }
+                }
+            }
+        }
+    }
+}
+
+// zeros for the pairs that name no matrix
+__global__ void __launch_bounds__(256) k_i4_unnamed(const int32_t * pairs, const int32_t * range, char * y, int64_t y_row, int64_t row_bytes) {
+    for (int c = range[0] + blockIdx.x; c < range[1]; c += gridDim.x) {
+        uint16_t * const to = (uint16_t *) (y + pairs[c] * y_row);
+        for (int64_t i = threadIdx.x; i < row_bytes / 2; i += blockDim.x) {
+            to[i] = 0;
+        }
+    }
+}
+
 // ---------------------------------------------------------------- pairs by matrix
 
 // Every (token, slot) pair under the matrix that its id names, in ascending order, and behind them the pairs whose id
@@ -401,6 +701,29 @@ template <int GM> void init_few() {
     raise((const void *) k_i4_few<2, 1, GM, false, false, 8>);
 }
 
+constexpr size_t many_lds(int cols) { return (size_t) 2 * cols * 256 + 2 * cols * 4; }
+
+template <int GM> void init_many() {
+    const auto raise = [](const void * f, int cols) { (void) hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int) many_lds(cols)); };
+    raise((const void *) k_i4_many<2, 2, 4, 4, GM, false>, 128);
+    raise((const void *) k_i4_many<2, 2, 4, 4, GM, true>, 128);
+    raise((const void *) k_i4_many<1, 4, 4, 2, GM, false>, 64);
+    raise((const void *) k_i4_many<1, 4, 4, 2, GM, true>, 64);
+}
+
+template <int GM>
+void pick_many(i4_many & p, bool glu, int cols, hipStream_t stream) {
+    const int rows = glu ? 64 : 128;
+    p.row_tiles = (int) ((p.nrows + rows - 1) / rows);
+    p.col_tiles = (p.ncols + cols - 1) / cols;
+    // lists: no more pieces than full ones and one cut short to a matrix
+    const int64_t pieces = p.bounds ? std::min<int64_t>(p.ncols, p.ncols / cols + p.n_matrices) : p.col_tiles;
+    const int64_t n = p.bounds ? pieces * p.row_tiles : (pieces * p.row_tiles + 7) / 8 * 8;
+    const auto go = [&](auto * kernel) { kernel<<<(unsigned) n, 256, many_lds(cols), stream>>>(p); };
+    cols == 128 ? (glu ? go(k_i4_many<2, 2, 4, 4, GM, true>) : go(k_i4_many<2, 2, 4, 4, GM, false>))
+                : (glu ? go(k_i4_many<1, 4, 4, 2, GM, true>) : go(k_i4_many<1, 4, 4, 2, GM, false>));
+}
+
 i4_matrix matrix_of(const bf16n_int4_weight & w) { return {w.codes, (const uint16_t *) w.scales, w.zeros, w.scales_f16 != 0}; }
 
 i4_launch launch_of(const bf16n_int4_weight & w, const bf16n_int4_weight * up, int64_t nrows) {
@@ -412,6 +735,22 @@ i4_launch launch_of(const bf16n_int4_weight & w, const bf16n_int4_weight * up, i
     p.n_groups = (int) ((w.K + w.group - 1) / w.group);
     p.nrows = nrows;
     return p;
+}
+
+// the sums of the activations' groups, and the products of many columns
+void run_many(const bf16n_int4_weight & w, const bf16n_int4_weight * up, i4_many & p, int64_t x_rows, void * workspace, int cols, hipStream_t stream) {
+    p.w = matrix_of(w);
+    p.up = matrix_of(up ? *up : w);
+    p.K = w.K;
+    p.group_log2 = 31 - __builtin_clz((unsigned) w.group);
+    p.n_groups = (int) ((w.K + w.group - 1) / w.group);
+    p.sum_group_log2 = std::min(p.group_log2, 7);
+    const int group = 1 << p.sum_group_log2, per = group / 32;
+    p.sums = (const u32x4_t *) workspace;
+    p.sums_row = (int) ((w.K + group - 1) / group);
+    const int64_t threads = x_rows * ((w.K / 32 + per - 1) / per * per);
+    k_i4_sums<<<(unsigned) ((threads + 255) / 256), 256, 0, stream>>>(p.x, p.x_row, w.K, group, x_rows, (u32x4_t *) workspace, p.sums_row);
+    (p.group_log2 >= 7 ? pick_many<0> : p.group_log2 == 6 ? pick_many<1> : pick_many<2>)(p, up != nullptr, cols, stream);
 }
 
 void run_few(i4_launch & p, bool glu, bool f32, int max_cols, int64_t matrices, int grid_y, int cus, hipStream_t stream) {
@@ -443,9 +782,29 @@ void int4_init() {
     init_few<0>();
     init_few<1>();
     init_few<2>();
+    init_many<0>();
+    init_many<1>();
+    init_many<2>();
 }
 
-void launch_int4_mmv(const bf16n_int4_weight & w, const bf16n_int4_weight * up, const bf16n_mmv_args & a, bool ids_i64, int cus, hipStream_t stream) {
+int64_t int4_workspace_bytes(const bf16n_int4_weight & w, int64_t x_rows) {
+    const int group = std::min(w.group, I4_STEP);
+    return x_rows * ((w.K + group - 1) / group) * 16;
+}
+
+void launch_int4_mmv(const bf16n_int4_weight & w, const bf16n_int4_weight * up, const bf16n_mmv_args & a, bool ids_i64, void * workspace,
+                     uint64_t workspace_bytes, int cus, hipStream_t stream) {
+    if (!a.ids && a.x_bf16 && a.ncols > 32 && (int64_t) workspace_bytes >= int4_workspace_bytes(w, a.ncols)) {
+        i4_many p = {};
+        p.x = (const char *) a.x; p.x_row = a.x_tok;
+        p.y = (char *) a.y; p.y_row = a.y_tok; p.y_bf16 = a.y_bf16 != 0;
+        p.nrows = a.nrows;
+        p.ncols = a.ncols;
+        p.n_used = 1; p.n_matrices = 1;
+        const int64_t tiles = ((a.nrows + 127) / 128) * ((a.ncols + 127) / 128);
+        run_many(w, up, p, a.ncols, workspace, tiles >= cus ? 128 : 64, stream);
+        return;
+    }
     i4_launch p = launch_of(w, up, a.nrows);
     p.x = (const char *) a.x; p.x_tok = a.x_tok; p.x_slot = a.x_slot;
     p.y = (char *) a.y; p.y_tok = a.y_tok; p.y_slot = a.y_slot; p.y_bf16 = a.y_bf16 != 0;
@@ -469,7 +828,22 @@ void launch_int4_route(const void * ids, bool i64, int64_t s0, int64_t s1, int n
 }
 
 void launch_int4_mm_ids(const bf16n_int4_weight & w, const bf16n_int4_weight * up, const void * x, int64_t x_row, bool per_slot, const int32_t * pairs,
-                        const int32_t * bounds, void * y, bool y_bf16, int64_t y_row, int n_matrices, int n_tok, int n_used, int cus, hipStream_t stream) {
+                        const int32_t * bounds, void * y, bool y_bf16, int64_t y_row, int n_matrices, int n_tok, int n_used, void * workspace, uint64_t workspace_bytes,
+                        int cus, hipStream_t stream) {
+    const int64_t x_rows = per_slot ? (int64_t) n_tok * n_used : n_tok;
+    const int64_t n_pairs = (int64_t) n_tok * n_used;
+    if (n_pairs > 16 * (int64_t) n_matrices && (int64_t) workspace_bytes >= int4_workspace_bytes(w, x_rows)) {
+        i4_many p = {};
+        p.x = (const char *) x; p.x_row = x_row * 2;
+        p.y = (char *) y; p.y_row = y_row * (y_bf16 ? 2 : 4); p.y_bf16 = y_bf16;
+        p.nrows = w.rows / n_matrices;
+        p.ncols = (int) n_pairs;
+        p.pairs = pairs; p.bounds = bounds;
+        p.n_matrices = n_matrices; p.n_used = n_used; p.per_slot = per_slot;
+        run_many(w, up, p, x_rows, workspace, n_pairs > 96 * (int64_t) n_matrices ? 128 : 64, stream);
+        k_i4_unnamed<<<(unsigned) std::min<int64_t>(n_pairs, 64), 256, 0, stream>>>(pairs, bounds + n_matrices, p.y, p.y_row, p.nrows * (y_bf16 ? 2 : 4));
+        return;
+    }
     i4_launch p = launch_of(w, up, w.rows / n_matrices);
     p.x = (const char *) x;
     p.x_tok = x_row * 2 * (per_slot ? n_used : 1);

@@ -108,11 +108,14 @@ void launch_router_topk_grouped(const router_grouped_args & a, int n_tok, hipStr
 
 // 4-bit weights with group scales (kernels_int4.hip)
 void int4_init();
-void launch_int4_mmv(const bf16n_int4_weight & w, const bf16n_int4_weight * up, const bf16n_mmv_args & a, bool ids_i64, int cus, hipStream_t stream);
+void launch_int4_mmv(const bf16n_int4_weight & w, const bf16n_int4_weight * up, const bf16n_mmv_args & a, bool ids_i64, void * workspace,
+                     uint64_t workspace_bytes, int cus, hipStream_t stream);
+int64_t int4_workspace_bytes(const bf16n_int4_weight & w, int64_t x_rows);
 void launch_int4_route(const void * ids, bool i64, int64_t s0, int64_t s1, int n_matrices, int n_tok, int n_used, int32_t * pairs, int32_t * bounds,
                        hipStream_t stream);
 void launch_int4_mm_ids(const bf16n_int4_weight & w, const bf16n_int4_weight * up, const void * x, int64_t x_row, bool per_slot, const int32_t * pairs,
-                        const int32_t * bounds, void * y, bool y_bf16, int64_t y_row, int n_matrices, int n_tok, int n_used, int cus, hipStream_t stream);
+                        const int32_t * bounds, void * y, bool y_bf16, int64_t y_row, int n_matrices, int n_tok, int n_used, void * workspace,
+                        uint64_t workspace_bytes, int cus, hipStream_t stream);
 
 // batched MoE prefill (kernels_mm_ids.hip)
 void mm_ids_init();

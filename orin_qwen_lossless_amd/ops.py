@@ -866,6 +866,9 @@ def moe_experts(x: torch.Tensor, gate: Weight, up: Weight, down: Weight, topk_we
 
 # ---------------------------------------------------------------- 4-bit weights with group scales
 
+INT4_FEW_TOKENS = 32  # columns from which a dense product takes a workspace (bf16n_int4_mmv)
+
+
 @dataclass(frozen=True)
 class Int4Weight:
     """A matrix (or a stack of matrices) of 4-bit codes with group scales on a device:
@@ -957,6 +960,12 @@ def _c_int4(w: Int4Weight) -> _lib.Int4Weight:
                            s.dtype is torch.float16)
 
 
+def _int4_workspace(w: Int4Weight, x_rows: int, device: torch.device) -> torch.Tensor:
+    """Workspace of the products of many columns (bf16n_int4_workspace_bytes): 16 bytes for every group of 128 columns, or
+    smaller, of an activation row."""
+    return torch.empty(16 * x_rows * -(-w.K // min(w.group, 128)), dtype=torch.uint8, device=device)
+
+
 def _int4_mmv(what: str, x: torch.Tensor, w: Int4Weight, up: Int4Weight | None, ids: torch.Tensor | None, rows_per_matrix: int,
               out_dtype: torch.dtype) -> torch.Tensor:
     cw = _c_int4(w)
@@ -1001,8 +1010,12 @@ def _int4_mmv(what: str, x: torch.Tensor, w: Int4Weight, up: Int4Weight | None, 
         isz, per_slot = 8 if i64 else 4, x.dim() == 3
         a = _lib.MmvArgs(x.data_ptr(), y.data_ptr(), ids.data_ptr(), x.stride(0) * xsz, n_used * n * osz, isz, ids.stride(0) * isz,
                          x.stride(1) * xsz if per_slot else 0, n * osz, n, 0, n, T * n_used, n_used, n_used if per_slot else 1, x_bf16, out_bf16)
+    ws, nws = None, 0
+    if ids is None and x_bf16 and T > INT4_FEW_TOKENS:
+        buf = _int4_workspace(w, T, dev)
+        ws, nws = buf.data_ptr(), buf.numel()
     with _on(dev):
-        _lib.check(_lib.lib().bf16n_int4_mmv(C.byref(cw), cu, C.byref(a), i64, _stream()))
+        _lib.check(_lib.lib().bf16n_int4_mmv(C.byref(cw), cu, C.byref(a), i64, ws, nws, _stream()))
     return y
 
 
@@ -1084,9 +1097,13 @@ def int4_moe_mm_ids(x: torch.Tensor, topk_ids: torch.Tensor, w: Int4Weight, n_ex
     if not (pairs.dtype is bounds.dtype is torch.int32 and pairs.numel() == T * n_used and bounds.numel() == n_experts + 2
             and pairs.is_contiguous() and bounds.is_contiguous() and pairs.device == dev and bounds.device == dev):
         raise ValueError("bf16n.int4_moe_mm_ids: routes must be int4_route's for these ids")
+    ws, nws = None, 0
+    if T * n_used > n_experts:
+        buf = _int4_workspace(w, T * n_used if per_slot else T, dev)
+        ws, nws = buf.data_ptr(), buf.numel()
     with _on(dev):
         _lib.check(_lib.lib().bf16n_int4_mm_ids(C.byref(cw), cu, x.data_ptr(), cw.K, per_slot, pairs.data_ptr(), bounds.data_ptr(), y.data_ptr(),
-                                                out_dtype is torch.bfloat16, N, n_experts, T, n_used, _stream()))
+                                                out_dtype is torch.bfloat16, N, n_experts, T, n_used, ws, nws, _stream()))
     return y
 
 
