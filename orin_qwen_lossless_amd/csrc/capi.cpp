@@ -711,7 +711,7 @@ void check_int4(const bf16n_int4_weight * w, const bf16n_int4_weight * up) {
         require(m->rows == 0 || (m->codes && m->scales), "int4: null codes or scales");
         require(((uintptr_t) m->codes & 15) == 0 && ((uintptr_t) m->scales & 1) == 0, "int4: codes must be 16-byte, scales 2-byte aligned");
     }
-    require(!up || (up->K == w->K && up->rows == w->rows && up->group == w->group), "int4: gate/up shapes and groups must match");
+    require(!up || (up->K == w->K && up->rows == w->rows && up->group == w->group && !up->zeros == !w->zeros), "int4: gate/up shapes, groups and zeros must match");
 }
 
 } // namespace
@@ -732,6 +732,7 @@ int bf16n_int4_mmv(const bf16n_int4_weight * w, const bf16n_int4_weight * up, co
         check_int4(w, up);
         require(a && a->ncols > 0, "int4_mmv: ncols out of range");
         require(a->row0 == 0 && a->nrows == a->rows_per_matrix, "int4_mmv: a product takes whole matrices");
+        require(a->nrows <= 1 << 30, "int4_mmv: too many rows in a matrix");
         if (a->nrows == 0) {
             return;
         }
@@ -773,7 +774,8 @@ int bf16n_int4_mm_ids(const bf16n_int4_weight * w, const bf16n_int4_weight * up,
         ensure_init();
         dev::g_last_kernel.name = nullptr;
         check_int4(w, up);
-        require(n_experts > 0 && n_experts <= 65534 && w->rows % n_experts == 0, "int4_mm_ids: rows must split into n_experts");
+        require(n_experts > 0 && n_experts <= 65534 && w->rows % n_experts == 0 && w->rows / n_experts <= 1 << 30,
+                "int4_mm_ids: rows must split into n_experts");
         require(n_tok > 0 && n_used > 0 && (int64_t) n_tok * n_used <= (1 << 28), "int4_mm_ids: sizes out of range");
         if (w->rows == 0) {
             return;

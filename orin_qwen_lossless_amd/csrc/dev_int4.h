@@ -70,8 +70,10 @@ __device__ __forceinline__ void f32_parts(float v, uint32_t & a, uint32_t & b, u
     c = __float_as_uint(l) >> 16;
 }
 
-__device__ __forceinline__ float i4_scale(uint32_t bits, bool f16) {
-    return f16 ? (float) __builtin_bit_cast(_Float16, (uint16_t) bits) : __uint_as_float(bits << 16);
+// f16: all ones or zero (a choice between two registers, not a branch)
+__device__ __forceinline__ float i4_scale(uint32_t bits, uint32_t f16) {
+    const float h = (float) __builtin_bit_cast(_Float16, (uint16_t) bits);
+    return __uint_as_float((__float_as_uint(h) & f16) | ((bits << 16) & ~f16));
 }
 
 } // namespace dev

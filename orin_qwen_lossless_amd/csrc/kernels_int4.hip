@@ -11,10 +11,10 @@ namespace {
 
 struct i4_launch {
     i4_matrix w, up;
-    int64_t K;                              // columns, a multiple of 32
+    int K;                                  // columns, a multiple of 32
     int group_log2, n_groups;
-    int64_t nrows;                          // rows of one matrix that are multiplied
-    const char * x; int64_t x_tok, x_slot;  // bytes
+    int nrows;                              // rows of one matrix
+    const char * x; int64_t x_tok, x_slot;  // bytes; a list's pair takes activation row pair (per_slot) or pair / n_used
     char * y; int64_t y_tok, y_slot;        // bytes
     bool y_bf16;
     int ncols, n_used;                      // columns (dense) or (token, slot) pairs
@@ -29,28 +29,35 @@ constexpr int I4_STEP = 128; // columns that a wavefront takes at a time: 32 to 
 
 // pitch of a row of activations in LDS, in elements: whole steps, and 16 bytes more so that the 16 rows of an operand lie in
 // different banks
-__host__ __device__ inline int64_t i4_pitch(int64_t K) { return (K + I4_STEP - 1) / I4_STEP * I4_STEP + 8; }
+__host__ __device__ inline int i4_pitch(int K) { return (K + I4_STEP - 1) / I4_STEP * I4_STEP + 8; }
 
 // Few columns.  One wavefront takes 16 rows of the matrix (of each of the two where they are gated) and 128 columns of it at
 // a time: a lane's 16 bytes are 32 codes of row lane % 16, turned into four operands of v_mfma_f32_16x16x32_bf16 whose other
 // operand is the activations, from LDS; result: lane = row of the matrix, register = activation row (so that a scale
 // is one value to a lane).  FP32 activations are three BF16 rows each (rows 4 t .. 4 t + 2 of the 16: one lane's registers).
-// The sums of the activations over a group, which the zero points need, come from one more product with ones.
+// The sums of the activations over a group, which the zero points need, are taken once, on the way into LDS.
+// A step's registers take the codes of the step U later as soon as its operands are made.
 // Wavefronts of a block share the rows (ksplit parts of K each, summed through LDS in a fixed order) or take other rows.
 // Bound by HBM where the matrix is large.
-template <int NT, int NM, int GM, bool GLU, bool XF32, int NW>
-__global__ void __launch_bounds__(NW * 64) k_i4_few(const i4_launch p) {
+template <int NT, int NM, int GM, bool GLU, bool XF32, bool ZEROS, int NW>
+__global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i4_launch p) {
     constexpr int U = NM == 1 ? 4 : 2;                  // steps whose codes are loaded ahead
     constexpr int NG = GM == 0 ? 1 : GM == 1 ? 2 : 4;   // groups in a step (128 and more columns, 64, 32)
     constexpr int CPT = XF32 ? 4 : 16;                  // columns in a tile of 16 activation rows
+    constexpr int NA = XF32 ? 1 : 4;                    // results of a lane in a tile
+    constexpr int TILE_ROWS = 16 * (GLU ? 1 : NM);
     extern __shared__ __align__(16) char lds[];
     uint16_t * const xs = (uint16_t *) lds;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m16 = lane & 15, q = lane >> 4;
-    const int64_t K = p.K, pitch = i4_pitch(K);
-    float * const red = (float *) (lds + (size_t) p.cols_per_pass * (XF32 ? 3 : 1) * pitch * 2);
+    const int lane = threadIdx.x & 63, m16 = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int K = p.K, pitch = i4_pitch(K), x_rows = p.cols_per_pass * (XF32 ? 3 : 1);
+    const int steps = (K + I4_STEP - 1) / I4_STEP;
+    float * const xsum = (float *) (xs + x_rows * pitch);          // [steps * NG][NT * CPT]
+    int64_t * const y_off = (int64_t *) (xsum + steps * NG * NT * CPT); // [NT * CPT]
+    float * const red = (float *) (y_off + NT * CPT);
 
     // which matrix, and its columns
-    int64_t matrix = 0;
+    int64_t matrix = 0, x_one = 0, y_one = 0;
     int c_begin = 0, c_end = p.ncols;
     bool named = true;
     if (p.ids) {
@@ -58,59 +65,100 @@ __global__ void __launch_bounds__(NW * 64) k_i4_few(const i4_launch p) {
         const char * at = p.ids + t * p.ids_s1 + i * p.ids_s0;
         matrix = p.ids_i64 ? *(const int64_t *) at : *(const int32_t *) at;
         named = matrix >= 0 && matrix < p.n_matrices;
-        matrix = named ? matrix : 0;
-        c_begin = blockIdx.y;
-        c_end = c_begin + 1;
+        x_one = t * p.x_tok + (i % p.x_per_slot) * p.x_slot;
+        y_one = t * p.y_tok + i * p.y_slot;
+        c_end = 1;
     } else if (p.bounds) {
         matrix = blockIdx.y;
         c_begin = p.bounds[matrix];
         c_end = p.bounds[matrix + 1];
         named = matrix < p.n_matrices; // behind the last one: pairs that name none
-        matrix = named ? matrix : 0;
     }
-    const int64_t row_base = matrix * p.nrows;
-    const int row_groups = NW / p.ksplit, kp = wave % p.ksplit;
-    constexpr int TILE_ROWS = 16 * (GLU ? 1 : NM);
-    const int64_t n_blocks = (p.nrows + (int64_t) row_groups * TILE_ROWS - 1) / (row_groups * TILE_ROWS);
-    const auto column = [&](int c, bool slot_of_x) -> int64_t { // byte offset of column c's activations or results
-        int t = c, i = 0;
+    const auto y_of = [&](int c) -> int64_t { return p.pairs ? p.pairs[c] * p.y_slot : y_one + c * p.y_tok; };
+    const auto x_of = [&](int c) -> int64_t {
         if (p.pairs) {
             const int pair = p.pairs[c];
-            t = pair / p.n_used;
-            i = pair % p.n_used;
-        } else if (p.ids) {
-            t = c / p.n_used;
-            i = c % p.n_used;
+            return p.x_per_slot > 1 ? pair * p.x_slot : pair / p.n_used * p.x_tok;
         }
-        return slot_of_x ? t * p.x_tok + (i % p.x_per_slot) * p.x_slot : t * p.y_tok + i * p.y_slot;
+        return x_one + c * p.x_tok;
     };
     if (!named) { // no such matrix: a row of zeros
         for (int c = c_begin + blockIdx.z; c < c_end; c += gridDim.z) {
-            for (int64_t r = blockIdx.x * (int64_t) blockDim.x + threadIdx.x; r < p.nrows; r += (int64_t) gridDim.x * blockDim.x) {
-                store_y(p.y + column(c, false), p.y_bf16, r, 0.f);
+            for (int r = blockIdx.x * blockDim.x + threadIdx.x; r < p.nrows; r += gridDim.x * blockDim.x) {
+                store_y(p.y + y_of(c), p.y_bf16, r, 0.f);
             }
         }
         return;
     }
 
-    const int steps = (int) ((K + I4_STEP - 1) / I4_STEP);
+    const int row_groups = NW / p.ksplit, kp = wave % p.ksplit;
     const int s0 = steps * kp / p.ksplit, s1 = steps * (kp + 1) / p.ksplit;
     const int n_chunks = (s1 - s0 + U - 1) / U;
-    int x_row = m16 < p.cols_per_pass ? m16 : p.cols_per_pass - 1; // rows beyond the columns repeat the last: their results are dropped
-    if (XF32) {
-        const int t = m16 >> 2, part = m16 & 3;
-        x_row = (t < p.cols_per_pass ? t : p.cols_per_pass - 1) * 3 + (part < 3 ? part : 2);
+    const int block_rows = row_groups * TILE_ROWS;
+    const int first_row = blockIdx.x * block_rows + wave / p.ksplit * TILE_ROWS, row_step = gridDim.x * block_rows;
+    // rows beyond the columns repeat the last: their results are dropped
+    int x_at[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const int c = min(t * CPT + (XF32 ? m16 >> 2 : m16), p.cols_per_pass - 1);
+        x_at[t] = (XF32 ? c * 3 + min(m16 & 3, 2) : c) * pitch + (GM == 0 ? q * 32 : q * 8);
     }
+    // a last step that is cut short: lanes behind the last column read the columns before it, against activations of zero
+    const int tail = (steps - 1) * I4_STEP + q * 32 < K ? 0 : q * 16;
+    const uint32_t f16[2] = {p.w.f16 ? ~0u : 0u, p.up.f16 ? ~0u : 0u};
 
     for (int c0 = c_begin + blockIdx.z * p.cols_per_pass; c0 < c_end; c0 += gridDim.z * p.cols_per_pass) {
         const int nc = min(c_end - c0, p.cols_per_pass);
-        // activations into LDS, in the operands' order, zeros behind the last column of the matrix
-        const int octs = (int) ((pitch - 8) / 8);
+
+        u32x4_t code[U * NM];
+        uint32_t sc[U * NM * NG], ze[U * NM * NG];
+        // where the loads are: a tile's place is the same for all lanes, a lane's offset in it the same for all tiles but one that
+        // the matrix ends in, whose lanes beyond repeat its last row
+        const uint8_t * codes[NM], * zeros[NM];
+        const uint16_t * scales[NM];
+        int code_off[NM], group_off[NM];
+        const auto at_tile = [&](int r0) {
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                const i4_matrix & w = GLU && m ? p.up : p.w;
+                const int r = min(r0 + (GLU ? 0 : 16 * m), p.nrows - 1);
+                const int64_t base = matrix * p.nrows + r;
+                codes[m] = w.codes + base * (K / 2);
+                scales[m] = w.scales + base * p.n_groups;
+                zeros[m] = w.zeros + base * p.n_groups;
+                const int row = min(m16, p.nrows - 1 - r);
+                code_off[m] = row * (K / 2) + q * 16;
+                group_off[m] = row * p.n_groups;
+            }
+        };
+        const auto load = [&](int s, int u) {
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                code[u * NM + m] = *(const u32x4_t *) (codes[m] + s * (I4_STEP / 2) + (code_off[m] - (s == steps - 1 ? tail : 0)));
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    const int gi = min((s * I4_STEP + g * (I4_STEP / NG)) >> p.group_log2, p.n_groups - 1);
+                    sc[(u * NM + m) * NG + g] = (scales[m] + gi)[group_off[m]];
+                    if constexpr (ZEROS) {
+                        ze[(u * NM + m) * NG + g] = (zeros[m] + gi)[group_off[m]];
+                    }
+                }
+            }
+        };
+        at_tile(first_row);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            load(min(s0 + u, s1 - 1), u);
+        }
+
+        // activations into LDS, in the operands' order, zeros behind the last column of the matrix, and their groups' sums
+        const int octs = (pitch - 8) / 8; // a multiple of 16: a row of 16 lanes has 128 columns of one activation row
         __syncthreads();
         for (int i = threadIdx.x; i < p.cols_per_pass * octs; i += NW * 64) {
             const int c = i / octs, o = i % octs;
             const bool in = c < nc && o * 8 < K;
-            const char * src = p.x + column(c0 + (c < nc ? c : 0), true);
+            const char * src = p.x + x_of(c0 + (c < nc ? c : 0));
+            float sum = 0.f;
             if constexpr (XF32) {
                 f32x4_t a = {}, b = {};
                 if (in) {
@@ -120,7 +168,9 @@ __global__ void __launch_bounds__(NW * 64) k_i4_few(const i4_launch p) {
                 uint32_t parts[3][8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    f32_parts(j < 4 ? a[j & 3] : b[j & 3], parts[0][j], parts[1][j], parts[2][j]);
+                    const float v = j < 4 ? a[j & 3] : b[j & 3];
+                    f32_parts(v, parts[0][j], parts[1][j], parts[2][j]);
+                    sum += v;
                 }
 #pragma unroll
                 for (int h = 0; h < 3; h++) {
@@ -134,176 +184,145 @@ __global__ void __launch_bounds__(NW * 64) k_i4_few(const i4_launch p) {
                     v = *(const u32x4_t *) (src + o * 16);
                 }
                 *(u32x4_t *) (xs + c * pitch + o * 8) = i4_order(v);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    sum += __uint_as_float(v[j] << 16) + __uint_as_float(v[j] & 0xFFFF0000u);
+                }
             }
+            sum = dpp_add<0xB1, 0xf>(sum); // over 4, 8 or 16 lanes: 32, 64 or 128 columns
+            sum = dpp_add<0x4E, 0xf>(sum);
+            if (GM < 2) {
+                sum = dpp_add<0x141, 0xf>(sum);
+            }
+            if (GM < 1) {
+                sum = dpp_add<0x140, 0xf>(sum);
+            }
+            constexpr int OG = 16 / NG;
+            if (o % OG == 0) {
+                xsum[o / OG * (NT * CPT) + c] = sum;
+            }
+        }
+        if (threadIdx.x < nc) {
+            y_off[threadIdx.x] = y_of(c0 + threadIdx.x);
         }
         __syncthreads();
 
-        // the codes, scales and zero points of U steps of a tile of rows
-        u32x4_t code_a[U * NM], code_b[U * NM];
-        uint32_t sc_a[U * NM * NG], sc_b[U * NM * NG], ze_a[U * NM * NG], ze_b[U * NM * NG];
-        const auto load = [&](int64_t tile, int chunk, u32x4_t * code, uint32_t * sc, uint32_t * ze) {
+        int parity = 0;
+        const f32x4_t none = {};
+        for (int r0 = first_row; r0 < p.nrows + wave / p.ksplit * TILE_ROWS; r0 += row_step) { // (the block's wavefronts make the same rounds)
+            float acc[NM * NT][NA];
 #pragma unroll
-            for (int m = 0; m < NM; m++) {
-                const i4_matrix & w = GLU && m ? p.up : p.w;
-                const int64_t r = min(tile * TILE_ROWS + (GLU ? 0 : 16 * m) + m16, p.nrows - 1) + row_base;
-                const uint8_t * row = w.codes + r * (K / 2);
-                const uint16_t * srow = w.scales + r * p.n_groups;
-                const uint8_t * zrow = w.zeros ? w.zeros + r * p.n_groups : nullptr;
+            for (int t = 0; t < NM * NT; t++) {
+#pragma unroll
+                for (int e = 0; e < NA; e++) {
+                    acc[t][e] = 0.f;
+                }
+            }
+            for (int chunk = 0; chunk < n_chunks; chunk++) {
+                int ahead = s0 + (chunk + 1) * U;
+                if (chunk + 1 == n_chunks) {
+                    at_tile(r0 + row_step); // behind the matrix: its last row, for nothing
+                    ahead = s0;
+                }
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    const int s = min(s0 + chunk * U + u, s1 - 1);
-                    const int64_t at = (int64_t) s * I4_STEP + q * 32;
-                    code[u * NM + m] = *(const u32x4_t *) (row + (at < K ? at : 0) / 2);
-#pragma unroll
-                    for (int g = 0; g < NG; g++) {
-                        const int gi = min((int) (((int64_t) s * I4_STEP + g * (I4_STEP / NG)) >> p.group_log2), p.n_groups - 1);
-                        sc[(u * NM + m) * NG + g] = srow[gi];
-                        ze[(u * NM + m) * NG + g] = zrow ? zrow[gi] : 8u;
-                    }
-                }
-            }
-        };
-        f32x4_t acc[NM * NT];
-        int parity = 0;
-        const auto compute = [&](int64_t tile, int chunk, const u32x4_t * code, const uint32_t * sc, const uint32_t * ze) {
-            if (chunk == 0) {
-#pragma unroll
-                for (int i = 0; i < NM * NT; i++) {
-                    acc[i] = f32x4_t{};
-                }
-            }
-            const f32x4_t none = {};
-            const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, u32x4_t{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int s = s0 + chunk * U + u;
-                if (s >= s1) {
-                    break;
-                }
-                u32x4_t d[NM];
-#pragma unroll
-                for (int m = 0; m < NM; m++) {
-                    d[m] = GM == 0 ? code[u * NM + m] : i4_transpose(code[u * NM + m]);
-                }
-                const uint16_t * xat = xs + x_row * pitch + s * I4_STEP + (GM == 0 ? q * 32 : q * 8);
-                f32x4_t part[NM * NT], xsum[NT];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    bf16x8_t wf[NM];
-#pragma unroll
-                    for (int m = 0; m < NM; m++) {
-                        wf[m] = i4_operand(d[m][j]);
-                    }
-                    constexpr int J0 = 4 / NG; // operands of a group
-                    const bool first = j % J0 == 0;
-#pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        // a second tile of activation rows lies CPT columns on
-                        const uint16_t * xt = xat + (t ? (int64_t) (min(x_row + t * CPT * (XF32 ? 3 : 1), p.cols_per_pass * (XF32 ? 3 : 1) - 1) - x_row) * pitch : 0);
-                        const bf16x8_t xf = __builtin_bit_cast(bf16x8_t, *(const u32x4_t *) (xt + (GM == 0 ? j * 8 : j * 32)));
-                        xsum[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf, ones, first ? none : xsum[t], 0, 0, 0);
+                    const int s = s0 + chunk * U + u;
+                    if (s < s1) {
+                        u32x4_t d[NM];
+                        float sv[NM * NG], zv[NM * NG];
 #pragma unroll
                         for (int m = 0; m < NM; m++) {
-                            part[m * NT + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf, wf[m], first ? none : part[m * NT + t], 0, 0, 0);
+                            d[m] = GM == 0 ? code[u * NM + m] : i4_transpose(code[u * NM + m]);
+#pragma unroll
+                            for (int g = 0; g < NG; g++) {
+                                sv[m * NG + g] = i4_scale(sc[(u * NM + m) * NG + g], f16[GLU && m]);
+                                zv[m * NG + g] = ZEROS ? (float) ze[(u * NM + m) * NG + g] : 8.f;
+                            }
                         }
-                    }
-                    if (j % J0 == J0 - 1) {
-                        const int g = j / J0;
 #pragma unroll
-                        for (int m = 0; m < NM; m++) {
-                            const float sv = i4_scale(sc[(u * NM + m) * NG + g], (GLU && m ? p.up : p.w).f16);
-                            const float zv = (float) ze[(u * NM + m) * NG + g];
+                        for (int g = 0; g < NG; g++) {
+                            f32x4_t part[NM * NT];
+#pragma unroll
+                            for (int j = g * 4 / NG; j < (g + 1) * 4 / NG; j++) {
+                                const bool first = j == g * 4 / NG;
+                                bf16x8_t wf[NM];
+#pragma unroll
+                                for (int m = 0; m < NM; m++) {
+                                    wf[m] = i4_operand(d[m][j]);
+                                }
+#pragma unroll
+                                for (int t = 0; t < NT; t++) {
+                                    const bf16x8_t xf = __builtin_bit_cast(bf16x8_t, *(const u32x4_t *) (xs + x_at[t] + s * I4_STEP + (GM == 0 ? j * 8 : j * 32)));
+#pragma unroll
+                                    for (int m = 0; m < NM; m++) {
+                                        part[m * NT + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf, wf[m], first ? none : part[m * NT + t], 0, 0, 0);
+                                    }
+                                }
+                            }
 #pragma unroll
                             for (int t = 0; t < NT; t++) {
+                                const float * at = xsum + (s * NG + g) * (NT * CPT) + t * CPT + q * NA;
+                                float x[NA];
+                                if constexpr (XF32) {
+                                    x[0] = at[0];
+                                } else {
+                                    *(f32x4_t *) x = *(const f32x4_t *) at;
+                                }
 #pragma unroll
-                                for (int i = 0; i < (XF32 ? 3 : 4); i++) {
-                                    acc[m * NT + t][i] = fmaf(sv, fmaf(-zv, xsum[t][i], part[m * NT + t][i]), acc[m * NT + t][i]);
+                                for (int m = 0; m < NM; m++) {
+                                    const f32x4_t & pt = part[m * NT + t];
+#pragma unroll
+                                    for (int e = 0; e < NA; e++) {
+                                        const float sum = XF32 ? pt[0] + (pt[1] + pt[2]) : pt[e];
+                                        acc[m * NT + t][e] = fmaf(sv[m * NG + g], fmaf(-zv[m * NG + g], x[e], sum), acc[m * NT + t][e]);
+                                    }
                                 }
                             }
                         }
                     }
+                    load(min(ahead + u, s1 - 1), u);
                 }
             }
-            if (chunk != n_chunks - 1) {
-                return;
-            }
             if (p.ksplit > 1) {
-                float * const buf = red + (size_t) parity * NW * 64 * 4 * NM * NT;
+                float * const buf = red + parity * (NW * 64 * NA * NM * NT);
                 parity ^= 1; // the next tile's sums go elsewhere: the barrier in between is one that the readers of this one pass
 #pragma unroll
                 for (int i = 0; i < NM * NT; i++) {
-                    *(f32x4_t *) (buf + ((wave * NM * NT + i) * 64 + lane) * 4) = acc[i];
+#pragma unroll
+                    for (int e = 0; e < NA; e++) {
+                        buf[((wave * NM * NT + i) * NA + e) * 64 + lane] = acc[i][e];
+                    }
                 }
                 __syncthreads();
                 if (kp != 0) {
-                    return;
+                    continue;
                 }
                 for (int k = 1; k < p.ksplit; k++) {
 #pragma unroll
                     for (int i = 0; i < NM * NT; i++) {
-                        acc[i] += *(const f32x4_t *) (buf + (((wave + k) * NM * NT + i) * 64 + lane) * 4);
+#pragma unroll
+                        for (int e = 0; e < NA; e++) {
+                            acc[i][e] += buf[(((wave + k) * NM * NT + i) * NA + e) * 64 + lane];
+                        }
                     }
                 }
             }
 #pragma unroll
             for (int t = 0; t < NT; t++) {
 #pragma unroll
-                for (int i = 0; i < (XF32 ? 1 : 4); i++) {
-                    const int c = t * CPT + (XF32 ? q : q * 4 + i);
+                for (int e = 0; e < NA; e++) {
+                    const int c = t * CPT + q * NA + e;
                     if (c < nc) {
-                        char * const y = p.y + column(c0 + c, false);
-                        const auto value = [&](int m) {
-                            const f32x4_t & a = acc[m * NT + t];
-                            return XF32 ? a[0] + (a[1] + a[2]) : a[i];
-                        };
-                        if constexpr (GLU) {
-                            const int64_t r = tile * TILE_ROWS + m16;
-                            if (r < p.nrows) {
-                                store_y(y, p.y_bf16, r, silu(value(0)) * value(1));
-                            }
-                        } else {
+                        char * const y = p.y + y_off[c];
 #pragma unroll
-                            for (int m = 0; m < NM; m++) {
-                                const int64_t r = tile * TILE_ROWS + 16 * m + m16;
-                                if (r < p.nrows) {
-                                    store_y(y, p.y_bf16, r, value(m));
-                                }
+                        for (int m = 0; m < (GLU ? 1 : NM); m++) {
+                            const int r = r0 + 16 * m + m16;
+                            if (r < p.nrows) {
+                                store_y(y, p.y_bf16, r, GLU ? silu(acc[t][e]) * acc[(GLU ? NT : 0) + t][e] : acc[m * NT + t][e]);
                             }
                         }
                     }
                 }
-            }
-        };
-
-        // the block's tiles, one chunk of steps after the other, the next one's loads ahead of this one's products
-        const int64_t mine = (n_blocks - blockIdx.x + gridDim.x - 1) / gridDim.x;
-        const int64_t total = mine * n_chunks;
-        int64_t lt = 0, ct = 0;
-        int lc = 0, cc = 0;
-        const auto tile_of = [&](int64_t i) { return (blockIdx.x + i * gridDim.x) * row_groups + wave / p.ksplit; };
-        const auto next = [&](int64_t & t, int & c) {
-            if (++c == n_chunks) {
-                c = 0;
-                t++;
-            }
-        };
-        if (total > 0) {
-            load(tile_of(0), 0, code_a, sc_a, ze_a);
-        }
-        for (int64_t it = 0; it < total; it += 2) {
-            next(lt, lc);
-            if (it + 1 < total) {
-                load(tile_of(lt), lc, code_b, sc_b, ze_b);
-            }
-            compute(tile_of(ct), cc, code_a, sc_a, ze_a);
-            next(ct, cc);
-            if (it + 1 < total) {
-                next(lt, lc);
-                if (it + 2 < total) {
-                    load(tile_of(lt), lc, code_a, sc_a, ze_a);
-                }
-                compute(tile_of(ct), cc, code_b, sc_b, ze_b);
-                next(ct, cc);
             }
         }
     }
@@ -514,7 +533,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
                 for (int n = 0; n < NT; n++) {
                     const int64_t at = row_of(n) * p.n_groups + gi;
                     const float z = of(n).zeros ? (float) of(n).zeros[at] : 8.f;
-                    const float sz = -i4_scale(of(n).scales[at], of(n).f16) * z;
+                    const float sz = -i4_scale(of(n).scales[at], of(n).f16 ? ~0u : 0u) * z;
                     uint32_t a, b, c;
                     f32_parts(g < p.sums_row ? sz : 0.f, a, b, c);
                     zf[n] = __builtin_bit_cast(bf16x8_t, u32x4_t{a | a << 16, b | a << 16, b | c << 16, 0});
@@ -540,7 +559,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
                 }
 #pragma unroll
                 for (int i = 0; i < NG; i++) {
-                    sv[n * NG + i] = i4_scale(sc[n * NG + i], of(n).f16);
+                    sv[n * NG + i] = i4_scale(sc[n * NG + i], of(n).f16 ? ~0u : 0u);
                 }
             }
 #pragma unroll
@@ -665,40 +684,56 @@ __global__ void __launch_bounds__(1024) k_i4_route(const char * ids, int64_t s0,
 
 // ---------------------------------------------------------------- dispatch
 
-template <int NT, int NM, int GM, bool GLU, bool XF32>
-void launch_few(const i4_launch & p, int grid_y, int grid_z, int cus, hipStream_t stream) {
-    constexpr int NW = 8;
-    const int64_t row_groups = NW / p.ksplit, tile_rows = 16 * (GLU ? 1 : NM);
-    const int64_t n_blocks = (p.nrows + row_groups * tile_rows - 1) / (row_groups * tile_rows);
-    const size_t lds = (size_t) p.cols_per_pass * (XF32 ? 3 : 1) * i4_pitch(p.K) * 2 + (p.ksplit > 1 ? 2 * NW * 64 * 16 * NM * NT : 0);
-    const int64_t per_cu = std::max<int64_t>(1, std::min<int64_t>(2, (int64_t) (LDS_BYTES / std::max<size_t>(lds, 1))));
-    const int64_t room = std::max<int64_t>(1, cus * per_cu / std::max(1, std::min(grid_y, 1 << 20)));
-    const int64_t rounds = (n_blocks + room - 1) / room;
-    const dim3 grid((unsigned) ((n_blocks + rounds - 1) / rounds), grid_y, grid_z);
-    k_i4_few<NT, NM, GM, GLU, XF32, NW><<<grid, NW * 64, lds, stream>>>(p);
-}
-
-template <int GM>
-void pick_few(const i4_launch & p, bool glu, bool f32, int nt, int grid_y, int grid_z, int cus, hipStream_t stream) {
-    if (glu) {
-        f32 ? launch_few<1, 2, GM, true, true>(p, grid_y, grid_z, cus, stream)
-            : nt == 1 ? launch_few<1, 2, GM, true, false>(p, grid_y, grid_z, cus, stream) : launch_few<2, 2, GM, true, false>(p, grid_y, grid_z, cus, stream);
-    } else {
-        f32 ? launch_few<1, 1, GM, false, true>(p, grid_y, grid_z, cus, stream)
-            : nt == 1 ? launch_few<1, 1, GM, false, false>(p, grid_y, grid_z, cus, stream) : launch_few<2, 1, GM, false, false>(p, grid_y, grid_z, cus, stream);
-    }
+// LDS of k_i4_few: activations, their groups' sums, the results' places, and two buffers for the parts of K
+size_t few_lds(int K, int cols, bool f32, int nt, int nm, int groups_per_step, int ksplit) {
+    const size_t steps = (size_t) (K + I4_STEP - 1) / I4_STEP, per_tile = f32 ? 4 : 16;
+    return (size_t) cols * (f32 ? 3 : 1) * i4_pitch(K) * 2 + steps * groups_per_step * nt * per_tile * 4 + nt * per_tile * 8
+           + (ksplit > 1 ? (size_t) 2 * 8 * 64 * 4 * (f32 ? 1 : 4) * nm * nt : 0);
 }
 
 constexpr size_t I4_FEW_LDS = 160 * 1024 - 1024;
 
-template <int GM> void init_few() {
-    const auto raise = [](const void * f) { (void) hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int) I4_FEW_LDS); };
-    raise((const void *) k_i4_few<1, 2, GM, true, true, 8>);
-    raise((const void *) k_i4_few<1, 2, GM, true, false, 8>);
-    raise((const void *) k_i4_few<2, 2, GM, true, false, 8>);
-    raise((const void *) k_i4_few<1, 1, GM, false, true, 8>);
-    raise((const void *) k_i4_few<1, 1, GM, false, false, 8>);
-    raise((const void *) k_i4_few<2, 1, GM, false, false, 8>);
+struct few_plan { int nt, grid_y, grid_z, cus; hipStream_t stream; bool raise_limits; };
+
+template <int NT, int GM, bool GLU, bool XF32, bool ZEROS>
+void launch_few(const i4_launch & p, const few_plan & f) {
+    constexpr int NW = 8, NM = GLU ? 2 : 1;
+    const auto kernel = k_i4_few<NT, NM, GM, GLU, XF32, ZEROS, NW>;
+    if (f.raise_limits) {
+        (void) hipFuncSetAttribute((const void *) kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int) I4_FEW_LDS);
+        return;
+    }
+    const int block_rows = NW / p.ksplit * 16;
+    const int n_blocks = (p.nrows + block_rows - 1) / block_rows;
+    const size_t lds = few_lds(p.K, p.cols_per_pass, XF32, NT, NM, GM == 0 ? 1 : GM == 1 ? 2 : 4, p.ksplit);
+    // one matrix: as many blocks as the device holds, each with its share of the rows; more matrices: a block to a piece of rows
+    const int room = f.cus * (int) std::min<size_t>(2, LDS_BYTES / lds);
+    const int rounds = f.grid_y > 1 ? 1 : (n_blocks + room - 1) / room;
+    kernel<<<dim3((n_blocks + rounds - 1) / rounds, f.grid_y, f.grid_z), NW * 64, lds, f.stream>>>(p);
+}
+
+template <int GM, bool ZEROS>
+void pick_few(const i4_launch & p, bool glu, bool f32, const few_plan & f) {
+    if (glu) {
+        f32 ? launch_few<1, GM, true, true, ZEROS>(p, f) : f.nt == 1 ? launch_few<1, GM, true, false, ZEROS>(p, f) : launch_few<2, GM, true, false, ZEROS>(p, f);
+    } else {
+        f32 ? launch_few<1, GM, false, true, ZEROS>(p, f) : f.nt == 1 ? launch_few<1, GM, false, false, ZEROS>(p, f) : launch_few<2, GM, false, false, ZEROS>(p, f);
+    }
+}
+
+void pick_few(const i4_launch & p, bool glu, bool f32, int gm, bool zeros, const few_plan & f) {
+    zeros ? (gm == 0 ? pick_few<0, true> : gm == 1 ? pick_few<1, true> : pick_few<2, true>)(p, glu, f32, f)
+          : (gm == 0 ? pick_few<0, false> : gm == 1 ? pick_few<1, false> : pick_few<2, false>)(p, glu, f32, f);
+}
+
+void init_few() {
+    for (int i = 0; i < 48; i++) { // every instance
+        const i4_launch none = {};
+        const few_plan f = {(i & 1) + 1, 0, 0, 0, nullptr, true};
+        if ((i & 24) != 24) {
+            pick_few(none, i & 2, i & 4, i >> 3 & 3, i & 32, f);
+        }
+    }
 }
 
 constexpr size_t many_lds(int cols) { return (size_t) 2 * cols * 256 + 2 * cols * 4; }
@@ -730,10 +765,10 @@ i4_launch launch_of(const bf16n_int4_weight & w, const bf16n_int4_weight * up, i
     i4_launch p = {};
     p.w = matrix_of(w);
     p.up = matrix_of(up ? *up : w);
-    p.K = w.K;
+    p.K = (int) w.K;
     p.group_log2 = 31 - __builtin_clz((unsigned) w.group);
     p.n_groups = (int) ((w.K + w.group - 1) / w.group);
-    p.nrows = nrows;
+    p.nrows = (int) nrows;
     return p;
 }
 
@@ -753,35 +788,30 @@ void run_many(const bf16n_int4_weight & w, const bf16n_int4_weight * up, i4_many
     (p.group_log2 >= 7 ? pick_many<0> : p.group_log2 == 6 ? pick_many<1> : pick_many<2>)(p, up != nullptr, cols, stream);
 }
 
-void run_few(i4_launch & p, bool glu, bool f32, int max_cols, int64_t matrices, int grid_y, int cus, hipStream_t stream) {
-    const int64_t pitch = i4_pitch(p.K) * 2 * (f32 ? 3 : 1);
-    const int steps = (int) ((p.K + I4_STEP - 1) / I4_STEP);
-    const int nm = glu ? 2 : 1;
-    int nt = !f32 && max_cols > 16 ? 2 : 1;
+void run_few(i4_launch & p, bool glu, bool f32, bool zeros, int max_cols, int64_t matrices, int grid_y, int cus, hipStream_t stream) {
+    const int steps = (p.K + I4_STEP - 1) / I4_STEP;
+    const int gm = p.group_log2 >= 7 ? 0 : p.group_log2 == 6 ? 1 : 2;
     // parts of K: as many as make two wavefronts for every SIMD of the device out of the tiles of 16 rows
     const int64_t tiles = (p.nrows + 15) / 16 * matrices;
     int ksplit = 1;
     while (ksplit < 8 && ksplit * 2 <= steps && tiles * ksplit < 8 * cus) {
         ksplit *= 2;
     }
-    const auto red = [&](int tiles_of_cols) { return ksplit > 1 ? (int64_t) 2 * 8 * 64 * 16 * nm * tiles_of_cols : 0; };
-    if (nt == 2 && 32 * pitch + red(2) > (int64_t) I4_FEW_LDS) {
-        nt = 1;
+    const auto fits = [&](int cols, int nt) { return few_lds(p.K, cols, f32, nt, glu ? 2 : 1, 1 << gm, ksplit) <= I4_FEW_LDS; };
+    const int nt = !f32 && max_cols > 16 && fits(32, 2) ? 2 : 1;
+    p.cols_per_pass = std::min(max_cols, f32 ? 4 : 16 * nt);
+    while (!fits(p.cols_per_pass, nt)) {
+        p.cols_per_pass--;
     }
-    const int64_t fit = ((int64_t) I4_FEW_LDS - red(nt)) / pitch;
-    p.cols_per_pass = (int) std::min<int64_t>({max_cols, f32 ? 4 : 16 * nt, fit});
     p.ksplit = ksplit;
-    const int passes = p.bounds ? 1 : p.ids ? 1 : (max_cols + p.cols_per_pass - 1) / p.cols_per_pass;
-    const int gm = p.group_log2 >= 7 ? 0 : p.group_log2 == 6 ? 1 : 2;
-    (gm == 0 ? pick_few<0> : gm == 1 ? pick_few<1> : pick_few<2>)(p, glu, f32, nt, grid_y, passes, cus, stream);
+    const int passes = p.bounds || p.ids ? 1 : std::min(65535, (max_cols + p.cols_per_pass - 1) / p.cols_per_pass);
+    pick_few(p, glu, f32, gm, zeros, {nt, grid_y, passes, cus, stream, false});
 }
 
 } // namespace
 
 void int4_init() {
-    init_few<0>();
-    init_few<1>();
-    init_few<2>();
+    init_few();
     init_many<0>();
     init_many<1>();
     init_many<2>();
@@ -814,9 +844,9 @@ void launch_int4_mmv(const bf16n_int4_weight & w, const bf16n_int4_weight * up, 
     p.ids = (const char *) a.ids; p.ids_s0 = a.ids_s0; p.ids_s1 = a.ids_s1; p.ids_i64 = ids_i64;
     p.n_matrices = a.ids ? w.rows / a.rows_per_matrix : 1;
     if (a.ids) {
-        run_few(p, up != nullptr, !a.x_bf16, 1, a.ncols, a.ncols, cus, stream);
+        run_few(p, up != nullptr, !a.x_bf16, w.zeros != nullptr, 1, a.ncols, a.ncols, cus, stream);
     } else {
-        run_few(p, up != nullptr, !a.x_bf16, a.ncols, 1, 1, cus, stream);
+        run_few(p, up != nullptr, !a.x_bf16, w.zeros != nullptr, a.ncols, 1, 1, cus, stream);
     }
 }
 
@@ -846,9 +876,8 @@ void launch_int4_mm_ids(const bf16n_int4_weight & w, const bf16n_int4_weight * u
     }
     i4_launch p = launch_of(w, up, w.rows / n_matrices);
     p.x = (const char *) x;
-    p.x_tok = x_row * 2 * (per_slot ? n_used : 1);
-    p.x_slot = x_row * 2;
-    p.x_per_slot = per_slot ? n_used : 1;
+    p.x_tok = p.x_slot = x_row * 2;
+    p.x_per_slot = per_slot ? 2 : 1;
     p.y = (char *) y;
     p.y_slot = y_row * (y_bf16 ? 2 : 4);
     p.y_tok = p.y_slot * n_used;
@@ -857,9 +886,9 @@ void launch_int4_mm_ids(const bf16n_int4_weight & w, const bf16n_int4_weight * u
     p.n_used = n_used;
     p.pairs = pairs; p.bounds = bounds;
     p.n_matrices = n_matrices;
-    const int64_t even = (p.ncols + n_matrices - 1) / n_matrices;
-    run_few(p, up != nullptr, false, (int) std::min<int64_t>(p.ncols, std::max<int64_t>(16, even + even / 2)), std::min<int64_t>(n_matrices, p.ncols),
-            n_matrices + 1, cus, stream);
+    const int even = (p.ncols + n_matrices - 1) / n_matrices;
+    const int cols = std::min(p.ncols, even <= 2 ? 4 : even <= 5 ? 8 : 16); // room for twice an even share
+    run_few(p, up != nullptr, false, w.zeros != nullptr, cols, std::min<int64_t>(n_matrices, p.ncols), n_matrices + 1, cus, stream);
 }
 
 } // namespace dev

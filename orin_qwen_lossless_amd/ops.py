@@ -971,8 +971,8 @@ def _int4_mmv(what: str, x: torch.Tensor, w: Int4Weight, up: Int4Weight | None, 
     cw = _c_int4(w)
     cu = None
     if up is not None:
-        if up.codes.shape != w.codes.shape or up.group != w.group:
-            raise ValueError(f"bf16n.{what}: gate/up shapes and groups must match")
+        if up.codes.shape != w.codes.shape or up.group != w.group or (up.zeros is None) != (w.zeros is None):
+            raise ValueError(f"bf16n.{what}: gate/up shapes, groups and zeros must match")
         cu = C.byref(_c_int4(up))
     _check_x(x, cw.K, "x")
     if out_dtype not in (torch.bfloat16, torch.float32):
@@ -1073,8 +1073,8 @@ def int4_moe_mm_ids(x: torch.Tensor, topk_ids: torch.Tensor, w: Int4Weight, n_ex
     cw = _c_int4(w)
     cu = None
     if up is not None:
-        if up.codes.shape != w.codes.shape or up.group != w.group:
-            raise ValueError("bf16n.int4_moe_mm_ids: gate/up shapes and groups must match")
+        if up.codes.shape != w.codes.shape or up.group != w.group or (up.zeros is None) != (w.zeros is None):
+            raise ValueError("bf16n.int4_moe_mm_ids: gate/up shapes, groups and zeros must match")
         cu = C.byref(_c_int4(up))
     _check_ids(topk_ids)
     _check_x(x, cw.K, "x")

@@ -30,7 +30,7 @@ def test_dense(ops, rows, K, tokens, group, zeros, f16):
         y, b = X.product(x, w)
         for out in (torch.float32, torch.bfloat16):
             X.check(ops.int4_mmv(x.cuda(), dw, out_dtype=out), y, X.rounded(y, b, out), (dtype, out))
-        w2, dw2 = weight(ops, rows, K, group, rows + K + 1, zeros, not f16)
+        w2, dw2 = weight(ops, rows, K, group, rows + K + 1, zeros, not f16)  # (gate and up may differ in the scales' type)
         h, hb = X.gated(y, b, *X.product(x, w2))
         X.check(ops.int4_mmv_glu2(x.cuda(), dw, dw2), h, hb, dtype)
 
@@ -251,6 +251,7 @@ def test_refusals(ops):
                  lambda: ops.int4_mmv(x, dw, ids.cpu(), 32), lambda: ops.int4_mmv(x[None], dw),
                  lambda: ops.int4_mmv(torch.zeros(1028, device="cuda", dtype=torch.bfloat16)[4:].view(4, 256), dw),
                  lambda: ops.int4_mmv_glu2(x, dw, weight(ops, 32, 256, 64, 1)[1]), lambda: ops.int4_mmv_glu2(x, dw, weight(ops, 64, 256, 32, 1)[1]),
+                 lambda: ops.int4_mmv_glu2(x, dw, weight(ops, 64, 256, 64, 1, False)[1]),
                  lambda: ops.int4_linear(x.float(), dw), lambda: ops.int4_linear(x[:, :32], dw),
                  lambda: ops.int4_moe_mm_ids(x, ids, dw, 3), lambda: ops.int4_moe_mm_ids(x.float(), ids, dw, 2),
                  lambda: ops.int4_moe_mm_ids(x, ids, dw, 2, routes=ops.int4_route(ids, 3)), lambda: ops.int4_route(ids[0], 2)):
