@@ -31,8 +31,9 @@ constexpr int I4_STEP = 128; // columns that a wavefront takes at a time: 32 to 
 // different banks
 __host__ __device__ inline int i4_pitch(int K) { return (K + I4_STEP - 1) / I4_STEP * I4_STEP + 8; }
 
-// Few columns.  One wavefront takes 16 rows of the matrix (of each of the two where they are gated) and 128 columns of it at
-// a time: a lane's 16 bytes are 32 codes of row lane % 16, turned into four operands of v_mfma_f32_16x16x32_bf16 whose other
+// Few columns.  One wavefront takes 16 rows of the matrix (of each of the two where they are gated) and 256 columns of it at
+// a time: a lane's 32 bytes are 64 codes of row lane % 16 (four lanes have 128 bytes of a row, a whole line: 64 of them at a time
+// took 72 us where the lines whole take @@), turned into eight operands of v_mfma_f32_16x16x32_bf16 whose other
 // operand is the activations, from LDS; result: lane = row of the matrix, register = activation row (so that a scale
 // is one value to a lane).  FP32 activations are three BF16 rows each (rows 4 t .. 4 t + 2 of the 16: one lane's registers).
 // The sums of the activations over a group, which the zero points need, are taken once, on the way into LDS.
@@ -41,8 +42,8 @@ __host__ __device__ inline int i4_pitch(int K) { return (K + I4_STEP - 1) / I4_S
 // Bound by HBM where the matrix is large.
 template <int NT, int NM, int GM, bool GLU, bool XF32, bool ZEROS, int NW>
 __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i4_launch p) {
-    constexpr int U = NM == 1 ? 4 : 2;                  // steps whose codes are loaded ahead
-    constexpr int NG = GM == 0 ? 1 : GM == 1 ? 2 : 4;   // groups in a step (128 and more columns, 64, 32)
+    constexpr int U = NM == 1 ? 2 : 1;                  // pairs of steps whose codes are loaded ahead
+    constexpr int NG = GM == 0 ? 1 : GM == 1 ? 2 : 4;   // groups in a step of 128 columns (128 and more columns, 64, 32)
     constexpr int CPT = XF32 ? 4 : 16;                  // columns in a tile of 16 activation rows
     constexpr int NA = XF32 ? 1 : 4;                    // results of a lane in a tile
     constexpr int TILE_ROWS = 16 * (GLU ? 1 : NM);
@@ -92,7 +93,7 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
     }
 
     const int row_groups = NW / p.ksplit, kp = wave % p.ksplit;
-    const int s0 = steps * kp / p.ksplit, s1 = steps * (kp + 1) / p.ksplit;
+    const int pairs = (steps + 1) / 2, s0 = pairs * kp / p.ksplit, s1 = pairs * (kp + 1) / p.ksplit;
     const int n_chunks = (s1 - s0 + U - 1) / U;
     const int block_rows = row_groups * TILE_ROWS;
     const int first_row = blockIdx.x * block_rows + wave / p.ksplit * TILE_ROWS, row_step = gridDim.x * block_rows;
@@ -101,22 +102,20 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
 #pragma unroll
     for (int t = 0; t < NT; t++) {
         const int c = min(t * CPT + (XF32 ? m16 >> 2 : m16), p.cols_per_pass - 1);
-        x_at[t] = (XF32 ? c * 3 + min(m16 & 3, 2) : c) * pitch + (GM == 0 ? q * 32 : q * 8);
+        x_at[t] = (XF32 ? c * 3 + min(m16 & 3, 2) : c) * pitch + (GM == 0 ? (q & 1) * 64 + (q >> 1) * 32 : q * 8);
     }
-    // a last step that is cut short: lanes behind the last column read the columns before it, against activations of zero
-    const int tail = (steps - 1) * I4_STEP + q * 32 < K ? 0 : q * 16;
+    // a last pair that is cut short: lanes behind the last column read the columns before it, against activations of zero
+    const int at_last = (pairs - 1) * 2 * I4_STEP + q * 64, tail[2] = {at_last < K ? 0 : q * 32, at_last + 32 < K ? 0 : q * 32 + 16};
     const uint32_t f16[2] = {p.w.f16 ? ~0u : 0u, p.up.f16 ? ~0u : 0u};
 
     for (int c0 = c_begin + blockIdx.z * p.cols_per_pass; c0 < c_end; c0 += gridDim.z * p.cols_per_pass) {
         const int nc = min(c_end - c0, p.cols_per_pass);
 
-        u32x4_t code[U * NM];
-        uint32_t sc[U * NM * NG], ze[U * NM * NG];
+        u32x4_t code[U * NM * 2];
         // where the loads are: a tile's place is the same for all lanes, a lane's offset in it the same for all tiles but one that
         // the matrix ends in, whose lanes beyond repeat its last row
-        const uint8_t * codes[NM], * zeros[NM];
-        const uint16_t * scales[NM];
-        int code_off[NM], group_off[NM];
+        const uint8_t * codes[NM];
+        int code_off[NM];
         const auto at_tile = [&](int r0) {
 #pragma unroll
             for (int m = 0; m < NM; m++) {
@@ -124,28 +123,47 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
                 const int r = min(r0 + (GLU ? 0 : 16 * m), p.nrows - 1);
                 const int64_t base = matrix * p.nrows + r;
                 codes[m] = w.codes + base * (K / 2);
-                scales[m] = w.scales + base * p.n_groups;
-                zeros[m] = w.zeros + base * p.n_groups;
-                const int row = min(m16, p.nrows - 1 - r);
-                code_off[m] = row * (K / 2) + q * 16;
-                group_off[m] = row * p.n_groups;
+                code_off[m] = min(m16, p.nrows - 1 - r) * (K / 2) + q * 32;
             }
         };
         const auto load = [&](int s, int u) {
 #pragma unroll
             for (int m = 0; m < NM; m++) {
-                code[u * NM + m] = *(const u32x4_t *) (codes[m] + s * (I4_STEP / 2) + (code_off[m] - (s == steps - 1 ? tail : 0)));
 #pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    const int gi = min((s * I4_STEP + g * (I4_STEP / NG)) >> p.group_log2, p.n_groups - 1);
-                    sc[(u * NM + m) * NG + g] = (scales[m] + gi)[group_off[m]];
-                    if constexpr (ZEROS) {
-                        ze[(u * NM + m) * NG + g] = (zeros[m] + gi)[group_off[m]];
+                for (int h = 0; h < 2; h++) {
+                    code[(u * NM + m) * 2 + h] = *(const u32x4_t *) (codes[m] + s * I4_STEP + h * 16 + (code_off[m] - (s == pairs - 1 ? tail[h] : 0)));
+                }
+            }
+        };
+        // Scales and zero points come by blocks of 16 groups, four of its row to a lane of each quarter, a block ahead; a step takes
+        // them from the quarter that has its group.  (A load of one scale by every lane for every 128 columns: 72 us where this takes @@.)
+        uint32_t sc[NM][2], ze[NM], sc_next[NM][2], ze_next[NM];
+        const auto block_of = [&](int s) { return (s * 2 * I4_STEP >> p.group_log2) >> 4; };
+        const auto first_of = [&](int block, int quarter) { return max(min(block * 16 + quarter * 4, p.n_groups - 4), 0); };
+        const auto load_block = [&](int r0, int block) {
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                const i4_matrix & w = GLU && m ? p.up : p.w;
+                const int r = min(r0 + (GLU ? 0 : 16 * m), p.nrows - 1);
+                const int64_t base = (matrix * p.nrows + r) * p.n_groups;
+                const int at = min(m16, p.nrows - 1 - r) * p.n_groups + first_of(block, q);
+                if (p.n_groups >= 4) {
+                    __builtin_memcpy(sc_next[m], w.scales + base + at, 8); // (aligned to two bytes)
+                    if (ZEROS) {
+                        __builtin_memcpy(&ze_next[m], w.zeros + base + at, 4);
+                    }
+                } else {
+                    const int i1 = min(1, p.n_groups - 1), i2 = min(2, p.n_groups - 1);
+                    sc_next[m][0] = w.scales[base + at] | (uint32_t) w.scales[base + at + i1] << 16;
+                    sc_next[m][1] = w.scales[base + at + i2];
+                    if (ZEROS) {
+                        ze_next[m] = w.zeros[base + at] | w.zeros[base + at + i1] << 8 | w.zeros[base + at + i2] << 16;
                     }
                 }
             }
         };
         at_tile(first_row);
+        load_block(first_row, block_of(s0));
 #pragma unroll
         for (int u = 0; u < U; u++) {
             load(min(s0 + u, s1 - 1), u);
@@ -228,53 +246,89 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
                 for (int u = 0; u < U; u++) {
                     const int s = s0 + chunk * U + u;
                     if (s < s1) {
-                        u32x4_t d[NM];
-                        float sv[NM * NG], zv[NM * NG];
+                        const int block = block_of(s);
+                        if (s == s0 || block != block_of(s - 1)) {
+#pragma unroll
+                            for (int m = 0; m < NM; m++) {
+                                sc[m][0] = sc_next[m][0];
+                                sc[m][1] = sc_next[m][1];
+                                ze[m] = ze_next[m];
+                            }
+                            const bool more = block < block_of(s1 - 1);
+                            load_block(more ? r0 : r0 + row_step, more ? block + 1 : block_of(s0));
+                        }
+                        // the words of the two steps: lanes of the upper half wave give theirs of the first for the lower half's of the second
+                        u32x4_t d[2][NM];
 #pragma unroll
                         for (int m = 0; m < NM; m++) {
-                            d[m] = GM == 0 ? code[u * NM + m] : i4_transpose(code[u * NM + m]);
+                            const u32x4_t & a = code[(u * NM + m) * 2], & b = code[(u * NM + m) * 2 + 1];
 #pragma unroll
-                            for (int g = 0; g < NG; g++) {
-                                sv[m * NG + g] = i4_scale(sc[(u * NM + m) * NG + g], f16[GLU && m]);
-                                zv[m * NG + g] = ZEROS ? (float) ze[(u * NM + m) * NG + g] : 8.f;
+                            for (int j = 0; j < 4; j++) {
+                                const auto r = __builtin_amdgcn_permlane32_swap(a[j], b[j], false, false);
+                                d[0][m][j] = r[0];
+                                d[1][m][j] = r[1];
                             }
                         }
 #pragma unroll
-                        for (int g = 0; g < NG; g++) {
-                            f32x4_t part[NM * NT];
+                        for (int h = 0; h < 2; h++) {
+                            if (h && s * 2 + 1 == steps) {
+                                break;
+                            }
+                            float sv[NM * NG], zv[NM * NG];
 #pragma unroll
-                            for (int j = g * 4 / NG; j < (g + 1) * 4 / NG; j++) {
-                                const bool first = j == g * 4 / NG;
-                                bf16x8_t wf[NM];
-#pragma unroll
-                                for (int m = 0; m < NM; m++) {
-                                    wf[m] = i4_operand(d[m][j]);
+                            for (int m = 0; m < NM; m++) {
+                                if (GM) {
+                                    d[h][m] = i4_transpose(d[h][m]); // (quarter 1 has the third 32 columns here, quarter 2 the second)
+                                    const uint32_t v = d[h][m][1];
+                                    d[h][m][1] = d[h][m][2];
+                                    d[h][m][2] = v;
                                 }
 #pragma unroll
-                                for (int t = 0; t < NT; t++) {
-                                    const bf16x8_t xf = __builtin_bit_cast(bf16x8_t, *(const u32x4_t *) (xs + x_at[t] + s * I4_STEP + (GM == 0 ? j * 8 : j * 32)));
-#pragma unroll
-                                    for (int m = 0; m < NM; m++) {
-                                        part[m * NT + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf, wf[m], first ? none : part[m * NT + t], 0, 0, 0);
-                                    }
+                                for (int g = 0; g < NG; g++) {
+                                    const int gi = min((s * 2 + h) * I4_STEP + g * (I4_STEP / NG) >> p.group_log2, p.n_groups - 1);
+                                    const int quarter = (gi >> 2) & 3, i = gi - first_of(block, quarter), from = (quarter * 16 + m16) * 4;
+                                    const uint32_t v = __builtin_amdgcn_ds_bpermute(from, i & 2 ? sc[m][1] : sc[m][0]);
+                                    sv[m * NG + g] = i4_scale(v >> (i & 1) * 16 & 0xFFFFu, f16[GLU && m]);
+                                    zv[m * NG + g] = ZEROS ? (float) ((uint32_t) __builtin_amdgcn_ds_bpermute(from, ze[m]) >> i * 8 & 0xFFu) : 8.f;
                                 }
                             }
 #pragma unroll
-                            for (int t = 0; t < NT; t++) {
-                                const float * at = xsum + (s * NG + g) * (NT * CPT) + t * CPT + q * NA;
-                                float x[NA];
-                                if constexpr (XF32) {
-                                    x[0] = at[0];
-                                } else {
-                                    *(f32x4_t *) x = *(const f32x4_t *) at;
+                            for (int g = 0; g < NG; g++) {
+                                f32x4_t part[NM * NT];
+#pragma unroll
+                                for (int j = g * 4 / NG; j < (g + 1) * 4 / NG; j++) {
+                                    const bool first = j == g * 4 / NG;
+                                    bf16x8_t wf[NM];
+#pragma unroll
+                                    for (int m = 0; m < NM; m++) {
+                                        wf[m] = i4_operand(d[h][m][j]);
+                                    }
+#pragma unroll
+                                    for (int t = 0; t < NT; t++) {
+                                        const bf16x8_t xf = __builtin_bit_cast(bf16x8_t, *(const u32x4_t *) (xs + x_at[t] + (s * 2 + h) * I4_STEP + (GM == 0 ? j * 8 : j * 32)));
+#pragma unroll
+                                        for (int m = 0; m < NM; m++) {
+                                            part[m * NT + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf, wf[m], first ? none : part[m * NT + t], 0, 0, 0);
+                                        }
+                                    }
                                 }
 #pragma unroll
-                                for (int m = 0; m < NM; m++) {
-                                    const f32x4_t & pt = part[m * NT + t];
+                                for (int t = 0; t < NT; t++) {
+                                    const float * at = xsum + ((s * 2 + h) * NG + g) * (NT * CPT) + t * CPT + q * NA;
+                                    float x[NA];
+                                    if constexpr (XF32) {
+                                        x[0] = at[0];
+                                    } else {
+                                        *(f32x4_t *) x = *(const f32x4_t *) at;
+                                    }
 #pragma unroll
-                                    for (int e = 0; e < NA; e++) {
-                                        const float sum = XF32 ? pt[0] + (pt[1] + pt[2]) : pt[e];
-                                        acc[m * NT + t][e] = fmaf(sv[m * NG + g], fmaf(-zv[m * NG + g], x[e], sum), acc[m * NT + t][e]);
+                                    for (int m = 0; m < NM; m++) {
+                                        const f32x4_t & pt = part[m * NT + t];
+#pragma unroll
+                                        for (int e = 0; e < NA; e++) {
+                                            const float sum = XF32 ? pt[0] + (pt[1] + pt[2]) : pt[e];
+                                            acc[m * NT + t][e] = fmaf(sv[m * NG + g], fmaf(-zv[m * NG + g], x[e], sum), acc[m * NT + t][e]);
+                                        }
                                     }
                                 }
                             }
@@ -794,7 +848,7 @@ void run_few(i4_launch & p, bool glu, bool f32, bool zeros, int max_cols, int64_
     // parts of K: as many as make two wavefronts for every SIMD of the device out of the tiles of 16 rows
     const int64_t tiles = (p.nrows + 15) / 16 * matrices;
     int ksplit = 1;
-    while (ksplit < 8 && ksplit * 2 <= steps && tiles * ksplit < 8 * cus) {
+    while (ksplit < 8 && ksplit * 4 <= steps + 1 && tiles * ksplit < 8 * cus) {
         ksplit *= 2;
     }
     const auto fits = [&](int cols, int nt) { return few_lds(p.K, cols, f32, nt, glu ? 2 : 1, 1 << gm, ksplit) <= I4_FEW_LDS; };
