@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(256) k_i4_sums(const char * x, int64_t x_row, 
 
 struct i4_many {
     i4_matrix w, up;
-    int64_t K, nrows;
+    int K, nrows;
     int group_log2, n_groups;
     const char * x; int64_t x_row;          // bytes
     char * y; int64_t y_row;                // bytes
@@ -449,7 +449,8 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     static_assert(THREADS == 256 && LOADS * THREADS == COLS * 16, "a thread copies the same place of rows 16 apart");
     extern __shared__ __align__(16) char lds[]; // two pieces of activations, then the columns' rows
     int32_t * const x_at = (int32_t *) (lds + 2 * COLS * 256), * const y_at = x_at + COLS;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m16 = lane & 15, q = lane >> 4;
+    const int lane = threadIdx.x & 63, m16 = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % WM, wn = wave / WM;
 
     // the block's rows and columns
@@ -511,43 +512,55 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     }
     __syncthreads();
 
-    const int64_t row0 = (int64_t) row_tile * ROWS;
+    const int row0 = row_tile * ROWS;
     const int S = (int) ((p.K + I4_STEP - 1) / I4_STEP), E = (p.sums_row + 15) / 16;
     const int place = threadIdx.x & 15, octet = place ^ (threadIdx.x >> 4); // what this thread copies: places of rows (threadIdx.x >> 4) + 16 i
-    const auto copy = [&](int step, int buf) {
-        char * const to = lds + buf * COLS * 256 + wave * 1024;
+    // (rows of the activations start below 2^32 bytes, the launch sees to it; octets behind the last column repeat one before it: the codes
+    // are zeros there)
+    uint32_t x_off[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) {
+        x_off[i] = (uint32_t) x_at[i * 16 + (threadIdx.x >> 4)] * (uint32_t) p.x_row + octet * 16;
+    }
+    const uint32_t tail = (S - 1) * I4_STEP + octet * 8 < p.K ? 0 : octet * 16;
+    const auto copy_sums = [&](int step, int buf) {
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
             const int64_t r = x_at[i * 16 + (threadIdx.x >> 4)];
-            const char * src;
-            if (step < E) {
-                src = (const char *) (p.sums + r * p.sums_row + min(step * 16 + octet, p.sums_row - 1));
-            } else {
-                const int64_t k = (int64_t) (step - E) * I4_STEP + octet * 8;
-                src = p.x + r * p.x_row + (k < p.K ? k : 0) * 2; // (behind the last column the codes are zeros)
-            }
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) src,
-                                             (__attribute__((address_space(3))) void *) (to + i * 4096), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (p.sums + r * p.sums_row + min(step * 16 + octet, p.sums_row - 1)),
+                                             (__attribute__((address_space(3))) void *) (lds + buf * (COLS * 256) + wave * 1024 + i * 4096), 16, 0, 0);
         }
     };
-    const auto row_of = [&](int n) -> int64_t { // this lane's row of tile n
-        const int t = GLU ? n % (NT / 2) : n;
-        return min(row0 + (wn * (GLU ? NT / 2 : NT) + t) * 16 + m16, p.nrows - 1) + matrix * p.nrows;
+    const auto copy = [&](int s, int buf) {
+        const char * const from = p.x + s * (I4_STEP * 2);
+        const uint32_t less = s == S - 1 ? tail : 0;
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (from + (x_off[i] - less)),
+                                             (__attribute__((address_space(3))) void *) (lds + buf * (COLS * 256) + wave * 1024 + i * 4096), 16, 0, 0);
+        }
     };
+    // a lane's row of tile n as an offset from the wavefront's first
+    const int wave_row = (int) min(row0 + wn * (GLU ? NT / 2 : NT) * 16, p.nrows - 1);
+    const int64_t wave_at = matrix * p.nrows + wave_row;
+    int row_off[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        row_off[n] = min((GLU ? n % (NT / 2) : n) * 16 + m16, (int) p.nrows - 1 - wave_row);
+    }
     const auto of = [&](int n) -> const i4_matrix & { return GLU && n >= NT / 2 ? p.up : p.w; };
-    u32x4_t code[NT], code_next[NT];
-    uint32_t sc[NT * NG], sc_next[NT * NG];
-    const auto load = [&](int s, u32x4_t * c, uint32_t * g) {
+    u32x4_t code[NT];
+    uint32_t sc[NT * NG];
+    const auto load = [&](int s) {
+        const bool there = s * I4_STEP + q * 32 < p.K;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            const int64_t r = row_of(n), at = (int64_t) s * I4_STEP + q * 32;
-            c[n] = *(const u32x4_t *) (of(n).codes + r * (p.K / 2) + (at < p.K ? at : 0) / 2);
-            if (at >= p.K) {
-                c[n] = u32x4_t{};
-            }
+            const uint8_t * from = of(n).codes + wave_at * (p.K / 2) + s * (I4_STEP / 2);
+            code[n] = *(const u32x4_t *) (from + (uint32_t) (row_off[n] * (int) (p.K / 2) + (there ? q * 16 : 0)));
 #pragma unroll
             for (int i = 0; i < NG; i++) {
-                g[n * NG + i] = of(n).scales[r * p.n_groups + min((int) (((int64_t) s * I4_STEP + i * (I4_STEP / NG)) >> p.group_log2), p.n_groups - 1)];
+                const int g = min((s * I4_STEP + i * (I4_STEP / NG)) >> p.group_log2, p.n_groups - 1);
+                sc[n * NG + i] = (of(n).scales + wave_at * p.n_groups + g)[(uint32_t) (row_off[n] * p.n_groups)];
             }
         }
     };
@@ -561,96 +574,119 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         }
     }
     const f32x4_t none = {};
-    const auto operand = [&](int buf, int m, int o) { // activations of tile m, eight columns from 8 o on
-        const char * at = lds + buf * COLS * 256 + (wm * MT * 16 + m * 16 + m16) * 256 + ((o ^ m16) * 16);
-        return __builtin_bit_cast(bf16x8_t, *(const u32x4_t *) at);
-    };
-    copy(0, 0);
-    for (int step = 0; step < E + S; step++) {
-        const int buf = step & 1;
+    const auto arrived = [] {
         __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0): this wavefront's copies are in LDS
         __syncthreads();                    // all of them are, and nothing reads the other buffer any more
-        if (step + 1 < E + S) {
-            copy(step + 1, buf ^ 1);
-            if (step + 1 >= E) {
-                load(step + 1 - E, code_next, sc_next);
-            }
-        }
-        if (step < E) {
-            // the zero points' part: groups step * 16 ..
-            const int left = p.sums_row - step * 16;
-            for (int j = 0; j < 4 && j * 4 < left; j++) {
-                const int g = step * 16 + j * 4 + q;
-                const int64_t gi = min((int) (((int64_t) g << p.sum_group_log2) >> p.group_log2), p.n_groups - 1);
-                bf16x8_t zf[NT];
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    const int64_t at = row_of(n) * p.n_groups + gi;
-                    const float z = of(n).zeros ? (float) of(n).zeros[at] : 8.f;
-                    const float sz = -i4_scale(of(n).scales[at], of(n).f16 ? ~0u : 0u) * z;
-                    uint32_t a, b, c;
-                    f32_parts(g < p.sums_row ? sz : 0.f, a, b, c);
-                    zf[n] = __builtin_bit_cast(bf16x8_t, u32x4_t{a | a << 16, b | a << 16, b | c << 16, 0});
-                }
-#pragma unroll
-                for (int m = 0; m < MT; m++) {
-                    const bf16x8_t xf = operand(buf, m, j * 4 + q);
-#pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf, zf[n], acc[m][n], 0, 0, 0);
-                    }
-                }
-            }
+    };
+    const int tiles = (wm * MT * 16 + m16) * 256;
+    const auto operand = [&](int at, int m) { return __builtin_bit_cast(bf16x8_t, *(const u32x4_t *) (lds + at + m * 4096)); };
+
+    copy_sums(0, 0);
+    for (int step = 0; step < E; step++) { // the zero points' part: groups step * 16 ..
+        const int buf = step & 1;
+        arrived();
+        if (step + 1 < E) {
+            copy_sums(step + 1, buf ^ 1);
         } else {
-            bf16x8_t wf[NT][4];
-            float sv[NT * NG];
+            copy(0, buf ^ 1);
+            load(0);
+        }
+        const int left = p.sums_row - step * 16;
+        for (int j = 0; j < 4 && j * 4 < left; j++) {
+            const int g = step * 16 + j * 4 + q;
+            const int64_t gi = min((int) (((int64_t) g << p.sum_group_log2) >> p.group_log2), p.n_groups - 1);
+            bf16x8_t zf[NT];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                const u32x4_t d = GM == 0 ? code[n] : i4_transpose(code[n]);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    wf[n][j] = i4_operand_in_order(d[j]);
-                }
-#pragma unroll
-                for (int i = 0; i < NG; i++) {
-                    sv[n * NG + i] = i4_scale(sc[n * NG + i], of(n).f16 ? ~0u : 0u);
-                }
+                const int64_t at = (wave_at + row_off[n]) * p.n_groups + gi;
+                const float z = of(n).zeros ? (float) of(n).zeros[at] : 8.f;
+                const float sz = -i4_scale(of(n).scales[at], of(n).f16 ? ~0u : 0u) * z;
+                uint32_t a, b, c;
+                f32_parts(g < p.sums_row ? sz : 0.f, a, b, c);
+                zf[n] = __builtin_bit_cast(bf16x8_t, u32x4_t{a | a << 16, b | a << 16, b | c << 16, 0});
             }
 #pragma unroll
             for (int m = 0; m < MT; m++) {
-                bf16x8_t xf[4];
+                const bf16x8_t xf = operand(tiles + buf * (COLS * 256) + ((j * 4 + q) ^ m16) * 16, m);
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    xf[j] = operand(buf, m, GM == 0 ? q * 4 + j : j * 4 + q);
-                }
-#pragma unroll
-                for (int i = 0; i < NG; i++) {
-                    constexpr int J = 4 / NG;
-                    f32x4_t part[NT];
-#pragma unroll
-                    for (int j = 0; j < J; j++) {
-#pragma unroll
-                        for (int n = 0; n < NT; n++) {
-                            part[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[i * J + j], wf[n][i * J + j], j ? part[n] : none, 0, 0, 0);
-                        }
-                    }
-#pragma unroll
-                    for (int n = 0; n < NT; n++) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            acc[m][n][e] = fmaf(sv[n * NG + i], part[n][e], acc[m][n][e]);
-                        }
-                    }
+                for (int n = 0; n < NT; n++) {
+                    acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf, zf[n], acc[m][n], 0, 0, 0);
                 }
             }
         }
+    }
+    int buf = E & 1;
+    int at[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        at[j] = tiles + buf * (COLS * 256) + ((GM == 0 ? q * 4 + j : j * 4 + q) ^ m16) * 16;
+    }
+    for (int s = 0; s < S; s++) {
+        arrived();
+        if (s + 1 < S) {
+            copy(s + 1, buf ^ 1);
+        }
+        bf16x8_t wf[NT][4], xs[2][4];
+        float sv[NT * NG];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            xs[0][j] = operand(at[j], 0);
+        }
+        const bool there = s * I4_STEP + q * 32 < p.K;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            code[n] = code_next[n];
+            u32x4_t d = code[n];
+            d = there ? d : u32x4_t{};
+            if (GM) {
+                d = i4_transpose(d);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                wf[n][j] = i4_operand_in_order(d[j]);
+            }
 #pragma unroll
             for (int i = 0; i < NG; i++) {
-                sc[n * NG + i] = sc_next[n * NG + i];
+                sv[n * NG + i] = i4_scale(sc[n * NG + i], of(n).f16 ? ~0u : 0u);
             }
+        }
+        if (s + 1 < S) {
+            load(s + 1);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            const bf16x8_t * const xf = xs[m & 1];
+            if (m + 1 < MT) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    xs[(m + 1) & 1][j] = operand(at[j], m + 1);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NG; i++) {
+                constexpr int J = 4 / NG;
+                f32x4_t part[NT];
+#pragma unroll
+                for (int j = 0; j < J; j++) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        part[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[i * J + j], wf[n][i * J + j], j ? part[n] : none, 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        acc[m][n][e] = fmaf(sv[n * NG + i], part[n][e], acc[m][n][e]);
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0); // (else the operands of all tiles are read first, and the registers spill)
+        }
+        const int flip = buf ? -COLS * 256 : COLS * 256;
+        buf ^= 1;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            at[j] += flip;
         }
     }
 #pragma unroll
@@ -662,7 +698,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
                 char * const y = p.y + y_at[c] * p.y_row;
 #pragma unroll
                 for (int n = 0; n < (GLU ? NT / 2 : NT); n++) {
-                    const int64_t r = row0 + (wn * (GLU ? NT / 2 : NT) + n) * 16 + m16;
+                    const int r = row0 + (wn * (GLU ? NT / 2 : NT) + n) * 16 + m16;
                     if (r < p.nrows) {
                         store_y(y, p.y_bf16, r, GLU ? silu(acc[m][n][e]) * acc[m][n + (GLU ? NT / 2 : 0)][e] : acc[m][n][e]);
                     }
@@ -830,7 +866,7 @@ i4_launch launch_of(const bf16n_int4_weight & w, const bf16n_int4_weight * up, i
 void run_many(const bf16n_int4_weight & w, const bf16n_int4_weight * up, i4_many & p, int64_t x_rows, void * workspace, int cols, hipStream_t stream) {
     p.w = matrix_of(w);
     p.up = matrix_of(up ? *up : w);
-    p.K = w.K;
+    p.K = (int) w.K;
     p.group_log2 = 31 - __builtin_clz((unsigned) w.group);
     p.n_groups = (int) ((w.K + w.group - 1) / w.group);
     p.sum_group_log2 = std::min(p.group_log2, 7);
@@ -878,11 +914,11 @@ int64_t int4_workspace_bytes(const bf16n_int4_weight & w, int64_t x_rows) {
 
 void launch_int4_mmv(const bf16n_int4_weight & w, const bf16n_int4_weight * up, const bf16n_mmv_args & a, bool ids_i64, void * workspace,
                      uint64_t workspace_bytes, int cus, hipStream_t stream) {
-    if (!a.ids && a.x_bf16 && a.ncols > 32 && (int64_t) workspace_bytes >= int4_workspace_bytes(w, a.ncols)) {
+    if (!a.ids && a.x_bf16 && a.ncols > 32 && a.x_tok >= 0 && a.ncols * a.x_tok < (int64_t) 1 << 32 && (int64_t) workspace_bytes >= int4_workspace_bytes(w, a.ncols)) {
         i4_many p = {};
         p.x = (const char *) a.x; p.x_row = a.x_tok;
         p.y = (char *) a.y; p.y_row = a.y_tok; p.y_bf16 = a.y_bf16 != 0;
-        p.nrows = a.nrows;
+        p.nrows = (int) a.nrows;
         p.ncols = a.ncols;
         p.n_used = 1; p.n_matrices = 1;
         const int64_t tiles = ((a.nrows + 127) / 128) * ((a.ncols + 127) / 128);
@@ -916,11 +952,11 @@ void launch_int4_mm_ids(const bf16n_int4_weight & w, const bf16n_int4_weight * u
                         int cus, hipStream_t stream) {
     const int64_t x_rows = per_slot ? (int64_t) n_tok * n_used : n_tok;
     const int64_t n_pairs = (int64_t) n_tok * n_used;
-    if (n_pairs > 16 * (int64_t) n_matrices && (int64_t) workspace_bytes >= int4_workspace_bytes(w, x_rows)) {
+    if (n_pairs > 16 * (int64_t) n_matrices && x_row >= 0 && x_rows * x_row < (int64_t) 1 << 31 && (int64_t) workspace_bytes >= int4_workspace_bytes(w, x_rows)) {
         i4_many p = {};
         p.x = (const char *) x; p.x_row = x_row * 2;
         p.y = (char *) y; p.y_row = y_row * (y_bf16 ? 2 : 4); p.y_bf16 = y_bf16;
-        p.nrows = w.rows / n_matrices;
+        p.nrows = (int) (w.rows / n_matrices);
         p.ncols = (int) n_pairs;
         p.pairs = pairs; p.bounds = bounds;
         p.n_matrices = n_matrices; p.n_used = n_used; p.per_slot = per_slot;
