@@ -495,13 +495,16 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         c0 = p.bounds[m] + k * COLS;
         nc = min(COLS, p.bounds[m + 1] - c0);
     } else {
-        // an XCD takes every eighth block: neighbours there are column tiles of the same rows
+        // An XCD takes every eighth block, which is made a contiguous part of the tiles here: four column tiles of one row tile
+        // after the other, so that what runs there at a time shares few pieces of activations (four times a row tile's bytes).
+        // 8192 x 2048, 8192 tokens: @@ us, 428 with all column tiles of a row tile side by side.
         const int n = p.row_tiles * p.col_tiles, per = (n + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
         if (id >= n) {
             return;
         }
-        row_tile = id / p.col_tiles;
-        c0 = id % p.col_tiles * COLS;
+        const int group = id / (p.row_tiles * 4), in = id - group * p.row_tiles * 4, wide = min(4, p.col_tiles - group * 4);
+        row_tile = in / wide;
+        c0 = (group * 4 + in % wide) * COLS;
         nc = min(COLS, p.ncols - c0);
     }
     for (int i = threadIdx.x; i < COLS; i += THREADS) {
@@ -522,7 +525,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     for (int i = 0; i < LOADS; i++) {
         x_off[i] = (uint32_t) x_at[i * 16 + (threadIdx.x >> 4)] * (uint32_t) p.x_row + octet * 16;
     }
-    const uint32_t tail = (S - 1) * I4_STEP + octet * 8 < p.K ? 0 : octet * 16;
+    const bool cut = p.K % I4_STEP != 0; // the last step is cut short
     const auto copy_sums = [&](int step, int buf) {
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
@@ -533,10 +536,15 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     };
     const auto copy = [&](int s, int buf) {
         const char * const from = p.x + s * (I4_STEP * 2);
-        const uint32_t less = s == S - 1 ? tail : 0;
+        if (cut && s == S - 1 && s * I4_STEP + octet * 8 >= p.K) {
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                x_off[i] -= octet * 16;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (from + (x_off[i] - less)),
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (from + x_off[i]),
                                              (__attribute__((address_space(3))) void *) (lds + buf * (COLS * 256) + wave * 1024 + i * 4096), 16, 0, 0);
         }
     };
@@ -550,13 +558,21 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     }
     const auto of = [&](int n) -> const i4_matrix & { return GLU && n >= NT / 2 ? p.up : p.w; };
     u32x4_t code[NT];
-    uint32_t sc[NT * NG];
+    uint32_t sc[NT * NG], code_off[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        code_off[n] = row_off[n] * (p.K / 2) + q * 16;
+    }
     const auto load = [&](int s) {
-        const bool there = s * I4_STEP + q * 32 < p.K;
+        if (cut && s == S - 1 && s * I4_STEP + q * 32 >= p.K) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                code_off[n] -= q * 16;
+            }
+        }
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            const uint8_t * from = of(n).codes + wave_at * (p.K / 2) + s * (I4_STEP / 2);
-            code[n] = *(const u32x4_t *) (from + (uint32_t) (row_off[n] * (int) (p.K / 2) + (there ? q * 16 : 0)));
+            code[n] = *(const u32x4_t *) (of(n).codes + wave_at * (p.K / 2) + s * (I4_STEP / 2) + code_off[n]);
 #pragma unroll
             for (int i = 0; i < NG; i++) {
                 const int g = min((s * I4_STEP + i * (I4_STEP / NG)) >> p.group_log2, p.n_groups - 1);
@@ -632,14 +648,15 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         for (int j = 0; j < 4; j++) {
             xs[0][j] = operand(at[j], 0);
         }
-        const bool there = s * I4_STEP + q * 32 < p.K;
+        if (cut && s == S - 1 && s * I4_STEP + q * 32 >= p.K) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                code[n] = u32x4_t{};
+            }
+        }
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            u32x4_t d = code[n];
-            d = there ? d : u32x4_t{};
-            if (GM) {
-                d = i4_transpose(d);
-            }
+            const u32x4_t d = GM ? i4_transpose(code[n]) : code[n];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 wf[n][j] = i4_operand_in_order(d[j]);
@@ -652,32 +669,45 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         if (s + 1 < S) {
             load(s + 1);
         }
+        // a tile's products over a group are added up while the matrix cores work on the next ones
+        f32x4_t part[2][NT];
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-            const bf16x8_t * const xf = xs[m & 1];
-            if (m + 1 < MT) {
+        for (int u = 0; u <= MT * NG; u++) {
+            const int m = u / NG, i = u % NG;
+            constexpr int J = 4 / NG;
+            if (i == 0 && m + 1 < MT) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     xs[(m + 1) & 1][j] = operand(at[j], m + 1);
                 }
             }
-#pragma unroll
-            for (int i = 0; i < NG; i++) {
-                constexpr int J = 4 / NG;
-                f32x4_t part[NT];
+            if (u < MT * NG) {
 #pragma unroll
                 for (int j = 0; j < J; j++) {
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
-                        part[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[i * J + j], wf[n][i * J + j], j ? part[n] : none, 0, 0, 0);
+                        part[u & 1][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xs[m & 1][i * J + j], wf[n][i * J + j], j ? part[u & 1][n] : none, 0, 0, 0);
                     }
                 }
+            }
+            if (u > 0) {
+                const int pm = (u - 1) / NG, pi = (u - 1) % NG;
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        acc[m][n][e] = fmaf(sv[n * NG + i], part[n][e], acc[m][n][e]);
+                        acc[pm][n][e] = fmaf(sv[n * NG + pi], part[(u - 1) & 1][n][e], acc[pm][n][e]);
                     }
+                }
+            }
+            if (u > 0 && u < MT * NG) {
+                if (i == 0 && m + 1 < MT) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0); // reads of LDS
+                }
+#pragma unroll
+                for (int k = 0; k < J * NT; k++) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);      // a product
+                    __builtin_amdgcn_sched_group_barrier(0x002, 4 / J, 0);  // additions
                 }
             }
             __builtin_amdgcn_sched_barrier(0); // (else the operands of all tiles are read first, and the registers spill)
