@@ -137,7 +137,8 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
         };
         // Scales and zero points come by blocks of 16 groups, four of its row to a lane of each quarter, a block ahead; a step takes
         // them from the quarter that has its group.  (A load of one scale by every lane for every 128 columns: 72 us where this takes @@.)
-        uint32_t sc[NM][2], ze[NM], sc_next[NM][2], ze_next[NM];
+        uint64_t sc[NM], sc_next[NM];
+        uint32_t ze[NM], ze_next[NM];
         const auto block_of = [&](int s) { return (s * 2 * I4_STEP >> p.group_log2) >> 4; };
         const auto first_of = [&](int block, int quarter) { return max(min(block * 16 + quarter * 4, p.n_groups - 4), 0); };
         const auto load_block = [&](int r0, int block) {
@@ -148,14 +149,13 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
                 const int64_t base = (matrix * p.nrows + r) * p.n_groups;
                 const int at = min(m16, p.nrows - 1 - r) * p.n_groups + first_of(block, q);
                 if (p.n_groups >= 4) {
-                    __builtin_memcpy(sc_next[m], w.scales + base + at, 8); // (aligned to two bytes)
+                    sc_next[m] = *(const u64_at_2 *) (w.scales + base + at);
                     if (ZEROS) {
-                        __builtin_memcpy(&ze_next[m], w.zeros + base + at, 4);
+                        ze_next[m] = *(const u32_at_1 *) (w.zeros + base + at);
                     }
                 } else {
                     const int i1 = min(1, p.n_groups - 1), i2 = min(2, p.n_groups - 1);
-                    sc_next[m][0] = w.scales[base + at] | (uint32_t) w.scales[base + at + i1] << 16;
-                    sc_next[m][1] = w.scales[base + at + i2];
+                    sc_next[m] = w.scales[base + at] | (uint32_t) w.scales[base + at + i1] << 16 | (uint64_t) w.scales[base + at + i2] << 32;
                     if (ZEROS) {
                         ze_next[m] = w.zeros[base + at] | w.zeros[base + at + i1] << 8 | w.zeros[base + at + i2] << 16;
                     }
@@ -250,8 +250,7 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
                         if (s == s0 || block != block_of(s - 1)) {
 #pragma unroll
                             for (int m = 0; m < NM; m++) {
-                                sc[m][0] = sc_next[m][0];
-                                sc[m][1] = sc_next[m][1];
+                                sc[m] = sc_next[m];
                                 ze[m] = ze_next[m];
                             }
                             const bool more = block < block_of(s1 - 1);
@@ -287,7 +286,7 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
                                 for (int g = 0; g < NG; g++) {
                                     const int gi = min((s * 2 + h) * I4_STEP + g * (I4_STEP / NG) >> p.group_log2, p.n_groups - 1);
                                     const int quarter = (gi >> 2) & 3, i = gi - first_of(block, quarter), from = (quarter * 16 + m16) * 4;
-                                    const uint32_t v = __builtin_amdgcn_ds_bpermute(from, i & 2 ? sc[m][1] : sc[m][0]);
+                                    const uint32_t v = __builtin_amdgcn_ds_bpermute(from, (uint32_t) (i & 2 ? sc[m] >> 32 : sc[m]));
                                     sv[m * NG + g] = i4_scale(v >> (i & 1) * 16 & 0xFFFFu, f16[GLU && m]);
                                     zv[m * NG + g] = ZEROS ? (float) ((uint32_t) __builtin_amdgcn_ds_bpermute(from, ze[m]) >> i * 8 & 0xFFu) : 8.f;
                                 }
@@ -447,8 +446,9 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     constexpr int THREADS = WM * WN * 64, COLS = WM * MT * 16, ROWS = WN * NT * 16 / (GLU ? 2 : 1);
     constexpr int NG = GM == 0 ? 1 : GM == 1 ? 2 : 4, LOADS = COLS * 16 / THREADS;
     static_assert(THREADS == 256 && LOADS * THREADS == COLS * 16, "a thread copies the same place of rows 16 apart");
-    extern __shared__ __align__(16) char lds[]; // two pieces of activations, then the columns' rows
-    int32_t * const x_at = (int32_t *) (lds + 2 * COLS * 256), * const y_at = x_at + COLS;
+    static_assert(WN * NT == 8, "a wavefront copies the codes of two tiles of rows");
+    extern __shared__ __align__(16) char lds[]; // two pieces of activations, two of codes
+    constexpr int CODES = 2 * COLS * 256;
     const int lane = threadIdx.x & 63, m16 = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % WM, wn = wave / WM;
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         // blocks are (matrix, piece of its columns) by row tile: the pieces are counted from the lists' bounds
         row_tile = blockIdx.x % p.row_tiles;
         int piece = blockIdx.x / p.row_tiles;
-        int * const found = x_at;
+        int * const found = (int *) lds;
         if (threadIdx.x == 0) {
             found[0] = -1;
         }
@@ -507,13 +507,14 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         c0 = (group * 4 + in % wide) * COLS;
         nc = min(COLS, p.ncols - c0);
     }
-    for (int i = threadIdx.x; i < COLS; i += THREADS) {
+    const auto pair_of = [&](int i) { // the list's pair, or the dense column, behind column i; columns that are not there repeat the last
         const int c = c0 + min(i, nc - 1);
-        const int pair = p.pairs ? p.pairs[c] : c;
-        x_at[i] = p.pairs && !p.per_slot ? pair / p.n_used : pair;
-        y_at[i] = pair;
-    }
-    __syncthreads();
+        return p.pairs ? p.pairs[c] : c;
+    };
+    const auto x_row_of = [&](int i) {
+        const int pair = pair_of(i);
+        return p.pairs && !p.per_slot ? pair / p.n_used : pair;
+    };
 
     const int row0 = row_tile * ROWS;
     const int S = (int) ((p.K + I4_STEP - 1) / I4_STEP), E = (p.sums_row + 15) / 16;
@@ -523,13 +524,13 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     uint32_t x_off[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; i++) {
-        x_off[i] = (uint32_t) x_at[i * 16 + (threadIdx.x >> 4)] * (uint32_t) p.x_row + octet * 16;
+        x_off[i] = (uint32_t) x_row_of(i * 16 + (threadIdx.x >> 4)) * (uint32_t) p.x_row + octet * 16;
     }
     const bool cut = p.K % I4_STEP != 0; // the last step is cut short
     const auto copy_sums = [&](int step, int buf) {
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
-            const int64_t r = x_at[i * 16 + (threadIdx.x >> 4)];
+            const int64_t r = x_row_of(i * 16 + (threadIdx.x >> 4));
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (p.sums + r * p.sums_row + min(step * 16 + octet, p.sums_row - 1)),
                                              (__attribute__((address_space(3))) void *) (lds + buf * (COLS * 256) + wave * 1024 + i * 4096), 16, 0, 0);
         }
@@ -557,26 +558,39 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         row_off[n] = min((GLU ? n % (NT / 2) : n) * 16 + m16, (int) p.nrows - 1 - wave_row);
     }
     const auto of = [&](int n) -> const i4_matrix & { return GLU && n >= NT / 2 ? p.up : p.w; };
-    u32x4_t code[NT];
-    uint32_t sc[NT * NG], code_off[NT];
+    // the codes of a step: a wavefront copies tiles of rows wave and wave + 4, four lanes to a row; places exchanged by the row's bits
+    uint32_t code_off[2];
+    const uint8_t * code_at[2];
+    const int chunk = (lane & 3) ^ (lane >> 4);
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        code_off[n] = row_off[n] * (p.K / 2) + q * 16;
+    for (int i = 0; i < 2; i++) {
+        const int t = i * 4 + wave, n = t % NT, r = row0 + (t / NT * (GLU ? NT / 2 : NT) + (GLU ? n % (NT / 2) : n)) * 16, first = min(r, p.nrows - 1);
+        code_at[i] = of(n).codes + (matrix * p.nrows + first) * (p.K / 2);
+        code_off[i] = min(lane >> 2, p.nrows - 1 - first) * (p.K / 2) + chunk * 16;
     }
-    const auto load = [&](int s) {
-        if (cut && s == S - 1 && s * I4_STEP + q * 32 >= p.K) {
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                code_off[n] -= q * 16;
-            }
+    const auto copy_codes = [&](int s, int buf) {
+        if (cut && s == S - 1 && s * I4_STEP + chunk * 32 >= p.K) {
+            code_off[0] -= chunk * 16;
+            code_off[1] -= chunk * 16;
         }
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            code[n] = *(const u32x4_t *) (of(n).codes + wave_at * (p.K / 2) + s * (I4_STEP / 2) + code_off[n]);
+        for (int i = 0; i < 2; i++) {
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (code_at[i] + s * (I4_STEP / 2) + code_off[i]),
+                                             (__attribute__((address_space(3))) void *) (lds + CODES + buf * 8192 + i * 4096 + wave * 1024), 16, 0, 0);
+        }
+    };
+    // scales by blocks of 16 groups, four of its row to a lane of each quarter, a block ahead
+    uint64_t sc[NT], sc_next[NT];
+    const auto block_of = [&](int s) { return (s * I4_STEP >> p.group_log2) >> 4; };
+    const auto first_of = [&](int block, int quarter) { return max(min(block * 16 + quarter * 4, p.n_groups - 4), 0); };
+    const auto load_block = [&](int block) {
 #pragma unroll
-            for (int i = 0; i < NG; i++) {
-                const int g = min((s * I4_STEP + i * (I4_STEP / NG)) >> p.group_log2, p.n_groups - 1);
-                sc[n * NG + i] = (of(n).scales + wave_at * p.n_groups + g)[(uint32_t) (row_off[n] * p.n_groups)];
+        for (int n = 0; n < NT; n++) {
+            const uint16_t * from = of(n).scales + wave_at * p.n_groups + (uint32_t) (row_off[n] * p.n_groups + first_of(block, q));
+            if (p.n_groups >= 4) {
+                sc_next[n] = *(const u64_at_2 *) from;
+            } else {
+                sc_next[n] = from[0] | (uint32_t) from[min(1, p.n_groups - 1)] << 16 | (uint64_t) from[min(2, p.n_groups - 1)] << 32;
             }
         }
     };
@@ -605,7 +619,8 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
             copy_sums(step + 1, buf ^ 1);
         } else {
             copy(0, buf ^ 1);
-            load(0);
+            copy_codes(0, buf ^ 1);
+            load_block(0);
         }
         const int left = p.sums_row - step * 16;
         for (int j = 0; j < 4 && j * 4 < left; j++) {
@@ -641,6 +656,22 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         arrived();
         if (s + 1 < S) {
             copy(s + 1, buf ^ 1);
+            copy_codes(s + 1, buf ^ 1);
+        }
+        const int block = block_of(s);
+        if (s == 0 || block != block_of(s - 1)) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                sc[n] = sc_next[n];
+            }
+            if (block < block_of(S - 1)) {
+                load_block(block + 1);
+            }
+        }
+        u32x4_t code[NT];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            code[n] = *(const u32x4_t *) (lds + CODES + buf * 8192 + (wn * NT + n) * 1024 + m16 * 64 + (q ^ (m16 >> 2)) * 16);
         }
         bf16x8_t wf[NT][4], xs[2][4];
         float sv[NT * NG];
@@ -663,11 +694,11 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
             }
 #pragma unroll
             for (int i = 0; i < NG; i++) {
-                sv[n * NG + i] = i4_scale(sc[n * NG + i], of(n).f16 ? ~0u : 0u);
+                const int g = min((s * I4_STEP + i * (I4_STEP / NG)) >> p.group_log2, p.n_groups - 1);
+                const int quarter = (g >> 2) & 3, e = g - first_of(block, quarter);
+                const uint32_t v = __builtin_amdgcn_ds_bpermute((quarter * 16 + m16) * 4, (uint32_t) (e & 2 ? sc[n] >> 32 : sc[n]));
+                sv[n * NG + i] = i4_scale(v >> (e & 1) * 16 & 0xFFFFu, of(n).f16 ? ~0u : 0u);
             }
-        }
-        if (s + 1 < S) {
-            load(s + 1);
         }
         // a tile's products over a group are added up while the matrix cores work on the next ones
         f32x4_t part[2][NT];
@@ -725,7 +756,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         for (int e = 0; e < 4; e++) {
             const int c = wm * MT * 16 + m * 16 + q * 4 + e;
             if (c < nc) {
-                char * const y = p.y + y_at[c] * p.y_row;
+                char * const y = p.y + pair_of(c) * p.y_row;
 #pragma unroll
                 for (int n = 0; n < (GLU ? NT / 2 : NT); n++) {
                     const int r = row0 + (wn * (GLU ? NT / 2 : NT) + n) * 16 + m16;
@@ -856,7 +887,7 @@ void init_few() {
     }
 }
 
-constexpr size_t many_lds(int cols) { return (size_t) 2 * cols * 256 + 2 * cols * 4; }
+constexpr size_t many_lds(int cols) { return (size_t) 2 * cols * 256 + 2 * 8192; }
 
 template <int GM> void init_many() {
     const auto raise = [](const void * f, int cols) { (void) hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int) many_lds(cols)); };
