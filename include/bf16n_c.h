@@ -202,8 +202,8 @@ typedef struct bf16n_int4_weight {
 int bf16n_int4_mmv(const bf16n_int4_weight * w, const bf16n_int4_weight * up, const bf16n_mmv_args * a, int ids_i64, void * workspace,
                    uint64_t workspace_bytes, void * stream);
 /* workspace of the products of many columns (more than 32 BF16 columns, or many pairs per matrix): 16-byte aligned device memory,
- * *bytes for x_rows rows of activations; a call that finds none or less (null and 0 are fine) takes the kernels for few columns. */
-int bf16n_int4_workspace_bytes(const bf16n_int4_weight * w, int64_t x_rows, uint64_t * bytes);
+ * *bytes for x_rows rows of activations and, in bf16n_int4_mm_ids, n_pairs = n_tok * n_used over n_experts (0 otherwise); a call that finds none or less (null and 0 are fine) takes the kernels for few columns. */
+int bf16n_int4_workspace_bytes(const bf16n_int4_weight * w, int64_t x_rows, int64_t n_pairs, int n_experts, uint64_t * bytes);
 /* The (token, slot) pairs t * n_used + slot sorted by the matrix that their id names, ascending within one; pairs whose id names
  * none (outside [0, n_matrices)) come last.  Every pair is listed, also where a token names a matrix twice.  pairs:
  * n_tok * n_used entries; bounds: n_matrices + 2 (matrix m has pairs[bounds[m]] .. pairs[bounds[m + 1] - 1], the last range is

@@ -69,7 +69,7 @@ SYMBOLS = {
     "bf16n_router_topk_strided": (_i, [_vp, _i64, _i, _i, _i, _i, _vp, _vp, _i64, _vp]),
     "bf16n_router_topk_route_fits": (_i, [_i, _i, _i]),
     "bf16n_router_topk_route": (_i, [_vp, _i64, _i, _i, _i, _i, _vp, _vp, _i64, _i, _i, _vp, _vp, _vp, _i, _i, _vp]),
-    "bf16n_int4_workspace_bytes": (_i, [_QP, _i64, C.POINTER(C.c_uint64)]),
+    "bf16n_int4_workspace_bytes": (_i, [_QP, _i64, _i64, _i, C.POINTER(C.c_uint64)]),
     "bf16n_int4_mmv": (_i, [_QP, _QP, _AP, _i, _vp, C.c_uint64, _vp]),
     "bf16n_int4_route": (_i, [_vp, _i, _i64, _i64, _i, _i, _i, _vp, _vp, _vp]),
     "bf16n_int4_mm_ids": (_i, [_QP, _QP, _vp, _i64, _i, _vp, _vp, _vp, _i, _i64, _i, _i, _i, _vp, C.c_uint64, _vp]),

@@ -716,11 +716,11 @@ void check_int4(const bf16n_int4_weight * w, const bf16n_int4_weight * up) {
 
 } // namespace
 
-int bf16n_int4_workspace_bytes(const bf16n_int4_weight * w, int64_t x_rows, uint64_t * bytes) {
+int bf16n_int4_workspace_bytes(const bf16n_int4_weight * w, int64_t x_rows, int64_t n_pairs, int n_experts, uint64_t * bytes) {
     return guarded([&] {
         check_int4(w, nullptr);
-        require(bytes && x_rows >= 0, "int4_workspace_bytes: null pointer or negative rows");
-        *bytes = (uint64_t) dev::int4_workspace_bytes(*w, x_rows);
+        require(bytes && x_rows >= 0 && n_pairs >= 0 && n_experts >= 0, "int4_workspace_bytes: null pointer or negative sizes");
+        *bytes = (uint64_t) dev::int4_workspace_bytes(*w, x_rows, n_pairs, n_experts);
     });
 }
 

@@ -388,8 +388,42 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
 // up to them, so that it runs on the matrix cores as well: eight columns for a group, X1 X2 X1 X3 X2 X1 0 0 against
 // Z1 Z1 Z2 Z1 Z2 Z3 0 0 (what is left out is below 2^-23 of the product), instead of four FMAs per result tile and group.
 
-// X of every activation row, in parts: one thread to 32 columns
-__global__ void __launch_bounds__(256) k_i4_sums(const char * x, int64_t x_row, int64_t K, int group, int64_t n_rows, u32x4_t * sums, int64_t sums_row) {
+// X of every activation row, in parts: one thread to 32 columns.  For lists of columns by matrix the last block counts the pieces of
+// `cols` columns of every matrix (and of the pairs that name none) instead and lists them: (matrix, piece), how many in table[0].
+__global__ void __launch_bounds__(256) k_i4_sums(const char * x, int64_t x_row, int K, int group, int64_t n_rows, u32x4_t * sums, int64_t sums_row,
+                                                 const int32_t * bounds, int n_matrices, int cols, int2 * table) {
+    if (bounds && blockIdx.x == gridDim.x - 1) {
+        __shared__ int of_wave[4];
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        int before = 0;
+        for (int b = 0; b <= n_matrices; b += 256) {
+            const int m = b + threadIdx.x;
+            const int n = m <= n_matrices ? (bounds[m + 1] - bounds[m] + cols - 1) / cols : 0;
+            int upto = n;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int v = __shfl_up(upto, o, 64);
+                upto += lane >= o ? v : 0;
+            }
+            if (lane == 63) {
+                of_wave[wave] = upto;
+            }
+            __syncthreads();
+            int at = before + upto - n;
+            for (int w = 0; w < 4; w++) {
+                at += w < wave ? of_wave[w] : 0;
+                before += of_wave[w];
+            }
+            for (int k = 0; k < n; k++) {
+                table[1 + at + k] = int2{m, k};
+            }
+            __syncthreads();
+        }
+        if (threadIdx.x == 0) {
+            table[0] = int2{before, 0};
+        }
+        return;
+    }
     const int per = group / 32;                               // threads to a group: 1, 2 or 4
     const int64_t segs = (K / 32 + per - 1) / per * per;
     const int64_t i = (int64_t) blockIdx.x * blockDim.x + threadIdx.x;
@@ -430,18 +464,17 @@ struct i4_many {
     int sum_group_log2;
     int ncols;
     const int32_t * pairs, * bounds;        // lists of columns by matrix, or null
+    const int2 * table;                     // and their pieces
     int n_matrices, n_used, per_slot;
     int row_tiles, col_tiles;               // dense: the grid
 };
-
-constexpr int MANY_MAX_MATRICES = 1024;
 
 // A block takes WM * MT * 16 columns and WN * NT * 16 rows (half of them of either matrix where they are gated) and 128 columns of K
 // at a time: the activations' piece goes straight into LDS (two buffers, 16-byte places exchanged by the row's low bits so that
 // the operands' reads find every bank), the codes into registers, both a step ahead; a wavefront turns its own codes into operands,
 // which serve MT tiles.  Every product over a group starts from zero and is added to the result times its scale.
 // Bound by the vector instructions beside the matrix cores' (nine for eight codes and tile of rows, four for a tile of results and group).
-template <int WM, int WN, int MT, int NT, int GM, bool GLU>
+template <int WM, int WN, int MT, int NT, int GM, bool GLU, bool LIST>
 __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     constexpr int THREADS = WM * WN * 64, COLS = WM * MT * 16, ROWS = WN * NT * 16 / (GLU ? 2 : 1);
     constexpr int NG = GM == 0 ? 1 : GM == 1 ? 2 : 4, LOADS = COLS * 16 / THREADS;
@@ -456,44 +489,28 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     // the block's rows and columns
     int64_t matrix = 0;
     int c0, nc, row_tile;
-    if (p.bounds) {
-        // blocks are (matrix, piece of its columns) by row tile: the pieces are counted from the lists' bounds
-        row_tile = blockIdx.x % p.row_tiles;
-        int piece = blockIdx.x / p.row_tiles;
-        int * const found = (int *) lds;
-        if (threadIdx.x == 0) {
-            found[0] = -1;
-        }
-        __syncthreads();
-        if (wave == 0) {
-            int before = 0;
-            for (int b = 0; b < p.n_matrices; b += 64) {
-                const int m = b + lane;
-                const int n = m < p.n_matrices ? p.bounds[m + 1] - p.bounds[m] : 0;
-                const int pieces = (n + COLS - 1) / COLS;
-                int upto = pieces;
-#pragma unroll
-                for (int o = 1; o < 64; o <<= 1) {
-                    const int v = __shfl_up(upto, o, 64);
-                    upto += lane >= o ? v : 0;
-                }
-                const int first = before + upto - pieces;
-                if (piece >= first && piece < first + pieces) {
-                    found[0] = m;
-                    found[1] = piece - first;
-                }
-                before += __shfl(upto, 63, 64);
-            }
-        }
-        __syncthreads();
-        const int m = found[0], k = found[1];
-        __syncthreads();
-        if (m < 0) {
+    if constexpr (LIST) {
+        // An XCD takes every eighth block, which is made a contiguous part of (piece, row tile) here: the row tiles of a piece read
+        // its activations from one L2.
+        const int n = p.table[0].x * p.row_tiles, per = (n + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+        if ((int) (blockIdx.x >> 3) >= per || id >= n) {
             return;
         }
+        const int2 piece = p.table[1 + id / p.row_tiles];
+        const int m = piece.x;
         matrix = m;
-        c0 = p.bounds[m] + k * COLS;
+        row_tile = id % p.row_tiles;
+        c0 = p.bounds[m] + piece.y * COLS;
         nc = min(COLS, p.bounds[m + 1] - c0);
+        if (m == p.n_matrices) { // zeros for the pairs that name none
+            const int from = row_tile * ROWS, rows = min(ROWS, p.nrows - from);
+            for (int i = threadIdx.x; i < nc * ROWS; i += THREADS) {
+                if (i % ROWS < rows) {
+                    store_y(p.y + p.pairs[c0 + i / ROWS] * p.y_row, p.y_bf16, from + i % ROWS, 0.f);
+                }
+            }
+            return;
+        }
     } else {
         // An XCD takes every eighth block, which is made a contiguous part of the tiles here: four column tiles of one row tile
         // after the other, so that what runs there at a time shares few pieces of activations (four times a row tile's bytes).
@@ -530,6 +547,9 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     const auto copy_sums = [&](int step, int buf) {
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
+            if (i * 16 >= nc) {
+                break;
+            }
             const int64_t r = x_row_of(i * 16 + (threadIdx.x >> 4));
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (p.sums + r * p.sums_row + min(step * 16 + octet, p.sums_row - 1)),
                                              (__attribute__((address_space(3))) void *) (lds + buf * (COLS * 256) + wave * 1024 + i * 4096), 16, 0, 0);
@@ -545,8 +565,10 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         }
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (from + x_off[i]),
-                                             (__attribute__((address_space(3))) void *) (lds + buf * (COLS * 256) + wave * 1024 + i * 4096), 16, 0, 0);
+            if (i * 16 < nc) { // (places of rows 16 i ..)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (from + x_off[i]),
+                                                 (__attribute__((address_space(3))) void *) (lds + buf * (COLS * 256) + wave * 1024 + i * 4096), 16, 0, 0);
+            }
         }
     };
     // a lane's row of tile n as an offset from the wavefront's first
@@ -608,10 +630,26 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0): this wavefront's copies are in LDS
         __syncthreads();                    // all of them are, and nothing reads the other buffer any more
     };
-    const int tiles = (wm * MT * 16 + m16) * 256;
-    const auto operand = [&](int at, int m) { return __builtin_bit_cast(bf16x8_t, *(const u32x4_t *) (lds + at + m * 4096)); };
+    // column tiles m * WM + wm are this wavefront's: those that the columns reach are spread over all
+    const int mt = ((nc + 15) / 16 - wm + WM - 1) / WM;
+    const int tiles = (wm * 16 + m16) * 256;
+    const auto operand = [&](int at, int m) { return __builtin_bit_cast(bf16x8_t, *(const u32x4_t *) (lds + at + m * (WM * 4096))); };
 
     copy_sums(0, 0);
+    uint32_t zs[4][NT], zz[4][NT]; // scales and zero points of the groups of a step, ahead of the wait
+    const auto load_zeros = [&](int step) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int64_t gi = min((int) (((int64_t) (step * 16 + j * 4 + q) << p.sum_group_log2) >> p.group_log2), p.n_groups - 1);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const int64_t at = (wave_at + row_off[n]) * p.n_groups + gi;
+                zs[j][n] = of(n).scales[at];
+                zz[j][n] = of(n).zeros ? of(n).zeros[at] : 8u;
+            }
+        }
+    };
+    load_zeros(0);
     for (int step = 0; step < E; step++) { // the zero points' part: groups step * 16 ..
         const int buf = step & 1;
         arrived();
@@ -623,27 +661,33 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
             load_block(0);
         }
         const int left = p.sums_row - step * 16;
-        for (int j = 0; j < 4 && j * 4 < left; j++) {
-            const int g = step * 16 + j * 4 + q;
-            const int64_t gi = min((int) (((int64_t) g << p.sum_group_log2) >> p.group_log2), p.n_groups - 1);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (j * 4 >= left) {
+                break;
+            }
             bf16x8_t zf[NT];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                const int64_t at = (wave_at + row_off[n]) * p.n_groups + gi;
-                const float z = of(n).zeros ? (float) of(n).zeros[at] : 8.f;
-                const float sz = -i4_scale(of(n).scales[at], of(n).f16 ? ~0u : 0u) * z;
+                const float sz = -i4_scale(zs[j][n], of(n).f16 ? ~0u : 0u) * (float) zz[j][n];
                 uint32_t a, b, c;
-                f32_parts(g < p.sums_row ? sz : 0.f, a, b, c);
+                f32_parts(j * 4 + q < left ? sz : 0.f, a, b, c);
                 zf[n] = __builtin_bit_cast(bf16x8_t, u32x4_t{a | a << 16, b | a << 16, b | c << 16, 0});
             }
 #pragma unroll
             for (int m = 0; m < MT; m++) {
+                if (LIST && m >= mt) {
+                    break;
+                }
                 const bf16x8_t xf = operand(tiles + buf * (COLS * 256) + ((j * 4 + q) ^ m16) * 16, m);
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf, zf[n], acc[m][n], 0, 0, 0);
                 }
             }
+        }
+        if (step + 1 < E) {
+            load_zeros(step + 1);
         }
     }
     int buf = E & 1;
@@ -706,13 +750,14 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         for (int u = 0; u <= MT * NG; u++) {
             const int m = u / NG, i = u % NG;
             constexpr int J = 4 / NG;
-            if (i == 0 && m + 1 < MT) {
+            const bool live = u < MT * NG && (!LIST || m < mt);
+            if (live) {
+                if (i == 0 && m + 1 < MT) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    xs[(m + 1) & 1][j] = operand(at[j], m + 1);
+                    for (int j = 0; j < 4; j++) {
+                        xs[(m + 1) & 1][j] = operand(at[j], m + 1);
+                    }
                 }
-            }
-            if (u < MT * NG) {
 #pragma unroll
                 for (int j = 0; j < J; j++) {
 #pragma unroll
@@ -731,7 +776,10 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
                     }
                 }
             }
-            if (u > 0 && u < MT * NG) {
+            if (!live) {
+                break;
+            }
+            if (!LIST && u > 0) {
                 if (i == 0 && m + 1 < MT) {
                     __builtin_amdgcn_sched_group_barrier(0x100, 4, 0); // reads of LDS
                 }
@@ -754,7 +802,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     for (int m = 0; m < MT; m++) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const int c = wm * MT * 16 + m * 16 + q * 4 + e;
+            const int c = (m * WM + wm) * 16 + q * 4 + e;
             if (c < nc) {
                 char * const y = p.y + pair_of(c) * p.y_row;
 #pragma unroll
@@ -765,16 +813,6 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
                     }
                 }
             }
-        }
-    }
-}
-
-// zeros for the pairs that name no matrix
-__global__ void __launch_bounds__(256) k_i4_unnamed(const int32_t * pairs, const int32_t * range, char * y, int64_t y_row, int64_t row_bytes) {
-    for (int c = range[0] + blockIdx.x; c < range[1]; c += gridDim.x) {
-        uint16_t * const to = (uint16_t *) (y + pairs[c] * y_row);
-        for (int64_t i = threadIdx.x; i < row_bytes / 2; i += blockDim.x) {
-            to[i] = 0;
         }
     }
 }
@@ -891,23 +929,33 @@ constexpr size_t many_lds(int cols) { return (size_t) 2 * cols * 256 + 2 * 8192;
 
 template <int GM> void init_many() {
     const auto raise = [](const void * f, int cols) { (void) hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int) many_lds(cols)); };
-    raise((const void *) k_i4_many<2, 2, 4, 4, GM, false>, 128);
-    raise((const void *) k_i4_many<2, 2, 4, 4, GM, true>, 128);
-    raise((const void *) k_i4_many<1, 4, 4, 2, GM, false>, 64);
-    raise((const void *) k_i4_many<1, 4, 4, 2, GM, true>, 64);
+    raise((const void *) k_i4_many<2, 2, 4, 4, GM, false, false>, 128);
+    raise((const void *) k_i4_many<2, 2, 4, 4, GM, true, false>, 128);
+    raise((const void *) k_i4_many<2, 2, 4, 4, GM, false, true>, 128);
+    raise((const void *) k_i4_many<2, 2, 4, 4, GM, true, true>, 128);
+    raise((const void *) k_i4_many<1, 4, 4, 2, GM, false, false>, 64);
+    raise((const void *) k_i4_many<1, 4, 4, 2, GM, true, false>, 64);
+    raise((const void *) k_i4_many<1, 4, 4, 2, GM, false, true>, 64);
+    raise((const void *) k_i4_many<1, 4, 4, 2, GM, true, true>, 64);
 }
 
 template <int GM>
 void pick_many(i4_many & p, bool glu, int cols, hipStream_t stream) {
     const int rows = glu ? 64 : 128;
-    p.row_tiles = (int) ((p.nrows + rows - 1) / rows);
+    p.row_tiles = (p.nrows + rows - 1) / rows;
     p.col_tiles = (p.ncols + cols - 1) / cols;
     // lists: no more pieces than full ones and one cut short to a matrix
-    const int64_t pieces = p.bounds ? std::min<int64_t>(p.ncols, p.ncols / cols + p.n_matrices) : p.col_tiles;
-    const int64_t n = p.bounds ? pieces * p.row_tiles : (pieces * p.row_tiles + 7) / 8 * 8;
-    const auto go = [&](auto * kernel) { kernel<<<(unsigned) n, 256, many_lds(cols), stream>>>(p); };
-    cols == 128 ? (glu ? go(k_i4_many<2, 2, 4, 4, GM, true>) : go(k_i4_many<2, 2, 4, 4, GM, false>))
-                : (glu ? go(k_i4_many<1, 4, 4, 2, GM, true>) : go(k_i4_many<1, 4, 4, 2, GM, false>));
+    const bool list = p.bounds != nullptr;
+    const int64_t pieces = list ? std::min<int64_t>(p.ncols, p.ncols / cols + p.n_matrices + 1) : p.col_tiles;
+    const unsigned n = (unsigned) ((pieces * p.row_tiles + 7) / 8 * 8);
+    const auto go = [&](auto * kernel) { kernel<<<n, 256, many_lds(cols), stream>>>(p); };
+    if (cols == 128) {
+        list ? (glu ? go(k_i4_many<2, 2, 4, 4, GM, true, true>) : go(k_i4_many<2, 2, 4, 4, GM, false, true>))
+             : (glu ? go(k_i4_many<2, 2, 4, 4, GM, true, false>) : go(k_i4_many<2, 2, 4, 4, GM, false, false>));
+    } else {
+        list ? (glu ? go(k_i4_many<1, 4, 4, 2, GM, true, true>) : go(k_i4_many<1, 4, 4, 2, GM, false, true>))
+             : (glu ? go(k_i4_many<1, 4, 4, 2, GM, true, false>) : go(k_i4_many<1, 4, 4, 2, GM, false, false>));
+    }
 }
 
 i4_matrix matrix_of(const bf16n_int4_weight & w) { return {w.codes, (const uint16_t *) w.scales, w.zeros, w.scales_f16 != 0}; }
@@ -935,7 +983,10 @@ void run_many(const bf16n_int4_weight & w, const bf16n_int4_weight * up, i4_many
     p.sums = (const u32x4_t *) workspace;
     p.sums_row = (int) ((w.K + group - 1) / group);
     const int64_t threads = x_rows * ((w.K / 32 + per - 1) / per * per);
-    k_i4_sums<<<(unsigned) ((threads + 255) / 256), 256, 0, stream>>>(p.x, p.x_row, w.K, group, x_rows, (u32x4_t *) workspace, p.sums_row);
+    int2 * const table = (int2 *) ((u32x4_t *) workspace + x_rows * p.sums_row);
+    p.table = table;
+    k_i4_sums<<<(unsigned) ((threads + 255) / 256 + (p.bounds ? 1 : 0)), 256, 0, stream>>>(p.x, p.x_row, p.K, group, x_rows, (u32x4_t *) workspace, p.sums_row,
+                                                                                         p.bounds, p.n_matrices, cols, table);
     (p.group_log2 >= 7 ? pick_many<0> : p.group_log2 == 6 ? pick_many<1> : pick_many<2>)(p, up != nullptr, cols, stream);
 }
 
@@ -968,14 +1019,15 @@ void int4_init() {
     init_many<2>();
 }
 
-int64_t int4_workspace_bytes(const bf16n_int4_weight & w, int64_t x_rows) {
+// sums of the activations' groups, and the pieces of lists (at most one of a matrix cut short, one of the pairs without a matrix)
+int64_t int4_workspace_bytes(const bf16n_int4_weight & w, int64_t x_rows, int64_t n_pairs, int n_matrices) {
     const int group = std::min(w.group, I4_STEP);
-    return x_rows * ((w.K + group - 1) / group) * 16;
+    return x_rows * ((w.K + group - 1) / group) * 16 + (n_pairs ? (n_pairs / 64 + n_matrices + 2) * 8 : 0);
 }
 
 void launch_int4_mmv(const bf16n_int4_weight & w, const bf16n_int4_weight * up, const bf16n_mmv_args & a, bool ids_i64, void * workspace,
                      uint64_t workspace_bytes, int cus, hipStream_t stream) {
-    if (!a.ids && a.x_bf16 && a.ncols > 32 && a.x_tok >= 0 && a.ncols * a.x_tok < (int64_t) 1 << 32 && (int64_t) workspace_bytes >= int4_workspace_bytes(w, a.ncols)) {
+    if (!a.ids && a.x_bf16 && a.ncols > 32 && a.x_tok >= 0 && a.ncols * a.x_tok < (int64_t) 1 << 32 && (int64_t) workspace_bytes >= int4_workspace_bytes(w, a.ncols, 0, 0)) {
         i4_many p = {};
         p.x = (const char *) a.x; p.x_row = a.x_tok;
         p.y = (char *) a.y; p.y_row = a.y_tok; p.y_bf16 = a.y_bf16 != 0;
@@ -1013,7 +1065,7 @@ void launch_int4_mm_ids(const bf16n_int4_weight & w, const bf16n_int4_weight * u
                         int cus, hipStream_t stream) {
     const int64_t x_rows = per_slot ? (int64_t) n_tok * n_used : n_tok;
     const int64_t n_pairs = (int64_t) n_tok * n_used;
-    if (n_pairs > 16 * (int64_t) n_matrices && x_row >= 0 && x_rows * x_row < (int64_t) 1 << 31 && (int64_t) workspace_bytes >= int4_workspace_bytes(w, x_rows)) {
+    if (n_pairs > 16 * (int64_t) n_matrices &&  x_row >= 0 && x_rows * x_row < (int64_t) 1 << 31 && (int64_t) workspace_bytes >= int4_workspace_bytes(w, x_rows, n_pairs, n_matrices)) {
         i4_many p = {};
         p.x = (const char *) x; p.x_row = x_row * 2;
         p.y = (char *) y; p.y_row = y_row * (y_bf16 ? 2 : 4); p.y_bf16 = y_bf16;
@@ -1021,8 +1073,7 @@ void launch_int4_mm_ids(const bf16n_int4_weight & w, const bf16n_int4_weight * u
         p.ncols = (int) n_pairs;
         p.pairs = pairs; p.bounds = bounds;
         p.n_matrices = n_matrices; p.n_used = n_used; p.per_slot = per_slot;
-        run_many(w, up, p, x_rows, workspace, n_pairs > 96 * (int64_t) n_matrices ? 128 : 64, stream);
-        k_i4_unnamed<<<(unsigned) std::min<int64_t>(n_pairs, 64), 256, 0, stream>>>(pairs, bounds + n_matrices, p.y, p.y_row, p.nrows * (y_bf16 ? 2 : 4));
+        run_many(w, up, p, x_rows, workspace, 64, stream);
         return;
     }
     i4_launch p = launch_of(w, up, w.rows / n_matrices);

@@ -110,7 +110,7 @@ void launch_router_topk_grouped(const router_grouped_args & a, int n_tok, hipStr
 void int4_init();
 void launch_int4_mmv(const bf16n_int4_weight & w, const bf16n_int4_weight * up, const bf16n_mmv_args & a, bool ids_i64, void * workspace,
                      uint64_t workspace_bytes, int cus, hipStream_t stream);
-int64_t int4_workspace_bytes(const bf16n_int4_weight & w, int64_t x_rows);
+int64_t int4_workspace_bytes(const bf16n_int4_weight & w, int64_t x_rows, int64_t n_pairs, int n_matrices);
 void launch_int4_route(const void * ids, bool i64, int64_t s0, int64_t s1, int n_matrices, int n_tok, int n_used, int32_t * pairs, int32_t * bounds,
                        hipStream_t stream);
 void launch_int4_mm_ids(const bf16n_int4_weight & w, const bf16n_int4_weight * up, const void * x, int64_t x_row, bool per_slot, const int32_t * pairs,

@@ -960,10 +960,11 @@ def _c_int4(w: Int4Weight) -> _lib.Int4Weight:
                            s.dtype is torch.float16)
 
 
-def _int4_workspace(w: Int4Weight, x_rows: int, device: torch.device) -> torch.Tensor:
-    """Workspace of the products of many columns (bf16n_int4_workspace_bytes): 16 bytes for every group of 128 columns, or
-    smaller, of an activation row."""
-    return torch.empty(16 * x_rows * -(-w.K // min(w.group, 128)), dtype=torch.uint8, device=device)
+def _int4_workspace(cw: _lib.Int4Weight, x_rows: int, device: torch.device, n_pairs: int = 0, n_experts: int = 0) -> torch.Tensor:
+    """Workspace of the products of many columns (bf16n_int4_workspace_bytes)."""
+    n = C.c_uint64()
+    _lib.check(_lib.lib().bf16n_int4_workspace_bytes(C.byref(cw), x_rows, n_pairs, n_experts, C.byref(n)))
+    return torch.empty(n.value, dtype=torch.uint8, device=device)
 
 
 def _int4_mmv(what: str, x: torch.Tensor, w: Int4Weight, up: Int4Weight | None, ids: torch.Tensor | None, rows_per_matrix: int,
@@ -1012,7 +1013,7 @@ def _int4_mmv(what: str, x: torch.Tensor, w: Int4Weight, up: Int4Weight | None, 
                          x.stride(1) * xsz if per_slot else 0, n * osz, n, 0, n, T * n_used, n_used, n_used if per_slot else 1, x_bf16, out_bf16)
     ws, nws = None, 0
     if ids is None and x_bf16 and T > INT4_FEW_TOKENS:
-        buf = _int4_workspace(w, T, dev)
+        buf = _int4_workspace(cw, T, dev)
         ws, nws = buf.data_ptr(), buf.numel()
     with _on(dev):
         _lib.check(_lib.lib().bf16n_int4_mmv(C.byref(cw), cu, C.byref(a), i64, ws, nws, _stream()))
@@ -1099,7 +1100,7 @@ def int4_moe_mm_ids(x: torch.Tensor, topk_ids: torch.Tensor, w: Int4Weight, n_ex
         raise ValueError("bf16n.int4_moe_mm_ids: routes must be int4_route's for these ids")
     ws, nws = None, 0
     if T * n_used > n_experts:
-        buf = _int4_workspace(w, T * n_used if per_slot else T, dev)
+        buf = _int4_workspace(cw, T * n_used if per_slot else T, dev, T * n_used, n_experts)
         ws, nws = buf.data_ptr(), buf.numel()
     with _on(dev):
         _lib.check(_lib.lib().bf16n_int4_mm_ids(C.byref(cw), cu, x.data_ptr(), cw.K, per_slot, pairs.data_ptr(), bounds.data_ptr(), y.data_ptr(),
