@@ -389,16 +389,16 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
 // Z1 Z1 Z2 Z1 Z2 Z3 0 0 (what is left out is below 2^-23 of the product), instead of four FMAs per result tile and group.
 
 // X of every activation row, in parts: one thread to 32 columns.  For lists of columns by matrix the last block counts the pieces of
-// `cols` columns of every matrix (and of the pairs that name none) instead and lists them: (matrix, piece), how many in table[0].
+// `cols` columns of every matrix (and of the pairs that name none) instead and lists them: (matrix, first column, columns), how many in table[0].
 __global__ void __launch_bounds__(256) k_i4_sums(const char * x, int64_t x_row, int K, int group, int64_t n_rows, u32x4_t * sums, int64_t sums_row,
-                                                 const int32_t * bounds, int n_matrices, int cols, int2 * table) {
+                                                 const int32_t * bounds, int n_matrices, int cols, int4 * table) {
     if (bounds && blockIdx.x == gridDim.x - 1) {
         __shared__ int of_wave[4];
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         int before = 0;
         for (int b = 0; b <= n_matrices; b += 256) {
             const int m = b + threadIdx.x;
-            const int n = m <= n_matrices ? (bounds[m + 1] - bounds[m] + cols - 1) / cols : 0;
+            const int from = m <= n_matrices ? bounds[m] : 0, to = m <= n_matrices ? bounds[m + 1] : 0, n = (to - from + cols - 1) / cols;
             int upto = n;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
@@ -415,12 +415,12 @@ __global__ void __launch_bounds__(256) k_i4_sums(const char * x, int64_t x_row, 
                 before += of_wave[w];
             }
             for (int k = 0; k < n; k++) {
-                table[1 + at + k] = int2{m, k};
+                table[1 + at + k] = int4{m, from + k * cols, min(cols, to - from - k * cols), 0};
             }
             __syncthreads();
         }
         if (threadIdx.x == 0) {
-            table[0] = int2{before, 0};
+            table[0] = int4{before, 0, 0, 0};
         }
         return;
     }
@@ -464,7 +464,7 @@ struct i4_many {
     int sum_group_log2;
     int ncols;
     const int32_t * pairs, * bounds;        // lists of columns by matrix, or null
-    const int2 * table;                     // and their pieces
+    const int4 * table;                     // and their pieces
     int n_matrices, n_used, per_slot;
     int row_tiles, col_tiles;               // dense: the grid
 };
@@ -496,12 +496,12 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         if ((int) (blockIdx.x >> 3) >= per || id >= n) {
             return;
         }
-        const int2 piece = p.table[1 + id / p.row_tiles];
+        const int4 piece = p.table[1 + id / p.row_tiles];
         const int m = piece.x;
         matrix = m;
         row_tile = id % p.row_tiles;
-        c0 = p.bounds[m] + piece.y * COLS;
-        nc = min(COLS, p.bounds[m + 1] - c0);
+        c0 = piece.y;
+        nc = piece.z;
         if (m == p.n_matrices) { // zeros for the pairs that name none
             const int from = row_tile * ROWS, rows = min(ROWS, p.nrows - from);
             for (int i = threadIdx.x; i < nc * ROWS; i += THREADS) {
@@ -635,7 +635,10 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     const int tiles = (wm * 16 + m16) * 256;
     const auto operand = [&](int at, int m) { return __builtin_bit_cast(bf16x8_t, *(const u32x4_t *) (lds + at + m * (WM * 4096))); };
 
-    copy_sums(0, 0);
+    if (E == 1) { // (a longer row's first step comes with the last sums)
+        copy_codes(0, 1);
+        load_block(0);
+    }
     uint32_t zs[4][NT], zz[4][NT]; // scales and zero points of the groups of a step, ahead of the wait
     const auto load_zeros = [&](int step) {
 #pragma unroll
@@ -650,12 +653,16 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         }
     };
     load_zeros(0);
+    copy_sums(0, 0);
+    if (E == 1) {
+        copy(0, 1);
+    }
     for (int step = 0; step < E; step++) { // the zero points' part: groups step * 16 ..
         const int buf = step & 1;
         arrived();
         if (step + 1 < E) {
             copy_sums(step + 1, buf ^ 1);
-        } else {
+        } else if (E > 1) {
             copy(0, buf ^ 1);
             copy_codes(0, buf ^ 1);
             load_block(0);
@@ -821,25 +828,49 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
 
 // Every (token, slot) pair under the matrix that its id names, in ascending order, and behind them the pairs whose id
 // names none: block e lists the pairs of id e (block n_matrices the others) behind those of the ids below it, which it counts
-// itself.  A wavefront takes a contiguous part of the ids and reads it twice.  Bound by latency: the ids are in L2.
-__global__ void __launch_bounds__(1024) k_i4_route(const char * ids, int64_t s0, int64_t s1, bool i64, int n_matrices, int n_pairs, int n_used,
+// itself.  A wavefront takes a contiguous part of the ids and reads it twice, four ids to a lane at a time where they lie in a row
+// (VECTOR).  Bound by latency: the ids are in L2.
+template <typename ID, bool VECTOR>
+__global__ void __launch_bounds__(1024) k_i4_route(const char * ids, int64_t s0, int64_t s1, int n_matrices, int n_pairs, int n_used,
                                                    int32_t * pairs, int32_t * bounds) {
+    constexpr int V = VECTOR ? 4 : 1, ROUND = 64 * V;
+    typedef ID vec_t __attribute__((ext_vector_type(4)));
     __shared__ int below_w[16], mine_w[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int64_t e = blockIdx.x;
-    const int per = ((n_pairs + waves - 1) / waves + 63) / 64 * 64;
+    const int e = blockIdx.x;
+    const int per = ((n_pairs + waves - 1) / waves + ROUND - 1) / ROUND * ROUND;
     const int lo = min(wave * per, n_pairs), hi = min(lo + per, n_pairs);
-    const auto id_of = [&](int i) -> int64_t {
-        const char * at = ids + (i / n_used) * s1 + (i % n_used) * s0;
-        const int64_t v = i64 ? *(const int64_t *) at : *(const int32_t *) at;
-        return v >= 0 && v < n_matrices ? v : n_matrices;
+    // a pair's matrix: n_matrices for ids that name none, -1 behind the last pair
+    const auto load = [&](int i, int (&v)[V]) {
+        ID at[V];
+        if (VECTOR && i + V <= n_pairs) {
+            const vec_t four = *(const vec_t *) (ids + (int64_t) i * sizeof(ID));
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                at[j] = four[j];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                const int p = min(i + j, n_pairs - 1);
+                at[j] = VECTOR ? ((const ID *) ids)[p] : *(const ID *) (ids + p / n_used * s1 + p % n_used * s0);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            v[j] = i + j >= hi ? -1 : at[j] >= 0 && at[j] < n_matrices ? (int) at[j] : n_matrices;
+        }
     };
     int below = 0, mine = 0;
 #pragma unroll 4
-    for (int b = lo; b < hi; b += 64) {
-        const int64_t v = b + lane < hi ? id_of(b + lane) : INT64_MAX;
-        below += __popcll(__ballot(v < e));
-        mine += __popcll(__ballot(v == e));
+    for (int b = lo; b < hi; b += ROUND) {
+        int v[V];
+        load(b + lane * V, v);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            below += __popcll(__ballot((unsigned) v[j] < (unsigned) e));
+            mine += __popcll(__ballot(v[j] == e));
+        }
     }
     if (lane == 0) {
         below_w[wave] = below;
@@ -861,13 +892,22 @@ __global__ void __launch_bounds__(1024) k_i4_route(const char * ids, int64_t s0,
         return;
     }
 #pragma unroll 4
-    for (int b = lo; b < hi; b += 64) {
-        const bool in = b + lane < hi && id_of(b + lane) == e;
-        const uint64_t at = __ballot(in);
-        if (in) {
-            pairs[start + __popcll(at & ((1ull << lane) - 1))] = b + lane;
+    for (int b = lo; b < hi; b += ROUND) {
+        int v[V];
+        load(b + lane * V, v);
+        int at = start;
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const uint64_t who = __ballot(v[j] == e);
+            at += __popcll(who & ((1ull << lane) - 1)); // lanes below: all of their ids come first
+            start += __popcll(who);
         }
-        start += __popcll(at);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            if (v[j] == e) {
+                pairs[at++] = b + lane * V + j;
+            }
+        }
     }
 }
 
@@ -983,7 +1023,7 @@ void run_many(const bf16n_int4_weight & w, const bf16n_int4_weight * up, i4_many
     p.sums = (const u32x4_t *) workspace;
     p.sums_row = (int) ((w.K + group - 1) / group);
     const int64_t threads = x_rows * ((w.K / 32 + per - 1) / per * per);
-    int2 * const table = (int2 *) ((u32x4_t *) workspace + x_rows * p.sums_row);
+    int4 * const table = (int4 *) ((u32x4_t *) workspace + x_rows * p.sums_row);
     p.table = table;
     k_i4_sums<<<(unsigned) ((threads + 255) / 256 + (p.bounds ? 1 : 0)), 256, 0, stream>>>(p.x, p.x_row, p.K, group, x_rows, (u32x4_t *) workspace, p.sums_row,
                                                                                          p.bounds, p.n_matrices, cols, table);
@@ -1022,7 +1062,7 @@ void int4_init() {
 // sums of the activations' groups, and the pieces of lists (at most one of a matrix cut short, one of the pairs without a matrix)
 int64_t int4_workspace_bytes(const bf16n_int4_weight & w, int64_t x_rows, int64_t n_pairs, int n_matrices) {
     const int group = std::min(w.group, I4_STEP);
-    return x_rows * ((w.K + group - 1) / group) * 16 + (n_pairs ? (n_pairs / 64 + n_matrices + 2) * 8 : 0);
+    return x_rows * ((w.K + group - 1) / group) * 16 + (n_pairs ? (n_pairs / 64 + n_matrices + 3) * 16 : 0);
 }
 
 void launch_int4_mmv(const bf16n_int4_weight & w, const bf16n_int4_weight * up, const bf16n_mmv_args & a, bool ids_i64, void * workspace,
@@ -1057,7 +1097,9 @@ void launch_int4_route(const void * ids, bool i64, int64_t s0, int64_t s1, int n
                        hipStream_t stream) {
     const int n = n_tok * n_used;
     const int threads = n <= 256 ? 256 : 1024;
-    k_i4_route<<<n_matrices + 1, threads, 0, stream>>>((const char *) ids, s0, s1, i64, n_matrices, n, n_used, pairs, bounds);
+    const bool row = s0 == (i64 ? 8 : 4) && (s1 == s0 * n_used || n_tok == 1) && (uintptr_t) ids % (4 * s0) == 0;
+    (i64 ? row ? k_i4_route<int64_t, true> : k_i4_route<int64_t, false> : row ? k_i4_route<int32_t, true> : k_i4_route<int32_t, false>)
+        <<<n_matrices + 1, threads, 0, stream>>>((const char *) ids, s0, s1, n_matrices, n, n_used, pairs, bounds);
 }
 
 void launch_int4_mm_ids(const bf16n_int4_weight & w, const bf16n_int4_weight * up, const void * x, int64_t x_row, bool per_slot, const int32_t * pairs,
