@@ -480,8 +480,9 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     constexpr int NG = GM == 0 ? 1 : GM == 1 ? 2 : 4, LOADS = COLS * 16 / THREADS;
     static_assert(THREADS == 256 && LOADS * THREADS == COLS * 16, "a thread copies the same place of rows 16 apart");
     static_assert(WN * NT == 8, "a wavefront copies the codes of two tiles of rows");
-    extern __shared__ __align__(16) char lds[]; // two pieces of activations, two of codes
+    extern __shared__ __align__(16) char lds[]; // two pieces of activations, two of codes, for lists the places of the results
     constexpr int CODES = 2 * COLS * 256;
+    int64_t * const y_at = (int64_t *) (lds + CODES + 2 * 8192);
     const int lane = threadIdx.x & 63, m16 = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % WM, wn = wave / WM;
@@ -524,24 +525,24 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         c0 = (group * 4 + in % wide) * COLS;
         nc = min(COLS, p.ncols - c0);
     }
-    const auto pair_of = [&](int i) { // the list's pair, or the dense column, behind column i; columns that are not there repeat the last
+    const auto x_row_of = [&](int i) { // the activation row behind column i; columns that are not there repeat the last
         const int c = c0 + min(i, nc - 1);
-        return p.pairs ? p.pairs[c] : c;
+        return !LIST ? c : p.per_slot ? p.pairs[c] : p.pairs[c] / p.n_used;
     };
-    const auto x_row_of = [&](int i) {
-        const int pair = pair_of(i);
-        return p.pairs && !p.per_slot ? pair / p.n_used : pair;
-    };
+    if (LIST && threadIdx.x < nc) {
+        y_at[threadIdx.x] = p.pairs[c0 + threadIdx.x] * p.y_row; // (read behind the barriers of the steps)
+    }
 
     const int row0 = row_tile * ROWS;
     const int S = (int) ((p.K + I4_STEP - 1) / I4_STEP), E = (p.sums_row + 15) / 16;
     const int place = threadIdx.x & 15, octet = place ^ (threadIdx.x >> 4); // what this thread copies: places of rows (threadIdx.x >> 4) + 16 i
     // (rows of the activations start below 2^32 bytes, the launch sees to it; octets behind the last column repeat one before it: the codes
     // are zeros there)
-    uint32_t x_off[LOADS];
+    uint32_t x_off[LOADS], x_at[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; i++) {
-        x_off[i] = (uint32_t) x_row_of(i * 16 + (threadIdx.x >> 4)) * (uint32_t) p.x_row + octet * 16;
+        x_at[i] = x_row_of(i * 16 + (threadIdx.x >> 4));
+        x_off[i] = x_at[i] * (uint32_t) p.x_row + octet * 16;
     }
     const bool cut = p.K % I4_STEP != 0; // the last step is cut short
     const auto copy_sums = [&](int step, int buf) {
@@ -550,7 +551,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
             if (i * 16 >= nc) {
                 break;
             }
-            const int64_t r = x_row_of(i * 16 + (threadIdx.x >> 4));
+            const int64_t r = x_at[i];
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (p.sums + r * p.sums_row + min(step * 16 + octet, p.sums_row - 1)),
                                              (__attribute__((address_space(3))) void *) (lds + buf * (COLS * 256) + wave * 1024 + i * 4096), 16, 0, 0);
         }
@@ -811,7 +812,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         for (int e = 0; e < 4; e++) {
             const int c = (m * WM + wm) * 16 + q * 4 + e;
             if (c < nc) {
-                char * const y = p.y + pair_of(c) * p.y_row;
+                char * const y = p.y + (LIST ? y_at[c] : (c0 + c) * p.y_row);
 #pragma unroll
                 for (int n = 0; n < (GLU ? NT / 2 : NT); n++) {
                     const int r = row0 + (wn * (GLU ? NT / 2 : NT) + n) * 16 + m16;
@@ -965,14 +966,12 @@ void init_few() {
     }
 }
 
-constexpr size_t many_lds(int cols) { return (size_t) 2 * cols * 256 + 2 * 8192; }
+constexpr size_t many_lds(int cols, bool list) { return (size_t) 2 * cols * 256 + 2 * 8192 + (list ? cols * 8 : 0); }
 
 template <int GM> void init_many() {
-    const auto raise = [](const void * f, int cols) { (void) hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int) many_lds(cols)); };
+    const auto raise = [](const void * f, int cols) { (void) hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int) many_lds(cols, true)); };
     raise((const void *) k_i4_many<2, 2, 4, 4, GM, false, false>, 128);
     raise((const void *) k_i4_many<2, 2, 4, 4, GM, true, false>, 128);
-    raise((const void *) k_i4_many<2, 2, 4, 4, GM, false, true>, 128);
-    raise((const void *) k_i4_many<2, 2, 4, 4, GM, true, true>, 128);
     raise((const void *) k_i4_many<1, 4, 4, 2, GM, false, false>, 64);
     raise((const void *) k_i4_many<1, 4, 4, 2, GM, true, false>, 64);
     raise((const void *) k_i4_many<1, 4, 4, 2, GM, false, true>, 64);
@@ -988,13 +987,13 @@ void pick_many(i4_many & p, bool glu, int cols, hipStream_t stream) {
     const bool list = p.bounds != nullptr;
     const int64_t pieces = list ? std::min<int64_t>(p.ncols, p.ncols / cols + p.n_matrices + 1) : p.col_tiles;
     const unsigned n = (unsigned) ((pieces * p.row_tiles + 7) / 8 * 8);
-    const auto go = [&](auto * kernel) { kernel<<<n, 256, many_lds(cols), stream>>>(p); };
-    if (cols == 128) {
-        list ? (glu ? go(k_i4_many<2, 2, 4, 4, GM, true, true>) : go(k_i4_many<2, 2, 4, 4, GM, false, true>))
-             : (glu ? go(k_i4_many<2, 2, 4, 4, GM, true, false>) : go(k_i4_many<2, 2, 4, 4, GM, false, false>));
+    const auto go = [&](auto * kernel) { kernel<<<n, 256, many_lds(cols, list), stream>>>(p); };
+    if (list) {
+        glu ? go(k_i4_many<1, 4, 4, 2, GM, true, true>) : go(k_i4_many<1, 4, 4, 2, GM, false, true>);
+    } else if (cols == 128) {
+        glu ? go(k_i4_many<2, 2, 4, 4, GM, true, false>) : go(k_i4_many<2, 2, 4, 4, GM, false, false>);
     } else {
-        list ? (glu ? go(k_i4_many<1, 4, 4, 2, GM, true, true>) : go(k_i4_many<1, 4, 4, 2, GM, false, true>))
-             : (glu ? go(k_i4_many<1, 4, 4, 2, GM, true, false>) : go(k_i4_many<1, 4, 4, 2, GM, false, false>));
+        glu ? go(k_i4_many<1, 4, 4, 2, GM, true, false>) : go(k_i4_many<1, 4, 4, 2, GM, false, false>);
     }
 }
 
