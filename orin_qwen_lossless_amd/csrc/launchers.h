@@ -103,8 +103,9 @@ struct router_grouped_args {
     bool sigmoid, top2, renorm;
     float scale;
     int32_t * ids; float * weights; int64_t out_stride;
+    int group_size; uint32_t group_factor; // of the launch
 };
-void launch_router_topk_grouped(const router_grouped_args & a, int n_tok, hipStream_t stream);
+void launch_router_topk_grouped(router_grouped_args a, int n_tok, hipStream_t stream);
 
 // 4-bit weights with group scales (kernels_int4.hip)
 void int4_init();
