@@ -1,4 +1,5 @@
-// The dense products' calls from Python in native code: mmv(x, w, out_bf16, multi_col) and linear(x, w, gemv_tokens, chunk_bytes).
+// The dense products' calls from Python in native code: mmv(x, w, out_bf16, multi_col) and linear(x, w, gemv_tokens, chunk_bytes);
+// those of 4-bit weights with group scales, int4_mmv and int4_moe_experts; and the selection, router_topk_grouped.
 //
 // A small product is bound by the host's call (512 x 2048, one token: the kernel takes 3 us, the call with its checks, result
 // and argument block in Python 9.2).  This does the same for the plain case: a two-dimensional tensor of the plain class on the
@@ -183,6 +184,254 @@ PyObject * linear(PyObject *, PyObject * const * args, Py_ssize_t n) {
     }
 }
 
+// ---------------------------------------------------------------- 4-bit weights with group scales, selection in groups
+
+typedef int (*int4_bytes_fn)(const bf16n_int4_weight *, int64_t, int64_t, int, uint64_t *);
+typedef int (*int4_mmv_fn)(const bf16n_int4_weight *, const bf16n_int4_weight *, const bf16n_mmv_args *, int, void *, uint64_t, void *);
+typedef int (*int4_route_fn)(const void *, int, int64_t, int64_t, int, int, int, int32_t *, int32_t *, void *);
+typedef int (*int4_mm_ids_fn)(const bf16n_int4_weight *, const bf16n_int4_weight *, const void *, int64_t, int, const int32_t *, const int32_t *, void *,
+                              int, int64_t, int, int, int, void *, uint64_t, void *);
+typedef int (*combine_fn)(const float *, const void *, int, void *, int, int, int, int64_t, void *);
+typedef int (*router_fn)(const float *, int64_t, const float *, int, int, int, int, int, int, int, int, float, int32_t *, float *, int64_t, void *);
+int4_bytes_fn g_int4_bytes = nullptr;
+int4_mmv_fn g_int4_mmv = nullptr;
+int4_route_fn g_int4_route = nullptr;
+int4_mm_ids_fn g_int4_mm_ids = nullptr;
+combine_fn g_combine = nullptr;
+router_fn g_router = nullptr;
+PyObject * s_codes, * s_scales, * s_zeros, * s_group;
+
+bool native() { return g_int4_mmv && !at::impl::torch_function_mode_enabled() && !c10::impl::dispatch_mode_enabled(); }
+
+at::TensorOptions on(const at::Tensor & like, at::ScalarType t) { return like.options().dtype(t).requires_grad(false); }
+void * stream_of(int device) { return (void *) c10::hip::getCurrentHIPStream((c10::DeviceIndex) device).stream(); }
+
+// an Int4Weight on the device, its tensors as their class has checked them
+bool int4_matrix(PyObject * o, int device, bf16n_int4_weight & w) {
+    const ref co(o, s_codes), sc(o, s_scales), ze(o, s_zeros);
+    if (!co.o || !sc.o || !ze.o) {
+        return false;
+    }
+    const at::Tensor * c = plain(co.o), * s = plain(sc.o), * z = ze.o == Py_None ? nullptr : plain(ze.o);
+    int64_t group;
+    if (!c || !s || (!z && ze.o != Py_None) || !number(o, s_group, group) || c->dim() != 2 || s->dim() != 2 || group < 32 || group > 1 << 30 ||
+        (group & (group - 1)) || c->scalar_type() != at::kByte || !c->is_contiguous() || !s->is_contiguous()) {
+        return false;
+    }
+    w = {};
+    w.rows = c->size(0);
+    w.K = 2 * c->size(1);
+    w.group = (int32_t) group;
+    w.scales_f16 = s->scalar_type() == at::kHalf;
+    const int64_t groups = (w.K + group - 1) / group;
+    if (c->get_device() != device || s->get_device() != device || (!w.scales_f16 && s->scalar_type() != at::kBFloat16) || s->size(0) != w.rows || s->size(1) != groups ||
+        (z && (z->get_device() != device || z->scalar_type() != at::kByte || !z->is_contiguous() || z->dim() != 2 || z->size(0) != w.rows || z->size(1) != groups))) {
+        return false;
+    }
+    w.codes = (const uint8_t *) c->data_ptr();
+    w.scales = s->data_ptr();
+    w.zeros = z ? (const uint8_t *) z->data_ptr() : nullptr;
+    return w.rows > 0;
+}
+bool alike(const bf16n_int4_weight & a, const bf16n_int4_weight & b) { return a.rows == b.rows && a.K == b.K && a.group == b.group && !a.zeros == !b.zeros; }
+
+// rows of K activations, 16-byte aligned as the kernels read them
+const at::Tensor * int4_x(PyObject * o, int device, int64_t K) {
+    const at::Tensor * x = plain(o);
+    if (!x || x->dim() != 2 || x->get_device() != device || (x->scalar_type() != at::kBFloat16 && x->scalar_type() != at::kFloat) || x->size(0) <= 0 ||
+        x->size(0) > 1 << 24 || x->size(1) != K || x->stride(1) != 1 || x->stride(0) * x->element_size() % 16 != 0 || (uintptr_t) x->data_ptr() % 16 != 0) {
+        return nullptr;
+    }
+    return x;
+}
+
+bf16n_mmv_args int4_args(const at::Tensor & x, const at::Tensor & y, int64_t rows) {
+    bf16n_mmv_args a = {};
+    a.x = (decltype(a.x)) x.data_ptr();
+    a.y = (decltype(a.y)) y.data_ptr();
+    a.x_tok = x.stride(0) * x.element_size();
+    a.y_tok = y.stride(0) * y.element_size();
+    a.rows_per_matrix = a.nrows = rows;
+    a.ncols = (int32_t) x.size(0);
+    a.n_used = a.x_per_slot = 1;
+    a.x_bf16 = x.scalar_type() == at::kBFloat16;
+    a.y_bf16 = y.scalar_type() == at::kBFloat16;
+    return a;
+}
+
+// int4_mmv(x, w, up or None, out_bf16, few_tokens): dense
+PyObject * int4_mmv(PyObject *, PyObject * const * args, Py_ssize_t n) {
+    try {
+        if (n != 5 || !native()) {
+            return not_taken();
+        }
+        const int device = c10::hip::current_device();
+        bf16n_int4_weight w, up;
+        const bool glu = args[2] != Py_None;
+        if (!int4_matrix(args[1], device, w) || (glu && (!int4_matrix(args[2], device, up) || !alike(w, up)))) {
+            return not_taken();
+        }
+        const at::Tensor * x = int4_x(args[0], device, w.K);
+        const int64_t few = PyLong_AsLongLong(args[4]);
+        if (!x || few < 0) {
+            return not_taken();
+        }
+        at::Tensor y = at::empty({x->size(0), w.rows}, on(*x, args[3] == Py_True ? at::kBFloat16 : at::kFloat)), space;
+        const bf16n_mmv_args a = int4_args(*x, y, w.rows);
+        uint64_t bytes = 0;
+        if (a.x_bf16 && x->size(0) > few) {
+            if (g_int4_bytes(&w, x->size(0), 0, 0, &bytes) != 0) {
+                return not_taken();
+            }
+            space = at::empty({(int64_t) bytes}, on(*x, at::kByte));
+        }
+        int status;
+        {
+            pybind11::gil_scoped_release free;
+            status = g_int4_mmv(&w, glu ? &up : nullptr, &a, 0, bytes ? space.data_ptr() : nullptr, bytes, stream_of(device));
+        }
+        return status == 0 ? THPVariable_Wrap(y) : PyLong_FromLong(status);
+    } catch (const std::exception &) {
+        return not_taken();
+    }
+}
+
+// int4_moe_experts(x, gate, up, down, topk_weights, topk_ids, n_experts, batched): the launches of the Python layer's, in its order
+PyObject * int4_moe_experts(PyObject *, PyObject * const * args, Py_ssize_t n) {
+    try {
+        if (n != 8 || !native()) {
+            return not_taken();
+        }
+        const int device = c10::hip::current_device();
+        bf16n_int4_weight gate, up, down;
+        if (!int4_matrix(args[1], device, gate) || !int4_matrix(args[2], device, up) || !int4_matrix(args[3], device, down) || !alike(gate, up)) {
+            return not_taken();
+        }
+        const at::Tensor * x = int4_x(args[0], device, gate.K), * wts = plain(args[4]), * ids = plain(args[5]);
+        const int64_t E = PyLong_AsLongLong(args[6]);
+        const bool batched = args[7] == Py_True;
+        if (!x || !wts || !ids || E <= 0 || E > 65534 || gate.rows % E || down.rows % E || down.K != gate.rows / E || !x->is_contiguous() || ids->dim() != 2 ||
+            (ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong) || ids->get_device() != device || ids->size(0) != x->size(0) || ids->size(1) <= 0 ||
+            ids->stride(1) != 1 || wts->dim() != 2 || wts->get_device() != device || !wts->is_contiguous() ||
+            (wts->scalar_type() != at::kFloat && wts->scalar_type() != at::kBFloat16) || wts->size(0) != ids->size(0) || wts->size(1) != ids->size(1)) {
+            return not_taken();
+        }
+        const int64_t T = ids->size(0), slots = ids->size(1), mid = gate.rows / E, out = down.rows / E, pairs = T * slots;
+        const bool x_bf16 = x->scalar_type() == at::kBFloat16;
+        if (T > 65535 || pairs > (batched ? 1 << 28 : 65535) || (batched && !x_bf16) || gate.rows / E > 1 << 30) {
+            return not_taken();
+        }
+        const int i64 = ids->scalar_type() == at::kLong, isz = i64 ? 8 : 4;
+        at::Tensor hidden = at::empty({pairs, mid}, on(*x, batched ? at::kBFloat16 : at::kFloat));
+        at::Tensor ys = at::empty({pairs, out}, on(*x, at::kFloat)), y = at::empty({T, out}, on(*x, at::kBFloat16)), lists, space;
+        uint64_t bytes = 0;
+        if (batched) {
+            uint64_t second = 0;
+            if (g_int4_bytes(&gate, T, pairs, (int) E, &bytes) != 0 || g_int4_bytes(&down, pairs, pairs, (int) E, &second) != 0) {
+                return not_taken();
+            }
+            bytes = std::max(bytes, second);
+            lists = at::empty({pairs + E + 2}, on(*x, at::kInt));
+            space = at::empty({(int64_t) bytes}, on(*x, at::kByte));
+        }
+        void * const stream = stream_of(device);
+        int status;
+        {
+            pybind11::gil_scoped_release free;
+            if (batched) {
+                int32_t * const sorted = (int32_t *) lists.data_ptr(), * const bounds = sorted + pairs;
+                status = g_int4_route(ids->data_ptr(), i64, isz, ids->stride(0) * isz, (int) E, (int) T, (int) slots, sorted, bounds, stream);
+                status = status ? status : g_int4_mm_ids(&gate, &up, x->data_ptr(), gate.K, 0, sorted, bounds, hidden.data_ptr(), 1, mid, (int) E, (int) T, (int) slots,
+                                                         space.data_ptr(), bytes, stream);
+                status = status ? status : g_int4_mm_ids(&down, nullptr, hidden.data_ptr(), mid, 1, sorted, bounds, ys.data_ptr(), 0, out, (int) E, (int) T, (int) slots,
+                                                         space.data_ptr(), bytes, stream);
+            } else {
+                bf16n_mmv_args a = int4_args(*x, hidden, mid);
+                a.ids = (decltype(a.ids)) ids->data_ptr();
+                a.ids_s0 = isz;
+                a.ids_s1 = ids->stride(0) * isz;
+                a.ncols = (int32_t) pairs;
+                a.n_used = (int32_t) slots;
+                a.y_slot = mid * 4;
+                a.y_tok = slots * a.y_slot;
+                bf16n_mmv_args b = int4_args(hidden, ys, out);
+                b.ids = a.ids;
+                b.ids_s0 = a.ids_s0;
+                b.ids_s1 = a.ids_s1;
+                b.n_used = b.x_per_slot = (int32_t) slots;
+                b.x_slot = a.y_slot;
+                b.x_tok = a.y_tok;
+                b.y_slot = out * 4;
+                b.y_tok = slots * b.y_slot;
+                status = g_int4_mmv(&gate, &up, &a, i64, nullptr, 0, stream);
+                status = status ? status : g_int4_mmv(&down, nullptr, &b, i64, nullptr, 0, stream);
+            }
+            status = status ? status : g_combine((const float *) ys.data_ptr(), wts->data_ptr(), wts->scalar_type() == at::kBFloat16, y.data_ptr(), 1, (int) T, (int) slots, out, stream);
+        }
+        return status == 0 ? THPVariable_Wrap(y) : PyLong_FromLong(status);
+    } catch (const std::exception &) {
+        return not_taken();
+    }
+}
+
+// router_topk_grouped(logits, k, bias or None, n_groups, topk_groups, sigmoid, top2, renorm, scale) -> (weights, ids)
+PyObject * router_topk_grouped(PyObject *, PyObject * const * args, Py_ssize_t n) {
+    try {
+        if (n != 9 || !native()) {
+            return not_taken();
+        }
+        const int device = c10::hip::current_device();
+        const at::Tensor * lg = plain(args[0]), * bias = args[2] == Py_None ? nullptr : plain(args[2]);
+        int64_t v[3];
+        for (int i = 0; i < 3; i++) {
+            PyObject * o = args[i ? 2 + i : 1];
+            if (!PyLong_Check(o)) {
+                return not_taken();
+            }
+            v[i] = PyLong_AsLongLong(o);
+        }
+        const double scale = PyFloat_AsDouble(args[8]);
+        if (PyErr_Occurred() || !lg || (!bias && args[2] != Py_None) || lg->dim() != 2 || lg->get_device() != device || lg->scalar_type() != at::kFloat || lg->stride(1) != 1 ||
+            lg->size(0) <= 0 || lg->size(0) > INT32_MAX || lg->size(1) > 1024 || v[0] <= 0 || v[0] > 64 || v[1] <= 0 || v[1] > 64 || v[2] <= 0 || v[2] > 64 ||
+            (bias && (bias->get_device() != device || bias->scalar_type() != at::kFloat || !bias->is_contiguous() || bias->numel() != lg->size(1)))) {
+            return not_taken();
+        }
+        const int64_t T = lg->size(0);
+        at::Tensor wts = at::empty({T, v[0]}, on(*lg, at::kFloat)), ids = at::empty({T, v[0]}, on(*lg, at::kInt));
+        const int status = g_router((const float *) lg->data_ptr(), lg->stride(0), bias ? (const float *) bias->data_ptr() : nullptr, (int) T, (int) lg->size(1), (int) v[1], (int) v[2],
+                                    (int) v[0], args[5] == Py_True, args[6] == Py_True, args[7] == Py_True, (float) scale, (int32_t *) ids.data_ptr(), (float *) wts.data_ptr(), v[0],
+                                    stream_of(device));
+        if (status != 0) {
+            return PyLong_FromLong(status);
+        }
+        PyObject * a = THPVariable_Wrap(wts), * b = THPVariable_Wrap(ids);
+        PyObject * both = a && b ? PyTuple_Pack(2, a, b) : nullptr;
+        Py_XDECREF(a);
+        Py_XDECREF(b);
+        return both;
+    } catch (const std::exception &) {
+        return not_taken();
+    }
+}
+
+PyObject * bind_int4(PyObject *, PyObject * const * args, Py_ssize_t n) {
+    if (n != 6) {
+        PyErr_SetString(PyExc_TypeError, "bind_int4: six addresses");
+        return nullptr;
+    }
+    g_int4_bytes = (int4_bytes_fn) PyLong_AsVoidPtr(args[0]);
+    g_int4_route = (int4_route_fn) PyLong_AsVoidPtr(args[2]);
+    g_int4_mm_ids = (int4_mm_ids_fn) PyLong_AsVoidPtr(args[3]);
+    g_combine = (combine_fn) PyLong_AsVoidPtr(args[4]);
+    g_router = (router_fn) PyLong_AsVoidPtr(args[5]);
+    g_int4_mmv = (int4_mmv_fn) PyLong_AsVoidPtr(args[1]);
+    if (PyErr_Occurred()) {
+        g_int4_mmv = nullptr;
+        return nullptr;
+    }
+    Py_RETURN_NONE;
+}
+
 PyObject * bind(PyObject *, PyObject * const * args, Py_ssize_t n) {
     if (n != 3) {
         PyErr_SetString(PyExc_TypeError, "bind: three addresses");
@@ -201,6 +450,11 @@ PyObject * bind(PyObject *, PyObject * const * args, Py_ssize_t n) {
 PyMethodDef g_methods[] = {
     {"mmv", (PyCFunction) (void (*)(void)) mmv, METH_FASTCALL, "the product, a status of the C ABI, or None: not taken"},
     {"linear", (PyCFunction) (void (*)(void)) linear, METH_FASTCALL, "the same for BF16 in and out and any number of tokens"},
+    {"int4_mmv", (PyCFunction) (void (*)(void)) int4_mmv, METH_FASTCALL, "the dense product, plain or gated, of 4-bit weights with group scales"},
+    {"int4_moe_experts", (PyCFunction) (void (*)(void)) int4_moe_experts, METH_FASTCALL, "routed experts on such weights"},
+    {"router_topk_grouped", (PyCFunction) (void (*)(void)) router_topk_grouped, METH_FASTCALL, "(weights, ids), a status of the C ABI, or None"},
+    {"bind_int4", (PyCFunction) (void (*)(void)) bind_int4, METH_FASTCALL,
+     "the addresses of bf16n_int4_workspace_bytes, _mmv, _route, _mm_ids, bf16n_moe_combine, bf16n_router_topk_grouped"},
     {"bind", (PyCFunction) (void (*)(void)) bind, METH_FASTCALL, "the addresses of bf16n_mmv, bf16n_gemv_max_tokens, bf16n_dequant"},
     {nullptr, nullptr, 0, nullptr},
 };
@@ -209,8 +463,10 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, g_methods, 
 } // namespace
 
 PyMODINIT_FUNC PyInit__host(void) {
-    PyObject ** const names[] = {&s_plane, &s_aux, &s_meta, &s_format, &s_K, &s_rows, &s_R, &s_cm, &s_frag, &s_w64, &s_off[0], &s_off[1], &s_off[2], &s_off[3]};
-    const char * const text[] = {"plane", "aux", "meta", "format", "K", "rows", "R", "chunk_major", "frag_order", "wave64", "off_a", "off_b", "off_c", "off_d"};
+    PyObject ** const names[] = {&s_plane, &s_aux, &s_meta, &s_format, &s_K, &s_rows, &s_R, &s_cm, &s_frag, &s_w64, &s_off[0], &s_off[1], &s_off[2], &s_off[3],
+                                 &s_codes, &s_scales, &s_zeros, &s_group};
+    const char * const text[] = {"plane", "aux", "meta", "format", "K", "rows", "R", "chunk_major", "frag_order", "wave64", "off_a", "off_b", "off_c", "off_d",
+                                 "codes", "scales", "zeros", "group"};
     for (size_t i = 0; i < sizeof(text) / sizeof(text[0]); i++) {
         if (!(*names[i] = PyUnicode_InternFromString(text[i]))) {
             return nullptr;

@@ -301,7 +301,7 @@ class _NoNativeCalls:
     def mmv(*_):
         return None
 
-    linear = mmv
+    linear = int4_mmv = int4_moe_experts = router_topk_grouped = mmv
 
 
 def _host():
@@ -313,6 +313,8 @@ def _host():
             if getattr(calls, "built_for", None) != torch_release():
                 raise ImportError("it was built for another release of torch")
             calls.bind(*(C.cast(f, C.c_void_p).value for f in (L.bf16n_mmv, L.bf16n_gemv_max_tokens, L.bf16n_dequant)))
+            calls.bind_int4(*(C.cast(f, C.c_void_p).value for f in (L.bf16n_int4_workspace_bytes, L.bf16n_int4_mmv, L.bf16n_int4_route, L.bf16n_int4_mm_ids,
+                                                                    L.bf16n_moe_combine, L.bf16n_router_topk_grouped)))
         except ImportError as e:
             warnings.warn(f"bf16n: dense products are called without their native part ({e}): a call takes about 4 us longer; "
                           "build it with `python -m orin_qwen_lossless_amd.build`", RuntimeWarning, stacklevel=3)
@@ -1025,17 +1027,29 @@ def int4_mmv(x: torch.Tensor, w: Int4Weight, ids: torch.Tensor | None = None, ro
     """mmv for 4-bit weights with group scales: x [tokens, K] BF16 or FP32 -> [tokens, rows], or with expert ids [tokens, n_used]
     the rows of the matrices that they name, [tokens, n_used, rows_per_matrix], zeros where an id names none.  No weight is
     rounded: exact codes, FP32 sums, the scales applied to the sums."""
+    if ids is None and rows_per_matrix == 0 and out_dtype in (torch.float32, torch.bfloat16):
+        y = (_host_calls or _host()).int4_mmv(x, w, None, out_dtype is torch.bfloat16, INT4_FEW_TOKENS)
+        if y is not None:
+            return _lib.check(y) if type(y) is int else y
     return _int4_mmv("int4_mmv", x, w, None, ids, rows_per_matrix, out_dtype)
 
 
 def int4_mmv_glu2(x: torch.Tensor, gate: Int4Weight, up: Int4Weight, ids: torch.Tensor | None = None, rows_per_matrix: int = 0,
                   out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """silu(gate x) * (up x) in one launch for two matrices of one shape and group, dense or with expert ids (mmv_glu2)."""
+    if ids is None and rows_per_matrix == 0 and out_dtype in (torch.float32, torch.bfloat16):
+        y = (_host_calls or _host()).int4_mmv(x, gate, up, out_dtype is torch.bfloat16, INT4_FEW_TOKENS)
+        if y is not None:
+            return _lib.check(y) if type(y) is int else y
     return _int4_mmv("int4_mmv_glu2", x, gate, up, ids, rows_per_matrix, out_dtype)
 
 
 def int4_linear(x: torch.Tensor, w: Int4Weight, bias: torch.Tensor | None = None) -> torch.Tensor:
     """y = x W^T (+ bias) in BF16 for any number of tokens; the bias is added in FP32 before the one rounding."""
+    if bias is None and x.dtype is torch.bfloat16:
+        y = (_host_calls or _host()).int4_mmv(x, w, None, True, INT4_FEW_TOKENS)
+        if y is not None:
+            return _lib.check(y) if type(y) is int else y
     if x.dtype is not torch.bfloat16:
         raise ValueError("bf16n.int4_linear: x must be bf16")
     if x.dim() == 0 or x.shape[-1] != w.K:
@@ -1131,6 +1145,11 @@ def int4_moe_experts_rows(x: torch.Tensor, gate: Int4Weight, up: Int4Weight, dow
 def int4_moe_experts(x: torch.Tensor, gate: Int4Weight, up: Int4Weight, down: Int4Weight, topk_weights: torch.Tensor,
                      topk_ids: torch.Tensor, n_experts: int) -> torch.Tensor:
     """Routed experts of one MoE layer on 4-bit weights with group scales, BF16 out (moe_experts)."""
+    if topk_ids.dim() == 2:
+        batched = int4_moe_experts_batched(topk_ids.shape[0], topk_ids.shape[1], n_experts)
+        y = (_host_calls or _host()).int4_moe_experts(x, gate, up, down, topk_weights, topk_ids, n_experts, batched)
+        if y is not None:
+            return _lib.check(y) if type(y) is int else y
     return moe_combine(int4_moe_experts_rows(x, gate, up, down, topk_ids, n_experts), topk_weights, torch.bfloat16)
 
 
@@ -1141,6 +1160,11 @@ def router_topk_grouped(logits: torch.Tensor, k: int, bias: torch.Tensor | None 
     and experts in n_groups equal groups, of which the topk_groups first by their largest c ("max") or the sum of their two
     largest ("top2") stay open: (weights f32 [T, k], ids int32 [T, k]) of the k largest c, ties to the lower index.  weights: p of the
     chosen, over their sum if renorm, times scale.  Scores are held in 64 bits.  out as in router_topk."""
+    if out is None and scoring in ("softmax", "sigmoid") and group_score in ("max", "top2"):
+        r = (_host_calls or _host()).router_topk_grouped(logits, k, bias, n_groups, n_groups if topk_groups is None else topk_groups, scoring == "sigmoid",
+                                                         group_score == "top2", bool(renorm), scale)
+        if r is not None:
+            return _lib.check(r) if type(r) is int else r
     if not (logits.is_cuda and logits.dim() == 2 and logits.dtype == torch.float32 and logits.stride(1) == 1):
         raise ValueError("bf16n.router_topk_grouped: logits must be f32 [tokens, n_experts], contiguous along experts")
     if scoring not in ("softmax", "sigmoid") or group_score not in ("max", "top2"):
