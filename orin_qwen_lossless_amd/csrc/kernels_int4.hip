@@ -169,55 +169,67 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
             load(min(s0 + u, s1 - 1), u);
         }
 
-        // activations into LDS, in the operands' order, zeros behind the last column of the matrix, and their groups' sums
+        // Activations into LDS, in the operands' order, zeros behind the last column of the matrix, and their groups' sums: a
+        // wavefront takes 512 columns of a row at a time and has AHEAD such pieces on the way.  (One after the other cost a latency
+        // each: 11 tokens of 1453 x 2560, gated, @@ us.)
+        constexpr int AHEAD = XF32 ? 2 : 4;
         const int octs = (pitch - 8) / 8; // a multiple of 16: a row of 16 lanes has 128 columns of one activation row
+        const int per_row = (octs + 63) / 64, pieces = p.cols_per_pass * per_row;
         __syncthreads();
-        for (int i = threadIdx.x; i < p.cols_per_pass * octs; i += NW * 64) {
-            const int c = i / octs, o = i % octs;
-            const bool in = c < nc && o * 8 < K;
-            const char * src = p.x + x_of(c0 + (c < nc ? c : 0));
-            float sum = 0.f;
-            if constexpr (XF32) {
-                f32x4_t a = {}, b = {};
-                if (in) {
-                    a = *(const f32x4_t *) (src + o * 32);
-                    b = *(const f32x4_t *) (src + o * 32 + 16);
-                }
-                uint32_t parts[3][8];
+        for (int first = wave; first < pieces; first += NW * AHEAD) {
+            f32x4_t va[AHEAD], vb[AHEAD];
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float v = j < 4 ? a[j & 3] : b[j & 3];
-                    f32_parts(v, parts[0][j], parts[1][j], parts[2][j]);
-                    sum += v;
-                }
-#pragma unroll
-                for (int h = 0; h < 3; h++) {
-                    const uint32_t * e = parts[h];
-                    *(u32x4_t *) (xs + (c * 3 + h) * pitch + o * 8) =
-                        u32x4_t{e[0] | e[2] << 16, e[4] | e[6] << 16, e[1] | e[3] << 16, e[5] | e[7] << 16};
-                }
-            } else {
-                u32x4_t v = {};
-                if (in) {
-                    v = *(const u32x4_t *) (src + o * 16);
-                }
-                *(u32x4_t *) (xs + c * pitch + o * 8) = i4_order(v);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    sum += __uint_as_float(v[j] << 16) + __uint_as_float(v[j] & 0xFFFF0000u);
+            for (int k = 0; k < AHEAD; k++) {
+                const int i = first + k * NW, c = i / per_row, o = (i - c * per_row) * 64 + lane;
+                va[k] = vb[k] = f32x4_t{};
+                if (i < pieces && c < nc && o * 8 < K) {
+                    const char * src = p.x + x_of(c0 + c) + o * (XF32 ? 32 : 16);
+                    va[k] = *(const f32x4_t *) src;
+                    if (XF32) {
+                        vb[k] = *(const f32x4_t *) (src + 16);
+                    }
                 }
             }
-            sum = dpp_add<0xB1, 0xf>(sum); // over 4, 8 or 16 lanes: 32, 64 or 128 columns
-            sum = dpp_add<0x4E, 0xf>(sum);
-            if (GM < 2) {
-                sum = dpp_add<0x141, 0xf>(sum);
-            }
-            if (GM < 1) {
-                sum = dpp_add<0x140, 0xf>(sum);
-            }
-            constexpr int OG = 16 / NG;
-            if (o % OG == 0) {
-                xsum[o / OG * (NT * CPT) + c] = sum;
+#pragma unroll
+            for (int k = 0; k < AHEAD; k++) {
+                const int i = first + k * NW, c = i / per_row, o = (i - c * per_row) * 64 + lane;
+                float sum = 0.f;
+                if (i < pieces && o < octs) { // (rows of 16 lanes are in or out as a whole)
+                    if constexpr (XF32) {
+                        uint32_t parts[3][8];
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const float v = j < 4 ? va[k][j & 3] : vb[k][j & 3];
+                            f32_parts(v, parts[0][j], parts[1][j], parts[2][j]);
+                            sum += v;
+                        }
+#pragma unroll
+                        for (int h = 0; h < 3; h++) {
+                            const uint32_t * e = parts[h];
+                            *(u32x4_t *) (xs + (c * 3 + h) * pitch + o * 8) =
+                                u32x4_t{e[0] | e[2] << 16, e[4] | e[6] << 16, e[1] | e[3] << 16, e[5] | e[7] << 16};
+                        }
+                    } else {
+                        const u32x4_t v = __builtin_bit_cast(u32x4_t, va[k]);
+                        *(u32x4_t *) (xs + c * pitch + o * 8) = i4_order(v);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            sum += __uint_as_float(v[j] << 16) + __uint_as_float(v[j] & 0xFFFF0000u);
+                        }
+                    }
+                }
+                sum = dpp_add<0xB1, 0xf>(sum); // over 4, 8 or 16 lanes: 32, 64 or 128 columns
+                sum = dpp_add<0x4E, 0xf>(sum);
+                if (GM < 2) {
+                    sum = dpp_add<0x141, 0xf>(sum);
+                }
+                if (GM < 1) {
+                    sum = dpp_add<0x140, 0xf>(sum);
+                }
+                constexpr int OG = 16 / NG;
+                if (i < pieces && o < octs && o % OG == 0) {
+                    xsum[o / OG * (NT * CPT) + c] = sum;
+                }
             }
         }
         if (threadIdx.x < nc) {
