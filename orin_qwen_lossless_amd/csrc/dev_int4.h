@@ -19,9 +19,12 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
-// loads of four scales and of four zero points, wherever a row begins
+// loads of two or four scales and of two, four or eight zero points, wherever a row begins
 typedef uint64_t __attribute__((aligned(2), may_alias)) u64_at_2;
+typedef uint32_t __attribute__((aligned(2), may_alias)) u32_at_2;
+typedef uint64_t __attribute__((aligned(1), may_alias)) u64_at_1;
 typedef uint32_t __attribute__((aligned(1), may_alias)) u32_at_1;
+typedef uint16_t __attribute__((aligned(1), may_alias)) u16_at_1;
 
 struct i4_matrix {
     const uint8_t * codes;   // [rows, K / 2], 16-byte aligned

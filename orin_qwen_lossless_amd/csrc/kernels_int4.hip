@@ -31,6 +31,45 @@ constexpr int I4_STEP = 128; // columns that a wavefront takes at a time: 32 to 
 // different banks
 __host__ __device__ inline int i4_pitch(int K) { return (K + I4_STEP - 1) / I4_STEP * I4_STEP + 8; }
 
+// The columns of a launch's block, shared by the two kernels for few columns: which matrix, where a column's activations and results are.
+struct i4_columns {
+    const i4_launch & p;
+    int64_t matrix = 0, x_one = 0, y_one = 0;
+    int begin = 0, end;
+    bool named = true; // false: the ids name no matrix
+    __device__ i4_columns(const i4_launch & p) : p(p), end(p.ncols) {
+        if (p.ids) {
+            const int t = blockIdx.y / p.n_used, i = blockIdx.y % p.n_used;
+            const char * at = p.ids + t * p.ids_s1 + i * p.ids_s0;
+            matrix = p.ids_i64 ? *(const int64_t *) at : *(const int32_t *) at;
+            named = matrix >= 0 && matrix < p.n_matrices;
+            x_one = t * p.x_tok + (i % p.x_per_slot) * p.x_slot;
+            y_one = t * p.y_tok + i * p.y_slot;
+            end = 1;
+        } else if (p.bounds) {
+            matrix = blockIdx.y;
+            begin = p.bounds[matrix];
+            end = p.bounds[matrix + 1];
+            named = matrix < p.n_matrices; // behind the last one: pairs that name none
+        }
+    }
+    __device__ int64_t y_of(int c) const { return p.pairs ? p.pairs[c] * p.y_slot : y_one + c * p.y_tok; }
+    __device__ int64_t x_of(int c) const {
+        if (p.pairs) {
+            const int pair = p.pairs[c];
+            return p.x_per_slot > 1 ? pair * p.x_slot : pair / p.n_used * p.x_tok;
+        }
+        return x_one + c * p.x_tok;
+    }
+    __device__ void zero() const { // no such matrix: rows of zeros
+        for (int c = begin + blockIdx.z; c < end; c += gridDim.z) {
+            for (int r = blockIdx.x * blockDim.x + threadIdx.x; r < p.nrows; r += gridDim.x * blockDim.x) {
+                store_y(p.y + y_of(c), p.y_bf16, r, 0.f);
+            }
+        }
+    }
+};
+
 // Few columns.  One wavefront takes 16 rows of the matrix (of each of the two where they are gated) and 256 columns of it at
 // a time: a lane's 32 bytes are 64 codes of row lane % 16 (four lanes have 128 bytes of a row, a whole line: 64 of them at a time
 // took 72 us where the lines whole take @@), turned into eight operands of v_mfma_f32_16x16x32_bf16 whose other
@@ -57,40 +96,13 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
     int64_t * const y_off = (int64_t *) (xsum + steps * NG * NT * CPT); // [NT * CPT]
     float * const red = (float *) (y_off + NT * CPT);
 
-    // which matrix, and its columns
-    int64_t matrix = 0, x_one = 0, y_one = 0;
-    int c_begin = 0, c_end = p.ncols;
-    bool named = true;
-    if (p.ids) {
-        const int t = blockIdx.y / p.n_used, i = blockIdx.y % p.n_used;
-        const char * at = p.ids + t * p.ids_s1 + i * p.ids_s0;
-        matrix = p.ids_i64 ? *(const int64_t *) at : *(const int32_t *) at;
-        named = matrix >= 0 && matrix < p.n_matrices;
-        x_one = t * p.x_tok + (i % p.x_per_slot) * p.x_slot;
-        y_one = t * p.y_tok + i * p.y_slot;
-        c_end = 1;
-    } else if (p.bounds) {
-        matrix = blockIdx.y;
-        c_begin = p.bounds[matrix];
-        c_end = p.bounds[matrix + 1];
-        named = matrix < p.n_matrices; // behind the last one: pairs that name none
-    }
-    const auto y_of = [&](int c) -> int64_t { return p.pairs ? p.pairs[c] * p.y_slot : y_one + c * p.y_tok; };
-    const auto x_of = [&](int c) -> int64_t {
-        if (p.pairs) {
-            const int pair = p.pairs[c];
-            return p.x_per_slot > 1 ? pair * p.x_slot : pair / p.n_used * p.x_tok;
-        }
-        return x_one + c * p.x_tok;
-    };
-    if (!named) { // no such matrix: a row of zeros
-        for (int c = c_begin + blockIdx.z; c < c_end; c += gridDim.z) {
-            for (int r = blockIdx.x * blockDim.x + threadIdx.x; r < p.nrows; r += gridDim.x * blockDim.x) {
-                store_y(p.y + y_of(c), p.y_bf16, r, 0.f);
-            }
-        }
+    const i4_columns cols(p);
+    if (!cols.named) {
+        cols.zero();
         return;
     }
+    const int64_t matrix = cols.matrix;
+    const int c_begin = cols.begin, c_end = cols.end;
 
     const int row_groups = NW / p.ksplit, kp = wave % p.ksplit;
     const int pairs = (steps + 1) / 2, s0 = pairs * kp / p.ksplit, s1 = pairs * (kp + 1) / p.ksplit;
@@ -183,7 +195,7 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
                 const int i = first + k * NW, c = i / per_row, o = (i - c * per_row) * 64 + lane;
                 va[k] = vb[k] = f32x4_t{};
                 if (i < pieces && c < nc && o * 8 < K) {
-                    const char * src = p.x + x_of(c0 + c) + o * (XF32 ? 32 : 16);
+                    const char * src = p.x + cols.x_of(c0 + c) + o * (XF32 ? 32 : 16);
                     va[k] = *(const f32x4_t *) src;
                     if (XF32) {
                         vb[k] = *(const f32x4_t *) (src + 16);
@@ -233,7 +245,7 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
             }
         }
         if (threadIdx.x < nc) {
-            y_off[threadIdx.x] = y_of(c0 + threadIdx.x);
+            y_off[threadIdx.x] = cols.y_of(c0 + threadIdx.x);
         }
         __syncthreads();
 
@@ -387,6 +399,195 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
                             }
                         }
                     }
+                }
+            }
+        }
+    }
+}
+
+// Few columns of a matrix whose rows are few as well: nothing is shared through LDS but the sums of the parts of K.  A
+// wavefront loads its codes, scales and activations, these as the operand's lanes hold them, at once, one latency in
+// all; the groups' sums of the activations come from products with ones.
+// 512 x 2048, one token: @@ us in a graph, @@ with the activations through LDS.  Bound by that latency.
+template <int NT, int GM, bool GLU, bool XF32, bool ZEROS>
+__global__ void __launch_bounds__(512, 2) k_i4_small(const i4_launch p) {
+    constexpr int NW = 8, NM = GLU ? 2 : 1, NG = GM == 0 ? 1 : GM == 1 ? 2 : 4, CPT = XF32 ? 4 : 16, NA = XF32 ? 1 : 4;
+    __shared__ float red[NW * NM * NT * NA * 64];
+    const int lane = threadIdx.x & 63, m16 = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const i4_columns cols(p);
+    if (!cols.named) {
+        cols.zero();
+        return;
+    }
+    const int K = p.K, steps = (K + I4_STEP - 1) / I4_STEP, n_pairs = (steps + 1) / 2, kp = wave % p.ksplit;
+    const int row_groups = NW / p.ksplit, r0 = (blockIdx.x * row_groups + wave / p.ksplit) * 16;
+    const int first = min(r0, p.nrows - 1), row = min(m16, p.nrows - 1 - first); // rows beyond the matrix repeat its last: dropped
+    const int64_t base = cols.matrix * p.nrows + first;
+    const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, u32x4_t{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
+    const f32x4_t none = {};
+    for (int c0 = cols.begin + blockIdx.z * p.cols_per_pass; c0 < cols.end; c0 += gridDim.z * p.cols_per_pass) {
+        const int nc = min(cols.end - c0, p.cols_per_pass);
+        const char * x_at[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            x_at[t] = p.x + cols.x_of(c0 + min(t * CPT + (XF32 ? m16 >> 2 : m16), nc - 1));
+        }
+        float acc[NM * NT][NA];
+#pragma unroll
+        for (int i = 0; i < NM * NT; i++) {
+#pragma unroll
+            for (int e = 0; e < NA; e++) {
+                acc[i][e] = 0.f;
+            }
+        }
+        for (int s = kp; s < n_pairs; s += p.ksplit) {
+            u32x4_t code[NM][2];
+            uint64_t sc[NM][NG == 4 ? 2 : 1], ze[NM]; // scales, 16 bits each, and zero points of the 2 NG groups
+            const int g0 = s * 2 * I4_STEP >> p.group_log2;
+            const bool whole = p.group_log2 <= 7 && g0 + 2 * NG <= p.n_groups;
+            const int at = s * 2 * I4_STEP + q * 64; // lanes behind the last column read columns before it, against activations of zero
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                const i4_matrix & w = GLU && m ? p.up : p.w;
+                const uint8_t * from = w.codes + base * (K / 2) + row * (K / 2);
+                code[m][0] = *(const u32x4_t *) (from + (at < K ? at : 0) / 2);
+                code[m][1] = *(const u32x4_t *) (from + (at + 32 < K ? at + 32 : 0) / 2);
+                const uint16_t * sat = w.scales + base * p.n_groups + row * p.n_groups;
+                const uint8_t * zat = w.zeros + base * p.n_groups + row * p.n_groups;
+                ze[m] = 0;
+                if (whole) {
+                    if (NG == 1) {
+                        sc[m][0] = *(const u32_at_2 *) (sat + g0);
+                    } else {
+                        sc[m][0] = *(const u64_at_2 *) (sat + g0);
+                        sc[m][NG == 4 ? 1 : 0] = *(const u64_at_2 *) (sat + g0 + (NG == 4 ? 4 : 0));
+                    }
+                    if (ZEROS) {
+                        ze[m] = NG == 1 ? *(const u16_at_1 *) (zat + g0) : NG == 2 ? *(const u32_at_1 *) (zat + g0) : *(const u64_at_1 *) (zat + g0);
+                    }
+                } else {
+                    sc[m][0] = sc[m][NG == 4 ? 1 : 0] = 0;
+#pragma unroll
+                    for (int g = 0; g < 2 * NG; g++) {
+                        const int gi = min((s * 2 * I4_STEP + g * (I4_STEP / NG)) >> p.group_log2, p.n_groups - 1);
+                        sc[m][g / 4] |= (uint64_t) sat[gi] << g % 4 * 16;
+                        ze[m] |= ZEROS ? (uint64_t) zat[gi] << g * 8 : 0;
+                    }
+                }
+            }
+            bf16x8_t xf[NT][8];
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int h = i / 4, j = i % 4;
+                    const int col = (s * 2 + h) * I4_STEP + (GM == 0 ? (q & 1) * 64 + (q >> 1) * 32 + j * 8 : j * 32 + q * 8);
+                    u32x4_t v = {};
+                    if constexpr (XF32) {
+                        f32x4_t a = {}, b = {};
+                        if (col < K) {
+                            a = *(const f32x4_t *) (x_at[t] + col * 4);
+                            b = *(const f32x4_t *) (x_at[t] + col * 4 + 16);
+                        }
+                        uint32_t e[8];
+#pragma unroll
+                        for (int l = 0; l < 8; l++) { // this lane's part of the three
+                            uint32_t f0, f1, f2;
+                            f32_parts(l < 4 ? a[l & 3] : b[l & 3], f0, f1, f2);
+                            e[l] = (m16 & 3) == 0 ? f0 : (m16 & 3) == 1 ? f1 : f2;
+                        }
+                        v = u32x4_t{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
+                    } else if (col < K) {
+                        v = *(const u32x4_t *) (x_at[t] + col * 2);
+                    }
+                    xf[t][i] = __builtin_bit_cast(bf16x8_t, v);
+                }
+            }
+            u32x4_t d[2][NM];
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) { // as in k_i4_few
+                    const auto r = __builtin_amdgcn_permlane32_swap(code[m][0][j], code[m][1][j], false, false);
+                    d[0][m][j] = r[0];
+                    d[1][m][j] = r[1];
+                }
+                if (GM) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const u32x4_t e = i4_transpose(d[h][m]);
+                        d[h][m] = u32x4_t{e[0], e[2], e[1], e[3]};
+                    }
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < 2 * NG; g++) {
+                f32x4_t part[NM * NT], xsum[NT];
+                constexpr int J = 4 / NG;
+#pragma unroll
+                for (int j = 0; j < J; j++) {
+                    const int i = g * J + j;
+                    bf16x8_t wf[NM];
+#pragma unroll
+                    for (int m = 0; m < NM; m++) {
+                        wf[m] = i4_operand_in_order(d[i / 4][m][i % 4]);
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        xsum[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[t][i], ones, j ? xsum[t] : none, 0, 0, 0);
+#pragma unroll
+                        for (int m = 0; m < NM; m++) {
+                            part[m * NT + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[t][i], wf[m], j ? part[m * NT + t] : none, 0, 0, 0);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int m = 0; m < NM; m++) {
+                    const float sv = i4_scale((uint32_t) (sc[m][g / 4] >> g % 4 * 16) & 0xFFFFu, (GLU && m ? p.up : p.w).f16 ? ~0u : 0u);
+                    const float zv = ZEROS ? (float) ((uint32_t) (ze[m] >> g * 8) & 0xFFu) : 8.f;
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        const f32x4_t & a = part[m * NT + t], & b = xsum[t];
+#pragma unroll
+                        for (int e = 0; e < NA; e++) {
+                            const float sum = XF32 ? a[0] + (a[1] + a[2]) : a[e], x = XF32 ? b[0] + (b[1] + b[2]) : b[e];
+                            acc[m * NT + t][e] = fmaf(sv, fmaf(-zv, x, sum), acc[m * NT + t][e]);
+                        }
+                    }
+                }
+            }
+        }
+        if (p.ksplit > 1) {
+            __syncthreads(); // (the last pass's sums have been read)
+#pragma unroll
+            for (int i = 0; i < NM * NT; i++) {
+#pragma unroll
+                for (int e = 0; e < NA; e++) {
+                    red[((wave * NM * NT + i) * NA + e) * 64 + lane] = acc[i][e];
+                }
+            }
+            __syncthreads();
+            if (kp != 0) {
+                continue;
+            }
+            for (int k = 1; k < p.ksplit; k++) {
+#pragma unroll
+                for (int i = 0; i < NM * NT; i++) {
+#pragma unroll
+                    for (int e = 0; e < NA; e++) {
+                        acc[i][e] += red[(((wave + k) * NM * NT + i) * NA + e) * 64 + lane];
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+#pragma unroll
+            for (int e = 0; e < NA; e++) {
+                const int c = t * CPT + q * NA + e;
+                if (c < nc && r0 + m16 < p.nrows) {
+                    store_y(p.y + cols.y_of(c0 + c), p.y_bf16, r0 + m16, GLU ? silu(acc[t][e]) * acc[(GLU ? NT : 0) + t][e] : acc[t][e]);
                 }
             }
         }
@@ -935,7 +1136,7 @@ size_t few_lds(int K, int cols, bool f32, int nt, int nm, int groups_per_step, i
 
 constexpr size_t I4_FEW_LDS = 160 * 1024 - 1024;
 
-struct few_plan { int nt, grid_y, grid_z, cus; hipStream_t stream; bool raise_limits; };
+struct few_plan { int nt, grid_y, grid_z, cus; hipStream_t stream; bool raise_limits, small; };
 
 template <int NT, int GM, bool GLU, bool XF32, bool ZEROS>
 void launch_few(const i4_launch & p, const few_plan & f) {
@@ -947,6 +1148,10 @@ void launch_few(const i4_launch & p, const few_plan & f) {
     }
     const int block_rows = NW / p.ksplit * 16;
     const int n_blocks = (p.nrows + block_rows - 1) / block_rows;
+    if (f.small) {
+        k_i4_small<NT, GM, GLU, XF32, ZEROS><<<dim3(n_blocks, f.grid_y, f.grid_z), NW * 64, 0, f.stream>>>(p);
+        return;
+    }
     const size_t lds = few_lds(p.K, p.cols_per_pass, XF32, NT, NM, GM == 0 ? 1 : GM == 1 ? 2 : 4, p.ksplit);
     // one matrix: as many blocks as the device holds, each with its share of the rows; more matrices: a block to a piece of rows
     const int room = f.cus * (int) std::min<size_t>(2, LDS_BYTES / lds);
@@ -971,7 +1176,7 @@ void pick_few(const i4_launch & p, bool glu, bool f32, int gm, bool zeros, const
 void init_few() {
     for (int i = 0; i < 48; i++) { // every instance
         const i4_launch none = {};
-        const few_plan f = {(i & 1) + 1, 0, 0, 0, nullptr, true};
+        const few_plan f = {(i & 1) + 1, 0, 0, 0, nullptr, true, false};
         if ((i & 24) != 24) {
             pick_few(none, i & 2, i & 4, i >> 3 & 3, i & 32, f);
         }
@@ -1058,7 +1263,10 @@ void run_few(i4_launch & p, bool glu, bool f32, bool zeros, int max_cols, int64_
     }
     p.ksplit = ksplit;
     const int passes = p.bounds || p.ids ? 1 : std::min(65535, (max_cols + p.cols_per_pass - 1) / p.cols_per_pass);
-    pick_few(p, glu, f32, gm, zeros, {nt, grid_y, passes, cus, stream, false});
+    // the kernel without activations in LDS: up to two tiles of rows for a CU (one with FP32 activations, whose lanes part them
+    // themselves).  us, with it / without, BF16, 16 tokens: 5120 x 2048 @@, 10240 x 2048 15.6 / 11.4; FP32, three: 8192 x 2048 14.4 / 8.9
+    const bool small = tiles <= (f32 ? 1 : 2) * cus;
+    pick_few(p, glu, f32, gm, zeros, {nt, grid_y, passes, cus, stream, false, small});
 }
 
 } // namespace
