@@ -1153,9 +1153,10 @@ void launch_few(const i4_launch & p, const few_plan & f) {
         return;
     }
     const size_t lds = few_lds(p.K, p.cols_per_pass, XF32, NT, NM, GM == 0 ? 1 : GM == 1 ? 2 : 4, p.ksplit);
-    // one matrix: as many blocks as the device holds, each with its share of the rows; more matrices: a block to a piece of rows
-    const int room = f.cus * (int) std::min<size_t>(2, LDS_BYTES / lds);
-    const int rounds = f.grid_y > 1 ? 1 : (n_blocks + room - 1) / room;
+    // one matrix: as many blocks as the device holds, each with its share of the rows; more matrices: a block to a piece of rows, or to as
+    // many as give a wavefront eight pairs of steps (77 tokens, 2048 x 512 of 256 experts: 66 us with two, 45 with eight)
+    const int room = f.cus * (int) std::min<size_t>(2, LDS_BYTES / lds), steps = (p.K + I4_STEP - 1) / I4_STEP;
+    const int rounds = f.grid_y == 1 ? (n_blocks + room - 1) / room : std::max(1, std::min<int>(16 * p.ksplit / steps, (int64_t) n_blocks * f.grid_y / (4 * f.cus)));
     kernel<<<dim3((n_blocks + rounds - 1) / rounds, f.grid_y, f.grid_z), NW * 64, lds, f.stream>>>(p);
 }
 
@@ -1286,7 +1287,13 @@ int64_t int4_workspace_bytes(const bf16n_int4_weight & w, int64_t x_rows, int64_
 
 void launch_int4_mmv(const bf16n_int4_weight & w, const bf16n_int4_weight * up, const bf16n_mmv_args & a, bool ids_i64, void * workspace,
                      uint64_t workspace_bytes, int cus, hipStream_t stream) {
-    if (!a.ids && a.x_bf16 && a.ncols > 32 && a.x_tok >= 0 && a.ncols * a.x_tok < (int64_t) 1 << 32 && (int64_t) workspace_bytes >= int4_workspace_bytes(w, a.ncols, 0, 0)) {
+    // Many columns where one pass of 32 is not all and the matrix has rows enough: its kernel takes 1.1 us a step however few its
+    // blocks are (one and a half to a CU add nothing), a pass of 32 columns over 16 rows costs 1 / 800 of that on a whole device.
+    // us, many / few: 5120 x 2048, 64 tokens 25.0 / 18.8, 200 25.9 / 50; 233 x 5440, 125 50 / 9.4; 512 x 2048, 512 25.1 / 15.3, 2048 26.6 / 49;
+    // 20000 x 2048, 64 25.9 / 36.9
+    const int64_t units = (a.nrows + 15) / 16 * ((a.ncols + 31) / 32), blocks = (a.nrows + 127) / 128 * ((a.ncols + 63) / 64);
+    const int64_t rounds = std::max<int64_t>(1, 2 * blocks / (3 * cus)), steps = (w.K + I4_STEP - 1) / I4_STEP;
+    if (!a.ids && a.x_bf16 && a.ncols > 32 && units > 800 * rounds + 2200 / steps && a.x_tok >= 0 && a.ncols * a.x_tok < (int64_t) 1 << 32 && (int64_t) workspace_bytes >= int4_workspace_bytes(w, a.ncols, 0, 0)) {
         i4_many p = {};
         p.x = (const char *) a.x; p.x_row = a.x_tok;
         p.y = (char *) a.y; p.y_row = a.y_tok; p.y_bf16 = a.y_bf16 != 0;
@@ -1326,7 +1333,8 @@ void launch_int4_mm_ids(const bf16n_int4_weight & w, const bf16n_int4_weight * u
                         int cus, hipStream_t stream) {
     const int64_t x_rows = per_slot ? (int64_t) n_tok * n_used : n_tok;
     const int64_t n_pairs = (int64_t) n_tok * n_used;
-    if (n_pairs > 16 * (int64_t) n_matrices &&  x_row >= 0 && x_rows * x_row < (int64_t) 1 << 31 && (int64_t) workspace_bytes >= int4_workspace_bytes(w, x_rows, n_pairs, n_matrices)) {
+    // many columns from 12 pairs to a matrix on.  256 experts, top-8, us with them / without: 300 tokens 142 / 131, 400 146 / 151, 512 153 / 176
+    if (n_pairs > 12 * (int64_t) n_matrices &&  x_row >= 0 && x_rows * x_row < (int64_t) 1 << 31 && (int64_t) workspace_bytes >= int4_workspace_bytes(w, x_rows, n_pairs, n_matrices)) {
         i4_many p = {};
         p.x = (const char *) x; p.x_row = x_row * 2;
         p.y = (char *) y; p.y_row = y_row * (y_bf16 ? 2 : 4); p.y_bf16 = y_bf16;

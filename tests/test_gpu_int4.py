@@ -21,7 +21,7 @@ def acts(tokens, K, seed, dtype=torch.bfloat16):
 @pytest.mark.parametrize("rows,K,tokens,group", [
     (1, 32, 1, 32), (15, 64, 2, 64), (17, 96, 3, 32), (33, 160, 5, 128), (256, 2048, 1, 128), (512, 2048, 16, 128), (300, 2048, 17, 64),
     (129, 2080, 33, 32), (70, 4096, 7, 256), (64, 512, 64, 512), (31, 1024, 100, 128), (40, 9600, 4, 4096), (20, 16384, 6, 64), (5000, 256, 1, 64),
-    (2500, 640, 20, 128)])
+    (2500, 640, 20, 128), (9000, 160, 3, 32), (16500, 96, 20, 64), (8700, 320, 40, 128), (4200, 2048, 4, 256), (70, 4160, 200, 64)])
 @pytest.mark.parametrize("zeros,f16", [(True, False), (False, True)])
 def test_dense(ops, rows, K, tokens, group, zeros, f16):
     w, dw = weight(ops, rows, K, group, rows + K, zeros, f16)
@@ -35,7 +35,8 @@ def test_dense(ops, rows, K, tokens, group, zeros, f16):
         X.check(ops.int4_mmv_glu2(x.cuda(), dw, dw2), h, hb, dtype)
 
 
-@pytest.mark.parametrize("rows,K,tokens,group", [(5, 64, 1, 32), (130, 2048, 9, 128), (257, 1056, 130, 64), (512, 2048, 517, 128), (1000, 512, 300, 32)])
+@pytest.mark.parametrize("rows,K,tokens,group", [(5, 64, 1, 32), (130, 2048, 9, 128), (257, 1056, 130, 64), (512, 2048, 517, 128), (1000, 512, 300, 32),
+                                                 (4100, 1056, 200, 64), (2050, 160, 3000, 128), (8300, 416, 70, 32), (1030, 4128, 1100, 32), (640, 2080, 4100, 512)])
 def test_linear(ops, rows, K, tokens, group):
     w, dw = weight(ops, rows, K, group, 3)
     x = acts(tokens, K, 4)
