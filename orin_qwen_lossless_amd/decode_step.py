@@ -30,7 +30,11 @@ SHAPES = {"qkv": (QKV_ROWS, K_MODEL, 1), "o": (K_MODEL, ATT, 1), "router": (E, K
 
 def encode_policy(ops, w_dev: torch.Tensor, n_matrices: int = 1, mode: str = "hybrid"):
     """[rows, K] BF16 device tensor -> (Weight in the layout of the mi355x policy, compressed bytes).  mode: the policy's
-    (hybrid, huffman or nibble: the 4-bit code for everything)."""
+    (hybrid, huffman or nibble: the 4-bit code for everything), or "int4": 4-bit weights with group scales, which are not
+    lossless (Int4Weight)."""
+    if mode == "int4":
+        w = ops.int4_quantize(w_dev)
+        return w, w.nbytes
     rows, k = w_dev.shape
     fmt, R, cm, _, w64 = ops.choose(rows // n_matrices, k, n_matrices, engine="mi355x", mode=mode, expert=n_matrices > 1)
     bits = w_dev.cpu().view(torch.int16).numpy().view(np.uint16)
@@ -42,7 +46,8 @@ def encode_policy(ops, w_dev: torch.Tensor, n_matrices: int = 1, mode: str = "hy
 def make_layer_sets(ops, gen_weights, n_sets: int, keep_bf16: bool, expert_mode: str = "hybrid"):
     """n_sets weight sets of one layer.  gen_weights(rows, K) -> BF16 device tensor.  Returns (encoded sets, BF16 sets or
     None, compressed bytes by matrix name of one set).  expert_mode "nibble": the expert stacks in the 4-bit code (7 %
-    more bytes than the policy's tiles, no decode chain: the form for decode at one or two tokens)."""
+    more bytes than the policy's tiles, no decode chain: the form for decode at one or two tokens).  "int4": 4-bit weights with
+    group scales (0.52 byte a weight, not lossless)."""
     enc_sets, raw_sets, nbytes = [], [] if keep_bf16 else None, {}
     for _ in range(n_sets):
         enc, raw = {}, {}
@@ -93,6 +98,9 @@ class Bf16nStep:
         """(ys [T, 9, K] FP32 per-slot outputs, wts [T, 9], ids [T, 9]).  logits: the router's, if the caller has them."""
         ops, routes = self.ops, None
         logits = ops.mmv(x2, w["router"]) if logits is None else logits
+        if isinstance(w["gate"], ops.Int4Weight):
+            wts, ids = ops.router_topk(logits, TOPK, out=self.routing)
+            return ops.int4_moe_experts_rows(x2, w["gate"], w["up"], w["down"], ids, EA), wts, ids
         batched = ops.moe_experts_batched(x2.shape[0], TOPK + 1, w["gate"], w["up"], w["down"], EA)
         if not batched and ops.topk_in_gemv_supported(w["gate"], w["up"], E, TOPK):
             # the gate / up GEMV selects the experts itself: no top-k launch
@@ -120,6 +128,8 @@ class Bf16nStep:
         x1 = self.ops.add_rmsnorm(h)
         for i in range(self.n_layers):
             x1, h = self.layer(self.sets[i % len(self.sets)], h, x1)
+        if isinstance(self.head, self.ops.Int4Weight):  # a draft copy of the output projection
+            return self.ops.int4_linear(x1, self.head)
         return self.ops.linear(x1, self.head) if self.head is not None else x1
 
 

@@ -9,7 +9,8 @@ registered from Python over the C ABI, with the reference's fake (meta) implemen
     y = torch.ops.bf16n.mmv(x, plane.cuda(), aux.cuda(), meta, None, 0, False)
 
 `meta` is the reference's list; bit 2 of meta[4] (flags) marks the wave64 layout.  The int4 / int2 baseline ops of the
-reference extension are not part of the BF16N path and are not registered.  encode_auto is this build's addition."""
+reference extension are not part of the BF16N path and are not registered.  This build's additions: encode_auto, and for 4-bit weights
+with group scales (ops.Int4Weight: codes, scales, zeros, group) int4_linear and int4_moe_experts, with router_topk_grouped."""
 from __future__ import annotations
 
 import torch
@@ -30,6 +31,11 @@ _lib.define("moe_mm_ids(Tensor x, Tensor topk_ids, Tensor plane, Tensor aux, int
 _lib.define("moe_combine(Tensor ys, Tensor topk_weights, bool out_bf16) -> Tensor")
 _lib.define("swiglu(Tensor g, Tensor u) -> Tensor")
 _lib.define("router_topk(Tensor logits, int k, bool renorm) -> (Tensor, Tensor)")
+_lib.define("router_topk_grouped(Tensor logits, int k, Tensor? bias, int n_groups, int topk_groups, str scoring, str group_score, "
+            "bool renorm, float scale) -> (Tensor, Tensor)")
+_lib.define("int4_linear(Tensor x, Tensor codes, Tensor scales, Tensor? zeros, int group, Tensor? bias) -> Tensor")
+_lib.define("int4_moe_experts(Tensor x, Tensor[] gate, Tensor[] up, Tensor[] down, int group, Tensor topk_weights, Tensor topk_ids, "
+            "int n_experts) -> Tensor")
 
 
 def meta_of(aux: torch.Tensor) -> list[int]:
@@ -110,11 +116,31 @@ def _router_topk(logits, k, renorm):
     return ops.router_topk(logits, k, renorm)
 
 
+def _router_topk_grouped(logits, k, bias, n_groups, topk_groups, scoring, group_score, renorm, scale):
+    return ops.router_topk_grouped(logits, k, bias, n_groups, topk_groups, scoring, group_score, renorm, scale)
+
+
+def _int4(tensors, group: int) -> ops.Int4Weight:
+    """[codes, scales] or [codes, scales, zeros]"""
+    if len(tensors) not in (2, 3):
+        raise ValueError("bf16n: a 4-bit weight is [codes, scales] or [codes, scales, zeros]")
+    return ops.Int4Weight(tensors[0], tensors[1], tensors[2] if len(tensors) == 3 else None, int(group))
+
+
+def _int4_linear(x, codes, scales, zeros, group, bias):
+    return ops.int4_linear(x, ops.Int4Weight(codes, scales, zeros, int(group)), bias)
+
+
+def _int4_moe_experts(x, gate, up, down, group, topk_weights, topk_ids, n_experts):
+    return ops.int4_moe_experts(x, _int4(gate, group), _int4(up, group), _int4(down, group), topk_weights, topk_ids, n_experts)
+
+
 _lib.impl("init", _init, "CompositeExplicitAutograd")
 _lib.impl("encode", _encode_cpu, "CPU")
 _lib.impl("encode_auto", _encode_auto_cpu, "CPU")
 for _name, _fn in (("dequant", _dequant), ("mmv", _mmv), ("mmv_glu", _mmv_glu), ("linear", _linear), ("get_rows", _get_rows),
-                   ("moe_mm_ids", _moe_mm_ids), ("moe_combine", _moe_combine), ("swiglu", _swiglu), ("router_topk", _router_topk)):
+                   ("moe_mm_ids", _moe_mm_ids), ("moe_combine", _moe_combine), ("swiglu", _swiglu), ("router_topk", _router_topk),
+                   ("router_topk_grouped", _router_topk_grouped), ("int4_linear", _int4_linear), ("int4_moe_experts", _int4_moe_experts)):
     _lib.impl(_name, _fn, "CUDA")
 
 
@@ -183,3 +209,18 @@ def _swiglu_fake(g, u):
 @torch.library.register_fake("bf16n::router_topk")
 def _router_topk_fake(logits, k, renorm):
     return logits.new_empty((logits.shape[0], k), dtype=torch.float32), logits.new_empty((logits.shape[0], k), dtype=torch.int32)
+
+
+@torch.library.register_fake("bf16n::router_topk_grouped")
+def _router_topk_grouped_fake(logits, k, bias, n_groups, topk_groups, scoring, group_score, renorm, scale):
+    return logits.new_empty((logits.shape[0], k), dtype=torch.float32), logits.new_empty((logits.shape[0], k), dtype=torch.int32)
+
+
+@torch.library.register_fake("bf16n::int4_linear")
+def _int4_linear_fake(x, codes, scales, zeros, group, bias):
+    return x.new_empty((*x.shape[:-1], codes.shape[0]))
+
+
+@torch.library.register_fake("bf16n::int4_moe_experts")
+def _int4_moe_experts_fake(x, gate, up, down, group, topk_weights, topk_ids, n_experts):
+    return x.new_empty((x.shape[0], down[0].shape[0] // n_experts), dtype=torch.bfloat16)

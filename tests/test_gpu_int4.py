@@ -227,6 +227,142 @@ def test_other_stream(ops):
     X.check(got, y, b)
 
 
+def test_with_and_without_the_native_calls(ops, monkeypatch):
+    """The calls from Python in native code and the general way launch the same kernels; both refuse the same."""
+    E, mid, K, group = 8, 64, 128, 32
+    w, up, down = (weight(ops, E * r, c, group, 70 + i)[1] for i, (r, c) in enumerate(((mid, K), (mid, K), (K, mid))))
+    x, logits = acts(30, K, 73).cuda(), torch.randn((30, E), generator=torch.Generator().manual_seed(74)).cuda()
+    wts, ids = ops.router_topk_grouped(logits, 2)
+
+    def results():
+        out = []
+        for a in (x, x[:3], x[:, :].float()[:5]):
+            out += [ops.int4_mmv(a, w), ops.int4_mmv(a, w, out_dtype=torch.bfloat16), ops.int4_mmv_glu2(a, w, up)]
+        out += [ops.int4_linear(x, w), ops.int4_linear(torch.cat([x] * 40), weight(ops, 4000, K, group, 75)[1])]
+        for t in (1, 3, 30):
+            for i, v in ((ids, wts), (ids.long(), wts.bfloat16())):
+                out.append(ops.int4_moe_experts(x[:t], w, up, down, v[:t].contiguous(), i[:t], E))
+        for kw in ({}, {"bias": logits[0].contiguous(), "n_groups": 4, "topk_groups": 2, "scoring": "sigmoid", "group_score": "top2", "renorm": False, "scale": 2.0}):
+            out += ops.router_topk_grouped(logits, 3, **kw)
+        return out
+
+    native = results()
+    with pytest.raises(ValueError):
+        ops.router_topk_grouped(logits, 3, n_groups=3)
+    monkeypatch.setattr(ops, "_host_calls", ops._NoNativeCalls)
+    for a, b in zip(native, results(), strict=True):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+    with pytest.raises(ValueError):
+        ops.router_topk_grouped(logits, 3, n_groups=3)
+
+
+def test_registered_operators(ops):
+    from orin_qwen_lossless_amd import torch_ops  # noqa: F401
+
+    B = torch.ops.bf16n
+    w, up, down = (weight(ops, 4 * r, c, 64, 80 + i)[1] for i, (r, c) in enumerate(((64, 128), (64, 128), (128, 64))))
+    x, logits = acts(5, 128, 83).cuda(), torch.randn((5, 4), generator=torch.Generator().manual_seed(84)).cuda()
+    wts, ids = B.router_topk_grouped(logits, 2, None, 1, 1, "softmax", "max", True, 1.0)
+    assert all(torch.equal(a, b) for a, b in zip((wts, ids), ops.router_topk_grouped(logits, 2)))
+    m = lambda t: [t.codes, t.scales, t.zeros]  # noqa: E731
+    assert torch.equal(B.int4_linear(x, *m(w), 64, None), ops.int4_linear(x, w))
+    assert torch.equal(B.int4_moe_experts(x, m(w), m(up), m(down), 64, wts, ids, 4), ops.int4_moe_experts(x, w, up, down, wts, ids, 4))
+
+
+def test_results_between_strides_and_behind_stay(ops):
+    """The C call with results further apart than their rows: what lies between and behind them is left as it was, in every kernel."""
+    import ctypes as C
+
+    from orin_qwen_lossless_amd import _lib
+
+    for rows, K, T, ws in ((40, 128, 3, False), (9000, 64, 20, False), (5000, 128, 300, True)):
+        w, dw = weight(ops, rows, K, 32, 90)
+        x = acts(T, K, 91)
+        xd, y = x.cuda(), torch.full((T + 1, rows + 24), 7.0, device="cuda")
+        a = _lib.MmvArgs(x=xd.data_ptr(), y=y.data_ptr(), x_tok=K * 2, y_tok=y.stride(0) * 4, rows_per_matrix=rows, nrows=rows, ncols=T, n_used=1, x_per_slot=1,
+                         x_bf16=1, y_bf16=0)
+        cw = ops._c_int4(dw)
+        space = ops._int4_workspace(cw, T, xd.device) if ws else None
+        _lib.check(_lib.lib().bf16n_int4_mmv(C.byref(cw), None, C.byref(a), 0, space.data_ptr() if ws else None, space.numel() if ws else 0, ops._stream()))
+        exact, bound = X.product(x, w)
+        X.check(y[:T, :rows], exact, bound)
+        assert (y[:T, rows:] == 7).all() and (y[T] == 7).all()
+
+
+def test_codes_beyond_four_gigabytes(ops):
+    """Places past 32 bits in the codes, for every kernel: the last rows of a large matrix are those of a small one."""
+    rows, K, group = 560000, 16384, 4096
+    g = torch.Generator(device="cuda").manual_seed(92)
+    codes = torch.randint(0, 256, (rows, K // 2), generator=g, dtype=torch.uint8, device="cuda")
+    scales = (torch.rand((rows, 4), generator=g, device="cuda") * 0.01).to(torch.bfloat16)
+    big = ops.Int4Weight(codes, scales, None, group)
+    tail = (codes[-64:].cpu(), scales[-64:].cpu(), None, group)
+    for T in (1, 20):
+        x = acts(T, K, 93)
+        y, b = X.product(x, tail)
+        X.check(ops.int4_mmv(x.cuda(), big)[:, -64:], y, b, T)
+    E = rows // 64
+    ids = torch.tensor([[E - 1, 0]] * 2, dtype=torch.int32, device="cuda")
+    x = acts(2, K, 94)
+    y, b = X.product(x, tail)
+    X.check(ops.int4_mmv(x.cuda(), big, ids, 64)[:, 0], y, b, "ids")
+    half = ops.Int4Weight(codes, scales, None, group)
+    ids = torch.full((40, 1), 1, dtype=torch.int32, device="cuda")  # two matrices of 280000 rows, the second one named: many columns
+    x = acts(40, K, 95)
+    y, b = X.product(x, tail)
+    X.check(ops.int4_moe_mm_ids(x.cuda(), ids, half, 2)[:, 0, -64:], y, b, "lists")
+
+
+def test_activations_beyond_four_gigabytes(ops):
+    """Activation rows so far apart that their places pass 32 bits: more columns than a pass has, all of them right."""
+    w, dw = weight(ops, 6000, 128, 64, 96)
+    far = torch.empty(70 * 35_000_000, dtype=torch.bfloat16, device="cuda").as_strided((70, 128), (35_000_000, 1))
+    x = acts(70, 128, 97)
+    far.copy_(x)
+    y, b = X.product(x, w)
+    X.check(ops.int4_mmv(far, dw), y, b)
+
+
+@pytest.mark.parametrize("T", [1, 5])
+def test_decode_step_with_experts_in_four_bits(ops, T):
+    """A layer of the decode step with such experts: the router's choice, and the experts' rows, from its own input."""
+    from orin_qwen_lossless_amd import decode_step as D
+    from orin_qwen_lossless_amd import synth
+
+    seed = [9000]
+
+    def gen(rows, k):
+        seed[0] += 1
+        return synth.weights_torch(rows, k, seed[0], "cuda")
+
+    sets, _, nbytes = D.make_layer_sets(ops, gen, 1, False, "int4")
+    assert isinstance(sets[0]["gate"], ops.Int4Weight) and nbytes["gate"] == sets[0]["gate"].nbytes
+    step = D.Bf16nStep(ops, sets, ops.int4_quantize(gen(512, D.K_MODEL)), 2, T)
+    x2 = acts(T, D.K_MODEL, 98).cuda()
+    ys, wts, ids = step.experts(sets[0], x2)
+    w, i = ops.router_topk(ops.mmv(x2, sets[0]["router"]), D.TOPK)
+    assert torch.equal(ids[:, :D.TOPK], i) and torch.equal(wts[:, :D.TOPK], w) and (ids[:, D.TOPK] == D.E).all()
+    batched = ops.int4_moe_experts_batched(T, D.TOPK + 1, D.EA)
+    cut = lambda m, e, n: (m.codes[e * n: e * n + n], m.scales[e * n: e * n + n], None, m.group)  # noqa: E731
+    for t in range(T):
+        for j in (0, D.TOPK):
+            e = int(ids[t, j])
+            h, hb = X.gated(*X.product(x2[t: t + 1], cut(sets[0]["gate"], e, D.N_MID)), *X.product(x2[t: t + 1], cut(sets[0]["up"], e, D.N_MID)))
+            if batched:
+                hb = X.rounded(h, hb, torch.bfloat16)
+            d = cut(sets[0]["down"], e, D.K_MODEL)
+            y, b = X.product(h, d)
+            u, s, z = X.parts(*d)
+            X.check(ys[t: t + 1, j], y, b * 1.01 + hb @ (s * (u - z)).abs().t(), (t, j))
+    h = acts(T, D.K_MODEL, 99).cuda()
+    graph, out = D.capture(step, h)
+    for k in range(3):
+        h.copy_(acts(T, D.K_MODEL, 100 + k))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, step(h)) and out.shape == (T, 512)
+
+
 def test_quantize(ops):
     """Codes are within half a step of the weight (and a rounding of the scale: the largest weight may lie past the last code by that)."""
     w = torch.randn((300, 1056), generator=torch.Generator().manual_seed(60)).mul_(0.02).to(torch.bfloat16)

@@ -1,0 +1,73 @@
+"""4-bit weights with group scales, without a GPU: what their class and the calls refuse, quantization, and the shapes under tracing."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import int4_exact as X
+from orin_qwen_lossless_amd import ops, torch_ops  # noqa: F401
+
+
+def parts(rows=6, K=128, group=64):
+    return X.make(rows, K, group, 1)
+
+
+def test_the_weights_class_refuses_what_the_kernels_do_not_take():
+    c, s, z = parts()
+    w = ops.Int4Weight(c, s, z, 64)
+    assert (w.rows, w.K, w.nbytes) == (6, 128, c.numel() + 2 * s.numel() + z.numel())
+    assert ops.Int4Weight(c, s[:, :1].contiguous(), None, 128).zeros is None
+    for bad in ((c.int(), s, z, 64), (c[:, ::2], s, z, 64), (c.reshape(-1), s, z, 64), (c[:, :24].contiguous(), s, z, 64), (c, s.float(), z, 64), (c, s[:5], z, 64),
+                (c, s, z[:, :1].contiguous(), 64), (c, s, z.int(), 64), (c, s, z, 32), (c, s, z, 48), (c, s, z, 16), (c, s, z, 64.0),
+                (torch.zeros((2, 8224), dtype=torch.uint8), torch.zeros((2, 129), dtype=torch.bfloat16), None, 128),
+                (c, s.t().contiguous().t(), z, 64)):
+        with pytest.raises(ValueError):
+            ops.Int4Weight(*bad)
+
+
+def test_calls_refuse_host_tensors():
+    w = ops.Int4Weight(*parts(), 64)
+    x, ids = torch.zeros((2, 128), dtype=torch.bfloat16), torch.zeros((2, 1), dtype=torch.int32)
+    for call in (lambda: ops.int4_mmv(x, w), lambda: ops.int4_mmv_glu2(x, w, w), lambda: ops.int4_linear(x, w), lambda: ops.int4_route(ids, 2),
+                 lambda: ops.int4_moe_mm_ids(x, ids, w, 2), lambda: ops.int4_moe_experts(x, w, w, w, torch.ones((2, 1)), ids, 2),
+                 lambda: ops.router_topk_grouped(torch.zeros((2, 8)), 2)):
+        with pytest.raises(ValueError):
+            call()
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+def test_quantize_values(symmetric):
+    """Weights that are codes already come back as they are; a group of zeros and one of a single value, too."""
+    g = torch.Generator().manual_seed(2)
+    u = torch.randint(-7, 8, (5, 96), generator=g).float()
+    u[:, 0::32], u[:, 1::32] = 7, -7  # every group has its ends
+    u[2, 32:64] = 0
+    w = (u * 0.25).to(torch.bfloat16)
+    q = ops.int4_quantize(w, 32, symmetric)
+    code, s, z = X.parts(q.codes, q.scales, q.zeros, 32)
+    got = s * (code - z)
+    if symmetric:
+        assert torch.equal(got, w.double())
+    else:  # 14 steps of 0.25 on 15: half a step, the zero point's rounding and the scale's
+        assert ((got - w.double()).abs() <= s * 1.0 + 15 * 2.0 ** -8 * s).all() and not got[2, 32:64].any()
+    assert ops.int4_quantize(w.view(5, 3, 32), 32, symmetric).rows == 15
+
+
+def test_quantize_refusals():
+    for bad in (lambda: ops.int4_quantize(torch.zeros(64)), lambda: ops.int4_quantize(torch.zeros((2, 48))), lambda: ops.int4_quantize(torch.zeros((2, 64)).half()),
+                lambda: ops.int4_quantize(torch.zeros((2, 64)), 24), lambda: ops.int4_quantize(torch.zeros((2, 64)), scale_dtype=torch.float32)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_shapes_under_tracing():
+    B = torch.ops.bf16n
+    with torch._subclasses.FakeTensorMode():
+        e = lambda *s, d=torch.bfloat16: torch.empty(s, dtype=d, device="cuda")  # noqa: E731
+        m = lambda r, k: [e(r, k // 2, d=torch.uint8), e(r, k // 64)]  # noqa: E731
+        y = B.int4_linear(e(2, 3, 128), *m(40, 128), None, 64, None)
+        assert y.shape == (2, 3, 40) and y.dtype == torch.bfloat16
+        y = B.int4_moe_experts(e(7, 128), m(4 * 64, 128), m(4 * 64, 128), m(4 * 128, 64), 64, e(7, 2, d=torch.float32), e(7, 2, d=torch.int32), 4)
+        assert y.shape == (7, 128) and y.dtype == torch.bfloat16
+        wts, ids = B.router_topk_grouped(e(7, 32, d=torch.float32), 4, None, 4, 2, "sigmoid", "top2", True, 1.0)
+        assert wts.shape == ids.shape == (7, 4) and wts.dtype == torch.float32 and ids.dtype == torch.int32
