@@ -71,14 +71,14 @@ struct i4_columns {
 };
 
 // Few columns.  One wavefront takes 16 rows of the matrix (of each of the two where they are gated) and 256 columns of it at
-// a time: a lane's 32 bytes are 64 codes of row lane % 16 (four lanes have 128 bytes of a row, a whole line: 64 of them at a time
-// took 72 us where the lines whole take @@), turned into eight operands of v_mfma_f32_16x16x32_bf16 whose other
+// a time: a lane's 32 bytes are 64 codes of row lane % 16 (four lanes have 128 bytes of a row, a whole
+// line), turned into eight operands of v_mfma_f32_16x16x32_bf16 whose other
 // operand is the activations, from LDS; result: lane = row of the matrix, register = activation row (so that a scale
 // is one value to a lane).  FP32 activations are three BF16 rows each (rows 4 t .. 4 t + 2 of the 16: one lane's registers).
 // The sums of the activations over a group, which the zero points need, are taken once, on the way into LDS.
 // A step's registers take the codes of the step U later as soon as its operands are made.
 // Wavefronts of a block share the rows (ksplit parts of K each, summed through LDS in a fixed order) or take other rows.
-// Bound by HBM where the matrix is large.
+// Bound by HBM where the matrix is large: 248320 x 2048, one token, 5.2 TB/s.
 template <int NT, int NM, int GM, bool GLU, bool XF32, bool ZEROS, int NW>
 __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i4_launch p) {
     constexpr int U = NM == 1 ? 2 : 1;                  // pairs of steps whose codes are loaded ahead
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
             }
         };
         // Scales and zero points come by blocks of 16 groups, four of its row to a lane of each quarter, a block ahead; a step takes
-        // them from the quarter that has its group.  (A load of one scale by every lane for every 128 columns: 72 us where this takes @@.)
+        // them from the quarter that has its group.  (A load of one scale by every lane for every 128 columns: 248320 x 2048, one token, 72 us where this takes 55.)
         uint64_t sc[NM], sc_next[NM];
         uint32_t ze[NM], ze_next[NM];
         const auto block_of = [&](int s) { return (s * 2 * I4_STEP >> p.group_log2) >> 4; };
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
 
         // Activations into LDS, in the operands' order, zeros behind the last column of the matrix, and their groups' sums: a
         // wavefront takes 512 columns of a row at a time and has AHEAD such pieces on the way.  (One after the other cost a latency
-        // each: 11 tokens of 1453 x 2560, gated, @@ us.)
+        // each: 16 tokens of 5120 x 2048 11.9 us, now 10.6.)
         constexpr int AHEAD = XF32 ? 2 : 4;
         const int octs = (pitch - 8) / 8; // a multiple of 16: a row of 16 lanes has 128 columns of one activation row
         const int per_row = (octs + 63) / 64, pieces = p.cols_per_pass * per_row;
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
 // Few columns of a matrix whose rows are few as well: nothing is shared through LDS but the sums of the parts of K.  A
 // wavefront loads its codes, scales and activations, these as the operand's lanes hold them, at once, one latency in
 // all; the groups' sums of the activations come from products with ones.
-// 512 x 2048, one token: @@ us in a graph, @@ with the activations through LDS.  Bound by that latency.
+// 512 x 2048, one token: 4.1 us in a graph, 5.5 with the activations through LDS; 1453 x 2560, gated, groups of 32, 11 tokens 7.8 / 14.3.  Bound by that latency.
 template <int NT, int GM, bool GLU, bool XF32, bool ZEROS>
 __global__ void __launch_bounds__(512, 2) k_i4_small(const i4_launch p) {
     constexpr int NW = 8, NM = GLU ? 2 : 1, NG = GM == 0 ? 1 : GM == 1 ? 2 : 4, CPT = XF32 ? 4 : 16, NA = XF32 ? 1 : 4;
@@ -686,16 +686,19 @@ struct i4_many {
 // at a time: the activations' piece goes straight into LDS (two buffers, 16-byte places exchanged by the row's low bits so that
 // the operands' reads find every bank), the codes into registers, both a step ahead; a wavefront turns its own codes into operands,
 // which serve MT tiles.  Every product over a group starts from zero and is added to the result times its scale.
-// Bound by the vector instructions beside the matrix cores' (nine for eight codes and tile of rows, four for a tile of results and group).
+// Bound by the vector instructions (nine for eight codes and tile of rows, four for a tile of results and group), the products and the
+// reads of LDS, which take turns more than they overlap: 8192 tokens of 8192 x 2048 reach 790 TFLOP/s, 2048 of 5120 x 2048 635.  (Without
+// the additions, without the conversions and without three of four products 302, 276 and 228 us of 313 remained.)
 template <int WM, int WN, int MT, int NT, int GM, bool GLU, bool LIST>
 __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     constexpr int THREADS = WM * WN * 64, COLS = WM * MT * 16, ROWS = WN * NT * 16 / (GLU ? 2 : 1);
     constexpr int NG = GM == 0 ? 1 : GM == 1 ? 2 : 4, LOADS = COLS * 16 / THREADS;
     static_assert(THREADS == 256 && LOADS * THREADS == COLS * 16, "a thread copies the same place of rows 16 apart");
-    static_assert(WN * NT == 8, "a wavefront copies the codes of two tiles of rows");
+    constexpr int CODE_BYTES = WN * NT * 1024, COPIES = WN * NT / 4; // codes of a step; a wavefront copies those of COPIES tiles of rows
+    static_assert(COPIES * 4 == WN * NT, "four wavefronts");
     extern __shared__ __align__(16) char lds[]; // two pieces of activations, two of codes, for lists the places of the results
     constexpr int CODES = 2 * COLS * 256;
-    int64_t * const y_at = (int64_t *) (lds + CODES + 2 * 8192);
+    int64_t * const y_at = (int64_t *) (lds + CODES + 2 * CODE_BYTES);
     const int lane = threadIdx.x & 63, m16 = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % WM, wn = wave / WM;
@@ -728,7 +731,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     } else {
         // An XCD takes every eighth block, which is made a contiguous part of the tiles here: four column tiles of one row tile
         // after the other, so that what runs there at a time shares few pieces of activations (four times a row tile's bytes).
-        // 8192 x 2048, 8192 tokens: @@ us, 428 with all column tiles of a row tile side by side.
+        // 8192 x 2048, 8192 tokens: 391 us where all column tiles of a row tile side by side took 428.
         const int n = p.row_tiles * p.col_tiles, per = (n + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
         if (id >= n) {
             return;
@@ -794,25 +797,27 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         row_off[n] = min((GLU ? n % (NT / 2) : n) * 16 + m16, (int) p.nrows - 1 - wave_row);
     }
     const auto of = [&](int n) -> const i4_matrix & { return GLU && n >= NT / 2 ? p.up : p.w; };
-    // the codes of a step: a wavefront copies tiles of rows wave and wave + 4, four lanes to a row; places exchanged by the row's bits
-    uint32_t code_off[2];
-    const uint8_t * code_at[2];
+    // the codes of a step: a wavefront copies tiles of rows wave, wave + 4 .., four lanes to a row; places exchanged by the row's bits
+    uint32_t code_off[COPIES];
+    const uint8_t * code_at[COPIES];
     const int chunk = (lane & 3) ^ (lane >> 4);
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < COPIES; i++) {
         const int t = i * 4 + wave, n = t % NT, r = row0 + (t / NT * (GLU ? NT / 2 : NT) + (GLU ? n % (NT / 2) : n)) * 16, first = min(r, p.nrows - 1);
         code_at[i] = of(n).codes + (matrix * p.nrows + first) * (p.K / 2);
         code_off[i] = min(lane >> 2, p.nrows - 1 - first) * (p.K / 2) + chunk * 16;
     }
     const auto copy_codes = [&](int s, int buf) {
         if (cut && s == S - 1 && s * I4_STEP + chunk * 32 >= p.K) {
-            code_off[0] -= chunk * 16;
-            code_off[1] -= chunk * 16;
+#pragma unroll
+            for (int i = 0; i < COPIES; i++) {
+                code_off[i] -= chunk * 16;
+            }
         }
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < COPIES; i++) {
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (code_at[i] + s * (I4_STEP / 2) + code_off[i]),
-                                             (__attribute__((address_space(3))) void *) (lds + CODES + buf * 8192 + i * 4096 + wave * 1024), 16, 0, 0);
+                                             (__attribute__((address_space(3))) void *) (lds + CODES + buf * CODE_BYTES + i * 4096 + wave * 1024), 16, 0, 0);
         }
     };
     // scales by blocks of 16 groups, four of its row to a lane of each quarter, a block ahead
@@ -936,7 +941,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
         u32x4_t code[NT];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            code[n] = *(const u32x4_t *) (lds + CODES + buf * 8192 + (wn * NT + n) * 1024 + m16 * 64 + (q ^ (m16 >> 2)) * 16);
+            code[n] = *(const u32x4_t *) (lds + CODES + buf * CODE_BYTES + (wn * NT + n) * 1024 + m16 * 64 + (q ^ (m16 >> 2)) * 16);
         }
         bf16x8_t wf[NT][4], xs[2][4];
         float sv[NT * NG];
@@ -999,16 +1004,6 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
             }
             if (!live) {
                 break;
-            }
-            if (!LIST && u > 0) {
-                if (i == 0 && m + 1 < MT) {
-                    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0); // reads of LDS
-                }
-#pragma unroll
-                for (int k = 0; k < J * NT; k++) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);      // a product
-                    __builtin_amdgcn_sched_group_barrier(0x002, 4 / J, 0);  // additions
-                }
             }
             __builtin_amdgcn_sched_barrier(0); // (else the operands of all tiles are read first, and the registers spill)
         }
@@ -1184,35 +1179,40 @@ void init_few() {
     }
 }
 
-constexpr size_t many_lds(int cols, bool list) { return (size_t) 2 * cols * 256 + 2 * 8192 + (list ? cols * 8 : 0); }
+// LDS of k_i4_many: two pieces of activations and of codes, for lists the places of the results
+constexpr size_t many_lds(int cols, int rows, bool list) { return (size_t) 2 * cols * 256 + 2 * rows * 64 + (list ? cols * 8 : 0); }
+
+// an instance of k_i4_many over WM * MT * 16 columns and WN * NT * 16 rows; without p: its LDS limit is raised
+template <int WM, int WN, int MT, int NT, int GM, bool LIST>
+void launch_many(const i4_many * p, bool glu, unsigned blocks, hipStream_t stream) {
+    constexpr int LDS = (int) many_lds(WM * MT * 16, WN * NT * 16, LIST);
+    const auto kernel = glu ? k_i4_many<WM, WN, MT, NT, GM, true, LIST> : k_i4_many<WM, WN, MT, NT, GM, false, LIST>;
+    if (p) {
+        kernel<<<blocks, 256, LDS, stream>>>(*p);
+    } else {
+        (void) hipFuncSetAttribute((const void *) kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    }
+}
 
 template <int GM> void init_many() {
-    const auto raise = [](const void * f, int cols) { (void) hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int) many_lds(cols, true)); };
-    raise((const void *) k_i4_many<2, 2, 4, 4, GM, false, false>, 128);
-    raise((const void *) k_i4_many<2, 2, 4, 4, GM, true, false>, 128);
-    raise((const void *) k_i4_many<1, 4, 4, 2, GM, false, false>, 64);
-    raise((const void *) k_i4_many<1, 4, 4, 2, GM, true, false>, 64);
-    raise((const void *) k_i4_many<1, 4, 4, 2, GM, false, true>, 64);
-    raise((const void *) k_i4_many<1, 4, 4, 2, GM, true, true>, 64);
+    for (const bool glu : {false, true}) {
+        launch_many<2, 2, 4, 4, GM, false>(nullptr, glu, 0, nullptr);
+        launch_many<1, 4, 4, 2, GM, false>(nullptr, glu, 0, nullptr);
+        launch_many<1, 4, 4, 2, GM, true>(nullptr, glu, 0, nullptr);
+    }
 }
 
 template <int GM>
 void pick_many(i4_many & p, bool glu, int cols, hipStream_t stream) {
-    const int rows = glu ? 64 : 128;
+    const bool list = p.bounds != nullptr;
+    const int rows = 128 / (glu ? 2 : 1);
     p.row_tiles = (p.nrows + rows - 1) / rows;
     p.col_tiles = (p.ncols + cols - 1) / cols;
     // lists: no more pieces than full ones and one cut short to a matrix
-    const bool list = p.bounds != nullptr;
     const int64_t pieces = list ? std::min<int64_t>(p.ncols, p.ncols / cols + p.n_matrices + 1) : p.col_tiles;
     const unsigned n = (unsigned) ((pieces * p.row_tiles + 7) / 8 * 8);
-    const auto go = [&](auto * kernel) { kernel<<<n, 256, many_lds(cols, list), stream>>>(p); };
-    if (list) {
-        glu ? go(k_i4_many<1, 4, 4, 2, GM, true, true>) : go(k_i4_many<1, 4, 4, 2, GM, false, true>);
-    } else if (cols == 128) {
-        glu ? go(k_i4_many<2, 2, 4, 4, GM, true, false>) : go(k_i4_many<2, 2, 4, 4, GM, false, false>);
-    } else {
-        glu ? go(k_i4_many<1, 4, 4, 2, GM, true, false>) : go(k_i4_many<1, 4, 4, 2, GM, false, false>);
-    }
+    list ? launch_many<1, 4, 4, 2, GM, true>(&p, glu, n, stream)
+         : cols == 128 ? launch_many<2, 2, 4, 4, GM, false>(&p, glu, n, stream) : launch_many<1, 4, 4, 2, GM, false>(&p, glu, n, stream);
 }
 
 i4_matrix matrix_of(const bf16n_int4_weight & w) { return {w.codes, (const uint16_t *) w.scales, w.zeros, w.scales_f16 != 0}; }
@@ -1265,7 +1265,7 @@ void run_few(i4_launch & p, bool glu, bool f32, bool zeros, int max_cols, int64_
     p.ksplit = ksplit;
     const int passes = p.bounds || p.ids ? 1 : std::min(65535, (max_cols + p.cols_per_pass - 1) / p.cols_per_pass);
     // the kernel without activations in LDS: up to two tiles of rows for a CU (one with FP32 activations, whose lanes part them
-    // themselves).  us, with it / without, BF16, 16 tokens: 5120 x 2048 @@, 10240 x 2048 15.6 / 11.4; FP32, three: 8192 x 2048 14.4 / 8.9
+    // themselves).  us, with it / without, BF16, 16 tokens: 5120 x 2048 9.2 / 10.6, 10240 x 2048 15.6 / 11.4; FP32, three: 8192 x 2048 14.4 / 8.9
     const bool small = tiles <= (f32 ? 1 : 2) * cus;
     pick_few(p, glu, f32, gm, zeros, {nt, grid_y, passes, cus, stream, false, small});
 }
@@ -1300,8 +1300,10 @@ void launch_int4_mmv(const bf16n_int4_weight & w, const bf16n_int4_weight * up, 
         p.nrows = (int) a.nrows;
         p.ncols = a.ncols;
         p.n_used = 1; p.n_matrices = 1;
+        // tiles of 128 x 128 (two blocks to a CU) where they make two rounds, of 128 x 64 (three) below: 5120 x 2048, 2048 tokens, 640
+        // tiles, 82.9 / 73.9 us, 4096 x 2048, 4096 tokens, 1024 tiles, 96.6 / 106.7
         const int64_t tiles = ((a.nrows + 127) / 128) * ((a.ncols + 127) / 128);
-        run_many(w, up, p, a.ncols, workspace, tiles >= cus ? 128 : 64, stream);
+        run_many(w, up, p, a.ncols, workspace, tiles >= 4 * cus ? 128 : 64, stream);
         return;
     }
     i4_launch p = launch_of(w, up, a.nrows);
