@@ -198,7 +198,8 @@ typedef struct bf16n_int4_weight {
  * zero points are applied to FP32 sums).  up given: silu(W x) * (up x), gate and up of one shape, K and group.  Arguments as in
  * bf16n_mmv_args (rows_per_matrix = nrows, row0 = 0; any number of dense columns, at most 65535 with ids); ids: int32, or int64 with
  * ids_i64; an id that names no matrix gives a column of zeros.  x: BF16 or FP32, 16-byte aligned columns.  The result must
- * not overlap x.  An activation that is not finite makes every result of its column not finite (NaN or infinite). */
+ * not overlap x.  An activation that is not finite makes every result of its column not finite (NaN or infinite); so may activations
+ * beyond 1e35, whose sums with the codes pass FP32's range before the scales are applied. */
 int bf16n_int4_mmv(const bf16n_int4_weight * w, const bf16n_int4_weight * up, const bf16n_mmv_args * a, int ids_i64, void * workspace,
                    uint64_t workspace_bytes, void * stream);
 /* workspace of the products of many columns (more than 32 BF16 columns, or many pairs per matrix): 16-byte aligned device memory,

@@ -871,7 +871,7 @@ def moe_experts(x: torch.Tensor, gate: Weight, up: Weight, down: Weight, topk_we
 INT4_FEW_TOKENS = 32  # columns from which a dense product takes a workspace (bf16n_int4_mmv)
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class Int4Weight:
     """A matrix (or a stack of matrices) of 4-bit codes with group scales on a device:
     w[r, k] = scales[r, k // group] * (code[r, k] - zeros[r, k // group]).
@@ -1026,7 +1026,8 @@ def int4_mmv(x: torch.Tensor, w: Int4Weight, ids: torch.Tensor | None = None, ro
              out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """mmv for 4-bit weights with group scales: x [tokens, K] BF16 or FP32 -> [tokens, rows], or with expert ids [tokens, n_used]
     the rows of the matrices that they name, [tokens, n_used, rows_per_matrix], zeros where an id names none.  No weight is
-    rounded: exact codes, FP32 sums, the scales applied to the sums."""
+    rounded: exact codes, FP32 sums, the scales applied to the sums.  The sums are of codes and activations before the scales: those of
+    activations beyond 1e35 may pass FP32's range where the scaled ones would not."""
     if ids is None and rows_per_matrix == 0 and out_dtype in (torch.float32, torch.bfloat16):
         y = (_host_calls or _host()).int4_mmv(x, w, None, out_dtype is torch.bfloat16, INT4_FEW_TOKENS)
         if y is not None:

@@ -191,18 +191,32 @@ def test_same_bits_again(ops):
     assert all(torch.equal(first, ops.int4_mmv(x, dw)) for _ in range(5))
 
 
-def test_not_finite(ops):
+@pytest.mark.parametrize("rows,T", [(64, 5), (8400, 5), (4000, 300)])
+def test_not_finite(ops, rows, T):
     """An activation that is not finite reaches every result of its own column and no other; so does a scale its row."""
-    _, dw = weight(ops, 64, 256, 64, 52)
+    _, dw = weight(ops, rows, 256, 64, 52)
+    others = torch.arange(T) != 2
     for dtype in (torch.bfloat16, torch.float32):
         for bad in (float("inf"), float("-inf"), float("nan")):
-            x = acts(5, 256, 53, dtype)
+            x = acts(T, 256, 53, dtype)
             x[2, 77] = bad
             y = ops.int4_mmv(x.cuda(), dw)
-            assert not torch.isfinite(y[2]).any() and torch.isfinite(y[[0, 1, 3, 4]]).all()
+            assert not torch.isfinite(y[2]).any() and torch.isfinite(y[others]).all()
     dw.scales[7, 1] = float("nan")
-    y = ops.int4_mmv(acts(5, 256, 54).cuda(), dw)
-    assert torch.isnan(y[:, 7]).all() and torch.isfinite(y[:, torch.arange(64) != 7]).all()
+    y = ops.int4_mmv(acts(T, 256, 54).cuda(), dw)
+    assert torch.isnan(y[:, 7]).all() and torch.isfinite(y[:, torch.arange(rows) != 7]).all()
+
+
+def test_nothing_to_do(ops):
+    """No tokens, no slots, no rows."""
+    w, up, down = (weight(ops, 4 * r, c, 32, 63 + i)[1] for i, (r, c) in enumerate(((32, 64), (32, 64), (64, 32))))
+    x, ids, wts = acts(3, 64, 66).cuda(), torch.zeros((3, 2), dtype=torch.int32, device="cuda"), torch.ones((3, 2), device="cuda")
+    assert ops.int4_moe_experts(x[:0], w, up, down, wts[:0], ids[:0], 4).shape == (0, 64)
+    assert not ops.int4_moe_experts(x, w, up, down, wts[:, :0].contiguous(), ids[:, :0], 4).any()
+    assert ops.int4_mmv(x[:0], w).shape == (0, 128) and ops.int4_moe_mm_ids(x[:0], ids[:0], w, 4).shape == (0, 2, 32)
+    assert ops.int4_mmv(x, ops.Int4Weight(w.codes[:0], w.scales[:0], w.zeros[:0], 32)).shape == (3, 0)
+    pairs, bounds = ops.int4_route(ids[:0], 4)
+    assert pairs.numel() == 0 and not bounds.any() and bounds.numel() == 6
 
 
 def test_large_and_small_f32(ops):
