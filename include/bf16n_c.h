@@ -196,7 +196,7 @@ typedef struct bf16n_int4_weight {
 } bf16n_int4_weight;
 /* bf16n_mmv for such a matrix: y = W x per column, sums in FP32, no weight rounded (the codes are exact operands; scales and
  * zero points are applied to FP32 sums).  up given: silu(W x) * (up x), gate and up of one shape, K and group.  Arguments as in
- * bf16n_mmv_args (rows_per_matrix = nrows, row0 = 0; any number of dense columns, at most 65535 with ids); ids: int32, or int64 with
+ * bf16n_mmv_args, with rows_per_matrix = nrows and row0 = 0; any number of dense columns, at most 65535 with ids; ids: int32, or int64 with
  * ids_i64; an id that names no matrix gives a column of zeros.  x: BF16 or FP32, 16-byte aligned columns.  The result must
  * not overlap x.  An activation that is not finite makes every result of its column not finite (NaN or infinite); so may activations
  * beyond 1e35, whose sums with the codes pass FP32's range before the scales are applied. */
