@@ -678,7 +678,8 @@ struct i4_many {
     int ncols;
     const int32_t * pairs, * bounds;        // lists of columns by matrix, or null
     const int4 * table;                     // and their pieces
-    int n_matrices, n_used, per_slot;
+    int n_matrices;
+    uint32_t per_token, one_used;           // pairs to a row of activations, and 2^32 over them
     int row_tiles, col_tiles;               // dense: the grid
 };
 
@@ -743,7 +744,12 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     }
     const auto x_row_of = [&](int i) { // the activation row behind column i; columns that are not there repeat the last
         const int c = c0 + min(i, nc - 1);
-        return !LIST ? c : p.per_slot ? p.pairs[c] : p.pairs[c] / p.n_used;
+        if constexpr (!LIST) {
+            return c;
+        } else { // a pair's token: by the reciprocal, rounded down, which is at most one too few
+            const uint32_t pair = p.pairs[c], token = __umulhi(pair, p.one_used);
+            return (int) (token + (pair - token * p.per_token >= p.per_token));
+        }
     };
     if (LIST && threadIdx.x < nc) {
         y_at[threadIdx.x] = p.pairs[c0 + threadIdx.x] * p.y_row; // (read behind the barriers of the steps)
@@ -862,12 +868,15 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     const auto load_zeros = [&](int step) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int64_t gi = min((int) (((int64_t) (step * 16 + j * 4 + q) << p.sum_group_log2) >> p.group_log2), p.n_groups - 1);
+            if (step * 16 + j * 4 >= p.sums_row) {
+                break;
+            }
+            const int gi = min((step * 16 + j * 4 + q) >> (p.group_log2 - p.sum_group_log2), p.n_groups - 1);
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                const int64_t at = (wave_at + row_off[n]) * p.n_groups + gi;
-                zs[j][n] = of(n).scales[at];
-                zz[j][n] = of(n).zeros ? of(n).zeros[at] : 8u;
+                const uint32_t at = row_off[n] * p.n_groups + gi;
+                zs[j][n] = (of(n).scales + wave_at * p.n_groups)[at];
+                zz[j][n] = of(n).zeros ? (of(n).zeros + wave_at * p.n_groups)[at] : 8u;
             }
         }
     };
@@ -1014,22 +1023,39 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
             at[j] += flip;
         }
     }
+    const auto write = [&](auto type) {
+        using T = decltype(type);
+        const int r = row0 + wn * (GLU ? NT / 2 : NT) * 16 + m16;
+        char * const y_lane = p.y + (int64_t) r * sizeof(T);
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
+        for (int m = 0; m < MT; m++) {
+            if (LIST && m >= mt) {
+                break;
+            }
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int c = (m * WM + wm) * 16 + q * 4 + e;
-            if (c < nc) {
-                char * const y = p.y + (LIST ? y_at[c] : (c0 + c) * p.y_row);
+            for (int e = 0; e < 4; e++) {
+                const int c = (m * WM + wm) * 16 + q * 4 + e;
+                if (c < nc) {
+                    T * const y = (T *) (y_lane + (LIST ? y_at[c] : (c0 + c) * p.y_row));
 #pragma unroll
-                for (int n = 0; n < (GLU ? NT / 2 : NT); n++) {
-                    const int r = row0 + (wn * (GLU ? NT / 2 : NT) + n) * 16 + m16;
-                    if (r < p.nrows) {
-                        store_y(y, p.y_bf16, r, GLU ? silu(acc[m][n][e]) * acc[m][n + (GLU ? NT / 2 : 0)][e] : acc[m][n][e]);
+                    for (int n = 0; n < (GLU ? NT / 2 : NT); n++) {
+                        if (r + n * 16 < p.nrows) {
+                            const float v = GLU ? silu(acc[m][n][e]) * acc[m][n + (GLU ? NT / 2 : 0)][e] : acc[m][n][e];
+                            if constexpr (sizeof(T) == 2) {
+                                y[n * 16] = __builtin_bit_cast(uint16_t, (__bf16) v);
+                            } else {
+                                y[n * 16] = v;
+                            }
+                        }
                     }
                 }
             }
         }
+    };
+    if (p.y_bf16) {
+        write(uint16_t{});
+    } else {
+        write(float{});
     }
 }
 
@@ -1299,7 +1325,7 @@ void launch_int4_mmv(const bf16n_int4_weight & w, const bf16n_int4_weight * up, 
         p.y = (char *) a.y; p.y_row = a.y_tok; p.y_bf16 = a.y_bf16 != 0;
         p.nrows = (int) a.nrows;
         p.ncols = a.ncols;
-        p.n_used = 1; p.n_matrices = 1;
+        p.n_matrices = 1;
         // tiles of 128 x 128 (two blocks to a CU) where they make two rounds, of 128 x 64 (three) below: 5120 x 2048, 2048 tokens, 640
         // tiles, 82.9 / 73.9 us, 4096 x 2048, 4096 tokens, 1024 tiles, 96.6 / 106.7
         const int64_t tiles = ((a.nrows + 127) / 128) * ((a.ncols + 127) / 128);
@@ -1343,7 +1369,8 @@ void launch_int4_mm_ids(const bf16n_int4_weight & w, const bf16n_int4_weight * u
         p.nrows = (int) (w.rows / n_matrices);
         p.ncols = (int) n_pairs;
         p.pairs = pairs; p.bounds = bounds;
-        p.n_matrices = n_matrices; p.n_used = n_used; p.per_slot = per_slot;
+        p.n_matrices = n_matrices;
+        p.per_token = per_slot ? 1 : n_used; p.one_used = (uint32_t) std::min<uint64_t>(~0u, (1ull << 32) / p.per_token);
         run_many(w, up, p, x_rows, workspace, 64, stream);
         return;
     }
