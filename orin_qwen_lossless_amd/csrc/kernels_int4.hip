@@ -691,7 +691,7 @@ struct i4_many {
 // reads of LDS, which take turns more than they overlap: 8192 tokens of 8192 x 2048 reach 790 TFLOP/s, 2048 of 5120 x 2048 635.  (Without
 // the additions, without the conversions and without three of four products 302, 276 and 228 us of 313 remained.)
 template <int WM, int WN, int MT, int NT, int GM, bool GLU, bool LIST>
-__global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
+__global__ void __launch_bounds__(WM * WN * 64, LIST ? 3 : 2) k_i4_many(const i4_many p) {
     constexpr int THREADS = WM * WN * 64, COLS = WM * MT * 16, ROWS = WN * NT * 16 / (GLU ? 2 : 1);
     constexpr int NG = GM == 0 ? 1 : GM == 1 ? 2 : 4, LOADS = COLS * 16 / THREADS;
     static_assert(THREADS == 256 && LOADS * THREADS == COLS * 16, "a thread copies the same place of rows 16 apart");
@@ -931,104 +931,108 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
     for (int j = 0; j < 4; j++) {
         at[j] = tiles + buf * (COLS * 256) + ((GM == 0 ? q * 4 + j : j * 4 + q) ^ m16) * 16;
     }
-    for (int s = 0; s < S; s++) {
-        arrived();
-        if (s + 1 < S) {
-            copy(s + 1, buf ^ 1);
-            copy_codes(s + 1, buf ^ 1);
-        }
-        const int block = block_of(s);
-        if (s == 0 || block != block_of(s - 1)) {
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                sc[n] = sc_next[n];
+    const auto steps = [&](auto tiles_of_columns) {
+        constexpr int M = decltype(tiles_of_columns)::value;
+        for (int s = 0; s < S; s++) {
+            arrived();
+            if (s + 1 < S) {
+                copy(s + 1, buf ^ 1);
+                copy_codes(s + 1, buf ^ 1);
             }
-            if (block < block_of(S - 1)) {
-                load_block(block + 1);
-            }
-        }
-        u32x4_t code[NT];
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-            code[n] = *(const u32x4_t *) (lds + CODES + buf * CODE_BYTES + (wn * NT + n) * 1024 + m16 * 64 + (q ^ (m16 >> 2)) * 16);
-        }
-        bf16x8_t wf[NT][4], xs[2][4];
-        float sv[NT * NG];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            xs[0][j] = operand(at[j], 0);
-        }
-        if (cut && s == S - 1 && s * I4_STEP + q * 32 >= p.K) {
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                code[n] = u32x4_t{};
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const u32x4_t d = GM ? i4_transpose(code[n]) : code[n];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                wf[n][j] = i4_operand_in_order(d[j]);
-            }
-#pragma unroll
-            for (int i = 0; i < NG; i++) {
-                const int g = min((s * I4_STEP + i * (I4_STEP / NG)) >> p.group_log2, p.n_groups - 1);
-                const int quarter = (g >> 2) & 3, e = g - first_of(block, quarter);
-                const uint32_t v = __builtin_amdgcn_ds_bpermute((quarter * 16 + m16) * 4, (uint32_t) (e & 2 ? sc[n] >> 32 : sc[n]));
-                sv[n * NG + i] = i4_scale(v >> (e & 1) * 16 & 0xFFFFu, of(n).f16 ? ~0u : 0u);
-            }
-        }
-        // a tile's products over a group are added up while the matrix cores work on the next ones
-        f32x4_t part[2][NT];
-#pragma unroll
-        for (int u = 0; u <= MT * NG; u++) {
-            const int m = u / NG, i = u % NG;
-            constexpr int J = 4 / NG;
-            const bool live = u < MT * NG && (!LIST || m < mt);
-            if (live) {
-                if (i == 0 && m + 1 < MT) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        xs[(m + 1) & 1][j] = operand(at[j], m + 1);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < J; j++) {
-#pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        part[u & 1][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xs[m & 1][i * J + j], wf[n][i * J + j], j ? part[u & 1][n] : none, 0, 0, 0);
-                    }
-                }
-            }
-            if (u > 0) {
-                const int pm = (u - 1) / NG, pi = (u - 1) % NG;
+            const int block = block_of(s);
+            if (s == 0 || block != block_of(s - 1)) {
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        acc[pm][n][e] = fmaf(sv[n * NG + pi], part[(u - 1) & 1][n][e], acc[pm][n][e]);
-                    }
+                    sc[n] = sc_next[n];
+                }
+                if (block < block_of(S - 1)) {
+                    load_block(block + 1);
                 }
             }
-            if (!live) {
-                break;
-            }
-            __builtin_amdgcn_sched_barrier(0); // (else the operands of all tiles are read first, and the registers spill)
-        }
-        const int flip = buf ? -COLS * 256 : COLS * 256;
-        buf ^= 1;
+            u32x4_t code[NT];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            at[j] += flip;
+            for (int n = 0; n < NT; n++) {
+                code[n] = *(const u32x4_t *) (lds + CODES + buf * CODE_BYTES + (wn * NT + n) * 1024 + m16 * 64 + (q ^ (m16 >> 2)) * 16);
+            }
+            bf16x8_t wf[NT][4], xs[2][4];
+            float sv[NT * NG];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                xs[0][j] = operand(at[j], 0);
+            }
+            if (cut && s == S - 1 && s * I4_STEP + q * 32 >= p.K) {
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    code[n] = u32x4_t{};
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const u32x4_t d = GM ? i4_transpose(code[n]) : code[n];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    wf[n][j] = i4_operand_in_order(d[j]);
+                }
+#pragma unroll
+                for (int i = 0; i < NG; i++) {
+                    const int g = min((s * I4_STEP + i * (I4_STEP / NG)) >> p.group_log2, p.n_groups - 1);
+                    const int quarter = (g >> 2) & 3, e = g - first_of(block, quarter);
+                    const uint32_t v = __builtin_amdgcn_ds_bpermute((quarter * 16 + m16) * 4, (uint32_t) (e & 2 ? sc[n] >> 32 : sc[n]));
+                    sv[n * NG + i] = i4_scale(v >> (e & 1) * 16 & 0xFFFFu, of(n).f16 ? ~0u : 0u);
+                }
+            }
+            // a tile's products over a group are added up while the matrix cores work on the next ones
+            f32x4_t part[2][NT];
+#pragma unroll
+            for (int u = 0; u <= M * NG; u++) {
+                const int m = u / NG, i = u % NG;
+                constexpr int J = 4 / NG;
+                const bool live = u < M * NG && (!LIST || GM || m < mt);
+                if (live) {
+                    if (i == 0 && m + 1 < M) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            xs[(m + 1) & 1][j] = operand(at[j], m + 1);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < J; j++) {
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
+                            part[u & 1][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xs[m & 1][i * J + j], wf[n][i * J + j], j ? part[u & 1][n] : none, 0, 0, 0);
+                        }
+                    }
+                }
+                if (u > 0) {
+                    const int pm = (u - 1) / NG, pi = (u - 1) % NG;
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            acc[pm][n][e] = fmaf(sv[n * NG + pi], part[(u - 1) & 1][n][e], acc[pm][n][e]);
+                        }
+                    }
+                }
+                if (!live) {
+                    break;
+                }
+                __builtin_amdgcn_sched_barrier(0); // (else the operands of all tiles are read first, and the registers spill)
+            }
+            const int flip = buf ? -COLS * 256 : COLS * 256;
+            buf ^= 1;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                at[j] += flip;
+            }
         }
-    }
-    const auto write = [&](auto type) {
+    };
+    const auto write = [&](auto tiles_of_columns, auto type) {
+        constexpr int M = decltype(tiles_of_columns)::value;
         using T = decltype(type);
         const int r = row0 + wn * (GLU ? NT / 2 : NT) * 16 + m16;
         char * const y_lane = p.y + (int64_t) r * sizeof(T);
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
+        for (int m = 0; m < M; m++) {
             if (LIST && m >= mt) {
                 break;
             }
@@ -1052,10 +1056,22 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) k_i4_many(const i4_many p) {
             }
         }
     };
-    if (p.y_bf16) {
-        write(uint16_t{});
+    const auto run = [&](auto tiles_of_columns) {
+        steps(tiles_of_columns);
+        if (p.y_bf16) {
+            write(tiles_of_columns, uint16_t{});
+        } else {
+            write(tiles_of_columns, float{});
+        }
+    };
+    // Lists: where a step is within a group, its loop ends at the last tile that has columns.  With smaller groups the branches cost so many
+    // registers that two blocks are on a CU where three could be: there two tiles or all four, the columns that are not there along
+    // with the others and then left out.  256 experts, 2048 tokens, groups of 64 337 -> 298 us, 32 424 -> 373; 700 tokens, 64 199 -> 171; but groups
+    // of 128, 2048 tokens 258 -> 266
+    if (LIST && GM && mt <= 2) {
+        run(std::integral_constant<int, 2>());
     } else {
-        write(float{});
+        run(std::integral_constant<int, MT>());
     }
 }
 
