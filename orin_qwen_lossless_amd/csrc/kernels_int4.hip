@@ -684,12 +684,12 @@ struct i4_many {
 };
 
 // A block takes WM * MT * 16 columns and WN * NT * 16 rows (half of them of either matrix where they are gated) and 128 columns of K
-// at a time: the activations' piece goes straight into LDS (two buffers, 16-byte places exchanged by the row's low bits so that
-// the operands' reads find every bank), the codes into registers, both a step ahead; a wavefront turns its own codes into operands,
-// which serve MT tiles.  Every product over a group starts from zero and is added to the result times its scale.
+// at a time: the activations' piece and the codes go straight into LDS a step ahead (two buffers, 16-byte places exchanged by the row's
+// low bits so that the operands' reads find every bank); a wavefront turns its own codes into operands, which serve MT tiles.  Every product over a group starts from zero and is added to the result times its scale.
 // Bound by the vector instructions (nine for eight codes and tile of rows, four for a tile of results and group), the products and the
-// reads of LDS, which take turns more than they overlap: 8192 tokens of 8192 x 2048 reach 790 TFLOP/s, 2048 of 5120 x 2048 635.  (Without
-// the additions, without the conversions and without three of four products 302, 276 and 228 us of 313 remained.)
+// reads of LDS, which take turns more than they overlap: 8192 tokens of 8192 x 2048 reach 790 TFLOP/s, 2048 of 5120 x 2048 700.  (Without
+// the additions, without the conversions and without three of four products 302, 276 and 228 us of 313 remained.)  Making the next
+// operands under this step's products, with a step's copies spread over it, came to the same times.
 template <int WM, int WN, int MT, int NT, int GM, bool GLU, bool LIST>
 __global__ void __launch_bounds__(WM * WN * 64, LIST ? 3 : 2) k_i4_many(const i4_many p) {
     constexpr int THREADS = WM * WN * 64, COLS = WM * MT * 16, ROWS = WN * NT * 16 / (GLU ? 2 : 1);
