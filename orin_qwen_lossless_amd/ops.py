@@ -869,6 +869,7 @@ def moe_experts(x: torch.Tensor, gate: Weight, up: Weight, down: Weight, topk_we
 # ---------------------------------------------------------------- 4-bit weights with group scales
 
 INT4_FEW_TOKENS = 32  # columns from which a dense product takes a workspace (bf16n_int4_mmv)
+INT4_ID_COLUMNS = 65535  # (token, slot) columns that one bf16n_int4_mmv call with ids takes
 
 
 @dataclass(frozen=True, eq=False)
@@ -970,7 +971,8 @@ def _int4_workspace(cw: _lib.Int4Weight, x_rows: int, device: torch.device, n_pa
 
 
 def _int4_mmv(what: str, x: torch.Tensor, w: Int4Weight, up: Int4Weight | None, ids: torch.Tensor | None, rows_per_matrix: int,
-              out_dtype: torch.dtype) -> torch.Tensor:
+              out_dtype: torch.dtype, out: torch.Tensor | None = None) -> torch.Tensor:
+    """out (with ids): where the result goes, contiguous and of its shape and type."""
     cw = _c_int4(w)
     cu = None
     if up is not None:
@@ -1004,7 +1006,7 @@ def _int4_mmv(what: str, x: torch.Tensor, w: Int4Weight, up: Int4Weight | None, 
         if not ((x.dim() == 2 and x.shape[0] == T) or (x.dim() == 3 and x.shape[0] == T and x.shape[1] == n_used)):
             raise ValueError(f"bf16n.{what}: x must be [tokens, K] or [tokens, n_used, K]")
         n = rows_per_matrix
-        y = torch.empty((T, n_used, n), dtype=out_dtype, device=dev)
+        y = torch.empty((T, n_used, n), dtype=out_dtype, device=dev) if out is None else out
         if T == 0 or n_used == 0:
             return y
         if cw.rows == 0:
@@ -1025,7 +1027,8 @@ def _int4_mmv(what: str, x: torch.Tensor, w: Int4Weight, up: Int4Weight | None, 
 def int4_mmv(x: torch.Tensor, w: Int4Weight, ids: torch.Tensor | None = None, rows_per_matrix: int = 0,
              out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """mmv for 4-bit weights with group scales: x [tokens, K] BF16 or FP32 -> [tokens, rows], or with expert ids [tokens, n_used]
-    the rows of the matrices that they name, [tokens, n_used, rows_per_matrix], zeros where an id names none.  No weight is
+    the rows of the matrices that they name, [tokens, n_used, rows_per_matrix], zeros where an id names none (at most
+    INT4_ID_COLUMNS ids a call).  No weight is
     rounded: exact codes, FP32 sums, the scales applied to the sums.  The sums are of codes and activations before the scales: those of
     activations beyond 1e35 may pass FP32's range where the scaled ones would not."""
     if ids is None and rows_per_matrix == 0 and out_dtype in (torch.float32, torch.bfloat16):
@@ -1124,7 +1127,7 @@ def int4_moe_mm_ids(x: torch.Tensor, topk_ids: torch.Tensor, w: Int4Weight, n_ex
 
 
 def int4_moe_experts_batched(n_tokens: int, n_used: int, n_experts: int) -> bool:
-    """Whether int4_moe_experts_rows sorts the pairs by expert first, rather than running every pair by itself."""
+    """Whether int4_moe_experts_rows sorts the pairs of BF16 activations by expert first, rather than running every pair by itself."""
     # (us, one by one / sorted: 256 experts, top-8, 16 / 32 / 48 tokens 73 / 114 / 157 against 80 / 117 / 140; 64, top-4, 16 / 24
     # 68 / 94 against 69 / 80; 8, top-2, 4 / 8 24 / 27 against 25 / 26)
     return n_tokens * n_used > n_experts
@@ -1133,23 +1136,36 @@ def int4_moe_experts_batched(n_tokens: int, n_used: int, n_experts: int) -> bool
 def int4_moe_experts_rows(x: torch.Tensor, gate: Int4Weight, up: Int4Weight, down: Int4Weight, topk_ids: torch.Tensor,
                           n_experts: int) -> torch.Tensor:
     """The per-(token, slot) outputs down_e(silu(gate_e x) * (up_e x)) of the routed experts, FP32 [T, n_used, H]
-    (moe_experts_rows).  While the pairs are few each is a column of its own with FP32 between the products; beyond that
-    the pairs are sorted by expert, every expert that is named is read once, and the hidden rows are BF16, the matrix cores' operand
-    (a relative 2^-9 each, as in moe_experts_rows; the sum over them averages it out)."""
+    (moe_experts_rows).  While the pairs are few each is a column of its own with FP32 between the products.  Beyond that
+    (int4_moe_experts_batched) BF16 activations have the pairs sorted by expert, every expert that is named is read once, and
+    the hidden rows are BF16, the matrix cores' operand (half a step each, a relative 2^-8 at most, as in moe_experts_rows).
+    FP32 activations keep FP32 between the products and a column to a pair whatever their number, which is what a caller takes
+    who does not want that rounding, and slower for many (256 experts of 512, top-8, whole calls, us, BF16 / FP32: 33 tokens 83 / 96, 300
+    131 / 640, 2048 262 / 3875)."""
     n_mid, n_out = gate.rows // max(n_experts, 1), down.rows // max(n_experts, 1)
     x = x.contiguous()
-    if int4_moe_experts_batched(x.shape[0], topk_ids.shape[1], n_experts):
+    T, n_used = x.shape[0], topk_ids.shape[1]
+    if x.dtype is torch.bfloat16 and int4_moe_experts_batched(T, n_used, n_experts):
         routes = int4_route(topk_ids, n_experts)
         hidden = int4_moe_mm_ids(x, topk_ids, gate, n_experts, up=up, out_dtype=torch.bfloat16, routes=routes)
         return int4_moe_mm_ids(hidden, topk_ids, down, n_experts, routes=routes)
-    return int4_mmv(int4_mmv_glu2(x, gate, up, topk_ids, n_mid), down, topk_ids, n_out)
+    if T * n_used <= INT4_ID_COLUMNS or T != topk_ids.shape[0]:
+        return int4_mmv(int4_mmv_glu2(x, gate, up, topk_ids, n_mid), down, topk_ids, n_out)
+    ys = torch.empty((T, n_used, n_out), dtype=torch.float32, device=x.device)
+    step = max(1, INT4_ID_COLUMNS // n_used)
+    for t in range(0, T, step):
+        ids = topk_ids[t: t + step]
+        hidden = int4_mmv_glu2(x[t: t + step], gate, up, ids, n_mid)
+        _int4_mmv("int4_moe_experts_rows", hidden, down, None, ids, n_out, torch.float32, ys[t: t + step])
+    return ys
 
 
 def int4_moe_experts(x: torch.Tensor, gate: Int4Weight, up: Int4Weight, down: Int4Weight, topk_weights: torch.Tensor,
                      topk_ids: torch.Tensor, n_experts: int) -> torch.Tensor:
-    """Routed experts of one MoE layer on 4-bit weights with group scales, BF16 out (moe_experts)."""
+    """Routed experts of one MoE layer on 4-bit weights with group scales, BF16 out (moe_experts); x BF16 or FP32, which
+    decides what the hidden rows are held in for many tokens (int4_moe_experts_rows)."""
     if topk_ids.dim() == 2:
-        batched = int4_moe_experts_batched(topk_ids.shape[0], topk_ids.shape[1], n_experts)
+        batched = x.dtype is torch.bfloat16 and int4_moe_experts_batched(topk_ids.shape[0], topk_ids.shape[1], n_experts)
         y = (_host_calls or _host()).int4_moe_experts(x, gate, up, down, topk_weights, topk_ids, n_experts, batched)
         if y is not None:
             return _lib.check(y) if type(y) is int else y
