@@ -929,17 +929,17 @@ def int4_quantize(w: torch.Tensor, group: int = 128, symmetric: bool = True, sca
     if scale_dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("bf16n.int4_quantize: scales are bf16 or f16")
     K = w.shape[-1]
-    if K % 32 or not 32 <= K <= 16384 or group < 32 or group & (group - 1):
+    if K % 32 or not 32 <= K <= 16384 or not isinstance(group, int) or not 32 <= group <= 1 << 30 or group & (group - 1):
         raise ValueError("bf16n.int4_quantize: K must be a multiple of 32 in [32, 16384], group a power of two from 32 on")
     w = w.reshape(-1, K)
-    rows, n = w.shape[0], -(-K // group)
+    rows, n, width = w.shape[0], -(-K // group), min(group, K)  # (a group past the last column is the row's columns alone)
     codes = torch.empty((rows, K // 2), dtype=torch.uint8, device=w.device)
     scales = torch.empty((rows, n), dtype=scale_dtype, device=w.device)
     zeros = None if symmetric else torch.empty((rows, n), dtype=torch.uint8, device=w.device)
-    step = max(1, DEQUANT_CHUNK_BYTES // (4 * K))
+    step = max(1, DEQUANT_CHUNK_BYTES // (4 * n * width))
     for r in range(0, rows, step):
         v = w[r: r + step].float()
-        v = torch.nn.functional.pad(v, (0, n * group - K)).view(v.shape[0], n, group)
+        v = torch.nn.functional.pad(v, (0, n * width - K)).view(v.shape[0], n, width)
         if symmetric:
             s = (v.abs().amax(2) / 7.0).to(scale_dtype)
             z = torch.full_like(s, 8.0, dtype=torch.float32)
@@ -949,7 +949,7 @@ def int4_quantize(w: torch.Tensor, group: int = 128, symmetric: bool = True, sca
             z = torch.nan_to_num(torch.round(-lo / s.float()), nan=8.0).clamp(0, 15)
             zeros[r: r + step] = z.to(torch.uint8)
         q = torch.nan_to_num(torch.round(v / s.float()[:, :, None]), nan=0.0).add_(z[:, :, None]).clamp_(0, 15).to(torch.uint8)
-        q = q.view(v.shape[0], n * group)[:, :K]
+        q = q.view(v.shape[0], n * width)[:, :K]
         codes[r: r + step] = q[:, 0::2] | (q[:, 1::2] << 4)
         scales[r: r + step] = s
     return Int4Weight(codes, scales, zeros, group)

@@ -71,3 +71,39 @@ def test_shapes_under_tracing():
         assert y.shape == (7, 128) and y.dtype == torch.bfloat16
         wts, ids = B.router_topk_grouped(e(7, 32, d=torch.float32), 4, None, 4, 2, "sigmoid", "top2", True, 1.0)
         assert wts.shape == ids.shape == (7, 4) and wts.dtype == torch.float32 and ids.dtype == torch.int32
+
+
+@pytest.mark.parametrize("rows,K,group", [(64, 64, 1 << 20), (300, 2080, 1 << 11), (3, 96, 1 << 30)])
+def test_quantize_takes_no_more_memory_for_wide_groups(rows, K, group, monkeypatch):
+    """A group past the last column is that row's columns alone: the largest temporary is a piece, whatever the group."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    monkeypatch.setattr(ops, "DEQUANT_CHUNK_BYTES", 1 << 18)
+    most = [0]
+
+    class Sizes(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            for t in out if isinstance(out, (tuple, list)) else (out,):
+                if isinstance(t, torch.Tensor):
+                    assert t.numel() <= limit, (func, t.shape)
+                    most[0] = max(most[0], t.numel())
+            return out
+
+    w = torch.randn((rows, K), generator=torch.Generator().manual_seed(3))
+    limit = max(rows * K, (1 << 18) // 4, -(-K // group) * min(group, 4096))
+    for symmetric in (True, False):
+        with Sizes():
+            q = ops.int4_quantize(w, group, symmetric)
+        assert q.group == group and q.scales.shape == (rows, -(-K // group))
+        if group >= K:  # one group to a row: the same as with the smallest such group
+            same = ops.int4_quantize(w, 1 << (K - 1).bit_length(), symmetric)
+            assert torch.equal(q.codes, same.codes) and torch.equal(q.scales, same.scales)
+            assert symmetric or torch.equal(q.zeros, same.zeros)
+    assert most[0] > 0
+
+
+def test_quantize_refuses_groups_that_no_weight_has():
+    for group in (1 << 31, 64.0, 0, -32):
+        with pytest.raises(ValueError):
+            ops.int4_quantize(torch.zeros((2, 64)), group)
