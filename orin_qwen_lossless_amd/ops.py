@@ -937,16 +937,24 @@ def int4_quantize(w: torch.Tensor, group: int = 128, symmetric: bool = True, sca
     scales = torch.empty((rows, n), dtype=scale_dtype, device=w.device)
     zeros = None if symmetric else torch.empty((rows, n), dtype=torch.uint8, device=w.device)
     step = max(1, DEQUANT_CHUNK_BYTES // (4 * n * width))
+
+    def scale_of(s):  # finite weights past what a scale can hold: the largest one, and the codes that are nearest with it
+        return torch.where(s.isfinite(), s.clamp_max(torch.finfo(scale_dtype).max), s).to(scale_dtype)
+
     for r in range(0, rows, step):
         v = w[r: r + step].float()
         v = torch.nn.functional.pad(v, (0, n * width - K)).view(v.shape[0], n, width)
         if symmetric:
-            s = (v.abs().amax(2) / 7.0).to(scale_dtype)
+            s = scale_of(v.abs().amax(2) / 7.0)
             z = torch.full_like(s, 8.0, dtype=torch.float32)
         else:
             lo = v.amin(2).clamp_max(0.0)
-            s = ((v.amax(2).clamp_min(0.0) - lo) / 15.0).to(scale_dtype)
-            z = torch.nan_to_num(torch.round(-lo / s.float()), nan=8.0).clamp(0, 15)
+            hi = v.amax(2).clamp_min(0.0)
+            step15 = (hi - lo) / 15.0
+            step15 = torch.where(step15.isinf(), hi / 15.0 - lo / 15.0, step15)  # (the range alone may pass FP32's)
+            s = scale_of(step15)
+            # (where the scale is cut down the zero point stays where it parts the range)
+            z = torch.nan_to_num(torch.round(-lo / torch.maximum(s.float(), step15 * (step15 > torch.finfo(scale_dtype).max))), nan=8.0).clamp(0, 15)
             zeros[r: r + step] = z.to(torch.uint8)
         q = torch.nan_to_num(torch.round(v / s.float()[:, :, None]), nan=0.0).add_(z[:, :, None]).clamp_(0, 15).to(torch.uint8)
         q = q.view(v.shape[0], n * width)[:, :K]

@@ -107,3 +107,22 @@ def test_quantize_refuses_groups_that_no_weight_has():
     for group in (1 << 31, 64.0, 0, -32):
         with pytest.raises(ValueError):
             ops.int4_quantize(torch.zeros((2, 64)), group)
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("top,scale_dtype", [(1e6, torch.float16), (3e38, torch.bfloat16), (3e38, torch.float16)])
+def test_quantize_of_weights_past_the_scales_range(symmetric, top, scale_dtype):
+    """Finite weights give finite ones, the nearest codes of the largest scale there is; other groups do not notice.  A group with a
+    weight that is not finite has no values."""
+    w = torch.zeros((2, 96))
+    w[0, 3], w[0, 5], w[1, 40] = top, -top, 2.0
+    q = ops.int4_quantize(w, 32, symmetric, scale_dtype)
+    code, s, z = X.parts(q.codes, q.scales, q.zeros, 32)
+    got = s * (code - z)
+    assert torch.isfinite(got).all() and got[0, 3] > 0 > got[0, 5] and abs(got[1, 40] - 2.0) <= 2.0 * 2.0 ** -8
+    largest = torch.finfo(scale_dtype).max
+    assert s[0, 0] == largest if top / 7.5 > largest else (got[0, 3] >= 0.9 * top and got[0, 5] <= -0.8 * top)
+    w[0, 3] = float("inf")
+    q = ops.int4_quantize(w, 32, symmetric, scale_dtype)
+    code, s, z = X.parts(q.codes, q.scales, q.zeros, 32)
+    assert not torch.isfinite(s[0, :32]).any() and torch.isfinite(s[0, 32:]).all()
