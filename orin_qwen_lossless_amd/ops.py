@@ -315,7 +315,7 @@ def _host():
             calls.bind(*(C.cast(f, C.c_void_p).value for f in (L.bf16n_mmv, L.bf16n_gemv_max_tokens, L.bf16n_dequant)))
             calls.bind_int4(*(C.cast(f, C.c_void_p).value for f in (L.bf16n_int4_workspace_bytes, L.bf16n_int4_mmv, L.bf16n_int4_route, L.bf16n_int4_mm_ids,
                                                                     L.bf16n_moe_combine, L.bf16n_router_topk_grouped)))
-        except ImportError as e:
+        except (ImportError, AttributeError) as e:  # (AttributeError: a module of an older build lacks a call)
             warnings.warn(f"bf16n: dense products are called without their native part ({e}): a call takes about 4 us longer; "
                           "build it with `python -m orin_qwen_lossless_amd.build`", RuntimeWarning, stacklevel=3)
             calls = _NoNativeCalls

@@ -126,3 +126,15 @@ def test_quantize_of_weights_past_the_scales_range(symmetric, top, scale_dtype):
     q = ops.int4_quantize(w, 32, symmetric, scale_dtype)
     code, s, z = X.parts(q.codes, q.scales, q.zeros, 32)
     assert not torch.isfinite(s[0, :32]).any() and torch.isfinite(s[0, 32:]).all()
+
+
+def test_native_calls_of_an_older_build_are_not_used(monkeypatch):
+    """An extension module of this torch's that was built before these calls came in: everything goes the general way, with a warning."""
+    import types
+
+    stale = types.SimpleNamespace(built_for=ops.torch_release(), bind=lambda *_: None, mmv=lambda *_: None, linear=lambda *_: None)
+    monkeypatch.setattr(ops.importlib, "import_module", lambda *_: stale)
+    monkeypatch.setattr(ops, "_host_calls", None)
+    with pytest.warns(RuntimeWarning, match="native part"):
+        assert ops._host() is ops._NoNativeCalls
+    assert ops._host().int4_mmv(None, None, None, False, 32) is None
