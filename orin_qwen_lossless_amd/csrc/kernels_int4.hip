@@ -598,8 +598,9 @@ __global__ void __launch_bounds__(512, 2) k_i4_small(const i4_launch p) {
 //
 // The zero points' part of a product,  - sum_g s[r, g] z[r, g] X[t, g]  with X the sum of the activations over group g (of 128
 // columns where it is larger), is a product of its own over the groups.  Both factors are cut into three BF16 parts that add
-// up to them, so that it runs on the matrix cores as well: eight columns for a group, X1 X2 X1 X3 X2 X1 0 0 against
-// Z1 Z1 Z2 Z1 Z2 Z3 0 0 (what is left out is below 2^-23 of the product), instead of four FMAs per result tile and group.
+// up to them, so that it runs on the matrix cores as well: eight columns for a group, X1 X2 X1 X3 X2 X1 X3 X2 against
+// Z1 Z1 Z2 Z1 Z2 Z3 Z2 Z3, instead of four FMAs per result tile and group.  A third part is below 2^-14 of its number, so what is left
+// out, X3 Z3, is below 2^-28 of the product.
 
 // X of every activation row, in parts: one thread to 32 columns.  For lists of columns by matrix the last block counts the pieces of
 // `cols` columns of every matrix (and of the pairs that name none) instead and lists them: (matrix, first column, columns), how many in table[0].
@@ -662,7 +663,7 @@ __global__ void __launch_bounds__(256) k_i4_sums(const char * x, int64_t x_row, 
     if (row < n_rows && seg % per == 0) {
         uint32_t a, b, c;
         f32_parts(v, a, b, c);
-        sums[row * sums_row + seg / per] = u32x4_t{a | b << 16, a | c << 16, b | a << 16, 0};
+        sums[row * sums_row + seg / per] = u32x4_t{a | b << 16, a | c << 16, b | a << 16, c | b << 16};
     }
 }
 
@@ -907,7 +908,7 @@ __global__ void __launch_bounds__(WM * WN * 64, LIST ? 3 : 2) k_i4_many(const i4
                 const float sz = -i4_scale(zs[j][n], of(n).f16 ? ~0u : 0u) * (float) zz[j][n];
                 uint32_t a, b, c;
                 f32_parts(j * 4 + q < left ? sz : 0.f, a, b, c);
-                zf[n] = __builtin_bit_cast(bf16x8_t, u32x4_t{a | a << 16, b | a << 16, b | c << 16, 0});
+                zf[n] = __builtin_bit_cast(bf16x8_t, u32x4_t{a | a << 16, b | a << 16, b | c << 16, b | c << 16});
             }
 #pragma unroll
             for (int m = 0; m < MT; m++) {
