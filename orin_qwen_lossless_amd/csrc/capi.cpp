@@ -275,7 +275,7 @@ int bf16n_mmv(const bf16n_weight * w, const bf16n_mmv_args * a, void * stream, i
     });
 }
 
-// The kernel instance that the calling thread's last product (bf16n_mmv*, bf16n_mm_ids*, bf16n_add_rmsnorm_mmv) chose, as the profiler prints it
+// The kernel instance that the calling thread's last product (bf16n_mmv*, bf16n_mm_ids*, bf16n_add_rmsnorm_mmv, bf16n_int4_mmv, bf16n_int4_mm_ids) chose, as the profiler prints it
 // ("k_w64_mmv<bf16_t, 4, 1, 2, 1>"); an empty string before the first one or after one on a path that leaves no note.  The pointer stays valid until the thread's next call of this function.
 const char * bf16n_last_kernel(void) {
     const dev::kernel_note & k = dev::g_last_kernel;

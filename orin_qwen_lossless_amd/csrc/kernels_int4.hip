@@ -3,6 +3,7 @@
 #include "launchers.h"
 
 #include <algorithm>
+#include <string>
 
 namespace bf16n {
 namespace dev {
@@ -1174,6 +1175,18 @@ size_t few_lds(int K, int cols, bool f32, int nt, int nm, int groups_per_step, i
 
 constexpr size_t I4_FEW_LDS = 160 * 1024 - 1024;
 
+// a kernel instance's template arguments as a profiler prints them (bf16n_last_kernel)
+std::string text_of(std::initializer_list<int> numbers, std::initializer_list<bool> flags, const char * last = "") {
+    std::string s;
+    for (const int n : numbers) {
+        s += (s.empty() ? "" : ", ") + std::to_string(n);
+    }
+    for (const bool f : flags) {
+        s += f ? ", true" : ", false";
+    }
+    return s + last;
+}
+
 struct few_plan { int nt, grid_y, grid_z, cus; hipStream_t stream; bool raise_limits, small; };
 
 template <int NT, int GM, bool GLU, bool XF32, bool ZEROS>
@@ -1187,6 +1200,8 @@ void launch_few(const i4_launch & p, const few_plan & f) {
     const int block_rows = NW / p.ksplit * 16;
     const int n_blocks = (p.nrows + block_rows - 1) / block_rows;
     if (f.small) {
+        static const std::string text = text_of({NT, GM}, {GLU, XF32, ZEROS});
+        note_kernel("k_i4_small", text.c_str(), 0);
         k_i4_small<NT, GM, GLU, XF32, ZEROS><<<dim3(n_blocks, f.grid_y, f.grid_z), NW * 64, 0, f.stream>>>(p);
         return;
     }
@@ -1195,6 +1210,9 @@ void launch_few(const i4_launch & p, const few_plan & f) {
     // many as give a wavefront eight pairs of steps (77 tokens, 2048 x 512 of 256 experts: 66 us with two, 45 with eight)
     const int room = f.cus * (int) std::min<size_t>(2, LDS_BYTES / lds), steps = (p.K + I4_STEP - 1) / I4_STEP;
     const int rounds = f.grid_y == 1 ? (n_blocks + room - 1) / room : std::max(1, std::min<int>(16 * p.ksplit / steps, (int64_t) n_blocks * f.grid_y / (4 * f.cus)));
+    static const std::string text = text_of({NT, NM, GM}, {GLU, XF32, ZEROS}, ", 8");
+    static_assert(NW == 8, "in the text");
+    note_kernel("k_i4_few", text.c_str(), 0);
     kernel<<<dim3((n_blocks + rounds - 1) / rounds, f.grid_y, f.grid_z), NW * 64, lds, f.stream>>>(p);
 }
 
@@ -1231,6 +1249,8 @@ void launch_many(const i4_many * p, bool glu, unsigned blocks, hipStream_t strea
     constexpr int LDS = (int) many_lds(WM * MT * 16, WN * NT * 16, LIST);
     const auto kernel = glu ? k_i4_many<WM, WN, MT, NT, GM, true, LIST> : k_i4_many<WM, WN, MT, NT, GM, false, LIST>;
     if (p) {
+        static const std::string text[2] = {text_of({WM, WN, MT, NT, GM}, {false, LIST}), text_of({WM, WN, MT, NT, GM}, {true, LIST})};
+        note_kernel("k_i4_many", text[glu].c_str(), 0);
         kernel<<<blocks, 256, LDS, stream>>>(*p);
     } else {
         (void) hipFuncSetAttribute((const void *) kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
