@@ -154,3 +154,43 @@ def test_columns_by_ids(ops, kernel, N, group, zeros, dtype, glu):
                 if glu:
                     y, b = X.gated(y, b, *X.product(xi, cut(w2, e)))
                 X.check(got[t, i: i + 1], y, b, (t, i))
+
+
+def test_activation_rows_too_far_apart_for_the_kernel_of_many_columns(ops):
+    """Its places of activations are 32 bits: a product that it would take otherwise goes to the kernels for few, dense and by lists."""
+    import ctypes as C
+
+    from orin_qwen_lossless_amd import _lib
+
+    w, dw = weight(ops, 8300, 416, 32, 440)
+    x = acts(70, 416, 441)
+    y, b = X.product(x, w)
+    X.check(ops.int4_mmv(x.cuda(), dw), y, b)
+    assert ops.last_kernel().startswith("k_i4_many<")
+    space = torch.empty(70 * 35_000_000, dtype=torch.bfloat16, device="cuda")
+    far = space.as_strided((70, 416), (35_000_000, 1))
+    far.copy_(x)
+    X.check(ops.int4_mmv(far, dw), y, b)
+    assert ops.last_kernel().startswith(("k_i4_few<", "k_i4_small<"))
+
+    E, N, K, T = 2, 165, 160, 40
+    w, dw = weight(ops, E * N, K, 64, 442)
+    x = acts(T, K, 443)
+    ids = ids_of([25, 10], 1, E, 444)
+    pairs, bounds = ops.int4_route(ids.cuda(), E)
+    cw, out = ops._c_int4(dw), {}
+    for apart in (K, 60_000_000):
+        rows = space.as_strided((T, K), (apart, 1))
+        rows.copy_(x)
+        got = torch.empty((T, N), device="cuda")
+        ws = ops._int4_workspace(cw, T, got.device, T, E)
+        _lib.check(_lib.lib().bf16n_int4_mm_ids(C.byref(cw), None, rows.data_ptr(), apart, 0, pairs.data_ptr(), bounds.data_ptr(), got.data_ptr(), 0, N, E, T, 1,
+                                                ws.data_ptr(), ws.numel(), ops._stream()))
+        assert ops.last_kernel().startswith("k_i4_many<") == (apart == K)
+        for t in range(T):
+            e = int(ids[t, 0])
+            if 0 <= e < E:
+                y, b = X.product(x[t: t + 1], (*(p[e * N: e * N + N] for p in w[:3]), 64))
+                X.check(got[t: t + 1], y, b, (apart, t))
+            else:
+                assert not got[t].any()
