@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
 
         // Activations into LDS, in the operands' order, zeros behind the last column of the matrix, and their groups' sums: a
         // wavefront takes 512 columns of a row at a time and has AHEAD such pieces on the way.  (One after the other cost a latency
-        // each: 16 tokens of 5120 x 2048 11.9 us, now 10.6.)
+        // each: 16 tokens of 5120 x 2048 in this kernel 11.9 us, now 10.8.)
         constexpr int AHEAD = XF32 ? 2 : 4;
         const int octs = (pitch - 8) / 8; // a multiple of 16: a row of 16 lanes has 128 columns of one activation row
         const int per_row = (octs + 63) / 64, pieces = p.cols_per_pass * per_row;
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(NW * 64, NT * NM > 2 ? 2 : 4) k_i4_few(const i
 // Few columns of a matrix whose rows are few as well: nothing is shared through LDS but the sums of the parts of K.  A
 // wavefront loads its codes, scales and activations, these as the operand's lanes hold them, at once, one latency in
 // all; the groups' sums of the activations come from products with ones.
-// 512 x 2048, one token: 4.1 us in a graph, 5.5 with the activations through LDS; 1453 x 2560, gated, groups of 32, 11 tokens 7.8 / 14.3.  Bound by that latency.
+// 512 x 2048, one token: 4.1 us in a graph, 5.8 with the activations through LDS; 1453 x 2560, gated, groups of 32, 11 tokens 7.8 / 14.5.  Bound by that latency.
 template <int NT, int GM, bool GLU, bool XF32, bool ZEROS>
 __global__ void __launch_bounds__(512, 2) k_i4_small(const i4_launch p) {
     constexpr int NW = 8, NM = GLU ? 2 : 1, NG = GM == 0 ? 1 : GM == 1 ? 2 : 4, CPT = XF32 ? 4 : 16, NA = XF32 ? 1 : 4;
@@ -689,8 +689,8 @@ struct i4_many {
 // at a time: the activations' piece and the codes go straight into LDS a step ahead (two buffers, 16-byte places exchanged by the row's
 // low bits so that the operands' reads find every bank); a wavefront turns its own codes into operands, which serve MT tiles.  Every product over a group starts from zero and is added to the result times its scale.
 // Bound by the vector instructions (nine for eight codes and tile of rows, four for a tile of results and group), the products and the
-// reads of LDS, which take turns more than they overlap: 8192 tokens of 8192 x 2048 reach 790 TFLOP/s, 2048 of 5120 x 2048 700.  (Without
-// the additions, without the conversions and without three of four products 302, 276 and 228 us of 313 remained.)  Making the next
+// reads of LDS, which take turns more than they overlap: 8192 tokens of 8192 x 2048 take 332 us, 830 TFLOP/s, 2048 of 5120 x 2048 64, 670.
+// (Of the 332 us without the additions 294 remained, without the conversions 309, without three of four products 234.)  Making the next
 // operands under this step's products, with a step's copies spread over it, came to the same times.
 template <int WM, int WN, int MT, int NT, int GM, bool GLU, bool LIST>
 __global__ void __launch_bounds__(WM * WN * 64, LIST ? 3 : 2) k_i4_many(const i4_many p) {
@@ -734,7 +734,7 @@ __global__ void __launch_bounds__(WM * WN * 64, LIST ? 3 : 2) k_i4_many(const i4
     } else {
         // An XCD takes every eighth block, which is made a contiguous part of the tiles here: four column tiles of one row tile
         // after the other, so that what runs there at a time shares few pieces of activations (four times a row tile's bytes).
-        // 8192 x 2048, 8192 tokens: 391 us where all column tiles of a row tile side by side took 428.
+        // 8192 x 2048, 8192 tokens: 332 us where all column tiles of a row tile side by side take 373.
         const int n = p.row_tiles * p.col_tiles, per = (n + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
         if (id >= n) {
             return;
@@ -1069,7 +1069,8 @@ __global__ void __launch_bounds__(WM * WN * 64, LIST ? 3 : 2) k_i4_many(const i4
     // Lists: where a step is within a group, its loop ends at the last tile that has columns.  With smaller groups the branches cost so many
     // registers that two blocks are on a CU where three could be: there two tiles or all four, the columns that are not there along
     // with the others and then left out.  256 experts, 2048 tokens, groups of 64 337 -> 298 us, 32 424 -> 373; 700 tokens, 64 199 -> 171; but groups
-    // of 128, 2048 tokens 258 -> 266
+    // of 128, 2048 tokens 258 -> 266.  (With the branches held to three blocks: groups of 64 295
+    // and, 700 tokens, 177; groups of 32 1303, the registers spill.)
     if (LIST && GM && mt <= 2) {
         run(std::integral_constant<int, 2>());
     } else {
@@ -1328,7 +1329,7 @@ void run_few(i4_launch & p, bool glu, bool f32, bool zeros, int max_cols, int64_
     p.ksplit = ksplit;
     const int passes = p.bounds || p.ids ? 1 : std::min(65535, (max_cols + p.cols_per_pass - 1) / p.cols_per_pass);
     // the kernel without activations in LDS: up to two tiles of rows for a CU (one with FP32 activations, whose lanes part them
-    // themselves).  us, with it / without, BF16, 16 tokens: 5120 x 2048 9.2 / 10.6, 10240 x 2048 15.6 / 11.4; FP32, three: 8192 x 2048 14.4 / 8.9
+    // themselves).  us, with it / without, BF16, 16 tokens: 5120 x 2048 9.4 / 10.8, 10240 x 2048 14.5 / 11.7; FP32, three: 8192 x 2048 12.7 / 8.7
     const bool small = tiles <= (f32 ? 1 : 2) * cus;
     pick_few(p, glu, f32, gm, zeros, {nt, grid_y, passes, cus, stream, false, small});
 }
@@ -1352,8 +1353,8 @@ void launch_int4_mmv(const bf16n_int4_weight & w, const bf16n_int4_weight * up, 
                      uint64_t workspace_bytes, int cus, hipStream_t stream) {
     // Many columns where one pass of 32 is not all and the matrix has rows enough: its kernel takes 1.1 us a step however few its
     // blocks are (one and a half to a CU add nothing), a pass of 32 columns over 16 rows costs 1 / 800 of that on a whole device.
-    // us, many / few: 5120 x 2048, 64 tokens 25.0 / 18.8, 200 25.9 / 50; 233 x 5440, 125 50 / 9.4; 512 x 2048, 512 25.1 / 15.3, 2048 26.6 / 49;
-    // 20000 x 2048, 64 25.9 / 36.9
+    // us, many / few: 5120 x 2048, 64 tokens 24.1 / 18.6, 200 25.3 / 50; 233 x 5440, 125 50 / 9.4; 512 x 2048, 512 24.1 / 15.0, 2048 25.7 / 49;
+    // 20000 x 2048, 64 24.6 / 36.8
     const int64_t units = (a.nrows + 15) / 16 * ((a.ncols + 31) / 32), blocks = (a.nrows + 127) / 128 * ((a.ncols + 63) / 64);
     const int64_t rounds = std::max<int64_t>(1, 2 * blocks / (3 * cus)), steps = (w.K + I4_STEP - 1) / I4_STEP;
     if (!a.ids && a.x_bf16 && a.ncols > 32 && units > 800 * rounds + 2200 / steps && a.x_tok >= 0 && a.ncols * a.x_tok < (int64_t) 1 << 32 && (int64_t) workspace_bytes >= int4_workspace_bytes(w, a.ncols, 0, 0)) {
@@ -1364,7 +1365,7 @@ void launch_int4_mmv(const bf16n_int4_weight & w, const bf16n_int4_weight * up, 
         p.ncols = a.ncols;
         p.n_matrices = 1;
         // tiles of 128 x 128 (two blocks to a CU) where they make two rounds, of 128 x 64 (three) below: 5120 x 2048, 2048 tokens, 640
-        // tiles, 82.9 / 73.9 us, 4096 x 2048, 4096 tokens, 1024 tiles, 96.6 / 106.7
+        // tiles, 77.7 / 69.3 us, 4096 x 2048, 4096 tokens, 1024 tiles, 94.0 / 98.9
         const int64_t tiles = ((a.nrows + 127) / 128) * ((a.ncols + 127) / 128);
         run_many(w, up, p, a.ncols, workspace, tiles >= 4 * cus ? 128 : 64, stream);
         return;
@@ -1398,8 +1399,8 @@ void launch_int4_mm_ids(const bf16n_int4_weight & w, const bf16n_int4_weight * u
                         int cus, hipStream_t stream) {
     const int64_t x_rows = per_slot ? (int64_t) n_tok * n_used : n_tok;
     const int64_t n_pairs = (int64_t) n_tok * n_used;
-    // many columns from 12 pairs to a matrix on.  256 experts, top-8, us with them / without: 300 tokens 142 / 131, 400 146 / 151, 512 153 / 176
-    if (n_pairs > 12 * (int64_t) n_matrices &&  x_row >= 0 && x_rows * x_row < (int64_t) 1 << 31 && (int64_t) workspace_bytes >= int4_workspace_bytes(w, x_rows, n_pairs, n_matrices)) {
+    // many columns from 12 pairs to a matrix on.  256 experts, top-8, us with them / without: 300 tokens 135 / 131, 400 140 / 150, 512 149 / 177
+    if (n_pairs > 12 * (int64_t) n_matrices && x_row >= 0 && x_rows * x_row < (int64_t) 1 << 31 && (int64_t) workspace_bytes >= int4_workspace_bytes(w, x_rows, n_pairs, n_matrices)) {
         i4_many p = {};
         p.x = (const char *) x; p.x_row = x_row * 2;
         p.y = (char *) y; p.y_row = y_row * (y_bf16 ? 2 : 4); p.y_bf16 = y_bf16;
