@@ -94,7 +94,7 @@ def _rows(v: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     t, k = v.shape
     blocks = torch.nn.functional.pad(v, (0, -k % BLOCK)).view(t, -1, BLOCK)
     m = blocks.abs().amax(2).clamp_min(SMALLEST)
-    q = (blocks * (LARGEST / m)[:, :, None]).to(E4M3)
+    q = (blocks * (torch.full_like(m, LARGEST) / m)[:, :, None]).to(E4M3)  # (a number over a tensor is a product with its reciprocal)
     return q.view(t, -1)[:, :k].contiguous(), m / LARGEST
 
 
@@ -251,7 +251,7 @@ def _in_blocks(v: torch.Tensor):
     for c in range(0, k, BLOCK):
         b = v[:, c: c + BLOCK]
         m = b.abs().max(1, keepdim=True).values.clamp_min(SMALLEST).float()
-        codes.append(_to_grid((b.float() * (LARGEST / m)).double()))
+        codes.append(_to_grid((b.float() * torch.true_divide(torch.tensor(LARGEST, device=m.device).expand_as(m), m)).double()))
         scales.append((m / LARGEST).double())
     return torch.cat(codes, 1), torch.cat(scales, 1)
 
