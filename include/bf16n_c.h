@@ -227,6 +227,61 @@ int bf16n_router_topk_grouped(const float * logits, int64_t logits_stride, const
                               int topk_groups, int k, int sigmoid, int top2, int renorm, float scale, int32_t * ids, float * weights,
                               int64_t out_stride, void * stream);
 
+/* ---- 8-bit floating point (e4m3) with a scale for every block of 128 (lossy; no counterpart in the reference) ---- */
+/*   w[r, k] = scales[r / 128, k / 128] * codes[r, k]
+ * codes: [rows, K] bytes of e4m3 (OCP: no infinities, 0x7F and 0xFF are NaN), 16-byte aligned device memory; n_matrices matrices of
+ * rows / n_matrices rows behind one another.  scales: FP32 (or BF16 with scales_bf16), [n_matrices * ceil(rows of one / 128),
+ * ceil(K / 128)]: blocks begin anew in every matrix, its last ones may be cut short.  K: a multiple of 16 in [16, 32768]. */
+typedef struct bf16n_fp8_weight {
+    const uint8_t * codes;
+    const void * scales;
+    int64_t K, rows, n_matrices;
+    int32_t scales_bf16, pad_;
+} bf16n_fp8_weight;
+/* Rows of activations or results.  kind: codes with a scale for every 128 columns, scales[r * scale_row + b * scale_block] (strides in
+ * elements), or BF16, or FP32 (no scales).  row: bytes between rows.  Read: at 16-byte aligned, row a multiple of 16.  Written:
+ * aligned to the elements (codes: to 16 bytes).  The codes of a block v are e4m3(v * (448 / m)), to nearest even, its scale is
+ * m / 448, m = max(max |v|, 2^-100); quotients and product are FP32.  A NaN has the code NaN; a block with an infinity has an
+ * infinite scale, so that a product with it is NaN throughout. */
+enum { BF16N_FP8_CODES = 0, BF16N_FP8_BF16 = 1, BF16N_FP8_F32 = 2 };
+typedef struct bf16n_fp8_rows {
+    void * at;
+    float * scales;
+    int64_t row, scale_row, scale_block;
+    int32_t kind, pad_;
+} bf16n_fp8_rows;
+/* BF16 or FP32 rows of K values (a multiple of 16 in [16, 32768]) as codes with scales. */
+int bf16n_fp8_quantize_rows(const bf16n_fp8_rows * x, const bf16n_fp8_rows * y, int64_t n_rows, int64_t K, void * stream);
+/* bf16n_add_rmsnorm with the norm in 8 bits: the FP32 value is rounded once, to its code.  y_sum (BF16 sum), y_norm (BF16 norm beside the
+ * codes) may be null.  n: a multiple of 16, at most 16384; every pointer 16-byte aligned. */
+int bf16n_add_rmsnorm_fp8(const uint16_t * a, const uint16_t * b, const uint16_t * c, const float * ys, const void * wts, int wts_bf16, int n_used,
+                          const uint16_t * gamma, const bf16n_fp8_rows * y, uint16_t * y_sum, uint16_t * y_norm, int n_tok, int64_t n, float eps,
+                          void * stream);
+/* y = W x per row of x: sums over a block of 128 columns on the matrix cores, scaled and added up in FP32.  up given: silu(W x) * (up x)
+ * (w and up of one shape).  Rows of x that are not codes are taken as what bf16n_fp8_quantize_rows makes of them.  y: BF16, FP32, or with
+ * up codes (rows of W a multiple of 16 then).  w has one matrix.  workspace: bf16n_fp8_workspace_bytes, 16-byte aligned (null if
+ * that is 0).  The result must not overlap x. */
+int bf16n_fp8_mm(const bf16n_fp8_weight * w, const bf16n_fp8_weight * up, const bf16n_fp8_rows * x, const bf16n_fp8_rows * y, int64_t n_rows,
+                 void * workspace, uint64_t workspace_bytes, void * stream);
+/* *bytes of workspace for bf16n_fp8_mm (n_pairs = 0) or bf16n_fp8_mm_ids (n_pairs = n_tok * n_used; listed: with pairs and bounds) */
+int bf16n_fp8_workspace_bytes(const bf16n_fp8_weight * w, int gate_up, int x_kind, int y_kind, int64_t x_rows, int64_t n_pairs, int listed,
+                              uint64_t * bytes);
+/* The same by matrix: row pair of y = W_e x for every (token, slot) pair t * n_used + slot, e its id; rows of zeros where an id names no
+ * matrix.  pairs, bounds: bf16n_int4_route's lists for the ids, or both null: every pair by itself (at most 65535).  x: a row for every
+ * token or, with per_slot, for every pair.  ids strides in bytes. */
+int bf16n_fp8_mm_ids(const bf16n_fp8_weight * w, const bf16n_fp8_weight * up, const bf16n_fp8_rows * x, int per_slot, const void * ids, int ids_i64,
+                     int64_t ids_s0, int64_t ids_s1, const int32_t * pairs, const int32_t * bounds, const bf16n_fp8_rows * y, int n_tok, int n_used,
+                     void * workspace, uint64_t workspace_bytes, void * stream);
+/* The routed experts of a layer: y[t] = sum over the slots of wts[t, slot] * down_e(silu(gate_e x[t]) * (up_e x[t])), hidden rows held in 8
+ * bits (from FP32 values), the slots' results in FP32 or, where the pairs are more than the experts, in BF16 (half a step each, at most
+ * 2^-9 of a slot's result, beside the 2^-4 of the codes).  wts null: y has a row of FP32 for every pair, unweighted.  wts: FP32 or BF16
+ * [n_tok, n_used].  y: BF16 or FP32, contiguous rows. */
+int bf16n_fp8_moe_experts(const bf16n_fp8_weight * gate, const bf16n_fp8_weight * up, const bf16n_fp8_weight * down, const bf16n_fp8_rows * x,
+                          const void * ids, int ids_i64, int64_t ids_s0, int64_t ids_s1, const void * wts, int wts_bf16, const bf16n_fp8_rows * y,
+                          int n_tok, int n_used, void * workspace, uint64_t workspace_bytes, void * stream);
+int bf16n_fp8_moe_experts_workspace_bytes(const bf16n_fp8_weight * gate, const bf16n_fp8_weight * down, int x_kind, int weighted, int n_tok, int n_used,
+                                          uint64_t * bytes);
+
 /* ---- load-time conversion and the registry of resident tensors: the reference's llama.cpp adapter without ggml types
  * (engines/llamacpp/patches/0002-ggml-cuda-thin-BF16N-adapter-over-the-shared-core.patch).  An engine stores a converted
  * tensor as rows * K bytes of device memory (the plane); the aux buffer is allocated here and found again by the

@@ -30,9 +30,20 @@ class Int4Weight(C.Structure):
                 ("group", C.c_int32), ("scales_f16", C.c_int32)]
 
 
+class Fp8Weight(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("K", C.c_int64), ("rows", C.c_int64), ("n_matrices", C.c_int64),
+                ("scales_bf16", C.c_int32), ("pad_", C.c_int32)]
+
+
+class Fp8Rows(C.Structure):
+    _fields_ = [("at", C.c_void_p), ("scales", C.c_void_p), ("row", C.c_int64), ("scale_row", C.c_int64), ("scale_block", C.c_int64),
+                ("kind", C.c_int32), ("pad_", C.c_int32)]
+
+
 # name -> (restype, argtypes); every symbol declared in include/bf16n_c.h
 _i, _i64, _u32, _vp, _cp = C.c_int, C.c_int64, C.c_uint32, C.c_void_p, C.c_char_p
 _WP, _AP, _QP = C.POINTER(Weight), C.POINTER(MmvArgs), C.POINTER(Int4Weight)
+_FP, _RP, _U64P = C.POINTER(Fp8Weight), C.POINTER(Fp8Rows), C.POINTER(C.c_uint64)
 SYMBOLS = {
     "bf16n_last_error": (_cp, []),
     "bf16n_last_kernel": (_cp, []),
@@ -74,6 +85,13 @@ SYMBOLS = {
     "bf16n_int4_route": (_i, [_vp, _i, _i64, _i64, _i, _i, _i, _vp, _vp, _vp]),
     "bf16n_int4_mm_ids": (_i, [_QP, _QP, _vp, _i64, _i, _vp, _vp, _vp, _i, _i64, _i, _i, _i, _vp, C.c_uint64, _vp]),
     "bf16n_router_topk_grouped": (_i, [_vp, _i64, _vp, _i, _i, _i, _i, _i, _i, _i, _i, C.c_float, _vp, _vp, _i64, _vp]),
+    "bf16n_fp8_quantize_rows": (_i, [_RP, _RP, _i64, _i64, _vp]),
+    "bf16n_add_rmsnorm_fp8": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _RP, _vp, _vp, _i, _i64, C.c_float, _vp]),
+    "bf16n_fp8_mm": (_i, [_FP, _FP, _RP, _RP, _i64, _vp, C.c_uint64, _vp]),
+    "bf16n_fp8_workspace_bytes": (_i, [_FP, _i, _i, _i, _i64, _i64, _i, _U64P]),
+    "bf16n_fp8_mm_ids": (_i, [_FP, _FP, _RP, _i, _vp, _i, _i64, _i64, _vp, _vp, _RP, _i, _i, _vp, C.c_uint64, _vp]),
+    "bf16n_fp8_moe_experts": (_i, [_FP, _FP, _FP, _RP, _vp, _i, _i64, _i64, _vp, _i, _RP, _i, _i, _vp, C.c_uint64, _vp]),
+    "bf16n_fp8_moe_experts_workspace_bytes": (_i, [_FP, _FP, _i, _i, _i, _i, _U64P]),
     "bf16n_adapter_choose": (_i, [_i64, _i64, _i64, _cp, _i64, _i, _i]),
     "bf16n_adapter_convert": (_i, [_vp, _vp, _i64, _i64, _i64, _i, _i, _i, _vp, _cp, _i, C.POINTER(_i)]),
     "bf16n_verify_roundtrip": (_i, [_WP, _vp, C.POINTER(_i)]),

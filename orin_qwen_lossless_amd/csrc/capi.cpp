@@ -82,6 +82,7 @@ per_device & ensure_init() {
         dev::mm_ids_init();
         dev::tile_init();
         dev::int4_init();
+        dev::fp8_init();
         void * p = nullptr;
         hip_check(hipGetSymbolAddress(&p, HIP_SYMBOL(scratch)), "hipGetSymbolAddress (routing lists)");
         d.lists = static_cast<route_lists *>(p);
@@ -275,7 +276,7 @@ int bf16n_mmv(const bf16n_weight * w, const bf16n_mmv_args * a, void * stream, i
     });
 }
 
-// The kernel instance that the calling thread's last product (bf16n_mmv*, bf16n_mm_ids*, bf16n_add_rmsnorm_mmv, bf16n_int4_mmv, bf16n_int4_mm_ids) chose, as the profiler prints it
+// The kernel instance that the calling thread's last product (bf16n_mmv*, bf16n_mm_ids*, bf16n_add_rmsnorm_mmv, bf16n_int4_mmv, bf16n_int4_mm_ids, bf16n_fp8_mm*) chose, as the profiler prints it
 // ("k_w64_mmv<bf16_t, 4, 1, 2, 1>"); an empty string before the first one or after one on a path that leaves no note.  The pointer stays valid until the thread's next call of this function.
 const char * bf16n_last_kernel(void) {
     const dev::kernel_note & k = dev::g_last_kernel;
@@ -805,6 +806,236 @@ int bf16n_router_topk_grouped(const float * logits, int64_t logits_stride, const
                                       ids, weights, out_stride};
         dev::launch_router_topk_grouped(a, n_tok, (hipStream_t) stream);
         launch_check("router_topk_grouped");
+    });
+}
+
+// ---------------------------------------------------------------- 8-bit floating point with a scale for every block of 128
+
+namespace {
+
+constexpr int64_t FP8_MAX_ROWS = 1 << 26, FP8_MAX_COLS = 1 << 28;
+
+void check_fp8(const bf16n_fp8_weight * w, const bf16n_fp8_weight * up) {
+    require(w != nullptr, "fp8: null weight");
+    for (const bf16n_fp8_weight * m : {w, up}) {
+        if (!m) {
+            continue;
+        }
+        require(m->K % 16 == 0 && m->K >= 16 && m->K <= 32768, "fp8: K must be a multiple of 16 in [16, 32768]");
+        require(m->n_matrices > 0 && m->n_matrices <= 65534 && m->rows >= 0 && m->rows % m->n_matrices == 0 && m->rows / m->n_matrices <= FP8_MAX_ROWS,
+                "fp8: rows must split into n_matrices (at most 65534, of at most 2^26 rows)");
+        require(m->rows == 0 || (m->codes && m->scales), "fp8: null codes or scales");
+        require(((uintptr_t) m->codes & 15) == 0 && ((uintptr_t) m->scales & (m->scales_bf16 ? 1 : 3)) == 0, "fp8: codes must be 16-byte aligned, scales to their elements");
+    }
+    require(!up || (up->K == w->K && up->rows == w->rows && up->n_matrices == w->n_matrices && !up->scales_bf16 == !w->scales_bf16), "fp8: gate/up shapes and scales must match");
+}
+
+void check_rows_in(const bf16n_fp8_rows * x) {
+    require(x && x->at, "fp8: null activations");
+    require(x->kind >= BF16N_FP8_CODES && x->kind <= BF16N_FP8_F32, "fp8: rows are codes, BF16 or FP32");
+    require(((uintptr_t) x->at & 15) == 0 && x->row % 16 == 0, "fp8: activations must be 16-byte aligned with 16-byte row strides");
+    require(x->kind != BF16N_FP8_CODES || (x->scales && ((uintptr_t) x->scales & 3) == 0), "fp8: codes need FP32 scales");
+}
+void check_rows_out(const bf16n_fp8_rows * y, int64_t n, bool codes) {
+    require(y && y->at, "fp8: null result");
+    require(y->kind == BF16N_FP8_BF16 || y->kind == BF16N_FP8_F32 || (codes && y->kind == BF16N_FP8_CODES), "fp8: results are BF16 or FP32 (gated ones may be codes)");
+    const int64_t el = y->kind == BF16N_FP8_CODES ? 16 : y->kind == BF16N_FP8_BF16 ? 2 : 4;
+    require((uintptr_t) y->at % el == 0 && y->row % el == 0, "fp8: results must be aligned to their elements, codes to 16 bytes");
+    if (y->kind == BF16N_FP8_CODES) {
+        require(y->scales && ((uintptr_t) y->scales & 3) == 0, "fp8: codes need FP32 scales");
+        require(n % 16 == 0, "fp8: results that are codes need a multiple of 16 rows in the matrix");
+    }
+}
+void check_workspace(const void * workspace, uint64_t have, uint64_t need) {
+    require(((uintptr_t) workspace & 15) == 0, "fp8: the workspace must be 16-byte aligned");
+    require(need == 0 || (workspace && have >= need), "fp8: the workspace is too small");
+}
+
+struct experts_plan { // offsets in the workspace
+    bool listed;
+    bool half; // slots' results in BF16
+    uint64_t lists, hidden, hidden_scales, ys, product, bytes;
+};
+experts_plan plan_experts(const bf16n_fp8_weight & gate, const bf16n_fp8_weight & down, int x_kind, bool weighted, int n_tok, int n_used) {
+    const int64_t pairs = (int64_t) n_tok * n_used, mid = gate.rows / gate.n_matrices, out = down.rows / down.n_matrices;
+    experts_plan e = {};
+    const auto take = [&](uint64_t & at, uint64_t n) {
+        at = e.bytes;
+        e.bytes += (n + 255) / 256 * 256;
+    };
+    // while the pairs are no more than the experts each is a column by itself
+    e.listed = pairs > gate.n_matrices;
+    e.half = e.listed && weighted && out % 8 == 0;
+    if (e.listed) {
+        take(e.lists, (pairs + gate.n_matrices + 2) * 4);
+        take(e.hidden_scales, pairs * ((mid + 127) / 128) * 4);
+    }
+    take(e.hidden, pairs * mid * (e.listed ? 1 : 4));
+    if (weighted) {
+        take(e.ys, pairs * out * (e.half ? 2 : 4));
+    }
+    const uint64_t a = dev::fp8_workspace_bytes(gate, true, x_kind, e.listed ? BF16N_FP8_CODES : BF16N_FP8_F32, n_tok, pairs, e.listed, !e.listed);
+    const uint64_t b = dev::fp8_workspace_bytes(down, false, e.listed ? BF16N_FP8_CODES : BF16N_FP8_F32, BF16N_FP8_F32, pairs, pairs, e.listed, !e.listed);
+    take(e.product, a > b ? a : b);
+    return e;
+}
+void check_experts(const bf16n_fp8_weight * gate, const bf16n_fp8_weight * up, const bf16n_fp8_weight * down, int n_tok, int n_used) {
+    check_fp8(gate, up);
+    check_fp8(down, nullptr);
+    require(down->n_matrices == gate->n_matrices && down->K == gate->rows / gate->n_matrices, "fp8_moe_experts: down takes the rows of gate and up, of as many experts");
+    require(n_tok > 0 && n_tok <= 65535 && n_used > 0 && n_used < 1024, "fp8_moe_experts: sizes out of range");
+}
+
+} // namespace
+
+int bf16n_fp8_quantize_rows(const bf16n_fp8_rows * x, const bf16n_fp8_rows * y, int64_t n_rows, int64_t K, void * stream) {
+    return guarded([&] {
+        ensure_init();
+        require(K % 16 == 0 && K >= 16 && K <= 32768 && n_rows > 0 && n_rows <= FP8_MAX_COLS, "fp8_quantize_rows: K must be a multiple of 16 in [16, 32768], rows 1 to 2^28");
+        check_rows_in(x);
+        require(x->kind != BF16N_FP8_CODES && y && y->kind == BF16N_FP8_CODES, "fp8_quantize_rows: BF16 or FP32 rows become codes");
+        check_rows_out(y, 0, true);
+        dev::launch_fp8_rows(*x, *y, n_rows, K, g_cus, (hipStream_t) stream);
+        launch_check("fp8_quantize_rows");
+    });
+}
+
+int bf16n_add_rmsnorm_fp8(const uint16_t * a, const uint16_t * b, const uint16_t * c, const float * ys, const void * wts, int wts_bf16, int n_used,
+                          const uint16_t * gamma, const bf16n_fp8_rows * y, uint16_t * y_sum, uint16_t * y_norm, int n_tok, int64_t n, float eps,
+                          void * stream) {
+    return guarded([&] {
+        ensure_init();
+        require(a && n_tok > 0 && n > 0 && n % 16 == 0 && n <= 16384, "add_rmsnorm_fp8: null pointer, empty input, or n no multiple of 16 up to 16384");
+        require(!ys || (wts && n_used > 0 && n_used < 1024), "add_rmsnorm_fp8: rows to combine need weights and a slot count below 1024");
+        require((((uintptr_t) a | (uintptr_t) b | (uintptr_t) c | (uintptr_t) ys | (uintptr_t) gamma | (uintptr_t) y_sum | (uintptr_t) y_norm) & 15) == 0,
+                "add_rmsnorm_fp8: rows must be 16-byte aligned");
+        require(y && y->kind == BF16N_FP8_CODES, "add_rmsnorm_fp8: the norm is codes with scales");
+        check_rows_out(y, 0, true);
+        dev::add_norm_args p{};
+        p.a = a; p.b = b; p.c = c; p.ys = ys; p.wts = wts; p.wts_bf16 = wts_bf16 != 0; p.n_used = n_used;
+        p.gamma = gamma; p.y_sum = y_sum; p.y_norm = y_norm; p.n = n; p.eps = eps;
+        dev::launch_add_rmsnorm_fp8(p, *y, n_tok, (hipStream_t) stream);
+        launch_check("add_rmsnorm_fp8");
+    });
+}
+
+int bf16n_fp8_workspace_bytes(const bf16n_fp8_weight * w, int gate_up, int x_kind, int y_kind, int64_t x_rows, int64_t n_pairs, int listed, uint64_t * bytes) {
+    return guarded([&] {
+        check_fp8(w, nullptr);
+        require(bytes && x_rows >= 0 && n_pairs >= 0, "fp8_workspace_bytes: null pointer or negative sizes");
+        *bytes = dev::fp8_workspace_bytes(*w, gate_up != 0, x_kind, y_kind, x_rows, n_pairs ? n_pairs : x_rows, n_pairs && listed, n_pairs && !listed);
+    });
+}
+
+int bf16n_fp8_mm(const bf16n_fp8_weight * w, const bf16n_fp8_weight * up, const bf16n_fp8_rows * x, const bf16n_fp8_rows * y, int64_t n_rows,
+                 void * workspace, uint64_t workspace_bytes, void * stream) {
+    return guarded([&] {
+        ensure_init();
+        dev::g_last_kernel.name = nullptr;
+        check_fp8(w, up);
+        require(w->n_matrices == 1, "fp8_mm: one matrix");
+        require(n_rows > 0 && n_rows <= FP8_MAX_COLS, "fp8_mm: rows out of range");
+        if (w->rows == 0) {
+            return;
+        }
+        check_rows_in(x);
+        check_rows_out(y, w->rows, up != nullptr);
+        check_workspace(workspace, workspace_bytes, dev::fp8_workspace_bytes(*w, up != nullptr, x->kind, y->kind, n_rows, n_rows, false, false));
+        dev::fp8_product a = {};
+        a.w = w; a.up = up; a.x = *x; a.y = *y; a.x_rows = a.n_cols = n_rows; a.per_token = a.n_used = 1;
+        dev::launch_fp8_product(a, workspace, g_cus, (hipStream_t) stream);
+        launch_check("fp8_mm");
+    });
+}
+
+int bf16n_fp8_mm_ids(const bf16n_fp8_weight * w, const bf16n_fp8_weight * up, const bf16n_fp8_rows * x, int per_slot, const void * ids, int ids_i64,
+                     int64_t ids_s0, int64_t ids_s1, const int32_t * pairs, const int32_t * bounds, const bf16n_fp8_rows * y, int n_tok, int n_used,
+                     void * workspace, uint64_t workspace_bytes, void * stream) {
+    return guarded([&] {
+        ensure_init();
+        dev::g_last_kernel.name = nullptr;
+        check_fp8(w, up);
+        require(n_tok > 0 && n_used > 0 && (int64_t) n_tok * n_used <= FP8_MAX_COLS, "fp8_mm_ids: sizes out of range");
+        require(!pairs == !bounds, "fp8_mm_ids: pairs and bounds, or neither");
+        const int64_t n = (int64_t) n_tok * n_used, x_rows = per_slot ? n : n_tok, ib = ids_i64 ? 8 : 4;
+        require(pairs || n <= 65535, "fp8_mm_ids: at most 65535 pairs without lists");
+        if (w->rows == 0) {
+            return;
+        }
+        require(pairs || (ids && (uintptr_t) ids % ib == 0 && ids_s0 % ib == 0 && ids_s1 % ib == 0), "fp8_mm_ids: ids must be aligned to their elements");
+        check_rows_in(x);
+        check_rows_out(y, w->rows / w->n_matrices, up != nullptr);
+        check_workspace(workspace, workspace_bytes, dev::fp8_workspace_bytes(*w, up != nullptr, x->kind, y->kind, x_rows, n, pairs != nullptr, !pairs));
+        dev::fp8_product a = {};
+        a.w = w; a.up = up; a.x = *x; a.y = *y; a.x_rows = x_rows; a.n_cols = n; a.per_token = per_slot ? 1 : n_used; a.n_used = n_used;
+        a.pairs = pairs; a.bounds = bounds;
+        if (!pairs) {
+            a.ids = ids; a.ids_i64 = ids_i64 != 0; a.ids_s0 = ids_s0; a.ids_s1 = ids_s1;
+        }
+        dev::launch_fp8_product(a, workspace, g_cus, (hipStream_t) stream);
+        launch_check("fp8_mm_ids");
+    });
+}
+
+int bf16n_fp8_moe_experts_workspace_bytes(const bf16n_fp8_weight * gate, const bf16n_fp8_weight * down, int x_kind, int weighted, int n_tok, int n_used, uint64_t * bytes) {
+    return guarded([&] {
+        check_experts(gate, nullptr, down, n_tok, n_used);
+        require(bytes != nullptr, "fp8_moe_experts_workspace_bytes: null pointer");
+        *bytes = plan_experts(*gate, *down, x_kind, weighted != 0, n_tok, n_used).bytes;
+    });
+}
+
+int bf16n_fp8_moe_experts(const bf16n_fp8_weight * gate, const bf16n_fp8_weight * up, const bf16n_fp8_weight * down, const bf16n_fp8_rows * x,
+                          const void * ids, int ids_i64, int64_t ids_s0, int64_t ids_s1, const void * wts, int wts_bf16, const bf16n_fp8_rows * y,
+                          int n_tok, int n_used, void * workspace, uint64_t workspace_bytes, void * stream) {
+    return guarded([&] {
+        ensure_init();
+        dev::g_last_kernel.name = nullptr;
+        require(up != nullptr, "fp8_moe_experts: null weight");
+        check_experts(gate, up, down, n_tok, n_used);
+        const int64_t n = (int64_t) n_tok * n_used, ib = ids_i64 ? 8 : 4;
+        const int E = (int) gate->n_matrices;
+        const int64_t mid = gate->rows / E, out = down->rows / E;
+        if (out == 0) {
+            return;
+        }
+        require(mid > 0, "fp8_moe_experts: empty gate and up");
+        require(ids && (uintptr_t) ids % ib == 0 && ids_s0 % ib == 0 && ids_s1 % ib == 0, "fp8_moe_experts: ids must be aligned to their elements");
+        check_rows_in(x);
+        check_rows_out(y, out, false);
+        require(y->row == out * (y->kind == BF16N_FP8_BF16 ? 2 : 4), "fp8_moe_experts: contiguous rows of results");
+        require(wts || y->kind == BF16N_FP8_F32, "fp8_moe_experts: the slots' own results are FP32");
+        const experts_plan e = plan_experts(*gate, *down, x->kind, wts != nullptr, n_tok, n_used);
+        check_workspace(workspace, workspace_bytes, e.bytes);
+        char * const ws = (char *) workspace;
+        const hipStream_t st = (hipStream_t) stream;
+        dev::fp8_product a = {}, b = {};
+        a.w = gate; a.up = up; a.x = *x; a.x_rows = n_tok; a.n_cols = n; a.per_token = a.n_used = n_used;
+        b.w = down; b.x_rows = b.n_cols = n; b.per_token = 1; b.n_used = n_used;
+        if (e.listed) {
+            int32_t * const pairs = (int32_t *) (ws + e.lists), * const bounds = pairs + n;
+            dev::launch_int4_route(ids, ids_i64 != 0, ids_s0, ids_s1, E, n_tok, n_used, pairs, bounds, st);
+            launch_check("fp8_moe_experts");
+            a.pairs = b.pairs = pairs; a.bounds = b.bounds = bounds;
+            a.y = {ws + e.hidden, (float *) (ws + e.hidden_scales), mid, 1, n, BF16N_FP8_CODES, 0};
+        } else {
+            a.ids = b.ids = ids; a.ids_i64 = b.ids_i64 = ids_i64 != 0; a.ids_s0 = b.ids_s0 = ids_s0; a.ids_s1 = b.ids_s1 = ids_s1;
+            a.y = {ws + e.hidden, nullptr, mid * 4, 0, 0, BF16N_FP8_F32, 0};
+        }
+        b.x = a.y;
+        b.y = wts ? bf16n_fp8_rows{ws + e.ys, nullptr, out * (e.half ? 2 : 4), 0, 0, e.half ? BF16N_FP8_BF16 : BF16N_FP8_F32, 0} : *y;
+        dev::launch_fp8_product(a, ws + e.product, g_cus, st);
+        launch_check("fp8_moe_experts");
+        dev::launch_fp8_product(b, ws + e.product, g_cus, st);
+        launch_check("fp8_moe_experts");
+        if (wts) {
+            if (e.half) {
+                dev::launch_fp8_combine(ws + e.ys, wts, wts_bf16 != 0, y->at, y->kind == BF16N_FP8_BF16, n_tok, n_used, out, st);
+            } else {
+                dev::launch_moe_combine((const float *) (ws + e.ys), wts, wts_bf16 != 0, y->at, y->kind == BF16N_FP8_BF16, n_tok, n_used, out, st);
+            }
+            launch_check("fp8_moe_experts");
+        }
     });
 }
 

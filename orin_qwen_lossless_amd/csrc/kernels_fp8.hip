@@ -1,0 +1,896 @@
+// Products in 8-bit floating point with a scale for every block of 128, and what makes rows of that form (gfx950).
+#include "dev_fp8.h"
+#include "launchers.h"
+
+#include <algorithm>
+#include <string>
+
+namespace bf16n {
+namespace dev {
+
+namespace {
+
+enum { CODES = BF16N_FP8_CODES, BF16 = BF16N_FP8_BF16, F32 = BF16N_FP8_F32 };
+
+struct fp8_launch {
+    const uint8_t * w, * up;                // codes
+    const void * ws, * ups;                 // scales
+    bool scales_bf16;
+    int K, KB, nrows, NB;                   // columns and their blocks; rows of one matrix and their blocks
+    int64_t n_matrices;
+    const char * x; int64_t x_row;          // bytes
+    const float * xs; int64_t xs_row, xs_block; // elements; of codes
+    int x_kind;
+    char * y; int64_t y_row;                // bytes
+    float * ys; int64_t ys_row, ys_block;   // of codes
+    int y_kind;
+    int ncols;                              // dense columns, or (token, slot) pairs
+    uint32_t per_token, one_per;            // the activation row of a pair is pair / per_token; 2^32 / per_token, rounded down
+    const char * ids; int64_t ids_s0, ids_s1; bool ids_i64; int n_used; // one matrix per pair
+    const int32_t * pairs, * bounds;        // pairs sorted by matrix
+    int ksplit, lds_cols;
+};
+
+__device__ __forceinline__ float scale_at(const void * s, bool bf16, int64_t i) {
+    return bf16 ? bf16_bits_to_f32(((const uint16_t *) s)[i]) : ((const float *) s)[i];
+}
+
+__device__ __forceinline__ int row_of_pair(const fp8_launch & p, uint32_t pair) {
+    const uint32_t t = __umulhi(pair, p.one_per); // at most one too few
+    return (int) (t + (pair - t * p.per_token >= p.per_token));
+}
+
+// results 4 q .. 4 q + 3 of 16 of one column; rows behind the matrix are left out
+template <int KIND>
+__device__ __forceinline__ void store4(const fp8_launch & p, int64_t y_index, int row, f32x4_t v) {
+    char * const at = p.y + y_index * p.y_row + (int64_t) row * (KIND == BF16 ? 2 : 4);
+    if (row + 4 <= p.nrows && ((uintptr_t) at & (KIND == BF16 ? 7 : 15)) == 0) {
+        if (KIND == BF16) {
+            *(u32x2_t *) at = u32x2_t{f32_to_bf16_rne(v[0]) | (uint32_t) f32_to_bf16_rne(v[1]) << 16, f32_to_bf16_rne(v[2]) | (uint32_t) f32_to_bf16_rne(v[3]) << 16};
+        } else {
+            *(f32x4_t *) at = v;
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if (row + e < p.nrows) {
+            if (KIND == BF16) {
+                ((uint16_t *) at)[e] = f32_to_bf16_rne(v[e]);
+            } else {
+                ((float *) at)[e] = v[e];
+            }
+        }
+    }
+}
+
+// rows of zeros for pairs whose id names no matrix: rows from .. from + n of the results
+__device__ __forceinline__ void zero_row(const fp8_launch & p, int64_t pair, int from, int n, int i, int step) {
+    n = min(n, p.nrows - from);
+    for (; i < n; i += step) {
+        const int r = from + i;
+        if (p.y_kind == F32) {
+            ((float *) (p.y + pair * p.y_row))[r] = 0.f;
+        } else if (p.y_kind == BF16) {
+            ((uint16_t *) (p.y + pair * p.y_row))[r] = 0;
+        } else {
+            (p.y + pair * p.y_row)[r] = 0;
+            if (r % FP8_BLOCK == 0) {
+                p.ys[pair * p.ys_row + r / FP8_BLOCK * p.ys_block] = FP8_SMALLEST / FP8_LARGEST;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ float gated(float g, float u) { return silu(g) * u; }
+
+// ---------------------------------------------------------------- few columns
+
+// One wavefront takes 16 rows of the matrix (of each of the two where they are gated) and its part of K; 16 CT columns are the
+// other operand.  A lane's two loads of a step are 16 bytes each of row lane % 16, so that four lanes have half a line and both
+// loads a whole one; weights go from memory to the operand's registers, D steps ahead.  Activations: codes come the same way
+// from L2 (XKIND 0), BF16 and FP32 rows are turned into codes by the block first and kept in LDS.  K in ksplit parts, summed
+// through LDS in a fixed order.
+template <int CT, bool GLU, int XKIND, int NW>
+__global__ void __launch_bounds__(NW * 64) k_fp8_few(const fp8_launch p) {
+    constexpr int NM = GLU ? 2 : 1, D = CT + NM <= 2 ? 8 : 4;
+    extern __shared__ __align__(16) char lds[];
+    const int lane = threadIdx.x & 63, m16 = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int KB = p.KB, pitch = KB * FP8_BLOCK + 16;
+    float * const lds_scales = (float *) (lds + p.lds_cols * pitch); // [lds_cols][KB]
+    f32x4_t * const red = (f32x4_t *) (lds + (XKIND == CODES ? 0 : (p.lds_cols * (pitch + KB * 4) + 15) / 16 * 16));
+
+    int64_t matrix = 0;
+    int begin = 0, end = p.ncols;
+    const int block_rows = NW / p.ksplit * 16, row0 = blockIdx.x * block_rows;
+    if (p.pairs) {
+        matrix = blockIdx.y;
+        begin = p.bounds[matrix];
+        end = p.bounds[matrix + 1];
+        if (matrix == p.n_matrices) {
+            for (int c = begin + blockIdx.z; c < end; c += gridDim.z) {
+                zero_row(p, p.pairs[c], row0, block_rows, threadIdx.x, NW * 64);
+            }
+            return;
+        }
+    } else if (p.ids) {
+        const int t = blockIdx.y / p.n_used, i = blockIdx.y % p.n_used;
+        const char * at = p.ids + t * p.ids_s1 + i * p.ids_s0;
+        matrix = p.ids_i64 ? *(const int64_t *) at : *(const int32_t *) at;
+        begin = blockIdx.y;
+        end = begin + 1;
+        if (matrix < 0 || matrix >= p.n_matrices) {
+            zero_row(p, blockIdx.y, row0, block_rows, threadIdx.x, NW * 64);
+            return;
+        }
+    }
+    const auto y_of = [&](int c) -> int64_t { return p.pairs ? p.pairs[c] : c; };
+    const auto x_of = [&](int c) -> int64_t { return p.pairs ? row_of_pair(p, p.pairs[c]) : p.ids ? row_of_pair(p, c) : c; };
+
+    const int kp = wave % p.ksplit, s0 = KB * kp / p.ksplit, s1 = KB * (kp + 1) / p.ksplit;
+    const int first = row0 + wave / p.ksplit * 16, row = min(first, p.nrows - 1); // (rows behind the matrix repeat its last: not stored)
+    const int64_t row_off = (int64_t) min(m16, p.nrows - 1 - row) * p.K + q * 16;
+    const uint8_t * from[NM];
+    const void * scales[NM];
+    int64_t scale_row = (matrix * p.NB + row / FP8_BLOCK) * KB;
+#pragma unroll
+    for (int m = 0; m < NM; m++) {
+        from[m] = (m ? p.up : p.w) + (matrix * p.nrows + row) * p.K;
+        scales[m] = m ? p.ups : p.ws;
+    }
+    const bool cut = p.K % FP8_BLOCK != 0;
+    // the last block's chunks behind the matrix's last column: the row's first instead, taken as zeros on both sides
+    const bool out0 = cut && (KB - 1) * FP8_BLOCK + q * 16 >= p.K, out1 = cut && (KB - 1) * FP8_BLOCK + q * 16 + 64 >= p.K;
+
+    const int pass = 16 * CT;
+    for (int c0 = begin + (p.ids ? 0 : p.pairs ? blockIdx.z : blockIdx.y) * pass; c0 < end; c0 += (p.ids ? 1 : p.pairs ? gridDim.z : gridDim.y) * pass) {
+        const int nc = min(end - c0, pass);
+        u32x4_t w[D][NM][2], x[D][CT][2];
+        float sx[D][CT];
+        const char * x_at[CT];
+        const float * xs_at[CT];
+        if (XKIND == CODES) {
+#pragma unroll
+            for (int t = 0; t < CT; t++) { // (columns behind the last repeat it: not stored)
+                const int64_t r = x_of(c0 + min(t * 16 + m16, nc - 1));
+                x_at[t] = p.x + r * p.x_row + q * 16;
+                xs_at[t] = p.xs + r * p.xs_row;
+            }
+        }
+        const auto load = [&](int s, int u) {
+            const bool last = cut && s == KB - 1;
+            const int64_t k0 = (int64_t) s * FP8_BLOCK - (last && out0 ? s * FP8_BLOCK + q * 16 : 0), k1 = (int64_t) s * FP8_BLOCK + 64 - (last && out1 ? s * FP8_BLOCK + 64 + q * 16 : 0);
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                w[u][m][0] = *(const u32x4_t *) (from[m] + row_off + k0);
+                w[u][m][1] = *(const u32x4_t *) (from[m] + row_off + k1);
+            }
+            if (XKIND == CODES) {
+#pragma unroll
+                for (int t = 0; t < CT; t++) {
+                    x[u][t][0] = *(const u32x4_t *) (x_at[t] + k0);
+                    x[u][t][1] = *(const u32x4_t *) (x_at[t] + k1);
+                    sx[u][t] = xs_at[t][s * p.xs_block];
+                }
+            }
+        };
+#pragma unroll
+        for (int u = 0; u < D; u++) {
+            if (s0 + u < s1) {
+                load(s0 + u, u);
+            }
+        }
+        if (XKIND != CODES) { // 16 lanes to a block of a column
+            __syncthreads();
+            for (int i = threadIdx.x >> 4; i < nc * KB; i += NW * 4) {
+                const int c = i / KB, b = i - c * KB, k = b * FP8_BLOCK + (threadIdx.x & 15) * 8;
+                const char * src = p.x + x_of(c0 + c) * p.x_row + (int64_t) k * (XKIND == BF16 ? 2 : 4);
+                float v[8] = {};
+                if (k < p.K) {
+                    if (XKIND == BF16) {
+                        bf16x8_to_f32(*(const u32x4_t *) src, v);
+                    } else {
+                        const f32x4_t a = *(const f32x4_t *) src, d = *(const f32x4_t *) (src + 16);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            v[j] = j < 4 ? a[j & 3] : d[j & 3];
+                        }
+                    }
+                }
+                const fp8_scales s = fp8_scales_of(row_max_dpp(most_of8(v)));
+                *(u32x2_t *) (lds + c * pitch + k) = fp8_pack8(v, s.inverse);
+                if ((threadIdx.x & 15) == 0) {
+                    lds_scales[c * KB + b] = s.scale;
+                }
+            }
+            __syncthreads();
+        }
+
+        f32x4_t acc[NM][CT] = {};
+        float sw[NM] = {}; // scales of 64 blocks, one to a lane
+        for (int base = s0; base < s1; base += D) {
+#pragma unroll
+            for (int u = 0; u < D; u++) {
+                const int s = base + u;
+                if (s >= s1) {
+                    break;
+                }
+                if ((s - s0) % 64 == 0) {
+#pragma unroll
+                    for (int m = 0; m < NM; m++) {
+                        sw[m] = scale_at(scales[m], p.scales_bf16, scale_row + min(s + lane, KB - 1));
+                    }
+                }
+                if (cut && s == KB - 1) {
+#pragma unroll
+                    for (int m = 0; m < NM; m++) {
+                        w[u][m][0] = out0 ? u32x4_t{} : w[u][m][0];
+                        w[u][m][1] = out1 ? u32x4_t{} : w[u][m][1];
+                    }
+                    if (XKIND == CODES) {
+#pragma unroll
+                        for (int t = 0; t < CT; t++) {
+                            x[u][t][0] = out0 ? u32x4_t{} : x[u][t][0];
+                            x[u][t][1] = out1 ? u32x4_t{} : x[u][t][1];
+                        }
+                    }
+                }
+                if (XKIND != CODES) {
+#pragma unroll
+                    for (int t = 0; t < CT; t++) {
+                        const int c = min(t * 16 + m16, nc - 1);
+                        const char * at = lds + c * pitch + s * FP8_BLOCK + q * 16;
+                        x[u][t][0] = *(const u32x4_t *) at;
+                        x[u][t][1] = *(const u32x4_t *) (at + 64);
+                        sx[u][t] = lds_scales[c * KB + s];
+                    }
+                }
+                f32x4_t part[NM][CT];
+                fp8_wide xw[CT];
+#pragma unroll
+                for (int t = 0; t < CT; t++) {
+                    xw[t] = fp8_widen(x[u][t][0], x[u][t][1]);
+                }
+#pragma unroll
+                for (int m = 0; m < NM; m++) {
+                    const fp8_wide ww = fp8_widen(w[u][m][0], w[u][m][1]);
+#pragma unroll
+                    for (int t = 0; t < CT; t++) {
+                        part[m][t] = fp8_sum16(ww, xw[t]);
+                    }
+                }
+#pragma unroll
+                for (int m = 0; m < NM; m++) {
+                    const float ws = __uint_as_float((uint32_t) __builtin_amdgcn_readlane((int) __float_as_uint(sw[m]), (s - s0) % 64));
+#pragma unroll
+                    for (int t = 0; t < CT; t++) {
+                        const float both = ws * sx[u][t];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            acc[m][t][e] = fmaf(part[m][t][e], both, acc[m][t][e]);
+                        }
+                    }
+                }
+                if (s + D < s1) {
+                    load(s + D, u);
+                }
+            }
+        }
+        if (p.ksplit > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+#pragma unroll
+                for (int t = 0; t < CT; t++) {
+                    red[((wave * NM + m) * CT + t) * 64 + lane] = acc[m][t];
+                }
+            }
+            __syncthreads();
+            if (kp != 0) {
+                continue;
+            }
+            for (int i = 1; i < p.ksplit; i++) {
+#pragma unroll
+                for (int m = 0; m < NM; m++) {
+#pragma unroll
+                    for (int t = 0; t < CT; t++) {
+                        acc[m][t] += red[(((wave + i) * NM + m) * CT + t) * 64 + lane];
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < CT; t++) {
+            const int c = t * 16 + m16;
+            if (c >= nc) {
+                continue;
+            }
+            f32x4_t v = acc[0][t];
+            if (GLU) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    v[e] = gated(v[e], acc[NM - 1][t][e]);
+                }
+            }
+            if (p.y_kind == BF16) {
+                store4<BF16>(p, y_of(c0 + c), first + 4 * q, v);
+            } else {
+                store4<F32>(p, y_of(c0 + c), first + 4 * q, v);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- many columns
+
+__device__ __align__(16) const uint32_t g_zeros[4] = {0, 0, 0, 0};
+
+// WR x WC wavefronts, RT x CT results of 16 x 16 to each.  Codes of both sides go straight into LDS, a step of 128 columns ahead:
+// rows of 128 bytes, their eight places of 16 bytes exchanged by the row's low bits so that the operands' reads find every
+// bank.  A step's products start from zero and are added to the results times their scales.  BF16 results are summed by the instruction
+// on the codes.  FP32 ones are summed from BF16 operands (fp8_sum16), and so are those that become codes with a scale, which a value
+// 1.5e-5 off would put on the other side of a border now and then (0.0015 of the norm of 300 rows of 1408 that are 0.0003 off so).
+// Lists: a block takes the columns of one matrix, COLS at a time.  OUT8: the results of ROWS = 128 rows leave as codes with a scale.
+template <int WR, int WC, int RT, int CT, bool GLU, bool LIST, int OUT>
+__global__ void __launch_bounds__(WR * WC * 64) k_fp8_many(const fp8_launch p) {
+    constexpr bool WIDE = OUT != BF16;
+    constexpr int NM = GLU ? 2 : 1, THREADS = WR * WC * 64, A_ROWS = WR * RT * 16, ROWS = A_ROWS / NM, COLS = WC * CT * 16;
+    constexpr int STAGE = (A_ROWS + COLS) * FP8_BLOCK, A_COPIES = A_ROWS * 8 / THREADS, B_COPIES = COLS * 8 / THREADS, TM = RT / NM;
+    static_assert(A_COPIES * THREADS == A_ROWS * 8 && B_COPIES * THREADS == COLS * 8, "whole copies");
+    static_assert(FP8_BLOCK % (TM * 16) == 0, "a wavefront's rows have one scale");
+    static_assert(OUT != CODES || ROWS == FP8_BLOCK, "a block of rows has one scale");
+    extern __shared__ __align__(16) char lds[];
+    const int lane = threadIdx.x & 63, m16 = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wave % WR, wc = wave / WR;
+    int64_t matrix = 0;
+    int begin = 0, end = p.ncols, row_tile;
+    if (LIST) {
+        matrix = blockIdx.y;
+        row_tile = blockIdx.x;
+        begin = p.bounds[matrix];
+        end = p.bounds[matrix + 1];
+        if (matrix == p.n_matrices) {
+            for (int c = begin + blockIdx.z; c < end; c += gridDim.z) {
+                zero_row(p, p.pairs[c], row_tile * ROWS, ROWS, threadIdx.x, THREADS);
+            }
+            return;
+        }
+        begin += blockIdx.z * COLS;
+    } else {
+        const int row_tiles = (p.nrows + ROWS - 1) / ROWS, col_tiles = (p.ncols + COLS - 1) / COLS;
+        const int n = row_tiles * col_tiles, per = (n + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+        if ((int) (blockIdx.x >> 3) >= per || id >= n) {
+            return;
+        }
+        const int group = id / (row_tiles * 4), in = id - group * row_tiles * 4, wide = min(4, col_tiles - group * 4);
+        row_tile = in / wide;
+        begin = (group * 4 + in % wide) * COLS;
+        end = min(end, begin + COLS);
+    }
+    const int row0 = row_tile * ROWS, KB = p.KB;
+    const bool cut = p.K % FP8_BLOCK != 0;
+
+    // what this thread copies: a place of rows (threadIdx.x >> 3) + i * THREADS / 8, chunk by the row's low bits
+    const int chunk = (threadIdx.x & 7) ^ ((threadIdx.x >> 3) & 7);
+    const bool behind = cut && (KB - 1) * FP8_BLOCK + chunk * 16 >= p.K;
+    const uint8_t * const w_base = p.w + (matrix * p.nrows + row0) * p.K, * const up_base = p.up + (matrix * p.nrows + row0) * p.K;
+    uint32_t a_off[A_COPIES];
+    const auto of_up = [&](int i) { return GLU && (i * (THREADS / 8) + wave * 8) / 16 % RT >= TM; };
+#pragma unroll
+    for (int i = 0; i < A_COPIES; i++) {
+        const int r = i * (THREADS / 8) + (threadIdx.x >> 3), t = r / 16;
+        a_off[i] = min((t / RT * TM + t % RT % TM) * 16 + r % 16, p.nrows - 1 - row0) * p.K + chunk * 16;
+    }
+    const int wave_row = row0 + wr * TM * 16;
+    const int64_t scale_row = (matrix * p.NB + min(wave_row, p.nrows - 1) / FP8_BLOCK) * KB;
+    const int frag0 = m16 * FP8_BLOCK + ((q ^ (m16 & 7)) << 4), frag1 = frag0 ^ 64;
+    const int a_frag = wr * RT * 16 * FP8_BLOCK, b_frag = A_ROWS * FP8_BLOCK + wc * 16 * FP8_BLOCK;
+
+    for (int c0 = begin; c0 < end; c0 += LIST ? gridDim.z * COLS : COLS) {
+        const int nc = min(end - c0, COLS);
+        const auto x_of = [&](int i) { return LIST ? row_of_pair(p, p.pairs[c0 + min(i, nc - 1)]) : c0 + min(i, nc - 1); };
+        const char * b_at[B_COPIES];
+#pragma unroll
+        for (int i = 0; i < B_COPIES; i++) {
+            b_at[i] = p.x + x_of(i * (THREADS / 8) + (threadIdx.x >> 3)) * p.x_row + chunk * 16;
+        }
+        const float * sx_at[CT];
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            sx_at[c] = p.xs + x_of((c * WC + wc) * 16 + m16) * p.xs_row;
+        }
+        float sx_next[CT], sw[NM];
+        const auto copy = [&](int s, int buf) {
+            const bool none = behind && s == KB - 1;
+#pragma unroll
+            for (int i = 0; i < A_COPIES; i++) {
+                const uint8_t * src = (of_up(i) ? up_base : w_base) + s * FP8_BLOCK + a_off[i];
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (none ? (const uint8_t *) g_zeros : src),
+                                                 (__attribute__((address_space(3))) void *) (lds + buf * STAGE + i * THREADS * 16 + wave * 1024), 16, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < B_COPIES; i++) {
+                if (!LIST || i * (THREADS / 8) < nc) {
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (none ? (const char *) g_zeros : b_at[i] + s * FP8_BLOCK),
+                                                     (__attribute__((address_space(3))) void *) (lds + buf * STAGE + A_ROWS * FP8_BLOCK + i * THREADS * 16 + wave * 1024), 16, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                sx_next[c] = sx_at[c][s * p.xs_block];
+            }
+        };
+        f32x4_t acc[RT][CT] = {};
+        __syncthreads(); // (a list's next columns: nothing reads LDS any more)
+        copy(0, 0);
+        // M: tiles of 16 columns to a wavefront, one loop for each number of them (with a branch around a tile's products the compiler puts
+        // their sums behind the branches, where on some ways too few cycles pass between a product and the read of its result)
+        const auto steps = [&](auto columns) {
+            constexpr int M = decltype(columns)::value;
+            for (int s = 0; s < KB; s++) {
+                __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0): this wavefront's copies are in LDS
+                __syncthreads();                    // all of them are, and nothing reads the other buffer any more
+                float sx[CT];
+#pragma unroll
+                for (int c = 0; c < CT; c++) {
+                    sx[c] = sx_next[c];
+                }
+                if (s % 64 == 0) {
+#pragma unroll
+                    for (int m = 0; m < NM; m++) {
+                        sw[m] = scale_at(m ? p.ups : p.ws, p.scales_bf16, scale_row + min(s + lane, KB - 1));
+                    }
+                }
+                if (s + 1 < KB) {
+                    copy(s + 1, (s + 1) & 1);
+                }
+                const char * const at = lds + (s & 1) * STAGE;
+                float both[NM][M];
+#pragma unroll
+                for (int m = 0; m < NM; m++) {
+                    const float ws = __uint_as_float((uint32_t) __builtin_amdgcn_readlane((int) __float_as_uint(sw[m]), s % 64));
+#pragma unroll
+                    for (int c = 0; c < M; c++) {
+                        both[m][c] = ws * sx[c];
+                    }
+                }
+                u32x4_t b[M][2];
+                fp8_wide bw[M];
+#pragma unroll
+                for (int c = 0; c < M; c++) {
+                    b[c][0] = *(const u32x4_t *) (at + b_frag + c * WC * 16 * FP8_BLOCK + frag0);
+                    b[c][1] = *(const u32x4_t *) (at + b_frag + c * WC * 16 * FP8_BLOCK + frag1);
+                    if constexpr (WIDE) {
+                        bw[c] = fp8_widen(b[c][0], b[c][1]);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < RT; t++) {
+                    const u32x4_t a0 = *(const u32x4_t *) (at + a_frag + t * 16 * FP8_BLOCK + frag0), a1 = *(const u32x4_t *) (at + a_frag + t * 16 * FP8_BLOCK + frag1);
+                    fp8_wide aw;
+                    if constexpr (WIDE) {
+                        aw = fp8_widen(a0, a1);
+                    }
+#pragma unroll
+                    for (int c = 0; c < M; c++) {
+                        f32x4_t part;
+                        if constexpr (WIDE) {
+                            part = fp8_sum16(aw, bw[c]);
+                        } else {
+                            part = fp8_sum8(a0, a1, b[c][0], b[c][1]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            acc[t][c][e] = fmaf(part[e], both[t / TM][c], acc[t][c][e]);
+                        }
+                    }
+                }
+            }
+        };
+        if constexpr (LIST) {
+            const int tiles = ((nc + 15) / 16 + WC - 1) / WC;
+            static_assert(CT == 4, "one loop each");
+            tiles == 1 ? steps(std::integral_constant<int, 1>{}) : tiles == 2 ? steps(std::integral_constant<int, 2>{})
+            : tiles == 3 ? steps(std::integral_constant<int, 3>{}) : steps(std::integral_constant<int, 4>{});
+        } else {
+            steps(std::integral_constant<int, CT>{});
+        }
+        if (GLU) {
+#pragma unroll
+            for (int t = 0; t < TM; t++) {
+#pragma unroll
+                for (int c = 0; c < CT; c++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        acc[t][c][e] = gated(acc[t][c][e], acc[RT - TM + t][c][e]);
+                    }
+                }
+            }
+        }
+        if constexpr (OUT == CODES) {
+            float * const most = (float *) lds; // [WR][COLS]
+            float mine[CT];
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                float v = 0.f;
+#pragma unroll
+                for (int t = 0; t < TM; t++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        v = fmaxf(v, wave_row + t * 16 + 4 * q + e < p.nrows ? fabsf(acc[t][c][e]) : 0.f);
+                    }
+                }
+                v = fmaxf(v, __shfl_xor(v, 16, 64));
+                mine[c] = fmaxf(v, __shfl_xor(v, 32, 64));
+            }
+            __syncthreads();
+            if (q == 0) {
+#pragma unroll
+                for (int c = 0; c < CT; c++) {
+                    most[wr * COLS + (c * WC + wc) * 16 + m16] = mine[c];
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                const int col = (c * WC + wc) * 16 + m16;
+                if (col >= nc) {
+                    continue;
+                }
+                float v = most[col];
+#pragma unroll
+                for (int i = 1; i < WR; i++) {
+                    v = fmaxf(v, most[i * COLS + col]);
+                }
+                const fp8_scales s = fp8_scales_of(v);
+                const int64_t y = LIST ? p.pairs[c0 + col] : c0 + col;
+                if (wr == 0 && q == 0) {
+                    p.ys[y * p.ys_row + row_tile * p.ys_block] = s.scale;
+                }
+#pragma unroll
+                for (int t = 0; t < TM; t++) {
+                    const int r = wave_row + t * 16 + 4 * q;
+                    if (r < p.nrows) { // (rows are a multiple of 16)
+                        *(uint32_t *) (p.y + y * p.y_row + r) = fp8_pack4(acc[t][c][0] * s.inverse, acc[t][c][1] * s.inverse, acc[t][c][2] * s.inverse, acc[t][c][3] * s.inverse);
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                const int col = (c * WC + wc) * 16 + m16;
+                if (col >= nc) {
+                    continue;
+                }
+                const int64_t y = LIST ? p.pairs[c0 + col] : c0 + col;
+#pragma unroll
+                for (int t = 0; t < TM; t++) {
+                    store4<OUT>(p, y, wave_row + t * 16 + 4 * q, acc[t][c]);
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- rows in 8 bits
+
+// A block of 128 values to 16 lanes.
+template <int KIND>
+__global__ void __launch_bounds__(256) k_fp8_rows(const char * x, int64_t x_row, uint8_t * y, int64_t y_row, float * s, int64_t s_row, int64_t s_block, int64_t rows, int K) {
+    const int KB = (K + FP8_BLOCK - 1) / FP8_BLOCK;
+    for (int64_t i = (int64_t) blockIdx.x * 16 + (threadIdx.x >> 4); i < rows * KB; i += (int64_t) gridDim.x * 16) {
+        const int64_t r = i / KB;
+        const int b = (int) (i - r * KB), k = b * FP8_BLOCK + (threadIdx.x & 15) * 8;
+        float v[8] = {};
+        if (k < K) {
+            const char * src = x + r * x_row + (int64_t) k * (KIND == BF16 ? 2 : 4);
+            if (KIND == BF16) {
+                bf16x8_to_f32(*(const u32x4_t *) src, v);
+            } else {
+                const f32x4_t a = *(const f32x4_t *) src, d = *(const f32x4_t *) (src + 16);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    v[j] = j < 4 ? a[j & 3] : d[j & 3];
+                }
+            }
+        }
+        const fp8_scales q = fp8_scales_of(row_max_dpp(most_of8(v)));
+        if (k < K) {
+            *(u32x2_t *) (y + r * y_row + k) = fp8_pack8(v, q.inverse);
+        }
+        if ((threadIdx.x & 15) == 0) {
+            s[r * s_row + b * s_block] = q.scale;
+        }
+    }
+}
+
+// The glue of a decode step (bf16n_add_rmsnorm) with its norm in 8 bits: a token's row in C pieces of eight elements to a thread,
+// 16 threads to a block of 128.  Sums are FP32, the slots' in bf16n_moe_combine's order.
+template <int C>
+__global__ void __launch_bounds__(256) k_add_rmsnorm_fp8(const add_norm_args p, uint8_t * y, int64_t y_row, float * s, int64_t s_row, int64_t s_block) {
+    __shared__ float wave_sq[4];
+    __shared__ float wsm[1024];
+    const int64_t tok = blockIdx.x, base = tok * p.n;
+    if (p.ys) {
+        for (int i = threadIdx.x; i < p.n_used; i += 256) {
+            const int64_t at = tok * p.n_used + i;
+            wsm[i] = p.wts_bf16 ? bf16_bits_to_f32(((const uint16_t *) p.wts)[at]) : ((const float *) p.wts)[at];
+        }
+        __syncthreads();
+    }
+    float v[C][8], sq = 0.f;
+#pragma unroll
+    for (int j = 0; j < C; j++) {
+        const int i0 = (j * 256 + threadIdx.x) * 8;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            v[j][e] = 0.f;
+        }
+        if (i0 < p.n) {
+            float f[8];
+            bf16x8_to_f32(*(const u32x4_t *) (p.a + base + i0), v[j]);
+            for (const uint16_t * more : {p.b, p.c}) {
+                if (more) {
+                    bf16x8_to_f32(*(const u32x4_t *) (more + base + i0), f);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        v[j][e] += f[e];
+                    }
+                }
+            }
+            if (p.ys) {
+                float acc[8] = {};
+                const float * row = p.ys + (tok * p.n_used) * p.n + i0;
+                for (int k = 0; k < p.n_used; k++) {
+                    const f32x4_t a = *(const f32x4_t *) (row + k * p.n), d = *(const f32x4_t *) (row + k * p.n + 4);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        acc[e] = fmaf(wsm[k], e < 4 ? a[e & 3] : d[e & 3], acc[e]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    v[j][e] += acc[e];
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            sq = fmaf(v[j][e], v[j][e], sq);
+        }
+    }
+    sq = wave_sum(sq);
+    if ((threadIdx.x & 63) == 0) {
+        wave_sq[threadIdx.x >> 6] = sq;
+    }
+    __syncthreads();
+    const float total = ((wave_sq[0] + wave_sq[1]) + wave_sq[2]) + wave_sq[3];
+    const float scale = 1.0f / sqrtf(total / (float) p.n + p.eps);
+#pragma unroll
+    for (int j = 0; j < C; j++) {
+        const int i0 = (j * 256 + threadIdx.x) * 8;
+        float g[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+        const bool in = i0 < p.n;
+        if (in && p.y_sum) {
+            *(u32x4_t *) (p.y_sum + base + i0) = u32x4_t{f32_to_bf16_rne(v[j][0]) | (uint32_t) f32_to_bf16_rne(v[j][1]) << 16, f32_to_bf16_rne(v[j][2]) | (uint32_t) f32_to_bf16_rne(v[j][3]) << 16,
+                                                         f32_to_bf16_rne(v[j][4]) | (uint32_t) f32_to_bf16_rne(v[j][5]) << 16, f32_to_bf16_rne(v[j][6]) | (uint32_t) f32_to_bf16_rne(v[j][7]) << 16};
+        }
+        if (in && p.gamma) {
+            bf16x8_to_f32(*(const u32x4_t *) (p.gamma + i0), g);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            v[j][e] = v[j][e] * scale * g[e];
+        }
+        if (in && p.y_norm) {
+            *(u32x4_t *) (p.y_norm + base + i0) = u32x4_t{f32_to_bf16_rne(v[j][0]) | (uint32_t) f32_to_bf16_rne(v[j][1]) << 16, f32_to_bf16_rne(v[j][2]) | (uint32_t) f32_to_bf16_rne(v[j][3]) << 16,
+                                                          f32_to_bf16_rne(v[j][4]) | (uint32_t) f32_to_bf16_rne(v[j][5]) << 16, f32_to_bf16_rne(v[j][6]) | (uint32_t) f32_to_bf16_rne(v[j][7]) << 16};
+        }
+        const fp8_scales q = fp8_scales_of(row_max_dpp(most_of8(v[j])));
+        if (in) {
+            *(u32x2_t *) (y + tok * y_row + i0) = fp8_pack8(v[j], q.inverse);
+            if ((threadIdx.x & 15) == 0) {
+                s[tok * s_row + i0 / FP8_BLOCK * s_block] = q.scale;
+            }
+        }
+    }
+}
+
+// y[t] = sum over the slots of w[t, k] * ys[t, k] for rows in BF16, slots in order, one fmaf each; n a multiple of 8
+__global__ void __launch_bounds__(256) k_fp8_combine(const uint16_t * ys, const void * w, bool w_bf16, char * y, bool y_bf16, int n_used, int64_t n) {
+    const int64_t t = blockIdx.y, i = ((int64_t) blockIdx.x * 256 + threadIdx.x) * 8;
+    if (i >= n) {
+        return;
+    }
+    float acc[8] = {};
+    for (int k = 0; k < n_used; k++) {
+        const int64_t s = t * n_used + k;
+        const float wk = scale_at(w, w_bf16, s);
+        float v[8];
+        bf16x8_to_f32(__builtin_nontemporal_load((const u32x4_t *) (ys + s * n + i)), v);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            acc[e] = fmaf(wk, v[e], acc[e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        store_y(y + t * n * (y_bf16 ? 2 : 4), y_bf16, i + e, acc[e]);
+    }
+}
+
+// ---------------------------------------------------------------- launches
+
+fp8_launch launch_of(const fp8_product & a) {
+    fp8_launch p = {};
+    const bf16n_fp8_weight & w = *a.w;
+    p.w = w.codes; p.ws = w.scales; p.scales_bf16 = w.scales_bf16 != 0;
+    if (a.up) {
+        p.up = a.up->codes; p.ups = a.up->scales;
+    }
+    p.K = (int) w.K; p.KB = (int) ((w.K + FP8_BLOCK - 1) / FP8_BLOCK);
+    p.n_matrices = w.n_matrices;
+    p.nrows = (int) (w.rows / w.n_matrices); p.NB = (p.nrows + FP8_BLOCK - 1) / FP8_BLOCK;
+    p.x = (const char *) a.x.at; p.x_row = a.x.row; p.xs = a.x.scales; p.xs_row = a.x.scale_row; p.xs_block = a.x.scale_block; p.x_kind = a.x.kind;
+    p.y = (char *) a.y.at; p.y_row = a.y.row; p.ys = a.y.scales; p.ys_row = a.y.scale_row; p.ys_block = a.y.scale_block; p.y_kind = a.y.kind;
+    p.ncols = (int) a.n_cols;
+    p.per_token = (uint32_t) a.per_token; p.one_per = (uint32_t) std::min<uint64_t>(~0u, (1ull << 32) / a.per_token);
+    p.ids = (const char *) a.ids; p.ids_i64 = a.ids_i64; p.ids_s0 = a.ids_s0; p.ids_s1 = a.ids_s1; p.n_used = a.n_used;
+    p.pairs = a.pairs; p.bounds = a.bounds;
+    return p;
+}
+
+// a kernel instance's template arguments (bf16n_last_kernel)
+std::string text_of(std::initializer_list<int> numbers) {
+    std::string s;
+    for (const int n : numbers) {
+        s += (s.empty() ? "" : ", ") + std::to_string(n);
+    }
+    return s;
+}
+
+template <int CT, bool GLU, int XKIND, int NW>
+void few_go(const fp8_launch & p, dim3 grid, size_t lds, hipStream_t stream) {
+    static const std::string text = text_of({CT, GLU, XKIND, NW});
+    note_kernel("k_fp8_few", text.c_str(), 0);
+    k_fp8_few<CT, GLU, XKIND, NW><<<grid, NW * 64, lds, stream>>>(p);
+}
+
+constexpr int FEW_LDS = 64 * 1024; // of a block, its sums over the parts of K and converted columns
+
+size_t few_red(int ct, bool glu, int nw) { return (size_t) nw * (glu ? 2 : 1) * ct * 1024; }
+size_t few_staged(int cols, int KB) { return ((size_t) cols * (KB * FP8_BLOCK + 16 + KB * 4) + 15) / 16 * 16; }
+
+void run_few(fp8_launch p, bool glu, int most_cols, int64_t busy, int y_blocks, int z_blocks, int cus, hipStream_t stream) {
+    const int ct = most_cols <= 16 ? 1 : 2;
+    const int64_t tiles = (p.nrows + 15) / 16 * busy;
+    const int nw = tiles <= 4 * cus ? 8 : 4;
+    p.ksplit = nw == 8 ? std::min(8, p.KB >= 8 ? 8 : p.KB >= 4 ? 4 : p.KB >= 2 ? 2 : 1) : tiles <= 16 * cus && p.KB >= 4 ? 4 : 1;
+    p.lds_cols = std::min(most_cols, 16 * ct);
+    const size_t lds = (p.x_kind == CODES ? 0 : few_staged(p.lds_cols, p.KB)) + (p.ksplit > 1 ? few_red(ct, glu, nw) : 0);
+    const int rows = nw / p.ksplit * 16;
+    const dim3 grid((p.nrows + rows - 1) / rows, y_blocks, z_blocks);
+    const auto by_kind = [&](auto c, auto g, auto n) {
+        constexpr int C = decltype(c)::value, N = decltype(n)::value;
+        constexpr bool G = decltype(g)::value;
+        p.x_kind == CODES ? few_go<C, G, CODES, N>(p, grid, lds, stream) : p.x_kind == BF16 ? few_go<C, G, BF16, N>(p, grid, lds, stream) : few_go<C, G, F32, N>(p, grid, lds, stream);
+    };
+    const auto by_nw = [&](auto c, auto g) { nw == 8 ? by_kind(c, g, std::integral_constant<int, 8>{}) : by_kind(c, g, std::integral_constant<int, 4>{}); };
+    const auto by_ct = [&](auto g) { ct == 1 ? by_nw(std::integral_constant<int, 1>{}, g) : by_nw(std::integral_constant<int, 2>{}, g); };
+    glu ? by_ct(std::true_type{}) : by_ct(std::false_type{});
+}
+
+template <int WR, int WC, int RT, int CT, bool GLU, bool LIST, int OUT>
+void many_go(const fp8_launch & p, int z_blocks, hipStream_t stream) {
+    constexpr int ROWS = WR * RT * 16 / (GLU ? 2 : 1), COLS = WC * CT * 16, LDS = 2 * (WR * RT * 16 + COLS) * FP8_BLOCK;
+    const int row_tiles = (p.nrows + ROWS - 1) / ROWS, col_tiles = (p.ncols + COLS - 1) / COLS;
+    const dim3 grid = LIST ? dim3(row_tiles, (unsigned) p.n_matrices + 1, z_blocks) : dim3((unsigned) (((int64_t) row_tiles * col_tiles + 7) / 8 * 8));
+    static const std::string text = text_of({WR, WC, RT, CT, GLU, LIST, OUT});
+    note_kernel("k_fp8_many", text.c_str(), 0);
+    k_fp8_many<WR, WC, RT, CT, GLU, LIST, OUT><<<grid, WR * WC * 64, LDS, stream>>>(p);
+}
+template <int WR, int WC, int RT, int CT, bool GLU, bool LIST, int OUT>
+void many_init() {
+    constexpr int COLS = WC * CT * 16, LDS = 2 * (WR * RT * 16 + COLS) * FP8_BLOCK;
+    (void) hipFuncSetAttribute((const void *) k_fp8_many<WR, WC, RT, CT, GLU, LIST, OUT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+}
+
+template <bool LIST>
+void run_many(const fp8_launch & p, bool glu, int z_blocks, hipStream_t stream) {
+    if (glu) {
+        p.y_kind == CODES ? many_go<4, 2, 4, 4, true, LIST, CODES>(p, z_blocks, stream)
+        : p.y_kind == BF16 ? many_go<4, 2, 4, 4, true, LIST, BF16>(p, z_blocks, stream) : many_go<4, 2, 4, 4, true, LIST, F32>(p, z_blocks, stream);
+    } else {
+        p.y_kind == BF16 ? many_go<2, 2, 4, 4, false, LIST, BF16>(p, z_blocks, stream) : many_go<2, 2, 4, 4, false, LIST, F32>(p, z_blocks, stream);
+    }
+}
+
+constexpr int FEW_COLUMNS = 32;
+
+bool few(const bf16n_fp8_weight & w, int64_t n_cols, bool listed, bool by_ids) {
+    return by_ids || (listed ? n_cols <= 12 * (int64_t) w.n_matrices : n_cols <= FEW_COLUMNS);
+}
+// whether the block converts rows that are not codes by itself
+bool converts(const bf16n_fp8_weight & w, int64_t n_cols, bool by_ids, bool glu) {
+    const int KB = (int) ((w.K + FP8_BLOCK - 1) / FP8_BLOCK), cols = by_ids ? 1 : (int) std::min<int64_t>(n_cols, FEW_COLUMNS);
+    return few_staged(cols, KB) + few_red(cols <= 16 ? 1 : 2, glu, 8) <= FEW_LDS;
+}
+size_t aligned(size_t n) { return (n + 255) / 256 * 256; }
+size_t codes_bytes(int64_t rows, int64_t K) { return aligned(rows * K) + aligned(rows * ((K + FP8_BLOCK - 1) / FP8_BLOCK) * 4); }
+
+} // namespace
+
+void fp8_init() {
+    many_init<4, 2, 4, 4, true, true, CODES>();
+    many_init<4, 2, 4, 4, true, true, BF16>();
+    many_init<4, 2, 4, 4, true, true, F32>();
+    many_init<4, 2, 4, 4, true, false, CODES>();
+    many_init<4, 2, 4, 4, true, false, BF16>();
+    many_init<4, 2, 4, 4, true, false, F32>();
+}
+
+void launch_fp8_rows(const bf16n_fp8_rows & x, const bf16n_fp8_rows & y, int64_t rows, int64_t K, int cus, hipStream_t stream) {
+    const int64_t items = rows * ((K + FP8_BLOCK - 1) / FP8_BLOCK);
+    const unsigned grid = (unsigned) std::min<int64_t>((items + 15) / 16, (int64_t) cus * 64);
+    (x.kind == BF16 ? k_fp8_rows<BF16> : k_fp8_rows<F32>)<<<grid, 256, 0, stream>>>((const char *) x.at, x.row, (uint8_t *) y.at, y.row, y.scales, y.scale_row, y.scale_block, rows, (int) K);
+}
+
+void launch_add_rmsnorm_fp8(const add_norm_args & a, const bf16n_fp8_rows & y, int n_tok, hipStream_t stream) {
+    const int64_t pieces = (a.n + 2047) / 2048;
+    (pieces == 1 ? k_add_rmsnorm_fp8<1> : pieces == 2 ? k_add_rmsnorm_fp8<2> : pieces <= 4 ? k_add_rmsnorm_fp8<4> : k_add_rmsnorm_fp8<8>)
+        <<<n_tok, 256, 0, stream>>>(a, (uint8_t *) y.at, y.row, y.scales, y.scale_row, y.scale_block);
+}
+
+uint64_t fp8_workspace_bytes(const bf16n_fp8_weight & w, bool glu, int x_kind, int y_kind, int64_t x_rows, int64_t n_cols, bool listed, bool by_ids) {
+    const bool f = few(w, n_cols, listed, by_ids);
+    uint64_t n = 0;
+    if (x_kind != CODES && (!f || listed || !converts(w, n_cols, by_ids, glu))) {
+        n += codes_bytes(x_rows, w.K);
+    }
+    if (y_kind == CODES && f) {
+        n += aligned(n_cols * (w.rows / w.n_matrices) * 4);
+    }
+    return n;
+}
+
+void launch_fp8_product(const fp8_product & a, void * workspace, int cus, hipStream_t stream) {
+    const bool glu = a.up != nullptr, listed = a.pairs != nullptr, by_ids = a.ids != nullptr;
+    const bool f = few(*a.w, a.n_cols, listed, by_ids);
+    fp8_launch p = launch_of(a);
+    char * ws = (char *) workspace;
+    if (p.x_kind != CODES && (!f || listed || !converts(*a.w, a.n_cols, by_ids, glu))) {
+        const bf16n_fp8_rows codes = {ws, (float *) (ws + aligned(a.x_rows * a.w->K)), a.w->K, 1, a.x_rows, CODES, 0};
+        launch_fp8_rows(a.x, codes, a.x_rows, a.w->K, cus, stream);
+        p.x = ws; p.x_row = a.w->K; p.xs = codes.scales; p.xs_row = 1; p.xs_block = a.x_rows; p.x_kind = CODES;
+        ws += codes_bytes(a.x_rows, a.w->K);
+    }
+    if (!f) {
+        listed ? run_many<true>(p, glu, 1, stream) : run_many<false>(p, glu, 1, stream);
+        return;
+    }
+    bf16n_fp8_rows plain = {};
+    if (p.y_kind == CODES) {
+        plain = {ws, nullptr, (int64_t) p.nrows * 4, 0, 0, F32, 0};
+        p.y = ws; p.y_row = plain.row; p.y_kind = F32;
+    }
+    if (by_ids) {
+        run_few(p, glu, 1, a.n_cols, (int) a.n_cols, 1, cus, stream);
+    } else if (listed) {
+        run_few(p, glu, 16, std::min<int64_t>(a.n_cols, p.n_matrices), (int) p.n_matrices + 1, 1, cus, stream);
+    } else {
+        const int ct = a.n_cols <= 16 ? 1 : 2, passes = (int) ((a.n_cols + 16 * ct - 1) / (16 * ct));
+        run_few(p, glu, (int) std::min<int64_t>(a.n_cols, 16 * ct), passes, passes, 1, cus, stream);
+    }
+    if (plain.at) {
+        launch_fp8_rows(plain, a.y, a.n_cols, p.nrows, cus, stream);
+    }
+}
+
+void launch_fp8_combine(const void * ys, const void * w, bool w_bf16, void * y, bool y_bf16, int n_tok, int n_used, int64_t n, hipStream_t stream) {
+    k_fp8_combine<<<dim3((unsigned) ((n / 8 + 255) / 256), (unsigned) n_tok), 256, 0, stream>>>((const uint16_t *) ys, w, w_bf16, (char *) y, y_bf16, n_used, n);
+}
+
+} // namespace dev
+} // namespace bf16n

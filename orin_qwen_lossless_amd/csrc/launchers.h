@@ -118,6 +118,22 @@ void launch_int4_mm_ids(const bf16n_int4_weight & w, const bf16n_int4_weight * u
                         const int32_t * bounds, void * y, bool y_bf16, int64_t y_row, int n_matrices, int n_tok, int n_used, void * workspace,
                         uint64_t workspace_bytes, int cus, hipStream_t stream);
 
+// 8-bit floating point with a scale for every block of 128 (kernels_fp8.hip)
+struct fp8_product {
+    const bf16n_fp8_weight * w, * up;       // up: gated
+    bf16n_fp8_rows x, y;
+    int64_t x_rows, n_cols;                 // n_cols: dense columns, or (token, slot) pairs
+    int per_token, n_used;                  // the activation row of a pair is pair / per_token
+    const void * ids; bool ids_i64; int64_t ids_s0, ids_s1; // one matrix per pair (strides in bytes), or
+    const int32_t * pairs, * bounds;        // pairs sorted by matrix, or neither
+};
+void fp8_init();
+void launch_fp8_rows(const bf16n_fp8_rows & x, const bf16n_fp8_rows & y, int64_t rows, int64_t K, int cus, hipStream_t stream);
+void launch_add_rmsnorm_fp8(const add_norm_args & a, const bf16n_fp8_rows & y, int n_tok, hipStream_t stream);
+uint64_t fp8_workspace_bytes(const bf16n_fp8_weight & w, bool glu, int x_kind, int y_kind, int64_t x_rows, int64_t n_cols, bool listed, bool by_ids);
+void launch_fp8_product(const fp8_product & a, void * workspace, int cus, hipStream_t stream);
+void launch_fp8_combine(const void * ys, const void * w, bool w_bf16, void * y, bool y_bf16, int n_tok, int n_used, int64_t n, hipStream_t stream);
+
 // batched MoE prefill (kernels_mm_ids.hip)
 void mm_ids_init();
 bool mm_ids_shape_ok(const bf16n_weight & w, const bf16n_weight * up);

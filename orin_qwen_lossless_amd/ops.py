@@ -1180,6 +1180,365 @@ def int4_moe_experts(x: torch.Tensor, gate: Int4Weight, up: Int4Weight, down: In
     return moe_combine(int4_moe_experts_rows(x, gate, up, down, topk_ids, n_experts), topk_weights, torch.bfloat16)
 
 
+# ---------------------------------------------------------------- 8-bit floating point with a scale for every block of 128
+
+FP8_BLOCK, FP8_LARGEST, FP8_SMALLEST, FP8_MAX_K = 128, 448.0, 2.0 ** -100, 32768
+_E4M3 = torch.float8_e4m3fn
+_FP8_KINDS = {_E4M3: 0, torch.bfloat16: 1, torch.float32: 2}  # include/bf16n_c.h
+
+
+@dataclass(frozen=True, eq=False)
+class Fp8Weight:
+    """A matrix (or a stack of n_matrices matrices) in 8-bit floating point with a scale for every block of 128 x 128, on a device:
+    w[r, k] = scales[r // 128, k // 128] * codes[r, k].
+
+    codes: float8_e4m3fn [rows, K]; scales: f32 or bf16 [n_matrices * ceil(rows of one / 128), ceil(K / 128)]: blocks begin anew in
+    every matrix, its last ones may be cut short.  Both contiguous and on one device.  K: a multiple of 16, at most 32768."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    n_matrices: int = 1
+
+    def __post_init__(self):
+        c, s, n = self.codes, self.scales, self.n_matrices
+        if c.dtype is not _E4M3 or c.dim() != 2 or not c.is_contiguous():
+            raise ValueError("bf16n.Fp8Weight: codes must be contiguous float8_e4m3fn [rows, K]")
+        if c.shape[1] % 16 or not 16 <= c.shape[1] <= FP8_MAX_K:
+            raise ValueError("bf16n.Fp8Weight: K must be a multiple of 16 in [16, 32768]")
+        if type(n) is not int or not 0 < n <= 65534 or c.shape[0] % n:
+            raise ValueError("bf16n.Fp8Weight: rows must split into n_matrices (at most 65534)")
+        shape = (n * -(-(c.shape[0] // n) // FP8_BLOCK), -(-c.shape[1] // FP8_BLOCK))
+        if s.dtype not in (torch.float32, torch.bfloat16) or tuple(s.shape) != shape or not s.is_contiguous():
+            raise ValueError(f"bf16n.Fp8Weight: scales must be contiguous f32 or bf16 {list(shape)}")
+        if s.device != c.device:
+            raise ValueError("bf16n.Fp8Weight: codes and scales on different devices")
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
+
+    @property
+    def K(self) -> int:
+        return self.codes.shape[1]
+
+    @property
+    def nbytes(self) -> int:
+        """Bytes the matrix occupies in device memory."""
+        return self.codes.numel() + self.scales.numel() * self.scales.element_size()
+
+    def to(self, device: torch.device | str) -> "Fp8Weight":
+        return Fp8Weight(self.codes.to(device), self.scales.to(device), self.n_matrices)
+
+
+@dataclass(frozen=True, eq=False)
+class Fp8Rows:
+    """Activations in 8-bit floating point with a scale for every 128 columns: x[t, k] = scales[t, k // 128] * codes[t, k].
+
+    codes: float8_e4m3fn [tokens, K], rows contiguous; scales: f32 [tokens, ceil(K / 128)] of any strides (the calls here leave those of a
+    block's tokens next to one another).  Both on one device."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self):
+        c, s = self.codes, self.scales
+        if c.dtype is not _E4M3 or c.dim() != 2 or (c.shape[1] > 1 and c.stride(1) != 1):
+            raise ValueError("bf16n.Fp8Rows: codes must be float8_e4m3fn [tokens, K], contiguous along K")
+        if s.dtype is not torch.float32 or tuple(s.shape) != (c.shape[0], -(-c.shape[1] // FP8_BLOCK)) or s.device != c.device:
+            raise ValueError(f"bf16n.Fp8Rows: scales must be f32 {[c.shape[0], -(-c.shape[1] // FP8_BLOCK)]} on the codes' device")
+
+    def dequant(self) -> torch.Tensor:
+        """The values it stands for, FP32 (torch operations)."""
+        return self.codes.float() * self.scales.repeat_interleave(FP8_BLOCK, 1)[:, : self.codes.shape[1]]
+
+
+def fp8_quantize(w: torch.Tensor, n_matrices: int = 1, scale_dtype: torch.dtype = torch.float32) -> Fp8Weight:
+    """The nearest codes of a BF16 / FP32 matrix [..., K] (leading axes are rows), on its device, for load time: torch operations in
+    pieces.  scale = max|w| / 448 of a block of 128 x 128; codes are taken against the rounded scale.  A block with a weight that is
+    not finite has no values."""
+    if w.dim() < 2 or w.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("bf16n.fp8_quantize: weight must be bf16 or f32, at least 2-D (rows x K)")
+    if scale_dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("bf16n.fp8_quantize: scales are f32 or bf16")
+    K = w.shape[-1]
+    w = w.reshape(-1, K)
+    if K % 16 or not 16 <= K <= FP8_MAX_K or type(n_matrices) is not int or not 0 < n_matrices <= 65534 or w.shape[0] % n_matrices:
+        raise ValueError("bf16n.fp8_quantize: K must be a multiple of 16 in [16, 32768], rows must split into n_matrices")
+    rows, kb = w.shape[0] // n_matrices, -(-K // FP8_BLOCK)
+    nb = -(-rows // FP8_BLOCK)
+    codes = torch.empty(w.shape, dtype=_E4M3, device=w.device)
+    scales = torch.empty((n_matrices * nb, kb), dtype=scale_dtype, device=w.device)
+    step = max(1, DEQUANT_CHUNK_BYTES // (4 * FP8_BLOCK * kb * FP8_BLOCK))  # blocks of rows in a piece
+    for m in range(n_matrices):
+        for b in range(0, nb, step):
+            lo, hi = m * rows + b * FP8_BLOCK, m * rows + min((b + step) * FP8_BLOCK, rows)
+            n = -(-(hi - lo) // FP8_BLOCK)
+            v = torch.nn.functional.pad(w[lo:hi].float(), (0, kb * FP8_BLOCK - K, 0, n * FP8_BLOCK - (hi - lo))).view(n, FP8_BLOCK, kb, FP8_BLOCK)
+            s = (v.abs().amax((1, 3)).clamp_min(FP8_SMALLEST) / FP8_LARGEST).to(scale_dtype)
+            scales[m * nb + b: m * nb + b + n] = s
+            q = (v / s.float()[:, None, :, None]).clamp_(-FP8_LARGEST, FP8_LARGEST).to(_E4M3)
+            codes[lo:hi] = q.view(n * FP8_BLOCK, kb * FP8_BLOCK)[: hi - lo, :K]
+    return Fp8Weight(codes, scales, n_matrices)
+
+
+def _c_fp8(w: Fp8Weight) -> _lib.Fp8Weight:
+    c, s = w.codes, w.scales
+    if not c.is_cuda:
+        raise ValueError("bf16n: an Fp8Weight must be on a device")
+    return _lib.Fp8Weight(c.data_ptr(), s.data_ptr(), c.shape[1], c.shape[0], w.n_matrices, s.dtype is torch.bfloat16, 0)
+
+
+def _c_rows(what: str, x, K: int | None = None) -> _lib.Fp8Rows:
+    """x: Fp8Rows, or a BF16 / FP32 tensor of any number of axes whose last is contiguous and whose others are one evenly spaced axis."""
+    if isinstance(x, Fp8Rows):
+        c, s = x.codes, x.scales
+        scales, s0, s1 = s.data_ptr(), s.stride(0), s.stride(1)
+    else:
+        c, scales, s0, s1 = x, None, 0, 0
+        if c.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError(f"bf16n.{what}: x must be bf16, f32 or Fp8Rows")
+    if not c.is_cuda:
+        raise ValueError(f"bf16n.{what}: x must be on a device")
+    if c.dim() != 2 or (K is not None and c.shape[1] != K):
+        raise ValueError(f"bf16n.{what}: x must be [tokens, K]" + ("" if K is None else f" with K = {K}"))
+    row = c.stride(0) * c.element_size()
+    if c.stride(1) != 1 or row % 16 or c.data_ptr() % 16:
+        raise ValueError(f"bf16n.{what}: x must be 16-byte aligned, contiguous along K, with row strides of a multiple of 16 bytes")
+    return _lib.Fp8Rows(c.data_ptr(), scales, row, s0, s1, _FP8_KINDS[c.dtype], 0)
+
+
+def _new_rows(tokens: int, K: int, device: torch.device) -> Fp8Rows:
+    return Fp8Rows(torch.empty((tokens, K), dtype=_E4M3, device=device), torch.empty((-(-K // FP8_BLOCK), tokens), dtype=torch.float32, device=device).t())
+
+
+def _fp8_out(tokens: int, n: int, out_dtype: torch.dtype, device: torch.device):
+    """(result, its rows for the C ABI)"""
+    if out_dtype is _E4M3:
+        y = _new_rows(tokens, n, device)
+        return y, _lib.Fp8Rows(y.codes.data_ptr(), y.scales.data_ptr(), n, 1, tokens, 0, 0)
+    y = torch.empty((tokens, n), dtype=out_dtype, device=device)
+    return y, _lib.Fp8Rows(y.data_ptr(), None, n * y.element_size(), 0, 0, _FP8_KINDS[out_dtype], 0)
+
+
+def _workspace(n: int, device: torch.device) -> tuple[int | None, torch.Tensor | None]:
+    t = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    return (t.data_ptr() if n else None), t
+
+
+def _device_of(x) -> torch.device:
+    return x.codes.device if isinstance(x, Fp8Rows) else x.device
+
+
+def fp8_quantize_rows(x: torch.Tensor) -> Fp8Rows:
+    """BF16 or FP32 activations [tokens, K] (K a multiple of 16, at most 32768) in 8 bits: for a block v of up to 128 columns with
+    m = max(max|v|, 2^-100) the scale m / 448 and the codes e4m3(v * (448 / m)), to nearest even (bf16n_fp8_quantize_rows)."""
+    cx = _c_rows("fp8_quantize_rows", x)
+    T, K = x.shape
+    if K % 16 or not 16 <= K <= FP8_MAX_K:
+        raise ValueError("bf16n.fp8_quantize_rows: K must be a multiple of 16 in [16, 32768]")
+    y, cy = _fp8_out(T, K, _E4M3, x.device)
+    if T:
+        with _on(x.device):
+            _lib.check(_lib.lib().bf16n_fp8_quantize_rows(C.byref(cx), C.byref(cy), T, K, _stream()))
+    return y
+
+
+def add_rmsnorm_fp8(a: torch.Tensor, b: torch.Tensor | None = None, c: torch.Tensor | None = None, ys: torch.Tensor | None = None,
+                    topk_weights: torch.Tensor | None = None, gamma: torch.Tensor | None = None, eps: float = 1e-6,
+                    want_sum: bool = False, want_norm: bool = False):
+    """add_rmsnorm with the norm in 8 bits: s = a + b + c + moe_combine(ys, topk_weights) in FP32, returns Fp8Rows of
+    s * rsqrt(mean(s^2) + eps) * gamma, whose FP32 value is rounded once, to its code.  With want_sum and want_norm a tuple: the rows, bf16(s),
+    the norm in BF16 (for a product that takes BF16, a router's).  a, b, c: [T, n] BF16 contiguous; ys: [T, n_used, n] FP32 with
+    topk_weights [T, n_used]; gamma: [n] BF16; n a multiple of 16, at most 16384."""
+    for t in (a, b, c):
+        if t is not None and not (t.is_cuda and t.dtype == torch.bfloat16 and t.is_contiguous() and t.shape == a.shape and t.dim() == 2):
+            raise ValueError("bf16n.add_rmsnorm_fp8: inputs must be contiguous bf16 [tokens, n] of one shape")
+    T, n = a.shape
+    if n % 16 or not 16 <= n <= 16384:
+        raise ValueError("bf16n.add_rmsnorm_fp8: n must be a multiple of 16 in [16, 16384]")
+    if gamma is not None and not (gamma.is_cuda and gamma.dtype == torch.bfloat16 and gamma.is_contiguous() and gamma.numel() == n):
+        raise ValueError("bf16n.add_rmsnorm_fp8: gamma must be contiguous bf16 [n]")
+    n_used = 0
+    if ys is not None:
+        if not (ys.is_cuda and ys.dtype == torch.float32 and ys.is_contiguous() and ys.dim() == 3 and ys.shape[0] == T and ys.shape[2] == n):
+            raise ValueError("bf16n.add_rmsnorm_fp8: ys must be contiguous f32 [tokens, n_used, n]")
+        n_used, w = ys.shape[1], topk_weights
+        if w is None or not (w.is_cuda and w.is_contiguous() and tuple(w.shape) == (T, n_used) and w.dtype in (torch.float32, torch.bfloat16)):
+            raise ValueError("bf16n.add_rmsnorm_fp8: topk_weights must be contiguous f32/bf16 [tokens, n_used]")
+        if n_used == 0:
+            ys = None
+    else:
+        topk_weights = None
+    if any(t is not None and t.device != a.device for t in (b, c, ys, topk_weights, gamma)):
+        raise ValueError("bf16n.add_rmsnorm_fp8: inputs on different devices")
+    y, cy = _fp8_out(T, n, _E4M3, a.device)
+    ysum = torch.empty_like(a) if want_sum else None
+    ynorm = torch.empty_like(a) if want_norm else None
+    if T:
+        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        with _on(a.device):
+            _lib.check(_lib.lib().bf16n_add_rmsnorm_fp8(
+                a.data_ptr(), ptr(b), ptr(c), ptr(ys), ptr(topk_weights) if ys is not None else None,
+                int(ys is not None and topk_weights.dtype == torch.bfloat16), n_used, ptr(gamma), C.byref(cy), ptr(ysum), ptr(ynorm), T, n,
+                C.c_float(eps), _stream()))
+    return (y, *(t for t in (ysum, ynorm) if t is not None)) if want_sum or want_norm else y
+
+
+def _fp8_mm(what: str, x, w: Fp8Weight, up: Fp8Weight | None, out_dtype: torch.dtype):
+    cw = _c_fp8(w)
+    if w.n_matrices != 1:
+        raise ValueError(f"bf16n.{what}: one matrix, not a stack")
+    cu = None
+    if up is not None:
+        if up.codes.shape != w.codes.shape or up.scales.dtype != w.scales.dtype or up.n_matrices != 1:
+            raise ValueError(f"bf16n.{what}: gate/up shapes and scales must match")
+        cu = C.byref(_c_fp8(up))
+    if out_dtype not in ((torch.bfloat16, torch.float32) if up is None else _FP8_KINDS):
+        raise ValueError(f"bf16n.{what}: results are bf16 or f32" + ("" if up is None else ", or float8_e4m3fn with scales"))
+    cx = _c_rows(what, x, w.K)
+    dev = _device_of(x)
+    if w.codes.device != dev or (up is not None and up.codes.device != dev):
+        raise ValueError(f"bf16n.{what}: operands on different devices")
+    T = (x.codes if isinstance(x, Fp8Rows) else x).shape[0]
+    if out_dtype is _E4M3 and (w.rows % 16 or w.rows == 0):
+        raise ValueError(f"bf16n.{what}: results in 8 bits need a multiple of 16 rows")
+    y, cy = _fp8_out(T, w.rows, out_dtype, dev)
+    if T == 0 or w.rows == 0:
+        return y
+    L, n = _lib.lib(), C.c_uint64()
+    _lib.check(L.bf16n_fp8_workspace_bytes(C.byref(cw), cu is not None, cx.kind, cy.kind, T, 0, 0, C.byref(n)))
+    ws, _keep = _workspace(n.value, dev)
+    with _on(dev):
+        _lib.check(L.bf16n_fp8_mm(C.byref(cw), cu, C.byref(cx), C.byref(cy), T, ws, n.value, _stream()))
+    return y
+
+
+def fp8_linear(x: torch.Tensor | Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """y = x W^T (+ bias) for any number of tokens: Fp8Rows [tokens, K], or BF16 / FP32 activations [..., K], which are taken as
+    fp8_quantize_rows makes them.  Products of a block of 128 columns are summed on the matrix cores and scaled in FP32; out BF16 or FP32
+    (the bias is added in FP32 before the one rounding)."""
+    if isinstance(x, Fp8Rows):
+        x2, lead = x, x.codes.shape[:1]
+    else:
+        if x.dim() == 0 or x.shape[-1] != w.K:
+            raise ValueError(f"bf16n.fp8_linear: x last dim must be K = {w.K}")
+        lead = x.shape[:-1]
+        x2 = x if x.dim() == 2 else x.reshape(-1, w.K)
+        if x2.stride(1) != 1 or x2.stride(0) * x2.element_size() % 16 or x2.data_ptr() % 16:
+            x2 = x2.clone(memory_format=torch.contiguous_format)
+    if bias is None:
+        y = _fp8_mm("fp8_linear", x2, w, None, out_dtype)
+    else:
+        if out_dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError("bf16n.fp8_linear: results are bf16 or f32")
+        y = _fp8_mm("fp8_linear", x2, w, None, torch.float32).add_(bias).to(out_dtype)
+    return y if len(lead) == 1 else y.view(*lead, w.rows)
+
+
+def fp8_linear_glu2(x: torch.Tensor | Fp8Rows, gate: Fp8Weight, up: Fp8Weight, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor | Fp8Rows:
+    """silu(gate x) * (up x) for two matrices of one shape, x [tokens, K] as in fp8_linear.  out BF16, FP32, or float8_e4m3fn: Fp8Rows of the FP32
+    values (rows of the matrices a multiple of 16), what the product behind it takes."""
+    return _fp8_mm("fp8_linear_glu2", x, gate, up, out_dtype)
+
+
+def _check_pairs(what: str, x, topk_ids: torch.Tensor, w: Fp8Weight, n_experts: int) -> int:
+    """The activation rows of a pair's token, or of the pair itself: n_used or 1."""
+    _check_ids(topk_ids)
+    if n_experts != w.n_matrices:
+        raise ValueError(f"bf16n.{what}: the weights are stacks of n_experts matrices")
+    T, n_used = topk_ids.shape
+    if topk_ids.device != _device_of(x) or w.codes.device != topk_ids.device:
+        raise ValueError(f"bf16n.{what}: operands on different devices")
+    rows = (x.codes if isinstance(x, Fp8Rows) else x).shape[0]
+    if rows not in (T, T * n_used):
+        raise ValueError(f"bf16n.{what}: x must have a row for every token or for every (token, slot)")
+    return n_used if rows == T else 1
+
+
+def fp8_moe_mm_ids(x: torch.Tensor | Fp8Rows, topk_ids: torch.Tensor, w: Fp8Weight, n_experts: int, up: Fp8Weight | None = None,
+                   out_dtype: torch.dtype = torch.float32, routes=None):
+    """moe_mm_ids in 8 bits: the rows of the matrices that the ids [T, n_used] name, times x: Fp8Rows or BF16 / FP32 [T, K], or [T * n_used, K] for an
+    activation row to every pair.  Returns [T, n_used, N], zeros for a pair whose id names no expert (a token may name one more than
+    once); up given: silu(w x) * (up x); out_dtype float8_e4m3fn (with up): Fp8Rows [T * n_used, N] for the product behind it.
+    routes: int4_route(topk_ids, n_experts) if the caller has it."""
+    per_token = _check_pairs("fp8_moe_mm_ids", x, topk_ids, w, n_experts)
+    cw, cx = _c_fp8(w), _c_rows("fp8_moe_mm_ids", x, w.K)
+    cu = None
+    if up is not None:
+        if up.codes.shape != w.codes.shape or up.scales.dtype != w.scales.dtype or up.n_matrices != w.n_matrices or up.codes.device != w.codes.device:
+            raise ValueError("bf16n.fp8_moe_mm_ids: gate/up shapes and scales must match")
+        cu = C.byref(_c_fp8(up))
+    if out_dtype not in ((torch.bfloat16, torch.float32) if up is None else _FP8_KINDS):
+        raise ValueError("bf16n.fp8_moe_mm_ids: results are bf16 or f32, or with up float8_e4m3fn with scales")
+    T, n_used = topk_ids.shape
+    N, dev, n = w.rows // n_experts, topk_ids.device, T * n_used
+    if out_dtype is _E4M3 and (N % 16 or N == 0):
+        raise ValueError("bf16n.fp8_moe_mm_ids: results in 8 bits need a multiple of 16 rows")
+    y, cy = _fp8_out(n, N, out_dtype, dev)
+    if n and N:
+        pairs = bounds = None
+        if n > n_experts or routes is not None:
+            pairs, bounds = routes if routes is not None else int4_route(topk_ids, n_experts)
+            if not (pairs.dtype is bounds.dtype is torch.int32 and pairs.numel() == n and bounds.numel() == n_experts + 2
+                    and pairs.is_contiguous() and bounds.is_contiguous() and pairs.device == dev and bounds.device == dev):
+                raise ValueError("bf16n.fp8_moe_mm_ids: routes must be int4_route's for these ids")
+        L, nb, sz = _lib.lib(), C.c_uint64(), topk_ids.element_size()
+        _lib.check(L.bf16n_fp8_workspace_bytes(C.byref(cw), cu is not None, cx.kind, cy.kind, n // per_token, n, pairs is not None, C.byref(nb)))
+        ws, _keep = _workspace(nb.value, dev)
+        with _on(dev):
+            _lib.check(L.bf16n_fp8_mm_ids(C.byref(cw), cu, C.byref(cx), per_token == 1 and n_used != 1, topk_ids.data_ptr(), sz == 8, sz, topk_ids.stride(0) * sz,
+                                          None if pairs is None else pairs.data_ptr(), None if bounds is None else bounds.data_ptr(), C.byref(cy), T, n_used,
+                                          ws, nb.value, _stream()))
+    return y if out_dtype is _E4M3 else y.view(T, n_used, N)
+
+
+def _fp8_experts(what: str, x, gate: Fp8Weight, up: Fp8Weight, down: Fp8Weight, topk_weights: torch.Tensor | None, topk_ids: torch.Tensor, n_experts: int):
+    if gate.codes.shape != up.codes.shape or gate.scales.dtype != up.scales.dtype or not gate.n_matrices == up.n_matrices == down.n_matrices == n_experts:
+        raise ValueError(f"bf16n.{what}: gate, up and down are stacks of n_experts matrices, gate and up of one shape")
+    if _check_pairs(what, x, topk_ids, gate, n_experts) != topk_ids.shape[1]:
+        raise ValueError(f"bf16n.{what}: x must be [tokens, K]")
+    cg, cu, cd, cx = _c_fp8(gate), _c_fp8(up), _c_fp8(down), _c_rows(what, x, gate.K)
+    T, n_used = topk_ids.shape
+    dev, out = topk_ids.device, down.rows // n_experts
+    if down.K != gate.rows // n_experts:
+        raise ValueError(f"bf16n.{what}: down takes the rows of gate and up")
+    if up.codes.device != dev or down.codes.device != dev:
+        raise ValueError(f"bf16n.{what}: operands on different devices")
+    w = topk_weights
+    if w is None:
+        y, cy = _fp8_out(T * n_used, out, torch.float32, dev)
+    else:
+        if not (w.is_cuda and w.device == dev and w.is_contiguous() and tuple(w.shape) == (T, n_used) and w.dtype in (torch.float32, torch.bfloat16)):
+            raise ValueError(f"bf16n.{what}: topk_weights must be contiguous f32/bf16 [tokens, n_used]")
+        y, cy = _fp8_out(T, out, torch.bfloat16, dev)
+    if T == 0 or out == 0 or n_used == 0:
+        return y if w is None else y.zero_()
+    L, nb, sz = _lib.lib(), C.c_uint64(), topk_ids.element_size()
+    _lib.check(L.bf16n_fp8_moe_experts_workspace_bytes(C.byref(cg), C.byref(cd), cx.kind, w is not None, T, n_used, C.byref(nb)))
+    ws, _keep = _workspace(nb.value, dev)
+    with _on(dev):
+        _lib.check(L.bf16n_fp8_moe_experts(C.byref(cg), C.byref(cu), C.byref(cd), C.byref(cx), topk_ids.data_ptr(), sz == 8, sz, topk_ids.stride(0) * sz,
+                                           None if w is None else w.data_ptr(), int(w is not None and w.dtype == torch.bfloat16), C.byref(cy), T, n_used,
+                                           ws, nb.value, _stream()))
+    return y
+
+
+def fp8_moe_experts_rows(x: torch.Tensor | Fp8Rows, gate: Fp8Weight, up: Fp8Weight, down: Fp8Weight, topk_ids: torch.Tensor, n_experts: int) -> torch.Tensor:
+    """The per-(token, slot) outputs down_e(silu(gate_e x) * (up_e x)) of the routed experts, FP32 [T, n_used, H] (moe_experts_rows), x [T, K] as in
+    fp8_linear; the hidden rows are held in 8 bits, each FP32 value rounded once to its code."""
+    T, n_used = topk_ids.shape if topk_ids.dim() == 2 else (0, 0)
+    return _fp8_experts("fp8_moe_experts_rows", x, gate, up, down, None, topk_ids, n_experts).view(T, n_used, down.rows // max(n_experts, 1))
+
+
+def fp8_moe_experts(x: torch.Tensor | Fp8Rows, gate: Fp8Weight, up: Fp8Weight, down: Fp8Weight, topk_weights: torch.Tensor,
+                    topk_ids: torch.Tensor, n_experts: int) -> torch.Tensor:
+    """Routed experts of one MoE layer in 8 bits, BF16 out (moe_experts).  Where the pairs are more than the experts the slots' results
+    are held in BF16 before their weighted sum in FP32 (half a step, 2^-9 of a slot's result, beside the 2^-4 of the codes)."""
+    if topk_weights is None:
+        raise ValueError("bf16n.fp8_moe_experts: topk_weights must be contiguous f32/bf16 [tokens, n_used]")
+    return _fp8_experts("fp8_moe_experts", x, gate, up, down, topk_weights, topk_ids, n_experts)
+
+
 def router_topk_grouped(logits: torch.Tensor, k: int, bias: torch.Tensor | None = None, n_groups: int = 1, topk_groups: int | None = None,
                         scoring: str = "softmax", group_score: str = "max", renorm: bool = True, scale: float = 1.0,
                         out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
