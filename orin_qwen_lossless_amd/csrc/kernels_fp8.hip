@@ -86,31 +86,33 @@ __device__ __forceinline__ float gated(float g, float u) { return silu(g) * u; }
 
 // ---------------------------------------------------------------- few columns
 
-// One wavefront takes 16 rows of the matrix (of each of the two where they are gated) and its part of K; 16 CT columns are the
-// other operand.  A lane's two loads of a step are 16 bytes each of row lane % 16, so that four lanes have half a line and both
-// loads a whole one; weights go from memory to the operand's registers, D steps ahead.  Activations: codes come the same way
-// from L2 (XKIND 0), BF16 and FP32 rows are turned into codes by the block first and kept in LDS.  K in ksplit parts, summed
-// through LDS in a fixed order.
+constexpr int FEW_PARTS = 64; // blocks of K that a wavefront takes at most: their scales are one register's lanes
+
+// One wavefront takes 16 rows of the matrix at a time (of each of the two where they are gated) and its part of K; up to 16 CT columns are the
+// other operand, from LDS, where the block has put their codes first (those of BF16 and FP32 rows it makes itself).  A lane's two
+// loads of a step are 16 bytes each of row lane % 16, so that four lanes have half a line and both loads a whole one; weights go
+// from memory to the operand's registers, D steps ahead, from one 16 rows on to the next.  K in ksplit parts, summed through LDS in a fixed order.
 template <int CT, bool GLU, int XKIND, int NW>
-__global__ void __launch_bounds__(NW * 64) k_fp8_few(const fp8_launch p) {
-    constexpr int NM = GLU ? 2 : 1, D = CT + NM <= 2 ? 8 : 4;
+__global__ void __launch_bounds__(NW * 64, CT * (GLU ? 2 : 1) == 1 ? 4 : CT * (GLU ? 2 : 1) == 2 ? 3 : 2) k_fp8_few(const fp8_launch p) {
+    constexpr int NM = GLU ? 2 : 1, D = GLU ? 2 : 4;
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, m16 = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int KB = p.KB, pitch = KB * FP8_BLOCK + 16;
     float * const lds_scales = (float *) (lds + p.lds_cols * pitch); // [lds_cols][KB]
-    f32x4_t * const red = (f32x4_t *) (lds + (XKIND == CODES ? 0 : (p.lds_cols * (pitch + KB * 4) + 15) / 16 * 16));
+    f32x4_t * const red = (f32x4_t *) (lds + (p.lds_cols * (pitch + KB * 4) + 15) / 16 * 16);
 
     int64_t matrix = 0;
     int begin = 0, end = p.ncols;
-    const int block_rows = NW / p.ksplit * 16, row0 = blockIdx.x * block_rows;
+    const int groups = NW / p.ksplit, kp = wave % p.ksplit, group = wave / p.ksplit;
+    const int row_step = gridDim.x * groups * 16;
     if (p.pairs) {
         matrix = blockIdx.y;
         begin = p.bounds[matrix];
         end = p.bounds[matrix + 1];
         if (matrix == p.n_matrices) {
             for (int c = begin + blockIdx.z; c < end; c += gridDim.z) {
-                zero_row(p, p.pairs[c], row0, block_rows, threadIdx.x, NW * 64);
+                zero_row(p, p.pairs[c], 0, p.nrows, blockIdx.x * NW * 64 + threadIdx.x, gridDim.x * NW * 64);
             }
             return;
         }
@@ -121,202 +123,193 @@ __global__ void __launch_bounds__(NW * 64) k_fp8_few(const fp8_launch p) {
         begin = blockIdx.y;
         end = begin + 1;
         if (matrix < 0 || matrix >= p.n_matrices) {
-            zero_row(p, blockIdx.y, row0, block_rows, threadIdx.x, NW * 64);
+            zero_row(p, blockIdx.y, 0, p.nrows, blockIdx.x * NW * 64 + threadIdx.x, gridDim.x * NW * 64);
             return;
         }
     }
     const auto y_of = [&](int c) -> int64_t { return p.pairs ? p.pairs[c] : c; };
     const auto x_of = [&](int c) -> int64_t { return p.pairs ? row_of_pair(p, p.pairs[c]) : p.ids ? row_of_pair(p, c) : c; };
 
-    const int kp = wave % p.ksplit, s0 = KB * kp / p.ksplit, s1 = KB * (kp + 1) / p.ksplit;
-    const int first = row0 + wave / p.ksplit * 16, row = min(first, p.nrows - 1); // (rows behind the matrix repeat its last: not stored)
-    const int64_t row_off = (int64_t) min(m16, p.nrows - 1 - row) * p.K + q * 16;
-    const uint8_t * from[NM];
-    const void * scales[NM];
-    int64_t scale_row = (matrix * p.NB + row / FP8_BLOCK) * KB;
-#pragma unroll
-    for (int m = 0; m < NM; m++) {
-        from[m] = (m ? p.up : p.w) + (matrix * p.nrows + row) * p.K;
-        scales[m] = m ? p.ups : p.ws;
-    }
-    const bool cut = p.K % FP8_BLOCK != 0;
-    // the last block's chunks behind the matrix's last column: the row's first instead, taken as zeros on both sides
-    const bool out0 = cut && (KB - 1) * FP8_BLOCK + q * 16 >= p.K, out1 = cut && (KB - 1) * FP8_BLOCK + q * 16 + 64 >= p.K;
+    const int s0 = KB * kp / p.ksplit, steps = KB * (kp + 1) / p.ksplit - s0; // (at most FEW_PARTS)
+    const bool cut = p.K % FP8_BLOCK != 0 && s0 + steps == KB;
+    // the last block's chunks behind the matrix's last column: the row's first instead, taken as zeros (the columns' are zeros in LDS)
+    const int last = (KB - 1) * FP8_BLOCK + q * 16;
+    const bool out0 = cut && last >= p.K, out1 = cut && last + 64 >= p.K;
 
-    const int pass = 16 * CT;
+    const int pass = p.lds_cols;
     for (int c0 = begin + (p.ids ? 0 : p.pairs ? blockIdx.z : blockIdx.y) * pass; c0 < end; c0 += (p.ids ? 1 : p.pairs ? gridDim.z : gridDim.y) * pass) {
         const int nc = min(end - c0, pass);
-        u32x4_t w[D][NM][2], x[D][CT][2];
-        float sx[D][CT];
-        const char * x_at[CT];
-        const float * xs_at[CT];
-        if (XKIND == CODES) {
-#pragma unroll
-            for (int t = 0; t < CT; t++) { // (columns behind the last repeat it: not stored)
-                const int64_t r = x_of(c0 + min(t * 16 + m16, nc - 1));
-                x_at[t] = p.x + r * p.x_row + q * 16;
-                xs_at[t] = p.xs + r * p.xs_row;
-            }
-        }
-        const auto load = [&](int s, int u) {
-            const bool last = cut && s == KB - 1;
-            const int64_t k0 = (int64_t) s * FP8_BLOCK - (last && out0 ? s * FP8_BLOCK + q * 16 : 0), k1 = (int64_t) s * FP8_BLOCK + 64 - (last && out1 ? s * FP8_BLOCK + 64 + q * 16 : 0);
+        u32x4_t w[D][NM][2];
+        const uint8_t * at[NM]; // the 16 rows whose loads are under way
+        const void * scales[NM];
+        uint32_t off = 0;
+        float sw[NM], sw_next[NM];
+        const auto at_rows = [&](int r0) { // rows behind the matrix repeat its last: not stored
+            const int row = min(r0, p.nrows - 1);
+            off = min(m16, p.nrows - 1 - row) * p.K + q * 16;
 #pragma unroll
             for (int m = 0; m < NM; m++) {
-                w[u][m][0] = *(const u32x4_t *) (from[m] + row_off + k0);
-                w[u][m][1] = *(const u32x4_t *) (from[m] + row_off + k1);
-            }
-            if (XKIND == CODES) {
-#pragma unroll
-                for (int t = 0; t < CT; t++) {
-                    x[u][t][0] = *(const u32x4_t *) (x_at[t] + k0);
-                    x[u][t][1] = *(const u32x4_t *) (x_at[t] + k1);
-                    sx[u][t] = xs_at[t][s * p.xs_block];
-                }
+                at[m] = (m ? p.up : p.w) + (matrix * p.nrows + row) * p.K + s0 * FP8_BLOCK;
+                sw_next[m] = scale_at(m ? p.ups : p.ws, p.scales_bf16, (matrix * p.NB + row / FP8_BLOCK) * KB + s0 + min(lane, steps - 1));
             }
         };
-#pragma unroll
-        for (int u = 0; u < D; u++) {
-            if (s0 + u < s1) {
-                load(s0 + u, u);
+        const auto load = [&](int i, int u) {
+            uint32_t k0 = off, k1 = off + 64;
+            if (cut && i == steps - 1) {
+                k0 -= out0 ? last : 0;
+                k1 -= out1 ? last + 64 : 0;
             }
-        }
-        if (XKIND != CODES) { // 16 lanes to a block of a column
-            __syncthreads();
-            for (int i = threadIdx.x >> 4; i < nc * KB; i += NW * 4) {
-                const int c = i / KB, b = i - c * KB, k = b * FP8_BLOCK + (threadIdx.x & 15) * 8;
-                const char * src = p.x + x_of(c0 + c) * p.x_row + (int64_t) k * (XKIND == BF16 ? 2 : 4);
-                float v[8] = {};
-                if (k < p.K) {
-                    if (XKIND == BF16) {
-                        bf16x8_to_f32(*(const u32x4_t *) src, v);
-                    } else {
-                        const f32x4_t a = *(const f32x4_t *) src, d = *(const f32x4_t *) (src + 16);
-#pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            v[j] = j < 4 ? a[j & 3] : d[j & 3];
-                        }
-                    }
-                }
-                const fp8_scales s = fp8_scales_of(row_max_dpp(most_of8(v)));
-                *(u32x2_t *) (lds + c * pitch + k) = fp8_pack8(v, s.inverse);
-                if ((threadIdx.x & 15) == 0) {
-                    lds_scales[c * KB + b] = s.scale;
-                }
-            }
-            __syncthreads();
-        }
-
-        f32x4_t acc[NM][CT] = {};
-        float sw[NM] = {}; // scales of 64 blocks, one to a lane
-        for (int base = s0; base < s1; base += D) {
-#pragma unroll
-            for (int u = 0; u < D; u++) {
-                const int s = base + u;
-                if (s >= s1) {
-                    break;
-                }
-                if ((s - s0) % 64 == 0) {
-#pragma unroll
-                    for (int m = 0; m < NM; m++) {
-                        sw[m] = scale_at(scales[m], p.scales_bf16, scale_row + min(s + lane, KB - 1));
-                    }
-                }
-                if (cut && s == KB - 1) {
-#pragma unroll
-                    for (int m = 0; m < NM; m++) {
-                        w[u][m][0] = out0 ? u32x4_t{} : w[u][m][0];
-                        w[u][m][1] = out1 ? u32x4_t{} : w[u][m][1];
-                    }
-                    if (XKIND == CODES) {
-#pragma unroll
-                        for (int t = 0; t < CT; t++) {
-                            x[u][t][0] = out0 ? u32x4_t{} : x[u][t][0];
-                            x[u][t][1] = out1 ? u32x4_t{} : x[u][t][1];
-                        }
-                    }
-                }
-                if (XKIND != CODES) {
-#pragma unroll
-                    for (int t = 0; t < CT; t++) {
-                        const int c = min(t * 16 + m16, nc - 1);
-                        const char * at = lds + c * pitch + s * FP8_BLOCK + q * 16;
-                        x[u][t][0] = *(const u32x4_t *) at;
-                        x[u][t][1] = *(const u32x4_t *) (at + 64);
-                        sx[u][t] = lds_scales[c * KB + s];
-                    }
-                }
-                f32x4_t part[NM][CT];
-                fp8_wide xw[CT];
-#pragma unroll
-                for (int t = 0; t < CT; t++) {
-                    xw[t] = fp8_widen(x[u][t][0], x[u][t][1]);
-                }
-#pragma unroll
-                for (int m = 0; m < NM; m++) {
-                    const fp8_wide ww = fp8_widen(w[u][m][0], w[u][m][1]);
-#pragma unroll
-                    for (int t = 0; t < CT; t++) {
-                        part[m][t] = fp8_sum16(ww, xw[t]);
-                    }
-                }
-#pragma unroll
-                for (int m = 0; m < NM; m++) {
-                    const float ws = __uint_as_float((uint32_t) __builtin_amdgcn_readlane((int) __float_as_uint(sw[m]), (s - s0) % 64));
-#pragma unroll
-                    for (int t = 0; t < CT; t++) {
-                        const float both = ws * sx[u][t];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            acc[m][t][e] = fmaf(part[m][t][e], both, acc[m][t][e]);
-                        }
-                    }
-                }
-                if (s + D < s1) {
-                    load(s + D, u);
-                }
-            }
-        }
-        if (p.ksplit > 1) {
-            __syncthreads();
 #pragma unroll
             for (int m = 0; m < NM; m++) {
-#pragma unroll
-                for (int t = 0; t < CT; t++) {
-                    red[((wave * NM + m) * CT + t) * 64 + lane] = acc[m][t];
-                }
+                // (an offset of a chunk behind the last column goes back to column 0: added in 64 bits)
+                w[u][m][0] = *(const u32x4_t *) (at[m] + i * FP8_BLOCK + (int64_t) (int32_t) k0);
+                w[u][m][1] = *(const u32x4_t *) (at[m] + i * FP8_BLOCK + (int64_t) (int32_t) k1);
             }
-            __syncthreads();
-            if (kp != 0) {
+        };
+        const int first_row = (blockIdx.x * groups + group) * 16;
+        at_rows(first_row);
+#pragma unroll
+        for (int u = 0; u < D; u++) {
+            if (u < steps) {
+                load(u, u);
+            }
+        }
+        // codes and scales of the columns, 16 lanes to a block of 128
+        __syncthreads();
+        for (int i = threadIdx.x >> 4; i < nc * KB; i += NW * 4) {
+            const int c = i / KB, b = i - c * KB, k = b * FP8_BLOCK + (threadIdx.x & 15) * 8;
+            const int64_t r = x_of(c0 + c);
+            const char * src = p.x + r * p.x_row + (int64_t) k * (XKIND == BF16 ? 2 : XKIND == F32 ? 4 : 1);
+            if (XKIND == CODES) {
+                *(u32x2_t *) (lds + c * pitch + k) = k < p.K ? *(const u32x2_t *) src : u32x2_t{};
+                if ((threadIdx.x & 15) == 0) {
+                    lds_scales[c * KB + b] = p.xs[r * p.xs_row + b * p.xs_block];
+                }
                 continue;
             }
-            for (int i = 1; i < p.ksplit; i++) {
+            float v[8] = {};
+            if (k < p.K) {
+                if (XKIND == BF16) {
+                    bf16x8_to_f32(*(const u32x4_t *) src, v);
+                } else {
+                    const f32x4_t a = *(const f32x4_t *) src, d = *(const f32x4_t *) (src + 16);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        v[j] = j < 4 ? a[j & 3] : d[j & 3];
+                    }
+                }
+            }
+            const fp8_scales s = fp8_scales_of(row_max_dpp(most_of8(v)));
+            *(u32x2_t *) (lds + c * pitch + k) = fp8_pack8(v, s.inverse);
+            if ((threadIdx.x & 15) == 0) {
+                lds_scales[c * KB + b] = s.scale;
+            }
+        }
+        __syncthreads();
+
+        const char * x_at[CT];
+        const float * sx_at[CT];
+#pragma unroll
+        for (int t = 0; t < CT; t++) { // (columns behind the last repeat it: not stored)
+            const int c = min(t * 16 + m16, nc - 1);
+            x_at[t] = lds + c * pitch + s0 * FP8_BLOCK + q * 16;
+            sx_at[t] = lds_scales + c * KB + s0;
+        }
+        for (int r0 = first_row; r0 < p.nrows + group * 16; r0 += row_step) { // (the block's wavefronts make the same rounds)
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                sw[m] = sw_next[m];
+            }
+            f32x4_t acc[NM][CT] = {};
+            const bool more = r0 + row_step < p.nrows + group * 16;
+            for (int base = 0; base < steps; base += D) {
+#pragma unroll
+                for (int u = 0; u < D; u++) {
+                    const int i = base + u;
+                    if (i >= steps) {
+                        break;
+                    }
+                    if (cut && i == steps - 1) {
+#pragma unroll
+                        for (int m = 0; m < NM; m++) {
+                            w[u][m][0] = out0 ? u32x4_t{} : w[u][m][0];
+                            w[u][m][1] = out1 ? u32x4_t{} : w[u][m][1];
+                        }
+                    }
+                    fp8_wide ww[NM];
+#pragma unroll
+                    for (int m = 0; m < NM; m++) {
+                        ww[m] = fp8_widen(w[u][m][0], w[u][m][1]);
+                    }
+                    if (i + D < steps) {
+                        load(i + D, u);
+                    }
+#pragma unroll
+                    for (int t = 0; t < CT; t++) {
+                        const fp8_wide xw = fp8_widen(*(const u32x4_t *) (x_at[t] + i * FP8_BLOCK), *(const u32x4_t *) (x_at[t] + i * FP8_BLOCK + 64));
+                        const float sx = sx_at[t][i];
+#pragma unroll
+                        for (int m = 0; m < NM; m++) {
+                            const f32x4_t part = fp8_sum16(ww[m], xw);
+                            const float both = __uint_as_float((uint32_t) __builtin_amdgcn_readlane((int) __float_as_uint(sw[m]), i)) * sx;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                acc[m][t][e] = fmaf(part[e], both, acc[m][t][e]);
+                            }
+                        }
+                    }
+                }
+            }
+            if (more) {
+                at_rows(r0 + row_step);
+#pragma unroll
+                for (int u = 0; u < D; u++) {
+                    if (u < steps) {
+                        load(u, u);
+                    }
+                }
+            }
+            if (p.ksplit > 1) {
+                __syncthreads();
 #pragma unroll
                 for (int m = 0; m < NM; m++) {
 #pragma unroll
                     for (int t = 0; t < CT; t++) {
-                        acc[m][t] += red[(((wave + i) * NM + m) * CT + t) * 64 + lane];
+                        red[((wave * NM + m) * CT + t) * 64 + lane] = acc[m][t];
+                    }
+                }
+                __syncthreads();
+                if (kp != 0) {
+                    continue;
+                }
+                for (int i = 1; i < p.ksplit; i++) {
+#pragma unroll
+                    for (int m = 0; m < NM; m++) {
+#pragma unroll
+                        for (int t = 0; t < CT; t++) {
+                            acc[m][t] += red[(((wave + i) * NM + m) * CT + t) * 64 + lane];
+                        }
                     }
                 }
             }
-        }
 #pragma unroll
-        for (int t = 0; t < CT; t++) {
-            const int c = t * 16 + m16;
-            if (c >= nc) {
-                continue;
-            }
-            f32x4_t v = acc[0][t];
-            if (GLU) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    v[e] = gated(v[e], acc[NM - 1][t][e]);
+            for (int t = 0; t < CT; t++) {
+                const int c = t * 16 + m16;
+                if (c >= nc) {
+                    continue;
                 }
-            }
-            if (p.y_kind == BF16) {
-                store4<BF16>(p, y_of(c0 + c), first + 4 * q, v);
-            } else {
-                store4<F32>(p, y_of(c0 + c), first + 4 * q, v);
+                f32x4_t v = acc[0][t];
+                if (GLU) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        v[e] = gated(v[e], acc[NM - 1][t][e]);
+                    }
+                }
+                if (p.y_kind == BF16) {
+                    store4<BF16>(p, y_of(c0 + c), r0 + 4 * q, v);
+                } else {
+                    store4<F32>(p, y_of(c0 + c), r0 + 4 * q, v);
+                }
             }
         }
     }
@@ -328,12 +321,13 @@ __device__ __align__(16) const uint32_t g_zeros[4] = {0, 0, 0, 0};
 
 // WR x WC wavefronts, RT x CT results of 16 x 16 to each.  Codes of both sides go straight into LDS, a step of 128 columns ahead:
 // rows of 128 bytes, their eight places of 16 bytes exchanged by the row's low bits so that the operands' reads find every
-// bank.  A step's products start from zero and are added to the results times their scales.  BF16 results are summed by the instruction
+// bank.  A step's products start from zero and are added to the results times their scales, those of a row of tiles while the next row's
+// are under way.  BF16 results are summed by the instruction
 // on the codes.  FP32 ones are summed from BF16 operands (fp8_sum16), and so are those that become codes with a scale, which a value
 // 1.5e-5 off would put on the other side of a border now and then (0.0015 of the norm of 300 rows of 1408 that are 0.0003 off so).
 // Lists: a block takes the columns of one matrix, COLS at a time.  OUT8: the results of ROWS = 128 rows leave as codes with a scale.
 template <int WR, int WC, int RT, int CT, bool GLU, bool LIST, int OUT>
-__global__ void __launch_bounds__(WR * WC * 64) k_fp8_many(const fp8_launch p) {
+__global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p) {
     constexpr bool WIDE = OUT != BF16;
     constexpr int NM = GLU ? 2 : 1, THREADS = WR * WC * 64, A_ROWS = WR * RT * 16, ROWS = A_ROWS / NM, COLS = WC * CT * 16;
     constexpr int STAGE = (A_ROWS + COLS) * FP8_BLOCK, A_COPIES = A_ROWS * 8 / THREADS, B_COPIES = COLS * 8 / THREADS, TM = RT / NM;
@@ -359,6 +353,8 @@ __global__ void __launch_bounds__(WR * WC * 64) k_fp8_many(const fp8_launch p) {
         }
         begin += blockIdx.z * COLS;
     } else {
+        // An XCD takes every eighth block, which is made a contiguous part of the tiles here: four column tiles of one row tile
+        // after the other, so that what runs there at a time shares few pieces of either side.
         const int row_tiles = (p.nrows + ROWS - 1) / ROWS, col_tiles = (p.ncols + COLS - 1) / COLS;
         const int n = row_tiles * col_tiles, per = (n + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
         if ((int) (blockIdx.x >> 3) >= per || id >= n) {
@@ -374,7 +370,6 @@ __global__ void __launch_bounds__(WR * WC * 64) k_fp8_many(const fp8_launch p) {
 
     // what this thread copies: a place of rows (threadIdx.x >> 3) + i * THREADS / 8, chunk by the row's low bits
     const int chunk = (threadIdx.x & 7) ^ ((threadIdx.x >> 3) & 7);
-    const bool behind = cut && (KB - 1) * FP8_BLOCK + chunk * 16 >= p.K;
     const uint8_t * const w_base = p.w + (matrix * p.nrows + row0) * p.K, * const up_base = p.up + (matrix * p.nrows + row0) * p.K;
     uint32_t a_off[A_COPIES];
     const auto of_up = [&](int i) { return GLU && (i * (THREADS / 8) + wave * 8) / 16 % RT >= TM; };
@@ -390,36 +385,51 @@ __global__ void __launch_bounds__(WR * WC * 64) k_fp8_many(const fp8_launch p) {
 
     for (int c0 = begin; c0 < end; c0 += LIST ? gridDim.z * COLS : COLS) {
         const int nc = min(end - c0, COLS);
-        const auto x_of = [&](int i) { return LIST ? row_of_pair(p, p.pairs[c0 + min(i, nc - 1)]) : c0 + min(i, nc - 1); };
+        const auto x_of = [&](int i) -> int64_t { return LIST ? row_of_pair(p, p.pairs[c0 + min(i, nc - 1)]) : c0 + min(i, nc - 1); };
         const char * b_at[B_COPIES];
+        const float * sx_at[CT];
 #pragma unroll
         for (int i = 0; i < B_COPIES; i++) {
             b_at[i] = p.x + x_of(i * (THREADS / 8) + (threadIdx.x >> 3)) * p.x_row + chunk * 16;
         }
-        const float * sx_at[CT];
 #pragma unroll
         for (int c = 0; c < CT; c++) {
             sx_at[c] = p.xs + x_of((c * WC + wc) * 16 + m16) * p.xs_row;
         }
         float sx_next[CT], sw[NM];
         const auto copy = [&](int s, int buf) {
-            const bool none = behind && s == KB - 1;
+            char * const to = lds + buf * STAGE + wave * 1024;
+            const uint8_t * const wk = w_base + s * FP8_BLOCK, * const uk = up_base + s * FP8_BLOCK;
+            const int64_t k = s * FP8_BLOCK, sk = s * p.xs_block;
+            if (cut && s == KB - 1) { // chunks behind the last column are zeros on both sides
+                const bool none = s * FP8_BLOCK + chunk * 16 >= p.K;
 #pragma unroll
-            for (int i = 0; i < A_COPIES; i++) {
-                const uint8_t * src = (of_up(i) ? up_base : w_base) + s * FP8_BLOCK + a_off[i];
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (none ? (const uint8_t *) g_zeros : src),
-                                                 (__attribute__((address_space(3))) void *) (lds + buf * STAGE + i * THREADS * 16 + wave * 1024), 16, 0, 0);
-            }
+                for (int i = 0; i < A_COPIES; i++) {
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (none ? (const uint8_t *) g_zeros : (of_up(i) ? uk : wk) + a_off[i]),
+                                                     (__attribute__((address_space(3))) void *) (to + i * THREADS * 16), 16, 0, 0);
+                }
 #pragma unroll
-            for (int i = 0; i < B_COPIES; i++) {
-                if (!LIST || i * (THREADS / 8) < nc) {
-                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (none ? (const char *) g_zeros : b_at[i] + s * FP8_BLOCK),
-                                                     (__attribute__((address_space(3))) void *) (lds + buf * STAGE + A_ROWS * FP8_BLOCK + i * THREADS * 16 + wave * 1024), 16, 0, 0);
+                for (int i = 0; i < B_COPIES; i++) {
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (none ? (const char *) g_zeros : b_at[i] + k),
+                                                     (__attribute__((address_space(3))) void *) (to + A_ROWS * FP8_BLOCK + i * THREADS * 16), 16, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < A_COPIES; i++) {
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) ((of_up(i) ? uk : wk) + a_off[i]),
+                                                     (__attribute__((address_space(3))) void *) (to + i * THREADS * 16), 16, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < B_COPIES; i++) {
+                    if (!LIST || i * (THREADS / 8) < nc) {
+                        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (b_at[i] + k),
+                                                         (__attribute__((address_space(3))) void *) (to + A_ROWS * FP8_BLOCK + i * THREADS * 16), 16, 0, 0);
+                    }
                 }
             }
 #pragma unroll
             for (int c = 0; c < CT; c++) {
-                sx_next[c] = sx_at[c][s * p.xs_block];
+                sx_next[c] = sx_at[c][sk];
             }
         };
         f32x4_t acc[RT][CT] = {};
@@ -429,61 +439,69 @@ __global__ void __launch_bounds__(WR * WC * 64) k_fp8_many(const fp8_launch p) {
         // their sums behind the branches, where on some ways too few cycles pass between a product and the read of its result)
         const auto steps = [&](auto columns) {
             constexpr int M = decltype(columns)::value;
-            for (int s = 0; s < KB; s++) {
-                __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0): this wavefront's copies are in LDS
-                __syncthreads();                    // all of them are, and nothing reads the other buffer any more
-                float sx[CT];
-#pragma unroll
-                for (int c = 0; c < CT; c++) {
-                    sx[c] = sx_next[c];
-                }
-                if (s % 64 == 0) {
-#pragma unroll
-                    for (int m = 0; m < NM; m++) {
-                        sw[m] = scale_at(m ? p.ups : p.ws, p.scales_bf16, scale_row + min(s + lane, KB - 1));
-                    }
-                }
-                if (s + 1 < KB) {
-                    copy(s + 1, (s + 1) & 1);
-                }
-                const char * const at = lds + (s & 1) * STAGE;
-                float both[NM][M];
+            for (int s64 = 0; s64 < KB; s64 += 64) { // 64 steps' scales of the wavefront's rows, one to a lane
 #pragma unroll
                 for (int m = 0; m < NM; m++) {
-                    const float ws = __uint_as_float((uint32_t) __builtin_amdgcn_readlane((int) __float_as_uint(sw[m]), s % 64));
-#pragma unroll
-                    for (int c = 0; c < M; c++) {
-                        both[m][c] = ws * sx[c];
-                    }
+                    sw[m] = scale_at(m ? p.ups : p.ws, p.scales_bf16, scale_row + min(s64 + lane, KB - 1));
                 }
-                u32x4_t b[M][2];
-                fp8_wide bw[M];
+                const int s_end = min(s64 + 64, KB);
+                for (int s = s64; s < s_end; s++) {
+                    __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0): this wavefront's copies are in LDS
+                    __syncthreads();                    // all of them are, and nothing reads the other buffer any more
+                    float both[NM][M];
 #pragma unroll
-                for (int c = 0; c < M; c++) {
-                    b[c][0] = *(const u32x4_t *) (at + b_frag + c * WC * 16 * FP8_BLOCK + frag0);
-                    b[c][1] = *(const u32x4_t *) (at + b_frag + c * WC * 16 * FP8_BLOCK + frag1);
-                    if constexpr (WIDE) {
-                        bw[c] = fp8_widen(b[c][0], b[c][1]);
-                    }
-                }
+                    for (int m = 0; m < NM; m++) {
+                        const float ws = __uint_as_float((uint32_t) __builtin_amdgcn_readlane((int) __float_as_uint(sw[m]), s - s64));
 #pragma unroll
-                for (int t = 0; t < RT; t++) {
-                    const u32x4_t a0 = *(const u32x4_t *) (at + a_frag + t * 16 * FP8_BLOCK + frag0), a1 = *(const u32x4_t *) (at + a_frag + t * 16 * FP8_BLOCK + frag1);
-                    fp8_wide aw;
-                    if constexpr (WIDE) {
-                        aw = fp8_widen(a0, a1);
-                    }
-#pragma unroll
-                    for (int c = 0; c < M; c++) {
-                        f32x4_t part;
-                        if constexpr (WIDE) {
-                            part = fp8_sum16(aw, bw[c]);
-                        } else {
-                            part = fp8_sum8(a0, a1, b[c][0], b[c][1]);
+                        for (int c = 0; c < M; c++) {
+                            both[m][c] = ws * sx_next[c];
                         }
+                    }
+                    if (s + 1 < KB) {
+                        copy(s + 1, (s + 1) & 1);
+                    }
+                    const char * const at = lds + (s & 1) * STAGE;
+                    u32x4_t b[M][2], a[2][2];
+                    fp8_wide bw[M];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            acc[t][c][e] = fmaf(part[e], both[t / TM][c], acc[t][c][e]);
+                    for (int c = 0; c < M; c++) {
+                        b[c][0] = *(const u32x4_t *) (at + b_frag + c * WC * 16 * FP8_BLOCK + frag0);
+                        b[c][1] = *(const u32x4_t *) (at + b_frag + c * WC * 16 * FP8_BLOCK + frag1);
+                        if constexpr (WIDE) {
+                            bw[c] = fp8_widen(b[c][0], b[c][1]);
+                        }
+                    }
+                    a[0][0] = *(const u32x4_t *) (at + a_frag + frag0);
+                    a[0][1] = *(const u32x4_t *) (at + a_frag + frag1);
+                    f32x4_t part[2][M];
+#pragma unroll
+                    for (int t = 0; t <= RT; t++) {
+                        if (t < RT) {
+                            if (t + 1 < RT) {
+                                a[(t + 1) & 1][0] = *(const u32x4_t *) (at + a_frag + (t + 1) * 16 * FP8_BLOCK + frag0);
+                                a[(t + 1) & 1][1] = *(const u32x4_t *) (at + a_frag + (t + 1) * 16 * FP8_BLOCK + frag1);
+                            }
+                            fp8_wide aw;
+                            if constexpr (WIDE) {
+                                aw = fp8_widen(a[t & 1][0], a[t & 1][1]);
+                            }
+#pragma unroll
+                            for (int c = 0; c < M; c++) {
+                                if constexpr (WIDE) {
+                                    part[t & 1][c] = fp8_sum16(aw, bw[c]);
+                                } else {
+                                    part[t & 1][c] = fp8_sum8(a[t & 1][0], a[t & 1][1], b[c][0], b[c][1]);
+                                }
+                            }
+                        }
+                        if (t > 0) {
+#pragma unroll
+                            for (int c = 0; c < M; c++) {
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    acc[t - 1][c][e] = fmaf(part[(t - 1) & 1][c][e], both[(t - 1) / TM][c], acc[t - 1][c][e]);
+                                }
+                            }
                         }
                     }
                 }
@@ -758,20 +776,30 @@ void few_go(const fp8_launch & p, dim3 grid, size_t lds, hipStream_t stream) {
     k_fp8_few<CT, GLU, XKIND, NW><<<grid, NW * 64, lds, stream>>>(p);
 }
 
-constexpr int FEW_LDS = 64 * 1024; // of a block, its sums over the parts of K and converted columns
+constexpr size_t FEW_LDS = 160 * 1024 - 1024;
 
-size_t few_red(int ct, bool glu, int nw) { return (size_t) nw * (glu ? 2 : 1) * ct * 1024; }
-size_t few_staged(int cols, int KB) { return ((size_t) cols * (KB * FP8_BLOCK + 16 + KB * 4) + 15) / 16 * 16; }
+size_t few_lds(int cols, int KB, int ct, bool glu, int nw, int ksplit) {
+    return ((size_t) cols * (KB * FP8_BLOCK + 16 + KB * 4) + 15) / 16 * 16 + (ksplit > 1 ? (size_t) nw * (glu ? 2 : 1) * ct * 1024 : 0);
+}
 
-void run_few(fp8_launch p, bool glu, int most_cols, int64_t busy, int y_blocks, int z_blocks, int cus, hipStream_t stream) {
-    const int ct = most_cols <= 16 ? 1 : 2;
+// cols: columns of a pass; busy: matrices or passes that have columns; blocks: of them all, grid.y
+void run_few(fp8_launch p, bool glu, int cols, int64_t busy, int y_blocks, int cus, hipStream_t stream) {
     const int64_t tiles = (p.nrows + 15) / 16 * busy;
     const int nw = tiles <= 4 * cus ? 8 : 4;
-    p.ksplit = nw == 8 ? std::min(8, p.KB >= 8 ? 8 : p.KB >= 4 ? 4 : p.KB >= 2 ? 2 : 1) : tiles <= 16 * cus && p.KB >= 4 ? 4 : 1;
-    p.lds_cols = std::min(most_cols, 16 * ct);
-    const size_t lds = (p.x_kind == CODES ? 0 : few_staged(p.lds_cols, p.KB)) + (p.ksplit > 1 ? few_red(ct, glu, nw) : 0);
-    const int rows = nw / p.ksplit * 16;
-    const dim3 grid((p.nrows + rows - 1) / rows, y_blocks, z_blocks);
+    int ksplit = nw == 8 ? 8 : tiles <= 16 * cus ? 4 : 1;
+    while (ksplit > 1 && p.KB < ksplit * 2) {
+        ksplit /= 2;
+    }
+    while ((p.KB + ksplit - 1) / ksplit > FEW_PARTS) {
+        ksplit *= 2;
+    }
+    p.ksplit = ksplit;
+    p.lds_cols = cols;
+    const int ct = cols <= 16 ? 1 : 2, rows = nw / ksplit * 16, n_blocks = (p.nrows + rows - 1) / rows;
+    const size_t lds = few_lds(cols, p.KB, ct, glu, nw, ksplit);
+    const int room = cus * (int) std::min<size_t>(nw == 8 ? 2 : 4, LDS_BYTES / lds);
+    const int rounds = (int) std::max<int64_t>(1, std::min<int64_t>(8, (int64_t) n_blocks * busy / room));
+    const dim3 grid((n_blocks + rounds - 1) / rounds, y_blocks, 1);
     const auto by_kind = [&](auto c, auto g, auto n) {
         constexpr int C = decltype(c)::value, N = decltype(n)::value;
         constexpr bool G = decltype(g)::value;
@@ -780,6 +808,22 @@ void run_few(fp8_launch p, bool glu, int most_cols, int64_t busy, int y_blocks, 
     const auto by_nw = [&](auto c, auto g) { nw == 8 ? by_kind(c, g, std::integral_constant<int, 8>{}) : by_kind(c, g, std::integral_constant<int, 4>{}); };
     const auto by_ct = [&](auto g) { ct == 1 ? by_nw(std::integral_constant<int, 1>{}, g) : by_nw(std::integral_constant<int, 2>{}, g); };
     glu ? by_ct(std::true_type{}) : by_ct(std::false_type{});
+}
+
+template <int CT, bool GLU, int NW>
+void few_init() {
+    (void) hipFuncSetAttribute((const void *) k_fp8_few<CT, GLU, CODES, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, (int) FEW_LDS);
+    (void) hipFuncSetAttribute((const void *) k_fp8_few<CT, GLU, BF16, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, (int) FEW_LDS);
+    (void) hipFuncSetAttribute((const void *) k_fp8_few<CT, GLU, F32, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, (int) FEW_LDS);
+}
+
+// columns of a pass of k_fp8_few: as many as are there, 32 at most, and what LDS holds
+int few_pass(int64_t cols, int KB, bool glu) {
+    int n = (int) std::min<int64_t>(cols, 32);
+    while (n > 1 && few_lds(n, KB, n <= 16 ? 1 : 2, glu, 8, 8) > FEW_LDS) {
+        n--;
+    }
+    return n;
 }
 
 template <int WR, int WC, int RT, int CT, bool GLU, bool LIST, int OUT>
@@ -812,17 +856,20 @@ constexpr int FEW_COLUMNS = 32;
 bool few(const bf16n_fp8_weight & w, int64_t n_cols, bool listed, bool by_ids) {
     return by_ids || (listed ? n_cols <= 12 * (int64_t) w.n_matrices : n_cols <= FEW_COLUMNS);
 }
-// whether the block converts rows that are not codes by itself
-bool converts(const bf16n_fp8_weight & w, int64_t n_cols, bool by_ids, bool glu) {
-    const int KB = (int) ((w.K + FP8_BLOCK - 1) / FP8_BLOCK), cols = by_ids ? 1 : (int) std::min<int64_t>(n_cols, FEW_COLUMNS);
-    return few_staged(cols, KB) + few_red(cols <= 16 ? 1 : 2, glu, 8) <= FEW_LDS;
-}
 size_t aligned(size_t n) { return (n + 255) / 256 * 256; }
 size_t codes_bytes(int64_t rows, int64_t K) { return aligned(rows * K) + aligned(rows * ((K + FP8_BLOCK - 1) / FP8_BLOCK) * 4); }
 
 } // namespace
 
 void fp8_init() {
+    few_init<1, false, 4>();
+    few_init<1, false, 8>();
+    few_init<2, false, 4>();
+    few_init<2, false, 8>();
+    few_init<1, true, 4>();
+    few_init<1, true, 8>();
+    few_init<2, true, 4>();
+    few_init<2, true, 8>();
     many_init<4, 2, 4, 4, true, true, CODES>();
     many_init<4, 2, 4, 4, true, true, BF16>();
     many_init<4, 2, 4, 4, true, true, F32>();
@@ -846,7 +893,7 @@ void launch_add_rmsnorm_fp8(const add_norm_args & a, const bf16n_fp8_rows & y, i
 uint64_t fp8_workspace_bytes(const bf16n_fp8_weight & w, bool glu, int x_kind, int y_kind, int64_t x_rows, int64_t n_cols, bool listed, bool by_ids) {
     const bool f = few(w, n_cols, listed, by_ids);
     uint64_t n = 0;
-    if (x_kind != CODES && (!f || listed || !converts(w, n_cols, by_ids, glu))) {
+    if (x_kind != CODES && !f) {
         n += codes_bytes(x_rows, w.K);
     }
     if (y_kind == CODES && f) {
@@ -860,7 +907,7 @@ void launch_fp8_product(const fp8_product & a, void * workspace, int cus, hipStr
     const bool f = few(*a.w, a.n_cols, listed, by_ids);
     fp8_launch p = launch_of(a);
     char * ws = (char *) workspace;
-    if (p.x_kind != CODES && (!f || listed || !converts(*a.w, a.n_cols, by_ids, glu))) {
+    if (p.x_kind != CODES && !f) {
         const bf16n_fp8_rows codes = {ws, (float *) (ws + aligned(a.x_rows * a.w->K)), a.w->K, 1, a.x_rows, CODES, 0};
         launch_fp8_rows(a.x, codes, a.x_rows, a.w->K, cus, stream);
         p.x = ws; p.x_row = a.w->K; p.xs = codes.scales; p.xs_row = 1; p.xs_block = a.x_rows; p.x_kind = CODES;
@@ -876,12 +923,12 @@ void launch_fp8_product(const fp8_product & a, void * workspace, int cus, hipStr
         p.y = ws; p.y_row = plain.row; p.y_kind = F32;
     }
     if (by_ids) {
-        run_few(p, glu, 1, a.n_cols, (int) a.n_cols, 1, cus, stream);
+        run_few(p, glu, 1, a.n_cols, (int) a.n_cols, cus, stream);
     } else if (listed) {
-        run_few(p, glu, 16, std::min<int64_t>(a.n_cols, p.n_matrices), (int) p.n_matrices + 1, 1, cus, stream);
+        run_few(p, glu, few_pass(std::min<int64_t>(a.n_cols, 16), p.KB, glu), std::min<int64_t>(a.n_cols, p.n_matrices), (int) p.n_matrices + 1, cus, stream);
     } else {
-        const int ct = a.n_cols <= 16 ? 1 : 2, passes = (int) ((a.n_cols + 16 * ct - 1) / (16 * ct));
-        run_few(p, glu, (int) std::min<int64_t>(a.n_cols, 16 * ct), passes, passes, 1, cus, stream);
+        const int pass = few_pass(a.n_cols, p.KB, glu), passes = (int) ((a.n_cols + pass - 1) / pass);
+        run_few(p, glu, pass, passes, passes, cus, stream);
     }
     if (plain.at) {
         launch_fp8_rows(plain, a.y, a.n_cols, p.nrows, cus, stream);
