@@ -28,7 +28,7 @@ struct fp8_launch {
     uint32_t per_token, one_per;            // the activation row of a pair is pair / per_token; 2^32 / per_token, rounded down
     const char * ids; int64_t ids_s0, ids_s1; bool ids_i64; int n_used; // one matrix per pair
     const int32_t * pairs, * bounds;        // pairs sorted by matrix
-    int ksplit, lds_cols;
+    int ksplit, lds_cols, cus;
 };
 
 __device__ __forceinline__ float scale_at(const void * s, bool bf16, int64_t i) {
@@ -141,7 +141,6 @@ __global__ void __launch_bounds__(NW * 64, CT * (GLU ? 2 : 1) == 1 ? 4 : CT * (G
         const int nc = min(end - c0, pass);
         u32x4_t w[D][NM][2];
         const uint8_t * at[NM]; // the 16 rows whose loads are under way
-        const void * scales[NM];
         uint32_t off = 0;
         float sw[NM], sw_next[NM];
         const auto at_rows = [&](int r0) { // rows behind the matrix repeat its last: not stored
@@ -319,19 +318,35 @@ __global__ void __launch_bounds__(NW * 64, CT * (GLU ? 2 : 1) == 1 ? 4 : CT * (G
 
 __device__ __align__(16) const uint32_t g_zeros[4] = {0, 0, 0, 0};
 
-// WR x WC wavefronts, RT x CT results of 16 x 16 to each.  Codes of both sides go straight into LDS, a step of 128 columns ahead:
+// rows of columns' codes that the threads copy at least, eight threads to a row
+__host__ __device__ constexpr int many_x_rows(int cols, int threads) { return (cols * 8 + threads - 1) / threads * (threads / 8); }
+// LDS of a step: the rows of both sides and the columns' scales (of 64 columns at least)
+__host__ __device__ constexpr int many_stage(int a_rows, int cols, int threads) {
+    return (a_rows + many_x_rows(cols, threads)) * FP8_BLOCK + (cols < 64 ? 64 : cols) * 4;
+}
+
+// vector memory operations under way: at most N, and no read of LDS
+template <int N> __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14); }
+// a barrier that waits for nothing by itself (__syncthreads also waits for every load, those of later steps among them)
+__device__ __forceinline__ void meet() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// WR x WC wavefronts, RT x CT results of 16 x 16 to each.  Codes of both sides go straight into LDS, S - 1 steps of 128 columns ahead:
 // rows of 128 bytes, their eight places of 16 bytes exchanged by the row's low bits so that the operands' reads find every
 // bank.  A step's products start from zero and are added to the results times their scales, those of a row of tiles while the next row's
 // are under way.  BF16 results are summed by the instruction
 // on the codes.  FP32 ones are summed from BF16 operands (fp8_sum16), and so are those that become codes with a scale, which a value
 // 1.5e-5 off would put on the other side of a border now and then (0.0015 of the norm of 300 rows of 1408 that are 0.0003 off so).
 // Lists: a block takes the columns of one matrix, COLS at a time.  OUT8: the results of ROWS = 128 rows leave as codes with a scale.
-template <int WR, int WC, int RT, int CT, bool GLU, bool LIST, int OUT>
+template <int WR, int WC, int RT, int CT, int S, bool GLU, bool LIST, int OUT>
 __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p) {
     constexpr bool WIDE = OUT != BF16;
-    constexpr int NM = GLU ? 2 : 1, THREADS = WR * WC * 64, A_ROWS = WR * RT * 16, ROWS = A_ROWS / NM, COLS = WC * CT * 16;
-    constexpr int STAGE = (A_ROWS + COLS) * FP8_BLOCK, A_COPIES = A_ROWS * 8 / THREADS, B_COPIES = COLS * 8 / THREADS, TM = RT / NM;
-    static_assert(A_COPIES * THREADS == A_ROWS * 8 && B_COPIES * THREADS == COLS * 8, "whole copies");
+    constexpr int NM = GLU ? 2 : 1, THREADS = WR * WC * 64, A_ROWS = WR * RT * 16, ROWS = A_ROWS / NM, COLS = WC * CT * 16, TM = RT / NM;
+    constexpr int SCALES = (A_ROWS + many_x_rows(COLS, THREADS)) * FP8_BLOCK, STAGE = many_stage(A_ROWS, COLS, THREADS), A_COPIES = A_ROWS * 8 / THREADS, B_COPIES = (COLS * 8 + THREADS - 1) / THREADS;
+    static_assert(A_COPIES * THREADS == A_ROWS * 8, "whole copies");
     static_assert(FP8_BLOCK % (TM * 16) == 0, "a wavefront's rows have one scale");
     static_assert(OUT != CODES || ROWS == FP8_BLOCK, "a block of rows has one scale");
     extern __shared__ __align__(16) char lds[];
@@ -387,80 +402,97 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
         const int nc = min(end - c0, COLS);
         const auto x_of = [&](int i) -> int64_t { return LIST ? row_of_pair(p, p.pairs[c0 + min(i, nc - 1)]) : c0 + min(i, nc - 1); };
         const char * b_at[B_COPIES];
-        const float * sx_at[CT];
 #pragma unroll
         for (int i = 0; i < B_COPIES; i++) {
             b_at[i] = p.x + x_of(i * (THREADS / 8) + (threadIdx.x >> 3)) * p.x_row + chunk * 16;
         }
+        const float * const sx_at = p.xs + x_of(threadIdx.x % COLS) * p.xs_row;
+        f32x4_t acc[RT][CT] = {};
+        // M: tiles of 16 columns to a wavefront, one loop for each number of them (with a branch around a tile's products the compiler puts
+        // their sums behind the branches, where on some ways too few cycles pass between a product and the read of its result)
+        const auto steps = [&](auto columns) {
+            constexpr int M = decltype(columns)::value, BM = (M * WC * 16 * 8 + THREADS - 1) / THREADS, COPIES = A_COPIES + BM + 1; // of a step
+            static_assert((S - 2) * COPIES < 64, "what the counter of loads can tell apart");
+            const auto copy = [&](int s) {
+                char * const to = lds + s % S * STAGE + wave * 1024;
+                const uint8_t * const wk = w_base + s * FP8_BLOCK, * const uk = up_base + s * FP8_BLOCK;
+                const int64_t k = s * FP8_BLOCK;
+                if (cut && s == KB - 1) { // chunks behind the last column are zeros on both sides
+                    const bool none = s * FP8_BLOCK + chunk * 16 >= p.K;
 #pragma unroll
-        for (int c = 0; c < CT; c++) {
-            sx_at[c] = p.xs + x_of((c * WC + wc) * 16 + m16) * p.xs_row;
-        }
-        float sx_next[CT], sw[NM];
-        const auto copy = [&](int s, int buf) {
-            char * const to = lds + buf * STAGE + wave * 1024;
-            const uint8_t * const wk = w_base + s * FP8_BLOCK, * const uk = up_base + s * FP8_BLOCK;
-            const int64_t k = s * FP8_BLOCK, sk = s * p.xs_block;
-            if (cut && s == KB - 1) { // chunks behind the last column are zeros on both sides
-                const bool none = s * FP8_BLOCK + chunk * 16 >= p.K;
+                    for (int i = 0; i < A_COPIES; i++) {
+                        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (none ? (const uint8_t *) g_zeros : (of_up(i) ? uk : wk) + a_off[i]),
+                                                         (__attribute__((address_space(3))) void *) (to + i * THREADS * 16), 16, 0, 0);
+                    }
 #pragma unroll
-                for (int i = 0; i < A_COPIES; i++) {
-                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (none ? (const uint8_t *) g_zeros : (of_up(i) ? uk : wk) + a_off[i]),
-                                                     (__attribute__((address_space(3))) void *) (to + i * THREADS * 16), 16, 0, 0);
-                }
+                    for (int i = 0; i < BM; i++) {
+                        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (none ? (const char *) g_zeros : b_at[i] + k),
+                                                         (__attribute__((address_space(3))) void *) (to + A_ROWS * FP8_BLOCK + i * THREADS * 16), 16, 0, 0);
+                    }
+                } else {
 #pragma unroll
-                for (int i = 0; i < B_COPIES; i++) {
-                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (none ? (const char *) g_zeros : b_at[i] + k),
-                                                     (__attribute__((address_space(3))) void *) (to + A_ROWS * FP8_BLOCK + i * THREADS * 16), 16, 0, 0);
-                }
-            } else {
+                    for (int i = 0; i < A_COPIES; i++) {
+                        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) ((of_up(i) ? uk : wk) + a_off[i]),
+                                                         (__attribute__((address_space(3))) void *) (to + i * THREADS * 16), 16, 0, 0);
+                    }
 #pragma unroll
-                for (int i = 0; i < A_COPIES; i++) {
-                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) ((of_up(i) ? uk : wk) + a_off[i]),
-                                                     (__attribute__((address_space(3))) void *) (to + i * THREADS * 16), 16, 0, 0);
-                }
-#pragma unroll
-                for (int i = 0; i < B_COPIES; i++) {
-                    if (!LIST || i * (THREADS / 8) < nc) {
+                    for (int i = 0; i < BM; i++) {
                         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (b_at[i] + k),
                                                          (__attribute__((address_space(3))) void *) (to + A_ROWS * FP8_BLOCK + i * THREADS * 16), 16, 0, 0);
                     }
                 }
-            }
-#pragma unroll
-            for (int c = 0; c < CT; c++) {
-                sx_next[c] = sx_at[c][sk];
-            }
-        };
-        f32x4_t acc[RT][CT] = {};
-        __syncthreads(); // (a list's next columns: nothing reads LDS any more)
-        copy(0, 0);
-        // M: tiles of 16 columns to a wavefront, one loop for each number of them (with a branch around a tile's products the compiler puts
-        // their sums behind the branches, where on some ways too few cycles pass between a product and the read of its result)
-        const auto steps = [&](auto columns) {
-            constexpr int M = decltype(columns)::value;
-            for (int s64 = 0; s64 < KB; s64 += 64) { // 64 steps' scales of the wavefront's rows, one to a lane
+                // the columns' scales, 64 to a wavefront (the same ones by several where there are fewer)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (sx_at + s * p.xs_block),
+                                                 (__attribute__((address_space(3))) void *) (lds + s % S * STAGE + SCALES + wave * 64 % COLS * 4), 4, 0, 0);
+            };
+            // 64 steps' scales of the wavefront's rows, one to a lane; waited for here: a wait at their use, in the loop, would be one for every
+            // copy under way
+            float sw[NM];
+            const auto load_scales = [&](int s) {
 #pragma unroll
                 for (int m = 0; m < NM; m++) {
-                    sw[m] = scale_at(m ? p.ups : p.ws, p.scales_bf16, scale_row + min(s64 + lane, KB - 1));
+                    sw[m] = scale_at(m ? p.ups : p.ws, p.scales_bf16, scale_row + min(s + lane, KB - 1));
+                    asm volatile("" : "+v"(sw[m]));
+                }
+            };
+            load_scales(0);
+            // (before a list's next columns: nothing reads LDS any more, no store is under way)
+            wait_loads<0>();
+            meet();
+#pragma unroll
+            for (int s = 0; s < S - 1; s++) {
+                if (s < KB) {
+                    copy(s);
+                }
+            }
+            for (int s64 = 0; s64 < KB; s64 += 64) {
+                if (s64 > 0) {
+                    load_scales(s64);
                 }
                 const int s_end = min(s64 + 64, KB);
                 for (int s = s64; s < s_end; s++) {
-                    __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0): this wavefront's copies are in LDS
-                    __syncthreads();                    // all of them are, and nothing reads the other buffer any more
+                    // this wavefront's copies of the step are in LDS; those of up to S - 2 later ones are under way
+                    if (S > 3 && s + 2 < KB) {
+                        wait_loads<(S > 3 ? 2 : 0) * COPIES>();
+                    } else if (S > 2 && s + 1 < KB) {
+                        wait_loads<(S > 2 ? 1 : 0) * COPIES>();
+                    } else {
+                        wait_loads<0>();
+                    }
+                    meet(); // all of the block's are, and nothing reads the buffer of the step before any more
+                    if (s + S - 1 < KB) {
+                        copy(s + S - 1);
+                    }
+                    const char * const at = lds + s % S * STAGE;
                     float both[NM][M];
 #pragma unroll
-                    for (int m = 0; m < NM; m++) {
-                        const float ws = __uint_as_float((uint32_t) __builtin_amdgcn_readlane((int) __float_as_uint(sw[m]), s - s64));
+                    for (int c = 0; c < M; c++) {
+                        const float sx = *(const float *) (at + SCALES + ((c * WC + wc) * 16 + m16) * 4);
 #pragma unroll
-                        for (int c = 0; c < M; c++) {
-                            both[m][c] = ws * sx_next[c];
+                        for (int m = 0; m < NM; m++) {
+                            both[m][c] = __uint_as_float((uint32_t) __builtin_amdgcn_readlane((int) __float_as_uint(sw[m]), s - s64)) * sx;
                         }
                     }
-                    if (s + 1 < KB) {
-                        copy(s + 1, (s + 1) & 1);
-                    }
-                    const char * const at = lds + (s & 1) * STAGE;
                     u32x4_t b[M][2], a[2][2];
                     fp8_wide bw[M];
 #pragma unroll
@@ -476,27 +508,26 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
                     f32x4_t part[2][M];
 #pragma unroll
                     for (int t = 0; t <= RT; t++) {
+                        fp8_wide aw;
                         if (t < RT) {
                             if (t + 1 < RT) {
                                 a[(t + 1) & 1][0] = *(const u32x4_t *) (at + a_frag + (t + 1) * 16 * FP8_BLOCK + frag0);
                                 a[(t + 1) & 1][1] = *(const u32x4_t *) (at + a_frag + (t + 1) * 16 * FP8_BLOCK + frag1);
                             }
-                            fp8_wide aw;
                             if constexpr (WIDE) {
                                 aw = fp8_widen(a[t & 1][0], a[t & 1][1]);
                             }
+                        }
 #pragma unroll
-                            for (int c = 0; c < M; c++) {
+                        for (int c = 0; c < M; c++) {
+                            if (t < RT) {
                                 if constexpr (WIDE) {
                                     part[t & 1][c] = fp8_sum16(aw, bw[c]);
                                 } else {
                                     part[t & 1][c] = fp8_sum8(a[t & 1][0], a[t & 1][1], b[c][0], b[c][1]);
                                 }
                             }
-                        }
-                        if (t > 0) {
-#pragma unroll
-                            for (int c = 0; c < M; c++) {
+                            if (t > 0) {
 #pragma unroll
                                 for (int e = 0; e < 4; e++) {
                                     acc[t - 1][c][e] = fmaf(part[(t - 1) & 1][c][e], both[(t - 1) / TM][c], acc[t - 1][c][e]);
@@ -504,14 +535,33 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
                             }
                         }
                     }
+                    if constexpr (!WIDE) { // in this order: a product, the additions of one a row of tiles before
+#pragma unroll
+                        for (int t = 0; t < RT; t++) {
+#pragma unroll
+                            for (int c = 0; c < M; c++) {
+                                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                                if (t > 0) {
+                                    __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+                                }
+                                if (c == 0 && t + 1 < RT) {
+                                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                                }
+                            }
+                        }
+                    }
                 }
             }
         };
-        if constexpr (LIST) {
+        if constexpr (LIST) { // (the lowest number that has them all: one for the block)
             const int tiles = ((nc + 15) / 16 + WC - 1) / WC;
-            static_assert(CT == 4, "one loop each");
-            tiles == 1 ? steps(std::integral_constant<int, 1>{}) : tiles == 2 ? steps(std::integral_constant<int, 2>{})
-            : tiles == 3 ? steps(std::integral_constant<int, 3>{}) : steps(std::integral_constant<int, 4>{});
+            static_assert(CT == 4 || CT == 2, "one loop each");
+            if constexpr (CT == 4) {
+                tiles == 1 ? steps(std::integral_constant<int, 1>{}) : tiles == 2 ? steps(std::integral_constant<int, 2>{})
+                : tiles == 3 ? steps(std::integral_constant<int, 3>{}) : steps(std::integral_constant<int, 4>{});
+            } else {
+                tiles == 1 ? steps(std::integral_constant<int, 1>{}) : steps(std::integral_constant<int, 2>{});
+            }
         } else {
             steps(std::integral_constant<int, CT>{});
         }
@@ -741,7 +791,7 @@ __global__ void __launch_bounds__(256) k_fp8_combine(const uint16_t * ys, const 
 
 // ---------------------------------------------------------------- launches
 
-fp8_launch launch_of(const fp8_product & a) {
+fp8_launch launch_of(const fp8_product & a, int cus) {
     fp8_launch p = {};
     const bf16n_fp8_weight & w = *a.w;
     p.w = w.codes; p.ws = w.scales; p.scales_bf16 = w.scales_bf16 != 0;
@@ -757,6 +807,7 @@ fp8_launch launch_of(const fp8_product & a) {
     p.per_token = (uint32_t) a.per_token; p.one_per = (uint32_t) std::min<uint64_t>(~0u, (1ull << 32) / a.per_token);
     p.ids = (const char *) a.ids; p.ids_i64 = a.ids_i64; p.ids_s0 = a.ids_s0; p.ids_s1 = a.ids_s1; p.n_used = a.n_used;
     p.pairs = a.pairs; p.bounds = a.bounds;
+    p.cus = cus;
     return p;
 }
 
@@ -826,29 +877,90 @@ int few_pass(int64_t cols, int KB, bool glu) {
     return n;
 }
 
-template <int WR, int WC, int RT, int CT, bool GLU, bool LIST, int OUT>
-void many_go(const fp8_launch & p, int z_blocks, hipStream_t stream) {
-    constexpr int ROWS = WR * RT * 16 / (GLU ? 2 : 1), COLS = WC * CT * 16, LDS = 2 * (WR * RT * 16 + COLS) * FP8_BLOCK;
-    const int row_tiles = (p.nrows + ROWS - 1) / ROWS, col_tiles = (p.ncols + COLS - 1) / COLS;
-    const dim3 grid = LIST ? dim3(row_tiles, (unsigned) p.n_matrices + 1, z_blocks) : dim3((unsigned) (((int64_t) row_tiles * col_tiles + 7) / 8 * 8));
-    static const std::string text = text_of({WR, WC, RT, CT, GLU, LIST, OUT});
+template <int WR, int WC, int RT, int CT, int S, bool GLU, bool LIST, int OUT>
+void many_go(const fp8_launch * p, hipStream_t stream) { // without p: its LDS limit is raised
+    constexpr int ROWS = WR * RT * 16 / (GLU ? 2 : 1), COLS = WC * CT * 16, LDS = S * many_stage(WR * RT * 16, COLS, WR * WC * 64);
+    static_assert((size_t) LDS <= LDS_BYTES, "fits");
+    const auto kernel = k_fp8_many<WR, WC, RT, CT, S, GLU, LIST, OUT>;
+    if (!p) {
+        (void) hipFuncSetAttribute((const void *) kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        return;
+    }
+    const int row_tiles = (p->nrows + ROWS - 1) / ROWS, col_tiles = (p->ncols + COLS - 1) / COLS;
+    const dim3 grid = LIST ? dim3(row_tiles, (unsigned) p->n_matrices + 1, 1) : dim3((unsigned) (((int64_t) row_tiles * col_tiles + 7) / 8 * 8));
+    static const std::string text = text_of({WR, WC, RT, CT, S, GLU, LIST, OUT});
     note_kernel("k_fp8_many", text.c_str(), 0);
-    k_fp8_many<WR, WC, RT, CT, GLU, LIST, OUT><<<grid, WR * WC * 64, LDS, stream>>>(p);
-}
-template <int WR, int WC, int RT, int CT, bool GLU, bool LIST, int OUT>
-void many_init() {
-    constexpr int COLS = WC * CT * 16, LDS = 2 * (WR * RT * 16 + COLS) * FP8_BLOCK;
-    (void) hipFuncSetAttribute((const void *) k_fp8_many<WR, WC, RT, CT, GLU, LIST, OUT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    kernel<<<grid, WR * WC * 64, LDS, stream>>>(*p);
 }
 
-template <bool LIST>
-void run_many(const fp8_launch & p, bool glu, int z_blocks, hipStream_t stream) {
-    if (glu) {
-        p.y_kind == CODES ? many_go<4, 2, 4, 4, true, LIST, CODES>(p, z_blocks, stream)
-        : p.y_kind == BF16 ? many_go<4, 2, 4, 4, true, LIST, BF16>(p, z_blocks, stream) : many_go<4, 2, 4, 4, true, LIST, F32>(p, z_blocks, stream);
-    } else {
-        p.y_kind == BF16 ? many_go<2, 2, 4, 4, false, LIST, BF16>(p, z_blocks, stream) : many_go<2, 2, 4, 4, false, LIST, F32>(p, z_blocks, stream);
+template <int WR, int WC, int RT, int CT, int S, bool GLU, bool LIST>
+void many_kinds(const fp8_launch * p, int y_kind, hipStream_t stream) {
+    if constexpr (GLU) {
+        if (!p || y_kind == CODES) {
+            many_go<WR, WC, RT, CT, S, GLU, LIST, CODES>(p, stream);
+        }
     }
+    if (!p || y_kind == BF16) {
+        many_go<WR, WC, RT, CT, S, GLU, LIST, BF16>(p, stream);
+    }
+    if (!p || y_kind == F32) {
+        many_go<WR, WC, RT, CT, S, GLU, LIST, F32>(p, stream);
+    }
+}
+
+// Tiles to choose from, and what a step of 128 columns of K takes, us: of one block to a CU, and of each where the CUs are full of them.
+struct tile_of { int rows, cols; float alone, full; };
+// the tile whose steps take least: those of one block or of the rounds that the tiles make
+int best_tile(const tile_of * tiles, int n, const fp8_launch & p) {
+    int best = 0;
+    float least = 0;
+    for (int i = 0; i < n; i++) {
+        const int64_t blocks = (int64_t) ((p.nrows + tiles[i].rows - 1) / tiles[i].rows) * ((p.ncols + tiles[i].cols - 1) / tiles[i].cols);
+        const float t = std::max(tiles[i].alone, (float) ((blocks + p.cus - 1) / p.cus) * tiles[i].full);
+        if (i == 0 || t < least) {
+            least = t;
+            best = i;
+        }
+    }
+    return best;
+}
+
+// without p: every instance's limit is raised
+void run_many(const fp8_launch * p, bool glu, bool list, hipStream_t stream) {
+    const int kind = p ? p->y_kind : 0;
+#define MANY(WHEN, N, ...) if (!p || ((WHEN) && best == N)) { many_kinds<__VA_ARGS__>(p, kind, stream); }
+#define MANY_ONE(WHEN, N, ...) if (!p || ((WHEN) && best == N)) { many_go<__VA_ARGS__>(p, stream); }
+    int best = 0;
+    if (p && list) {
+        // gate and up of 256 experts of 512 x 2048, us with 128 columns to a block / 64: 1024 tokens 137 / 154, 2048 182 / 215, 8192 538 / 670; down: 1024
+        // 75 / 68, 2048 94 / 94, 4096 152 / 167
+        best = !glu && p->ncols <= 64 * p->n_matrices ? 1 : 0;
+    } else if (p && glu) { // (1408 x 2048, 300 columns 15 us with 16 columns, 18 with 32, 24 with 64, 34 with 128; 2048 x 2048, 2048 columns 70, 49, 48, 37)
+        const tile_of tiles[] = {{128, 128, 2.0f, 2.05f}, {128, 64, 1.4f, 1.45f}, {128, 32, 1.1f, 0.75f}, {128, 16, 0.85f, 0.54f}};
+        best = best_tile(tiles, 4, *p);
+    } else if (p && kind == BF16) {
+        // (5120 x 2048, us in this order: 128 columns 33, 17, 12, 8.6; 1024: 38, 22.7, 21.8, 22.6; 2048: 40, 38, 33, 42; 8192 x 2048, 8192: 157, 176, 198, 244)
+        const tile_of tiles[] = {{256, 256, 2.0f, 2.0f}, {128, 128, 0.95f, 0.685f}, {128, 64, 0.62f, 0.387f}, {64, 64, 0.45f, 0.238f}};
+        best = best_tile(tiles, 4, *p);
+    } else if (p) { // (5120 x 2048: 64 columns 15 us, 10.7; 2048: 50, 54)
+        const tile_of tiles[] = {{128, 64, 0.88f, 0.6f}, {64, 64, 0.62f, 0.33f}};
+        best = best_tile(tiles, 2, *p);
+    }
+    MANY(glu && list, 0, 4, 2, 4, 4, 2, true, true)
+    MANY(!glu && list, 0, 2, 2, 4, 4, 2, false, true)
+    MANY(!glu && list, 1, 2, 2, 4, 2, 2, false, true)
+    MANY(glu && !list, 0, 4, 2, 4, 4, 2, true, false)
+    MANY(glu && !list, 1, 4, 2, 4, 2, 2, true, false)
+    MANY(glu && !list, 2, 4, 1, 4, 2, 2, true, false)
+    MANY(glu && !list, 3, 4, 1, 4, 1, 2, true, false)
+    MANY_ONE(!glu && !list && kind == BF16, 0, 2, 4, 8, 4, 2, false, false, BF16)
+    MANY_ONE(!glu && !list && kind == BF16, 1, 2, 2, 4, 4, 2, false, false, BF16)
+    MANY_ONE(!glu && !list && kind == BF16, 2, 2, 2, 4, 2, 2, false, false, BF16)
+    MANY_ONE(!glu && !list && kind == BF16, 3, 2, 2, 2, 2, 3, false, false, BF16)
+    MANY_ONE(!glu && !list && kind == F32, 0, 2, 2, 4, 2, 2, false, false, F32)
+    MANY_ONE(!glu && !list && kind == F32, 1, 2, 2, 2, 2, 2, false, false, F32)
+#undef MANY
+#undef MANY_ONE
 }
 
 constexpr int FEW_COLUMNS = 32;
@@ -870,12 +982,7 @@ void fp8_init() {
     few_init<1, true, 8>();
     few_init<2, true, 4>();
     few_init<2, true, 8>();
-    many_init<4, 2, 4, 4, true, true, CODES>();
-    many_init<4, 2, 4, 4, true, true, BF16>();
-    many_init<4, 2, 4, 4, true, true, F32>();
-    many_init<4, 2, 4, 4, true, false, CODES>();
-    many_init<4, 2, 4, 4, true, false, BF16>();
-    many_init<4, 2, 4, 4, true, false, F32>();
+    run_many(nullptr, false, false, nullptr);
 }
 
 void launch_fp8_rows(const bf16n_fp8_rows & x, const bf16n_fp8_rows & y, int64_t rows, int64_t K, int cus, hipStream_t stream) {
@@ -905,7 +1012,7 @@ uint64_t fp8_workspace_bytes(const bf16n_fp8_weight & w, bool glu, int x_kind, i
 void launch_fp8_product(const fp8_product & a, void * workspace, int cus, hipStream_t stream) {
     const bool glu = a.up != nullptr, listed = a.pairs != nullptr, by_ids = a.ids != nullptr;
     const bool f = few(*a.w, a.n_cols, listed, by_ids);
-    fp8_launch p = launch_of(a);
+    fp8_launch p = launch_of(a, cus);
     char * ws = (char *) workspace;
     if (p.x_kind != CODES && !f) {
         const bf16n_fp8_rows codes = {ws, (float *) (ws + aligned(a.x_rows * a.w->K)), a.w->K, 1, a.x_rows, CODES, 0};
@@ -914,7 +1021,7 @@ void launch_fp8_product(const fp8_product & a, void * workspace, int cus, hipStr
         ws += codes_bytes(a.x_rows, a.w->K);
     }
     if (!f) {
-        listed ? run_many<true>(p, glu, 1, stream) : run_many<false>(p, glu, 1, stream);
+        run_many(&p, glu, listed, stream);
         return;
     }
     bf16n_fp8_rows plain = {};
