@@ -1,5 +1,6 @@
 // The dense products' calls from Python in native code: mmv(x, w, out_bf16, multi_col) and linear(x, w, gemv_tokens, chunk_bytes);
-// those of 4-bit weights with group scales, int4_mmv and int4_moe_experts; and the selection, router_topk_grouped.
+// those of 4-bit weights with group scales, int4_mmv and int4_moe_experts; the selection, router_topk_grouped; and those in 8-bit
+// floating point, fp8_mm, fp8_moe_experts and add_rmsnorm_fp8.
 //
 // A small product is bound by the host's call (512 x 2048, one token: the kernel takes 3 us, the call with its checks, result
 // and argument block in Python 9.2).  This does the same for the plain case: a two-dimensional tensor of the plain class on the
@@ -414,6 +415,278 @@ PyObject * router_topk_grouped(PyObject *, PyObject * const * args, Py_ssize_t n
     }
 }
 
+// ---------------------------------------------------------------- 8-bit floating point with a scale for every block of 128
+
+typedef int (*fp8_bytes_fn)(const bf16n_fp8_weight *, int, int, int, int64_t, int64_t, int, uint64_t *);
+typedef int (*fp8_mm_fn)(const bf16n_fp8_weight *, const bf16n_fp8_weight *, const bf16n_fp8_rows *, const bf16n_fp8_rows *, int64_t, void *, uint64_t, void *);
+typedef int (*fp8_experts_bytes_fn)(const bf16n_fp8_weight *, const bf16n_fp8_weight *, int, int, int, int, uint64_t *);
+typedef int (*fp8_experts_fn)(const bf16n_fp8_weight *, const bf16n_fp8_weight *, const bf16n_fp8_weight *, const bf16n_fp8_rows *, const void *, int, int64_t, int64_t,
+                              const void *, int, const bf16n_fp8_rows *, int, int, void *, uint64_t, void *);
+typedef int (*fp8_norm_fn)(const uint16_t *, const uint16_t *, const uint16_t *, const float *, const void *, int, int, const uint16_t *, const bf16n_fp8_rows *, uint16_t *,
+                           uint16_t *, int, int64_t, float, void *);
+fp8_bytes_fn g_fp8_bytes = nullptr;
+fp8_mm_fn g_fp8_mm = nullptr;
+fp8_experts_bytes_fn g_fp8_experts_bytes = nullptr;
+fp8_experts_fn g_fp8_experts = nullptr;
+fp8_norm_fn g_fp8_norm = nullptr;
+PyObject * s_n_matrices;
+
+bool native_fp8() { return g_fp8_mm && !at::impl::torch_function_mode_enabled() && !c10::impl::dispatch_mode_enabled(); }
+int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+
+// an Fp8Weight on the device, its tensors as their class has checked them
+bool fp8_matrix(PyObject * o, int device, bf16n_fp8_weight & w) {
+    const ref co(o, s_codes), sc(o, s_scales);
+    if (!co.o || !sc.o) {
+        return false;
+    }
+    const at::Tensor * c = plain(co.o), * s = plain(sc.o);
+    int64_t n;
+    if (!c || !s || !number(o, s_n_matrices, n) || n <= 0 || c->dim() != 2 || s->dim() != 2 || c->scalar_type() != at::kFloat8_e4m3fn || !c->is_contiguous() ||
+        !s->is_contiguous() || c->get_device() != device || s->get_device() != device || c->size(0) <= 0 || c->size(0) % n) {
+        return false;
+    }
+    w = {};
+    w.codes = (const uint8_t *) c->data_ptr();
+    w.scales = s->data_ptr();
+    w.K = c->size(1);
+    w.rows = c->size(0);
+    w.n_matrices = n;
+    w.scales_bf16 = s->scalar_type() == at::kBFloat16;
+    return (w.scales_bf16 || s->scalar_type() == at::kFloat) && s->size(0) == n * blocks_of(w.rows / n) && s->size(1) == blocks_of(w.K);
+}
+bool alike(const bf16n_fp8_weight & a, const bf16n_fp8_weight & b) { return a.rows == b.rows && a.K == b.K && a.n_matrices == b.n_matrices && a.scales_bf16 == b.scales_bf16; }
+
+struct fp8_x {
+    bf16n_fp8_rows r;
+    int64_t rows;
+    at::TensorOptions like;
+    // BF16 or FP32 rows of K values, or Fp8Rows
+    bool get(PyObject * o, int device, int64_t K) {
+        r = {};
+        const at::Tensor * x;
+        if (THPVariable_CheckExact(o)) {
+            x = plain(o);
+            if (!x || (x->scalar_type() != at::kBFloat16 && x->scalar_type() != at::kFloat)) {
+                return false;
+            }
+            r.kind = x->scalar_type() == at::kBFloat16 ? BF16N_FP8_BF16 : BF16N_FP8_F32;
+            return rest(*x, device, K);
+        }
+        const ref co(o, s_codes), sc(o, s_scales); // (the object keeps its tensors for the call)
+        if (!co.o || !sc.o) {
+            return false;
+        }
+        x = plain(co.o);
+        const at::Tensor * s = plain(sc.o);
+        if (!x || !s || x->scalar_type() != at::kFloat8_e4m3fn || s->scalar_type() != at::kFloat || s->get_device() != device || x->dim() != 2 || s->dim() != 2 ||
+            s->size(0) != x->size(0) || s->size(1) != blocks_of(K)) {
+            return false;
+        }
+        r.kind = BF16N_FP8_CODES;
+        r.scales = (float *) s->data_ptr();
+        r.scale_row = s->stride(0);
+        r.scale_block = s->stride(1);
+        return rest(*x, device, K);
+    }
+    bool rest(const at::Tensor & x, int device, int64_t K) {
+        if (x.dim() != 2 || x.get_device() != device || x.size(0) <= 0 || x.size(0) > 1 << 28 || x.size(1) != K || x.stride(1) != 1) {
+            return false;
+        }
+        r.at = x.data_ptr();
+        r.row = x.stride(0) * x.element_size();
+        rows = x.size(0);
+        like = x.options().requires_grad(false);
+        return r.row % 16 == 0 && (uintptr_t) r.at % 16 == 0;
+    }
+};
+
+// results: a tensor, or codes and scales
+struct fp8_y {
+    at::Tensor y, scales;
+    bf16n_fp8_rows r = {};
+    fp8_y(int64_t rows, int64_t n, int kind, const at::TensorOptions & like) {
+        y = at::empty({rows, n}, like.dtype(kind == BF16N_FP8_CODES ? at::kFloat8_e4m3fn : kind == BF16N_FP8_BF16 ? at::kBFloat16 : at::kFloat));
+        r.at = y.data_ptr();
+        r.row = n * y.element_size();
+        r.kind = kind;
+        if (kind == BF16N_FP8_CODES) {
+            scales = at::empty_strided({rows, blocks_of(n)}, {1, rows}, like.dtype(at::kFloat));
+            r.scales = (float *) scales.data_ptr();
+            r.scale_row = 1;
+            r.scale_block = rows;
+        }
+    }
+};
+
+PyObject * tuple_of(std::initializer_list<const at::Tensor *> tensors) { // those that are there
+    Py_ssize_t n = 0, i = 0;
+    for (const at::Tensor * t : tensors) {
+        n += t->defined();
+    }
+    PyObject * all = PyTuple_New(n);
+    for (const at::Tensor * t : tensors) {
+        if (all && t->defined()) {
+            PyObject * o = THPVariable_Wrap(*t);
+            if (!o) {
+                Py_DECREF(all);
+                return nullptr;
+            }
+            PyTuple_SET_ITEM(all, i++, o);
+        }
+    }
+    return all;
+}
+
+// fp8_mm(x, w, up or None, kind of the result): the product, or (codes, scales)
+PyObject * fp8_mm(PyObject *, PyObject * const * args, Py_ssize_t n) {
+    try {
+        if (n != 4 || !native_fp8()) {
+            return not_taken();
+        }
+        const int device = c10::hip::current_device();
+        bf16n_fp8_weight w, up;
+        const bool glu = args[2] != Py_None;
+        const int64_t kind = PyLong_AsLongLong(args[3]);
+        fp8_x x;
+        if (kind < 0 || kind > BF16N_FP8_F32 || !fp8_matrix(args[1], device, w) || w.n_matrices != 1 || (glu && (!fp8_matrix(args[2], device, up) || !alike(w, up))) ||
+            !x.get(args[0], device, w.K) || (kind == BF16N_FP8_CODES && (!glu || w.rows % 16))) {
+            return not_taken();
+        }
+        uint64_t bytes = 0;
+        if (g_fp8_bytes(&w, glu, x.r.kind, (int) kind, x.rows, 0, 0, &bytes) != 0) {
+            return not_taken();
+        }
+        fp8_y y(x.rows, w.rows, (int) kind, x.like);
+        at::Tensor space;
+        if (bytes) {
+            space = at::empty({(int64_t) bytes}, x.like.dtype(at::kByte));
+        }
+        int status;
+        {
+            pybind11::gil_scoped_release free;
+            status = g_fp8_mm(&w, glu ? &up : nullptr, &x.r, &y.r, x.rows, bytes ? space.data_ptr() : nullptr, bytes, stream_of(device));
+        }
+        return status != 0 ? PyLong_FromLong(status) : kind == BF16N_FP8_CODES ? tuple_of({&y.y, &y.scales}) : THPVariable_Wrap(y.y);
+    } catch (const std::exception &) {
+        return not_taken();
+    }
+}
+
+// fp8_moe_experts(x, gate, up, down, topk_weights, topk_ids, n_experts) -> BF16 rows
+PyObject * fp8_moe_experts(PyObject *, PyObject * const * args, Py_ssize_t n) {
+    try {
+        if (n != 7 || !native_fp8()) {
+            return not_taken();
+        }
+        const int device = c10::hip::current_device();
+        bf16n_fp8_weight gate, up, down;
+        const int64_t E = PyLong_AsLongLong(args[6]);
+        if (E <= 0 || !fp8_matrix(args[1], device, gate) || !fp8_matrix(args[2], device, up) || !fp8_matrix(args[3], device, down) || !alike(gate, up) || gate.n_matrices != E ||
+            down.n_matrices != E || down.K != gate.rows / E) {
+            return not_taken();
+        }
+        fp8_x x;
+        const at::Tensor * wts = plain(args[4]), * ids = plain(args[5]);
+        if (!wts || !ids || !x.get(args[0], device, gate.K) || ids->dim() != 2 || (ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong) || ids->get_device() != device ||
+            ids->size(0) != x.rows || ids->size(1) <= 0 || ids->size(1) >= 1024 || x.rows > 65535 || ids->stride(1) != 1 || wts->dim() != 2 || wts->get_device() != device ||
+            !wts->is_contiguous() || (wts->scalar_type() != at::kFloat && wts->scalar_type() != at::kBFloat16) || wts->size(0) != x.rows || wts->size(1) != ids->size(1)) {
+            return not_taken();
+        }
+        const int T = (int) x.rows, slots = (int) ids->size(1), i64 = ids->scalar_type() == at::kLong, isz = i64 ? 8 : 4;
+        uint64_t bytes = 0;
+        if (g_fp8_experts_bytes(&gate, &down, x.r.kind, 1, T, slots, &bytes) != 0) {
+            return not_taken();
+        }
+        fp8_y y(T, down.rows / E, BF16N_FP8_BF16, x.like);
+        at::Tensor space = at::empty({(int64_t) bytes}, x.like.dtype(at::kByte));
+        int status;
+        {
+            pybind11::gil_scoped_release free;
+            status = g_fp8_experts(&gate, &up, &down, &x.r, ids->data_ptr(), i64, isz, ids->stride(0) * isz, wts->data_ptr(), wts->scalar_type() == at::kBFloat16, &y.r, T, slots,
+                                   space.data_ptr(), bytes, stream_of(device));
+        }
+        return status != 0 ? PyLong_FromLong(status) : THPVariable_Wrap(y.y);
+    } catch (const std::exception &) {
+        return not_taken();
+    }
+}
+
+// add_rmsnorm_fp8(a, b, c, ys, topk_weights, gamma (each of these five or None), eps, want_sum, want_norm) -> (codes, scales[, sum][, norm])
+PyObject * add_rmsnorm_fp8(PyObject *, PyObject * const * args, Py_ssize_t n) {
+    try {
+        if (n != 9 || !native_fp8()) {
+            return not_taken();
+        }
+        const int device = c10::hip::current_device();
+        const at::Tensor * t[6];
+        for (int i = 0; i < 6; i++) {
+            t[i] = args[i] == Py_None ? nullptr : plain(args[i]);
+            if (args[i] != Py_None && (!t[i] || t[i]->get_device() != device || !t[i]->is_contiguous())) {
+                return not_taken();
+            }
+        }
+        const at::Tensor * a = t[0], * ys = t[3], * wts = t[4], * gamma = t[5];
+        const double eps = PyFloat_AsDouble(args[6]);
+        if (PyErr_Occurred() || !a || a->dim() != 2 || a->size(0) <= 0 || a->size(0) > INT32_MAX || (gamma && (gamma->scalar_type() != at::kBFloat16 || gamma->numel() != a->size(1)))) {
+            return not_taken();
+        }
+        const int64_t T = a->size(0), K = a->size(1);
+        for (int i = 0; i < 3; i++) {
+            if (t[i] && (t[i]->scalar_type() != at::kBFloat16 || t[i]->dim() != 2 || t[i]->size(0) != T || t[i]->size(1) != K)) {
+                return not_taken();
+            }
+        }
+        int64_t slots = 0;
+        if (ys) {
+            slots = ys->dim() == 3 ? ys->size(1) : 0;
+            if (slots <= 0 || ys->scalar_type() != at::kFloat || ys->size(0) != T || ys->size(2) != K || !wts || wts->dim() != 2 || wts->size(0) != T || wts->size(1) != slots ||
+                (wts->scalar_type() != at::kFloat && wts->scalar_type() != at::kBFloat16)) {
+                return not_taken();
+            }
+        }
+        if (K % 16 || K < 16 || K > 16384) {
+            return not_taken();
+        }
+        fp8_y y(T, K, BF16N_FP8_CODES, on(*a, at::kBFloat16));
+        at::Tensor sum, norm;
+        if (args[7] == Py_True) {
+            sum = at::empty({T, K}, on(*a, at::kBFloat16));
+        }
+        if (args[8] == Py_True) {
+            norm = at::empty({T, K}, on(*a, at::kBFloat16));
+        }
+        const auto at_of = [](const at::Tensor * v) { return v ? v->data_ptr() : nullptr; };
+        int status;
+        {
+            pybind11::gil_scoped_release free;
+            status = g_fp8_norm((const uint16_t *) a->data_ptr(), (const uint16_t *) at_of(t[1]), (const uint16_t *) at_of(t[2]), (const float *) at_of(ys), ys ? at_of(wts) : nullptr,
+                                ys && wts->scalar_type() == at::kBFloat16, (int) slots, (const uint16_t *) at_of(gamma), &y.r, sum.defined() ? (uint16_t *) sum.data_ptr() : nullptr,
+                                norm.defined() ? (uint16_t *) norm.data_ptr() : nullptr, (int) T, K, (float) eps, stream_of(device));
+        }
+        return status != 0 ? PyLong_FromLong(status) : tuple_of({&y.y, &y.scales, &sum, &norm});
+    } catch (const std::exception &) {
+        return not_taken();
+    }
+}
+
+PyObject * bind_fp8(PyObject *, PyObject * const * args, Py_ssize_t n) {
+    if (n != 5) {
+        PyErr_SetString(PyExc_TypeError, "bind_fp8: five addresses");
+        return nullptr;
+    }
+    g_fp8_bytes = (fp8_bytes_fn) PyLong_AsVoidPtr(args[0]);
+    g_fp8_experts_bytes = (fp8_experts_bytes_fn) PyLong_AsVoidPtr(args[2]);
+    g_fp8_experts = (fp8_experts_fn) PyLong_AsVoidPtr(args[3]);
+    g_fp8_norm = (fp8_norm_fn) PyLong_AsVoidPtr(args[4]);
+    g_fp8_mm = (fp8_mm_fn) PyLong_AsVoidPtr(args[1]);
+    if (PyErr_Occurred()) {
+        g_fp8_mm = nullptr;
+        return nullptr;
+    }
+    Py_RETURN_NONE;
+}
+
 PyObject * bind_int4(PyObject *, PyObject * const * args, Py_ssize_t n) {
     if (n != 6) {
         PyErr_SetString(PyExc_TypeError, "bind_int4: six addresses");
@@ -455,6 +728,11 @@ PyMethodDef g_methods[] = {
     {"router_topk_grouped", (PyCFunction) (void (*)(void)) router_topk_grouped, METH_FASTCALL, "(weights, ids), a status of the C ABI, or None"},
     {"bind_int4", (PyCFunction) (void (*)(void)) bind_int4, METH_FASTCALL,
      "the addresses of bf16n_int4_workspace_bytes, _mmv, _route, _mm_ids, bf16n_moe_combine, bf16n_router_topk_grouped"},
+    {"fp8_mm", (PyCFunction) (void (*)(void)) fp8_mm, METH_FASTCALL, "the dense product in 8 bits, plain or gated: results, (codes, scales), a status or None"},
+    {"fp8_moe_experts", (PyCFunction) (void (*)(void)) fp8_moe_experts, METH_FASTCALL, "routed experts in 8 bits"},
+    {"add_rmsnorm_fp8", (PyCFunction) (void (*)(void)) add_rmsnorm_fp8, METH_FASTCALL, "(codes, scales[, sum][, norm]), a status of the C ABI, or None"},
+    {"bind_fp8", (PyCFunction) (void (*)(void)) bind_fp8, METH_FASTCALL,
+     "the addresses of bf16n_fp8_workspace_bytes, _fp8_mm, _fp8_moe_experts_workspace_bytes, _fp8_moe_experts, bf16n_add_rmsnorm_fp8"},
     {"bind", (PyCFunction) (void (*)(void)) bind, METH_FASTCALL, "the addresses of bf16n_mmv, bf16n_gemv_max_tokens, bf16n_dequant"},
     {nullptr, nullptr, 0, nullptr},
 };
@@ -464,9 +742,9 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, g_methods, 
 
 PyMODINIT_FUNC PyInit__host(void) {
     PyObject ** const names[] = {&s_plane, &s_aux, &s_meta, &s_format, &s_K, &s_rows, &s_R, &s_cm, &s_frag, &s_w64, &s_off[0], &s_off[1], &s_off[2], &s_off[3],
-                                 &s_codes, &s_scales, &s_zeros, &s_group};
+                                 &s_codes, &s_scales, &s_zeros, &s_group, &s_n_matrices};
     const char * const text[] = {"plane", "aux", "meta", "format", "K", "rows", "R", "chunk_major", "frag_order", "wave64", "off_a", "off_b", "off_c", "off_d",
-                                 "codes", "scales", "zeros", "group"};
+                                 "codes", "scales", "zeros", "group", "n_matrices"};
     for (size_t i = 0; i < sizeof(text) / sizeof(text[0]); i++) {
         if (!(*names[i] = PyUnicode_InternFromString(text[i]))) {
             return nullptr;

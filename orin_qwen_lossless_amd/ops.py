@@ -301,7 +301,7 @@ class _NoNativeCalls:
     def mmv(*_):
         return None
 
-    linear = int4_mmv = int4_moe_experts = router_topk_grouped = mmv
+    linear = int4_mmv = int4_moe_experts = router_topk_grouped = fp8_mm = fp8_moe_experts = add_rmsnorm_fp8 = mmv
 
 
 def _host():
@@ -315,6 +315,8 @@ def _host():
             calls.bind(*(C.cast(f, C.c_void_p).value for f in (L.bf16n_mmv, L.bf16n_gemv_max_tokens, L.bf16n_dequant)))
             calls.bind_int4(*(C.cast(f, C.c_void_p).value for f in (L.bf16n_int4_workspace_bytes, L.bf16n_int4_mmv, L.bf16n_int4_route, L.bf16n_int4_mm_ids,
                                                                     L.bf16n_moe_combine, L.bf16n_router_topk_grouped)))
+            calls.bind_fp8(*(C.cast(f, C.c_void_p).value for f in (L.bf16n_fp8_workspace_bytes, L.bf16n_fp8_mm, L.bf16n_fp8_moe_experts_workspace_bytes,
+                                                                   L.bf16n_fp8_moe_experts, L.bf16n_add_rmsnorm_fp8)))
         except (ImportError, AttributeError) as e:  # (AttributeError: a module of an older build lacks a call)
             warnings.warn(f"bf16n: dense products are called without their native part ({e}): a call takes about 4 us longer; "
                           "build it with `python -m orin_qwen_lossless_amd.build`", RuntimeWarning, stacklevel=3)
@@ -1252,6 +1254,13 @@ class Fp8Rows:
         return self.codes.float() * self.scales.repeat_interleave(FP8_BLOCK, 1)[:, : self.codes.shape[1]]
 
 
+def _rows_of(codes: torch.Tensor, scales: torch.Tensor) -> Fp8Rows:
+    """Fp8Rows of tensors that a call here made (no checks: 2 us of a call's 5)."""
+    r = object.__new__(Fp8Rows)
+    r.__dict__.update(codes=codes, scales=scales)
+    return r
+
+
 def fp8_quantize(w: torch.Tensor, n_matrices: int = 1, scale_dtype: torch.dtype = torch.float32) -> Fp8Weight:
     """The nearest codes of a BF16 / FP32 matrix [..., K] (leading axes are rows), on its device, for load time: torch operations in
     pieces.  scale = max|w| / 448 of a block of 128 x 128; codes are taken against the rounded scale.  A block with a weight that is
@@ -1350,6 +1359,12 @@ def add_rmsnorm_fp8(a: torch.Tensor, b: torch.Tensor | None = None, c: torch.Ten
     s * rsqrt(mean(s^2) + eps) * gamma, whose FP32 value is rounded once, to its code.  With want_sum and want_norm a tuple: the rows, bf16(s),
     the norm in BF16 (for a product that takes BF16, a router's).  a, b, c: [T, n] BF16 contiguous; ys: [T, n_used, n] FP32 with
     topk_weights [T, n_used]; gamma: [n] BF16; n a multiple of 16, at most 16384."""
+    r = (_host_calls or _host()).add_rmsnorm_fp8(a, b, c, ys, topk_weights, gamma, eps, bool(want_sum), bool(want_norm))
+    if r is not None:
+        if type(r) is int:
+            return _lib.check(r)
+        y = _rows_of(r[0], r[1])
+        return (y, *r[2:]) if want_sum or want_norm else y
     for t in (a, b, c):
         if t is not None and not (t.is_cuda and t.dtype == torch.bfloat16 and t.is_contiguous() and t.shape == a.shape and t.dim() == 2):
             raise ValueError("bf16n.add_rmsnorm_fp8: inputs must be contiguous bf16 [tokens, n] of one shape")
@@ -1417,6 +1432,10 @@ def fp8_linear(x: torch.Tensor | Fp8Rows, w: Fp8Weight, bias: torch.Tensor | Non
     """y = x W^T (+ bias) for any number of tokens: Fp8Rows [tokens, K], or BF16 / FP32 activations [..., K], which are taken as
     fp8_quantize_rows makes them.  Products of a block of 128 columns are summed on the matrix cores and scaled in FP32; out BF16 or FP32
     (the bias is added in FP32 before the one rounding)."""
+    if bias is None and out_dtype in (torch.bfloat16, torch.float32):
+        y = (_host_calls or _host()).fp8_mm(x, w, None, 1 if out_dtype is torch.bfloat16 else 2)
+        if y is not None:
+            return _lib.check(y) if type(y) is int else y
     if isinstance(x, Fp8Rows):
         x2, lead = x, x.codes.shape[:1]
     else:
@@ -1438,6 +1457,10 @@ def fp8_linear(x: torch.Tensor | Fp8Rows, w: Fp8Weight, bias: torch.Tensor | Non
 def fp8_linear_glu2(x: torch.Tensor | Fp8Rows, gate: Fp8Weight, up: Fp8Weight, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor | Fp8Rows:
     """silu(gate x) * (up x) for two matrices of one shape, x [tokens, K] as in fp8_linear.  out BF16, FP32, or float8_e4m3fn: Fp8Rows of the FP32
     values (rows of the matrices a multiple of 16), what the product behind it takes."""
+    if out_dtype in _FP8_KINDS:
+        y = (_host_calls or _host()).fp8_mm(x, gate, up, _FP8_KINDS[out_dtype])
+        if y is not None:
+            return _lib.check(y) if type(y) is int else _rows_of(*y) if type(y) is tuple else y
     return _fp8_mm("fp8_linear_glu2", x, gate, up, out_dtype)
 
 
@@ -1536,6 +1559,9 @@ def fp8_moe_experts(x: torch.Tensor | Fp8Rows, gate: Fp8Weight, up: Fp8Weight, d
     are held in BF16 before their weighted sum in FP32 (half a step, 2^-9 of a slot's result, beside the 2^-4 of the codes)."""
     if topk_weights is None:
         raise ValueError("bf16n.fp8_moe_experts: topk_weights must be contiguous f32/bf16 [tokens, n_used]")
+    y = (_host_calls or _host()).fp8_moe_experts(x, gate, up, down, topk_weights, topk_ids, n_experts)
+    if y is not None:
+        return _lib.check(y) if type(y) is int else y
     return _fp8_experts("fp8_moe_experts", x, gate, up, down, topk_weights, topk_ids, n_experts)
 
 
