@@ -854,6 +854,8 @@ void check_workspace(const void * workspace, uint64_t have, uint64_t need) {
 struct experts_plan { // offsets in the workspace
     bool listed;
     bool half; // slots' results in BF16
+    bool fused; // down and the weighted sum in one launch
+    int hidden_kind; // hidden rows as down takes them: codes, or FP32 where its blocks make the codes
     uint64_t lists, hidden, hidden_scales, ys, product, bytes;
 };
 experts_plan plan_experts(const bf16n_fp8_weight & gate, const bf16n_fp8_weight & down, int x_kind, bool weighted, int n_tok, int n_used) {
@@ -866,16 +868,20 @@ experts_plan plan_experts(const bf16n_fp8_weight & gate, const bf16n_fp8_weight 
     // while the pairs are no more than the experts each is a column by itself
     e.listed = pairs > gate.n_matrices;
     e.half = e.listed && weighted && out % 8 == 0;
+    e.fused = !e.listed && weighted && dev::fp8_down_fits(down, n_used);
+    e.hidden_kind = e.listed && !dev::fp8_few_listed(gate, pairs) ? BF16N_FP8_CODES : BF16N_FP8_F32;
     if (e.listed) {
         take(e.lists, (pairs + gate.n_matrices + 2) * 4);
+    }
+    if (e.hidden_kind == BF16N_FP8_CODES) {
         take(e.hidden_scales, pairs * ((mid + 127) / 128) * 4);
     }
-    take(e.hidden, pairs * mid * (e.listed ? 1 : 4));
-    if (weighted) {
+    take(e.hidden, pairs * mid * (e.hidden_kind == BF16N_FP8_CODES ? 1 : 4));
+    if (weighted && !e.fused) {
         take(e.ys, pairs * out * (e.half ? 2 : 4));
     }
-    const uint64_t a = dev::fp8_workspace_bytes(gate, true, x_kind, e.listed ? BF16N_FP8_CODES : BF16N_FP8_F32, n_tok, pairs, e.listed, !e.listed);
-    const uint64_t b = dev::fp8_workspace_bytes(down, false, e.listed ? BF16N_FP8_CODES : BF16N_FP8_F32, BF16N_FP8_F32, pairs, pairs, e.listed, !e.listed);
+    const uint64_t a = dev::fp8_workspace_bytes(gate, true, x_kind, e.hidden_kind, n_tok, pairs, e.listed, !e.listed);
+    const uint64_t b = dev::fp8_workspace_bytes(down, false, e.hidden_kind, BF16N_FP8_F32, pairs, pairs, e.listed, !e.listed);
     take(e.product, a > b ? a : b);
     return e;
 }
@@ -1017,12 +1023,20 @@ int bf16n_fp8_moe_experts(const bf16n_fp8_weight * gate, const bf16n_fp8_weight 
             dev::launch_int4_route(ids, ids_i64 != 0, ids_s0, ids_s1, E, n_tok, n_used, pairs, bounds, st);
             launch_check("fp8_moe_experts");
             a.pairs = b.pairs = pairs; a.bounds = b.bounds = bounds;
-            a.y = {ws + e.hidden, (float *) (ws + e.hidden_scales), mid, 1, n, BF16N_FP8_CODES, 0};
         } else {
             a.ids = b.ids = ids; a.ids_i64 = b.ids_i64 = ids_i64 != 0; a.ids_s0 = b.ids_s0 = ids_s0; a.ids_s1 = b.ids_s1 = ids_s1;
-            a.y = {ws + e.hidden, nullptr, mid * 4, 0, 0, BF16N_FP8_F32, 0};
         }
+        a.y = e.hidden_kind == BF16N_FP8_CODES ? bf16n_fp8_rows{ws + e.hidden, (float *) (ws + e.hidden_scales), mid, 1, n, BF16N_FP8_CODES, 0}
+                                               : bf16n_fp8_rows{ws + e.hidden, nullptr, mid * 4, 0, 0, BF16N_FP8_F32, 0};
         b.x = a.y;
+        if (e.fused) {
+            b.y = *y;
+            dev::launch_fp8_product(a, ws + e.product, g_cus, st);
+            launch_check("fp8_moe_experts");
+            dev::launch_fp8_down(b, wts, wts_bf16 != 0, n_tok, g_cus, st);
+            launch_check("fp8_moe_experts");
+            return;
+        }
         b.y = wts ? bf16n_fp8_rows{ws + e.ys, nullptr, out * (e.half ? 2 : 4), 0, 0, e.half ? BF16N_FP8_BF16 : BF16N_FP8_F32, 0} : *y;
         dev::launch_fp8_product(a, ws + e.product, g_cus, st);
         launch_check("fp8_moe_experts");

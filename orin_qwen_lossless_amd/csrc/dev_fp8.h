@@ -44,6 +44,13 @@ __device__ __forceinline__ float row_max_dpp(float v) {
     return fmaxf(v, __uint_as_float(dpp_take<0x140, 0xf>(__float_as_uint(v))));
 }
 
+// the same of eight lanes
+__device__ __forceinline__ float eight_max_dpp(float v) {
+    v = fmaxf(v, __uint_as_float(dpp_take<0xB1, 0xf>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(dpp_take<0x4E, 0xf>(__float_as_uint(v))));
+    return fmaxf(v, __uint_as_float(dpp_take<0x141, 0xf>(__float_as_uint(v))));
+}
+
 __device__ __forceinline__ float most_of8(const float (&v)[8]) {
     return fmaxf(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))), fmaxf(fmaxf(fabsf(v[4]), fabsf(v[5])), fmaxf(fabsf(v[6]), fabsf(v[7]))));
 }

@@ -29,6 +29,7 @@ struct fp8_launch {
     const char * ids; int64_t ids_s0, ids_s1; bool ids_i64; int n_used; // one matrix per pair
     const int32_t * pairs, * bounds;        // pairs sorted by matrix
     int ksplit, lds_cols, cus;
+    uint32_t one_block;                     // 2^32 / KB, rounded up: exact for the items of a pass (below 2^32 / KB)
 };
 
 __device__ __forceinline__ float scale_at(const void * s, bool bf16, int64_t i) {
@@ -92,9 +93,10 @@ constexpr int FEW_PARTS = 64; // blocks of K that a wavefront takes at most: the
 // other operand, from LDS, where the block has put their codes first (those of BF16 and FP32 rows it makes itself).  A lane's two
 // loads of a step are 16 bytes each of row lane % 16, so that four lanes have half a line and both loads a whole one; weights go
 // from memory to the operand's registers, D steps ahead, from one 16 rows on to the next.  K in ksplit parts, summed through LDS in a fixed order.
-template <int CT, bool GLU, int XKIND, int NW>
-__global__ void __launch_bounds__(NW * 64, CT * (GLU ? 2 : 1) == 1 ? 4 : CT * (GLU ? 2 : 1) == 2 ? 3 : 2) k_fp8_few(const fp8_launch p) {
-    constexpr int NM = GLU ? 2 : 1, D = GLU ? 2 : 4;
+// ONE: 16 rows to a block and at most four steps of them to a wavefront, all loaded at once: no register is kept for the next 16 rows.
+template <int CT, bool GLU, int XKIND, int NW, bool ONE>
+__global__ void __launch_bounds__(NW * 64, ONE ? 2 : CT * (GLU ? 2 : 1) == 1 ? 4 : CT * (GLU ? 2 : 1) == 2 ? 3 : 2) k_fp8_few(const fp8_launch p) {
+    constexpr int NM = GLU ? 2 : 1, D = GLU && !ONE ? 2 : 4;
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, m16 = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -104,7 +106,7 @@ __global__ void __launch_bounds__(NW * 64, CT * (GLU ? 2 : 1) == 1 ? 4 : CT * (G
 
     int64_t matrix = 0;
     int begin = 0, end = p.ncols;
-    const int groups = NW / p.ksplit, kp = wave % p.ksplit, group = wave / p.ksplit;
+    const int ksplit = ONE ? NW : p.ksplit, groups = NW / ksplit, kp = wave % ksplit, group = wave / ksplit;
     const int row_step = gridDim.x * groups * 16;
     if (p.pairs) {
         matrix = blockIdx.y;
@@ -130,13 +132,14 @@ __global__ void __launch_bounds__(NW * 64, CT * (GLU ? 2 : 1) == 1 ? 4 : CT * (G
     const auto y_of = [&](int c) -> int64_t { return p.pairs ? p.pairs[c] : c; };
     const auto x_of = [&](int c) -> int64_t { return p.pairs ? row_of_pair(p, p.pairs[c]) : p.ids ? row_of_pair(p, c) : c; };
 
-    const int s0 = KB * kp / p.ksplit, steps = KB * (kp + 1) / p.ksplit - s0; // (at most FEW_PARTS)
+    const int s0 = KB * kp / ksplit, steps = KB * (kp + 1) / ksplit - s0; // (at most FEW_PARTS)
     const bool cut = p.K % FP8_BLOCK != 0 && s0 + steps == KB;
     // the last block's chunks behind the matrix's last column: the row's first instead, taken as zeros (the columns' are zeros in LDS)
     const int last = (KB - 1) * FP8_BLOCK + q * 16;
     const bool out0 = cut && last >= p.K, out1 = cut && last + 64 >= p.K;
 
     const int pass = p.lds_cols;
+    const auto column_of = [&](int i) { return KB == 1 ? i : (int) __umulhi((uint32_t) i, p.one_block); }; // i / KB
     for (int c0 = begin + (p.ids ? 0 : p.pairs ? blockIdx.z : blockIdx.y) * pass; c0 < end; c0 += (p.ids ? 1 : p.pairs ? gridDim.z : gridDim.y) * pass) {
         const int nc = min(end - c0, pass);
         u32x4_t w[D][NM][2];
@@ -173,35 +176,63 @@ __global__ void __launch_bounds__(NW * 64, CT * (GLU ? 2 : 1) == 1 ? 4 : CT * (G
                 load(u, u);
             }
         }
-        // codes and scales of the columns, 16 lanes to a block of 128
+        // Codes and scales of the columns, eight lanes to a block of 128 (with 16 the quotients and the maximum across them were twice as
+        // much work to a block: 19 columns of 2576 in 91 blocks 12.1 us), several blocks' loads under way.
         __syncthreads();
-        for (int i = threadIdx.x >> 4; i < nc * KB; i += NW * 4) {
-            const int c = i / KB, b = i - c * KB, k = b * FP8_BLOCK + (threadIdx.x & 15) * 8;
-            const int64_t r = x_of(c0 + c);
-            const char * src = p.x + r * p.x_row + (int64_t) k * (XKIND == BF16 ? 2 : XKIND == F32 ? 4 : 1);
-            if (XKIND == CODES) {
-                *(u32x2_t *) (lds + c * pitch + k) = k < p.K ? *(const u32x2_t *) src : u32x2_t{};
-                if ((threadIdx.x & 15) == 0) {
-                    lds_scales[c * KB + b] = p.xs[r * p.xs_row + b * p.xs_block];
-                }
-                continue;
-            }
-            float v[8] = {};
-            if (k < p.K) {
-                if (XKIND == BF16) {
-                    bf16x8_to_f32(*(const u32x4_t *) src, v);
-                } else {
-                    const f32x4_t a = *(const f32x4_t *) src, d = *(const f32x4_t *) (src + 16);
+        constexpr int AHEAD = (XKIND == F32 ? 2 : 4) / (CT == 1 && !ONE ? 2 : 1), GROUPS = NW * 8;
+        const int items = nc * KB;
+        for (int base = 0; base < items; base += GROUPS * AHEAD) {
+            u32x4_t raw[AHEAD][XKIND == F32 ? 4 : XKIND == BF16 ? 2 : 1];
+            float scale[AHEAD];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        v[j] = j < 4 ? a[j & 3] : d[j & 3];
+            for (int j = 0; j < AHEAD; j++) {
+                if (base + j * GROUPS >= items) {
+                    break;
+                }
+                const int i = min(base + j * GROUPS + (int) (threadIdx.x >> 3), items - 1), c = column_of(i), b = i - c * KB, k = b * FP8_BLOCK + (threadIdx.x & 7) * 16;
+                const int64_t r = x_of(c0 + c);
+#pragma unroll
+                for (u32x4_t & v : raw[j]) {
+                    v = u32x4_t{};
+                }
+                if (k < p.K) {
+                    const char * const src = p.x + r * p.x_row + (int64_t) k * (XKIND == BF16 ? 2 : XKIND == F32 ? 4 : 1);
+#pragma unroll
+                    for (int e = 0; e < (int) (sizeof(raw[j]) / 16); e++) {
+                        raw[j][e] = *(const u32x4_t *) (src + e * 16);
                     }
                 }
+                if (XKIND == CODES) {
+                    scale[j] = p.xs[r * p.xs_row + b * p.xs_block];
+                }
             }
-            const fp8_scales s = fp8_scales_of(row_max_dpp(most_of8(v)));
-            *(u32x2_t *) (lds + c * pitch + k) = fp8_pack8(v, s.inverse);
-            if ((threadIdx.x & 15) == 0) {
-                lds_scales[c * KB + b] = s.scale;
+#pragma unroll
+            for (int j = 0; j < AHEAD; j++) {
+                if (base + j * GROUPS >= items) {
+                    break;
+                }
+                const int i = min(base + j * GROUPS + (int) (threadIdx.x >> 3), items - 1), c = column_of(i), b = i - c * KB, k = b * FP8_BLOCK + (threadIdx.x & 7) * 16;
+                u32x4_t codes = raw[j][0]; // (the last item's by several where the items end: the same ones)
+                if constexpr (XKIND != CODES) {
+                    float v[2][8];
+                    if constexpr (XKIND == BF16) {
+                        bf16x8_to_f32(raw[j][0], v[0]);
+                        bf16x8_to_f32(raw[j][XKIND == BF16], v[1]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            v[e >> 3][e & 7] = __uint_as_float(raw[j][e >> 2][e & 3]);
+                        }
+                    }
+                    const fp8_scales s = fp8_scales_of(eight_max_dpp(fmaxf(most_of8(v[0]), most_of8(v[1]))));
+                    const u32x2_t lo = fp8_pack8(v[0], s.inverse), hi = fp8_pack8(v[1], s.inverse);
+                    codes = u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+                    scale[j] = s.scale;
+                }
+                *(u32x4_t *) (lds + c * pitch + k) = codes;
+                if ((threadIdx.x & 7) == 0) {
+                    lds_scales[c * KB + b] = scale[j];
+                }
             }
         }
         __syncthreads();
@@ -220,8 +251,8 @@ __global__ void __launch_bounds__(NW * 64, CT * (GLU ? 2 : 1) == 1 ? 4 : CT * (G
                 sw[m] = sw_next[m];
             }
             f32x4_t acc[NM][CT] = {};
-            const bool more = r0 + row_step < p.nrows + group * 16;
-            for (int base = 0; base < steps; base += D) {
+            const bool more = !ONE && r0 + row_step < p.nrows + group * 16;
+            for (int base = 0; base < (ONE ? 1 : steps); base += D) {
 #pragma unroll
                 for (int u = 0; u < D; u++) {
                     const int i = base + u;
@@ -240,7 +271,7 @@ __global__ void __launch_bounds__(NW * 64, CT * (GLU ? 2 : 1) == 1 ? 4 : CT * (G
                     for (int m = 0; m < NM; m++) {
                         ww[m] = fp8_widen(w[u][m][0], w[u][m][1]);
                     }
-                    if (i + D < steps) {
+                    if (!ONE && i + D < steps) {
                         load(i + D, u);
                     }
 #pragma unroll
@@ -268,7 +299,7 @@ __global__ void __launch_bounds__(NW * 64, CT * (GLU ? 2 : 1) == 1 ? 4 : CT * (G
                     }
                 }
             }
-            if (p.ksplit > 1) {
+            if (ksplit > 1) {
                 __syncthreads();
 #pragma unroll
                 for (int m = 0; m < NM; m++) {
@@ -281,7 +312,7 @@ __global__ void __launch_bounds__(NW * 64, CT * (GLU ? 2 : 1) == 1 ? 4 : CT * (G
                 if (kp != 0) {
                     continue;
                 }
-                for (int i = 1; i < p.ksplit; i++) {
+                for (int i = 1; i < ksplit; i++) {
 #pragma unroll
                     for (int m = 0; m < NM; m++) {
 #pragma unroll
@@ -311,6 +342,116 @@ __global__ void __launch_bounds__(NW * 64, CT * (GLU ? 2 : 1) == 1 ? 4 : CT * (G
                 }
             }
         }
+    }
+}
+
+// The second products of a token's experts and their weighted sum in one launch, for few tokens (a launch of one token's slots and one of
+// their sum: 2048 x 512, eight slots 5.5 + 4.0 us; this 5.5): a block takes 16 rows of a token's result, a wavefront the slots wave, wave + 8 ..,
+// and the sum is made in the order of the slots, one fmaf each (bf16n_moe_combine's).  Hidden rows: FP32, made codes by the block.
+__global__ void __launch_bounds__(512, 4) k_fp8_down(const fp8_launch p, const void * wts, bool wts_bf16) {
+    constexpr int NW = 8, D = 4;
+    extern __shared__ __align__(16) char lds[];
+    const int lane = threadIdx.x & 63, m16 = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int KB = p.KB, pitch = KB * FP8_BLOCK + 16, slots = p.n_used, token = blockIdx.y, row0 = blockIdx.x * 16;
+    float * const lds_scales = (float *) (lds + slots * pitch);  // [slots][KB]
+    float * const res = lds_scales + slots * KB;                 // [slots][16]
+    const bool cut = p.K % FP8_BLOCK != 0;
+    const int last = (KB - 1) * FP8_BLOCK + q * 16;
+    const bool out0 = cut && last >= p.K, out1 = cut && last + 64 >= p.K;
+    const int64_t row_off = (int64_t) min(m16, p.nrows - 1 - row0) * p.K + q * 16;
+
+    u32x4_t w[D][2];
+    float sw = 0.f;
+    const uint8_t * at = p.w;
+    const auto matrix_of = [&](int slot) -> int64_t {
+        const char * id = p.ids + token * p.ids_s1 + slot * p.ids_s0;
+        const int64_t m = p.ids_i64 ? *(const int64_t *) id : *(const int32_t *) id;
+        return m >= 0 && m < p.n_matrices ? m : -1;
+    };
+    const auto load = [&](int s, int u) {
+        const bool end = cut && s == KB - 1;
+        const int64_t k = (int64_t) s * FP8_BLOCK;
+        w[u][0] = *(const u32x4_t *) (at + row_off + (end && out0 ? -q * 16 : k));
+        w[u][1] = *(const u32x4_t *) (at + row_off + (end && out1 ? -q * 16 : k + 64));
+    };
+    const auto begin = [&](int64_t matrix) {
+        at = p.w + (matrix * p.nrows + row0) * p.K;
+        sw = scale_at(p.ws, p.scales_bf16, (matrix * p.NB + row0 / FP8_BLOCK) * KB + min(lane, KB - 1));
+#pragma unroll
+        for (int u = 0; u < D; u++) {
+            if (u < KB) {
+                load(u, u);
+            }
+        }
+    };
+    int64_t matrix = wave < slots ? matrix_of(wave) : -1;
+    if (matrix >= 0) {
+        begin(matrix);
+    }
+    for (int i = threadIdx.x >> 4; i < slots * KB; i += NW * 4) {
+        const int c = i / KB, b = i - c * KB, k = b * FP8_BLOCK + (threadIdx.x & 15) * 8;
+        float v[8] = {};
+        if (k < p.K) {
+            const char * src = p.x + ((int64_t) token * slots + c) * p.x_row + (int64_t) k * 4;
+            const f32x4_t lo = *(const f32x4_t *) src, hi = *(const f32x4_t *) (src + 16);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                v[e] = e < 4 ? lo[e & 3] : hi[e & 3];
+            }
+        }
+        const fp8_scales s = fp8_scales_of(row_max_dpp(most_of8(v)));
+        *(u32x2_t *) (lds + c * pitch + k) = fp8_pack8(v, s.inverse);
+        if ((threadIdx.x & 15) == 0) {
+            lds_scales[c * KB + b] = s.scale;
+        }
+    }
+    __syncthreads();
+    for (int slot = wave; slot < slots; slot += NW) {
+        f32x4_t acc = {};
+        if (matrix >= 0) {
+            const char * const x_at = lds + slot * pitch + q * 16;
+            for (int base = 0; base < KB; base += D) {
+#pragma unroll
+                for (int u = 0; u < D; u++) {
+                    const int s = base + u;
+                    if (s >= KB) {
+                        break;
+                    }
+                    if (cut && s == KB - 1) {
+                        w[u][0] = out0 ? u32x4_t{} : w[u][0];
+                        w[u][1] = out1 ? u32x4_t{} : w[u][1];
+                    }
+                    const fp8_wide ww = fp8_widen(w[u][0], w[u][1]);
+                    if (s + D < KB) {
+                        load(s + D, u);
+                    }
+                    const fp8_wide xw = fp8_widen(*(const u32x4_t *) (x_at + s * FP8_BLOCK), *(const u32x4_t *) (x_at + s * FP8_BLOCK + 64));
+                    const float both = __uint_as_float((uint32_t) __builtin_amdgcn_readlane((int) __float_as_uint(sw), s)) * lds_scales[slot * KB + s];
+                    const f32x4_t part = fp8_sum16(ww, xw);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        acc[e] = fmaf(part[e], both, acc[e]);
+                    }
+                }
+            }
+        }
+        if (m16 == 0) {
+            *(f32x4_t *) (res + slot * 16 + 4 * q) = acc;
+        }
+        matrix = slot + NW < slots ? matrix_of(slot + NW) : -1;
+        if (matrix >= 0) {
+            begin(matrix);
+        }
+    }
+    __syncthreads();
+    const int r = row0 + threadIdx.x;
+    if (threadIdx.x < 16 && r < p.nrows) {
+        float acc = 0.f;
+        for (int i = 0; i < slots; i++) {
+            acc = fmaf(scale_at(wts, wts_bf16, (int64_t) token * slots + i), res[i * 16 + threadIdx.x], acc);
+        }
+        store_y(p.y + token * p.y_row, p.y_kind == BF16, r, acc);
     }
 }
 
@@ -366,7 +507,7 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
             }
             return;
         }
-        begin += blockIdx.z * COLS;
+        begin += (gridDim.z - 1 - blockIdx.z) * COLS; // (later passes of long lists first)
     } else {
         // An XCD takes every eighth block, which is made a contiguous part of the tiles here: four column tiles of one row tile
         // after the other, so that what runs there at a time shares few pieces of either side.
@@ -674,58 +815,75 @@ __global__ void __launch_bounds__(256) k_fp8_rows(const char * x, int64_t x_row,
     }
 }
 
-// The glue of a decode step (bf16n_add_rmsnorm) with its norm in 8 bits: a token's row in C pieces of eight elements to a thread,
-// 16 threads to a block of 128.  Sums are FP32, the slots' in bf16n_moe_combine's order.
-template <int C>
-__global__ void __launch_bounds__(256) k_add_rmsnorm_fp8(const add_norm_args p, uint8_t * y, int64_t y_row, float * s, int64_t s_row, int64_t s_block) {
-    __shared__ float wave_sq[4];
-    __shared__ float wsm[1024];
+__device__ __forceinline__ u32x4_t to_bf16x8(const float (&v)[8]) {
+    return u32x4_t{f32_to_bf16_rne(v[0]) | (uint32_t) f32_to_bf16_rne(v[1]) << 16, f32_to_bf16_rne(v[2]) | (uint32_t) f32_to_bf16_rne(v[3]) << 16,
+                   f32_to_bf16_rne(v[4]) | (uint32_t) f32_to_bf16_rne(v[5]) << 16, f32_to_bf16_rne(v[6]) | (uint32_t) f32_to_bf16_rne(v[7]) << 16};
+}
+
+// The glue of a decode step (bf16n_add_rmsnorm) with its norm in 8 bits: a block to a token, C pieces of eight elements to a thread, 16 threads to
+// a block of 128.  Sums are FP32, the slots' in bf16n_moe_combine's order, eight slots' rows on the way at a time (one after the other:
+// 333 tokens of 2576 with eight slots 10.9 us).  A row stays in registers between the sum of its squares and its codes.
+template <int C, bool SLOTS>
+__global__ void __launch_bounds__(1024) k_add_rmsnorm_fp8(const add_norm_args p, uint8_t * y, int64_t y_row, float * s, int64_t s_row, int64_t s_block) {
+    __shared__ float wave_sq[16];
+    __shared__ float wsm[SLOTS ? 1024 : 1];
     const int64_t tok = blockIdx.x, base = tok * p.n;
-    if (p.ys) {
-        for (int i = threadIdx.x; i < p.n_used; i += 256) {
+    const int threads = blockDim.x;
+    if (SLOTS) {
+        for (int i = threadIdx.x; i < p.n_used; i += threads) {
             const int64_t at = tok * p.n_used + i;
             wsm[i] = p.wts_bf16 ? bf16_bits_to_f32(((const uint16_t *) p.wts)[at]) : ((const float *) p.wts)[at];
         }
         __syncthreads();
     }
     float v[C][8], sq = 0.f;
+    u32x4_t gamma[C];
 #pragma unroll
     for (int j = 0; j < C; j++) {
-        const int i0 = (j * 256 + threadIdx.x) * 8;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            v[j][e] = 0.f;
-        }
+        const int i0 = (j * threads + threadIdx.x) * 8;
+        u32x4_t a = {}, b = {}, c = {};
+        gamma[j] = u32x4_t{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u}; // ones
+        float acc[8] = {};
         if (i0 < p.n) {
-            float f[8];
-            bf16x8_to_f32(*(const u32x4_t *) (p.a + base + i0), v[j]);
-            for (const uint16_t * more : {p.b, p.c}) {
-                if (more) {
-                    bf16x8_to_f32(*(const u32x4_t *) (more + base + i0), f);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        v[j][e] += f[e];
-                    }
-                }
+            a = *(const u32x4_t *) (p.a + base + i0);
+            if (p.b) {
+                b = *(const u32x4_t *) (p.b + base + i0);
             }
-            if (p.ys) {
-                float acc[8] = {};
+            if (p.c) {
+                c = *(const u32x4_t *) (p.c + base + i0);
+            }
+            if (p.gamma) {
+                gamma[j] = *(const u32x4_t *) (p.gamma + i0);
+            }
+            if (SLOTS) {
                 const float * row = p.ys + (tok * p.n_used) * p.n + i0;
-                for (int k = 0; k < p.n_used; k++) {
-                    const f32x4_t a = *(const f32x4_t *) (row + k * p.n), d = *(const f32x4_t *) (row + k * p.n + 4);
+                for (int k0 = 0; k0 < p.n_used; k0 += 8) {
+                    f32x4_t lo[8], hi[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        acc[e] = fmaf(wsm[k], e < 4 ? a[e & 3] : d[e & 3], acc[e]);
+                    for (int k = 0; k < 8; k++) { // (a slot past the last: the last row again, unused)
+                        const float * at = row + (int64_t) min(k0 + k, p.n_used - 1) * p.n;
+                        lo[k] = *(const f32x4_t *) at;
+                        hi[k] = *(const f32x4_t *) (at + 4);
                     }
-                }
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    v[j][e] += acc[e];
+                    for (int k = 0; k < 8; k++) {
+                        if (k0 + k < p.n_used) {
+#pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                acc[e] = fmaf(wsm[k0 + k], e < 4 ? lo[k][e & 3] : hi[k][e & 3], acc[e]);
+                            }
+                        }
+                    }
                 }
             }
         }
+        float fb[8], fc[8];
+        bf16x8_to_f32(a, v[j]);
+        bf16x8_to_f32(b, fb);
+        bf16x8_to_f32(c, fc);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
+            v[j][e] = ((v[j][e] + fb[e]) + fc[e]) + acc[e];
             sq = fmaf(v[j][e], v[j][e], sq);
         }
     }
@@ -734,27 +892,26 @@ __global__ void __launch_bounds__(256) k_add_rmsnorm_fp8(const add_norm_args p, 
         wave_sq[threadIdx.x >> 6] = sq;
     }
     __syncthreads();
-    const float total = ((wave_sq[0] + wave_sq[1]) + wave_sq[2]) + wave_sq[3];
+    float total = 0.f;
+    for (int i = 0; i < threads >> 6; i++) {
+        total += wave_sq[i];
+    }
     const float scale = 1.0f / sqrtf(total / (float) p.n + p.eps);
 #pragma unroll
     for (int j = 0; j < C; j++) {
-        const int i0 = (j * 256 + threadIdx.x) * 8;
-        float g[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+        const int i0 = (j * threads + threadIdx.x) * 8;
         const bool in = i0 < p.n;
         if (in && p.y_sum) {
-            *(u32x4_t *) (p.y_sum + base + i0) = u32x4_t{f32_to_bf16_rne(v[j][0]) | (uint32_t) f32_to_bf16_rne(v[j][1]) << 16, f32_to_bf16_rne(v[j][2]) | (uint32_t) f32_to_bf16_rne(v[j][3]) << 16,
-                                                         f32_to_bf16_rne(v[j][4]) | (uint32_t) f32_to_bf16_rne(v[j][5]) << 16, f32_to_bf16_rne(v[j][6]) | (uint32_t) f32_to_bf16_rne(v[j][7]) << 16};
+            *(u32x4_t *) (p.y_sum + base + i0) = to_bf16x8(v[j]);
         }
-        if (in && p.gamma) {
-            bf16x8_to_f32(*(const u32x4_t *) (p.gamma + i0), g);
-        }
+        float g[8];
+        bf16x8_to_f32(gamma[j], g);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             v[j][e] = v[j][e] * scale * g[e];
         }
         if (in && p.y_norm) {
-            *(u32x4_t *) (p.y_norm + base + i0) = u32x4_t{f32_to_bf16_rne(v[j][0]) | (uint32_t) f32_to_bf16_rne(v[j][1]) << 16, f32_to_bf16_rne(v[j][2]) | (uint32_t) f32_to_bf16_rne(v[j][3]) << 16,
-                                                          f32_to_bf16_rne(v[j][4]) | (uint32_t) f32_to_bf16_rne(v[j][5]) << 16, f32_to_bf16_rne(v[j][6]) | (uint32_t) f32_to_bf16_rne(v[j][7]) << 16};
+            *(u32x4_t *) (p.y_norm + base + i0) = to_bf16x8(v[j]);
         }
         const fp8_scales q = fp8_scales_of(row_max_dpp(most_of8(v[j])));
         if (in) {
@@ -808,8 +965,11 @@ fp8_launch launch_of(const fp8_product & a, int cus) {
     p.ids = (const char *) a.ids; p.ids_i64 = a.ids_i64; p.ids_s0 = a.ids_s0; p.ids_s1 = a.ids_s1; p.n_used = a.n_used;
     p.pairs = a.pairs; p.bounds = a.bounds;
     p.cus = cus;
+    p.one_block = (uint32_t) (((1ull << 32) + p.KB - 1) / p.KB);
     return p;
 }
+
+constexpr size_t FEW_LDS = 160 * 1024 - 1024;
 
 // a kernel instance's template arguments (bf16n_last_kernel)
 std::string text_of(std::initializer_list<int> numbers) {
@@ -820,17 +980,64 @@ std::string text_of(std::initializer_list<int> numbers) {
     return s;
 }
 
-template <int CT, bool GLU, int XKIND, int NW>
-void few_go(const fp8_launch & p, dim3 grid, size_t lds, hipStream_t stream) {
-    static const std::string text = text_of({CT, GLU, XKIND, NW});
+// without p: the LDS limit is raised
+template <int CT, bool GLU, int XKIND, int NW, bool ONE>
+void few_go(const fp8_launch * p, dim3 grid, size_t lds, hipStream_t stream) {
+    const auto kernel = k_fp8_few<CT, GLU, XKIND, NW, ONE>;
+    if (!p) {
+        (void) hipFuncSetAttribute((const void *) kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int) FEW_LDS);
+        return;
+    }
+    static const std::string text = text_of({CT, GLU, XKIND, NW, ONE});
     note_kernel("k_fp8_few", text.c_str(), 0);
-    k_fp8_few<CT, GLU, XKIND, NW><<<grid, NW * 64, lds, stream>>>(p);
+    kernel<<<grid, NW * 64, lds, stream>>>(*p);
 }
-
-constexpr size_t FEW_LDS = 160 * 1024 - 1024;
 
 size_t few_lds(int cols, int KB, int ct, bool glu, int nw, int ksplit) {
     return ((size_t) cols * (KB * FP8_BLOCK + 16 + KB * 4) + 15) / 16 * 16 + (ksplit > 1 ? (size_t) nw * (glu ? 2 : 1) * ct * 1024 : 0);
+}
+
+enum { FEW_ONE, FEW_EIGHT, FEW_FOUR }; // all at once; eight wavefronts; four
+// without p: every instance's limit is raised
+void few_instance(const fp8_launch * p, int ct, bool glu, int shape, dim3 grid, size_t lds, hipStream_t stream) {
+    const auto by_kind = [&](auto c, auto g, auto n, auto one) {
+        constexpr int CT = decltype(c)::value, NW = decltype(n)::value;
+        constexpr bool GLU = decltype(g)::value, ONE = decltype(one)::value;
+        if (!p || p->x_kind == CODES) {
+            few_go<CT, GLU, CODES, NW, ONE>(p, grid, lds, stream);
+        }
+        if (!p || p->x_kind == BF16) {
+            few_go<CT, GLU, BF16, NW, ONE>(p, grid, lds, stream);
+        }
+        if (!p || p->x_kind == F32) {
+            few_go<CT, GLU, F32, NW, ONE>(p, grid, lds, stream);
+        }
+    };
+    const auto by_shape = [&](auto c, auto g) {
+        if (!p || shape == FEW_ONE) {
+            by_kind(c, g, std::integral_constant<int, 8>{}, std::true_type{});
+        }
+        if (!p || shape == FEW_EIGHT) {
+            by_kind(c, g, std::integral_constant<int, 8>{}, std::false_type{});
+        }
+        if (!p || shape == FEW_FOUR) {
+            by_kind(c, g, std::integral_constant<int, 4>{}, std::false_type{});
+        }
+    };
+    const auto by_ct = [&](auto g) {
+        if (!p || ct == 1) {
+            by_shape(std::integral_constant<int, 1>{}, g);
+        }
+        if (!p || ct == 2) {
+            by_shape(std::integral_constant<int, 2>{}, g);
+        }
+    };
+    if (!p || glu) {
+        by_ct(std::true_type{});
+    }
+    if (!p || !glu) {
+        by_ct(std::false_type{});
+    }
 }
 
 // cols: columns of a pass; busy: matrices or passes that have columns; blocks: of them all, grid.y
@@ -838,7 +1045,7 @@ void run_few(fp8_launch p, bool glu, int cols, int64_t busy, int y_blocks, int c
     const int64_t tiles = (p.nrows + 15) / 16 * busy;
     const int nw = tiles <= 4 * cus ? 8 : 4;
     int ksplit = nw == 8 ? 8 : tiles <= 16 * cus ? 4 : 1;
-    while (ksplit > 1 && p.KB < ksplit * 2) {
+    while (ksplit > 1 && p.KB < ksplit) {
         ksplit /= 2;
     }
     while ((p.KB + ksplit - 1) / ksplit > FEW_PARTS) {
@@ -848,24 +1055,13 @@ void run_few(fp8_launch p, bool glu, int cols, int64_t busy, int y_blocks, int c
     p.lds_cols = cols;
     const int ct = cols <= 16 ? 1 : 2, rows = nw / ksplit * 16, n_blocks = (p.nrows + rows - 1) / rows;
     const size_t lds = few_lds(cols, p.KB, ct, glu, nw, ksplit);
+    if (ksplit == 8 && tiles <= 2 * cus && p.KB <= 32) { // (else 512 x 2048, one column 6.7 us for 4.5; 1453 x 2576, 19 columns 10.2 for 9.2)
+        few_instance(&p, ct, glu, FEW_ONE, dim3(n_blocks, y_blocks), lds, stream);
+        return;
+    }
     const int room = cus * (int) std::min<size_t>(nw == 8 ? 2 : 4, LDS_BYTES / lds);
     const int rounds = (int) std::max<int64_t>(1, std::min<int64_t>(8, (int64_t) n_blocks * busy / room));
-    const dim3 grid((n_blocks + rounds - 1) / rounds, y_blocks, 1);
-    const auto by_kind = [&](auto c, auto g, auto n) {
-        constexpr int C = decltype(c)::value, N = decltype(n)::value;
-        constexpr bool G = decltype(g)::value;
-        p.x_kind == CODES ? few_go<C, G, CODES, N>(p, grid, lds, stream) : p.x_kind == BF16 ? few_go<C, G, BF16, N>(p, grid, lds, stream) : few_go<C, G, F32, N>(p, grid, lds, stream);
-    };
-    const auto by_nw = [&](auto c, auto g) { nw == 8 ? by_kind(c, g, std::integral_constant<int, 8>{}) : by_kind(c, g, std::integral_constant<int, 4>{}); };
-    const auto by_ct = [&](auto g) { ct == 1 ? by_nw(std::integral_constant<int, 1>{}, g) : by_nw(std::integral_constant<int, 2>{}, g); };
-    glu ? by_ct(std::true_type{}) : by_ct(std::false_type{});
-}
-
-template <int CT, bool GLU, int NW>
-void few_init() {
-    (void) hipFuncSetAttribute((const void *) k_fp8_few<CT, GLU, CODES, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, (int) FEW_LDS);
-    (void) hipFuncSetAttribute((const void *) k_fp8_few<CT, GLU, BF16, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, (int) FEW_LDS);
-    (void) hipFuncSetAttribute((const void *) k_fp8_few<CT, GLU, F32, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, (int) FEW_LDS);
+    few_instance(&p, ct, glu, nw == 8 ? FEW_EIGHT : FEW_FOUR, dim3((n_blocks + rounds - 1) / rounds, y_blocks), lds, stream);
 }
 
 // columns of a pass of k_fp8_few: as many as are there, 32 at most, and what LDS holds
@@ -887,7 +1083,8 @@ void many_go(const fp8_launch * p, hipStream_t stream) { // without p: its LDS l
         return;
     }
     const int row_tiles = (p->nrows + ROWS - 1) / ROWS, col_tiles = (p->ncols + COLS - 1) / COLS;
-    const dim3 grid = LIST ? dim3(row_tiles, (unsigned) p->n_matrices + 1, 1) : dim3((unsigned) (((int64_t) row_tiles * col_tiles + 7) / 8 * 8));
+    // lists: two blocks take a long one's passes in turn (8192 tokens of 256 experts, gate and up: 537 us with one, 465 with two or four)
+    const dim3 grid = LIST ? dim3(row_tiles, (unsigned) p->n_matrices + 1, p->ncols > 96 * p->n_matrices ? 2 : 1) : dim3((unsigned) (((int64_t) row_tiles * col_tiles + 7) / 8 * 8));
     static const std::string text = text_of({WR, WC, RT, CT, S, GLU, LIST, OUT});
     note_kernel("k_fp8_many", text.c_str(), 0);
     kernel<<<grid, WR * WC * 64, LDS, stream>>>(*p);
@@ -965,6 +1162,10 @@ void run_many(const fp8_launch * p, bool glu, bool list, hipStream_t stream) {
 
 constexpr int FEW_COLUMNS = 32;
 
+// Whether the blocks of the kernel for few columns turn rows that are not codes into them, each for itself, rather than a launch ahead of it:
+// 12 cycles of a block's CU for a block of 128 against 3 us (2576 columns of K: 19 columns 400 blocks, 32 670)
+bool converts(int KB, int64_t cols) { return KB * cols <= 512; }
+
 bool few(const bf16n_fp8_weight & w, int64_t n_cols, bool listed, bool by_ids) {
     return by_ids || (listed ? n_cols <= 12 * (int64_t) w.n_matrices : n_cols <= FEW_COLUMNS);
 }
@@ -974,14 +1175,8 @@ size_t codes_bytes(int64_t rows, int64_t K) { return aligned(rows * K) + aligned
 } // namespace
 
 void fp8_init() {
-    few_init<1, false, 4>();
-    few_init<1, false, 8>();
-    few_init<2, false, 4>();
-    few_init<2, false, 8>();
-    few_init<1, true, 4>();
-    few_init<1, true, 8>();
-    few_init<2, true, 4>();
-    few_init<2, true, 8>();
+    (void) hipFuncSetAttribute((const void *) k_fp8_down, hipFuncAttributeMaxDynamicSharedMemorySize, (int) FEW_LDS);
+    few_instance(nullptr, 0, false, 0, dim3(), 0, nullptr);
     run_many(nullptr, false, false, nullptr);
 }
 
@@ -992,15 +1187,22 @@ void launch_fp8_rows(const bf16n_fp8_rows & x, const bf16n_fp8_rows & y, int64_t
 }
 
 void launch_add_rmsnorm_fp8(const add_norm_args & a, const bf16n_fp8_rows & y, int n_tok, hipStream_t stream) {
-    const int64_t pieces = (a.n + 2047) / 2048;
-    (pieces == 1 ? k_add_rmsnorm_fp8<1> : pieces == 2 ? k_add_rmsnorm_fp8<2> : pieces <= 4 ? k_add_rmsnorm_fp8<4> : k_add_rmsnorm_fp8<8>)
-        <<<n_tok, 256, 0, stream>>>(a, (uint8_t *) y.at, y.row, y.scales, y.scale_row, y.scale_block);
+    const int pieces = (int) ((a.n + 7) / 8), threads = std::min(1024, (pieces + 63) / 64 * 64);
+    (a.ys ? (pieces <= 1024 ? k_add_rmsnorm_fp8<1, true> : k_add_rmsnorm_fp8<2, true>) : (pieces <= 1024 ? k_add_rmsnorm_fp8<1, false> : k_add_rmsnorm_fp8<2, false>))<<<n_tok, threads, 0, stream>>>(a, (uint8_t *) y.at, y.row, y.scales, y.scale_row, y.scale_block);
+}
+
+bool fp8_few_listed(const bf16n_fp8_weight & w, int64_t n_pairs) { return few(w, n_pairs, true, false); }
+
+// whether rows of activations become codes in a launch of their own
+static bool in_launch(const bf16n_fp8_weight & w, int x_kind, int64_t n_cols, bool listed, bool by_ids) {
+    const int KB = (int) ((w.K + FP8_BLOCK - 1) / FP8_BLOCK);
+    return x_kind != CODES && !(few(w, n_cols, listed, by_ids) && converts(KB, by_ids ? 1 : listed ? std::min<int64_t>(n_cols, 16) : n_cols));
 }
 
 uint64_t fp8_workspace_bytes(const bf16n_fp8_weight & w, bool glu, int x_kind, int y_kind, int64_t x_rows, int64_t n_cols, bool listed, bool by_ids) {
     const bool f = few(w, n_cols, listed, by_ids);
     uint64_t n = 0;
-    if (x_kind != CODES && !f) {
+    if (in_launch(w, x_kind, n_cols, listed, by_ids)) {
         n += codes_bytes(x_rows, w.K);
     }
     if (y_kind == CODES && f) {
@@ -1014,7 +1216,7 @@ void launch_fp8_product(const fp8_product & a, void * workspace, int cus, hipStr
     const bool f = few(*a.w, a.n_cols, listed, by_ids);
     fp8_launch p = launch_of(a, cus);
     char * ws = (char *) workspace;
-    if (p.x_kind != CODES && !f) {
+    if (in_launch(*a.w, p.x_kind, a.n_cols, listed, by_ids)) {
         const bf16n_fp8_rows codes = {ws, (float *) (ws + aligned(a.x_rows * a.w->K)), a.w->K, 1, a.x_rows, CODES, 0};
         launch_fp8_rows(a.x, codes, a.x_rows, a.w->K, cus, stream);
         p.x = ws; p.x_row = a.w->K; p.xs = codes.scales; p.xs_row = 1; p.xs_block = a.x_rows; p.x_kind = CODES;
@@ -1040,6 +1242,18 @@ void launch_fp8_product(const fp8_product & a, void * workspace, int cus, hipStr
     if (plain.at) {
         launch_fp8_rows(plain, a.y, a.n_cols, p.nrows, cus, stream);
     }
+}
+
+// LDS of k_fp8_down
+static size_t down_lds(int slots, int KB) { return (size_t) slots * (KB * FP8_BLOCK + 16 + KB * 4 + 64); }
+bool fp8_down_fits(const bf16n_fp8_weight & down, int n_used) {
+    const int KB = (int) ((down.K + FP8_BLOCK - 1) / FP8_BLOCK);
+    return KB <= FEW_PARTS && down_lds(n_used, KB) <= FEW_LDS;
+}
+void launch_fp8_down(const fp8_product & a, const void * wts, bool wts_bf16, int n_tok, int cus, hipStream_t stream) {
+    const fp8_launch p = launch_of(a, cus);
+    note_kernel("k_fp8_down", nullptr, 0);
+    k_fp8_down<<<dim3((p.nrows + 15) / 16, n_tok), 512, down_lds(p.n_used, p.KB), stream>>>(p, wts, wts_bf16);
 }
 
 void launch_fp8_combine(const void * ys, const void * w, bool w_bf16, void * y, bool y_bf16, int n_tok, int n_used, int64_t n, hipStream_t stream) {
