@@ -192,5 +192,24 @@ __device__ __forceinline__ float wave_sum_cols(float v) {
     return dpp_add<0x143, 0xc>(v); // row_bcast:31 into rows 2 and 3
 }
 
+// the same lanes' sums as wave_sum_dpp, in 64 bits; every lane gets the result
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ double dpp_add64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int) u, CTRL, ROW_MASK, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, (int) (u >> 32), CTRL, ROW_MASK, 0xf, false);
+    return v + __builtin_bit_cast(double, (uint64_t) hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+    v = dpp_add64<0xB1, 0xf>(v);
+    v = dpp_add64<0x4E, 0xf>(v);
+    v = dpp_add64<0x141, 0xf>(v);
+    v = dpp_add64<0x140, 0xf>(v);
+    v = dpp_add64<0x142, 0xa>(v);
+    v = dpp_add64<0x143, 0xc>(v);
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int) u, 63), hi = __builtin_amdgcn_readlane((int) (u >> 32), 63);
+    return __builtin_bit_cast(double, (uint64_t) hi << 32 | lo);
+}
+
 } // namespace dev
 } // namespace bf16n

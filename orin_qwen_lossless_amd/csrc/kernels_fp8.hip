@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 namespace bf16n {
 namespace dev {
@@ -821,11 +822,14 @@ __device__ __forceinline__ u32x4_t to_bf16x8(const float (&v)[8]) {
 }
 
 // The glue of a decode step (bf16n_add_rmsnorm) with its norm in 8 bits: a block to a token, C pieces of eight elements to a thread, 16 threads to
-// a block of 128.  Sums are FP32, the slots' in bf16n_moe_combine's order, eight slots' rows on the way at a time (one after the other:
-// 333 tokens of 2576 with eight slots 10.9 us).  A row stays in registers between the sum of its squares and its codes.
+// a block of 128, eight slots' rows on the way at a time (one after the other: 333 tokens of 2576 with eight slots 10.9 us).  A row stays
+// in registers between the sum of its squares and its codes.  The slots' sum, the squares' and the norm are held in 64 bits and become
+// FP32 once, ahead of the scales: a code is off by a whole step, a sixteenth of its value, wherever an error of a last place carries a value over the
+// middle of two codes, which 32 bits did to one or two of 858 thousand (and were 8.9 us there for 9.6).
+// 8192 tokens of 2048: 22.9 us, 134 MB at 5.8 TB/s; one token 2.8, the chain of its loads, sum and scale.
 template <int C, bool SLOTS>
 __global__ void __launch_bounds__(1024) k_add_rmsnorm_fp8(const add_norm_args p, uint8_t * y, int64_t y_row, float * s, int64_t s_row, int64_t s_block) {
-    __shared__ float wave_sq[16];
+    __shared__ double wave_sq[16];
     __shared__ float wsm[SLOTS ? 1024 : 1];
     const int64_t tok = blockIdx.x, base = tok * p.n;
     const int threads = blockDim.x;
@@ -836,14 +840,15 @@ __global__ void __launch_bounds__(1024) k_add_rmsnorm_fp8(const add_norm_args p,
         }
         __syncthreads();
     }
-    float v[C][8], sq = 0.f;
+    std::conditional_t<SLOTS, double, float> v[C][8];
+    double sq = 0;
     u32x4_t gamma[C];
 #pragma unroll
     for (int j = 0; j < C; j++) {
         const int i0 = (j * threads + threadIdx.x) * 8;
         u32x4_t a = {}, b = {}, c = {};
         gamma[j] = u32x4_t{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u}; // ones
-        float acc[8] = {};
+        double acc[8] = {};
         if (i0 < p.n) {
             a = *(const u32x4_t *) (p.a + base + i0);
             if (p.b) {
@@ -870,52 +875,57 @@ __global__ void __launch_bounds__(1024) k_add_rmsnorm_fp8(const add_norm_args p,
                         if (k0 + k < p.n_used) {
 #pragma unroll
                             for (int e = 0; e < 8; e++) {
-                                acc[e] = fmaf(wsm[k0 + k], e < 4 ? lo[k][e & 3] : hi[k][e & 3], acc[e]);
+                                acc[e] = fma((double) wsm[k0 + k], (double) (e < 4 ? lo[k][e & 3] : hi[k][e & 3]), acc[e]);
                             }
                         }
                     }
                 }
             }
         }
-        float fb[8], fc[8];
-        bf16x8_to_f32(a, v[j]);
+        float fa[8], fb[8], fc[8];
+        bf16x8_to_f32(a, fa);
         bf16x8_to_f32(b, fb);
         bf16x8_to_f32(c, fc);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            v[j][e] = ((v[j][e] + fb[e]) + fc[e]) + acc[e];
-            sq = fmaf(v[j][e], v[j][e], sq);
+            // (a sum of BF16 numbers is exact in FP32 unless they are 2^16 apart)
+            v[j][e] = SLOTS ? (double) ((fa[e] + fb[e]) + fc[e]) + acc[e] : (fa[e] + fb[e]) + fc[e];
+            sq = fma((double) v[j][e], (double) v[j][e], sq);
         }
     }
-    sq = wave_sum(sq);
+    sq = wave_sum64(sq);
     if ((threadIdx.x & 63) == 0) {
         wave_sq[threadIdx.x >> 6] = sq;
     }
     __syncthreads();
-    float total = 0.f;
+    double total = 0;
     for (int i = 0; i < threads >> 6; i++) {
         total += wave_sq[i];
     }
-    const float scale = 1.0f / sqrtf(total / (float) p.n + p.eps);
+    const double scale = 1.0 / sqrt(total / (double) p.n + (double) p.eps);
 #pragma unroll
     for (int j = 0; j < C; j++) {
         const int i0 = (j * threads + threadIdx.x) * 8;
         const bool in = i0 < p.n;
+        float g[8], y32[8];
         if (in && p.y_sum) {
-            *(u32x4_t *) (p.y_sum + base + i0) = to_bf16x8(v[j]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                y32[e] = (float) v[j][e];
+            }
+            *(u32x4_t *) (p.y_sum + base + i0) = to_bf16x8(y32);
         }
-        float g[8];
         bf16x8_to_f32(gamma[j], g);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            v[j][e] = v[j][e] * scale * g[e];
+            y32[e] = (float) ((double) v[j][e] * scale * (double) g[e]);
         }
         if (in && p.y_norm) {
-            *(u32x4_t *) (p.y_norm + base + i0) = to_bf16x8(v[j]);
+            *(u32x4_t *) (p.y_norm + base + i0) = to_bf16x8(y32);
         }
-        const fp8_scales q = fp8_scales_of(row_max_dpp(most_of8(v[j])));
+        const fp8_scales q = fp8_scales_of(row_max_dpp(most_of8(y32)));
         if (in) {
-            *(u32x2_t *) (y + tok * y_row + i0) = fp8_pack8(v[j], q.inverse);
+            *(u32x2_t *) (y + tok * y_row + i0) = fp8_pack8(y32, q.inverse);
             if ((threadIdx.x & 15) == 0) {
                 s[tok * s_row + i0 / FP8_BLOCK * s_block] = q.scale;
             }

@@ -7,24 +7,6 @@ namespace dev {
 
 namespace {
 
-// the same lanes' sums as wave_sum_dpp, in 64 bits; every lane gets the result
-template <int CTRL, int ROW_MASK>
-__device__ __forceinline__ double dpp_add64(double v) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int) u, CTRL, ROW_MASK, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, (int) (u >> 32), CTRL, ROW_MASK, 0xf, false);
-    return v + __builtin_bit_cast(double, (uint64_t) hi << 32 | lo);
-}
-__device__ __forceinline__ double wave_add(double v) {
-    v = dpp_add64<0xB1, 0xf>(v);
-    v = dpp_add64<0x4E, 0xf>(v);
-    v = dpp_add64<0x141, 0xf>(v);
-    v = dpp_add64<0x140, 0xf>(v);
-    v = dpp_add64<0x142, 0xa>(v);
-    v = dpp_add64<0x143, 0xc>(v);
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = __builtin_amdgcn_readlane((int) u, 63), hi = __builtin_amdgcn_readlane((int) (u >> 32), 63);
-    return __builtin_bit_cast(double, (uint64_t) hi << 32 | lo);
-}
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     v = max(v, dpp_take<0xB1, 0xf>(v));
     v = max(v, dpp_take<0x4E, 0xf>(v));
@@ -88,7 +70,7 @@ __global__ void __launch_bounds__(256) k_router_grouped(const router_grouped_arg
             score[q] = logit[q] == -INFINITY ? 0.0 : logit[q] == mx ? 1.0 : exp((double) logit[q] - (double) mx);
             sum += score[q];
         }
-        sum = wave_add(sum);
+        sum = wave_sum64(sum);
 #pragma unroll
         for (int q = 0; q < NQ; q++) {
             score[q] = sum > 0 ? score[q] / sum : 0.0;
@@ -198,7 +180,7 @@ __global__ void __launch_bounds__(256) k_router_grouped(const router_grouped_arg
         mine_id = lane == j ? id : mine_id; // k <= 64
     }
     const double p = lane < a.k ? mine[mine_id] : 0.0;
-    const double top = a.renorm ? wave_add(p) : 1.0;
+    const double top = a.renorm ? wave_sum64(p) : 1.0;
     if (lane < a.k) {
         a.ids[token * a.out_stride + lane] = mine_id;
         a.weights[token * a.out_stride + lane] = (float) ((a.renorm ? top > 0 ? p / top : 0.0 : p) * (double) a.scale);
