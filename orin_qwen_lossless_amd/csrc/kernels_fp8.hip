@@ -510,16 +510,18 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
         }
         begin += (gridDim.z - 1 - blockIdx.z) * COLS; // (later passes of long lists first)
     } else {
-        // An XCD takes every eighth block, which is made a contiguous part of the tiles here: four column tiles of one row tile
-        // after the other, so that what runs there at a time shares few pieces of either side.
+        // An XCD takes every eighth block, which is made a contiguous part of the tiles here: WIDEST column tiles of one row tile
+        // after the other, more of them where they are the smaller, so that what runs there at a time shares few pieces of either side
+        // (gated, BF16 results, us with four everywhere: 2048 x 2048, 128 columns 13.8 for 10.9; 1408 x 2048, 600 16.4 for 15.7).
         const int row_tiles = (p.nrows + ROWS - 1) / ROWS, col_tiles = (p.ncols + COLS - 1) / COLS;
         const int n = row_tiles * col_tiles, per = (n + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
         if ((int) (blockIdx.x >> 3) >= per || id >= n) {
             return;
         }
-        const int group = id / (row_tiles * 4), in = id - group * row_tiles * 4, wide = min(4, col_tiles - group * 4);
+        constexpr int WIDEST = A_ROWS <= COLS ? 4 : A_ROWS <= 2 * COLS ? 6 : A_ROWS <= 4 * COLS ? 8 : A_ROWS <= 8 * COLS ? 12 : 24;
+        const int group = id / (row_tiles * WIDEST), in = id - group * row_tiles * WIDEST, wide = min(WIDEST, col_tiles - group * WIDEST);
         row_tile = in / wide;
-        begin = (group * 4 + in % wide) * COLS;
+        begin = (group * WIDEST + in % wide) * COLS;
         end = min(end, begin + COLS);
     }
     const int row0 = row_tile * ROWS, KB = p.KB;
@@ -597,10 +599,11 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
                     asm volatile("" : "+v"(sw[m]));
                 }
             };
-            load_scales(0);
             // (before a list's next columns: nothing reads LDS any more, no store is under way)
-            wait_loads<0>();
-            meet();
+            if (LIST) {
+                wait_loads<0>();
+                meet();
+            }
 #pragma unroll
             for (int s = 0; s < S - 1; s++) {
                 if (s < KB) {
@@ -608,9 +611,7 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
                 }
             }
             for (int s64 = 0; s64 < KB; s64 += 64) {
-                if (s64 > 0) {
-                    load_scales(s64);
-                }
+                load_scales(s64);
                 const int s_end = min(s64 + 64, KB);
                 for (int s = s64; s < s_end; s++) {
                     // this wavefront's copies of the step are in LDS; those of up to S - 2 later ones are under way
@@ -635,29 +636,36 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
                             both[m][c] = __uint_as_float((uint32_t) __builtin_amdgcn_readlane((int) __float_as_uint(sw[m]), s - s64)) * sx;
                         }
                     }
-                    u32x4_t b[M][2], a[2][2];
+                    u32x4_t b[M][2], a[WIDE ? RT : 2][2];
                     fp8_wide bw[M];
 #pragma unroll
                     for (int c = 0; c < M; c++) {
                         b[c][0] = *(const u32x4_t *) (at + b_frag + c * WC * 16 * FP8_BLOCK + frag0);
                         b[c][1] = *(const u32x4_t *) (at + b_frag + c * WC * 16 * FP8_BLOCK + frag1);
-                        if constexpr (WIDE) {
+                    }
+#pragma unroll
+                    for (int t = 0; t < (WIDE ? RT : 1); t++) {
+                        a[t][0] = *(const u32x4_t *) (at + a_frag + t * 16 * FP8_BLOCK + frag0);
+                        a[t][1] = *(const u32x4_t *) (at + a_frag + t * 16 * FP8_BLOCK + frag1);
+                    }
+                    if constexpr (WIDE) { // (the compiler puts every read right ahead of its use: 2048 tokens of 256 experts 196 us for 192)
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int c = 0; c < M; c++) {
                             bw[c] = fp8_widen(b[c][0], b[c][1]);
                         }
                     }
-                    a[0][0] = *(const u32x4_t *) (at + a_frag + frag0);
-                    a[0][1] = *(const u32x4_t *) (at + a_frag + frag1);
                     f32x4_t part[2][M];
 #pragma unroll
                     for (int t = 0; t <= RT; t++) {
                         fp8_wide aw;
                         if (t < RT) {
-                            if (t + 1 < RT) {
+                            if (!WIDE && t + 1 < RT) {
                                 a[(t + 1) & 1][0] = *(const u32x4_t *) (at + a_frag + (t + 1) * 16 * FP8_BLOCK + frag0);
                                 a[(t + 1) & 1][1] = *(const u32x4_t *) (at + a_frag + (t + 1) * 16 * FP8_BLOCK + frag1);
                             }
                             if constexpr (WIDE) {
-                                aw = fp8_widen(a[t & 1][0], a[t & 1][1]);
+                                aw = fp8_widen(a[t][0], a[t][1]);
                             }
                         }
 #pragma unroll
@@ -826,7 +834,7 @@ __device__ __forceinline__ u32x4_t to_bf16x8(const float (&v)[8]) {
 // in registers between the sum of its squares and its codes.  The slots' sum, the squares' and the norm are held in 64 bits and become
 // FP32 once, ahead of the scales: a code is off by a whole step, a sixteenth of its value, wherever an error of a last place carries a value over the
 // middle of two codes, which 32 bits did to one or two of 858 thousand (and were 8.9 us there for 9.6).
-// 8192 tokens of 2048: 22.9 us, 134 MB at 5.8 TB/s; one token 2.8, the chain of its loads, sum and scale.
+// 8192 tokens of 2048: 22.9 us, 118 MB at 5.2 TB/s; one token 2.8, the chain of its loads, sum and scale.
 template <int C, bool SLOTS>
 __global__ void __launch_bounds__(1024) k_add_rmsnorm_fp8(const add_norm_args p, uint8_t * y, int64_t y_row, float * s, int64_t s_row, int64_t s_block) {
     __shared__ double wave_sq[16];
