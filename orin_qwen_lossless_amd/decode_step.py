@@ -30,10 +30,10 @@ SHAPES = {"qkv": (QKV_ROWS, K_MODEL, 1), "o": (K_MODEL, ATT, 1), "router": (E, K
 
 def encode_policy(ops, w_dev: torch.Tensor, n_matrices: int = 1, mode: str = "hybrid"):
     """[rows, K] BF16 device tensor -> (Weight in the layout of the mi355x policy, compressed bytes).  mode: the policy's
-    (hybrid, huffman or nibble: the 4-bit code for everything), or "int4": 4-bit weights with group scales, which are not
-    lossless (Int4Weight)."""
-    if mode == "int4":
-        w = ops.int4_quantize(w_dev)
+    (hybrid, huffman or nibble: the 4-bit code for everything), or one that is not lossless: "int4", 4-bit weights with group scales
+    (Int4Weight), "fp8", 8-bit floating point with block scales (Fp8Weight)."""
+    if mode in ("int4", "fp8"):
+        w = ops.int4_quantize(w_dev) if mode == "int4" else ops.fp8_quantize(w_dev, n_matrices)
         return w, w.nbytes
     rows, k = w_dev.shape
     fmt, R, cm, _, w64 = ops.choose(rows // n_matrices, k, n_matrices, engine="mi355x", mode=mode, expert=n_matrices > 1)
@@ -43,17 +43,18 @@ def encode_policy(ops, w_dev: torch.Tensor, n_matrices: int = 1, mode: str = "hy
     return ops.upload(torch.from_numpy(plane), ta, ops.parse_header(ta), w_dev.device), plane.size + aux.size
 
 
-def make_layer_sets(ops, gen_weights, n_sets: int, keep_bf16: bool, expert_mode: str = "hybrid"):
+def make_layer_sets(ops, gen_weights, n_sets: int, keep_bf16: bool, expert_mode: str = "hybrid", dense_mode: str = "hybrid"):
     """n_sets weight sets of one layer.  gen_weights(rows, K) -> BF16 device tensor.  Returns (encoded sets, BF16 sets or
     None, compressed bytes by matrix name of one set).  expert_mode "nibble": the expert stacks in the 4-bit code (7 %
     more bytes than the policy's tiles, no decode chain: the form for decode at one or two tokens).  "int4": 4-bit weights with
-    group scales (0.52 byte a weight, not lossless)."""
+    group scales (0.52 byte a weight, not lossless); "fp8": 8-bit floating point with block scales (one byte a weight, not lossless).
+    dense_mode "fp8": qkv and o in the same form (the router is always lossless)."""
     enc_sets, raw_sets, nbytes = [], [] if keep_bf16 else None, {}
     for _ in range(n_sets):
         enc, raw = {}, {}
         for name, (rows, k, nm) in SHAPES.items():
             w = gen_weights(rows, k)
-            enc[name], nbytes[name] = encode_policy(ops, w, nm, expert_mode if nm > 1 else "hybrid")
+            enc[name], nbytes[name] = encode_policy(ops, w, nm, expert_mode if nm > 1 else dense_mode if name in ("qkv", "o") else "hybrid")
             if keep_bf16:
                 raw[name] = w
         enc_sets.append(enc)
@@ -92,7 +93,15 @@ class Bf16nStep:
 
     def __init__(self, ops, sets, head, n_layers: int, n_tok: int):
         self.ops, self.sets, self.head, self.n_layers = ops, sets, head, n_layers
-        self.routing = routing_buffers(n_tok, sets[0]["qkv"].plane.device)
+        self.routing = routing_buffers(n_tok, sets[0]["router"].plane.device)
+
+    def linear(self, x, w):
+        ops = self.ops
+        return (ops.fp8_linear if isinstance(w, ops.Fp8Weight) else ops.int4_linear if isinstance(w, ops.Int4Weight) else ops.linear)(x, w)
+
+    def norm_for(self, w):
+        """The glue whose norm is what a product on w takes: codes with scales, or BF16."""
+        return self.ops.add_rmsnorm_fp8 if isinstance(w, self.ops.Fp8Weight) else self.ops.add_rmsnorm
 
     def experts(self, w, x2, logits=None):
         """(ys [T, 9, K] FP32 per-slot outputs, wts [T, 9], ids [T, 9]).  logits: the router's, if the caller has them."""
@@ -101,6 +110,9 @@ class Bf16nStep:
         if isinstance(w["gate"], ops.Int4Weight):
             wts, ids = ops.router_topk(logits, TOPK, out=self.routing)
             return ops.int4_moe_experts_rows(x2, w["gate"], w["up"], w["down"], ids, EA), wts, ids
+        if isinstance(w["gate"], ops.Fp8Weight):
+            wts, ids = ops.router_topk(logits, TOPK, out=self.routing)
+            return ops.fp8_moe_experts_rows(x2, w["gate"], w["up"], w["down"], ids, EA), wts, ids
         batched = ops.moe_experts_batched(x2.shape[0], TOPK + 1, w["gate"], w["up"], w["down"], EA)
         if not batched and ops.topk_in_gemv_supported(w["gate"], w["up"], E, TOPK):
             # the gate / up GEMV selects the experts itself: no top-k launch
@@ -113,24 +125,25 @@ class Bf16nStep:
             wts, ids = ops.router_topk(logits, TOPK, out=self.routing)
         return ops.moe_experts_rows(x2, w["gate"], w["up"], w["down"], ids, EA, routes), wts, ids
 
-    def layer(self, w, h, x1):
+    def layer(self, w, h, x1, norm=None):
+        """norm: the glue behind the experts (norm_for the matrix that takes the layer's norm), BF16 if none is named."""
         ops = self.ops
-        q = ops.linear(x1, w["qkv"])
-        o = ops.linear(q[:, :ATT], w["o"])
+        q = self.linear(x1, w["qkv"])
+        o = self.linear(q[:, :ATT], w["o"])
         if ops.add_rmsnorm_mmv_supported(w["router"], h.shape[0], h, o):
             x2, h2, logits = ops.add_rmsnorm_mmv(h, w["router"], o)  # the router forms its own input
         else:
             (x2, h2), logits = ops.add_rmsnorm(h, o, want_sum=True), None
         ys, wts, _ = self.experts(w, x2, logits)
-        return ops.add_rmsnorm(h2, ys=ys, topk_weights=wts, want_sum=True)  # (x1', h')
+        return (norm or ops.add_rmsnorm)(h2, ys=ys, topk_weights=wts, want_sum=True)  # (x1', h')
 
     def __call__(self, h):
-        x1 = self.ops.add_rmsnorm(h)
+        x1 = self.norm_for(self.sets[0]["qkv"])(h)
         for i in range(self.n_layers):
-            x1, h = self.layer(self.sets[i % len(self.sets)], h, x1)
-        if isinstance(self.head, self.ops.Int4Weight):  # a draft copy of the output projection
-            return self.ops.int4_linear(x1, self.head)
-        return self.ops.linear(x1, self.head) if self.head is not None else x1
+            behind = self.head if i + 1 == self.n_layers else self.sets[(i + 1) % len(self.sets)]["qkv"]
+            x1, h = self.layer(self.sets[i % len(self.sets)], h, x1, self.norm_for(behind))
+        # (the head may be a draft copy of the output projection)
+        return self.linear(x1, self.head) if self.head is not None else x1
 
 
 class Bf16Step:

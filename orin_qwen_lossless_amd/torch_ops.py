@@ -10,7 +10,9 @@ registered from Python over the C ABI, with the reference's fake (meta) implemen
 
 `meta` is the reference's list; bit 2 of meta[4] (flags) marks the wave64 layout.  The int4 / int2 baseline ops of the
 reference extension are not part of the BF16N path and are not registered.  This build's additions: encode_auto, and for 4-bit weights
-with group scales (ops.Int4Weight: codes, scales, zeros, group) int4_linear and int4_moe_experts, with router_topk_grouped."""
+with group scales (ops.Int4Weight: codes, scales, zeros, group) int4_linear and int4_moe_experts, with router_topk_grouped; for 8-bit
+floating point with block scales (ops.Fp8Weight: codes, scales; activations BF16 / FP32 without x_scales, or codes with them)
+fp8_quantize_rows, add_rmsnorm_fp8, fp8_linear, fp8_linear_glu2 and fp8_moe_experts."""
 from __future__ import annotations
 
 import torch
@@ -35,6 +37,12 @@ _lib.define("router_topk_grouped(Tensor logits, int k, Tensor? bias, int n_group
             "bool renorm, float scale) -> (Tensor, Tensor)")
 _lib.define("int4_linear(Tensor x, Tensor codes, Tensor scales, Tensor? zeros, int group, Tensor? bias) -> Tensor")
 _lib.define("int4_moe_experts(Tensor x, Tensor[] gate, Tensor[] up, Tensor[] down, int group, Tensor topk_weights, Tensor topk_ids, "
+            "int n_experts) -> Tensor")
+_lib.define("fp8_quantize_rows(Tensor x) -> (Tensor, Tensor)")
+_lib.define("add_rmsnorm_fp8(Tensor a, Tensor? b, Tensor? c, Tensor? ys, Tensor? topk_weights, Tensor? gamma, float eps) -> (Tensor, Tensor, Tensor)")
+_lib.define("fp8_linear(Tensor x, Tensor? x_scales, Tensor codes, Tensor scales, Tensor? bias, bool out_bf16) -> Tensor")
+_lib.define("fp8_linear_glu2(Tensor x, Tensor? x_scales, Tensor gate, Tensor gate_scales, Tensor up, Tensor up_scales, bool out_bf16) -> Tensor")
+_lib.define("fp8_moe_experts(Tensor x, Tensor? x_scales, Tensor[] gate, Tensor[] up, Tensor[] down, Tensor topk_weights, Tensor topk_ids, "
             "int n_experts) -> Tensor")
 
 
@@ -135,12 +143,46 @@ def _int4_moe_experts(x, gate, up, down, group, topk_weights, topk_ids, n_expert
     return ops.int4_moe_experts(x, _int4(gate, group), _int4(up, group), _int4(down, group), topk_weights, topk_ids, n_experts)
 
 
+def _fp8_rows(x, x_scales):
+    return x if x_scales is None else ops.Fp8Rows(x, x_scales)
+
+
+def _fp8(tensors, n_experts: int) -> ops.Fp8Weight:
+    if len(tensors) != 2:
+        raise ValueError("bf16n: an 8-bit weight is [codes, scales]")
+    return ops.Fp8Weight(tensors[0], tensors[1], int(n_experts))
+
+
+def _fp8_quantize_rows(x):
+    r = ops.fp8_quantize_rows(x)
+    return r.codes, r.scales
+
+
+def _add_rmsnorm_fp8(a, b, c, ys, topk_weights, gamma, eps):
+    r, total = ops.add_rmsnorm_fp8(a, b, c, ys, topk_weights, gamma, eps, want_sum=True)
+    return r.codes, r.scales, total
+
+
+def _fp8_linear(x, x_scales, codes, scales, bias, out_bf16):
+    return ops.fp8_linear(_fp8_rows(x, x_scales), ops.Fp8Weight(codes, scales), bias, _dt(out_bf16))
+
+
+def _fp8_linear_glu2(x, x_scales, gate, gate_scales, up, up_scales, out_bf16):
+    return ops.fp8_linear_glu2(_fp8_rows(x, x_scales), ops.Fp8Weight(gate, gate_scales), ops.Fp8Weight(up, up_scales), _dt(out_bf16))
+
+
+def _fp8_moe_experts(x, x_scales, gate, up, down, topk_weights, topk_ids, n_experts):
+    return ops.fp8_moe_experts(_fp8_rows(x, x_scales), _fp8(gate, n_experts), _fp8(up, n_experts), _fp8(down, n_experts), topk_weights, topk_ids, n_experts)
+
+
 _lib.impl("init", _init, "CompositeExplicitAutograd")
 _lib.impl("encode", _encode_cpu, "CPU")
 _lib.impl("encode_auto", _encode_auto_cpu, "CPU")
 for _name, _fn in (("dequant", _dequant), ("mmv", _mmv), ("mmv_glu", _mmv_glu), ("linear", _linear), ("get_rows", _get_rows),
                    ("moe_mm_ids", _moe_mm_ids), ("moe_combine", _moe_combine), ("swiglu", _swiglu), ("router_topk", _router_topk),
-                   ("router_topk_grouped", _router_topk_grouped), ("int4_linear", _int4_linear), ("int4_moe_experts", _int4_moe_experts)):
+                   ("router_topk_grouped", _router_topk_grouped), ("int4_linear", _int4_linear), ("int4_moe_experts", _int4_moe_experts),
+                   ("fp8_quantize_rows", _fp8_quantize_rows), ("add_rmsnorm_fp8", _add_rmsnorm_fp8), ("fp8_linear", _fp8_linear),
+                   ("fp8_linear_glu2", _fp8_linear_glu2), ("fp8_moe_experts", _fp8_moe_experts)):
     _lib.impl(_name, _fn, "CUDA")
 
 
@@ -223,4 +265,33 @@ def _int4_linear_fake(x, codes, scales, zeros, group, bias):
 
 @torch.library.register_fake("bf16n::int4_moe_experts")
 def _int4_moe_experts_fake(x, gate, up, down, group, topk_weights, topk_ids, n_experts):
+    return x.new_empty((x.shape[0], down[0].shape[0] // n_experts), dtype=torch.bfloat16)
+
+
+def _fp8_rows_fake(x):
+    return x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty((-(-x.shape[1] // ops.FP8_BLOCK), x.shape[0]), dtype=torch.float32).t()
+
+
+@torch.library.register_fake("bf16n::fp8_quantize_rows")
+def _fp8_quantize_rows_fake(x):
+    return _fp8_rows_fake(x)
+
+
+@torch.library.register_fake("bf16n::add_rmsnorm_fp8")
+def _add_rmsnorm_fp8_fake(a, b, c, ys, topk_weights, gamma, eps):
+    return (*_fp8_rows_fake(a), torch.empty_like(a))
+
+
+@torch.library.register_fake("bf16n::fp8_linear")
+def _fp8_linear_fake(x, x_scales, codes, scales, bias, out_bf16):
+    return x.new_empty((*x.shape[:-1], codes.shape[0]), dtype=_dt(out_bf16))
+
+
+@torch.library.register_fake("bf16n::fp8_linear_glu2")
+def _fp8_linear_glu2_fake(x, x_scales, gate, gate_scales, up, up_scales, out_bf16):
+    return x.new_empty((x.shape[0], gate.shape[0]), dtype=_dt(out_bf16))
+
+
+@torch.library.register_fake("bf16n::fp8_moe_experts")
+def _fp8_moe_experts_fake(x, x_scales, gate, up, down, topk_weights, topk_ids, n_experts):
     return x.new_empty((x.shape[0], down[0].shape[0] // n_experts), dtype=torch.bfloat16)
