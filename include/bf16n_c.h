@@ -252,7 +252,7 @@ typedef struct bf16n_fp8_rows {
 } bf16n_fp8_rows;
 /* BF16 or FP32 rows of K values (a multiple of 16 in [16, 32768]) as codes with scales. */
 int bf16n_fp8_quantize_rows(const bf16n_fp8_rows * x, const bf16n_fp8_rows * y, int64_t n_rows, int64_t K, void * stream);
-/* bf16n_add_rmsnorm with the norm in 8 bits: the FP32 value is rounded once, to its code.  y_sum (BF16 sum), y_norm (BF16 norm beside the
+/* bf16n_add_rmsnorm with the norm in 8 bits: sums and norm are held in 64 bits, the FP32 value is rounded once, to its code.  y_sum (BF16 sum), y_norm (BF16 norm beside the
  * codes) may be null.  n: a multiple of 16, at most 16384; every pointer 16-byte aligned. */
 int bf16n_add_rmsnorm_fp8(const uint16_t * a, const uint16_t * b, const uint16_t * c, const float * ys, const void * wts, int wts_bf16, int n_used,
                           const uint16_t * gamma, const bf16n_fp8_rows * y, uint16_t * y_sum, uint16_t * y_norm, int n_tok, int64_t n, float eps,
@@ -273,7 +273,7 @@ int bf16n_fp8_mm_ids(const bf16n_fp8_weight * w, const bf16n_fp8_weight * up, co
                      int64_t ids_s0, int64_t ids_s1, const int32_t * pairs, const int32_t * bounds, const bf16n_fp8_rows * y, int n_tok, int n_used,
                      void * workspace, uint64_t workspace_bytes, void * stream);
 /* The routed experts of a layer: y[t] = sum over the slots of wts[t, slot] * down_e(silu(gate_e x[t]) * (up_e x[t])), hidden rows held in 8
- * bits (from FP32 values), the slots' results in FP32 or, where the pairs are more than the experts, in BF16 (half a step each, at most
+ * bits (from FP32 values), the slots' results in FP32 or, where the pairs are more than 64 or than the experts, in BF16 (half a step each, at most
  * 2^-9 of a slot's result, beside the 2^-4 of the codes).  wts null: y has a row of FP32 for every pair, unweighted.  wts: FP32 or BF16
  * [n_tok, n_used].  y: BF16 or FP32, contiguous rows. */
 int bf16n_fp8_moe_experts(const bf16n_fp8_weight * gate, const bf16n_fp8_weight * up, const bf16n_fp8_weight * down, const bf16n_fp8_rows * x,

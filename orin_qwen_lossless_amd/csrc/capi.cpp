@@ -858,6 +858,10 @@ struct experts_plan { // offsets in the workspace
     int hidden_kind; // hidden rows as down takes them: codes, or FP32 where its blocks make the codes
     uint64_t lists, hidden, hidden_scales, ys, product, bytes;
 };
+// As many pairs are products by themselves, each reading its matrix, before they are listed by expert for three launches more (256 experts of
+// 512 x 2048, top-8, us by themselves / listed: 8 tokens 41 / 44, 12 68 / 62, 32 127 / 110; 64 of 1024 x 1024, top-6: 6 33 / 34, 8 42 / 39), and as many as there are experts.
+constexpr int64_t FP8_SINGLE_PAIRS = 64;
+
 experts_plan plan_experts(const bf16n_fp8_weight & gate, const bf16n_fp8_weight & down, int x_kind, bool weighted, int n_tok, int n_used) {
     const int64_t pairs = (int64_t) n_tok * n_used, mid = gate.rows / gate.n_matrices, out = down.rows / down.n_matrices;
     experts_plan e = {};
@@ -865,11 +869,11 @@ experts_plan plan_experts(const bf16n_fp8_weight & gate, const bf16n_fp8_weight 
         at = e.bytes;
         e.bytes += (n + 255) / 256 * 256;
     };
-    // while the pairs are no more than the experts each is a column by itself
-    e.listed = pairs > gate.n_matrices;
+    // few pairs: each is a column by itself
+    e.listed = pairs > std::min<int64_t>(gate.n_matrices, FP8_SINGLE_PAIRS);
     e.half = e.listed && weighted && out % 8 == 0;
     e.fused = !e.listed && weighted && dev::fp8_down_fits(down, n_used);
-    e.hidden_kind = e.listed && !dev::fp8_few_listed(gate, pairs) ? BF16N_FP8_CODES : BF16N_FP8_F32;
+    e.hidden_kind = e.listed ? BF16N_FP8_CODES : BF16N_FP8_F32;
     if (e.listed) {
         take(e.lists, (pairs + gate.n_matrices + 2) * 4);
     }

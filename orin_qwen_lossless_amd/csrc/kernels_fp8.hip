@@ -29,7 +29,7 @@ struct fp8_launch {
     uint32_t per_token, one_per;            // the activation row of a pair is pair / per_token; 2^32 / per_token, rounded down
     const char * ids; int64_t ids_s0, ids_s1; bool ids_i64; int n_used; // one matrix per pair
     const int32_t * pairs, * bounds;        // pairs sorted by matrix
-    int ksplit, lds_cols, cus;
+    int ksplit, lds_cols, cus, passes, tiles;
     uint32_t one_block;                     // 2^32 / KB, rounded up: exact for the items of a pass (below 2^32 / KB)
 };
 
@@ -109,17 +109,7 @@ __global__ void __launch_bounds__(NW * 64, ONE ? 2 : CT * (GLU ? 2 : 1) == 1 ? 4
     int begin = 0, end = p.ncols;
     const int ksplit = ONE ? NW : p.ksplit, groups = NW / ksplit, kp = wave % ksplit, group = wave / ksplit;
     const int row_step = gridDim.x * groups * 16;
-    if (p.pairs) {
-        matrix = blockIdx.y;
-        begin = p.bounds[matrix];
-        end = p.bounds[matrix + 1];
-        if (matrix == p.n_matrices) {
-            for (int c = begin + blockIdx.z; c < end; c += gridDim.z) {
-                zero_row(p, p.pairs[c], 0, p.nrows, blockIdx.x * NW * 64 + threadIdx.x, gridDim.x * NW * 64);
-            }
-            return;
-        }
-    } else if (p.ids) {
+    if (p.ids) {
         const int t = blockIdx.y / p.n_used, i = blockIdx.y % p.n_used;
         const char * at = p.ids + t * p.ids_s1 + i * p.ids_s0;
         matrix = p.ids_i64 ? *(const int64_t *) at : *(const int32_t *) at;
@@ -130,8 +120,7 @@ __global__ void __launch_bounds__(NW * 64, ONE ? 2 : CT * (GLU ? 2 : 1) == 1 ? 4
             return;
         }
     }
-    const auto y_of = [&](int c) -> int64_t { return p.pairs ? p.pairs[c] : c; };
-    const auto x_of = [&](int c) -> int64_t { return p.pairs ? row_of_pair(p, p.pairs[c]) : p.ids ? row_of_pair(p, c) : c; };
+    const auto x_of = [&](int c) -> int64_t { return p.ids ? row_of_pair(p, c) : c; };
 
     const int s0 = KB * kp / ksplit, steps = KB * (kp + 1) / ksplit - s0; // (at most FEW_PARTS)
     const bool cut = p.K % FP8_BLOCK != 0 && s0 + steps == KB;
@@ -141,7 +130,7 @@ __global__ void __launch_bounds__(NW * 64, ONE ? 2 : CT * (GLU ? 2 : 1) == 1 ? 4
 
     const int pass = p.lds_cols;
     const auto column_of = [&](int i) { return KB == 1 ? i : (int) __umulhi((uint32_t) i, p.one_block); }; // i / KB
-    for (int c0 = begin + (p.ids ? 0 : p.pairs ? blockIdx.z : blockIdx.y) * pass; c0 < end; c0 += (p.ids ? 1 : p.pairs ? gridDim.z : gridDim.y) * pass) {
+    for (int c0 = p.ids ? begin : blockIdx.y * pass; c0 < end; c0 += p.ids ? 1 : gridDim.y * pass) {
         const int nc = min(end - c0, pass);
         u32x4_t w[D][NM][2];
         const uint8_t * at[NM]; // the 16 rows whose loads are under way
@@ -337,9 +326,9 @@ __global__ void __launch_bounds__(NW * 64, ONE ? 2 : CT * (GLU ? 2 : 1) == 1 ? 4
                     }
                 }
                 if (p.y_kind == BF16) {
-                    store4<BF16>(p, y_of(c0 + c), r0 + 4 * q, v);
+                    store4<BF16>(p, c0 + c, r0 + 4 * q, v);
                 } else {
-                    store4<F32>(p, y_of(c0 + c), r0 + 4 * q, v);
+                    store4<F32>(p, c0 + c, r0 + 4 * q, v);
                 }
             }
         }
@@ -476,18 +465,74 @@ __device__ __forceinline__ void meet() {
     asm volatile("" ::: "memory");
 }
 
+// the sum over this lane and those below it
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int dpp_below(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xf, false); }
+__device__ __forceinline__ int wave_scan(int v) {
+    v = dpp_below<0x111, 0xf>(v); // row_shr 1, 2, 4, 8
+    v = dpp_below<0x112, 0xf>(v);
+    v = dpp_below<0x114, 0xf>(v);
+    v = dpp_below<0x118, 0xf>(v);
+    v = dpp_below<0x142, 0xa>(v); // row_bcast 15, 31
+    return dpp_below<0x143, 0xc>(v);
+}
+
+// The columns of pass `pass` of all lists, `cols` to a pass: every wavefront looks for itself, eight lists to a lane, 512 at a time.  matrix: -1 if
+// there are fewer passes.
+struct list_pass { int matrix, begin, end; };
+__device__ __forceinline__ list_pass find_pass(const int32_t * bounds, int n_matrices, int pass, int cols) {
+    constexpr int PER = 8;
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int m0 = 0; m0 <= n_matrices; m0 += 64 * PER) { // (n_matrices: the pairs that name none)
+        int b[PER + 1], mine = 0;
+#pragma unroll
+        for (int i = 0; i <= PER; i++) {
+            b[i] = bounds[min(m0 + lane * PER + i, n_matrices + 1)];
+        }
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            mine += (b[i + 1] - b[i] + cols - 1) / cols;
+        }
+        const int upto = before + wave_scan(mine);
+        const uint64_t behind = __ballot(upto > pass);
+        if (behind) {
+            const int owner = __builtin_ctzll(behind);
+            int left = pass - (upto - mine), matrix = 0, begin = 0, end = 0;
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int n = (b[i + 1] - b[i] + cols - 1) / cols;
+                if (left >= 0 && left < n) {
+                    matrix = m0 + lane * PER + i;
+                    begin = b[i] + left * cols;
+                    end = min(b[i + 1], begin + cols);
+                }
+                left -= n;
+            }
+            return {__builtin_amdgcn_readlane(matrix, owner), __builtin_amdgcn_readlane(begin, owner), __builtin_amdgcn_readlane(end, owner)};
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return {-1, 0, 0};
+}
+
 // WR x WC wavefronts, RT x CT results of 16 x 16 to each.  Codes of both sides go straight into LDS, S - 1 steps of 128 columns ahead:
 // rows of 128 bytes, their eight places of 16 bytes exchanged by the row's low bits so that the operands' reads find every
 // bank.  A step's products start from zero and are added to the results times their scales, those of a row of tiles while the next row's
 // are under way.  BF16 results are summed by the instruction
 // on the codes.  FP32 ones are summed from BF16 operands (fp8_sum16), and so are those that become codes with a scale, which a value
 // 1.5e-5 off would put on the other side of a border now and then (0.0015 of the norm of 300 rows of 1408 that are 0.0003 off so).
-// Lists: a block takes the columns of one matrix, COLS at a time.  OUT8: the results of ROWS = 128 rows leave as codes with a scale.
+// OUT codes: the results of ROWS = 128 rows leave as codes with a scale.
+// Lists: a block to 64 columns of one matrix (every pass a block of its own: where one block took a list's passes in turn, and a CU had one such block
+// with 128 columns, gate and up of 2048 tokens of 256 experts of 512 x 2048 took 190 us for 152, of 512 tokens 128 for 111).  Gate and up: the scales of
+// the columns in registers, so that two blocks' stages are the whole of a CU's LDS.  Down, whose K is short: two row tiles to a block, the second's
+// copies under the first's last products (2048 tokens, one / two / four: 98, 93, 102).
 template <int WR, int WC, int RT, int CT, int S, bool GLU, bool LIST, int OUT>
 __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p) {
-    constexpr bool WIDE = OUT != BF16;
+    constexpr bool WIDE = OUT != BF16, SX_REGS = LIST && GLU, TILES = LIST && !GLU;
+    static_assert(!TILES || S == 2, "a step ahead");
     constexpr int NM = GLU ? 2 : 1, THREADS = WR * WC * 64, A_ROWS = WR * RT * 16, ROWS = A_ROWS / NM, COLS = WC * CT * 16, TM = RT / NM;
-    constexpr int SCALES = (A_ROWS + many_x_rows(COLS, THREADS)) * FP8_BLOCK, STAGE = many_stage(A_ROWS, COLS, THREADS), A_COPIES = A_ROWS * 8 / THREADS, B_COPIES = (COLS * 8 + THREADS - 1) / THREADS;
+    constexpr int SCALES = (A_ROWS + many_x_rows(COLS, THREADS)) * FP8_BLOCK, STAGE = SX_REGS ? (A_ROWS + COLS) * FP8_BLOCK : many_stage(A_ROWS, COLS, THREADS), A_COPIES = A_ROWS * 8 / THREADS, B_COPIES = (COLS * 8 + THREADS - 1) / THREADS;
     static_assert(A_COPIES * THREADS == A_ROWS * 8, "whole copies");
     static_assert(FP8_BLOCK % (TM * 16) == 0, "a wavefront's rows have one scale");
     static_assert(OUT != CODES || ROWS == FP8_BLOCK, "a block of rows has one scale");
@@ -496,20 +541,8 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave % WR, wc = wave / WR;
     int64_t matrix = 0;
-    int begin = 0, end = p.ncols, row_tile;
-    if (LIST) {
-        matrix = blockIdx.y;
-        row_tile = blockIdx.x;
-        begin = p.bounds[matrix];
-        end = p.bounds[matrix + 1];
-        if (matrix == p.n_matrices) {
-            for (int c = begin + blockIdx.z; c < end; c += gridDim.z) {
-                zero_row(p, p.pairs[c], row_tile * ROWS, ROWS, threadIdx.x, THREADS);
-            }
-            return;
-        }
-        begin += (gridDim.z - 1 - blockIdx.z) * COLS; // (later passes of long lists first)
-    } else {
+    int begin = 0, end = p.ncols, row_tile = TILES ? blockIdx.x * p.tiles : blockIdx.x;
+    if (!LIST) {
         // An XCD takes every eighth block, which is made a contiguous part of the tiles here: WIDEST column tiles of one row tile
         // after the other, more of them where they are the smaller, so that what runs there at a time shares few pieces of either side
         // (gated, BF16 results, us with four everywhere: 2048 x 2048, 128 columns 13.8 for 10.9; 1408 x 2048, 600 16.4 for 15.7).
@@ -525,11 +558,11 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
         end = min(end, begin + COLS);
     }
     const int row0 = row_tile * ROWS, KB = p.KB;
+    const int n_tiles = TILES ? min(p.tiles, (p.nrows + ROWS - 1) / ROWS - row_tile) : 1, n_steps = n_tiles * KB;
     const bool cut = p.K % FP8_BLOCK != 0;
 
     // what this thread copies: a place of rows (threadIdx.x >> 3) + i * THREADS / 8, chunk by the row's low bits
     const int chunk = (threadIdx.x & 7) ^ ((threadIdx.x >> 3) & 7);
-    const uint8_t * const w_base = p.w + (matrix * p.nrows + row0) * p.K, * const up_base = p.up + (matrix * p.nrows + row0) * p.K;
     uint32_t a_off[A_COPIES];
     const auto of_up = [&](int i) { return GLU && (i * (THREADS / 8) + wave * 8) / 16 % RT >= TM; };
 #pragma unroll
@@ -538,12 +571,30 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
         a_off[i] = min((t / RT * TM + t % RT % TM) * 16 + r % 16, p.nrows - 1 - row0) * p.K + chunk * 16;
     }
     const int wave_row = row0 + wr * TM * 16;
-    const int64_t scale_row = (matrix * p.NB + min(wave_row, p.nrows - 1) / FP8_BLOCK) * KB;
     const int frag0 = m16 * FP8_BLOCK + ((q ^ (m16 & 7)) << 4), frag1 = frag0 ^ 64;
     const int a_frag = wr * RT * 16 * FP8_BLOCK, b_frag = A_ROWS * FP8_BLOCK + wc * 16 * FP8_BLOCK;
 
-    for (int c0 = begin; c0 < end; c0 += LIST ? gridDim.z * COLS : COLS) {
-        const int nc = min(end - c0, COLS);
+    // Lists: the passes of all matrices in a row, COLS columns each; a block takes the passes blockIdx.y, + gridDim.y ..
+    for (int pass = blockIdx.y; pass < (LIST ? p.passes : 1); pass += gridDim.y) {
+        if (LIST) {
+            const list_pass f = find_pass(p.bounds, (int) p.n_matrices, pass, COLS);
+            if (f.matrix < 0) {
+                return;
+            }
+            matrix = f.matrix;
+            begin = f.begin;
+            end = f.end;
+            __syncthreads(); // nothing reads LDS any more
+            if (matrix == p.n_matrices) {
+                for (int c = begin; c < end; c++) {
+                    zero_row(p, p.pairs[c], row0, n_tiles * ROWS, threadIdx.x, THREADS);
+                }
+                continue;
+            }
+        }
+        const uint8_t * const w_base = p.w + (matrix * p.nrows + row0) * p.K, * const up_base = p.up + (matrix * p.nrows + row0) * p.K;
+        const int64_t scale_row = (matrix * p.NB + min(wave_row, p.nrows - 1) / FP8_BLOCK) * KB;
+        const int c0 = begin, nc = end - begin;
         const auto x_of = [&](int i) -> int64_t { return LIST ? row_of_pair(p, p.pairs[c0 + min(i, nc - 1)]) : c0 + min(i, nc - 1); };
         const char * b_at[B_COPIES];
 #pragma unroll
@@ -551,16 +602,43 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
             b_at[i] = p.x + x_of(i * (THREADS / 8) + (threadIdx.x >> 3)) * p.x_row + chunk * 16;
         }
         const float * const sx_at = p.xs + x_of(threadIdx.x % COLS) * p.xs_row;
+        const float * sxr_at[CT];
+        if constexpr (SX_REGS) {
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                sxr_at[c] = p.xs + x_of((c * WC + wc) * 16 + m16) * p.xs_row;
+            }
+        }
         f32x4_t acc[RT][CT] = {};
+        const auto store = [&](auto columns, int tile) {
+            if constexpr (OUT != CODES) {
+#pragma unroll
+                for (int c = 0; c < decltype(columns)::value; c++) {
+                    const int col = (c * WC + wc) * 16 + m16;
+                    if (col >= nc) {
+                        continue;
+                    }
+                    const int64_t y = LIST ? p.pairs[c0 + col] : c0 + col;
+#pragma unroll
+                    for (int t = 0; t < TM; t++) {
+                        store4<OUT>(p, y, wave_row + tile * ROWS + t * 16 + 4 * q, acc[t][c]);
+                    }
+                }
+            }
+        };
         // M: tiles of 16 columns to a wavefront, one loop for each number of them (with a branch around a tile's products the compiler puts
         // their sums behind the branches, where on some ways too few cycles pass between a product and the read of its result)
         const auto steps = [&](auto columns) {
-            constexpr int M = decltype(columns)::value, BM = (M * WC * 16 * 8 + THREADS - 1) / THREADS, COPIES = A_COPIES + BM + 1; // of a step
+            constexpr int M = decltype(columns)::value, BM = (M * WC * 16 * 8 + THREADS - 1) / THREADS, COPIES = A_COPIES + BM + (SX_REGS ? M : 1); // of a step
+            float sx_next[SX_REGS ? M : 1];
             static_assert((S - 2) * COPIES < 64, "what the counter of loads can tell apart");
-            const auto copy = [&](int s) {
-                char * const to = lds + s % S * STAGE + wave * 1024;
-                const uint8_t * const wk = w_base + s * FP8_BLOCK, * const uk = up_base + s * FP8_BLOCK;
+            int v_copy = 0, s_copy = 0; // what is copied next, of all steps and of the tile's
+            int64_t tile_copy = 0;
+            const auto copy = [&] {
+                char * const to = lds + v_copy % S * STAGE + wave * 1024;
+                const int s = s_copy;
                 const int64_t k = s * FP8_BLOCK;
+                const uint8_t * const wk = w_base + tile_copy + k, * const uk = up_base + k;
                 if (cut && s == KB - 1) { // chunks behind the last column are zeros on both sides
                     const bool none = s * FP8_BLOCK + chunk * 16 >= p.K;
 #pragma unroll
@@ -586,8 +664,21 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
                     }
                 }
                 // the columns' scales, 64 to a wavefront (the same ones by several where there are fewer)
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (sx_at + s * p.xs_block),
-                                                 (__attribute__((address_space(3))) void *) (lds + s % S * STAGE + SCALES + wave * 64 % COLS * 4), 4, 0, 0);
+                if constexpr (!SX_REGS) {
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (sx_at + s * p.xs_block),
+                                                     (__attribute__((address_space(3))) void *) (lds + v_copy % S * STAGE + SCALES + wave * 64 % COLS * 4), 4, 0, 0);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < M; c++) {
+                        sx_next[c] = sxr_at[c][s * p.xs_block];
+                    }
+                }
+                v_copy++;
+                s_copy++;
+                if (TILES && s_copy == KB) {
+                    s_copy = 0;
+                    tile_copy += (int64_t) ROWS * p.K;
+                }
             };
             // 64 steps' scales of the wavefront's rows, one to a lane; waited for here: a wait at their use, in the loop, would be one for every
             // copy under way
@@ -595,42 +686,46 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
             const auto load_scales = [&](int s) {
 #pragma unroll
                 for (int m = 0; m < NM; m++) {
-                    sw[m] = scale_at(m ? p.ups : p.ws, p.scales_bf16, scale_row + min(s + lane, KB - 1));
+                    sw[m] = scale_at(m ? p.ups : p.ws, p.scales_bf16, scale_row + min(s + lane, n_steps - 1));
                     asm volatile("" : "+v"(sw[m]));
                 }
             };
-            // (before a list's next columns: nothing reads LDS any more, no store is under way)
-            if (LIST) {
-                wait_loads<0>();
-                meet();
-            }
 #pragma unroll
             for (int s = 0; s < S - 1; s++) {
-                if (s < KB) {
-                    copy(s);
+                if (s < n_steps) {
+                    copy();
                 }
             }
-            for (int s64 = 0; s64 < KB; s64 += 64) {
+            int s_tile = 0, tile = 0;
+            for (int s64 = 0; s64 < n_steps; s64 += 64) {
                 load_scales(s64);
-                const int s_end = min(s64 + 64, KB);
+                const int s_end = min(s64 + 64, n_steps);
                 for (int s = s64; s < s_end; s++) {
                     // this wavefront's copies of the step are in LDS; those of up to S - 2 later ones are under way
-                    if (S > 3 && s + 2 < KB) {
+                    if (S > 3 && s + 2 < n_steps) {
                         wait_loads<(S > 3 ? 2 : 0) * COPIES>();
-                    } else if (S > 2 && s + 1 < KB) {
+                    } else if (S > 2 && s + 1 < n_steps) {
                         wait_loads<(S > 2 ? 1 : 0) * COPIES>();
                     } else {
                         wait_loads<0>();
                     }
+                    float sx_now[M];
+                    if constexpr (SX_REGS) {
+#pragma unroll
+                        for (int c = 0; c < M; c++) {
+                            asm volatile("" : "+v"(sx_next[c]));
+                            sx_now[c] = sx_next[c];
+                        }
+                    }
                     meet(); // all of the block's are, and nothing reads the buffer of the step before any more
-                    if (s + S - 1 < KB) {
-                        copy(s + S - 1);
+                    if (v_copy < n_steps) {
+                        copy();
                     }
                     const char * const at = lds + s % S * STAGE;
                     float both[NM][M];
 #pragma unroll
                     for (int c = 0; c < M; c++) {
-                        const float sx = *(const float *) (at + SCALES + ((c * WC + wc) * 16 + m16) * 4);
+                        const float sx = SX_REGS ? sx_now[c] : *(const float *) (at + SCALES + ((c * WC + wc) * 16 + m16) * 4);
 #pragma unroll
                         for (int m = 0; m < NM; m++) {
                             both[m][c] = __uint_as_float((uint32_t) __builtin_amdgcn_readlane((int) __float_as_uint(sw[m]), s - s64)) * sx;
@@ -699,6 +794,18 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
                                 }
                             }
                         }
+                    }
+                    if (TILES && ++s_tile == KB) {
+                        store(columns, tile);
+#pragma unroll
+                        for (int t = 0; t < RT; t++) {
+#pragma unroll
+                            for (int c = 0; c < M; c++) {
+                                acc[t][c] = f32x4_t{};
+                            }
+                        }
+                        s_tile = 0;
+                        tile++;
                     }
                 }
             }
@@ -775,19 +882,8 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
                     }
                 }
             }
-        } else {
-#pragma unroll
-            for (int c = 0; c < CT; c++) {
-                const int col = (c * WC + wc) * 16 + m16;
-                if (col >= nc) {
-                    continue;
-                }
-                const int64_t y = LIST ? p.pairs[c0 + col] : c0 + col;
-#pragma unroll
-                for (int t = 0; t < TM; t++) {
-                    store4<OUT>(p, y, wave_row + t * 16 + 4 * q, acc[t][c]);
-                }
-            }
+        } else if constexpr (!TILES) {
+            store(std::integral_constant<int, CT>{}, 0);
         }
     }
 }
@@ -1093,7 +1189,7 @@ int few_pass(int64_t cols, int KB, bool glu) {
 
 template <int WR, int WC, int RT, int CT, int S, bool GLU, bool LIST, int OUT>
 void many_go(const fp8_launch * p, hipStream_t stream) { // without p: its LDS limit is raised
-    constexpr int ROWS = WR * RT * 16 / (GLU ? 2 : 1), COLS = WC * CT * 16, LDS = S * many_stage(WR * RT * 16, COLS, WR * WC * 64);
+    constexpr int ROWS = WR * RT * 16 / (GLU ? 2 : 1), COLS = WC * CT * 16, LDS = S * (LIST && GLU ? (WR * RT * 16 + COLS) * FP8_BLOCK : many_stage(WR * RT * 16, COLS, WR * WC * 64));
     static_assert((size_t) LDS <= LDS_BYTES, "fits");
     const auto kernel = k_fp8_many<WR, WC, RT, CT, S, GLU, LIST, OUT>;
     if (!p) {
@@ -1101,11 +1197,13 @@ void many_go(const fp8_launch * p, hipStream_t stream) { // without p: its LDS l
         return;
     }
     const int row_tiles = (p->nrows + ROWS - 1) / ROWS, col_tiles = (p->ncols + COLS - 1) / COLS;
-    // lists: two blocks take a long one's passes in turn (8192 tokens of 256 experts, gate and up: 537 us with one, 465 with two or four)
-    const dim3 grid = LIST ? dim3(row_tiles, (unsigned) p->n_matrices + 1, p->ncols > 96 * p->n_matrices ? 2 : 1) : dim3((unsigned) (((int64_t) row_tiles * col_tiles + 7) / 8 * 8));
+    fp8_launch q = *p;
+    q.passes = (int) (p->n_matrices + 1 + p->ncols / COLS); // at most
+    q.tiles = LIST && !GLU && p->nrows % ROWS == 0 ? 2 : 1;
+    const dim3 grid = LIST ? dim3((row_tiles + q.tiles - 1) / q.tiles, std::min(q.passes, 65535)) : dim3((unsigned) (((int64_t) row_tiles * col_tiles + 7) / 8 * 8));
     static const std::string text = text_of({WR, WC, RT, CT, S, GLU, LIST, OUT});
     note_kernel("k_fp8_many", text.c_str(), 0);
-    kernel<<<grid, WR * WC * 64, LDS, stream>>>(*p);
+    kernel<<<grid, WR * WC * 64, LDS, stream>>>(q);
 }
 
 template <int WR, int WC, int RT, int CT, int S, bool GLU, bool LIST>
@@ -1147,9 +1245,7 @@ void run_many(const fp8_launch * p, bool glu, bool list, hipStream_t stream) {
 #define MANY_ONE(WHEN, N, ...) if (!p || ((WHEN) && best == N)) { many_go<__VA_ARGS__>(p, stream); }
     int best = 0;
     if (p && list) {
-        // gate and up of 256 experts of 512 x 2048, us with 128 columns to a block / 64: 1024 tokens 137 / 154, 2048 182 / 215, 8192 538 / 670; down: 1024
-        // 75 / 68, 2048 94 / 94, 4096 152 / 167
-        best = !glu && p->ncols <= 64 * p->n_matrices ? 1 : 0;
+        best = 0;
     } else if (p && glu) { // (1408 x 2048, 300 columns 15 us with 16 columns, 18 with 32, 24 with 64, 34 with 128; 2048 x 2048, 2048 columns 70, 49, 48, 37)
         const tile_of tiles[] = {{128, 128, 2.0f, 2.05f}, {128, 64, 1.4f, 1.45f}, {128, 32, 1.1f, 0.75f}, {128, 16, 0.85f, 0.54f}};
         best = best_tile(tiles, 4, *p);
@@ -1161,9 +1257,8 @@ void run_many(const fp8_launch * p, bool glu, bool list, hipStream_t stream) {
         const tile_of tiles[] = {{128, 64, 0.88f, 0.6f}, {64, 64, 0.62f, 0.33f}};
         best = best_tile(tiles, 2, *p);
     }
-    MANY(glu && list, 0, 4, 2, 4, 4, 2, true, true)
-    MANY(!glu && list, 0, 2, 2, 4, 4, 2, false, true)
-    MANY(!glu && list, 1, 2, 2, 4, 2, 2, false, true)
+    MANY(glu && list, 0, 4, 1, 4, 4, 2, true, true)
+    MANY(!glu && list, 0, 2, 2, 4, 2, 2, false, true)
     MANY(glu && !list, 0, 4, 2, 4, 4, 2, true, false)
     MANY(glu && !list, 1, 4, 2, 4, 2, 2, true, false)
     MANY(glu && !list, 2, 4, 1, 4, 2, 2, true, false)
@@ -1184,9 +1279,7 @@ constexpr int FEW_COLUMNS = 32;
 // 12 cycles of a block's CU for a block of 128 against 3 us (2576 columns of K: 19 columns 400 blocks, 32 670)
 bool converts(int KB, int64_t cols) { return KB * cols <= 512; }
 
-bool few(const bf16n_fp8_weight & w, int64_t n_cols, bool listed, bool by_ids) {
-    return by_ids || (listed ? n_cols <= 12 * (int64_t) w.n_matrices : n_cols <= FEW_COLUMNS);
-}
+bool few(int64_t n_cols, bool listed, bool by_ids) { return by_ids || (!listed && n_cols <= FEW_COLUMNS); }
 size_t aligned(size_t n) { return (n + 255) / 256 * 256; }
 size_t codes_bytes(int64_t rows, int64_t K) { return aligned(rows * K) + aligned(rows * ((K + FP8_BLOCK - 1) / FP8_BLOCK) * 4); }
 
@@ -1209,16 +1302,14 @@ void launch_add_rmsnorm_fp8(const add_norm_args & a, const bf16n_fp8_rows & y, i
     (a.ys ? (pieces <= 1024 ? k_add_rmsnorm_fp8<1, true> : k_add_rmsnorm_fp8<2, true>) : (pieces <= 1024 ? k_add_rmsnorm_fp8<1, false> : k_add_rmsnorm_fp8<2, false>))<<<n_tok, threads, 0, stream>>>(a, (uint8_t *) y.at, y.row, y.scales, y.scale_row, y.scale_block);
 }
 
-bool fp8_few_listed(const bf16n_fp8_weight & w, int64_t n_pairs) { return few(w, n_pairs, true, false); }
-
 // whether rows of activations become codes in a launch of their own
 static bool in_launch(const bf16n_fp8_weight & w, int x_kind, int64_t n_cols, bool listed, bool by_ids) {
     const int KB = (int) ((w.K + FP8_BLOCK - 1) / FP8_BLOCK);
-    return x_kind != CODES && !(few(w, n_cols, listed, by_ids) && converts(KB, by_ids ? 1 : listed ? std::min<int64_t>(n_cols, 16) : n_cols));
+    return x_kind != CODES && !(few(n_cols, listed, by_ids) && converts(KB, by_ids ? 1 : n_cols));
 }
 
 uint64_t fp8_workspace_bytes(const bf16n_fp8_weight & w, bool glu, int x_kind, int y_kind, int64_t x_rows, int64_t n_cols, bool listed, bool by_ids) {
-    const bool f = few(w, n_cols, listed, by_ids);
+    const bool f = few(n_cols, listed, by_ids);
     uint64_t n = 0;
     if (in_launch(w, x_kind, n_cols, listed, by_ids)) {
         n += codes_bytes(x_rows, w.K);
@@ -1231,7 +1322,7 @@ uint64_t fp8_workspace_bytes(const bf16n_fp8_weight & w, bool glu, int x_kind, i
 
 void launch_fp8_product(const fp8_product & a, void * workspace, int cus, hipStream_t stream) {
     const bool glu = a.up != nullptr, listed = a.pairs != nullptr, by_ids = a.ids != nullptr;
-    const bool f = few(*a.w, a.n_cols, listed, by_ids);
+    const bool f = few(a.n_cols, listed, by_ids);
     fp8_launch p = launch_of(a, cus);
     char * ws = (char *) workspace;
     if (in_launch(*a.w, p.x_kind, a.n_cols, listed, by_ids)) {
@@ -1251,8 +1342,6 @@ void launch_fp8_product(const fp8_product & a, void * workspace, int cus, hipStr
     }
     if (by_ids) {
         run_few(p, glu, 1, a.n_cols, (int) a.n_cols, cus, stream);
-    } else if (listed) {
-        run_few(p, glu, few_pass(std::min<int64_t>(a.n_cols, 16), p.KB, glu), std::min<int64_t>(a.n_cols, p.n_matrices), (int) p.n_matrices + 1, cus, stream);
     } else {
         const int pass = few_pass(a.n_cols, p.KB, glu), passes = (int) ((a.n_cols + pass - 1) / pass);
         run_few(p, glu, pass, passes, passes, cus, stream);

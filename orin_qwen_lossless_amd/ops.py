@@ -1185,6 +1185,7 @@ def int4_moe_experts(x: torch.Tensor, gate: Int4Weight, up: Int4Weight, down: In
 # ---------------------------------------------------------------- 8-bit floating point with a scale for every block of 128
 
 FP8_BLOCK, FP8_LARGEST, FP8_SMALLEST, FP8_MAX_K = 128, 448.0, 2.0 ** -100, 32768
+FP8_SINGLE_PAIRS = 64  # as many (token, slot) pairs are products by themselves; more, or more than there are experts, are listed by expert
 _E4M3 = torch.float8_e4m3fn
 _FP8_KINDS = {_E4M3: 0, torch.bfloat16: 1, torch.float32: 2}  # include/bf16n_c.h
 
@@ -1500,7 +1501,7 @@ def fp8_moe_mm_ids(x: torch.Tensor | Fp8Rows, topk_ids: torch.Tensor, w: Fp8Weig
     y, cy = _fp8_out(n, N, out_dtype, dev)
     if n and N:
         pairs = bounds = None
-        if n > n_experts or routes is not None:
+        if n > min(n_experts, FP8_SINGLE_PAIRS) or routes is not None:
             pairs, bounds = routes if routes is not None else int4_route(topk_ids, n_experts)
             if not (pairs.dtype is bounds.dtype is torch.int32 and pairs.numel() == n and bounds.numel() == n_experts + 2
                     and pairs.is_contiguous() and bounds.is_contiguous() and pairs.device == dev and bounds.device == dev):
@@ -1555,7 +1556,7 @@ def fp8_moe_experts_rows(x: torch.Tensor | Fp8Rows, gate: Fp8Weight, up: Fp8Weig
 
 def fp8_moe_experts(x: torch.Tensor | Fp8Rows, gate: Fp8Weight, up: Fp8Weight, down: Fp8Weight, topk_weights: torch.Tensor,
                     topk_ids: torch.Tensor, n_experts: int) -> torch.Tensor:
-    """Routed experts of one MoE layer in 8 bits, BF16 out (moe_experts).  Where the pairs are more than the experts the slots' results
+    """Routed experts of one MoE layer in 8 bits, BF16 out (moe_experts).  Where the pairs are more than 64, or than the experts, the slots' results
     are held in BF16 before their weighted sum in FP32 (half a step, 2^-9 of a slot's result, beside the 2^-4 of the codes)."""
     if topk_weights is None:
         raise ValueError("bf16n.fp8_moe_experts: topk_weights must be contiguous f32/bf16 [tokens, n_used]")
