@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
     const int a_frag = wr * RT * 16 * FP8_BLOCK, b_frag = A_ROWS * FP8_BLOCK + wc * 16 * FP8_BLOCK;
 
     // Lists: the passes of all matrices in a row, COLS columns each; a block takes the passes blockIdx.y, + gridDim.y ..
-    for (int pass = blockIdx.y; pass < (LIST ? p.passes : 1); pass += gridDim.y) {
+    for (int pass = LIST ? blockIdx.y : 0; pass < (LIST ? p.passes : 1); pass += LIST ? gridDim.y : 1) {
         if (LIST) {
             const list_pass f = find_pass(p.bounds, (int) p.n_matrices, pass, COLS);
             if (f.matrix < 0) {
@@ -966,16 +966,17 @@ __global__ void __launch_bounds__(1024) k_add_rmsnorm_fp8(const add_norm_args p,
             }
             if (SLOTS) {
                 const float * row = p.ys + (tok * p.n_used) * p.n + i0;
-                for (int k0 = 0; k0 < p.n_used; k0 += 8) {
-                    f32x4_t lo[8], hi[8];
+constexpr int WAY = C == 1 ? 8 : 4; // (registers)
+                                for (int k0 = 0; k0 < p.n_used; k0 += WAY) {
+                    f32x4_t lo[WAY], hi[WAY];
 #pragma unroll
-                    for (int k = 0; k < 8; k++) { // (a slot past the last: the last row again, unused)
+                    for (int k = 0; k < WAY; k++) { // (a slot past the last: the last row again, unused)
                         const float * at = row + (int64_t) min(k0 + k, p.n_used - 1) * p.n;
                         lo[k] = *(const f32x4_t *) at;
                         hi[k] = *(const f32x4_t *) (at + 4);
                     }
 #pragma unroll
-                    for (int k = 0; k < 8; k++) {
+                    for (int k = 0; k < WAY; k++) {
                         if (k0 + k < p.n_used) {
 #pragma unroll
                             for (int e = 0; e < 8; e++) {
