@@ -48,7 +48,7 @@ __device__ __forceinline__ void store4(const fp8_launch & p, int64_t y_index, in
     char * const at = p.y + y_index * p.y_row + (int64_t) row * (KIND == BF16 ? 2 : 4);
     if (row + 4 <= p.nrows && ((uintptr_t) at & (KIND == BF16 ? 7 : 15)) == 0) {
         if (KIND == BF16) {
-            *(u32x2_t *) at = u32x2_t{f32_to_bf16_rne(v[0]) | (uint32_t) f32_to_bf16_rne(v[1]) << 16, f32_to_bf16_rne(v[2]) | (uint32_t) f32_to_bf16_rne(v[3]) << 16};
+            *(u32x2_t *) at = u32x2_t{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
         } else {
             *(f32x4_t *) at = v;
         }
@@ -58,7 +58,7 @@ __device__ __forceinline__ void store4(const fp8_launch & p, int64_t y_index, in
     for (int e = 0; e < 4; e++) {
         if (row + e < p.nrows) {
             if (KIND == BF16) {
-                ((uint16_t *) at)[e] = f32_to_bf16_rne(v[e]);
+                ((uint16_t *) at)[e] = (uint16_t) bf16_pair(v[e], 0.f);
             } else {
                 ((float *) at)[e] = v[e];
             }
@@ -921,8 +921,7 @@ __global__ void __launch_bounds__(256) k_fp8_rows(const char * x, int64_t x_row,
 }
 
 __device__ __forceinline__ u32x4_t to_bf16x8(const float (&v)[8]) {
-    return u32x4_t{f32_to_bf16_rne(v[0]) | (uint32_t) f32_to_bf16_rne(v[1]) << 16, f32_to_bf16_rne(v[2]) | (uint32_t) f32_to_bf16_rne(v[3]) << 16,
-                   f32_to_bf16_rne(v[4]) | (uint32_t) f32_to_bf16_rne(v[5]) << 16, f32_to_bf16_rne(v[6]) | (uint32_t) f32_to_bf16_rne(v[7]) << 16};
+    return u32x4_t{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7])};
 }
 
 // The glue of a decode step (bf16n_add_rmsnorm) with its norm in 8 bits: a block to a token, C pieces of eight elements to a thread, 16 threads to
@@ -1055,9 +1054,17 @@ __global__ void __launch_bounds__(256) k_fp8_combine(const uint16_t * ys, const 
             acc[e] = fmaf(wk, v[e], acc[e]);
         }
     }
+    char * const at = y + (t * n + i) * (y_bf16 ? 2 : 4);
+    if ((uintptr_t) at & 15) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        store_y(y + t * n * (y_bf16 ? 2 : 4), y_bf16, i + e, acc[e]);
+        for (int e = 0; e < 8; e++) {
+            store_y(at, y_bf16, e, acc[e]);
+        }
+    } else if (y_bf16) {
+        *(u32x4_t *) at = to_bf16x8(acc);
+    } else {
+        *(f32x4_t *) at = f32x4_t{acc[0], acc[1], acc[2], acc[3]};
+        *(f32x4_t *) (at + 16) = f32x4_t{acc[4], acc[5], acc[6], acc[7]};
     }
 }
 
