@@ -1254,16 +1254,16 @@ void run_many(const fp8_launch * p, bool glu, bool list, hipStream_t stream) {
     int best = 0;
     if (p && list) {
         best = 0;
-    } else if (p && glu) { // (1408 x 2048, 300 columns 15 us with 16 columns, 18 with 32, 24 with 64, 34 with 128; 2048 x 2048, 2048 columns 70, 49, 48, 37)
+    } else if (p && glu) { // (codes, us in this order: 1408 x 2048, 300 columns 34, 23, 17, 15; 2048 x 2048, 2048 columns 39, 47, 47, 67)
         const tile_of tiles[] = {{128, 128, 2.0f, 2.05f}, {128, 64, 1.4f, 1.45f}, {128, 32, 1.1f, 0.75f}, {128, 16, 0.85f, 0.54f}};
         best = best_tile(tiles, 4, *p);
     } else if (p && kind == BF16) {
-        // (5120 x 2048, us in this order: 128 columns 33, 17, 12, 8.6; 1024: 38, 22.7, 21.8, 22.6; 2048: 40, 38, 33, 42; 8192 x 2048, 8192: 157, 176, 198, 244)
+        // (5120 x 2048, us in this order: 128 columns 33, 16, 11, 9.1; 1024: 39, 23, 21, 22; 2048: 40, 36, 32, 41; 8192 x 2048, 8192: 152, 171, 189, 235)
         const tile_of tiles[] = {{256, 256, 2.0f, 2.0f}, {128, 128, 0.95f, 0.685f}, {128, 64, 0.62f, 0.387f}, {64, 64, 0.45f, 0.238f}};
         best = best_tile(tiles, 4, *p);
-    } else if (p) { // (5120 x 2048: 64 columns 15 us, 10.7; 2048: 50, 54)
-        const tile_of tiles[] = {{128, 64, 0.88f, 0.6f}, {64, 64, 0.62f, 0.33f}};
-        best = best_tile(tiles, 2, *p);
+    } else if (p) { // (5120 x 2048, us in this order: 64 columns 29, 15, 10.5; 2048: 65, 50, 56; 8192 x 2048, 8192: 264, 293, 336)
+        const tile_of tiles[] = {{256, 128, 2.0f, 2.05f}, {128, 64, 0.88f, 0.6f}, {64, 64, 0.62f, 0.33f}};
+        best = best_tile(tiles, 3, *p);
     }
     MANY(glu && list, 0, 4, 1, 4, 4, 2, true, true)
     MANY(!glu && list, 0, 2, 2, 4, 2, 2, false, true)
@@ -1275,8 +1275,9 @@ void run_many(const fp8_launch * p, bool glu, bool list, hipStream_t stream) {
     MANY_ONE(!glu && !list && kind == BF16, 1, 2, 2, 4, 4, 2, false, false, BF16)
     MANY_ONE(!glu && !list && kind == BF16, 2, 2, 2, 4, 2, 2, false, false, BF16)
     MANY_ONE(!glu && !list && kind == BF16, 3, 2, 2, 2, 2, 3, false, false, BF16)
-    MANY_ONE(!glu && !list && kind == F32, 0, 2, 2, 4, 2, 2, false, false, F32)
-    MANY_ONE(!glu && !list && kind == F32, 1, 2, 2, 2, 2, 2, false, false, F32)
+    MANY_ONE(!glu && !list && kind == F32, 0, 4, 2, 4, 4, 2, false, false, F32)
+    MANY_ONE(!glu && !list && kind == F32, 1, 2, 2, 4, 2, 2, false, false, F32)
+    MANY_ONE(!glu && !list && kind == F32, 2, 2, 2, 2, 2, 2, false, false, F32)
 #undef MANY
 #undef MANY_ONE
 }
