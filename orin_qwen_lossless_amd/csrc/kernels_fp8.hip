@@ -29,7 +29,7 @@ struct fp8_launch {
     uint32_t per_token, one_per;            // the activation row of a pair is pair / per_token; 2^32 / per_token, rounded down
     const char * ids; int64_t ids_s0, ids_s1; bool ids_i64; int n_used; // one matrix per pair
     const int32_t * pairs, * bounds;        // pairs sorted by matrix
-    int ksplit, lds_cols, cus, passes, tiles;
+    int ksplit, lds_cols, cus, tiles;
     uint32_t one_block;                     // 2^32 / KB, rounded up: exact for the items of a pass (below 2^32 / KB)
 };
 
@@ -477,6 +477,8 @@ __device__ __forceinline__ int wave_scan(int v) {
     return dpp_below<0x143, 0xc>(v);
 }
 
+constexpr int LIST_GROUP = 4;
+
 // The columns of pass `pass` of all lists, `cols` to a pass: every wavefront looks for itself, eight lists to a lane, 512 at a time.  matrix: -1 if
 // there are fewer passes.
 struct list_pass { int matrix, begin, end; };
@@ -523,10 +525,10 @@ __device__ __forceinline__ list_pass find_pass(const int32_t * bounds, int n_mat
 // on the codes.  FP32 ones are summed from BF16 operands (fp8_sum16), and so are those that become codes with a scale, which a value
 // 1.5e-5 off would put on the other side of a border now and then (0.0015 of the norm of 300 rows of 1408 that are 0.0003 off so).
 // OUT codes: the results of ROWS = 128 rows leave as codes with a scale.
-// Lists: a block to 64 columns of one matrix (every pass a block of its own: where one block took a list's passes in turn, and a CU had one such block
-// with 128 columns, gate and up of 2048 tokens of 256 experts of 512 x 2048 took 190 us for 152, of 512 tokens 128 for 111).  Gate and up: the scales of
-// the columns in registers, so that two blocks' stages are the whole of a CU's LDS.  Down, whose K is short: two row tiles to a block, the second's
-// copies under the first's last products (2048 tokens, one / two / four: 98, 93, 102).
+// Lists: a block to 64 columns of one matrix, every pass a block of its own.  Gate and up: the scales of the columns in registers, so that two blocks'
+// stages are the whole of a CU's LDS (one block with 128 columns that took a list's passes in turn: 2048 tokens of 256 experts of 512 x 2048 190 us,
+// 512 tokens 128; now 145 and 104).  Down, whose K is short: two row tiles to a block, the second's copies under the first's last products (2048 tokens,
+// one / two / four: 98, 93, 102).
 template <int WR, int WC, int RT, int CT, int S, bool GLU, bool LIST, int OUT>
 __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p) {
     constexpr bool WIDE = OUT != BF16, SX_REGS = LIST && GLU, TILES = LIST && !GLU;
@@ -541,8 +543,21 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave % WR, wc = wave / WR;
     int64_t matrix = 0;
-    int begin = 0, end = p.ncols, row_tile = TILES ? blockIdx.x * p.tiles : blockIdx.x;
-    if (!LIST) {
+    int begin = 0, end = p.ncols, row_tile;
+    if (LIST) {
+        // An XCD takes every eighth block: LIST_GROUP passes in a row of the same rows are one XCD's, whose L2 then has the rows of a list's
+        // later passes (gate and up of 2048 tokens of 256 experts 152 us without, 145 so; with 2, 8, 16 148, 146, 147).
+        const int row_tiles = ((p.nrows + ROWS - 1) / ROWS + p.tiles - 1) / p.tiles;
+        const int64_t id = (int64_t) blockIdx.y * gridDim.x + blockIdx.x, slot = id >> 3, item = slot / LIST_GROUP * 8 + (id & 7);
+        row_tile = (int) (item % row_tiles) * p.tiles;
+        const list_pass f = find_pass(p.bounds, (int) p.n_matrices, (int) (item / row_tiles * LIST_GROUP + slot % LIST_GROUP), COLS);
+        if (f.matrix < 0) {
+            return;
+        }
+        matrix = f.matrix;
+        begin = f.begin;
+        end = f.end;
+    } else {
         // An XCD takes every eighth block, which is made a contiguous part of the tiles here: WIDEST column tiles of one row tile
         // after the other, more of them where they are the smaller, so that what runs there at a time shares few pieces of either side
         // (gated, BF16 results, us with four everywhere: 2048 x 2048, 128 columns 13.8 for 10.9; 1408 x 2048, 600 16.4 for 15.7).
@@ -574,317 +589,304 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
     const int frag0 = m16 * FP8_BLOCK + ((q ^ (m16 & 7)) << 4), frag1 = frag0 ^ 64;
     const int a_frag = wr * RT * 16 * FP8_BLOCK, b_frag = A_ROWS * FP8_BLOCK + wc * 16 * FP8_BLOCK;
 
-    // Lists: the passes of all matrices in a row, COLS columns each; a block takes the passes blockIdx.y, + gridDim.y ..
-    for (int pass = LIST ? blockIdx.y : 0; pass < (LIST ? p.passes : 1); pass += LIST ? gridDim.y : 1) {
-        if (LIST) {
-            const list_pass f = find_pass(p.bounds, (int) p.n_matrices, pass, COLS);
-            if (f.matrix < 0) {
-                return;
-            }
-            matrix = f.matrix;
-            begin = f.begin;
-            end = f.end;
-            __syncthreads(); // nothing reads LDS any more
-            if (matrix == p.n_matrices) {
-                for (int c = begin; c < end; c++) {
-                    zero_row(p, p.pairs[c], row0, n_tiles * ROWS, threadIdx.x, THREADS);
-                }
-                continue;
-            }
+    if (LIST && matrix == p.n_matrices) {
+        for (int c = begin; c < end; c++) {
+            zero_row(p, p.pairs[c], row0, n_tiles * ROWS, threadIdx.x, THREADS);
         }
-        const uint8_t * const w_base = p.w + (matrix * p.nrows + row0) * p.K, * const up_base = p.up + (matrix * p.nrows + row0) * p.K;
-        const int64_t scale_row = (matrix * p.NB + min(wave_row, p.nrows - 1) / FP8_BLOCK) * KB;
-        const int c0 = begin, nc = end - begin;
-        const auto x_of = [&](int i) -> int64_t { return LIST ? row_of_pair(p, p.pairs[c0 + min(i, nc - 1)]) : c0 + min(i, nc - 1); };
-        const char * b_at[B_COPIES];
+        return;
+    }
+    const uint8_t * const w_base = p.w + (matrix * p.nrows + row0) * p.K, * const up_base = p.up + (matrix * p.nrows + row0) * p.K;
+    const int64_t scale_row = (matrix * p.NB + min(wave_row, p.nrows - 1) / FP8_BLOCK) * KB;
+    const int c0 = begin, nc = end - begin;
+    const auto x_of = [&](int i) -> int64_t { return LIST ? row_of_pair(p, p.pairs[c0 + min(i, nc - 1)]) : c0 + min(i, nc - 1); };
+    const char * b_at[B_COPIES];
 #pragma unroll
-        for (int i = 0; i < B_COPIES; i++) {
-            b_at[i] = p.x + x_of(i * (THREADS / 8) + (threadIdx.x >> 3)) * p.x_row + chunk * 16;
+    for (int i = 0; i < B_COPIES; i++) {
+        b_at[i] = p.x + x_of(i * (THREADS / 8) + (threadIdx.x >> 3)) * p.x_row + chunk * 16;
+    }
+    const float * const sx_at = p.xs + x_of(threadIdx.x % COLS) * p.xs_row;
+    const float * sxr_at[CT];
+    if constexpr (SX_REGS) {
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            sxr_at[c] = p.xs + x_of((c * WC + wc) * 16 + m16) * p.xs_row;
         }
-        const float * const sx_at = p.xs + x_of(threadIdx.x % COLS) * p.xs_row;
-        const float * sxr_at[CT];
-        if constexpr (SX_REGS) {
+    }
+    f32x4_t acc[RT][CT] = {};
+    const auto store = [&](auto columns, int tile) {
+        if constexpr (OUT != CODES) {
 #pragma unroll
-            for (int c = 0; c < CT; c++) {
-                sxr_at[c] = p.xs + x_of((c * WC + wc) * 16 + m16) * p.xs_row;
-            }
-        }
-        f32x4_t acc[RT][CT] = {};
-        const auto store = [&](auto columns, int tile) {
-            if constexpr (OUT != CODES) {
-#pragma unroll
-                for (int c = 0; c < decltype(columns)::value; c++) {
-                    const int col = (c * WC + wc) * 16 + m16;
-                    if (col >= nc) {
-                        continue;
-                    }
-                    const int64_t y = LIST ? p.pairs[c0 + col] : c0 + col;
-#pragma unroll
-                    for (int t = 0; t < TM; t++) {
-                        store4<OUT>(p, y, wave_row + tile * ROWS + t * 16 + 4 * q, acc[t][c]);
-                    }
-                }
-            }
-        };
-        // M: tiles of 16 columns to a wavefront, one loop for each number of them (with a branch around a tile's products the compiler puts
-        // their sums behind the branches, where on some ways too few cycles pass between a product and the read of its result)
-        const auto steps = [&](auto columns) {
-            constexpr int M = decltype(columns)::value, BM = (M * WC * 16 * 8 + THREADS - 1) / THREADS, COPIES = A_COPIES + BM + (SX_REGS ? M : 1); // of a step
-            float sx_next[SX_REGS ? M : 1];
-            static_assert((S - 2) * COPIES < 64, "what the counter of loads can tell apart");
-            int v_copy = 0, s_copy = 0; // what is copied next, of all steps and of the tile's
-            int64_t tile_copy = 0;
-            const auto copy = [&] {
-                char * const to = lds + v_copy % S * STAGE + wave * 1024;
-                const int s = s_copy;
-                const int64_t k = s * FP8_BLOCK;
-                const uint8_t * const wk = w_base + tile_copy + k, * const uk = up_base + k;
-                if (cut && s == KB - 1) { // chunks behind the last column are zeros on both sides
-                    const bool none = s * FP8_BLOCK + chunk * 16 >= p.K;
-#pragma unroll
-                    for (int i = 0; i < A_COPIES; i++) {
-                        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (none ? (const uint8_t *) g_zeros : (of_up(i) ? uk : wk) + a_off[i]),
-                                                         (__attribute__((address_space(3))) void *) (to + i * THREADS * 16), 16, 0, 0);
-                    }
-#pragma unroll
-                    for (int i = 0; i < BM; i++) {
-                        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (none ? (const char *) g_zeros : b_at[i] + k),
-                                                         (__attribute__((address_space(3))) void *) (to + A_ROWS * FP8_BLOCK + i * THREADS * 16), 16, 0, 0);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < A_COPIES; i++) {
-                        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) ((of_up(i) ? uk : wk) + a_off[i]),
-                                                         (__attribute__((address_space(3))) void *) (to + i * THREADS * 16), 16, 0, 0);
-                    }
-#pragma unroll
-                    for (int i = 0; i < BM; i++) {
-                        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (b_at[i] + k),
-                                                         (__attribute__((address_space(3))) void *) (to + A_ROWS * FP8_BLOCK + i * THREADS * 16), 16, 0, 0);
-                    }
-                }
-                // the columns' scales, 64 to a wavefront (the same ones by several where there are fewer)
-                if constexpr (!SX_REGS) {
-                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (sx_at + s * p.xs_block),
-                                                     (__attribute__((address_space(3))) void *) (lds + v_copy % S * STAGE + SCALES + wave * 64 % COLS * 4), 4, 0, 0);
-                } else {
-#pragma unroll
-                    for (int c = 0; c < M; c++) {
-                        sx_next[c] = sxr_at[c][s * p.xs_block];
-                    }
-                }
-                v_copy++;
-                s_copy++;
-                if (TILES && s_copy == KB) {
-                    s_copy = 0;
-                    tile_copy += (int64_t) ROWS * p.K;
-                }
-            };
-            // 64 steps' scales of the wavefront's rows, one to a lane; waited for here: a wait at their use, in the loop, would be one for every
-            // copy under way
-            float sw[NM];
-            const auto load_scales = [&](int s) {
-#pragma unroll
-                for (int m = 0; m < NM; m++) {
-                    sw[m] = scale_at(m ? p.ups : p.ws, p.scales_bf16, scale_row + min(s + lane, n_steps - 1));
-                    asm volatile("" : "+v"(sw[m]));
-                }
-            };
-#pragma unroll
-            for (int s = 0; s < S - 1; s++) {
-                if (s < n_steps) {
-                    copy();
-                }
-            }
-            int s_tile = 0, tile = 0;
-            for (int s64 = 0; s64 < n_steps; s64 += 64) {
-                load_scales(s64);
-                const int s_end = min(s64 + 64, n_steps);
-                for (int s = s64; s < s_end; s++) {
-                    // this wavefront's copies of the step are in LDS; those of up to S - 2 later ones are under way
-                    if (S > 3 && s + 2 < n_steps) {
-                        wait_loads<(S > 3 ? 2 : 0) * COPIES>();
-                    } else if (S > 2 && s + 1 < n_steps) {
-                        wait_loads<(S > 2 ? 1 : 0) * COPIES>();
-                    } else {
-                        wait_loads<0>();
-                    }
-                    float sx_now[M];
-                    if constexpr (SX_REGS) {
-#pragma unroll
-                        for (int c = 0; c < M; c++) {
-                            asm volatile("" : "+v"(sx_next[c]));
-                            sx_now[c] = sx_next[c];
-                        }
-                    }
-                    meet(); // all of the block's are, and nothing reads the buffer of the step before any more
-                    if (v_copy < n_steps) {
-                        copy();
-                    }
-                    const char * const at = lds + s % S * STAGE;
-                    float both[NM][M];
-#pragma unroll
-                    for (int c = 0; c < M; c++) {
-                        const float sx = SX_REGS ? sx_now[c] : *(const float *) (at + SCALES + ((c * WC + wc) * 16 + m16) * 4);
-#pragma unroll
-                        for (int m = 0; m < NM; m++) {
-                            both[m][c] = __uint_as_float((uint32_t) __builtin_amdgcn_readlane((int) __float_as_uint(sw[m]), s - s64)) * sx;
-                        }
-                    }
-                    u32x4_t b[M][2], a[WIDE ? RT : 2][2];
-                    fp8_wide bw[M];
-#pragma unroll
-                    for (int c = 0; c < M; c++) {
-                        b[c][0] = *(const u32x4_t *) (at + b_frag + c * WC * 16 * FP8_BLOCK + frag0);
-                        b[c][1] = *(const u32x4_t *) (at + b_frag + c * WC * 16 * FP8_BLOCK + frag1);
-                    }
-#pragma unroll
-                    for (int t = 0; t < (WIDE ? RT : 1); t++) {
-                        a[t][0] = *(const u32x4_t *) (at + a_frag + t * 16 * FP8_BLOCK + frag0);
-                        a[t][1] = *(const u32x4_t *) (at + a_frag + t * 16 * FP8_BLOCK + frag1);
-                    }
-                    if constexpr (WIDE) { // (the compiler puts every read right ahead of its use: 2048 tokens of 256 experts 196 us for 192)
-                        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                        for (int c = 0; c < M; c++) {
-                            bw[c] = fp8_widen(b[c][0], b[c][1]);
-                        }
-                    }
-                    f32x4_t part[2][M];
-#pragma unroll
-                    for (int t = 0; t <= RT; t++) {
-                        fp8_wide aw;
-                        if (t < RT) {
-                            if (!WIDE && t + 1 < RT) {
-                                a[(t + 1) & 1][0] = *(const u32x4_t *) (at + a_frag + (t + 1) * 16 * FP8_BLOCK + frag0);
-                                a[(t + 1) & 1][1] = *(const u32x4_t *) (at + a_frag + (t + 1) * 16 * FP8_BLOCK + frag1);
-                            }
-                            if constexpr (WIDE) {
-                                aw = fp8_widen(a[t][0], a[t][1]);
-                            }
-                        }
-#pragma unroll
-                        for (int c = 0; c < M; c++) {
-                            if (t < RT) {
-                                if constexpr (WIDE) {
-                                    part[t & 1][c] = fp8_sum16(aw, bw[c]);
-                                } else {
-                                    part[t & 1][c] = fp8_sum8(a[t & 1][0], a[t & 1][1], b[c][0], b[c][1]);
-                                }
-                            }
-                            if (t > 0) {
-#pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    acc[t - 1][c][e] = fmaf(part[(t - 1) & 1][c][e], both[(t - 1) / TM][c], acc[t - 1][c][e]);
-                                }
-                            }
-                        }
-                    }
-                    if constexpr (!WIDE) { // in this order: a product, the additions of one a row of tiles before
-#pragma unroll
-                        for (int t = 0; t < RT; t++) {
-#pragma unroll
-                            for (int c = 0; c < M; c++) {
-                                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                                if (t > 0) {
-                                    __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
-                                }
-                                if (c == 0 && t + 1 < RT) {
-                                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-                                }
-                            }
-                        }
-                    }
-                    if (TILES && ++s_tile == KB) {
-                        store(columns, tile);
-#pragma unroll
-                        for (int t = 0; t < RT; t++) {
-#pragma unroll
-                            for (int c = 0; c < M; c++) {
-                                acc[t][c] = f32x4_t{};
-                            }
-                        }
-                        s_tile = 0;
-                        tile++;
-                    }
-                }
-            }
-        };
-        if constexpr (LIST) { // (the lowest number that has them all: one for the block)
-            const int tiles = ((nc + 15) / 16 + WC - 1) / WC;
-            static_assert(CT == 4 || CT == 2, "one loop each");
-            if constexpr (CT == 4) {
-                tiles == 1 ? steps(std::integral_constant<int, 1>{}) : tiles == 2 ? steps(std::integral_constant<int, 2>{})
-                : tiles == 3 ? steps(std::integral_constant<int, 3>{}) : steps(std::integral_constant<int, 4>{});
-            } else {
-                tiles == 1 ? steps(std::integral_constant<int, 1>{}) : steps(std::integral_constant<int, 2>{});
-            }
-        } else {
-            steps(std::integral_constant<int, CT>{});
-        }
-        if (GLU) {
-#pragma unroll
-            for (int t = 0; t < TM; t++) {
-#pragma unroll
-                for (int c = 0; c < CT; c++) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        acc[t][c][e] = gated(acc[t][c][e], acc[RT - TM + t][c][e]);
-                    }
-                }
-            }
-        }
-        if constexpr (OUT == CODES) {
-            float * const most = (float *) lds; // [WR][COLS]
-            float mine[CT];
-#pragma unroll
-            for (int c = 0; c < CT; c++) {
-                float v = 0.f;
-#pragma unroll
-                for (int t = 0; t < TM; t++) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        v = fmaxf(v, wave_row + t * 16 + 4 * q + e < p.nrows ? fabsf(acc[t][c][e]) : 0.f);
-                    }
-                }
-                v = fmaxf(v, __shfl_xor(v, 16, 64));
-                mine[c] = fmaxf(v, __shfl_xor(v, 32, 64));
-            }
-            __syncthreads();
-            if (q == 0) {
-#pragma unroll
-                for (int c = 0; c < CT; c++) {
-                    most[wr * COLS + (c * WC + wc) * 16 + m16] = mine[c];
-                }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int c = 0; c < CT; c++) {
+            for (int c = 0; c < decltype(columns)::value; c++) {
                 const int col = (c * WC + wc) * 16 + m16;
                 if (col >= nc) {
                     continue;
                 }
-                float v = most[col];
-#pragma unroll
-                for (int i = 1; i < WR; i++) {
-                    v = fmaxf(v, most[i * COLS + col]);
-                }
-                const fp8_scales s = fp8_scales_of(v);
                 const int64_t y = LIST ? p.pairs[c0 + col] : c0 + col;
-                if (wr == 0 && q == 0) {
-                    p.ys[y * p.ys_row + row_tile * p.ys_block] = s.scale;
-                }
 #pragma unroll
                 for (int t = 0; t < TM; t++) {
-                    const int r = wave_row + t * 16 + 4 * q;
-                    if (r < p.nrows) { // (rows are a multiple of 16)
-                        *(uint32_t *) (p.y + y * p.y_row + r) = fp8_pack4(acc[t][c][0] * s.inverse, acc[t][c][1] * s.inverse, acc[t][c][2] * s.inverse, acc[t][c][3] * s.inverse);
-                    }
+                    store4<OUT>(p, y, wave_row + tile * ROWS + t * 16 + 4 * q, acc[t][c]);
                 }
             }
-        } else if constexpr (!TILES) {
-            store(std::integral_constant<int, CT>{}, 0);
         }
+    };
+    // M: tiles of 16 columns to a wavefront, one loop for each number of them (with a branch around a tile's products the compiler puts
+    // their sums behind the branches, where on some ways too few cycles pass between a product and the read of its result)
+    const auto steps = [&](auto columns) {
+        constexpr int M = decltype(columns)::value, BM = (M * WC * 16 * 8 + THREADS - 1) / THREADS, COPIES = A_COPIES + BM + (SX_REGS ? M : 1); // of a step
+        float sx_next[SX_REGS ? M : 1];
+        static_assert((S - 2) * COPIES < 64, "what the counter of loads can tell apart");
+        int v_copy = 0, s_copy = 0; // what is copied next, of all steps and of the tile's
+        int64_t tile_copy = 0;
+        const auto copy = [&] {
+            char * const to = lds + v_copy % S * STAGE + wave * 1024;
+            const int s = s_copy;
+            const int64_t k = s * FP8_BLOCK;
+            const uint8_t * const wk = w_base + tile_copy + k, * const uk = up_base + k;
+            if (cut && s == KB - 1) { // chunks behind the last column are zeros on both sides
+                const bool none = s * FP8_BLOCK + chunk * 16 >= p.K;
+#pragma unroll
+                for (int i = 0; i < A_COPIES; i++) {
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (none ? (const uint8_t *) g_zeros : (of_up(i) ? uk : wk) + a_off[i]),
+                                                     (__attribute__((address_space(3))) void *) (to + i * THREADS * 16), 16, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < BM; i++) {
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (none ? (const char *) g_zeros : b_at[i] + k),
+                                                     (__attribute__((address_space(3))) void *) (to + A_ROWS * FP8_BLOCK + i * THREADS * 16), 16, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < A_COPIES; i++) {
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) ((of_up(i) ? uk : wk) + a_off[i]),
+                                                     (__attribute__((address_space(3))) void *) (to + i * THREADS * 16), 16, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < BM; i++) {
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (b_at[i] + k),
+                                                     (__attribute__((address_space(3))) void *) (to + A_ROWS * FP8_BLOCK + i * THREADS * 16), 16, 0, 0);
+                }
+            }
+            // the columns' scales, 64 to a wavefront (the same ones by several where there are fewer)
+            if constexpr (!SX_REGS) {
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *) (sx_at + s * p.xs_block),
+                                                 (__attribute__((address_space(3))) void *) (lds + v_copy % S * STAGE + SCALES + wave * 64 % COLS * 4), 4, 0, 0);
+            } else {
+#pragma unroll
+                for (int c = 0; c < M; c++) {
+                    sx_next[c] = sxr_at[c][s * p.xs_block];
+                }
+            }
+            v_copy++;
+            s_copy++;
+            if (TILES && s_copy == KB) {
+                s_copy = 0;
+                tile_copy += (int64_t) ROWS * p.K;
+            }
+        };
+        // 64 steps' scales of the wavefront's rows, one to a lane; waited for here: a wait at their use, in the loop, would be one for every
+        // copy under way
+        float sw[NM];
+        const auto load_scales = [&](int s) {
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                sw[m] = scale_at(m ? p.ups : p.ws, p.scales_bf16, scale_row + min(s + lane, n_steps - 1));
+                asm volatile("" : "+v"(sw[m]));
+            }
+        };
+#pragma unroll
+        for (int s = 0; s < S - 1; s++) {
+            if (s < n_steps) {
+                copy();
+            }
+        }
+        int s_tile = 0, tile = 0;
+        for (int s64 = 0; s64 < n_steps; s64 += 64) {
+            load_scales(s64);
+            const int s_end = min(s64 + 64, n_steps);
+            for (int s = s64; s < s_end; s++) {
+                // this wavefront's copies of the step are in LDS; those of up to S - 2 later ones are under way
+                if (S > 3 && s + 2 < n_steps) {
+                    wait_loads<(S > 3 ? 2 : 0) * COPIES>();
+                } else if (S > 2 && s + 1 < n_steps) {
+                    wait_loads<(S > 2 ? 1 : 0) * COPIES>();
+                } else {
+                    wait_loads<0>();
+                }
+                float sx_now[M];
+                if constexpr (SX_REGS) {
+#pragma unroll
+                    for (int c = 0; c < M; c++) {
+                        asm volatile("" : "+v"(sx_next[c]));
+                        sx_now[c] = sx_next[c];
+                    }
+                }
+                meet(); // all of the block's are, and nothing reads the buffer of the step before any more
+                if (v_copy < n_steps) {
+                    copy();
+                }
+                const char * const at = lds + s % S * STAGE;
+                float both[NM][M];
+#pragma unroll
+                for (int c = 0; c < M; c++) {
+                    const float sx = SX_REGS ? sx_now[c] : *(const float *) (at + SCALES + ((c * WC + wc) * 16 + m16) * 4);
+#pragma unroll
+                    for (int m = 0; m < NM; m++) {
+                        both[m][c] = __uint_as_float((uint32_t) __builtin_amdgcn_readlane((int) __float_as_uint(sw[m]), s - s64)) * sx;
+                    }
+                }
+                u32x4_t b[M][2], a[WIDE ? RT : 2][2];
+                fp8_wide bw[M];
+#pragma unroll
+                for (int c = 0; c < M; c++) {
+                    b[c][0] = *(const u32x4_t *) (at + b_frag + c * WC * 16 * FP8_BLOCK + frag0);
+                    b[c][1] = *(const u32x4_t *) (at + b_frag + c * WC * 16 * FP8_BLOCK + frag1);
+                }
+#pragma unroll
+                for (int t = 0; t < (WIDE ? RT : 1); t++) {
+                    a[t][0] = *(const u32x4_t *) (at + a_frag + t * 16 * FP8_BLOCK + frag0);
+                    a[t][1] = *(const u32x4_t *) (at + a_frag + t * 16 * FP8_BLOCK + frag1);
+                }
+                if constexpr (WIDE) { // (the compiler puts every read right ahead of its use: 2048 tokens of 256 experts 196 us for 192)
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int c = 0; c < M; c++) {
+                        bw[c] = fp8_widen(b[c][0], b[c][1]);
+                    }
+                }
+                f32x4_t part[2][M];
+#pragma unroll
+                for (int t = 0; t <= RT; t++) {
+                    fp8_wide aw;
+                    if (t < RT) {
+                        if (!WIDE && t + 1 < RT) {
+                            a[(t + 1) & 1][0] = *(const u32x4_t *) (at + a_frag + (t + 1) * 16 * FP8_BLOCK + frag0);
+                            a[(t + 1) & 1][1] = *(const u32x4_t *) (at + a_frag + (t + 1) * 16 * FP8_BLOCK + frag1);
+                        }
+                        if constexpr (WIDE) {
+                            aw = fp8_widen(a[t][0], a[t][1]);
+                        }
+                    }
+#pragma unroll
+                    for (int c = 0; c < M; c++) {
+                        if (t < RT) {
+                            if constexpr (WIDE) {
+                                part[t & 1][c] = fp8_sum16(aw, bw[c]);
+                            } else {
+                                part[t & 1][c] = fp8_sum8(a[t & 1][0], a[t & 1][1], b[c][0], b[c][1]);
+                            }
+                        }
+                        if (t > 0) {
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                acc[t - 1][c][e] = fmaf(part[(t - 1) & 1][c][e], both[(t - 1) / TM][c], acc[t - 1][c][e]);
+                            }
+                        }
+                    }
+                }
+                if constexpr (!WIDE) { // in this order: a product, the additions of one a row of tiles before
+#pragma unroll
+                    for (int t = 0; t < RT; t++) {
+#pragma unroll
+                        for (int c = 0; c < M; c++) {
+                            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                            if (t > 0) {
+                                __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+                            }
+                            if (c == 0 && t + 1 < RT) {
+                                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                            }
+                        }
+                    }
+                }
+                if (TILES && ++s_tile == KB) {
+                    store(columns, tile);
+#pragma unroll
+                    for (int t = 0; t < RT; t++) {
+#pragma unroll
+                        for (int c = 0; c < M; c++) {
+                            acc[t][c] = f32x4_t{};
+                        }
+                    }
+                    s_tile = 0;
+                    tile++;
+                }
+            }
+        }
+    };
+    if constexpr (LIST) { // (the lowest number that has them all: one for the block)
+        const int tiles = ((nc + 15) / 16 + WC - 1) / WC;
+        static_assert(CT == 4 || CT == 2, "one loop each");
+        if constexpr (CT == 4) {
+            tiles == 1 ? steps(std::integral_constant<int, 1>{}) : tiles == 2 ? steps(std::integral_constant<int, 2>{})
+            : tiles == 3 ? steps(std::integral_constant<int, 3>{}) : steps(std::integral_constant<int, 4>{});
+        } else {
+            tiles == 1 ? steps(std::integral_constant<int, 1>{}) : steps(std::integral_constant<int, 2>{});
+        }
+    } else {
+        steps(std::integral_constant<int, CT>{});
+    }
+    if (GLU) {
+#pragma unroll
+        for (int t = 0; t < TM; t++) {
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    acc[t][c][e] = gated(acc[t][c][e], acc[RT - TM + t][c][e]);
+                }
+            }
+        }
+    }
+    if constexpr (OUT == CODES) {
+        float * const most = (float *) lds; // [WR][COLS]
+        float mine[CT];
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            float v = 0.f;
+#pragma unroll
+            for (int t = 0; t < TM; t++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    v = fmaxf(v, wave_row + t * 16 + 4 * q + e < p.nrows ? fabsf(acc[t][c][e]) : 0.f);
+                }
+            }
+            v = fmaxf(v, __shfl_xor(v, 16, 64));
+            mine[c] = fmaxf(v, __shfl_xor(v, 32, 64));
+        }
+        __syncthreads();
+        if (q == 0) {
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                most[wr * COLS + (c * WC + wc) * 16 + m16] = mine[c];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            const int col = (c * WC + wc) * 16 + m16;
+            if (col >= nc) {
+                continue;
+            }
+            float v = most[col];
+#pragma unroll
+            for (int i = 1; i < WR; i++) {
+                v = fmaxf(v, most[i * COLS + col]);
+            }
+            const fp8_scales s = fp8_scales_of(v);
+            const int64_t y = LIST ? p.pairs[c0 + col] : c0 + col;
+            if (wr == 0 && q == 0) {
+                p.ys[y * p.ys_row + row_tile * p.ys_block] = s.scale;
+            }
+#pragma unroll
+            for (int t = 0; t < TM; t++) {
+                const int r = wave_row + t * 16 + 4 * q;
+                if (r < p.nrows) { // (rows are a multiple of 16)
+                    *(uint32_t *) (p.y + y * p.y_row + r) = fp8_pack4(acc[t][c][0] * s.inverse, acc[t][c][1] * s.inverse, acc[t][c][2] * s.inverse, acc[t][c][3] * s.inverse);
+                }
+            }
+        }
+    } else if constexpr (!TILES) {
+        store(std::integral_constant<int, CT>{}, 0);
     }
 }
 
@@ -1206,9 +1208,14 @@ void many_go(const fp8_launch * p, hipStream_t stream) { // without p: its LDS l
     }
     const int row_tiles = (p->nrows + ROWS - 1) / ROWS, col_tiles = (p->ncols + COLS - 1) / COLS;
     fp8_launch q = *p;
-    q.passes = (int) (p->n_matrices + 1 + p->ncols / COLS); // at most
     q.tiles = LIST && !GLU && p->nrows % ROWS == 0 ? 2 : 1;
-    const dim3 grid = LIST ? dim3((row_tiles + q.tiles - 1) / q.tiles, std::min(q.passes, 65535)) : dim3((unsigned) (((int64_t) row_tiles * col_tiles + 7) / 8 * 8));
+    dim3 grid((unsigned) (((int64_t) row_tiles * col_tiles + 7) / 8 * 8));
+    if (LIST) {
+        const int64_t passes = p->n_matrices + 1 + p->ncols / COLS; // at most
+        const int64_t items = (passes + LIST_GROUP - 1) / LIST_GROUP * ((row_tiles + q.tiles - 1) / q.tiles), blocks = (items + 7) / 8 * 8 * LIST_GROUP;
+        grid.x = (unsigned) std::min<int64_t>(blocks, 1 << 20);
+        grid.y = (unsigned) ((blocks + grid.x - 1) / grid.x);
+    }
     static const std::string text = text_of({WR, WC, RT, CT, S, GLU, LIST, OUT});
     note_kernel("k_fp8_many", text.c_str(), 0);
     kernel<<<grid, WR * WC * 64, LDS, stream>>>(q);
