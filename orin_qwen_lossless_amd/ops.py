@@ -1356,8 +1356,8 @@ def fp8_quantize_rows(x: torch.Tensor) -> Fp8Rows:
 def add_rmsnorm_fp8(a: torch.Tensor, b: torch.Tensor | None = None, c: torch.Tensor | None = None, ys: torch.Tensor | None = None,
                     topk_weights: torch.Tensor | None = None, gamma: torch.Tensor | None = None, eps: float = 1e-6,
                     want_sum: bool = False, want_norm: bool = False):
-    """add_rmsnorm with the norm in 8 bits: s = a + b + c + moe_combine(ys, topk_weights) in FP32, returns Fp8Rows of
-    s * rsqrt(mean(s^2) + eps) * gamma, whose FP32 value is rounded once, to its code.  With want_sum and want_norm a tuple: the rows, bf16(s),
+    """add_rmsnorm with the norm in 8 bits: s = a + b + c + moe_combine(ys, topk_weights), returns Fp8Rows of
+    s * rsqrt(mean(s^2) + eps) * gamma, held in 64 bits up to its FP32 value, which is rounded once, to its code.  With want_sum and want_norm a tuple: the rows, bf16(s),
     the norm in BF16 (for a product that takes BF16, a router's).  a, b, c: [T, n] BF16 contiguous; ys: [T, n_used, n] FP32 with
     topk_weights [T, n_used]; gamma: [n] BF16; n a multiple of 16, at most 16384."""
     r = (_host_calls or _host()).add_rmsnorm_fp8(a, b, c, ys, topk_weights, gamma, eps, bool(want_sum), bool(want_norm))
