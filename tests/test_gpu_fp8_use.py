@@ -385,3 +385,26 @@ def test_decode_step_in_8_bits(ops, T, dense):
         assert torch.equal(out, step(h)) and out.shape == (T, 512)
     # without an output projection the step ends in the norm as BF16 numbers
     assert D.Bf16nStep(ops, sets, None, 1, T)(h).dtype is torch.bfloat16
+
+
+@pytest.mark.parametrize("T,n_used,E,N,K", [(90, 2, 3, 384, 272), (70, 3, 4, 256, 4400), (200, 1, 2, 1024, 144), (65, 2, 5, 640, 9104)])
+def test_lists_by_row_tiles(ops, T, n_used, E, N, K):
+    """Two row tiles to a block: an odd number of them, a last block of columns that is cut, more steps than a register's lanes have scales."""
+    (c, s), (cu, su) = X.matrix(N, K, 41, E, True), X.matrix(N, K, 42, E, True)
+    ids = ids_for(T, n_used, E, 43)
+    x, q, xs = give(X.rows(T, K, 44, False), "rows")
+    for out in (torch.bfloat16, torch.float32):
+        check(ops.fp8_moe_mm_ids(x, ids.cuda(), weight(ops, c, s, E), E, out_dtype=out).view(T * n_used, N), *by_pair(q, xs, c, s, ids, E, out))
+        y, dy = X.gated(*by_pair(q, xs, c, s, ids, E, out), *by_pair(q, xs, cu, su, ids, E, out))
+        check(ops.fp8_moe_mm_ids(x, ids.cuda(), weight(ops, c, s, E), E, weight(ops, cu, su, E), out).view(T * n_used, N), y, dy)
+
+
+def test_more_lists_than_a_wavefront_finds_at_once(ops):
+    """1200 matrices: lists are looked for 512 at a time."""
+    E, N, K, T = 1200, 16, 32, 700
+    c, s = X.matrix(N, K, 45, E)
+    ids = torch.randint(-1, E + 1, (T, 2), generator=torch.Generator().manual_seed(46))
+    ids[:200, 0] = E - 1
+    x, q, xs = give(X.rows(T, K, 47, False), "f32")
+    for out in (torch.bfloat16, torch.float32):
+        check(ops.fp8_moe_mm_ids(x, ids.cuda(), weight(ops, c, s, E), E, out_dtype=out).view(2 * T, N), *by_pair(q, xs, c, s, ids, E, out))
