@@ -506,16 +506,24 @@ struct fp8_y {
     at::Tensor y, scales;
     bf16n_fp8_rows r = {};
     fp8_y(int64_t rows, int64_t n, int kind, const at::TensorOptions & like) {
-        y = at::empty({rows, n}, like.dtype(kind == BF16N_FP8_CODES ? at::kFloat8_e4m3fn : kind == BF16N_FP8_BF16 ? at::kBFloat16 : at::kFloat));
-        r.at = y.data_ptr();
-        r.row = n * y.element_size();
         r.kind = kind;
-        if (kind == BF16N_FP8_CODES) {
-            scales = at::empty_strided({rows, blocks_of(n)}, {1, rows}, like.dtype(at::kFloat));
-            r.scales = (float *) scales.data_ptr();
-            r.scale_row = 1;
-            r.scale_block = rows;
+        if (kind != BF16N_FP8_CODES) {
+            y = at::empty({rows, n}, like.dtype(kind == BF16N_FP8_BF16 ? at::kBFloat16 : at::kFloat));
+            r.at = y.data_ptr();
+            r.row = n * y.element_size();
+            return;
         }
+        // codes and scales share an allocation (with one for each a norm of one token took 5.9 us, now 4.9)
+        const int64_t codes = (rows * n + 255) / 256 * 256, blocks = blocks_of(n);
+        y = at::empty({codes + rows * blocks * 4}, like.dtype(at::kFloat8_e4m3fn));
+        y.unsafeGetTensorImpl()->set_sizes_contiguous({rows, n});
+        scales = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(y.storage()), y.key_set(), caffe2::TypeMeta::Make<float>());
+        scales.unsafeGetTensorImpl()->set_sizes_and_strides(c10::IntArrayRef({rows, blocks}), c10::IntArrayRef({1, rows}), codes / 4);
+        r.at = y.data_ptr();
+        r.row = n;
+        r.scales = (float *) scales.data_ptr();
+        r.scale_row = 1;
+        r.scale_block = rows;
     }
 };
 
