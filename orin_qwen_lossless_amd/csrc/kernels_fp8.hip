@@ -94,6 +94,7 @@ constexpr int FEW_PARTS = 64; // blocks of K that a wavefront takes at most: the
 // other operand, from LDS, where the block has put their codes first (those of BF16 and FP32 rows it makes itself).  A lane's two
 // loads of a step are 16 bytes each of row lane % 16, so that four lanes have half a line and both loads a whole one; weights go
 // from memory to the operand's registers, D steps ahead, from one 16 rows on to the next.  K in ksplit parts, summed through LDS in a fixed order.
+// 248320 x 2048, one column: 98 us, 5.2 TB/s, what a copy has; 512 x 2048: 4.5, a launch and the latency of its loads.
 // ONE: 16 rows to a block and at most four steps of them to a wavefront, all loaded at once: no register is kept for the next 16 rows.
 template <int CT, bool GLU, int XKIND, int NW, bool ONE>
 __global__ void __launch_bounds__(NW * 64, ONE ? 2 : CT * (GLU ? 2 : 1) == 1 ? 4 : CT * (GLU ? 2 : 1) == 2 ? 3 : 2) k_fp8_few(const fp8_launch p) {
@@ -336,7 +337,7 @@ __global__ void __launch_bounds__(NW * 64, ONE ? 2 : CT * (GLU ? 2 : 1) == 1 ? 4
 }
 
 // The second products of a token's experts and their weighted sum in one launch, for few tokens (a launch of one token's slots and one of
-// their sum: 2048 x 512, eight slots 5.5 + 4.0 us; this 5.5): a block takes 16 rows of a token's result, a wavefront the slots wave, wave + 8 ..,
+// their sum: 2048 x 512, eight slots 5.5 + 4.0 us; this 6.4): a block takes 16 rows of a token's result, a wavefront the slots wave, wave + 8 ..,
 // and the sum is made in the order of the slots, one fmaf each (bf16n_moe_combine's).  Hidden rows: FP32, made codes by the block.
 __global__ void __launch_bounds__(512, 4) k_fp8_down(const fp8_launch p, const void * wts, bool wts_bf16) {
     constexpr int NW = 8, D = 4;
@@ -746,7 +747,7 @@ __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p
                     a[t][0] = *(const u32x4_t *) (at + a_frag + t * 16 * FP8_BLOCK + frag0);
                     a[t][1] = *(const u32x4_t *) (at + a_frag + t * 16 * FP8_BLOCK + frag1);
                 }
-                if constexpr (WIDE) { // (the compiler puts every read right ahead of its use: 2048 tokens of 256 experts 196 us for 192)
+                if constexpr (WIDE) { // (else the compiler puts every read right ahead of its use: 300 columns of 1408 x 2048, gated, 16.2 us for 15.3)
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int c = 0; c < M; c++) {
@@ -931,7 +932,7 @@ __device__ __forceinline__ u32x4_t to_bf16x8(const float (&v)[8]) {
 // in registers between the sum of its squares and its codes.  The slots' sum, the squares' and the norm are held in 64 bits and become
 // FP32 once, ahead of the scales: a code is off by a whole step, a sixteenth of its value, wherever an error of a last place carries a value over the
 // middle of two codes, which 32 bits did to one or two of 858 thousand (and were 8.9 us there for 9.6).
-// 8192 tokens of 2048: 22.9 us, 118 MB at 5.2 TB/s; one token 2.8, the chain of its loads, sum and scale.
+// 8192 tokens of 2048: 22.1 us, 118 MB at 5.3 TB/s; one token 2.7, the chain of its loads, sum and scale.
 template <int C, bool SLOTS>
 __global__ void __launch_bounds__(1024) k_add_rmsnorm_fp8(const add_norm_args p, uint8_t * y, int64_t y_row, float * s, int64_t s_row, int64_t s_block) {
     __shared__ double wave_sq[16];
@@ -1179,7 +1180,7 @@ void run_few(fp8_launch p, bool glu, int cols, int64_t busy, int y_blocks, int c
     p.lds_cols = cols;
     const int ct = cols <= 16 ? 1 : 2, rows = nw / ksplit * 16, n_blocks = (p.nrows + rows - 1) / rows;
     const size_t lds = few_lds(cols, p.KB, ct, glu, nw, ksplit);
-    if (ksplit == 8 && tiles <= 2 * cus && p.KB <= 32) { // (else 512 x 2048, one column 6.7 us for 4.5; 1453 x 2576, 19 columns 10.2 for 9.2)
+    if (ksplit == 8 && tiles <= 2 * cus && p.KB <= 32) { // (else 512 x 2048, one column 6.7 us for 4.5; 1453 x 2576, 19 columns 10.2 for 8.4)
         few_instance(&p, ct, glu, FEW_ONE, dim3(n_blocks, y_blocks), lds, stream);
         return;
     }
