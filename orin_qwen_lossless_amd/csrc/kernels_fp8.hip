@@ -94,7 +94,7 @@ constexpr int FEW_PARTS = 64; // blocks of K that a wavefront takes at most: the
 // other operand, from LDS, where the block has put their codes first (those of BF16 and FP32 rows it makes itself).  A lane's two
 // loads of a step are 16 bytes each of row lane % 16, so that four lanes have half a line and both loads a whole one; weights go
 // from memory to the operand's registers, D steps ahead, from one 16 rows on to the next.  K in ksplit parts, summed through LDS in a fixed order.
-// 248320 x 2048, one column: 98 us, 5.2 TB/s, what a copy has; 512 x 2048: 4.5, a launch and the latency of its loads.
+// 512 x 2048, one column: 4.5 us, a launch and the latency of its loads.
 // ONE: 16 rows to a block and at most four steps of them to a wavefront, all loaded at once: no register is kept for the next 16 rows.
 template <int CT, bool GLU, int XKIND, int NW, bool ONE>
 __global__ void __launch_bounds__(NW * 64, ONE ? 2 : CT * (GLU ? 2 : 1) == 1 ? 4 : CT * (GLU ? 2 : 1) == 2 ? 3 : 2) k_fp8_few(const fp8_launch p) {
@@ -1145,8 +1145,10 @@ void few_instance(const fp8_launch * p, int ct, bool glu, int shape, dim3 grid, 
         if (!p || shape == FEW_EIGHT) {
             by_kind(c, g, std::integral_constant<int, 8>{}, std::false_type{});
         }
-        if (!p || shape == FEW_FOUR) {
-            by_kind(c, g, std::integral_constant<int, 4>{}, std::false_type{});
+        if constexpr (decltype(c)::value == 1) { // (single pairs)
+            if (!p || shape == FEW_FOUR) {
+                by_kind(c, g, std::integral_constant<int, 4>{}, std::false_type{});
+            }
         }
     };
     const auto by_ct = [&](auto g) {
@@ -1168,7 +1170,7 @@ void few_instance(const fp8_launch * p, int ct, bool glu, int shape, dim3 grid, 
 // cols: columns of a pass; busy: matrices or passes that have columns; blocks: of them all, grid.y
 void run_few(fp8_launch p, bool glu, int cols, int64_t busy, int y_blocks, int cus, hipStream_t stream) {
     const int64_t tiles = (p.nrows + 15) / 16 * busy;
-    const int nw = tiles <= 4 * cus ? 8 : 4;
+    const int ct = cols <= 16 ? 1 : 2, nw = ct == 2 || tiles <= 4 * cus ? 8 : 4; // (four: single pairs, many of them)
     int ksplit = nw == 8 ? 8 : tiles <= 16 * cus ? 4 : 1;
     while (ksplit > 1 && p.KB < ksplit) {
         ksplit /= 2;
@@ -1178,7 +1180,7 @@ void run_few(fp8_launch p, bool glu, int cols, int64_t busy, int y_blocks, int c
     }
     p.ksplit = ksplit;
     p.lds_cols = cols;
-    const int ct = cols <= 16 ? 1 : 2, rows = nw / ksplit * 16, n_blocks = (p.nrows + rows - 1) / rows;
+    const int rows = nw / ksplit * 16, n_blocks = (p.nrows + rows - 1) / rows;
     const size_t lds = few_lds(cols, p.KB, ct, glu, nw, ksplit);
     if (ksplit == 8 && tiles <= 2 * cus && p.KB <= 32) { // (else 512 x 2048, one column 6.7 us for 4.5; 1453 x 2576, 19 columns 10.2 for 8.4)
         few_instance(&p, ct, glu, FEW_ONE, dim3(n_blocks, y_blocks), lds, stream);
@@ -1265,6 +1267,9 @@ void run_many(const fp8_launch * p, bool glu, bool list, hipStream_t stream) {
     } else if (p && glu) { // (codes, us in this order: 1408 x 2048, 300 columns 34, 23, 17, 15; 2048 x 2048, 2048 columns 39, 47, 47, 67)
         const tile_of tiles[] = {{128, 128, 2.0f, 2.05f}, {128, 64, 1.4f, 1.45f}, {128, 32, 1.1f, 0.75f}, {128, 16, 0.85f, 0.54f}};
         best = best_tile(tiles, 4, *p);
+    } else if (p && p->ncols <= 16) {
+        // (Us of 64 x 64 tiles, 128 x 16, 64 x 16, one column: BF16 results 20480 x 2048 11.0, 9.2, 9.9, 16384 x 8192 29, 27, 21; FP32 248320 x 2048 101, 86, 87, 16384 x 8192 43, 31, 26.)
+        best = (p->nrows + 63) / 64 <= p->cus ? 5 : 4;
     } else if (p && kind == BF16) {
         // (5120 x 2048, us in this order: 128 columns 33, 16, 11, 9.1; 1024: 39, 23, 21, 22; 2048: 40, 36, 32, 41; 8192 x 2048, 8192: 152, 171, 189, 235)
         const tile_of tiles[] = {{256, 256, 2.0f, 2.0f}, {128, 128, 0.95f, 0.685f}, {128, 64, 0.62f, 0.387f}, {64, 64, 0.45f, 0.238f}};
@@ -1283,20 +1288,35 @@ void run_many(const fp8_launch * p, bool glu, bool list, hipStream_t stream) {
     MANY_ONE(!glu && !list && kind == BF16, 1, 2, 2, 4, 4, 2, false, false, BF16)
     MANY_ONE(!glu && !list && kind == BF16, 2, 2, 2, 4, 2, 2, false, false, BF16)
     MANY_ONE(!glu && !list && kind == BF16, 3, 2, 2, 2, 2, 3, false, false, BF16)
+    MANY_ONE(!glu && !list && kind == BF16, 4, 4, 1, 2, 1, 3, false, false, BF16)
+    MANY_ONE(!glu && !list && kind == BF16, 5, 4, 1, 1, 1, 4, false, false, BF16)
     MANY_ONE(!glu && !list && kind == F32, 0, 4, 2, 4, 4, 2, false, false, F32)
     MANY_ONE(!glu && !list && kind == F32, 1, 2, 2, 4, 2, 2, false, false, F32)
     MANY_ONE(!glu && !list && kind == F32, 2, 2, 2, 2, 2, 2, false, false, F32)
+    MANY_ONE(!glu && !list && kind == F32, 4, 4, 1, 2, 1, 3, false, false, F32)
+    MANY_ONE(!glu && !list && kind == F32, 5, 4, 1, 1, 1, 4, false, false, F32)
 #undef MANY
 #undef MANY_ONE
 }
 
-constexpr int FEW_COLUMNS = 32;
 
 // Whether the blocks of the kernel for few columns turn rows that are not codes into them, each for itself, rather than a launch ahead of it:
 // 12 cycles of a block's CU for a block of 128 against 3 us (2576 columns of K: 19 columns 400 blocks, 32 670)
 bool converts(int KB, int64_t cols) { return KB * cols <= 512; }
 
-bool few(int64_t n_cols, bool listed, bool by_ids) { return by_ids || (!listed && n_cols <= FEW_COLUMNS); }
+// Whether the kernel for few columns takes them: single pairs, and matrices of so few times 16 rows, times 16 columns, that two of these at most come to a CU.  Us of it /
+// of tiles, results in BF16: 4096 x 2048, 1 column 4.8 / 9.0, 32 6.9 / 9.1; 5120 x 2048, 16 6.8 / 9.1, 20 9.7 / 9.1; 12288 x 2048, 1 11.5 / 9.7; 248320 x 2048, 1 100.9 / 90.1, 32 164 / 102;
+// 1408 x 2048, 64 6.3 / 8.9, 100 10.8 / 8.8; 4096 x 8192, 32 20 / 28, 8192 x 8192, 20 32 / 28.  Where K is short tiles are level (512 x 512, 1 4.7 / 4.4), and 17 columns and more theirs
+// (32 5.3 / 4.5).
+constexpr int FEW_UNITS = 512;
+bool few(const bf16n_fp8_weight & w, int64_t n_cols, bool listed, bool by_ids) {
+    if (by_ids || listed) {
+        return by_ids;
+    }
+    const int KB = (int) ((w.K + FP8_BLOCK - 1) / FP8_BLOCK);
+    const int pass = std::min(16, few_pass(n_cols, KB, true));
+    return (n_cols <= 16 || KB >= 8) && (n_cols + pass - 1) / pass * ((w.rows + 15) / 16) <= FEW_UNITS;
+}
 size_t aligned(size_t n) { return (n + 255) / 256 * 256; }
 size_t codes_bytes(int64_t rows, int64_t K) { return aligned(rows * K) + aligned(rows * ((K + FP8_BLOCK - 1) / FP8_BLOCK) * 4); }
 
@@ -1322,11 +1342,11 @@ void launch_add_rmsnorm_fp8(const add_norm_args & a, const bf16n_fp8_rows & y, i
 // whether rows of activations become codes in a launch of their own
 static bool in_launch(const bf16n_fp8_weight & w, int x_kind, int64_t n_cols, bool listed, bool by_ids) {
     const int KB = (int) ((w.K + FP8_BLOCK - 1) / FP8_BLOCK);
-    return x_kind != CODES && !(few(n_cols, listed, by_ids) && converts(KB, by_ids ? 1 : n_cols));
+    return x_kind != CODES && !(few(w, n_cols, listed, by_ids) && converts(KB, by_ids ? 1 : std::min<int64_t>(n_cols, 32)));
 }
 
 uint64_t fp8_workspace_bytes(const bf16n_fp8_weight & w, bool glu, int x_kind, int y_kind, int64_t x_rows, int64_t n_cols, bool listed, bool by_ids) {
-    const bool f = few(n_cols, listed, by_ids);
+    const bool f = few(w, n_cols, listed, by_ids);
     uint64_t n = 0;
     if (in_launch(w, x_kind, n_cols, listed, by_ids)) {
         n += codes_bytes(x_rows, w.K);
@@ -1339,7 +1359,7 @@ uint64_t fp8_workspace_bytes(const bf16n_fp8_weight & w, bool glu, int x_kind, i
 
 void launch_fp8_product(const fp8_product & a, void * workspace, int cus, hipStream_t stream) {
     const bool glu = a.up != nullptr, listed = a.pairs != nullptr, by_ids = a.ids != nullptr;
-    const bool f = few(a.n_cols, listed, by_ids);
+    const bool f = few(*a.w, a.n_cols, listed, by_ids);
     fp8_launch p = launch_of(a, cus);
     char * ws = (char *) workspace;
     if (in_launch(*a.w, p.x_kind, a.n_cols, listed, by_ids)) {

@@ -18,8 +18,8 @@ def names(kernel):
 
 
 # (rows, K, tokens, results) -> what k_fp8_few or k_fp8_many are instances of
-FEW = [(512, 2048, 1, 1, 8, 1), (512, 2048, 17, 2, 8, 1), (9000, 640, 3, 1, 8, 0), (9000, 640, 32, 2, 8, 0), (512, 8192, 2, 1, 8, 0), (20000, 272, 2, 1, 4, 0), (20000, 272, 31, 2, 4, 0),
-       (90000, 144, 1, 1, 4, 0)]
+FEW = [(512, 2048, 1, 1, 8, 1), (512, 2048, 17, 2, 8, 1), (8000, 640, 3, 1, 8, 0), (4000, 1040, 32, 2, 8, 1), (512, 8192, 2, 1, 8, 0), (400, 8192, 31, 2, 8, 0), (512, 2048, 200, 2, 8, 1),
+       (300, 9104, 70, 1, 8, 0), (16, 1040, 8000, 2, 8, 1)]
 
 
 @pytest.mark.parametrize("R,K,T,ct,nw,one", FEW)
@@ -31,13 +31,43 @@ def test_every_form_for_few_columns(ops, R, K, T, ct, nw, one, kind):
     name, numbers = names(ops.last_kernel())
     assert name == "k_fp8_few" and (numbers[0], numbers[3], numbers[4]) == (ct, nw, one), ops.last_kernel()
     check(got, *X.product(q, xs, c, s))
-    if R <= 9000:
-        check(ops.fp8_linear_glu2(x, weight(ops, c, s), weight(ops, c, s), torch.float32), *X.gated(*[*X.product(q, xs, c, s)] * 2))
+    check(ops.fp8_linear_glu2(x, weight(ops, c, s), weight(ops, c, s), torch.float32), *X.gated(*[*X.product(q, xs, c, s)] * 2))
+    assert names(ops.last_kernel())[0] == "k_fp8_few"
+
+
+# few columns of many rows: narrow tiles
+NARROW = [(9000, 640, 3, 1), (9000, 144, 16, 1), (20000, 272, 2, 2), (90000, 144, 1, 2), (40000, 2576, 13, 2)]
+
+
+@pytest.mark.parametrize("R,K,T,rt", NARROW)
+@pytest.mark.parametrize("kind,out", [("bf16", torch.bfloat16), ("f32", torch.float32), ("rows", torch.float32), ("rows", torch.bfloat16)])
+def test_narrow_tiles(ops, R, K, T, rt, kind, out):
+    c, s = (t.cuda() for t in X.matrix(R, K, 48, bf16=kind == "f32"))
+    x, q, xs = give(X.rows(T, K, 49), kind)
+    got = ops.fp8_linear(x, ops.Fp8Weight(c, s), out_dtype=out)
+    name, numbers = names(ops.last_kernel())
+    assert name == "k_fp8_many" and numbers[:4] == [4, 1, rt, 1], ops.last_kernel()
+    y, dy = X.product(q.cuda(), xs.cuda(), c, s, out)
+    check(got, y.cpu(), dy.cpu())
+
+
+@pytest.mark.parametrize("T,n_used,E,N,K,nw", [(8, 8, 128, 528, 272, 4), (1, 60, 64, 512, 64, 4), (60, 1, 64, 8000, 144, 4), (1, 2, 4, 512, 2048, 8)])
+def test_single_pairs(ops, T, n_used, E, N, K, nw):
+    (c, s), (cu, su) = X.matrix(N, K, 50, E), X.matrix(N, K, 51, E)
+    ids = ids_for(T, n_used, E, 52)
+    x, q, xs = give(X.rows(T, K, 53, False), "bf16")
+    y, dy = by_pair(q, xs, c, s, ids, E, torch.float32)
+    got = ops.fp8_moe_mm_ids(x, ids.cuda(), weight(ops, c, s, E), E)
+    name, numbers = names(ops.last_kernel())
+    assert name == "k_fp8_few" and numbers[3] == nw, ops.last_kernel()
+    check(got.view(T * n_used, N), y, dy)
+    y, dy = X.gated(y, dy, *by_pair(q, xs, cu, su, ids, E, torch.float32))
+    check(ops.fp8_moe_mm_ids(x, ids.cuda(), weight(ops, c, s, E), E, weight(ops, cu, su, E)).view(T * n_used, N), y, dy)
 
 
 MANY = [((8192, 272, 8192), torch.bfloat16, (2, 4, 8, 4)), ((2000, 144, 4096), torch.bfloat16, (2, 2, 4, 4)), ((5120, 272, 500), torch.bfloat16, (2, 2, 2, 2)), ((5120, 272, 1024), torch.bfloat16, (2, 2, 4, 2)),
-        ((520, 272, 100), torch.bfloat16, (2, 2, 2, 2)), ((4096, 144, 4096), torch.float32, (4, 2, 4, 4)), ((5120, 272, 2050), torch.float32, (2, 2, 4, 2)), ((300, 9104, 70), torch.float32, (2, 2, 2, 2)),
-        ((300, 9104, 70), torch.bfloat16, (2, 2, 2, 2))]
+        ((520, 272, 100), torch.bfloat16, (2, 2, 2, 2)), ((4096, 144, 4096), torch.float32, (4, 2, 4, 4)), ((5120, 272, 2050), torch.float32, (2, 2, 4, 2)), ((4096, 9104, 70), torch.float32, (2, 2, 2, 2)),
+        ((4096, 9104, 70), torch.bfloat16, (2, 2, 2, 2))]
 
 
 @pytest.mark.parametrize("shape,out,tile", MANY)
@@ -52,7 +82,7 @@ def test_every_tile_of_the_dense_product(ops, shape, out, tile):
     check(got, y.cpu(), dy.cpu())
 
 
-GATED = [((1024, 144, 2050), (4, 2, 4, 4)), ((2048, 144, 2050), (4, 1, 4, 2)), ((2048, 272, 700), (4, 2, 4, 2)), ((1408, 272, 500), (4, 1, 4, 1)), ((1408, 272, 100), (4, 1, 4, 1)), ((144, 9104, 40), (4, 1, 4, 1))]
+GATED = [((1024, 144, 2050), (4, 2, 4, 4)), ((2048, 144, 2050), (4, 1, 4, 2)), ((2048, 272, 700), (4, 2, 4, 2)), ((1408, 272, 500), (4, 1, 4, 1)), ((1408, 272, 100), (4, 1, 4, 1)), ((2064, 9104, 70), (4, 1, 4, 1))]
 
 
 @pytest.mark.parametrize("shape,tile", GATED)
