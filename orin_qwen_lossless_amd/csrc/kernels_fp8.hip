@@ -1269,14 +1269,15 @@ void run_many(const fp8_launch * p, bool glu, bool list, hipStream_t stream) {
         best = best_tile(tiles, 4, *p);
     } else if (p && p->ncols <= 16) {
         // (Us of 64 x 64 tiles, 128 x 16, 64 x 16, one column: BF16 results 20480 x 2048 11.0, 9.2, 9.9, 16384 x 8192 29, 27, 21; FP32 248320 x 2048 101, 86, 87, 16384 x 8192 43, 31, 26.)
-        best = (p->nrows + 63) / 64 <= p->cus ? 5 : 4;
+        best = (p->nrows + 63) / 64 <= p->cus ? 9 : 8;
     } else if (p && kind == BF16) {
-        // (5120 x 2048, us in this order: 128 columns 33, 16, 11, 9.1; 1024: 39, 23, 21, 22; 2048: 40, 36, 32, 41; 8192 x 2048, 8192: 152, 171, 189, 235)
-        const tile_of tiles[] = {{256, 256, 2.0f, 2.0f}, {128, 128, 0.95f, 0.685f}, {128, 64, 0.62f, 0.387f}, {64, 64, 0.45f, 0.238f}};
+        // (5120 x 2048, us in this order: 128 columns 33, 16, 11, 9.1; 1024: 39, 23, 21, 22; 2048: 40, 36, 32, 41; 8192 x 2048, 8192: 152, 171, 189, 235;
+        // the last two, 64 columns 9.4, 7.6; 150 10.0, 9.3; 300 11.4, 15.6)
+        const tile_of tiles[] = {{256, 256, 2.0f, 2.0f}, {128, 128, 0.95f, 0.685f}, {128, 64, 0.62f, 0.387f}, {64, 64, 0.45f, 0.238f}, {32, 64, 0.33f, 0.22f}};
+        best = best_tile(tiles, 5, *p);
+    } else if (p) { // (5120 x 2048, us in this order: 64 columns 29, 15, 10.5; 2048: 65, 50, 56; 8192 x 2048, 8192: 264, 293, 336; the last two, 64 columns 11.1, 9.3; 150 11.6, 12.6)
+        const tile_of tiles[] = {{256, 128, 2.0f, 2.05f}, {128, 64, 0.88f, 0.6f}, {64, 64, 0.62f, 0.33f}, {32, 64, 0.51f, 0.32f}};
         best = best_tile(tiles, 4, *p);
-    } else if (p) { // (5120 x 2048, us in this order: 64 columns 29, 15, 10.5; 2048: 65, 50, 56; 8192 x 2048, 8192: 264, 293, 336)
-        const tile_of tiles[] = {{256, 128, 2.0f, 2.05f}, {128, 64, 0.88f, 0.6f}, {64, 64, 0.62f, 0.33f}};
-        best = best_tile(tiles, 3, *p);
     }
     MANY(glu && list, 0, 4, 1, 4, 4, 2, true, true)
     MANY(!glu && list, 0, 2, 2, 4, 2, 2, false, true)
@@ -1288,13 +1289,15 @@ void run_many(const fp8_launch * p, bool glu, bool list, hipStream_t stream) {
     MANY_ONE(!glu && !list && kind == BF16, 1, 2, 2, 4, 4, 2, false, false, BF16)
     MANY_ONE(!glu && !list && kind == BF16, 2, 2, 2, 4, 2, 2, false, false, BF16)
     MANY_ONE(!glu && !list && kind == BF16, 3, 2, 2, 2, 2, 3, false, false, BF16)
-    MANY_ONE(!glu && !list && kind == BF16, 4, 4, 1, 2, 1, 3, false, false, BF16)
-    MANY_ONE(!glu && !list && kind == BF16, 5, 4, 1, 1, 1, 4, false, false, BF16)
+    MANY_ONE(!glu && !list && kind == BF16, 4, 2, 2, 1, 2, 4, false, false, BF16)
+    MANY_ONE(!glu && !list && kind == BF16, 8, 4, 1, 2, 1, 3, false, false, BF16)
+    MANY_ONE(!glu && !list && kind == BF16, 9, 4, 1, 1, 1, 4, false, false, BF16)
     MANY_ONE(!glu && !list && kind == F32, 0, 4, 2, 4, 4, 2, false, false, F32)
     MANY_ONE(!glu && !list && kind == F32, 1, 2, 2, 4, 2, 2, false, false, F32)
     MANY_ONE(!glu && !list && kind == F32, 2, 2, 2, 2, 2, 2, false, false, F32)
-    MANY_ONE(!glu && !list && kind == F32, 4, 4, 1, 2, 1, 3, false, false, F32)
-    MANY_ONE(!glu && !list && kind == F32, 5, 4, 1, 1, 1, 4, false, false, F32)
+    MANY_ONE(!glu && !list && kind == F32, 3, 2, 2, 1, 2, 4, false, false, F32)
+    MANY_ONE(!glu && !list && kind == F32, 8, 4, 1, 2, 1, 3, false, false, F32)
+    MANY_ONE(!glu && !list && kind == F32, 9, 4, 1, 1, 1, 4, false, false, F32)
 #undef MANY
 #undef MANY_ONE
 }
@@ -1305,8 +1308,8 @@ void run_many(const fp8_launch * p, bool glu, bool list, hipStream_t stream) {
 bool converts(int KB, int64_t cols) { return KB * cols <= 512; }
 
 // Whether the kernel for few columns takes them: single pairs, and matrices of so few times 16 rows, times 16 columns, that two of these at most come to a CU.  Us of it /
-// of tiles, results in BF16: 4096 x 2048, 1 column 4.8 / 9.0, 32 6.9 / 9.1; 5120 x 2048, 16 6.8 / 9.1, 20 9.7 / 9.1; 12288 x 2048, 1 11.5 / 9.7; 248320 x 2048, 1 100.9 / 90.1, 32 164 / 102;
-// 1408 x 2048, 64 6.3 / 8.9, 100 10.8 / 8.8; 4096 x 8192, 32 20 / 28, 8192 x 8192, 20 32 / 28.  Where K is short tiles are level (512 x 512, 1 4.7 / 4.4), and 17 columns and more theirs
+// of tiles, results in BF16: 4096 x 2048, 1 column 4.8 / 9.0, 32 6.9 / 7.4; 5120 x 2048, 16 6.8 / 9.1, 20 9.7 / 7.4; 12288 x 2048, 1 11.5 / 9.7; 248320 x 2048, 1 101 / 90, 32 164 / 102;
+// 1408 x 2048, 64 6.3 / 7.5, 100 10.8 / 7.5; 4096 x 8192, 32 20 / 28, 8192 x 8192, 20 32 / 28.  Where K is short tiles are level (512 x 512, 1 4.7 / 4.4), and 17 columns and more theirs
 // (32 5.3 / 4.5).
 constexpr int FEW_UNITS = 512;
 bool few(const bf16n_fp8_weight & w, int64_t n_cols, bool listed, bool by_ids) {

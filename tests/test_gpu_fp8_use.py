@@ -66,8 +66,8 @@ def test_single_pairs(ops, T, n_used, E, N, K, nw):
 
 
 MANY = [((8192, 272, 8192), torch.bfloat16, (2, 4, 8, 4)), ((2000, 144, 4096), torch.bfloat16, (2, 2, 4, 4)), ((5120, 272, 500), torch.bfloat16, (2, 2, 2, 2)), ((5120, 272, 1024), torch.bfloat16, (2, 2, 4, 2)),
-        ((520, 272, 100), torch.bfloat16, (2, 2, 2, 2)), ((4096, 144, 4096), torch.float32, (4, 2, 4, 4)), ((5120, 272, 2050), torch.float32, (2, 2, 4, 2)), ((4096, 9104, 70), torch.float32, (2, 2, 2, 2)),
-        ((4096, 9104, 70), torch.bfloat16, (2, 2, 2, 2))]
+        ((520, 272, 100), torch.bfloat16, (2, 2, 1, 2)), ((4096, 144, 4096), torch.float32, (4, 2, 4, 4)), ((5120, 272, 2050), torch.float32, (2, 2, 4, 2)), ((5120, 272, 150), torch.float32, (2, 2, 2, 2)),
+        ((4096, 9104, 70), torch.float32, (2, 2, 1, 2)), ((4096, 9104, 70), torch.bfloat16, (2, 2, 1, 2))]
 
 
 @pytest.mark.parametrize("shape,out,tile", MANY)
