@@ -1264,9 +1264,16 @@ void run_many(const fp8_launch * p, bool glu, bool list, hipStream_t stream) {
     int best = 0;
     if (p && list) {
         best = 0;
-    } else if (p && glu) { // (codes, us in this order: 1408 x 2048, 300 columns 34, 23, 17, 15; 2048 x 2048, 2048 columns 39, 47, 47, 67)
+    } else if (p && glu && kind == CODES) { // ( us in this order: 1408 x 2048, 300 columns 34, 23, 17, 15; 2048 x 2048, 2048 columns 39, 47, 47, 67)
         const tile_of tiles[] = {{128, 128, 2.0f, 2.05f}, {128, 64, 1.4f, 1.45f}, {128, 32, 1.1f, 0.75f}, {128, 16, 0.85f, 0.54f}};
         best = best_tile(tiles, 4, *p);
+    } else if (p && glu && p->ncols <= 16) { // (BF16 / FP32 results with 64 x 16 and 128 x 16: 12288 x 2048, 8 columns 10.8 / 11.4 us, 15.3 / 15.6; 65536 x 2048, 4 54.7 / 55.3, 51.3 / 47.7)
+        best = (p->nrows + 63) / 64 <= 2 * p->cus ? 6 : 3;
+    } else if (p && glu) {
+        // (128 x 128, 64 x 64, 32 x 64, 128 x 16, us: BF16 results 1408 x 2048, 300 columns 22, 11.8, 9.9, 13.6; 2048 x 2048, 2048 24, 28, 33, 53; FP32 33, 15.6, 12.6, 15.4 and 38, 40, 46, 65)
+        const tile_of bf16[] = {{128, 128, 1.2f, 1.45f}, {64, 64, 0.6f, 0.43f}, {32, 64, 0.47f, 0.26f}}, f32[] = {{128, 128, 2.0f, 2.2f}, {64, 64, 0.83f, 0.63f}, {32, 64, 0.62f, 0.38f}};
+        const int of[] = {0, 5, 4};
+        best = of[best_tile(kind == BF16 ? bf16 : f32, 3, *p)];
     } else if (p && p->ncols <= 16) {
         // (Us of 64 x 64 tiles, 128 x 16, 64 x 16, one column: BF16 results 20480 x 2048 11.0, 9.2, 9.9, 16384 x 8192 29, 27, 21; FP32 248320 x 2048 101, 86, 87, 16384 x 8192 43, 31, 26.)
         best = (p->nrows + 63) / 64 <= p->cus ? 9 : 8;
@@ -1282,9 +1289,15 @@ void run_many(const fp8_launch * p, bool glu, bool list, hipStream_t stream) {
     MANY(glu && list, 0, 4, 1, 4, 4, 2, true, true)
     MANY(!glu && list, 0, 2, 2, 4, 2, 2, false, true)
     MANY(glu && !list, 0, 4, 2, 4, 4, 2, true, false)
-    MANY(glu && !list, 1, 4, 2, 4, 2, 2, true, false)
-    MANY(glu && !list, 2, 4, 1, 4, 2, 2, true, false)
+    MANY_ONE(glu && !list && kind == CODES, 1, 4, 2, 4, 2, 2, true, false, CODES)
+    MANY_ONE(glu && !list && kind == CODES, 2, 4, 1, 4, 2, 2, true, false, CODES)
     MANY(glu && !list, 3, 4, 1, 4, 1, 2, true, false)
+    MANY_ONE(glu && !list && kind == BF16, 4, 2, 2, 2, 2, 3, true, false, BF16)
+    MANY_ONE(glu && !list && kind == F32, 4, 2, 2, 2, 2, 3, true, false, F32)
+    MANY_ONE(glu && !list && kind == BF16, 5, 2, 2, 4, 2, 2, true, false, BF16)
+    MANY_ONE(glu && !list && kind == F32, 5, 2, 2, 4, 2, 2, true, false, F32)
+    MANY_ONE(glu && !list && kind == BF16, 6, 4, 1, 2, 1, 3, true, false, BF16)
+    MANY_ONE(glu && !list && kind == F32, 6, 4, 1, 2, 1, 3, true, false, F32)
     MANY_ONE(!glu && !list && kind == BF16, 0, 2, 4, 8, 4, 2, false, false, BF16)
     MANY_ONE(!glu && !list && kind == BF16, 1, 2, 2, 4, 4, 2, false, false, BF16)
     MANY_ONE(!glu && !list && kind == BF16, 2, 2, 2, 4, 2, 2, false, false, BF16)

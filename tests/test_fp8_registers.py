@@ -22,6 +22,6 @@ def test_no_kernel_spills(tmp_path):
     run("clang-offload-bundler", "--type=o", "--unbundle", "--targets=hipv4-amdgcn-amd-amdhsa--gfx950", f"--input={fat}", f"--output={code}")
     notes = run("llvm-readelf", "--notes", code)
     found = {name: int(count) for name, count in re.findall(r"\.name:\s+(\S+)\n(?:(?!\.name:).)*?\.vgpr_spill_count:\s+(\d+)", notes, re.S)}
-    for kernel, instances in (("k_fp8_few", 30), ("k_fp8_many", 30), ("k_add_rmsnorm_fp8", 4), ("k_fp8_down", 1), ("k_fp8_combine", 1), ("k_fp8_rows", 2)):
+    for kernel, instances in (("k_fp8_few", 30), ("k_fp8_many", 32), ("k_add_rmsnorm_fp8", 4), ("k_fp8_down", 1), ("k_fp8_combine", 1), ("k_fp8_rows", 2)):
         mine = {n: c for n, c in found.items() if re.search(rf"\d{kernel}(I|E)", n)}
         assert len(mine) == instances and not any(mine.values()), (kernel, mine)

@@ -82,13 +82,17 @@ def test_every_tile_of_the_dense_product(ops, shape, out, tile):
     check(got, y.cpu(), dy.cpu())
 
 
-GATED = [((1024, 144, 2050), (4, 2, 4, 4)), ((2048, 144, 2050), (4, 1, 4, 2)), ((2048, 272, 700), (4, 2, 4, 2)), ((1408, 272, 500), (4, 1, 4, 1)), ((1408, 272, 100), (4, 1, 4, 1)), ((2064, 9104, 70), (4, 1, 4, 1))]
+# (rows, K, tokens) -> the tile of results that are codes, and of others
+GATED = [((1024, 144, 2050), (4, 2, 4, 4), (2, 2, 4, 2)), ((2048, 144, 2050), (4, 1, 4, 2), (2, 2, 4, 2)), ((2048, 272, 700), (4, 2, 4, 2), (2, 2, 2, 2)), ((1408, 272, 500), (4, 1, 4, 1), (2, 2, 2, 2)),
+         ((1408, 272, 100), (4, 1, 4, 1), (2, 2, 2, 2)), ((2064, 9104, 70), (4, 1, 4, 1), (2, 2, 2, 2)), ((2048, 144, 4096), (4, 2, 4, 4), (4, 2, 4, 4)), ((9008, 144, 9), (4, 1, 4, 1), (4, 1, 2, 1)),
+         ((70000, 144, 3), (4, 1, 4, 1), (4, 1, 4, 1))]
 
 
-@pytest.mark.parametrize("shape,tile", GATED)
+@pytest.mark.parametrize("shape,codes,others", GATED)
 @pytest.mark.parametrize("out", [X.E4M3, torch.bfloat16, torch.float32])
-def test_every_tile_of_the_gated_product(ops, shape, tile, out):
+def test_every_tile_of_the_gated_product(ops, shape, codes, others, out):
     R, K, T = shape
+    tile = codes if out is X.E4M3 else others
     (c, s), (cu, su) = ([t.cuda() for t in X.matrix(R, K, 15 + i)] for i in range(2))
     q, xs = (t.cuda() for t in X.quantize(X.rows(T, K, 17, False)))
     got = ops.fp8_linear_glu2(ops.Fp8Rows(q, xs), ops.Fp8Weight(c, s), ops.Fp8Weight(cu, su), out)
