@@ -273,8 +273,7 @@ int bf16n_fp8_mm_ids(const bf16n_fp8_weight * w, const bf16n_fp8_weight * up, co
                      int64_t ids_s0, int64_t ids_s1, const int32_t * pairs, const int32_t * bounds, const bf16n_fp8_rows * y, int n_tok, int n_used,
                      void * workspace, uint64_t workspace_bytes, void * stream);
 /* The routed experts of a layer: y[t] = sum over the slots of wts[t, slot] * down_e(silu(gate_e x[t]) * (up_e x[t])), hidden rows held in 8
- * bits (from FP32 values), the slots' results in FP32 or, where the pairs are more than 64 or than the experts, in BF16 (half a step each, at most
- * 2^-9 of a slot's result, beside the 2^-4 of the codes).  wts null: y has a row of FP32 for every pair, unweighted.  wts: FP32 or BF16
+ * bits (from FP32 values), the slots' results and their sum in FP32.  wts null: y has a row of FP32 for every pair, unweighted.  wts: FP32 or BF16
  * [n_tok, n_used].  y: BF16 or FP32, contiguous rows. */
 int bf16n_fp8_moe_experts(const bf16n_fp8_weight * gate, const bf16n_fp8_weight * up, const bf16n_fp8_weight * down, const bf16n_fp8_rows * x,
                           const void * ids, int ids_i64, int64_t ids_s0, int64_t ids_s1, const void * wts, int wts_bf16, const bf16n_fp8_rows * y,

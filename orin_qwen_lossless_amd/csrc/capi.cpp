@@ -853,7 +853,6 @@ void check_workspace(const void * workspace, uint64_t have, uint64_t need) {
 
 struct experts_plan { // offsets in the workspace
     bool listed;
-    bool half; // slots' results in BF16
     bool fused; // down and the weighted sum in one launch
     int hidden_kind; // hidden rows as down takes them: codes, or FP32 where its blocks make the codes
     uint64_t lists, hidden, hidden_scales, ys, product, bytes;
@@ -871,7 +870,6 @@ experts_plan plan_experts(const bf16n_fp8_weight & gate, const bf16n_fp8_weight 
     };
     // few pairs: each is a column by itself
     e.listed = pairs > std::min<int64_t>(gate.n_matrices, FP8_SINGLE_PAIRS);
-    e.half = e.listed && weighted && out % 8 == 0;
     e.fused = !e.listed && weighted && dev::fp8_down_fits(down, n_used);
     e.hidden_kind = e.listed ? BF16N_FP8_CODES : BF16N_FP8_F32;
     if (e.listed) {
@@ -882,7 +880,7 @@ experts_plan plan_experts(const bf16n_fp8_weight & gate, const bf16n_fp8_weight 
     }
     take(e.hidden, pairs * mid * (e.hidden_kind == BF16N_FP8_CODES ? 1 : 4));
     if (weighted && !e.fused) {
-        take(e.ys, pairs * out * (e.half ? 2 : 4));
+        take(e.ys, pairs * out * 4);
     }
     const uint64_t a = dev::fp8_workspace_bytes(gate, true, x_kind, e.hidden_kind, n_tok, pairs, e.listed, !e.listed);
     const uint64_t b = dev::fp8_workspace_bytes(down, false, e.hidden_kind, BF16N_FP8_F32, pairs, pairs, e.listed, !e.listed);
@@ -1041,14 +1039,14 @@ int bf16n_fp8_moe_experts(const bf16n_fp8_weight * gate, const bf16n_fp8_weight 
             launch_check("fp8_moe_experts");
             return;
         }
-        b.y = wts ? bf16n_fp8_rows{ws + e.ys, nullptr, out * (e.half ? 2 : 4), 0, 0, e.half ? BF16N_FP8_BF16 : BF16N_FP8_F32, 0} : *y;
+        b.y = wts ? bf16n_fp8_rows{ws + e.ys, nullptr, out * 4, 0, 0, BF16N_FP8_F32, 0} : *y;
         dev::launch_fp8_product(a, ws + e.product, g_cus, st);
         launch_check("fp8_moe_experts");
         dev::launch_fp8_product(b, ws + e.product, g_cus, st);
         launch_check("fp8_moe_experts");
         if (wts) {
-            if (e.half) {
-                dev::launch_fp8_combine(ws + e.ys, wts, wts_bf16 != 0, y->at, y->kind == BF16N_FP8_BF16, n_tok, n_used, out, st);
+            if (out % 8 == 0) {
+                dev::launch_fp8_combine((const float *) (ws + e.ys), wts, wts_bf16 != 0, y->at, y->kind == BF16N_FP8_BF16, n_tok, n_used, out, st);
             } else {
                 dev::launch_moe_combine((const float *) (ws + e.ys), wts, wts_bf16 != 0, y->at, y->kind == BF16N_FP8_BF16, n_tok, n_used, out, st);
             }

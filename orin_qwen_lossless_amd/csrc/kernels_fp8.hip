@@ -1040,8 +1040,8 @@ constexpr int WAY = C == 1 ? 8 : 4; // (registers)
     }
 }
 
-// y[t] = sum over the slots of w[t, k] * ys[t, k] for rows in BF16, slots in order, one fmaf each; n a multiple of 8
-__global__ void __launch_bounds__(256) k_fp8_combine(const uint16_t * ys, const void * w, bool w_bf16, char * y, bool y_bf16, int n_used, int64_t n) {
+// y[t] = sum over the slots of w[t, k] * ys[t, k] for rows in FP32, slots in order, one fmaf each; n a multiple of 8
+__global__ void __launch_bounds__(256) k_fp8_combine(const float * ys, const void * w, bool w_bf16, char * y, bool y_bf16, int n_used, int64_t n) {
     const int64_t t = blockIdx.y, i = ((int64_t) blockIdx.x * 256 + threadIdx.x) * 8;
     if (i >= n) {
         return;
@@ -1050,11 +1050,10 @@ __global__ void __launch_bounds__(256) k_fp8_combine(const uint16_t * ys, const 
     for (int k = 0; k < n_used; k++) {
         const int64_t s = t * n_used + k;
         const float wk = scale_at(w, w_bf16, s);
-        float v[8];
-        bf16x8_to_f32(__builtin_nontemporal_load((const u32x4_t *) (ys + s * n + i)), v);
+        const f32x4_t lo = __builtin_nontemporal_load((const f32x4_t *) (ys + s * n + i)), hi = __builtin_nontemporal_load((const f32x4_t *) (ys + s * n + i + 4));
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            acc[e] = fmaf(wk, v[e], acc[e]);
+            acc[e] = fmaf(wk, e < 4 ? lo[e & 3] : hi[e & 3], acc[e]);
         }
     }
     char * const at = y + (t * n + i) * (y_bf16 ? 2 : 4);
@@ -1416,8 +1415,8 @@ void launch_fp8_down(const fp8_product & a, const void * wts, bool wts_bf16, int
     k_fp8_down<<<dim3((p.nrows + 15) / 16, n_tok), 512, down_lds(p.n_used, p.KB), stream>>>(p, wts, wts_bf16);
 }
 
-void launch_fp8_combine(const void * ys, const void * w, bool w_bf16, void * y, bool y_bf16, int n_tok, int n_used, int64_t n, hipStream_t stream) {
-    k_fp8_combine<<<dim3((unsigned) ((n / 8 + 255) / 256), (unsigned) n_tok), 256, 0, stream>>>((const uint16_t *) ys, w, w_bf16, (char *) y, y_bf16, n_used, n);
+void launch_fp8_combine(const float * ys, const void * w, bool w_bf16, void * y, bool y_bf16, int n_tok, int n_used, int64_t n, hipStream_t stream) {
+    k_fp8_combine<<<dim3((unsigned) ((n / 8 + 255) / 256), (unsigned) n_tok), 256, 0, stream>>>(ys, w, w_bf16, (char *) y, y_bf16, n_used, n);
 }
 
 } // namespace dev

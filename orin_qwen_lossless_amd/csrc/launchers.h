@@ -135,7 +135,7 @@ void launch_fp8_product(const fp8_product & a, void * workspace, int cus, hipStr
 // the slots' products (by ids, FP32 rows of x) and their weighted sum: a.y has a row for every token
 bool fp8_down_fits(const bf16n_fp8_weight & down, int n_used);
 void launch_fp8_down(const fp8_product & a, const void * wts, bool wts_bf16, int n_tok, int cus, hipStream_t stream);
-void launch_fp8_combine(const void * ys, const void * w, bool w_bf16, void * y, bool y_bf16, int n_tok, int n_used, int64_t n, hipStream_t stream);
+void launch_fp8_combine(const float * ys, const void * w, bool w_bf16, void * y, bool y_bf16, int n_tok, int n_used, int64_t n, hipStream_t stream);
 
 // batched MoE prefill (kernels_mm_ids.hip)
 void mm_ids_init();

@@ -1556,8 +1556,7 @@ def fp8_moe_experts_rows(x: torch.Tensor | Fp8Rows, gate: Fp8Weight, up: Fp8Weig
 
 def fp8_moe_experts(x: torch.Tensor | Fp8Rows, gate: Fp8Weight, up: Fp8Weight, down: Fp8Weight, topk_weights: torch.Tensor,
                     topk_ids: torch.Tensor, n_experts: int) -> torch.Tensor:
-    """Routed experts of one MoE layer in 8 bits, BF16 out (moe_experts).  Where the pairs are more than 64, or than the experts, the slots' results
-    are held in BF16 before their weighted sum in FP32 (half a step, 2^-9 of a slot's result, beside the 2^-4 of the codes)."""
+    """Routed experts of one MoE layer in 8 bits, BF16 out (moe_experts): fp8_moe_experts_rows and their weighted sum, in FP32 until its one rounding."""
     if topk_weights is None:
         raise ValueError("bf16n.fp8_moe_experts: topk_weights must be contiguous f32/bf16 [tokens, n_used]")
     y = (_host_calls or _host()).fp8_moe_experts(x, gate, up, down, topk_weights, topk_ids, n_experts)
