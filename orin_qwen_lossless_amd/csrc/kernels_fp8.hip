@@ -929,7 +929,7 @@ __device__ __forceinline__ u32x4_t to_bf16x8(const float (&v)[8]) {
 
 // The glue of a decode step (bf16n_add_rmsnorm) with its norm in 8 bits: a block to a token, C pieces of eight elements to a thread, 16 threads to
 // a block of 128, eight slots' rows on the way at a time (one after the other: 333 tokens of 2576 with eight slots 10.9 us).  A row stays
-// in registers between the sum of its squares and its codes.  The slots' sum, the squares' and the norm are held in 64 bits and become
+// in registers between the sum of its squares and its codes.  Every sum and the norm are held in 64 bits and become
 // FP32 once, ahead of the scales: a code is off by a whole step, a sixteenth of its value, wherever an error of a last place carries a value over the
 // middle of two codes, which 32 bits did to one or two of 858 thousand (and were 8.9 us there for 9.6).
 // 8192 tokens of 2048: 22.1 us, 118 MB at 5.3 TB/s; one token 2.7, the chain of its loads, sum and scale.
@@ -946,7 +946,7 @@ __global__ void __launch_bounds__(1024) k_add_rmsnorm_fp8(const add_norm_args p,
         }
         __syncthreads();
     }
-    std::conditional_t<SLOTS, double, float> v[C][8];
+    double v[C][8];
     double sq = 0;
     u32x4_t gamma[C];
 #pragma unroll
@@ -968,8 +968,8 @@ __global__ void __launch_bounds__(1024) k_add_rmsnorm_fp8(const add_norm_args p,
             }
             if (SLOTS) {
                 const float * row = p.ys + (tok * p.n_used) * p.n + i0;
-constexpr int WAY = C == 1 ? 8 : 4; // (registers)
-                                for (int k0 = 0; k0 < p.n_used; k0 += WAY) {
+                constexpr int WAY = C == 1 ? 8 : 4; // (registers)
+                for (int k0 = 0; k0 < p.n_used; k0 += WAY) {
                     f32x4_t lo[WAY], hi[WAY];
 #pragma unroll
                     for (int k = 0; k < WAY; k++) { // (a slot past the last: the last row again, unused)
@@ -995,9 +995,20 @@ constexpr int WAY = C == 1 ? 8 : 4; // (registers)
         bf16x8_to_f32(c, fc);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            // (a sum of BF16 numbers is exact in FP32 unless they are 2^16 apart)
-            v[j][e] = SLOTS ? (double) ((fa[e] + fb[e]) + fc[e]) + acc[e] : (fa[e] + fb[e]) + fc[e];
-            sq = fma((double) v[j][e], (double) v[j][e], sq);
+            v[j][e] = (double) fa[e] + (double) fb[e];
+        }
+        if (p.c) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                v[j][e] += (double) fc[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if (SLOTS) {
+                v[j][e] += acc[e];
+            }
+            sq = fma(v[j][e], v[j][e], sq);
         }
     }
     sq = wave_sum64(sq);
@@ -1025,7 +1036,7 @@ constexpr int WAY = C == 1 ? 8 : 4; // (registers)
         bf16x8_to_f32(gamma[j], g);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            y32[e] = (float) ((double) v[j][e] * scale * (double) g[e]);
+            y32[e] = (float) (v[j][e] * scale * (double) g[e]);
         }
         if (in && p.y_norm) {
             *(u32x4_t *) (p.y_norm + base + i0) = to_bf16x8(y32);
