@@ -1372,6 +1372,9 @@ static bool in_launch(const bf16n_fp8_weight & w, int x_kind, int64_t n_cols, bo
 }
 
 uint64_t fp8_workspace_bytes(const bf16n_fp8_weight & w, bool glu, int x_kind, int y_kind, int64_t x_rows, int64_t n_cols, bool listed, bool by_ids) {
+    if (n_cols == 0) { // (the sizes of a pass and their number are for columns that there are)
+        return 0;
+    }
     const bool f = few(w, n_cols, listed, by_ids);
     uint64_t n = 0;
     if (in_launch(w, x_kind, n_cols, listed, by_ids)) {
