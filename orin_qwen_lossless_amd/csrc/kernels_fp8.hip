@@ -1,5 +1,6 @@
 // Products in 8-bit floating point with a scale for every block of 128, and what makes rows of that form (gfx950).
 #include "dev_fp8.h"
+#include "launch_dims.h"
 #include "launchers.h"
 
 #include <algorithm>
@@ -344,9 +345,11 @@ __global__ void __launch_bounds__(512, 4) k_fp8_down(const fp8_launch p, const v
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, m16 = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int KB = p.KB, pitch = KB * FP8_BLOCK + 16, slots = p.n_used, token = blockIdx.y, row0 = blockIdx.x * 16;
-    float * const lds_scales = (float *) (lds + slots * pitch);  // [slots][KB]
-    float * const res = lds_scales + slots * KB;                 // [slots][16]
+    const int KB = p.KB, slots = p.n_used, token = blockIdx.y, row0 = blockIdx.x * 16;
+    const fp8_down_lds in = fp8_down_layout(slots, KB);
+    const int pitch = in.pitch;
+    float * const lds_scales = (float *) (lds + in.scales);  // [slots][KB]
+    float * const res = (float *) (lds + in.results);        // [slots][16]
     const bool cut = p.K % FP8_BLOCK != 0;
     const int last = (KB - 1) * FP8_BLOCK + q * 16;
     const bool out0 = cut && last >= p.K, out1 = cut && last + 64 >= p.K;
@@ -1417,16 +1420,14 @@ void launch_fp8_product(const fp8_product & a, void * workspace, int cus, hipStr
     }
 }
 
-// LDS of k_fp8_down
-static size_t down_lds(int slots, int KB) { return (size_t) slots * (KB * FP8_BLOCK + 16 + KB * 4 + 64); }
 bool fp8_down_fits(const bf16n_fp8_weight & down, int n_used) {
     const int KB = (int) ((down.K + FP8_BLOCK - 1) / FP8_BLOCK);
-    return KB <= FEW_PARTS && down_lds(n_used, KB) <= FEW_LDS;
+    return KB <= FEW_PARTS && fp8_down_layout(n_used, KB).bytes <= (int) FEW_LDS; // (n_used below 1024)
 }
 void launch_fp8_down(const fp8_product & a, const void * wts, bool wts_bf16, int n_tok, int cus, hipStream_t stream) {
     const fp8_launch p = launch_of(a, cus);
     note_kernel("k_fp8_down", nullptr, 0);
-    k_fp8_down<<<dim3((p.nrows + 15) / 16, n_tok), 512, down_lds(p.n_used, p.KB), stream>>>(p, wts, wts_bf16);
+    k_fp8_down<<<dim3((p.nrows + 15) / 16, n_tok), 512, fp8_down_layout(p.n_used, p.KB).bytes, stream>>>(p, wts, wts_bf16);
 }
 
 void launch_fp8_combine(const float * ys, const void * w, bool w_bf16, void * y, bool y_bf16, int n_tok, int n_used, int64_t n, hipStream_t stream) {

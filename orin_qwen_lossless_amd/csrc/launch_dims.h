@@ -18,5 +18,13 @@ inline int spread_waves(int64_t waves, int cus, int full) {
     return even < full * up(up(waves, full), cus) ? (int) even : full;
 }
 
+// LDS of k_fp8_down in bytes: the slots' codes (a row for each, 16 bytes further apart than it is long), their scales, 16 results for each slot, which
+// are stored four at a time: from a multiple of 16 bytes on, whatever the number of scales.
+struct fp8_down_lds { int pitch, scales, results, bytes; };
+constexpr fp8_down_lds fp8_down_layout(int slots, int blocks) {
+    const int pitch = blocks * 128 + 16, scales = slots * pitch, results = (scales + slots * blocks * 4 + 15) / 16 * 16;
+    return {pitch, scales, results, results + slots * 64};
+}
+
 } // namespace dev
 } // namespace bf16n
