@@ -263,7 +263,8 @@ int bf16n_add_rmsnorm_fp8(const uint16_t * a, const uint16_t * b, const uint16_t
  * that is 0).  The result must not overlap x. */
 int bf16n_fp8_mm(const bf16n_fp8_weight * w, const bf16n_fp8_weight * up, const bf16n_fp8_rows * x, const bf16n_fp8_rows * y, int64_t n_rows,
                  void * workspace, uint64_t workspace_bytes, void * stream);
-/* *bytes of workspace for bf16n_fp8_mm (n_pairs = 0) or bf16n_fp8_mm_ids (n_pairs = n_tok * n_used; listed: with pairs and bounds) */
+/* *bytes of workspace for bf16n_fp8_mm (n_pairs = 0) or bf16n_fp8_mm_ids (n_pairs = n_tok * n_used; listed: with pairs and bounds): enough
+ * for these rows and for fewer of them, so that one workspace of the longest batch's size serves every other */
 int bf16n_fp8_workspace_bytes(const bf16n_fp8_weight * w, int gate_up, int x_kind, int y_kind, int64_t x_rows, int64_t n_pairs, int listed,
                               uint64_t * bytes);
 /* The same by matrix: row pair of y = W_e x for every (token, slot) pair t * n_used + slot, e its id; rows of zeros where an id names no
@@ -278,6 +279,7 @@ int bf16n_fp8_mm_ids(const bf16n_fp8_weight * w, const bf16n_fp8_weight * up, co
 int bf16n_fp8_moe_experts(const bf16n_fp8_weight * gate, const bf16n_fp8_weight * up, const bf16n_fp8_weight * down, const bf16n_fp8_rows * x,
                           const void * ids, int ids_i64, int64_t ids_s0, int64_t ids_s1, const void * wts, int wts_bf16, const bf16n_fp8_rows * y,
                           int n_tok, int n_used, void * workspace, uint64_t workspace_bytes, void * stream);
+/* *bytes of workspace for n_tok tokens or fewer of them */
 int bf16n_fp8_moe_experts_workspace_bytes(const bf16n_fp8_weight * gate, const bf16n_fp8_weight * down, int x_kind, int weighted, int n_tok, int n_used,
                                           uint64_t * bytes);
 

@@ -9,6 +9,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cstdint>
 #include <functional>
@@ -860,6 +861,7 @@ struct experts_plan { // offsets in the workspace
 // As many pairs are products by themselves, each reading its matrix, before they are listed by expert for three launches more (256 experts of
 // 512 x 2048, top-8, us by themselves / listed: 8 tokens 41 / 44, 12 68 / 62, 32 127 / 110; 64 of 1024 x 1024, top-6: 6 33 / 34, 8 42 / 39), and as many as there are experts.
 constexpr int64_t FP8_SINGLE_PAIRS = 64;
+int64_t single_pairs(const bf16n_fp8_weight & gate) { return std::min<int64_t>(gate.n_matrices, FP8_SINGLE_PAIRS); }
 
 experts_plan plan_experts(const bf16n_fp8_weight & gate, const bf16n_fp8_weight & down, int x_kind, bool weighted, int n_tok, int n_used) {
     const int64_t pairs = (int64_t) n_tok * n_used, mid = gate.rows / gate.n_matrices, out = down.rows / down.n_matrices;
@@ -869,7 +871,7 @@ experts_plan plan_experts(const bf16n_fp8_weight & gate, const bf16n_fp8_weight 
         e.bytes += (n + 255) / 256 * 256;
     };
     // few pairs: each is a column by itself
-    e.listed = pairs > std::min<int64_t>(gate.n_matrices, FP8_SINGLE_PAIRS);
+    e.listed = pairs > single_pairs(gate);
     e.fused = !e.listed && weighted && dev::fp8_down_fits(down, n_used);
     e.hidden_kind = e.listed ? BF16N_FP8_CODES : BF16N_FP8_F32;
     if (e.listed) {
@@ -931,7 +933,7 @@ int bf16n_fp8_workspace_bytes(const bf16n_fp8_weight * w, int gate_up, int x_kin
     return guarded([&] {
         check_fp8(w, nullptr);
         require(bytes && x_rows >= 0 && n_pairs >= 0, "fp8_workspace_bytes: null pointer or negative sizes");
-        *bytes = dev::fp8_workspace_bytes(*w, gate_up != 0, x_kind, y_kind, x_rows, n_pairs ? n_pairs : x_rows, n_pairs && listed, n_pairs && !listed);
+        *bytes = dev::fp8_workspace_upto(*w, gate_up != 0, x_kind, y_kind, x_rows, n_pairs ? n_pairs : x_rows, n_pairs && listed, n_pairs && !listed);
     });
 }
 
@@ -989,7 +991,9 @@ int bf16n_fp8_moe_experts_workspace_bytes(const bf16n_fp8_weight * gate, const b
     return guarded([&] {
         check_experts(gate, nullptr, down, n_tok, n_used);
         require(bytes != nullptr, "fp8_moe_experts_workspace_bytes: null pointer");
-        *bytes = plan_experts(*gate, *down, x_kind, weighted != 0, n_tok, n_used).bytes;
+        const uint64_t mine = plan_experts(*gate, *down, x_kind, weighted != 0, n_tok, n_used).bytes;
+        const int alone = std::min(n_tok, (int) (single_pairs(*gate) / n_used)); // the most tokens whose pairs are products by themselves (either way's workspace grows with them)
+        *bytes = alone > 0 ? std::max(mine, plan_experts(*gate, *down, x_kind, weighted != 0, alone, n_used).bytes) : mine;
     });
 }
 

@@ -1338,14 +1338,12 @@ bool converts(int KB, int64_t cols) { return KB * cols <= 512; }
 // 1408 x 2048, 64 6.3 / 7.5, 100 10.8 / 7.5; 4096 x 8192, 32 20 / 28, 8192 x 8192, 20 32 / 28.  Where K is short tiles are level (512 x 512, 1 4.7 / 4.4), and 17 columns and more theirs
 // (32 5.3 / 4.5).
 constexpr int FEW_UNITS = 512;
-bool few(const bf16n_fp8_weight & w, int64_t n_cols, bool listed, bool by_ids) {
-    if (by_ids || listed) {
-        return by_ids;
-    }
+int64_t few_limit(const bf16n_fp8_weight & w) { // the most columns of a dense product that it takes
     const int KB = (int) ((w.K + FP8_BLOCK - 1) / FP8_BLOCK);
-    const int pass = std::min(16, few_pass(n_cols, KB, true));
-    return (n_cols <= 16 || KB >= 8) && (n_cols + pass - 1) / pass * ((w.rows + 15) / 16) <= FEW_UNITS;
+    const int64_t n = FEW_UNITS / std::max<int64_t>(1, (w.rows + 15) / 16) * few_pass(16, KB, true);
+    return KB >= 8 ? n : std::min<int64_t>(n, 16);
 }
+bool few(const bf16n_fp8_weight & w, int64_t n_cols, bool listed, bool by_ids) { return by_ids || (!listed && n_cols <= few_limit(w)); }
 size_t aligned(size_t n) { return (n + 255) / 256 * 256; }
 size_t codes_bytes(int64_t rows, int64_t K) { return aligned(rows * K) + aligned(rows * ((K + FP8_BLOCK - 1) / FP8_BLOCK) * 4); }
 
@@ -1387,6 +1385,12 @@ uint64_t fp8_workspace_bytes(const bf16n_fp8_weight & w, bool glu, int x_kind, i
         n += aligned(n_cols * (w.rows / w.n_matrices) * 4);
     }
     return n;
+}
+
+uint64_t fp8_workspace_upto(const bf16n_fp8_weight & w, bool glu, int x_kind, int y_kind, int64_t x_rows, int64_t n_cols, bool listed, bool by_ids) {
+    const uint64_t n = fp8_workspace_bytes(w, glu, x_kind, y_kind, x_rows, n_cols, listed, by_ids);
+    const int64_t most = few_limit(w); // (both kernels' workspaces grow with the columns)
+    return listed || by_ids || n_cols <= most ? n : std::max(n, fp8_workspace_bytes(w, glu, x_kind, y_kind, most, most, false, false));
 }
 
 void launch_fp8_product(const fp8_product & a, void * workspace, int cus, hipStream_t stream) {
