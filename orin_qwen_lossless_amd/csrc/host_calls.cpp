@@ -11,6 +11,7 @@
 #include <algorithm>
 
 #include <ATen/ATen.h>
+#include <ATen/EmptyTensor.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
@@ -513,12 +514,11 @@ struct fp8_y {
             r.row = n * y.element_size();
             return;
         }
-        // codes and scales share an allocation (with one for each a norm of one token took 5.9 us, now 4.9)
-        const int64_t codes = (rows * n + 255) / 256 * 256, blocks = blocks_of(n);
-        y = at::empty({codes + rows * blocks * 4}, like.dtype(at::kFloat8_e4m3fn));
-        y.unsafeGetTensorImpl()->set_sizes_contiguous({rows, n});
-        scales = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(y.storage()), y.key_set(), caffe2::TypeMeta::Make<float>());
-        scales.unsafeGetTensorImpl()->set_sizes_and_strides(c10::IntArrayRef({rows, blocks}), c10::IntArrayRef({1, rows}), codes / 4);
+        // A storage for each (torch neither saves nor traces tensors of two types that share one).  The scales' comes from the codes' allocator, past the
+        // dispatcher.
+        const int64_t blocks = blocks_of(n);
+        y = at::empty({rows, n}, like.dtype(at::kFloat8_e4m3fn));
+        scales = at::Tensor(at::detail::empty_strided_generic({rows, blocks}, {1, rows}, y.storage().allocator(), y.key_set(), at::kFloat));
         r.at = y.data_ptr();
         r.row = n;
         r.scales = (float *) scales.data_ptr();
