@@ -831,9 +831,10 @@ void check_fp8(const bf16n_fp8_weight * w, const bf16n_fp8_weight * up) {
     require(!up || (up->K == w->K && up->rows == w->rows && up->n_matrices == w->n_matrices && !up->scales_bf16 == !w->scales_bf16), "fp8: gate/up shapes and scales must match");
 }
 
+void check_kind(int kind) { require(kind >= BF16N_FP8_CODES && kind <= BF16N_FP8_F32, "fp8: rows are codes, BF16 or FP32"); }
 void check_rows_in(const bf16n_fp8_rows * x) {
     require(x && x->at, "fp8: null activations");
-    require(x->kind >= BF16N_FP8_CODES && x->kind <= BF16N_FP8_F32, "fp8: rows are codes, BF16 or FP32");
+    check_kind(x->kind);
     require(((uintptr_t) x->at & 15) == 0 && x->row % 16 == 0, "fp8: activations must be 16-byte aligned with 16-byte row strides");
     require(x->kind != BF16N_FP8_CODES || (x->scales && ((uintptr_t) x->scales & 3) == 0), "fp8: codes need FP32 scales");
 }
@@ -932,7 +933,9 @@ int bf16n_add_rmsnorm_fp8(const uint16_t * a, const uint16_t * b, const uint16_t
 int bf16n_fp8_workspace_bytes(const bf16n_fp8_weight * w, int gate_up, int x_kind, int y_kind, int64_t x_rows, int64_t n_pairs, int listed, uint64_t * bytes) {
     return guarded([&] {
         check_fp8(w, nullptr);
-        require(bytes && x_rows >= 0 && n_pairs >= 0, "fp8_workspace_bytes: null pointer or negative sizes");
+        require(bytes && x_rows >= 0 && n_pairs >= 0 && x_rows <= FP8_MAX_COLS && n_pairs <= FP8_MAX_COLS, "fp8_workspace_bytes: null pointer, or rows or pairs not in [0, 2^28]");
+        check_kind(x_kind);
+        check_kind(y_kind);
         *bytes = dev::fp8_workspace_upto(*w, gate_up != 0, x_kind, y_kind, x_rows, n_pairs ? n_pairs : x_rows, n_pairs && listed, n_pairs && !listed);
     });
 }
@@ -991,6 +994,7 @@ int bf16n_fp8_moe_experts_workspace_bytes(const bf16n_fp8_weight * gate, const b
     return guarded([&] {
         check_experts(gate, nullptr, down, n_tok, n_used);
         require(bytes != nullptr, "fp8_moe_experts_workspace_bytes: null pointer");
+        check_kind(x_kind);
         const uint64_t mine = plan_experts(*gate, *down, x_kind, weighted != 0, n_tok, n_used).bytes;
         const int alone = std::min(n_tok, (int) (single_pairs(*gate) / n_used)); // the most tokens whose pairs are products by themselves (either way's workspace grows with them)
         *bytes = alone > 0 ? std::max(mine, plan_experts(*gate, *down, x_kind, weighted != 0, alone, n_used).bytes) : mine;

@@ -48,3 +48,15 @@ def test_the_same_of_the_experts(E, mid, K, n_used, x_kind, weighted):
         _lib.check(_lib.lib().bf16n_fp8_moe_experts_workspace_bytes(C.byref(gate), C.byref(down), x_kind, weighted, tokens, n_used, C.byref(n)))
         sizes.append(n.value)
     assert sizes == sorted(sizes)
+
+
+def test_sizes_and_kinds_that_the_calls_refuse():
+    """No size for them either: 2^62 rows passed 64 bits and came back as none."""
+    L, n, w = _lib.lib(), C.c_uint64(), weight(4 * 128, 256, 4)
+    ask = lambda *a: L.bf16n_fp8_workspace_bytes(C.byref(w), *a, C.byref(n))  # noqa: E731
+    assert ask(1, BF16, CODES, 1 << 28, 1 << 28, 0) == 0 and n.value == (1 << 28) * 128 * 4  # (the blocks make the codes of so short rows)
+    for bad in ((0, BF16, BF16, (1 << 28) + 1, 0, 0), (0, BF16, BF16, 1 << 62, 0, 0), (0, CODES, BF16, 1, 1 << 62, 1), (0, 3, BF16, 1, 0, 0), (0, -1, BF16, 1, 0, 0), (0, CODES, 3, 1, 0, 0)):
+        assert ask(*bad) == _lib.EINVAL and L.bf16n_last_error().startswith(b"bf16n: fp8"), bad
+    down = weight(1024, 128, 4)
+    for kind in (-1, 3):
+        assert L.bf16n_fp8_moe_experts_workspace_bytes(C.byref(w), C.byref(down), kind, 1, 10, 2, C.byref(n)) == _lib.EINVAL
