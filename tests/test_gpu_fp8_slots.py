@@ -70,3 +70,28 @@ def test_as_many_pairs_as_are_by_themselves_and_one_more(ops):
         total = (y.view(T, n_used, K) * wts.double()[:, :, None]).sum(1)
         got = ops.fp8_moe_experts(x, g, u, d, wts.cuda(), ids.cuda(), E).cpu().double()
         assert (got - total).norm() <= 2.0 ** -9 * 1.03 * total.norm()
+
+
+@pytest.mark.parametrize("T,n_used,out", [(70, 8, 520), (300, 3, 64), (90, 2, 33)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_results_at_places_of_any_alignment(ops, T, n_used, out, dtype):
+    """The same results wherever they are written (C call), and nothing around them."""
+    from orin_qwen_lossless_amd import _lib
+
+    E, mid, K, L, n = 8, 144, 64, _lib.lib(), C.c_uint64()
+    g, u, d = weight(ops, *X.matrix(mid, K, 61, E), E), weight(ops, *X.matrix(mid, K, 62, E), E), weight(ops, *X.matrix(out, mid, 63, E), E)
+    ids = ids_for(T, n_used, E, 67).to(torch.int32).cuda()
+    wts = torch.randn((T, n_used), generator=torch.Generator().manual_seed(68)).cuda()
+    x, _, _ = give(X.rows(T, K, 69, False), "bf16")
+    cg, cu, cd, cx = ops._c_fp8(g), ops._c_fp8(u), ops._c_fp8(d), ops._c_rows("test", x, K)
+    _lib.check(L.bf16n_fp8_moe_experts_workspace_bytes(C.byref(cg), C.byref(cd), cx.kind, 1, T, n_used, C.byref(n)))
+    ws = torch.empty(n.value, dtype=torch.uint8, device="cuda")
+    want = experts_f32(ops, x, g, u, d, wts, ids).to(dtype)
+    assert torch.equal(want, ops.fp8_moe_experts(x, g, u, d, wts, ids, E).to(dtype)) or dtype is torch.float32
+    for off in (8, 9, 10, 12):
+        y = torch.full((T * out + 24,), 9.0, dtype=dtype, device="cuda")
+        cy = _lib.Fp8Rows(y[off:].data_ptr(), None, out * y.element_size(), 0, 0, 1 if dtype is torch.bfloat16 else 2, 0)
+        _lib.check(L.bf16n_fp8_moe_experts(C.byref(cg), C.byref(cu), C.byref(cd), C.byref(cx), ids.data_ptr(), 0, 4, n_used * 4, wts.data_ptr(), 0, C.byref(cy), T, n_used, ws.data_ptr(), n.value,
+                                           ops._stream()))
+        assert torch.equal(y[off: off + T * out].view(T, out), want), off
+        assert (y[:off] == 9).all() and (y[off + T * out:] == 9).all(), off
