@@ -55,8 +55,9 @@ def test_slots_in_fp32(ops, T, n_used, E, mid, K, out):
 
 
 def test_as_many_pairs_as_are_by_themselves_and_one_more(ops):
-    """Where pairs become lists nothing is lost: the norm of the error stays that of the result's rounding (2^-9 / sqrt(3) of values evenly spread between
-    powers of two, 2^-9 * 1.03 of the worst)."""
+    """Where pairs become lists nothing is lost: the norm of the error stays that of the result's own rounding, 1.66e-3 of that of normal numbers (half a step is
+    2^-8 of a power of two; 2^-7 / sqrt(28) of numbers evenly spread from one to the next), within 3 % of it for 2048 of them.  A rounding of each slot
+    beside it makes 2.2e-3 and more."""
     E, mid, K, n_used = 64, 512, 256, 8
     (cg, sg), (cu, su), (cd, sd) = X.matrix(mid, K, 71, E), X.matrix(mid, K, 72, E), X.matrix(K, mid, 73, E)
     g, u, d = weight(ops, cg, sg, E), weight(ops, cu, su, E), weight(ops, cd, sd, E)
@@ -69,7 +70,7 @@ def test_as_many_pairs_as_are_by_themselves_and_one_more(ops):
         y, _ = by_pair(hidden.codes.cpu(), hidden.scales.cpu(), cd, sd, ids, E, torch.float32)
         total = (y.view(T, n_used, K) * wts.double()[:, :, None]).sum(1)
         got = ops.fp8_moe_experts(x, g, u, d, wts.cuda(), ids.cuda(), E).cpu().double()
-        assert (got - total).norm() <= 2.0 ** -9 * 1.03 * total.norm()
+        assert (got - total).norm() <= 1.85e-3 * total.norm()
 
 
 @pytest.mark.parametrize("T,n_used,out", [(70, 8, 520), (300, 3, 64), (90, 2, 33)])
