@@ -258,7 +258,8 @@ int bf16n_add_rmsnorm_fp8(const uint16_t * a, const uint16_t * b, const uint16_t
                           const uint16_t * gamma, const bf16n_fp8_rows * y, uint16_t * y_sum, uint16_t * y_norm, int n_tok, int64_t n, float eps,
                           void * stream);
 /* y = W x per row of x: sums over a block of 128 columns on the matrix cores, scaled and added up in FP32.  up given: silu(W x) * (up x)
- * (w and up of one shape).  Rows of x that are not codes are taken as what bf16n_fp8_quantize_rows makes of them.  y: BF16, FP32, or with
+ * (w and up of one shape).  FP32 results, codes and few rows: sums of exact products; BF16 results of many rows: of every eight columns' products what is
+ * below 2^-13 of the largest may be dropped.  Rows of x that are not codes are taken as what bf16n_fp8_quantize_rows makes of them.  y: BF16, FP32, or with
  * up codes (rows of W a multiple of 16 then).  w has one matrix.  workspace: bf16n_fp8_workspace_bytes, 16-byte aligned (null if
  * that is 0).  The result must not overlap x. */
 int bf16n_fp8_mm(const bf16n_fp8_weight * w, const bf16n_fp8_weight * up, const bf16n_fp8_rows * x, const bf16n_fp8_rows * y, int64_t n_rows,

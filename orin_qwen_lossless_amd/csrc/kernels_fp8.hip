@@ -532,7 +532,7 @@ __device__ __forceinline__ list_pass find_pass(const int32_t * bounds, int n_mat
 // Lists: a block to 64 columns of one matrix, every pass a block of its own.  Gate and up: the scales of the columns in registers, so that two blocks'
 // stages are the whole of a CU's LDS (one block with 128 columns that took a list's passes in turn: 2048 tokens of 256 experts of 512 x 2048 190 us,
 // 512 tokens 128; now 145 and 104).  Down, whose K is short: two row tiles to a block, the second's copies under the first's last products (2048 tokens,
-// one / two / four: 98, 93, 102).
+// one / two / four: 110, 105, 107 with FP32 results, 98, 93, 102 with BF16 ones).
 template <int WR, int WC, int RT, int CT, int S, bool GLU, bool LIST, int OUT>
 __global__ void __launch_bounds__(WR * WC * 64, 2) k_fp8_many(const fp8_launch p) {
     constexpr bool WIDE = OUT != BF16, SX_REGS = LIST && GLU, TILES = LIST && !GLU;
@@ -934,8 +934,8 @@ __device__ __forceinline__ u32x4_t to_bf16x8(const float (&v)[8]) {
 // a block of 128, eight slots' rows on the way at a time (one after the other: 333 tokens of 2576 with eight slots 10.9 us).  A row stays
 // in registers between the sum of its squares and its codes.  Every sum and the norm are held in 64 bits and become
 // FP32 once, ahead of the scales: a code is off by a whole step, a sixteenth of its value, wherever an error of a last place carries a value over the
-// middle of two codes, which 32 bits did to one or two of 858 thousand (and were 8.9 us there for 9.6).
-// 8192 tokens of 2048: 22.1 us, 118 MB at 5.3 TB/s; one token 2.7, the chain of its loads, sum and scale.
+// middle of two codes, which 32 bits did to one or two of 858 thousand (and were 8.9 us there for 9.7).
+// 8192 tokens of 2048: 22.1 us, 118 MB at 5.3 TB/s (two inputs in turn; three 23.8); one token 2.5, the chain of its loads, sum and scale.
 template <int C, bool SLOTS>
 __global__ void __launch_bounds__(1024) k_add_rmsnorm_fp8(const add_norm_args p, uint8_t * y, int64_t y_row, float * s, int64_t s_row, int64_t s_block) {
     __shared__ double wave_sq[16];
@@ -1245,7 +1245,8 @@ void many_kinds(const fp8_launch * p, int y_kind, hipStream_t stream) {
     }
 }
 
-// Tiles to choose from, and what a step of 128 columns of K takes, us: of one block to a CU, and of each where the CUs are full of them.
+// Tiles to choose from, and what a step of 128 columns of K takes, us: of one block to a CU, and of each where the CUs are full of them.  Here and in
+// run_many: calls behind one another on two inputs in turn (on three 8192 x 2048 by 8192 columns, 152, takes 173: they pass the caches, and power holds the clock).
 struct tile_of { int rows, cols; float alone, full; };
 // the tile whose steps take least: those of one block or of the rounds that the tiles make
 int best_tile(const tile_of * tiles, int n, const fp8_launch & p) {
