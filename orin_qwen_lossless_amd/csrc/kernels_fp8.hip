@@ -1033,6 +1033,7 @@ __global__ void __launch_bounds__(1024) k_add_rmsnorm_fp8(const add_norm_args p,
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 y32[e] = (float) v[j][e];
+                asm("" : "+v"(y32[e])); // (else the two roundings become one from 64 bits to BF16, six instructions an element: 8192 x 2048 1.2 us)
             }
             *(u32x4_t *) (p.y_sum + base + i0) = to_bf16x8(y32);
         }
