@@ -502,6 +502,11 @@ struct fp8_x {
     }
 };
 
+// a tensor beside `first`, which torch has just made, from the same allocator and past the dispatcher (0.3 us less than at::empty)
+at::Tensor beside(const at::Tensor & first, at::IntArrayRef sizes, at::IntArrayRef strides, at::ScalarType type) {
+    return at::Tensor(at::detail::empty_strided_generic(sizes, strides, first.storage().allocator(), first.key_set(), type));
+}
+
 // results: a tensor, or codes and scales
 struct fp8_y {
     at::Tensor y, scales;
@@ -514,11 +519,10 @@ struct fp8_y {
             r.row = n * y.element_size();
             return;
         }
-        // A storage for each (torch neither saves nor traces tensors of two types that share one).  The scales' comes from the codes' allocator, past the
-        // dispatcher.
+        // (a storage for each: torch neither saves nor traces tensors of two types that share one)
         const int64_t blocks = blocks_of(n);
         y = at::empty({rows, n}, like.dtype(at::kFloat8_e4m3fn));
-        scales = at::Tensor(at::detail::empty_strided_generic({rows, blocks}, {1, rows}, y.storage().allocator(), y.key_set(), at::kFloat));
+        scales = beside(y, {rows, blocks}, {1, rows}, at::kFloat);
         r.at = y.data_ptr();
         r.row = n;
         r.scales = (float *) scales.data_ptr();
@@ -659,10 +663,10 @@ PyObject * add_rmsnorm_fp8(PyObject *, PyObject * const * args, Py_ssize_t n) {
         fp8_y y(T, K, BF16N_FP8_CODES, on(*a, at::kBFloat16));
         at::Tensor sum, norm;
         if (args[7] == Py_True) {
-            sum = at::empty({T, K}, on(*a, at::kBFloat16));
+            sum = beside(y.y, {T, K}, {K, 1}, at::kBFloat16);
         }
         if (args[8] == Py_True) {
-            norm = at::empty({T, K}, on(*a, at::kBFloat16));
+            norm = beside(y.y, {T, K}, {K, 1}, at::kBFloat16);
         }
         const auto at_of = [](const at::Tensor * v) { return v ? v->data_ptr() : nullptr; };
         int status;
