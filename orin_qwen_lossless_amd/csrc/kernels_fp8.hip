@@ -934,8 +934,8 @@ __device__ __forceinline__ u32x4_t to_bf16x8(const float (&v)[8]) {
 // a block of 128, eight slots' rows on the way at a time (one after the other: 333 tokens of 2576 with eight slots 10.9 us).  A row stays
 // in registers between the sum of its squares and its codes.  Every sum and the norm are held in 64 bits and become
 // FP32 once, ahead of the scales: a code is off by a whole step, a sixteenth of its value, wherever an error of a last place carries a value over the
-// middle of two codes, which 32 bits did to one or two of 858 thousand (and were 8.9 us there for 9.7).
-// 8192 tokens of 2048: 22.1 us, 118 MB at 5.3 TB/s (two inputs in turn; three 23.8); one token 2.5, the chain of its loads, sum and scale.
+// middle of two codes, which 32 bits did to one or two of 858 thousand (and were 8.9 us there for 9.3).
+// 8192 tokens of 2048: 21.1 us, 118 MB at 5.6 TB/s (two inputs in turn; three 22.5); one token 2.4, the chain of its loads, sum and scale.
 template <int C, bool SLOTS>
 __global__ void __launch_bounds__(1024) k_add_rmsnorm_fp8(const add_norm_args p, uint8_t * y, int64_t y_row, float * s, int64_t s_row, int64_t s_block) {
     __shared__ double wave_sq[16];
