@@ -130,9 +130,9 @@ struct fp8_product {
 void fp8_init();
 void launch_fp8_rows(const bf16n_fp8_rows & x, const bf16n_fp8_rows & y, int64_t rows, int64_t K, int cus, hipStream_t stream);
 void launch_add_rmsnorm_fp8(const add_norm_args & a, const bf16n_fp8_rows & y, int n_tok, hipStream_t stream);
-// what a product needs; what it and every smaller one of the same kind need
-uint64_t fp8_workspace_upto(const bf16n_fp8_weight & w, bool glu, int x_kind, int y_kind, int64_t x_rows, int64_t n_cols, bool listed, bool by_ids);
+// what a product needs; what it and every one of fewer columns need
 uint64_t fp8_workspace_bytes(const bf16n_fp8_weight & w, bool glu, int x_kind, int y_kind, int64_t x_rows, int64_t n_cols, bool listed, bool by_ids);
+uint64_t fp8_workspace_upto(const bf16n_fp8_weight & w, bool glu, int x_kind, int y_kind, int64_t x_rows, int64_t n_cols, bool listed, bool by_ids);
 void launch_fp8_product(const fp8_product & a, void * workspace, int cus, hipStream_t stream);
 // the slots' products (by ids, FP32 rows of x) and their weighted sum: a.y has a row for every token
 bool fp8_down_fits(const bf16n_fp8_weight & down, int n_used);
